@@ -626,6 +626,58 @@ int mf_simplicial_packed_fwd(const MfSimplicialPackedArgs* args, void* stream);
 int mf_simplicial_packed_bwd(const MfSimplicialPackedArgs* args, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* Gated feed-forward block                                                    */
+/* ------------------------------------------------------------------------- */
+
+#define MF_ACT_SILU 0      /* z / (1 + exp(-z)) */
+#define MF_ACT_GELU_TANH 1 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+
+/*
+ * The gated counterpart of `Mlp` (transformer.py:137-152); no reference operator.  For each of `rows` tokens
+ *   [gate up] = x w_in^T + b_in,  act = f(gate) * up,  y = act w_out^T + b_out
+ * with w_in (2*hidden, dim), the gate's rows first, w_out (dim_out, hidden) and optional biases (NULL).  dtype is bf16 or fp16, of
+ * every tensor but the gradients of the parameters, which come in grad_dtype (dtype or fp32).  Widths are multiples of 8; any
+ * number of rows.
+ * Forward: writes act (rows, hidden), y (rows, dim_out) and, where `pre` is given, the pre-activations (rows, 2*hidden).
+ * Backward: reads x, w_in, w_out, pre, act and grad_y; writes those of grad_x, grad_w_in, grad_w_out, grad_b_in, grad_b_out that are
+ * not NULL.  Sums are in fp32 and in a fixed order; pre, act and the gradients of the pre-activations are rounded to dtype.
+ * Workspace (backward): mf_gated_mlp_bwd_workspace_bytes, for the same gradients.  An expired device-side wait is reported by
+ * mf_gated_mlp_status (which synchronises `stream`); the outputs of such a call are undefined.
+ */
+typedef struct MfGatedMlpArgs {
+  int64_t rows;
+  int32_t dim, hidden, dim_out;
+  int32_t dtype;
+  int32_t grad_dtype;
+  int32_t activation; /* MF_ACT_* */
+  const void* x;
+  const void* w_in;
+  const void* w_out;
+  const void* b_in;
+  const void* b_out;
+  void* pre;
+  void* act;
+  void* y;
+  const void* grad_y; /* backward from here on */
+  void* grad_x;
+  void* grad_w_in;
+  void* grad_w_out;
+  void* grad_b_in;
+  void* grad_b_out;
+  void* workspace;
+  size_t workspace_bytes;
+} MfGatedMlpArgs;
+
+size_t mf_gated_mlp_bwd_workspace_bytes(const MfGatedMlpArgs* args);
+int mf_gated_mlp_fwd(const MfGatedMlpArgs* args, void* stream);
+int mf_gated_mlp_bwd(const MfGatedMlpArgs* args, void* stream);
+int mf_gated_mlp_status(int32_t* host_status, void* stream);
+/* Runs the call with the hand-offs of one kind withheld (0 operands, 1 stages, 2 accumulators, 3 drained accumulators) and waits that
+ * expire after limit_cycles; returns the status it left and clears it.  The call's outputs are undefined. */
+int mf_selftest_gated_mlp_give_up(const MfGatedMlpArgs* args, int32_t backward, int32_t kind, int64_t limit_cycles, int32_t* host_status,
+                                  void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Equivariant coordinate head                                               */
 /* ------------------------------------------------------------------------- */
 

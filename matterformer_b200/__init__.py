@@ -10,6 +10,7 @@ from .simplicial import (
     simplicial_attention_cuda,
 )
 from .batching import AttentionCostBatchSampler, simplicial_tile_steps
+from .gated import gated_mlp, gated_mlp_status
 from .hostio import HostPipelinedSimplicial
 from .sampler import GraphedDenoiser, edm_sample
 from .sparse import (
@@ -25,6 +26,8 @@ from .sparse import (
 )
 
 __all__ = [
+    "gated_mlp",
+    "gated_mlp_status",
     "GraphedDenoiser",
     "edm_sample",
     "AttentionCostBatchSampler",

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
-from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
@@ -26,6 +26,7 @@ MF_DTYPE_F32, MF_DTYPE_BF16, MF_DTYPE_F16 = 0, 1, 2
 MF_PRECISION = {"bf16_tc": 0, "tf32": 1, "ieee_fp32": 2}
 MF_BACKEND = {"auto": 0, "generic": 1, "tcgen05": 2, "tcgen05_tiles": 3}
 MF_SPARSE_BACKEND = {"auto": 0, "mma": 1, "tcgen05": 2}
+MF_ACT_SILU, MF_ACT_GELU_TANH = 0, 1
 
 # Every symbol include/matterformer_b200.h declares.
 EXPORTED_SYMBOLS = (
@@ -95,6 +96,11 @@ EXPORTED_SYMBOLS = (
     "mf_pair_head_bwd_workspace_bytes",
     "mf_pair_head_fwd",
     "mf_pair_head_bwd",
+    "mf_gated_mlp_bwd_workspace_bytes",
+    "mf_gated_mlp_fwd",
+    "mf_gated_mlp_bwd",
+    "mf_gated_mlp_status",
+    "mf_selftest_gated_mlp_give_up",
     "mf_profile_enable",
     "mf_profile_read",
 )
@@ -294,6 +300,14 @@ class MfPairHeadArgs(Structure):
     ]
 
 
+class MfGatedMlpArgs(Structure):
+    _fields_ = [("rows", c_int64)] + \
+               [(n, c_int32) for n in ("dim", "hidden", "dim_out", "dtype", "grad_dtype", "activation")] + \
+               [(n, c_void_p) for n in ("x", "w_in", "w_out", "b_in", "b_out", "pre", "act", "y", "grad_y", "grad_x", "grad_w_in",
+                                        "grad_w_out", "grad_b_in", "grad_b_out", "workspace")] + \
+               [("workspace_bytes", c_size_t)]  # fmt: skip
+
+
 _LIB = None
 
 
@@ -431,6 +445,15 @@ def lib() -> ctypes.CDLL:
     for fn in (L.mf_pair_head_fwd, L.mf_pair_head_bwd):
         fn.argtypes = [POINTER(MfPairHeadArgs), c_void_p]
         fn.restype = c_int32
+    L.mf_gated_mlp_bwd_workspace_bytes.argtypes = [POINTER(MfGatedMlpArgs)]
+    L.mf_gated_mlp_bwd_workspace_bytes.restype = c_size_t
+    for fn in (L.mf_gated_mlp_fwd, L.mf_gated_mlp_bwd):
+        fn.argtypes = [POINTER(MfGatedMlpArgs), c_void_p]
+        fn.restype = c_int32
+    L.mf_gated_mlp_status.argtypes = [POINTER(c_int32), c_void_p]
+    L.mf_gated_mlp_status.restype = c_int32
+    L.mf_selftest_gated_mlp_give_up.argtypes = [POINTER(MfGatedMlpArgs), c_int32, c_int32, c_int64, POINTER(c_int32), c_void_p]
+    L.mf_selftest_gated_mlp_give_up.restype = c_int32
     L.mf_simplicial_fwd_backend.argtypes = [POINTER(MfSimplicialFwdArgs)]
     L.mf_simplicial_fwd_backend.restype = c_int32
     L.mf_simplicial_bwd_backend.argtypes = [POINTER(MfSimplicialBwdArgs)]

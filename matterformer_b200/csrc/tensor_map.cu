@@ -4,6 +4,8 @@
 
 #include <mutex>
 
+#include "../../include/matterformer_b200.h"
+
 namespace mf {
 namespace {
 
@@ -34,36 +36,57 @@ static thread_local int g_last_encode_result = 0;
 int last_tensor_map_result() { return g_last_encode_result; }
 
 namespace {
-// `rank` dimensions from the innermost, 64 bf16 elements wide; strides in bytes of dimensions 1, 2, ...
-bool encode_rows(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box_rows) {
+// `rank` dimensions from the innermost, boxes of box_rows lines of 128 bytes; strides in bytes of dimensions 1, 2, ...
+bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, int box_cols, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+            int box_rows) {
   EncodeTiledFn fn = encoder();
   g_last_encode_result = -1;  // refused before the driver was asked
   if (!fn || !base || box_rows <= 0 || box_rows > 256 || box_rows % 8) return false;
   for (int i = 1; i < rank; ++i)
     if (dims[i] == 0 || strides[i - 1] % 16) return false;
   if (reinterpret_cast<uintptr_t>(base) & 15u) return false;  // the copy engine needs a 16-byte aligned base
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1};
   const cuuint32_t elem_strides[4] = {1, 1, 1, 1};
   CUtensorMap tmp;
-  auto encode = [&]() {
-    return fn(&tmp, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, elem_strides,
+  auto call = [&]() {
+    return fn(&tmp, type, rank, const_cast<void*>(base), dims, strides, box, elem_strides,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
-  CUresult r = encode();
+  CUresult r = call();
   if (r == CUDA_ERROR_INVALID_CONTEXT) {
     // The encoder wants a context bound to the calling thread.  A host thread that has only been handed cached
     // device memory so far (the backward thread of an autograd engine, say) has none yet: a no-op runtime call
     // binds the device's primary context, then the encoding goes through.
     (void)cudaFree(nullptr);
-    r = encode();
+    r = call();
   }
   g_last_encode_result = (int)r;
   if (r != CUDA_SUCCESS) return false;
   *map = tmp;
   return true;
 }
+bool encode_rows(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box_rows) {
+  return encode(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 64, rank, dims, strides, box_rows);
+}
 }  // namespace
+
+bool make_tensor_map(CUtensorMap* map, const void* base, int dtype, int rank, const long long* dims, const long long* strides, int box_cols,
+                     int box_rows) {
+  const int size = dtype == MF_DTYPE_F32 ? 4 : 2;
+  g_last_encode_result = -1;
+  if (rank < 2 || rank > 4 || box_cols * size != 128) return false;
+  cuuint64_t d[4], s[3];
+  for (int i = 0; i < rank; ++i) {
+    if (dims[i] <= 0) return false;
+    d[i] = (cuuint64_t)dims[i];
+    if (i) s[i - 1] = (cuuint64_t)strides[i - 1];
+  }
+  const CUtensorMapDataType type = dtype == MF_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == MF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(map, base, type, box_cols, rank, d, s, box_rows);
+}
 
 bool make_rows_tensor_map(CUtensorMap* map, const void* base, int rows_per_matrix, int matrices, int box_rows) {
   if (rows_per_matrix < 0 || matrices < 0) return false;

@@ -1,0 +1,131 @@
+"""Gated feed-forward block: two projections, an activation of one times the other, and the projection back.
+
+``gated_mlp(x, w_in, w_out, b_in, b_out)`` = ``(act(gate) * up) @ w_out.T + b_out`` with ``gate, up = (x @ w_in.T + b_in).chunk(2, -1)``,
+the gated counterpart of the trunk's MLP (models/transformer.py:137-152 of the reference has the plain one; it has no operator of this
+name).  Both projections, the activation and the product are one kernel, forward; backward, the gradient of the activation is
+formed in the epilogue of the product that would otherwise store it.  All products run on this library's tcgen05 kernels.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .linear import bf16_copy
+
+_CODE = {torch.bfloat16: _lib.MF_DTYPE_BF16, torch.float16: _lib.MF_DTYPE_F16}
+ACTIVATIONS = {"silu": _lib.MF_ACT_SILU, "gelu_tanh": _lib.MF_ACT_GELU_TANH}
+
+
+def _ready(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and on a 16-byte boundary, as the kernels read it."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _args(x, w_in, w_out, b_in, b_out, activation, grad_dtype):
+    a = _lib.MfGatedMlpArgs()
+    a.rows, a.dim, a.hidden, a.dim_out = x.shape[0], x.shape[1], w_out.shape[1], w_out.shape[0]
+    a.dtype, a.activation = _CODE[x.dtype], ACTIVATIONS[activation]
+    a.grad_dtype = _lib.MF_DTYPE_F32 if grad_dtype == torch.float32 else a.dtype
+    a.x, a.w_in, a.w_out, a.b_in, a.b_out = _ptr(x), _ptr(w_in), _ptr(w_out), _ptr(b_in), _ptr(b_out)
+    return a
+
+
+class _GatedMlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_in, w_out, b_in, b_out, activation):
+        ctx.shape, ctx.activation, ctx.grad_dtype = x.shape, activation, w_in.dtype
+        x2 = _ready(x.reshape(-1, x.shape[-1]))
+        params = [_ready(bf16_copy(p) if p is not None and p.dtype != x.dtype else p) for p in (w_in, w_out, b_in, b_out)]
+        rows, F = x2.shape[0], w_out.shape[1]
+        y = torch.empty((rows, w_out.shape[0]), device=x.device, dtype=x.dtype)
+        act = torch.empty((rows, F), device=x.device, dtype=x.dtype)
+        keep = any(ctx.needs_input_grad)
+        pre = torch.empty((rows, 2 * F), device=x.device, dtype=x.dtype) if keep else None
+        a = _args(x2, *params, activation, ctx.grad_dtype)
+        a.pre, a.act, a.y = _ptr(pre), _ptr(act), _ptr(y)
+        _lib.launch(_lib.lib().mf_gated_mlp_fwd, x.device, ctypes.byref(a))
+        if keep:
+            ctx.save_for_backward(x2, *params, pre, act)
+        return y.view(*x.shape[:-1], w_out.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, w_in, w_out, b_in, b_out, pre, act = ctx.saved_tensors
+        grad_y = _ready(grad_y.reshape(-1, w_out.shape[0]).to(x.dtype))
+        a = _args(x, w_in, w_out, b_in, b_out, ctx.activation, ctx.grad_dtype)
+        wanted = [t if need else None for t, need in zip((x, w_in, w_out, b_in, b_out), ctx.needs_input_grad)]
+        grads = [None if t is None else torch.empty(t.shape, device=x.device, dtype=x.dtype if i == 0 else ctx.grad_dtype)
+                 for i, t in enumerate(wanted)]  # fmt: skip
+        a.pre, a.act, a.grad_y = _ptr(pre), _ptr(act), _ptr(grad_y)
+        a.grad_x, a.grad_w_in, a.grad_w_out, a.grad_b_in, a.grad_b_out = (_ptr(g) for g in grads)
+        L = _lib.lib()
+        need = L.mf_gated_mlp_bwd_workspace_bytes(ctypes.byref(a))
+        ws = torch.empty(max(need, 16), device=x.device, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _lib.launch(L.mf_gated_mlp_bwd, x.device, ctypes.byref(a))
+        if grads[0] is not None:
+            grads[0] = grads[0].view(ctx.shape)
+        return (*grads, None)
+
+
+def gated_mlp_applies(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> bool:
+    """Whether the kernels take these operands: CUDA, 16-bit ``x``, parameters of its type (or fp32 beside bf16), widths that are
+    multiples of 8."""
+    return (x.is_cuda and x.dtype in _CODE and w_in.ndim == w_out.ndim == 2 and w_in.dtype == w_out.dtype
+            and (w_in.dtype == x.dtype or (w_in.dtype == torch.float32 and x.dtype == torch.bfloat16))
+            and all(n % 8 == 0 and n > 0 for n in (w_in.shape[1], w_out.shape[1], w_out.shape[0])))  # fmt: skip
+
+
+def _check(x, w_in, w_out, b_in, b_out, activation):
+    if not x.is_cuda:
+        raise RuntimeError("gated_mlp requires CUDA tensors")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"gated_mlp: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    if x.dtype not in _CODE:
+        raise RuntimeError(f"gated_mlp only supports float16/bfloat16 inputs, got {x.dtype}")
+    params = [p for p in (w_in, w_out, b_in, b_out) if p is not None]
+    if any(p.dtype != w_in.dtype for p in params) or not (w_in.dtype == x.dtype or (w_in.dtype, x.dtype) == (torch.float32, torch.bfloat16)):
+        raise RuntimeError(f"gated_mlp: parameters must share the type of x, or be float32 beside bfloat16; got x {x.dtype}, "
+                           f"parameters {[str(p.dtype) for p in params]}")  # fmt: skip
+    if any(p.device != x.device for p in params):
+        raise ValueError("gated_mlp: x and the parameters must be on one device")
+    if x.ndim < 1 or w_in.ndim != 2 or w_out.ndim != 2 or w_in.shape != (2 * w_out.shape[1], x.shape[-1]):
+        raise ValueError(f"gated_mlp: x (..., C), w_in (2 F, C) and w_out (O, F) expected, got {tuple(x.shape)}, {tuple(w_in.shape)}, "
+                         f"{tuple(w_out.shape)}")  # fmt: skip
+    if (b_in is not None and b_in.shape != w_in.shape[:1]) or (b_out is not None and b_out.shape != w_out.shape[:1]):
+        raise ValueError("gated_mlp: b_in must have shape (2 F,) and b_out (O,)")
+    if any(n < 8 or n % 8 for n in (x.shape[-1], *w_out.shape)):
+        raise ValueError(f"gated_mlp: widths must be positive multiples of 8, got C={x.shape[-1]}, F={w_out.shape[1]}, O={w_out.shape[0]}")
+
+
+def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
+              b_out: Optional[torch.Tensor] = None, *, activation: str = "silu") -> torch.Tensor:  # fmt: skip
+    """``x`` (..., C) bf16 or fp16; ``w_in`` (2 F, C) with the gate's rows first, ``w_out`` (O, F), biases (2 F,) and (O,) or None, of
+    ``x``'s type, or fp32 beside a bf16 ``x`` (their bf16 copies compute, their gradients are fp32; see
+    :func:`matterformer_b200.linear.bf16_copies`).  ``activation``: "silu" or "gelu_tanh".  Returns (..., O) in ``x``'s type.
+
+    Sums are in fp32 in a fixed order.  The hidden values, and for the backward pass the pre-activations and their gradients, are
+    rounded to ``x``'s type.  C, F and O are multiples of 8.  The gradient is once differentiable."""
+    _check(x, w_in, w_out, b_in, b_out, activation)
+    return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, activation)
+
+
+def gated_mlp_status(device=None) -> int:
+    """Status word of the block's kernels: 0, or the code of an expired device-side wait (the outputs of that call are undefined).
+    Synchronises the current stream."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    out = ctypes.c_int32(0)
+    _lib.launch(_lib.lib().mf_gated_mlp_status, dev, ctypes.byref(out))
+    return int(out.value)
