@@ -23,67 +23,93 @@ bool map16(CUtensorMap* map, const void* base, long long rows, long long cols, l
   return make_tensor_map(map, base, std::is_same<T, __nv_bfloat16>::value ? MF_DTYPE_BF16 : MF_DTYPE_F16, 2, dims, strides, 64, box_rows);
 }
 
-int clusters(long long tiles) { return (int)(tiles < kPairs ? tiles : kPairs); }
-
-template <typename T, bool kAMn, bool kBMn, int kN, Epilogue kEpi>
-int launch(const Params& p, cudaStream_t stream, const char* what) {
-  auto kernel = gemm_kernel<T, kAMn, kBMn, kN, kEpi>;
-  constexpr int kSmem = Shape<kN, kEpi>::kSmem;
+template <typename T, bool kAMn, bool kBMn, Epilogue kEpi, int kAct>
+int launch_kernel(const Params& p, int pairs, cudaStream_t stream, const char* what) {
+  auto kernel = gemm_kernel<T, kAMn, kBMn, kEpi, kAct>;
+  constexpr int kSmem = Shape<kEpi>::kSmem;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return cuda_error(e, what);
-  const long long tiles = (long long)((p.m + 255) / 256) * ((p.n + (kEpi == kGate ? kN / 2 : kN) - 1) / (kEpi == kGate ? kN / 2 : kN)) * p.splits;
   cudaLaunchAttribute attributes[2] = {};
   attributes[0].id = cudaLaunchAttributeClusterDimension;
   attributes[0].val.clusterDim.x = 2, attributes[0].val.clusterDim.y = 1, attributes[0].val.clusterDim.z = 1;
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(2 * clusters(tiles)), config.blockDim = dim3(kThreads), config.dynamicSmemBytes = kSmem, config.stream = stream;
+  config.gridDim = dim3(2 * pairs), config.blockDim = dim3(kThreads), config.dynamicSmemBytes = kSmem, config.stream = stream;
   config.attrs = attributes, config.numAttrs = 2;
   const cudaError_t l = cudaLaunchKernelEx(&config, kernel, p);
   return l == cudaSuccess ? MF_OK : cuda_error(l, what);
 }
 
-// ---- planes of partial sums ----------------------------------------------------------------------------------------
-template <typename TOut>
-__global__ void add_planes_kernel(const float* __restrict__ planes, int n, long long count, TOut* __restrict__ out) {
+int tiles_of(long long rows, long long cols, int width) { return (int)(((rows + kTile - 1) / kTile) * ((cols + width - 1) / width)); }
+
+// Tiles of full width in whole rounds of the pairs; a last round that would leave at least half (three quarters) of them without work is
+// cut into tiles of half (a quarter of) the width.  29 696 x 512 over 2048: 232 tiles are 3.1 rounds.
+template <typename T, bool kAMn, bool kBMn, Epilogue kEpi>
+int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
+  const int tiles = tiles_of(p.one.m, p.one.n, kEpi == kGate ? kTile / 2 : kTile), rest = tiles % kPairs;
+  p.cut = rest == 0 || 2 * rest > kPairs ? 1 : kEpi == kGate || 4 * rest > kPairs ? 2 : 4;
+  p.whole = p.cut == 1 ? tiles : tiles - rest;
+  p.tiles = p.whole + (tiles - p.whole) * p.cut;
+  const int pairs = p.tiles < kPairs ? p.tiles : kPairs;
+  if constexpr (kEpi == kStore) return launch_kernel<T, kAMn, kBMn, kEpi, 0>(p, pairs, stream, what);
+  else
+    return activation == MF_ACT_SILU ? launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_SILU>(p, pairs, stream, what)
+                                     : launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_GELU_TANH>(p, pairs, stream, what);
+}
+
+// ---- gradients of the weights --------------------------------------------------------------------------------------
+// Both are sums over the tokens, of [dg du] x and of dy h: one launch for the tiles of both.  Whole rounds of tiles walk all tokens;
+// the tiles behind them are cut into pieces of the tokens, each with a plane of partial sums of its own, which add_planes_kernel adds in order.
+struct WeightPlan {
+  int k_blocks, tiles1, tiles2, whole, rest, pieces, per;
+};
+WeightPlan weight_plan(const MfGatedMlpArgs* a) {
+  WeightPlan w;
+  w.k_blocks = (int)((a->rows + kBlockK - 1) / kBlockK);
+  w.tiles1 = a->grad_w_in ? tiles_of(2ll * a->hidden, a->dim, kTile) : 0;
+  w.tiles2 = a->grad_w_out ? tiles_of(a->dim_out, a->hidden, kTile) : 0;
+  const int tiles = w.tiles1 + w.tiles2;
+  w.rest = tiles % kPairs;
+  w.whole = tiles - w.rest;
+  w.pieces = 1, w.per = w.k_blocks;
+  // The number of pieces with the least estimated time: rounds of the longest piece, 0.3 us for a block of 64 tokens, and 0.1 us for
+  // each plane's way to memory and back.
+  double least = 1e30;
+  for (int s = 1; w.rest && s <= kPairs && s <= w.k_blocks; ++s) {
+    const int per = (w.k_blocks + s - 1) / s;
+    if ((w.k_blocks + per - 1) / per != s) continue;  // a piece would be empty
+    const double us = 0.3 * ((w.rest * s + kPairs - 1) / kPairs) * per + (s > 1 ? 0.1 * w.rest * s : 0.);
+    if (us < least) least = us, w.pieces = s, w.per = per;
+  }
+  if (w.pieces == 1) w.whole = tiles, w.rest = 0;
+  return w;
+}
+size_t plane_bytes(const WeightPlan& w) { return (size_t)w.rest * w.pieces * kTile * kTile * 4; }
+
+template <typename T, typename TOut>
+__global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict__ planes, WeightPlan w, TOut* __restrict__ out1, int m1, int n1,
+                                                         TOut* __restrict__ out2, int m2, int n2) {
   wait_for_previous();
-  const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
-  if (i >= count) return;
-  float4 s = *reinterpret_cast<const float4*>(planes + i);
-  for (int k = 1; k < n; ++k) {
-    const float4 v = *reinterpret_cast<const float4*>(planes + k * count + i);
+  const int tile = w.whole + blockIdx.x;
+  const bool second = tile >= w.tiles1;
+  const int m = second ? m2 : m1, n = second ? n2 : n1;
+  TOut* out = second ? out2 : out1;
+  int tm, tn;
+  tile_at(second ? tile - w.tiles1 : tile, (m + kTile - 1) / kTile, (n + kTile - 1) / kTile, tm, tn);
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 6), col = 4 * (threadIdx.x & 63);
+  if (tm * kTile + row >= m || tn * kTile + col >= n) return;
+  const float* from = planes + ((size_t)blockIdx.x * kTile + row) * kTile + col;
+  const size_t stride = (size_t)w.rest * kTile * kTile;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int q = 0; q < w.pieces; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(from + q * stride);
     s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
   }
-  if constexpr (sizeof(TOut) == 4) {
-    *reinterpret_cast<float4*>(out + i) = s;
-  } else {
-    *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<TOut>(s.x, s.y), pack2<TOut>(s.z, s.w));
-  }
-}
-
-// How many pieces the tokens are cut into for a weight gradient of `tiles` tiles: the piece count with the shortest longest run of 64-token
-// blocks, each plane of sums counted with what it moves.
-int token_splits(long long tiles, int k_blocks, long long values) {
-  int best = 1;
-  double least = 1e30;
-  for (int s = 1; s <= 16 && (s == 1 || k_blocks / s >= 8); ++s) {
-    const int per = (k_blocks + s - 1) / s;
-    if ((k_blocks + per - 1) / per != s) continue;
-    const double blocks = (double)((tiles * s + kPairs - 1) / kPairs) * per * 0.29, planes = s > 1 ? 8e-6 * s * (double)values / 6.5 : 0.;
-    if (blocks + planes < least) least = blocks + planes, best = s;
-  }
-  return best;
-}
-
-struct Weight {  // gradient of an (m, n) weight over the tokens
-  int m, n, splits, per_split;
-};
-Weight weight_plan(long long rows, int m, int n) {
-  const long long tiles = (long long)((m + 255) / 256) * ((n + 255) / 256);
-  const int k_blocks = (int)((rows + kBlockK - 1) / kBlockK);
-  const int s = token_splits(tiles, k_blocks, (long long)m * n);
-  return {m, n, s, (k_blocks + s - 1) / s};
+  TOut* to = out + (size_t)(tm * kTile + row) * n + tn * kTile + col;
+  if constexpr (sizeof(TOut) == 4) *reinterpret_cast<float4*>(to) = s;
+  else *reinterpret_cast<uint2*>(to) = make_uint2(pack2<TOut>(s.x, s.y), pack2<TOut>(s.z, s.w));
 }
 
 size_t pieces(const MfGatedMlpArgs* a, bool backward, size_t (&at)[4]) {  // gradient of the pre-activations | planes | bias sums | their bands
@@ -91,15 +117,7 @@ size_t pieces(const MfGatedMlpArgs* a, bool backward, size_t (&at)[4]) {  // gra
   at[0] = 0;
   if (!backward || rows == 0) return 0;
   at[1] = at[0] + align_up(rows * 2 * F * size, 256);
-  size_t planes = 0;
-  if (a->grad_w_in) {
-    const Weight w = weight_plan(a->rows, 2 * a->hidden, a->dim);
-    if (w.splits > 1) planes = (size_t)w.splits * w.m * w.n * 4;
-  }
-  if (a->grad_w_out) {
-    const Weight w = weight_plan(a->rows, a->dim_out, a->hidden);
-    if (w.splits > 1 && (size_t)w.splits * w.m * w.n * 4 > planes) planes = (size_t)w.splits * w.m * w.n * 4;
-  }
+  const size_t planes = a->grad_w_in || a->grad_w_out ? plane_bytes(weight_plan(a)) : 0;
   at[2] = at[1] + align_up(planes, 256);
   const long long bands = (a->rows + 31) / 32;
   at[3] = at[2] + (a->grad_b_in ? align_up((size_t)bands * 2 * F * 4, 256) : 0);
@@ -125,10 +143,9 @@ int check(const MfGatedMlpArgs* a) {
   return MF_OK;
 }
 
-Params common(const MfGatedMlpArgs* a, int m, int n, int k, const BoundedWaits& waits) {
+Params common(long long m, long long n, long long k, const BoundedWaits& waits) {
   Params p{};
-  p.m = m, p.n = n, p.k = k, p.splits = 1, p.k_blocks_per_split = (k + kBlockK - 1) / kBlockK;
-  p.activation = a->activation, p.waits = waits;
+  p.one.m = (int)m, p.one.n = (int)n, p.k = (int)k, p.waits = waits;
   return p;
 }
 
@@ -140,59 +157,62 @@ Params common(const MfGatedMlpArgs* a, int m, int n, int k, const BoundedWaits& 
     }                                                                                                          \
   } while (0)
 
-// D (m, n) = A B^T + bias, tiles of 256 or 128 columns, whichever leaves fewer columns to the longest-running pair
-template <typename T, bool kAMn, bool kBMn>
-int product(Params& p, cudaStream_t stream, const char* what) {
-  const long long tm = (p.m + 255) / 256, wide = (tm * ((p.n + 255) / 256) + kPairs - 1) / kPairs * 2, narrow = (tm * ((p.n + 127) / 128) + kPairs - 1) / kPairs;
-  return narrow < wide ? launch<T, kAMn, kBMn, 128, kStore>(p, stream, what) : launch<T, kAMn, kBMn, 256, kStore>(p, stream, what);
-}
-
 template <typename T>
 int forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t stream) {
   const long long M = a->rows, C = a->dim, F = a->hidden, O = a->dim_out;
   const T* w_in = static_cast<const T*>(a->w_in);
-  Params p = common(a, (int)M, (int)F, (int)C, waits);
+  Params p = common(M, F, C, waits);
   p.bias = a->b_in, p.keep_pre = a->pre != nullptr;
-  MF_MAP(map16<T>(&p.a, a->x, M, C, C, 64));
-  MF_MAP(map16<T>(&p.b, w_in, F, C, C, 64));
+  MF_MAP(map16<T>(&p.one.a, a->x, M, C, C, 64));
+  MF_MAP(map16<T>(&p.one.b, w_in, F, C, C, 64));
   MF_MAP(map16<T>(&p.b2, w_in + F * C, F, C, C, 64));
-  MF_MAP(map16<T>(&p.out, a->act, M, F, F, 32));
+  MF_MAP(map16<T>(&p.one.out, a->act, M, F, F, 32));
   if (a->pre) {
     MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32));
     MF_MAP(map16<T>(&p.pre2, static_cast<T*>(a->pre) + F, M, F, 2 * F, 32));
   }
-  int rc = launch<T, false, false, 256, kGate>(p, stream, "gated_mlp gate product");
+  int rc = launch<T, false, false, kGate>(p, a->activation, stream, "gated_mlp gate product");
   if (rc != MF_OK) return rc;
-  p = common(a, (int)M, (int)O, (int)F, waits);
+  p = common(M, O, F, waits);
   p.bias = a->b_out;
-  MF_MAP(map16<T>(&p.a, a->act, M, F, F, 64));
-  MF_MAP(map16<T>(&p.b, a->w_out, O, F, F, 64));
-  MF_MAP(map16<T>(&p.out, a->y, M, O, O, 32));
-  return product<T, false, false>(p, stream, "gated_mlp output product");
+  MF_MAP(map16<T>(&p.one.a, a->act, M, F, F, 64));
+  MF_MAP(map16<T>(&p.one.b, a->w_out, O, F, F, 64));
+  MF_MAP(map16<T>(&p.one.out, a->y, M, O, O, 32));
+  return launch<T, false, false, kStore>(p, 0, stream, "gated_mlp output product");
 }
 
-// gradient (m, n) of a weight: the sum over the tokens of left (tokens, m) x right (tokens, n)
+// One of the two weight gradients: the sum over the tokens of left (tokens, m) x right (tokens, n).
 template <typename T>
-int weight_gradient(const MfGatedMlpArgs* a, const void* left, int m, const void* right, int n, void* out, float* planes, const BoundedWaits& waits,
-                    cudaStream_t stream) {
-  const Weight w = weight_plan(a->rows, m, n);
-  Params p = common(a, m, n, (int)a->rows, waits);
-  p.splits = w.splits, p.k_blocks_per_split = w.per_split;
-  MF_MAP(map16<T>(&p.a, left, a->rows, m, m, 64));
-  MF_MAP(map16<T>(&p.b, right, a->rows, n, n, 64));
-  const bool direct = w.splits == 1;
-  if (direct && a->grad_dtype != MF_DTYPE_F32) {
-    MF_MAP(map16<T>(&p.out, out, m, n, n, 32));
-    return launch<T, true, true, 256, kStore>(p, stream, "gated_mlp weight gradient");
+bool weight_problem(Problem& q, const MfGatedMlpArgs* a, const void* left, long long m, const void* right, long long n, void* out) {
+  const long long dims[2] = {n, m}, strides[1] = {4 * n};
+  q.m = (int)m, q.n = (int)n;
+  return map16<T>(&q.a, left, a->rows, m, m, 64) && map16<T>(&q.b, right, a->rows, n, n, 64) &&
+         (a->grad_dtype == MF_DTYPE_F32 ? make_tensor_map(&q.out, out, MF_DTYPE_F32, 2, dims, strides, 32, 32) : map16<T>(&q.out, out, m, n, n, 32));
+}
+
+template <typename T>
+int weight_gradients(const MfGatedMlpArgs* a, const void* grad_pre, float* planes, const BoundedWaits& waits, cudaStream_t stream) {
+  const int C = a->dim, F = a->hidden, O = a->dim_out;
+  const WeightPlan w = weight_plan(a);
+  Params p{};
+  p.k = (int)a->rows, p.waits = waits, p.wide_out = a->grad_dtype == MF_DTYPE_F32;
+  p.whole = w.whole, p.rest = w.rest, p.per = w.per, p.first2 = w.tiles1, p.tiles = w.whole + w.rest * w.pieces;
+  p.one.m = 2 * F, p.one.n = C;
+  if (w.tiles1) MF_MAP(weight_problem<T>(p.one, a, grad_pre, 2 * F, a->x, C, a->grad_w_in));
+  if (w.tiles2) MF_MAP(weight_problem<T>(p.two, a, a->grad_y, O, a->act, F, a->grad_w_out));
+  if (w.rest) {
+    const long long dims[2] = {kTile, (long long)w.rest * w.pieces * kTile}, strides[1] = {4 * kTile};
+    MF_MAP(make_tensor_map(&p.pre, planes, MF_DTYPE_F32, 2, dims, strides, 32, 32));
   }
-  const long long dims[3] = {n, m, w.splits}, strides[2] = {4ll * n, 4ll * n * m};
-  MF_MAP(make_tensor_map(&p.out, direct ? out : planes, MF_DTYPE_F32, 3, dims, strides, 32, 32));
-  const int rc = launch<T, true, true, 256, kStoreF32>(p, stream, "gated_mlp weight gradient");
-  if (rc != MF_OK || direct) return rc;
-  const long long count = (long long)m * n;
-  const dim3 grid((unsigned)((count / 4 + 255) / 256));
-  if (a->grad_dtype == MF_DTYPE_F32) launch_dependent(add_planes_kernel<float>, grid, dim3(256), 0, stream, planes, w.splits, count, static_cast<float*>(out));
-  else launch_dependent(add_planes_kernel<T>, grid, dim3(256), 0, stream, planes, w.splits, count, static_cast<T*>(out));
+  const int rc = launch_kernel<T, true, true, kWeight, 0>(p, p.tiles < kPairs ? p.tiles : kPairs, stream, "gated_mlp weight gradients");
+  if (rc != MF_OK || w.rest == 0) return rc;
+  auto add = [&](auto* out1) {
+    using TOut = std::remove_pointer_t<decltype(out1)>;
+    launch_dependent(add_planes_kernel<T, TOut>, dim3(w.rest, kTile / 4), dim3(256), 0, stream, planes, w, static_cast<TOut*>(a->grad_w_in), 2 * F, C,
+                     static_cast<TOut*>(a->grad_w_out), O, F);
+  };
+  if (p.wide_out) add(static_cast<float*>(nullptr));
+  else add(static_cast<T*>(nullptr));
   MF_CHECK_LAUNCH("add_planes_kernel");
   return MF_OK;
 }
@@ -207,25 +227,24 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
   float *planes = reinterpret_cast<float*>(ws + at[1]), *sums = reinterpret_cast<float*>(ws + at[2]), *bands = reinterpret_cast<float*>(ws + at[3]);
   int rc;
   if (a->grad_x || a->grad_w_in || a->grad_b_in) {
-    Params p = common(a, (int)M, (int)F, (int)O, waits);
+    Params p = common(M, F, O, waits);
     p.column_sums = a->grad_b_in ? sums : nullptr;
-    MF_MAP(map16<T>(&p.a, a->grad_y, M, O, O, 64));
-    MF_MAP(map16<T>(&p.b, a->w_out, O, F, F, 64));
+    MF_MAP(map16<T>(&p.one.a, a->grad_y, M, O, O, 64));
+    MF_MAP(map16<T>(&p.one.b, a->w_out, O, F, F, 64));
     MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32));
     MF_MAP(map16<T>(&p.pre2, static_cast<const T*>(a->pre) + F, M, F, 2 * F, 32));
-    MF_MAP(map16<T>(&p.out, grad_pre, M, F, 2 * F, 32));
+    MF_MAP(map16<T>(&p.one.out, grad_pre, M, F, 2 * F, 32));
     MF_MAP(map16<T>(&p.out2, grad_pre + F, M, F, 2 * F, 32));
-    if ((rc = launch<T, false, true, 256, kGateGrad>(p, stream, "gated_mlp gate gradient")) != MF_OK) return rc;
+    if ((rc = launch<T, false, true, kGateGrad>(p, a->activation, stream, "gated_mlp gate gradient")) != MF_OK) return rc;
   }
   if (a->grad_x) {
-    Params p = common(a, (int)M, (int)C, (int)(2 * F), waits);
-    MF_MAP(map16<T>(&p.a, grad_pre, M, 2 * F, 2 * F, 64));
-    MF_MAP(map16<T>(&p.b, a->w_in, 2 * F, C, C, 64));
-    MF_MAP(map16<T>(&p.out, a->grad_x, M, C, C, 32));
-    if ((rc = product<T, false, true>(p, stream, "gated_mlp input gradient")) != MF_OK) return rc;
+    Params p = common(M, C, 2 * F, waits);
+    MF_MAP(map16<T>(&p.one.a, grad_pre, M, 2 * F, 2 * F, 64));
+    MF_MAP(map16<T>(&p.one.b, a->w_in, 2 * F, C, C, 64));
+    MF_MAP(map16<T>(&p.one.out, a->grad_x, M, C, C, 32));
+    if ((rc = launch<T, false, true, kStore>(p, 0, stream, "gated_mlp input gradient")) != MF_OK) return rc;
   }
-  if (a->grad_w_in && (rc = weight_gradient<T>(a, grad_pre, (int)(2 * F), a->x, (int)C, a->grad_w_in, planes, waits, stream)) != MF_OK) return rc;
-  if (a->grad_w_out && (rc = weight_gradient<T>(a, a->grad_y, (int)O, a->act, (int)F, a->grad_w_out, planes, waits, stream)) != MF_OK) return rc;
+  if ((a->grad_w_in || a->grad_w_out) && (rc = weight_gradients<T>(a, grad_pre, planes, waits, stream)) != MF_OK) return rc;
   if (a->grad_b_in && (rc = column_sums(sums, MF_DTYPE_F32, (M + 31) / 32, (int)(2 * F), a->grad_b_in, a->grad_dtype, bands, stream)) != MF_OK) return rc;
   if (a->grad_b_out && (rc = column_sums(a->grad_y, a->dtype, M, (int)O, a->grad_b_out, a->grad_dtype, bands, stream)) != MF_OK) return rc;
   return MF_OK;

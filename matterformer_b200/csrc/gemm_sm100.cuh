@@ -2,10 +2,13 @@
 // tensor copies, the element-wise work around the product in its epilogue.  gated_mlp.cu has the operators and the reasons for
 // the tiles.
 //
-// Two CTAs of a cluster work on one 256 x kN tile (cta_group::2): each holds 128 rows of A and half of B's rows in its shared memory
+// Two CTAs of a cluster work on one 256 x 256 tile (cta_group::2): each holds 128 rows of A and half of B's rows in its shared memory
 // and 128 rows of the result in its tensor memory, so that a byte from L2 serves twice the products that a CTA alone would
 // get from it.  Warp 0 copies, warp 1 of the even CTA issues the products, warps 4-11 of both store the result: they work on one
 // of two accumulators while the products of the next tile fill the other.  The CTAs walk the tiles with the stride of the grid.
+// 256 columns at 8192 x 2048 x 4096: 95 us, 1441 TFLOP/s (cuBLAS at 8192^3: 1644); 128 columns: 108 us, the copies bound it.
+//
+// A last round of tiles that would leave half of the pairs or more without work is cut into tiles of 128 or 64 columns.
 //
 // An operand is stored with its contracted dimension innermost ("K-major": A (M, K), B (N, K)) or outermost (MN-major: A (K, M),
 // B (K, N)); both land as boxes of 64 lines of 128 bytes that the shared-memory descriptors describe.  Boxes beyond the matrix are
@@ -25,38 +28,48 @@ namespace gemm {
 
 __device__ int32_t g_gemm_status = 0;  // MF_ERR_DEVICE_TIMEOUT after an expired wait
 
-enum Epilogue { kGate, kGateGrad, kStore, kStoreF32 };
+// kGate: two projections, activation and product;  kGateGrad: its gradient;  kStore: the product and a bias;  kWeight: one or two
+// products over the same long dimension, which is cut into pieces for the tiles behind the last whole round
+enum Epilogue { kGate, kGateGrad, kStore, kWeight };
 
 constexpr int kBlockK = 64;                       // elements of the contracted dimension in a stage
 constexpr int kBoxBytes = 64 * 128;               // 64 lines of 64 16-bit elements
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (4 + kEpilogueWarps);
+constexpr int kStageBytes = 4 * kBoxBytes;        // 128 rows of A, 128 of B
 constexpr int kStageBuffer = 32 * 128;            // what a warp hands to the copy engine at once: 32 rows of 128 bytes
-constexpr int kMaxSmem = 232448;
+constexpr int kTile = 256;
+constexpr int kTmemCols = 512;
 
-template <int kN, Epilogue kEpi>
+template <Epilogue kEpi>
 struct Shape {
-  static constexpr int kBoxesA = 2, kBoxesB = kN / 2 / 64;  // of one CTA
-  static constexpr int kStageBytes = (kBoxesA + kBoxesB) * kBoxBytes;
-  static constexpr int kBuffers = kEpi == kGateGrad ? 4 : kEpi == kGate ? 3 : 2;  // of 4 KB for each storing warp
+  static constexpr int kBuffers = kEpi == kGateGrad ? 4 : 2;  // of 4 KB for each storing warp
   static constexpr int kBufferBytes = kEpilogueWarps * kBuffers * kStageBuffer;
-  static constexpr int kStages = (kMaxSmem - 1024 - 1024 - kBufferBytes) / kStageBytes < 8 ? (kMaxSmem - 1024 - 1024 - kBufferBytes) / kStageBytes : 8;
+  static constexpr int kStages = kEpi == kGateGrad ? 3 : 5;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kBufferBytes;
-  static_assert(kStages >= 3, "too few stages");
-  static constexpr int kTmemCols = 2 * kN;
+  static_assert(kSmem + 1024 <= 232448, "shared memory");
+};
+
+struct Problem {
+  CUtensorMap a, b;  // boxes of 64 lines
+  CUtensorMap out;   // boxes of 32 lines (kWeight: fp32 or 16-bit elements)
+  int m, n;
 };
 
 struct Params {
-  CUtensorMap a, b;         // boxes of 64 lines; b: of the even CTA's half where the halves are different matrices (kGate)
-  CUtensorMap b2;           // kGate: the odd CTA's (the rows of the up projection)
-  CUtensorMap out, out2;    // boxes of 32 lines.  kGate: hidden | -;  kGateGrad: gradients of gate | up;  else the result
-  CUtensorMap pre, pre2;    // pre-activations of gate | up (kGate: written if keep_pre; kGateGrad: read)
-  const void* bias;         // kGate: (2 F), kStore: (N); may be null
-  float* column_sums;       // kGateGrad: (ceil(M / 32), 2 F) partial sums of the stored rows, or null
-  int m, n, k;              // kGate, kGateGrad: n = F
-  int splits, k_blocks_per_split;  // kStoreF32: the contracted dimension in `splits` pieces, each with a plane of its own
-  int activation;
+  Problem one;
+  Problem two;              // kWeight: the second product
+  CUtensorMap b2;           // kGate: the rows of the up projection, the odd CTA's
+  CUtensorMap out2;         // kGateGrad: gradients of up
+  CUtensorMap pre, pre2;    // pre-activations of gate | up (kGate: written if keep_pre; kGateGrad: read); kWeight: pre = planes of partial sums
+  const void* bias;         // kGate: (2 n), kStore: (n); may be null
+  float* column_sums;       // kGateGrad: (ceil(m / 32), 2 n) sums of the stored rows, or null
+  int k;
+  int whole, cut, tiles;    // tiles of full width, columns of a later one = full width / cut, pieces of work in all
+  int first2;               // kWeight: the second product's first tile
+  int rest, per;            // kWeight: tiles that are cut along the contracted dimension, and how many blocks a piece has
   int keep_pre;
+  int wide_out;             // kWeight: fp32 results
   BoundedWaits waits;       // kinds: 0 operands, 1 stages, 2 accumulators, 3 drained accumulators
 };
 
@@ -99,6 +112,9 @@ __device__ __forceinline__ void umma_commit2(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
                "h"((uint16_t)3)
                : "memory");
+}
+__device__ __forceinline__ void umma_commit_own(uint64_t* bar) {  // in this CTA only
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // One 64 x 64 box into this CTA; its bytes are counted on the barrier `bar` (a cluster address) of the even CTA.
 __device__ __forceinline__ void load_box2(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -159,70 +175,161 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
 
-// kind::f16 with fp32 sums: D format (bits 4-5) 1 = f32, A (7-9) and B (10-12) 0 = f16, 1 = bf16
-template <typename T, bool kAMn, bool kBMn, int kN>
+// kind::f16 with fp32 sums: D format (bits 4-5) 1 = f32, A (7-9) and B (10-12) 0 = f16, 1 = bf16; the columns go to bits 17-22
+template <typename T, bool kAMn, bool kBMn>
 __host__ __device__ constexpr uint32_t instruction() {
   constexpr uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)kAMn << 15) | ((uint32_t)kBMn << 16) | ((uint32_t)(kN >> 3) << 17) | ((256u >> 4) << 24);
+  return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)kAMn << 15) | ((uint32_t)kBMn << 16) | ((256u >> 4) << 24);
 }
 
 // ---- activations ---------------------------------------------------------------------------------------------------
 // act(z) = z s(w(z)) with the logistic function s: w = z is SiLU; w = 2 sqrt(2/pi) (z + 0.044715 z^3) is GELU in its tanh form, since
 // (1 + tanh(a)) / 2 = s(2 a), and nothing cancels for large negative z.  The derivative is s + z s (1 - s) w'.
-// Beyond |z| = 64 both are 0 or z (1 for the derivative) in fp32: the clamp keeps the cube and w' finite.
-struct Act {
-  float value, slope;
-};
-template <bool kSlope>
-__device__ __forceinline__ Act activation(float z, int kind) {
-  float w = z, dw = 1.f;
-  if (kind == MF_ACT_GELU_TANH) {
-    const float c = fminf(fmaxf(z, -64.f), 64.f), c2 = c * c;
-    w = 1.5957691216057308f * c * (1.f + 0.044715f * c2);
-    dw = 1.5957691216057308f * (1.f + 3.f * 0.044715f * c2);
+// Beyond |z| = 64 GELU is 0 or z in fp32: the clamp keeps the cube and w' finite.
+template <int kAct>
+__device__ __forceinline__ float2 logistic2(float2 z, float2& slope) {  // slope: w'
+  constexpr float kLog2e = 1.4426950408889634f;
+  float2 w = mul2(z, make_float2(-kLog2e, -kLog2e));
+  if constexpr (kAct == MF_ACT_GELU_TANH) {
+    constexpr float kBeta = 1.5957691216057308f, kKappa = 0.044715f;
+    const float2 c = make_float2(fminf(fmaxf(z.x, -64.f), 64.f), fminf(fmaxf(z.y, -64.f), 64.f)), c2 = mul2(c, c);
+    const float a = -kLog2e * kBeta;
+    w = mul2(c, fma2(c2, make_float2(a * kKappa, a * kKappa), make_float2(a, a)));
+    slope = fma2(c2, make_float2(3.f * kBeta * kKappa, 3.f * kBeta * kKappa), make_float2(kBeta, kBeta));
   }
-  const float s = __fdividef(1.f, 1.f + __expf(-w));
-  Act r;
-  r.value = z * s;
-  r.slope = kSlope ? s + r.value * (1.f - s) * dw : 0.f;
-  return r;
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(w.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(w.y));
+  e = add2(e, make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
+  return e;
+}
+template <int kAct>
+__device__ __forceinline__ float2 activation2(float2 z) {
+  float2 unused;
+  return mul2(z, logistic2<kAct>(z, unused));
+}
+// act(z) and act'(z)
+template <int kAct>
+__device__ __forceinline__ void activation2(float2 z, float2& value, float2& slope) {
+  float2 dw;
+  const float2 s = logistic2<kAct>(z, dw);
+  value = mul2(z, s);
+  float2 t = mul2(value, fma2(s, make_float2(-1.f, -1.f), make_float2(1.f, 1.f)));
+  if constexpr (kAct == MF_ACT_GELU_TANH) t = mul2(t, dw);
+  slope = add2(s, t);
 }
 
-// Eight values of a bias from column c on (a multiple of 8); zeros behind the last.
+// Eight 16-bit values of a bias from column c on (a multiple of 8); zeros from column n on (n = 0: there is no bias).
 template <typename T>
-__device__ __forceinline__ void bias8(const T* bias, int c, int n, float (&b)[8]) {
-  const uint4 v = c < n ? __ldg(reinterpret_cast<const uint4*>(bias + c)) : make_uint4(0u, 0u, 0u, 0u);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack2<T>(w[i]);
-    b[2 * i] = f.x, b[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ uint4 bias8(const T* bias, int c, int n) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (c < n) v = *reinterpret_cast<const uint4*>(bias + c);
+  return v;
 }
 
 // Where 16 bytes `chunk` of line `row` of a box lie.
 __device__ __forceinline__ uint32_t box_chunk(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
-// Tiles are walked in groups of rows that stay in L2 together: all columns of kGroup row tiles, the row tiles fastest.
-constexpr int kGroup = 8;
-struct Tile {
-  int m, n, split;
-};
-__device__ __forceinline__ Tile tile_at(int t, int tiles_m, int tiles_n) {
-  Tile r;
-  const int plane = tiles_m * tiles_n;
-  r.split = t / plane;
-  t -= r.split * plane;
-  const int group = t / (kGroup * tiles_n), first = group * kGroup, rows = min(kGroup, tiles_m - first);
-  t -= first * tiles_n;
-  r.m = first + t % rows;
-  r.n = t / rows;
-  return r;
+// Column sums of a warp's buffer of 32 lines: 1 x 32 ones times the lines, on mma.sync; lane l returns columns 2 l and 2 l + 1.  As
+// loads and additions they were a fifth of the instructions around the product.
+template <typename T>
+__device__ __forceinline__ float2 column_sums32(uint32_t buffer, int lane) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  const uint32_t one = kBf16 ? 0x3f803f80u : 0x3c003c00u;
+  float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {  // 16 columns
+    float d[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // 16 lines
+      uint32_t b[4];
+      const uint32_t at = buffer + box_chunk(16 * k + (lane & 15), 2 * c + (lane >> 4));
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
+                   : "r"(at)
+                   : "memory");
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (kBf16)
+          asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %4, %4, %4}, {%5, %6}, {%0, %1, %2, %3};"
+              : "+f"(d[t][0]), "+f"(d[t][1]), "+f"(d[t][2]), "+f"(d[t][3])
+              : "r"(one), "r"(b[2 * t]), "r"(b[2 * t + 1]));
+        else
+          asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %4, %4, %4}, {%5, %6}, {%0, %1, %2, %3};"
+              : "+f"(d[t][0]), "+f"(d[t][1]), "+f"(d[t][2]), "+f"(d[t][3])
+              : "r"(one), "r"(b[2 * t]), "r"(b[2 * t + 1]));
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)  // every line of the result is the same: lanes 4 i .. 4 i + 3 keep the eight columns i
+      if ((lane >> 2) == 2 * c + t) sum = make_float2(d[t][0], d[t][1]);
+  }
+  return sum;
 }
 
-template <typename T, bool kAMn, bool kBMn, int kN, Epilogue kEpi>
+// ---- the order of the work -----------------------------------------------------------------------------------------
+// What a pair does at a time: `cols` columns from `col` of the rows from `row` on, over the blocks [k0, k1) of the contracted dimension.
+struct Work {
+  int row, col, cols, k0, k1;
+  bool second;  // of the second product (kWeight)
+  int plane;    // where a part of a tile goes; -1: the whole
+};
+
+// Tiles are walked in groups of rows that stay in L2 together: all columns of kGroup row tiles, the row tiles fastest.
+constexpr int kGroup = 8;
+__host__ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int& m, int& n) {
+  const int group = t / (kGroup * tiles_n), first = group * kGroup, rows = tiles_m - first < kGroup ? tiles_m - first : kGroup;
+  t -= first * tiles_n;
+  m = first + t % rows;
+  n = t / rows;
+}
+
+template <Epilogue kEpi>
+struct Walk {
+  const Params& p;
+  int pairs, k_blocks, tiles_m, tiles_n, t;
+  __device__ Walk(const Params& q, int pair, int pairs_) : p(q), pairs(pairs_), t(pair) {
+    k_blocks = (p.k + kBlockK - 1) / kBlockK;
+    tiles_m = (p.one.m + kTile - 1) / kTile;
+    tiles_n = (p.one.n + full() - 1) / full();
+  }
+  __device__ static constexpr int full() { return kEpi == kGate ? kTile / 2 : kTile; }
+  __device__ bool next(Work& w) {
+    if (t >= p.tiles) return false;
+    const bool whole = t < p.whole;
+    int m, n;
+    w.second = false, w.plane = -1, w.cols = full(), w.k0 = 0, w.k1 = k_blocks;
+    if constexpr (kEpi == kWeight) {
+      // The same piece of all cut tiles comes before the next piece of any: pairs that work at the same time read the same stretch of
+      // the operands.  (Equal shares of all blocks in a row, where each pair is somewhere else, took 210 us instead of 100 on
+      // 29 696 tokens: all operands came from memory again and again.)
+      int tile = t;
+      if (!whole) {
+        const int u = t - p.whole;
+        tile = p.whole + u % p.rest;
+        w.k0 = u / p.rest * p.per, w.k1 = min(k_blocks, w.k0 + p.per), w.plane = u;
+      }
+      w.second = tile >= p.first2;
+      if (w.second) tile_at(tile - p.first2, (p.two.m + kTile - 1) / kTile, (p.two.n + kTile - 1) / kTile, m, n);
+      else tile_at(tile, tiles_m, tiles_n, m, n);
+      w.col = n * kTile;
+    } else {
+      const int part = whole ? 0 : (t - p.whole) % p.cut, tile = whole ? t : p.whole + (t - p.whole) / p.cut;
+      if (!whole) w.cols = full() / p.cut;
+      tile_at(tile, tiles_m, tiles_n, m, n);
+      w.col = n * full() + part * w.cols;
+    }
+    w.row = m * kTile;
+    t += pairs;
+    return true;
+  }
+};
+
+template <typename T, bool kAMn, bool kBMn, Epilogue kEpi, int kAct>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Params p) {
-  using Sh = Shape<kN, kEpi>;
+  using Sh = Shape<kEpi>;
   constexpr int kStages = Sh::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -232,10 +339,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  constexpr int kTileN = kEpi == kGate ? kN / 2 : kN;  // columns of the result in a tile
-  const int tiles_m = (p.m + 255) / 256, tiles_n = (p.n + kTileN - 1) / kTileN;
-  const int tiles = tiles_m * tiles_n * p.splits;
-  const int k_blocks = (p.k + kBlockK - 1) / kBlockK;
 
   if (threadIdx.x == 0) {
     const int w = p.waits.withheld;
@@ -246,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     mbar_fence_init();
   }
   if (warp == 2) {
-    tmem_alloc2(&tmem_base_s, Sh::kTmemCols);
+    tmem_alloc2(&tmem_base_s, kTmemCols);
     tmem_relinquish2();
   }
   tc_fence_before_sync();
@@ -256,34 +359,41 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   launch_dependents();
   wait_for_previous();
 
+  Walk<kEpi> walk(p, pair, pairs);
+  Work w;
   bool bad = false;
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
     if (elect_one()) {
       uint32_t it = 0;
-      for (int t = pair; t < tiles && !bad; t += pairs) {
-        const Tile tile = tile_at(t, tiles_m, tiles_n);
-        const int kb0 = tile.split * p.k_blocks_per_split, kb1 = min(k_blocks, kb0 + p.k_blocks_per_split);
-        const int row = tile.m * 256 + 128 * (int)rank;
-        const CUtensorMap* bmap = kEpi == kGate && rank ? &p.b2 : &p.b;
-        const int col = kEpi == kGate ? tile.n * kTileN : tile.n * kN + (kN / 2) * (int)rank;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      while (!bad && walk.next(w)) {
+        const CUtensorMap* amap = kEpi == kWeight && w.second ? &p.two.a : &p.one.a;
+        const CUtensorMap* bmap = kEpi == kWeight && w.second ? &p.two.b : kEpi == kGate && rank ? &p.b2 : &p.one.b;
+        const int row = w.row + 128 * (int)rank;
+        const int col = kEpi == kGate ? w.col : w.col + w.cols / 2 * (int)rank;
+        const bool two = (kEpi == kGate ? w.cols : w.cols / 2) > 64;  // boxes of B (a tile of 64 columns uses half of its box)
+        for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int s = it % kStages;
-          const uint32_t phase = (it / kStages) & 1;
-          if (it >= kStages && !mbar_wait_for(&bar_empty[s], phase ^ 1, p.waits.limit)) {
+          if (it >= kStages && !mbar_wait_for(&bar_empty[s], ((it / kStages) & 1) ^ 1, p.waits.limit)) {
             bad = true;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&bar_full[s], 2 * Sh::kStageBytes);
-          const uint32_t bar = map_to_rank(smem_u32(&bar_full[s]), 0), dst = smem + s * Sh::kStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&bar_full[s], 2 * (two ? 4 : 3) * kBoxBytes);
+          const uint32_t bar = map_to_rank(smem_u32(&bar_full[s]), 0), dst = smem + s * kStageBytes;
 #pragma unroll
-          for (int i = 0; i < Sh::kBoxesA; ++i)
-            load_box2(dst + i * kBoxBytes, &p.a, kAMn ? row + 64 * i : kb * kBlockK, kAMn ? kb * kBlockK : row + 64 * i, bar);
+          for (int i = 0; i < 2; ++i)
+            load_box2(dst + i * kBoxBytes, amap, kAMn ? row + 64 * i : kb * kBlockK, kAMn ? kb * kBlockK : row + 64 * i, bar);
 #pragma unroll
-          for (int i = 0; i < Sh::kBoxesB; ++i)
-            load_box2(dst + (Sh::kBoxesA + i) * kBoxBytes, bmap, kBMn ? col + 64 * i : kb * kBlockK, kBMn ? kb * kBlockK : col + 64 * i, bar);
+          for (int i = 0; i < 2; ++i)
+            if (i == 0 || two)
+              load_box2(dst + (2 + i) * kBoxBytes, bmap, kBMn ? col + 64 * i : kb * kBlockK, kBMn ? kb * kBlockK : col + 64 * i, bar);
         }
       }
+      // The last products' arrivals on the stages of both CTAs are waited for as well: they come from the even CTA, and one that found the
+      // odd one gone would write to whatever runs there next.
+      if (!bad)
+        for (uint32_t i = it > kStages ? it - kStages : 0; i < it && !bad; ++i)
+          bad = !mbar_wait_for(&bar_empty[i % kStages], (i / kStages) & 1, p.waits.limit);
       if (bad && rank == 0) {  // copies that still fly write to these CTAs: their bytes arrive here (once a wait has lasted its second, all have)
         for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
           if (!mbar_wait(&bar_full[i % kStages], (i / kStages) & 1)) break;
@@ -292,241 +402,265 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   } else if (warp == 1 && rank == 0) {
     // ---------------------------------------------------------------- products
     if (elect_one()) {
-      constexpr uint32_t idesc = instruction<T, kAMn, kBMn, kN>();
       // K-major: 16 elements of a line further on; MN-major: 16 lines further on, 64-wide chunks a box apart
       constexpr uint32_t kStepA = kAMn ? 16 * 128 : 32, kStepB = kBMn ? 16 * 128 : 32;
       const uint64_t a0 = make_smem_desc_sw128(smem, kAMn ? kBoxBytes : 0, 1024);
-      const uint64_t b0 = make_smem_desc_sw128(smem + Sh::kBoxesA * kBoxBytes, kBMn ? kBoxBytes : 0, 1024);
+      const uint64_t b0 = make_smem_desc_sw128(smem + 2 * kBoxBytes, kBMn ? kBoxBytes : 0, 1024);
       uint32_t it = 0;
-      int n = 0;
-      for (int t = pair; t < tiles && !bad; t += pairs, ++n) {
-        const Tile tile = tile_at(t, tiles_m, tiles_n);
-        const int kb0 = tile.split * p.k_blocks_per_split, kb1 = min(k_blocks, kb0 + p.k_blocks_per_split);
+      for (int n = 0; !bad && walk.next(w); ++n) {
         const int buf = n & 1;
         if (n >= 2 && !mbar_wait_for(&bar_drained[buf], ((n >> 1) & 1) ^ 1, p.waits.limit)) {
           bad = true;
           break;
         }
         tc_fence_after_sync();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const uint32_t idesc = instruction<T, kAMn, kBMn>() | ((uint32_t)((kEpi == kGate ? 2 * w.cols : w.cols) >> 3) << 17);
+        for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int s = it % kStages;
           if (!mbar_wait_for(&bar_full[s], (it / kStages) & 1, p.waits.limit)) {
             bad = true;
             break;
           }
           tc_fence_after_sync();
-          const uint64_t a = desc_advance(a0, s * Sh::kStageBytes), b = desc_advance(b0, s * Sh::kStageBytes);
+          const uint64_t a = desc_advance(a0, s * kStageBytes), b = desc_advance(b0, s * kStageBytes);
 #pragma unroll
           for (int k = 0; k < kBlockK / 16; ++k)
-            umma2(tmem + buf * kN, desc_advance(a, k * kStepA), desc_advance(b, k * kStepB), idesc, kb > kb0 || k > 0);
+            umma2(tmem + buf * kTile, desc_advance(a, k * kStepA), desc_advance(b, k * kStepB), idesc, kb > w.k0 || k > 0);
           umma_commit2(&bar_empty[s]);
         }
         if (!bad) umma_commit2(&bar_acc[buf]);
       }
       if (bad) {  // no product may still run when the tensor memory is freed
-        umma_commit2(&bar_end);
+        umma_commit_own(&bar_end);
         mbar_wait(&bar_end, 0);
       }
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- results
     const int ew = warp - 4, quad = warp & 3, half = ew >> 2;
-    const uint32_t buffers = smem + kStages * Sh::kStageBytes + ew * Sh::kBuffers * kStageBuffer;
+    const uint32_t buffers = smem + kStages * kStageBytes + ew * Sh::kBuffers * kStageBuffer;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * quad) << 16);
-    int n = 0;
-    uint32_t chunk = 0, fetched = 0;  // chunks of columns, counted over all tiles
-    constexpr int kHalf = kTileN / 2;              // columns of the result that this warp stores
-    constexpr int kChunks = kHalf / 64;
+    const int lane_row = 128 * (int)rank + 32 * quad;
+    uint32_t chunk = 0, fetched = 0;  // chunks of 64 columns (buffers handed over), counted over all tiles
 
-    // the pre-activations of chunk c of tile t, the i-th in all, on their way to buffers 2 (i & 1) and 2 (i & 1) + 1
-    auto fetch = [&](int t, int c) {
+    // a line of 64 16-bit columns of this lane's row, then the box
+    auto put = [&](uint32_t dst, const uint32_t* words) {
+#pragma unroll
+      for (int v = 0; v < 8; ++v) sts128(dst + box_chunk(lane, v), make_uint4(words[4 * v], words[4 * v + 1], words[4 * v + 2], words[4 * v + 3]));
+      fence_smem_to_async_proxy();
+      __syncwarp();
+    };
+    auto next_buffer = [&]() {  // of two in turn, once its previous contents have left
+      if (lane == 0) store_wait_read<1>();
+      __syncwarp();
+      return buffers + (chunk++ & 1) * kStageBuffer;
+    };
+    // Columns of a tile that this warp stores: half of them, all of them or none where they are a single chunk.
+    auto mine = [&](const Work& x, int& first) {
+      const int chunks = x.cols >= 128 ? x.cols / 128 : half == 0;
+      first = half * (x.cols / 2);
+      return chunks;
+    };
+    // kGateGrad: the pre-activations of 64 columns on their way to buffers 2 (i & 1) and 2 (i & 1) + 1
+    auto fetch = [&](int col, int row) {
       const uint32_t i = fetched++;
-      const Tile tile = tile_at(t, tiles_m, tiles_n);
-      const int row = tile.m * 256 + 128 * (int)rank + 32 * quad, col = tile.n * kTileN + half * kHalf + 64 * c;
       uint64_t* bar = &bar_in[2 * ew + (i & 1)];
       const uint32_t dst = buffers + 2 * (i & 1) * kStageBuffer;
       mbar_arrive_expect_tx(bar, 2 * kStageBuffer);
       load_box(dst, &p.pre, col, row, bar);
       load_box(dst + kStageBuffer, &p.pre2, col, row, bar);
     };
-    if (kEpi == kGateGrad && pair < tiles && lane == 0) fetch(pair, 0);
+    Work later;  // kGateGrad: the tile after this one
+    bool more = walk.next(later);
+    if constexpr (kEpi == kGateGrad) {
+      // a pair's later tiles are no wider: a warp with nothing to store in one has nothing in any after it
+      int first;
+      if (lane == 0 && more && mine(later, first)) fetch(later.col + first, later.row + lane_row);
+    }
 
-    for (int t = pair; t < tiles; t += pairs, ++n) {
-      const Tile tile = tile_at(t, tiles_m, tiles_n);
-      const int row0 = tile.m * 256 + 128 * (int)rank + 32 * quad, col0 = tile.n * kTileN + half * kHalf;
-      const int buf = n & 1;
+    for (int n = 0; more; ++n) {
+      w = later;
+      more = walk.next(later);
+      const int buf = n & 1, row0 = w.row + lane_row;
+      int first;
+      const int chunks = mine(w, first), col0 = w.col + first;
+      const uint32_t acc = lane_base + buf * kTile;
+      const T* bias = static_cast<const T*>(p.bias);
+      const int bias_n = bias ? p.one.n : 0;
+      uint4 bias_gate[2], bias_up[2];
+      if constexpr (kEpi == kGate) {
+#pragma unroll
+        for (int v = 0; v < 2; ++v) bias_gate[v] = bias8(bias, col0 + 8 * v, bias_n), bias_up[v] = bias8(bias + bias_n, col0 + 8 * v, bias_n);
+      }
       if (!mbar_wait_for(&bar_acc[buf], (n >> 1) & 1, p.waits.limit)) bad = true;
       bad = __any_sync(0xffffffffu, bad);
       if (bad) break;
       tc_fence_after_sync();
-      const uint32_t acc = lane_base + buf * kN;
+      auto drained = [&]() {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(map_to_rank(smem_u32(&bar_drained[buf]), 0));
+      };
+      if (chunks == 0) drained();
 
       if constexpr (kEpi == kGate) {
-        const T* bias = static_cast<const T*>(p.bias);
-        if (lane == 0) store_wait_read<0>();  // of the tile before
-        __syncwarp();
+        if (chunks) {  // 64 columns of gate and of up
+          // the hidden values go to a buffer as they are formed; the words of gate and up wait in registers for theirs
+          uint32_t words[2][32], g[2][16], u[2][16];
+          const uint32_t hidden = next_buffer();
+          tmem_ld16(acc + first, g[0]);
+          tmem_ld16(acc + w.cols + first, u[0]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t g[32], u[32];
-          tmem_ld32(acc + half * kHalf + 32 * c, g);
-          tmem_ld32(acc + kTileN + half * kHalf + 32 * c, u);
-          tmem_ld_wait();
-          if (c == 1) {
-            tc_fence_before_sync();
-            if (lane == 0) arrive_cluster(map_to_rank(smem_u32(&bar_drained[buf]), 0));
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld_wait();
+            const uint4 bg[2] = {bias_gate[0], bias_gate[1]}, bu[2] = {bias_up[0], bias_up[1]};
+            if (c < 3) {
+              tmem_ld16(acc + first + 16 * (c + 1), g[(c + 1) & 1]);
+              tmem_ld16(acc + w.cols + first + 16 * (c + 1), u[(c + 1) & 1]);
+#pragma unroll
+              for (int v = 0; v < 2; ++v) {
+                const int at = col0 + 16 * (c + 1) + 8 * v;
+                bias_gate[v] = bias8(bias, at, bias_n), bias_up[v] = bias8(bias + bias_n, at, bias_n);
+              }
+            } else {
+              drained();
+            }
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              const uint32_t bgw[4] = {bg[v].x, bg[v].y, bg[v].z, bg[v].w}, buw[4] = {bu[v].x, bu[v].y, bu[v].z, bu[v].w};
+              uint32_t hw[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int i = 8 * v + 2 * e;
+                const float2 gate = add2(make_float2(__uint_as_float(g[c & 1][i]), __uint_as_float(g[c & 1][i + 1])), unpack2<T>(bgw[e]));
+                const float2 up = add2(make_float2(__uint_as_float(u[c & 1][i]), __uint_as_float(u[c & 1][i + 1])), unpack2<T>(buw[e]));
+                const float2 h = mul2(activation2<kAct>(gate), up);
+                const int at = 8 * c + 4 * v + e;
+                hw[e] = pack2<T>(h.x, h.y);
+                words[0][at] = pack2<T>(gate.x, gate.y), words[1][at] = pack2<T>(up.x, up.y);
+              }
+              sts128(hidden + box_chunk(lane, 2 * c + v), make_uint4(hw[0], hw[1], hw[2], hw[3]));
+            }
           }
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            float bg[8] = {}, bu[8] = {};
-            if (bias) {
-              bias8(bias, col0 + 32 * c + 8 * v, p.n, bg);
-              bias8(bias + p.n, col0 + 32 * c + 8 * v, p.n, bu);
-            }
-            uint32_t hw[4], gw[4], uw[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float g0 = __uint_as_float(g[8 * v + 2 * e]) + bg[2 * e], g1 = __uint_as_float(g[8 * v + 2 * e + 1]) + bg[2 * e + 1];
-              const float u0 = __uint_as_float(u[8 * v + 2 * e]) + bu[2 * e], u1 = __uint_as_float(u[8 * v + 2 * e + 1]) + bu[2 * e + 1];
-              hw[e] = pack2<T>(activation<false>(g0, p.activation).value * u0, activation<false>(g1, p.activation).value * u1);
-              gw[e] = pack2<T>(g0, g1), uw[e] = pack2<T>(u0, u1);
-            }
-            const uint32_t at = buffers + box_chunk(lane, 4 * c + v);
-            sts128(at, make_uint4(hw[0], hw[1], hw[2], hw[3]));
-            if (p.keep_pre) {
-              sts128(at + kStageBuffer, make_uint4(gw[0], gw[1], gw[2], gw[3]));
-              sts128(at + 2 * kStageBuffer, make_uint4(uw[0], uw[1], uw[2], uw[3]));
-            }
-          }
-        }
-        fence_smem_to_async_proxy();
-        __syncwarp();
-        if (lane == 0 && row0 < p.m && col0 < p.n) {
-          store_box(&p.out, buffers, col0, row0);
+          fence_smem_to_async_proxy();
+          __syncwarp();
+          const bool stores = lane == 0 && row0 < p.one.m && col0 < p.one.n;
+          if (stores) store_box(&p.one.out, hidden, col0, row0);
+          if (lane == 0) store_commit();
           if (p.keep_pre) {
-            store_box(&p.pre, buffers + kStageBuffer, col0, row0);
-            store_box(&p.pre2, buffers + 2 * kStageBuffer, col0, row0);
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+              const uint32_t dst = next_buffer();
+              put(dst, words[side]);
+              if (stores) store_box(side ? &p.pre2 : &p.pre, dst, col0, row0);
+              if (lane == 0) store_commit();
+            }
           }
-          store_commit();
         }
       } else if constexpr (kEpi == kGateGrad) {
 #pragma unroll 1
-        for (int c = 0; c < kChunks; ++c, ++chunk) {
+        for (int c = 0; c < chunks; ++c, ++chunk) {
           // the next chunk's pre-activations, once the buffers' previous results have left
-          const bool last = c == kChunks - 1;
-          if (lane == 0 && (!last || t + pairs < tiles)) {
+          const bool last = c == chunks - 1;
+          int f;
+          if (lane == 0 && (!last || (more && mine(later, f)))) {
             store_wait_read<0>();
-            fetch(last ? t + pairs : t, last ? 0 : c + 1);
+            if (!last) fetch(col0 + 64 * (c + 1), row0);
+            else fetch(later.col + f, later.row + lane_row);
           }
+          uint32_t d[2][16];
+          tmem_ld16(acc + first + 64 * c, d[0]);
           if (!mbar_wait_for(&bar_in[2 * ew + (chunk & 1)], (chunk >> 1) & 1, p.waits.limit)) bad = true;
           bad = __any_sync(0xffffffffu, bad);
           if (bad) break;
           const uint32_t gate = buffers + 2 * (chunk & 1) * kStageBuffer, up = gate + kStageBuffer;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t d[32];
-            tmem_ld32(acc + half * kHalf + 64 * c + 32 * h, d);
-            tmem_ld_wait();
+          for (int q = 0; q < 4; ++q) {
+            uint4 gw[2], uw[2];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const uint32_t at = box_chunk(lane, 4 * h + v);
-              const uint4 gw = lds128(gate + at), uw = lds128(up + at);
-              const uint32_t gs[4] = {gw.x, gw.y, gw.z, gw.w}, us[4] = {uw.x, uw.y, uw.z, uw.w};
+            for (int v = 0; v < 2; ++v) gw[v] = lds128(gate + box_chunk(lane, 2 * q + v)), uw[v] = lds128(up + box_chunk(lane, 2 * q + v));
+            tmem_ld_wait();
+            if (q < 3) tmem_ld16(acc + first + 64 * c + 16 * (q + 1), d[(q + 1) & 1]);
+            else if (last) drained();
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              const uint32_t gs[4] = {gw[v].x, gw[v].y, gw[v].z, gw[v].w}, us[4] = {uw[v].x, uw[v].y, uw[v].z, uw[v].w};
               uint32_t dg[4], du[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float2 g = unpack2<T>(gs[e]), u = unpack2<T>(us[e]);
-                const float d0 = __uint_as_float(d[8 * v + 2 * e]), d1 = __uint_as_float(d[8 * v + 2 * e + 1]);
-                const Act a0 = activation<true>(g.x, p.activation), a1 = activation<true>(g.y, p.activation);
-                dg[e] = pack2<T>(d0 * u.x * a0.slope, d1 * u.y * a1.slope);
-                du[e] = pack2<T>(d0 * a0.value, d1 * a1.value);
+                const float2 grad = make_float2(__uint_as_float(d[q & 1][8 * v + 2 * e]), __uint_as_float(d[q & 1][8 * v + 2 * e + 1]));
+                float2 value, slope;
+                activation2<kAct>(unpack2<T>(gs[e]), value, slope);
+                const float2 a = mul2(mul2(grad, unpack2<T>(us[e])), slope), b = mul2(grad, value);
+                dg[e] = pack2<T>(a.x, a.y), du[e] = pack2<T>(b.x, b.y);
               }
-              sts128(gate + at, make_uint4(dg[0], dg[1], dg[2], dg[3]));
-              sts128(up + at, make_uint4(du[0], du[1], du[2], du[3]));
+              sts128(gate + box_chunk(lane, 2 * q + v), make_uint4(dg[0], dg[1], dg[2], dg[3]));
+              sts128(up + box_chunk(lane, 2 * q + v), make_uint4(du[0], du[1], du[2], du[3]));
             }
-          }
-          if (last) {
-            tc_fence_before_sync();
-            if (lane == 0) arrive_cluster(map_to_rank(smem_u32(&bar_drained[buf]), 0));
           }
           fence_smem_to_async_proxy();
           __syncwarp();
           const int col = col0 + 64 * c;
-          if (lane == 0 && row0 < p.m && col < p.n) {
-            store_box(&p.out, gate, col, row0);
+          if (lane == 0 && row0 < p.one.m && col < p.one.n) {
+            store_box(&p.one.out, gate, col, row0);
             store_box(&p.out2, up, col, row0);
             store_commit();
           }
-          if (p.column_sums && row0 < p.m) {  // of the values as stored: a lane adds two columns of the 32 rows (rows beyond the last are zeros)
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-              float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-              for (int r = 0; r < 32; ++r) {
-                const float2 v = unpack2<T>(lds32((side ? up : gate) + box_chunk(r, lane >> 2) + 4 * (lane & 3)));
-                sum.x += v.x, sum.y += v.y;
-              }
-              const int cc = col + 2 * lane;
-              if (cc < p.n) *reinterpret_cast<float2*>(p.column_sums + (size_t)(row0 >> 5) * (2 * (size_t)p.n) + side * (size_t)p.n + cc) = sum;
+          if (p.column_sums && row0 < p.one.m) {  // of the values as stored (rows beyond the last are zeros)
+            const float2 dg = column_sums32<T>(gate, lane), du = column_sums32<T>(up, lane);
+            if (col + 2 * lane < p.one.n) {
+              float* to = p.column_sums + (size_t)(row0 >> 5) * (2 * (size_t)p.one.n) + col + 2 * lane;
+              *reinterpret_cast<float2*>(to) = dg;
+              *reinterpret_cast<float2*>(to + p.one.n) = du;
             }
             __syncwarp();
           }
         }
         if (bad) break;
-      } else if constexpr (kEpi == kStore) {
-        const T* bias = static_cast<const T*>(p.bias);
-#pragma unroll 1
-        for (int c = 0; c < kChunks; ++c, ++chunk) {
-          uint32_t words[32];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t d[32];
-            tmem_ld32(acc + half * kHalf + 64 * c + 32 * h, d);
-            tmem_ld_wait();
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              float b[8] = {};
-              if (bias) bias8(bias, col0 + 64 * c + 32 * h + 8 * v, p.n, b);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                words[16 * h + 4 * v + e] = pack2<T>(__uint_as_float(d[8 * v + 2 * e]) + b[2 * e], __uint_as_float(d[8 * v + 2 * e + 1]) + b[2 * e + 1]);
-            }
-          }
-          if (c == kChunks - 1) {
-            tc_fence_before_sync();
-            if (lane == 0) arrive_cluster(map_to_rank(smem_u32(&bar_drained[buf]), 0));
-          }
-          const uint32_t dst = buffers + (chunk & 1) * kStageBuffer;
-          if (lane == 0) store_wait_read<1>();
-          __syncwarp();
-#pragma unroll
-          for (int v = 0; v < 8; ++v) sts128(dst + box_chunk(lane, v), make_uint4(words[4 * v], words[4 * v + 1], words[4 * v + 2], words[4 * v + 3]));
-          fence_smem_to_async_proxy();
-          __syncwarp();
-          if (lane == 0 && row0 < p.m && col0 + 64 * c < p.n) {
-            store_box(&p.out, dst, col0 + 64 * c, row0);
-            store_commit();
-          }
-        }
       } else {
+        const Problem& prob = kEpi == kWeight && w.second ? p.two : p.one;
+        if (kEpi == kWeight && (w.plane >= 0 || p.wide_out)) {  // 32 fp32 columns at a time: a part of a tile, or an fp32 result
 #pragma unroll 1
-        for (int c = 0; c < kHalf / 32; ++c, ++chunk) {
-          uint32_t d[32];
-          tmem_ld32(acc + half * kHalf + 32 * c, d);
-          tmem_ld_wait();
-          if (c == kHalf / 32 - 1) {
-            tc_fence_before_sync();
-            if (lane == 0) arrive_cluster(map_to_rank(smem_u32(&bar_drained[buf]), 0));
+          for (int c = 0; c < 2 * chunks; ++c) {
+            uint32_t d[32];
+            tmem_ld32(acc + first + 32 * c, d);
+            tmem_ld_wait();
+            if (c == 2 * chunks - 1) drained();
+            const uint32_t dst = next_buffer();
+            put(dst, d);
+            if (lane == 0 && row0 < prob.m && col0 + 32 * c < prob.n) {
+              if (w.plane >= 0) store_box(&p.pre, dst, first + 32 * c, w.plane * kTile + lane_row);
+              else store_box(&prob.out, dst, col0 + 32 * c, row0);
+            }
+            if (lane == 0) store_commit();  // (a group for every buffer, stored or not: next_buffer counts them)
           }
-          const uint32_t dst = buffers + (chunk & 1) * kStageBuffer;
-          if (lane == 0) store_wait_read<1>();
-          __syncwarp();
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < chunks; ++c) {
+            uint32_t words[32];
 #pragma unroll
-          for (int v = 0; v < 8; ++v) sts128(dst + box_chunk(lane, v), make_uint4(d[4 * v], d[4 * v + 1], d[4 * v + 2], d[4 * v + 3]));
-          fence_smem_to_async_proxy();
-          __syncwarp();
-          if (lane == 0 && row0 < p.m && col0 + 32 * c < p.n) {
-            store_box3(&p.out, dst, col0 + 32 * c, row0, tile.split);
-            store_commit();
+            for (int h = 0; h < 2; ++h) {
+              uint32_t d[32];
+              uint4 b[4];
+              tmem_ld32(acc + first + 64 * c + 32 * h, d);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) b[v] = kEpi == kStore ? bias8(bias, col0 + 64 * c + 32 * h + 8 * v, bias_n) : make_uint4(0u, 0u, 0u, 0u);
+              tmem_ld_wait();
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                const uint32_t bw[4] = {b[v].x, b[v].y, b[v].z, b[v].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 x = add2(make_float2(__uint_as_float(d[8 * v + 2 * e]), __uint_as_float(d[8 * v + 2 * e + 1])), unpack2<T>(bw[e]));
+                  words[16 * h + 4 * v + e] = pack2<T>(x.x, x.y);
+                }
+              }
+            }
+            if (c == chunks - 1) drained();
+            const uint32_t dst = next_buffer();
+            put(dst, words);
+            if (lane == 0 && row0 < prob.m && col0 + 64 * c < prob.n) store_box(&prob.out, dst, col0 + 64 * c, row0);
+            if (lane == 0) store_commit();
           }
         }
       }
@@ -544,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   cluster_sync();  // no arrival, copy or product of either CTA is outstanding
   if (warp == 2) {
     tc_fence_after_sync();
-    tmem_dealloc2(tmem, Sh::kTmemCols);
+    tmem_dealloc2(tmem, kTmemCols);
   }
 }
 
