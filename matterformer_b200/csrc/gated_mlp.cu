@@ -254,6 +254,7 @@ int run_forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t
   const int rc = check(a);
   if (rc != MF_OK || a->rows == 0) return rc;
   MF_CHECK_ARG(a->y, "%s: null tensor", kName);
+  if (a->rows <= kSmallRows && waits.withheld < 0) return gated_mlp_small_forward(a, stream);
   return a->dtype == MF_DTYPE_BF16 ? forward<__nv_bfloat16>(a, waits, stream) : forward<__half>(a, waits, stream);
 }
 

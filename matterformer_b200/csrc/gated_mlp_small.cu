@@ -1,0 +1,201 @@
+// Gated feed-forward block for few tokens (one molecule, single tokens): both products stream the weights once.
+//
+// With at most 32 tokens every weight meets few operands: reading the weights bounds the block, 2 bytes for 2 * 32 operations at most.  The
+// weights are the 16-row operand of mma.sync, the tokens its 8 columns, so that one token costs what eight do and nothing is
+// padded to a 256-row tile.  A CTA owns 16 hidden channels (of gate and of up) or 16 output channels; its eight warps, and those
+// of up to eight CTAs of a cluster where there are few channels, share the contracted dimension, and their sums meet in shared memory,
+// added in the order of warps and CTAs.  A lane reads 16 bytes of a weight row and of a token at a time: which k an operand's register
+// stands for is free as long as both sides agree, so no layout of the instruction reaches memory.
+#include "common.cuh"
+#include "gated_mlp.cuh"
+
+namespace mf {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kStep = 32;  // k of one step: 16 bytes for each of four lanes
+
+struct SmallParams {
+  const void* x;     // (rows, k)
+  const void* w;     // (n, k); kGate: (2 n, k)
+  const void* bias;  // (n) or (2 n), or null
+  void* out;         // (rows, n)
+  void* pre;         // kGate: (rows, 2 n) or null
+  int rows, n, k;
+  int activation;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 load16(const void* base, size_t bytes, bool valid) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (valid) v = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(base) + bytes));
+  return v;
+}
+// weights are read once: past L1
+__device__ __forceinline__ uint4 stream16(const void* base, size_t bytes, bool valid) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (valid)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(static_cast<const char*>(base) + bytes));
+  return v;
+}
+
+template <typename T, int kTiles, bool kGate>  // kTiles: of eight tokens
+__global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p) {
+  constexpr int kSides = kGate ? 2 : 1, kRows = 16 * kSides, kTokens = 8 * kTiles, kBatch = kTiles == 4 ? 2 : 4;
+  __shared__ float part[kWarps][kRows][kTokens + 1];
+  __shared__ float sums[kRows][kTokens + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t rank, ranks;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  const int n0 = (int)(blockIdx.x / ranks) * 16;
+  const int steps = (p.k + kStep - 1) / kStep, slices = kWarps * (int)ranks, slice = (int)rank * kWarps + warp;
+  const int s0 = (int)((long long)steps * slice / slices), s1 = (int)((long long)steps * (slice + 1) / slices);
+
+  size_t row[kSides][2];  // byte offsets of this lane's two weight rows
+  bool ok[2] = {n0 + g < p.n, n0 + g + 8 < p.n};
+#pragma unroll
+  for (int side = 0; side < kSides; ++side)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) row[side][r] = ((size_t)side * p.n + n0 + g + 8 * r) * p.k * 2;
+  // no value is read before the kernels before this one have ended; the weights may already move to L2
+  launch_dependents();
+  for (int s = s0 + t; s < s1; s += 4)  // (64 bytes of a row a step: one lane in four asks for each)
+#pragma unroll
+    for (int side = 0; side < kSides; ++side)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (ok[r]) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.w) + row[side][r] + (size_t)s * (2 * kStep)));
+  wait_for_previous();
+
+  float acc[kSides][kTiles][4] = {};
+  for (int s = s0; s < s1; s += kBatch) {
+    uint4 w[kBatch][kSides][2], x[kBatch][kTiles];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int k = (s + b) * kStep + 8 * t;
+      const bool in = s + b < s1 && k < p.k;
+#pragma unroll
+      for (int side = 0; side < kSides; ++side)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) w[b][side][r] = stream16(p.w, row[side][r] + (size_t)k * 2, in && ok[r]);
+#pragma unroll
+      for (int n = 0; n < kTiles; ++n) x[b][n] = load16(p.x, ((size_t)(8 * n + g) * p.k + k) * 2, in && 8 * n + g < p.rows);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+      for (int side = 0; side < kSides; ++side) {
+        const uint4 lo = w[b][side][0], hi = w[b][side][1];
+        const uint32_t a0[4] = {lo.x, hi.x, lo.y, hi.y}, a1[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          mma<T>(acc[side][n], a0, x[b][n].x, x[b][n].y);
+          mma<T>(acc[side][n], a1, x[b][n].z, x[b][n].w);
+        }
+      }
+  }
+#pragma unroll
+  for (int side = 0; side < kSides; ++side)
+#pragma unroll
+    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[warp][16 * side + g + 8 * (i >> 1)][8 * n + 2 * t + (i & 1)] = acc[side][n][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * kTokens; i += kWarps * 32) {
+    const int r = i / kTokens, c = i % kTokens;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += part[w][r][c];
+    sums[r][c] = s;
+  }
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&sums[0][0]);
+  auto total = [&](int r, int c) {
+    if (ranks == 1) return sums[r][c];
+    float s = 0.f;
+    for (uint32_t q = 0; q < ranks; ++q) {
+      uint32_t at;
+      float v;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(mine + 4u * (uint32_t)(r * (kTokens + 1) + c)), "r"(q));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+      s += v;
+    }
+    return s;
+  };
+  const T* bias = static_cast<const T*>(p.bias);
+  const bool biased = bias != nullptr;
+  // the CTAs of a cluster store every ranks-th token
+  for (int i = threadIdx.x; i < 16 * kTokens; i += kWarps * 32) {
+    const int r = i & 15, c = i >> 4, n = n0 + r;
+    if (c >= p.rows || n >= p.n || c % ranks != rank) continue;
+    float a = total(r, c);
+    if (biased) a += to_f32(bias[n]);
+    if constexpr (kGate) {
+      float u = total(16 + r, c);
+      if (biased) u += to_f32(bias[p.n + n]);
+      if (p.pre) {
+        T* pre = static_cast<T*>(p.pre) + (size_t)c * 2 * p.n + n;
+        pre[0] = from_f32<T>(a), pre[p.n] = from_f32<T>(u);
+      }
+      const float2 f = p.activation == MF_ACT_SILU ? activation2<MF_ACT_SILU>(make_float2(a, a)) : activation2<MF_ACT_GELU_TANH>(make_float2(a, a));
+      a = f.x * u;
+    }
+    static_cast<T*>(p.out)[(size_t)c * p.n + n] = from_f32<T>(a);
+  }
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // the sums stay until all have read
+}
+
+template <typename T, int kTiles, bool kGate>
+int launch(const SmallParams& p, cudaStream_t stream, const char* what) {
+  const int tiles = (p.n + 15) / 16, steps = (p.k + kStep - 1) / kStep;
+  // enough CTAs for three on every SM, while a warp keeps two steps at least
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks < 3 * 148 && steps / (2 * ranks * kWarps) >= 2) ranks *= 2;
+  cudaLaunchAttribute attributes[2] = {};
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = ranks, attributes[1].val.clusterDim.y = 1, attributes[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)(tiles * ranks)), config.blockDim = dim3(kWarps * 32), config.stream = stream;
+  config.attrs = attributes, config.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&config, small_kernel<T, kTiles, kGate>, p);
+  return e == cudaSuccess ? MF_OK : cuda_error(e, what);
+}
+
+template <typename T, bool kGate>
+int launch_tokens(const SmallParams& p, cudaStream_t stream, const char* what) {
+  return p.rows <= 8 ? launch<T, 1, kGate>(p, stream, what) : p.rows <= 16 ? launch<T, 2, kGate>(p, stream, what) : launch<T, 4, kGate>(p, stream, what);
+}
+
+template <typename T>
+int forward(const MfGatedMlpArgs* a, cudaStream_t stream) {
+  const int rows = (int)a->rows;
+  const int rc = launch_tokens<T, true>({a->x, a->w_in, a->b_in, a->act, a->pre, rows, a->hidden, a->dim, a->activation}, stream, "gated_mlp gate product");
+  if (rc != MF_OK) return rc;
+  return launch_tokens<T, false>({a->act, a->w_out, a->b_out, a->y, nullptr, rows, a->dim_out, a->hidden, 0}, stream, "gated_mlp output product");
+}
+
+}  // namespace
+
+int gated_mlp_small_forward(const MfGatedMlpArgs* a, cudaStream_t stream) {
+  return a->dtype == MF_DTYPE_BF16 ? forward<__nv_bfloat16>(a, stream) : forward<__half>(a, stream);
+}
+
+}  // namespace mf

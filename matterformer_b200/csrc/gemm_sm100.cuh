@@ -20,6 +20,7 @@
 #include <cuda_runtime.h>
 
 #include "common.cuh"
+#include "gated_mlp.cuh"
 #include "sm100_primitives.cuh"
 #include "tensor_map.cuh"
 
@@ -182,45 +183,6 @@ template <typename T, bool kAMn, bool kBMn>
 __host__ __device__ constexpr uint32_t instruction() {
   constexpr uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)kAMn << 15) | ((uint32_t)kBMn << 16) | ((256u >> 4) << 24);
-}
-
-// ---- activations ---------------------------------------------------------------------------------------------------
-// act(z) = z s(w(z)) with the logistic function s: w = z is SiLU; w = 2 sqrt(2/pi) (z + 0.044715 z^3) is GELU in its tanh form, since
-// (1 + tanh(a)) / 2 = s(2 a), and nothing cancels for large negative z.  The derivative is s + z s (1 - s) w'.
-// Beyond |z| = 64 GELU is 0 or z in fp32: the clamp keeps the cube and w' finite.
-template <int kAct>
-__device__ __forceinline__ float2 logistic2(float2 z, float2& slope) {  // slope: w'
-  constexpr float kLog2e = 1.4426950408889634f;
-  float2 w = mul2(z, make_float2(-kLog2e, -kLog2e));
-  if constexpr (kAct == MF_ACT_GELU_TANH) {
-    constexpr float kBeta = 1.5957691216057308f, kKappa = 0.044715f;
-    const float2 c = make_float2(fminf(fmaxf(z.x, -64.f), 64.f), fminf(fmaxf(z.y, -64.f), 64.f)), c2 = mul2(c, c);
-    const float a = -kLog2e * kBeta;
-    w = mul2(c, fma2(c2, make_float2(a * kKappa, a * kKappa), make_float2(a, a)));
-    slope = fma2(c2, make_float2(3.f * kBeta * kKappa, 3.f * kBeta * kKappa), make_float2(kBeta, kBeta));
-  }
-  float2 e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(w.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(w.y));
-  e = add2(e, make_float2(1.f, 1.f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(e.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(e.y));
-  return e;
-}
-template <int kAct>
-__device__ __forceinline__ float2 activation2(float2 z) {
-  float2 unused;
-  return mul2(z, logistic2<kAct>(z, unused));
-}
-// act(z) and act'(z)
-template <int kAct>
-__device__ __forceinline__ void activation2(float2 z, float2& value, float2& slope) {
-  float2 dw;
-  const float2 s = logistic2<kAct>(z, dw);
-  value = mul2(z, s);
-  float2 t = mul2(value, fma2(s, make_float2(-1.f, -1.f), make_float2(1.f, 1.f)));
-  if constexpr (kAct == MF_ACT_GELU_TANH) t = mul2(t, dw);
-  slope = add2(s, t);
 }
 
 // Eight 16-bit values of a bias from column c on (a multiple of 8); zeros from column n on (n = 0: there is no bias).
