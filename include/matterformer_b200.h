@@ -626,6 +626,50 @@ int mf_simplicial_packed_fwd(const MfSimplicialPackedArgs* args, void* stream);
 int mf_simplicial_packed_bwd(const MfSimplicialPackedArgs* args, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* Rotary positions                                                           */
+/* ------------------------------------------------------------------------- */
+
+#define MF_ROTARY_HALF 0        /* pair p: channels p and p + P */
+#define MF_ROTARY_INTERLEAVED 1 /* pair p: channels 2 p and 2 p + 1 */
+#define MF_POSITION_I32 0
+#define MF_POSITION_I64 1
+#define MF_POSITION_F32 2
+#define MF_POSITION_F64 3
+
+/*
+ * Rotates the channel pairs of the heads of up to three tensors by angles that depend on their tokens' positions, the operator that
+ * `RotaryMultiheadAttention.forward` applies to its queries and keys (regular_attention.py:208-271) in the forms that language models
+ * have it: both pair layouts, a part of the head, positions of one or several axes, any table of frequencies.
+ * Pair p of P = axes * pairs turns by positions[b, n, p / pairs] * frequencies[p] radians and is scaled by `amplitude`; channels from
+ * 2 P on are copied, and so are all channels of a tensor with rotates = 0 (the values of a packed projection).  inverse = 1: by the
+ * opposite angles, which is the backward pass.
+ * `frequencies` is a HOST array of P doubles, copied by the call.  positions: (tokens, axes) for each batch entry, position_batch
+ * elements apart (0: the same for all).  Tensors: fp32, bf16 or fp16, strides in elements, channels adjacent; out may be in if their strides
+ * agree.  Any sizes and alignment to an element; 16-byte accesses are used where all strides and sizes are multiples.  P <= 128.
+ */
+typedef struct MfRotaryTensor {
+  const void* in;
+  void* out;
+  int32_t heads, rotates;
+  int64_t in_batch, in_token, in_head;
+  int64_t out_batch, out_token, out_head;
+} MfRotaryTensor;
+
+typedef struct MfRotaryArgs {
+  int32_t batch, tokens, head_dim;
+  int32_t axes, pairs;
+  int32_t dtype, layout, position_type, inverse, tensors;
+  float amplitude;
+  int32_t reserved0;
+  const void* positions;
+  int64_t position_batch;
+  const double* frequencies;
+  MfRotaryTensor tensor[3];
+} MfRotaryArgs;
+
+int mf_rotary(const MfRotaryArgs* args, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Gated feed-forward block                                                    */
 /* ------------------------------------------------------------------------- */
 

@@ -27,6 +27,8 @@ MF_PRECISION = {"bf16_tc": 0, "tf32": 1, "ieee_fp32": 2}
 MF_BACKEND = {"auto": 0, "generic": 1, "tcgen05": 2, "tcgen05_tiles": 3}
 MF_SPARSE_BACKEND = {"auto": 0, "mma": 1, "tcgen05": 2}
 MF_ACT_SILU, MF_ACT_GELU_TANH = 0, 1
+MF_ROTARY = {"half": 0, "interleaved": 1}
+MF_POSITION = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
 # Every symbol include/matterformer_b200.h declares.
 EXPORTED_SYMBOLS = (
@@ -96,6 +98,7 @@ EXPORTED_SYMBOLS = (
     "mf_pair_head_bwd_workspace_bytes",
     "mf_pair_head_fwd",
     "mf_pair_head_bwd",
+    "mf_rotary",
     "mf_gated_mlp_bwd_workspace_bytes",
     "mf_gated_mlp_fwd",
     "mf_gated_mlp_bwd",
@@ -300,6 +303,18 @@ class MfPairHeadArgs(Structure):
     ]
 
 
+class MfRotaryTensor(Structure):
+    _fields_ = [("input", c_void_p), ("out", c_void_p), ("heads", c_int32), ("rotates", c_int32)] + \
+               [(n, c_int64) for n in ("in_batch", "in_token", "in_head", "out_batch", "out_token", "out_head")]  # fmt: skip
+
+
+class MfRotaryArgs(Structure):
+    _fields_ = [(n, c_int32) for n in ("batch", "tokens", "head_dim", "axes", "pairs", "dtype", "layout", "position_type", "inverse",
+                                       "tensors")] + \
+               [("amplitude", c_float), ("reserved0", c_int32), ("positions", c_void_p), ("position_batch", c_int64),
+                ("frequencies", POINTER(c_double)), ("tensor", MfRotaryTensor * 3)]  # fmt: skip
+
+
 class MfGatedMlpArgs(Structure):
     _fields_ = [("rows", c_int64)] + \
                [(n, c_int32) for n in ("dim", "hidden", "dim_out", "dtype", "grad_dtype", "activation")] + \
@@ -445,6 +460,8 @@ def lib() -> ctypes.CDLL:
     for fn in (L.mf_pair_head_fwd, L.mf_pair_head_bwd):
         fn.argtypes = [POINTER(MfPairHeadArgs), c_void_p]
         fn.restype = c_int32
+    L.mf_rotary.argtypes = [POINTER(MfRotaryArgs), c_void_p]
+    L.mf_rotary.restype = c_int32
     L.mf_gated_mlp_bwd_workspace_bytes.argtypes = [POINTER(MfGatedMlpArgs)]
     L.mf_gated_mlp_bwd_workspace_bytes.restype = c_size_t
     for fn in (L.mf_gated_mlp_fwd, L.mf_gated_mlp_bwd):
