@@ -644,8 +644,8 @@ int mf_simplicial_packed_bwd(const MfSimplicialPackedArgs* args, void* stream);
  * 2 P on are copied, and so are all channels of a tensor with rotates = 0 (the values of a packed projection).  inverse = 1: by the
  * opposite angles, which is the backward pass.
  * `frequencies` is a HOST array of P doubles, copied by the call.  positions: (tokens, axes) for each batch entry, position_batch
- * elements apart (0: the same for all).  Tensors: fp32, bf16 or fp16, strides in elements, channels adjacent; out may be in if their strides
- * agree.  Any sizes and alignment to an element; 16-byte accesses are used where all strides and sizes are multiples.  P <= 128.
+ * elements apart (0: the same for all).  Tensors: fp32, bf16 or fp16, strides in elements, channels adjacent, out apart from every
+ * in.  Any sizes and alignment to an element; 16-byte accesses are used where head_dim, strides and addresses are multiples.  P <= 128.
  */
 typedef struct MfRotaryTensor {
   const void* in;

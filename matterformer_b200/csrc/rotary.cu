@@ -3,9 +3,10 @@
 //   (a, b) -> amplitude * (a cos - b sin, a sin + b cos),   pair p of P = axes * pairs uses axis p / pairs and its own frequency;
 //   half layout: a = x[p], b = x[p + P];   interleaved: a = x[2 p], b = x[2 p + 1];   channels from 2 P on are copied.
 //
-// The backward pass is the same rotation by the opposite angle.  Every value is read and written once: memory bounds it.  A block takes some
-// tokens of one tensor, computes their cosines and sines once into shared memory, for all heads, and walks the rows (token, head) in
-// the order in which they lie in memory, 16 bytes at a time where sizes, strides and addresses allow it, else 8, 4 or a single element.
+// The backward pass is the same rotation by the opposite angle.  Every value is read and written once: memory bounds it.  A warp takes a few
+// tokens: its lanes form the tokens' cosines and sines, once for all heads of all tensors, into a table of the warp in shared memory, and
+// then move the tokens' rows, 16 bytes at a time where sizes, strides and addresses allow it, else 8, 4 or a single element.  Warps wait
+// for nobody, so that one's arithmetic hides behind the others' loads.
 //
 // Angles are formed in turns in 64 bits, position * (frequency / 2 pi), and lose their whole turns there: a position of a million
 // and a frequency of 1 would leave 4 digits of an angle in 32 bits.  What remains is at most half a turn: its sine and cosine are taken in
@@ -16,7 +17,8 @@ namespace mf {
 namespace {
 
 constexpr int kMaxPairs = 128;
-constexpr int kThreads = 256;
+constexpr int kWarps = 4;
+constexpr int kBatch = 4;  // items of a lane in flight
 
 struct RotaryTensor {
   const void* in;
@@ -29,10 +31,11 @@ struct RotaryParams {
   RotaryTensor tensor[3];
   const void* positions;
   long long position_batch;
-  long long places;  // batch * tokens
-  int tokens, head_dim, axes, pairs, position_type;
-  int block_tokens;
+  int batch, tokens, head_dim, axes, pairs, position_type;
+  int warp_tokens, tensors;
+  int parts;  // warps that share a token's heads (gridDim.y)
   float amplitude, sign;
+  int half, piece;
 };
 
 __device__ __forceinline__ double position_at(const RotaryParams& p, long long i) {
@@ -44,124 +47,270 @@ __device__ __forceinline__ double position_at(const RotaryParams& p, long long i
   }
 }
 
-template <int kBytes>
-struct Raw;
-template <>
-struct Raw<16> { using type = uint4; };
-template <>
-struct Raw<8> { using type = uint2; };
-template <>
-struct Raw<4> { using type = uint32_t; };
-template <>
-struct Raw<2> { using type = uint16_t; };
-
+// kVec elements as 32-bit registers
 template <typename T, int kVec>
-union Pack {
-  typename Raw<sizeof(T) * kVec>::type raw;
-  T v[kVec];
-  __device__ Pack() {}
+struct Vec {
+  static constexpr int kBytes = sizeof(T) * kVec;
+  uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x, w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+  }
+  __device__ __forceinline__ void get(float (&v)[kVec]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = __uint_as_float(w[e]);
+    } else if constexpr (kVec == 1) {
+      v[0] = unpack2<T>(w[0]).x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; e += 2) {
+        const float2 f = unpack2<T>(w[e / 2]);
+        v[e] = f.x, v[e + 1] = f.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[kVec]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) w[e] = __float_as_uint(v[e]);
+    } else if constexpr (kVec == 1) {
+      w[0] = pack2<T>(v[0], 0.f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; e += 2) w[e / 2] = pack2<T>(v[e], v[e + 1]);
+    }
+  }
 };
-template <typename T, int kVec>
-__device__ __forceinline__ Pack<T, kVec> load(const T* p) {
-  Pack<T, kVec> r;
-  r.raw = __ldg(reinterpret_cast<const typename Raw<sizeof(T) * kVec>::type*>(p));
-  return r;
-}
-template <typename T, int kVec>
-__device__ __forceinline__ void store(T* p, const Pack<T, kVec>& v) {
-  *reinterpret_cast<typename Raw<sizeof(T) * kVec>::type*>(p) = v.raw;
+
+// cos and sin of kPairs pairs from one on, in 16-byte loads where there are four: P is a multiple of kPairs then
+template <int kPairs>
+__device__ __forceinline__ void angles(const float* cosine, const float* sine, float (&c)[kPairs], float (&s)[kPairs]) {
+  if constexpr (kPairs >= 4) {
+#pragma unroll
+    for (int e = 0; e < kPairs; e += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(cosine + e), w = *reinterpret_cast<const float4*>(sine + e);
+      c[e] = v.x, c[e + 1] = v.y, c[e + 2] = v.z, c[e + 3] = v.w;
+      s[e] = w.x, s[e + 1] = w.y, s[e + 2] = w.z, s[e + 3] = w.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) c[e] = cosine[e], s[e] = sine[e];
+  }
 }
 
-// A unit is what a thread does of a row: kVec pairs of the half layout (two vectors), kVec / 2 pairs of the interleaved one (one vector;
-// kVec 1: one pair, two elements), or a vector of the copied channels.
-template <typename T, int kVec, bool kHalf>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 table[];  // (block_tokens, P): cosine, sine
-  const RotaryTensor& x = p.tensor[blockIdx.y];
-  const int P = p.axes * p.pairs;
-  constexpr int kPairs = kHalf || kVec == 1 ? kVec : kVec / 2;  // of a rotating unit
-  const long long first = (long long)blockIdx.x * p.block_tokens;
-  const int count = (int)(p.places - first < p.block_tokens ? p.places - first : p.block_tokens);
-  wait_for_previous();
+// The partners of the channels from `at` on, `from` their address: P channels further on or back, in pieces of 1, 2 or 4 elements which lie
+// within one half each.  Channels from 2 P on have none.
+template <typename T, int kVec, int kPiece>
+__device__ __forceinline__ void partners_of(Vec<T, kVec>& c, const T* from, int at, int P) {
+  constexpr int kWords = sizeof(T) * kPiece / 4 ? sizeof(T) * kPiece / 4 : 1;
+  uint32_t half = 0;
+#pragma unroll
+  for (int e = 0; e < kVec; e += kPiece) {
+    Vec<T, kPiece> v;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) v.w[w] = 0;
+    if (at + e < 2 * P) v.load(from + e + (at + e < P ? P : -P));
+    if constexpr (sizeof(T) * kPiece == 2) {
+      if (e % 2 == 0) half = v.w[0];
+      else c.w[e / 2] = half | v.w[0] << 16;
+    } else {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) c.w[e / kPiece * kWords + w] = v.w[w];
+    }
+  }
+}
+template <typename T, int kVec>
+__device__ __forceinline__ void partners(Vec<T, kVec>& c, const T* from, int at, int P, int piece) {
+  if (kVec > 4 && piece == 4) partners_of<T, kVec, kVec < 4 ? kVec : 4>(c, from, at, P);
+  else if (kVec > 2 && piece == 2) partners_of<T, kVec, 2>(c, from, at, P);
+  else partners_of<T, kVec, 1>(c, from, at, P);
+}
+
+// What an item of a lane is:
+//   kHalves       kVec pairs of the half layout, two vectors; or a vector of the copied channels (P a multiple of kVec)
+//   kHalvesMixed  a vector, whose partners are fetched in pieces of `piece` elements, the power of two in P (they come from L1)
+//   kNeighbours   a vector of kVec / 2 pairs of the interleaved layout
+//   kSingle       a pair of either layout, element by element
+enum Mode { kHalves, kHalvesMixed, kNeighbours, kSingle };
+
+template <typename T, int kVec, Mode kMode>
+__global__ void __launch_bounds__(32 * kWarps) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  extern __shared__ __align__(16) float tables[];  // (warp, cosine | sine, warp_tokens, P)
+  constexpr bool kTwo = kMode == kHalves || kMode == kSingle;  // a rotating item is two vectors
+  constexpr int kPairs = kMode == kNeighbours ? kVec / 2 : kVec;
+  constexpr int kInFlight = kMode == kHalvesMixed ? 2 : kBatch;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int P = p.axes * p.pairs, rotating = kMode == kHalvesMixed ? 2 * P / kVec + 1 : (P + kPairs - 1) / kPairs;
+  const int units = kTwo ? rotating + (p.head_dim - 2 * P) / kVec : p.head_dim / kVec;
+  // tokens of one batch entry
+  const int tiles = (p.tokens + p.warp_tokens - 1) / p.warp_tokens;
+  const long long tile = (long long)blockIdx.x * kWarps + warp;
+  const int b = tile <= 0x7fffffffll ? (int)tile / tiles : (int)(tile / tiles), n0 = (int)(tile - (long long)b * tiles) * p.warp_tokens;
+  const int count = b < p.batch ? min(p.tokens - n0, p.warp_tokens) : 0;
+  float* cosine = tables + warp * 2 * p.warp_tokens * P;
+  float* sine = cosine + p.warp_tokens * P;
   launch_dependents();
-  if (x.rotates) {
-    for (int i = threadIdx.x; i < count * P; i += kThreads) {
-      const int token = i / P, pair = i - token * P;
-      const long long place = first + token, b = place / p.tokens, n = place - b * p.tokens;
-      double t = position_at(p, b * p.position_batch + n * p.axes + pair / p.pairs) * p.turns[pair];
-      t -= rint(t);
+  wait_for_previous();
+  const long long at0 = b * p.position_batch + (long long)n0 * p.axes;
+  for (int pair = lane; pair < P; pair += 32) {
+    const double frequency = p.turns[pair];
+    const int axis = p.axes == 1 ? 0 : pair / p.pairs;
+    for (int t = 0; t < count; ++t) {
+      double turns = position_at(p, at0 + t * p.axes + axis) * frequency;
+      turns -= rint(turns);
       float s, c;
-      sincospif(2.f * (float)t, &s, &c);
-      table[i] = make_float2(p.amplitude * c, p.sign * p.amplitude * s);
-    }
-    __syncthreads();
-  }
-  const int rotating = P / kPairs, copied = (p.head_dim - 2 * P) / kVec, units = rotating + copied;
-  const int rows = count * x.heads;
-  const bool token_first = x.in_token < x.in_head;  // the rows of one head follow each other
-  const int at_once = kThreads / units > 0 ? kThreads / units : 1;
-  for (int u = threadIdx.x % units; u < units; u += kThreads) {  // (more units than threads: each takes several)
-    const int j = units > kThreads ? 0 : threadIdx.x / units;
-    if (j >= at_once) break;
-#pragma unroll 2
-    for (int r = j; r < rows; r += at_once) {
-      const int head = token_first ? r / count : r % x.heads, token = token_first ? r - head * count : r / x.heads;
-      const long long place = first + token, b = place / p.tokens, n = place - b * p.tokens;
-      const T* in = static_cast<const T*>(x.in) + b * x.in_batch + n * x.in_token + head * x.in_head;
-      T* out = static_cast<T*>(x.out) + b * x.out_batch + n * x.out_token + head * x.out_head;
-      if (u >= rotating) {
-        const int at = 2 * P + (u - rotating) * kVec;
-        store<T, kVec>(out + at, load<T, kVec>(in + at));
-        continue;
+      if constexpr (sizeof(T) == 4) {
+        sincospif(2.f * (float)turns, &s, &c);
+      } else {  // 2^-21 of a pair's length, which is rounded to 2^-9 or 2^-12 of the value
+        const float angle = 6.283185307179586f * (float)turns;
+        s = __sinf(angle), c = __cosf(angle);
       }
-      const float2* cs = table + token * P + u * kPairs;
-      if constexpr (kHalf || kVec == 1) {
-        const int at = kHalf ? u * kVec : 2 * u, other = kHalf ? at + P : at + 1;
-        Pack<T, kVec> a = load<T, kVec>(in + at), c = load<T, kVec>(in + other);
-        if (x.rotates) {
+      cosine[t * P + pair] = p.amplitude * c, sine[t * P + pair] = p.sign * p.amplitude * s;
+    }
+  }
+  __syncwarp();
+  for (int which = 0; which < p.tensors; ++which) {
+    const RotaryTensor& x = p.tensor[which];
+    const T* in = static_cast<const T*>(x.in) + b * x.in_batch + n0 * x.in_token;
+    T* out = static_cast<T*>(x.out) + b * x.out_batch + n0 * x.out_token;
+    // (token, head, unit) of this lane's items, 32 * parts further on each time
+    const int h_units = x.heads * units, total = count * h_units, step = 32 * p.parts;
+    int i = 32 * blockIdx.y + lane;
+    int token = i / h_units, head = (i - token * h_units) / units, u = i - token * h_units - head * units;
+    const int step_t = step / h_units, step_h = (step - step_t * h_units) / units, step_u = step - step_t * h_units - step_h * units;
+    while (i < total) {
+      Vec<T, kVec> a[kInFlight], c[kInFlight];
+      T* to[kInFlight];
+      int angle[kInFlight], other[kInFlight];  // the first angle, -1: copied; distance of the second vector, 0: one, -1: no item
+      int channel[kInFlight];
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            const float va = to_f32<T>(a.v[e]), vc = to_f32<T>(c.v[e]);
-            const float2 w = cs[e];
-            a.v[e] = from_f32<T>(va * w.x - vc * w.y);
-            c.v[e] = from_f32<T>(va * w.y + vc * w.x);
-          }
+      for (int k = 0; k < kInFlight; ++k) {
+        other[k] = -1;
+        if (i < total) {
+          const bool turns = u < rotating;
+          const int at = !kTwo || (kMode == kHalves && turns) ? u * kVec : turns ? (p.half ? u : 2 * u) : 2 * P + (u - rotating) * kVec;
+          other[k] = kTwo && turns ? (kMode == kHalves || p.half ? P : 1) : 0;
+          angle[k] = turns && x.rotates ? token * P + (kMode == kHalvesMixed ? 0 : u * kPairs) : -1;
+          channel[k] = at;
+          const T* from = in + token * x.in_token + head * x.in_head + at;
+          to[k] = out + token * x.out_token + head * x.out_head + at;
+          a[k].load(from);
+          if (kTwo && other[k]) c[k].load(from + other[k]);
+          if constexpr (kMode == kHalvesMixed)
+            if (angle[k] >= 0) partners(c[k], from, at, P, p.piece);
         }
-        store<T, kVec>(out + at, a);
-        store<T, kVec>(out + other, c);
-      } else {
-        Pack<T, kVec> a = load<T, kVec>(in + u * kVec);
-        if (x.rotates) {
+        i += step, token += step_t, head += step_h, u += step_u;
+        if (u >= units) u -= units, ++head;
+        if (head >= x.heads) head -= x.heads, ++token;
+      }
 #pragma unroll
-          for (int e = 0; e < kVec; e += 2) {
-            const float va = to_f32<T>(a.v[e]), vc = to_f32<T>(a.v[e + 1]);
-            const float2 w = cs[e / 2];
-            a.v[e] = from_f32<T>(va * w.x - vc * w.y);
-            a.v[e + 1] = from_f32<T>(va * w.y + vc * w.x);
+      for (int k = 0; k < kInFlight; ++k) {
+        if (other[k] < 0) break;
+        if (angle[k] >= 0) {
+          float cs[kPairs], sn[kPairs], va[kVec];
+          a[k].get(va);
+          if constexpr (kMode == kHalvesMixed) {
+            float vc[kVec];
+            c[k].get(vc);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+              const int at = channel[k] + e;
+              if (at < 2 * P) {
+                const int pair = angle[k] + (at < P ? at : at - P);
+                va[e] = at < P ? va[e] * cosine[pair] - vc[e] * sine[pair] : vc[e] * sine[pair] + va[e] * cosine[pair];
+              }
+            }
+          } else if constexpr (kTwo) {
+            float vc[kVec];
+            c[k].get(vc);
+            angles<kPairs>(cosine + angle[k], sine + angle[k], cs, sn);
+            if constexpr (kVec >= 2) {
+#pragma unroll
+              for (int e = 0; e < kVec; e += 2) {
+                const float2 v = make_float2(va[e], va[e + 1]), w = make_float2(vc[e], vc[e + 1]);
+                const float2 co = make_float2(cs[e], cs[e + 1]), si = make_float2(sn[e], sn[e + 1]);
+                const float2 y = fma2(v, si, mul2(w, co)), z = mul2(w, si);
+                const float2 r = fma2(v, co, make_float2(-z.x, -z.y));
+                va[e] = r.x, va[e + 1] = r.y, vc[e] = y.x, vc[e + 1] = y.y;
+              }
+            } else {
+              const float v = va[0], w = vc[0];
+              va[0] = v * cs[0] - w * sn[0], vc[0] = v * sn[0] + w * cs[0];
+            }
+            c[k].set(vc);
+          } else {
+            const int pair = channel[k] / 2;
+            if (pair + kPairs <= P && P % kPairs == 0) {
+              angles<kPairs>(cosine + angle[k], sine + angle[k], cs, sn);
+            } else {  // (the table has room for a vector behind its last pair)
+#pragma unroll
+              for (int e = 0; e < kPairs; ++e) cs[e] = cosine[angle[k] + e], sn[e] = sine[angle[k] + e];
+            }
+#pragma unroll
+            for (int e = 0; e < kVec; e += 2) {
+              const float v = va[e], w = va[e + 1];
+              if (pair + e / 2 < P) va[e] = v * cs[e / 2] - w * sn[e / 2], va[e + 1] = v * sn[e / 2] + w * cs[e / 2];
+            }
           }
+          a[k].set(va);
         }
-        store<T, kVec>(out + u * kVec, a);
+        a[k].store(to[k]);
+        if (kTwo && other[k]) c[k].store(to[k] + other[k]);
       }
     }
   }
 }
 
-template <typename T, int kVec>
-int launch(const RotaryParams& p, int tensors, bool half, cudaStream_t stream) {
-  const long long blocks = (p.places + p.block_tokens - 1) / p.block_tokens;
-  const dim3 grid((unsigned)blocks, (unsigned)tensors);
-  const size_t smem = (size_t)p.block_tokens * p.axes * p.pairs * sizeof(float2);
-  const cudaError_t e = half ? launch_dependent(rotary_kernel<T, kVec, true>, grid, dim3(kThreads), smem, stream, p)
-                             : launch_dependent(rotary_kernel<T, kVec, false>, grid, dim3(kThreads), smem, stream, p);
+template <typename T, int kVec, Mode kMode>
+int launch(RotaryParams& p, cudaStream_t stream) {
+  const int P = p.axes * p.pairs;
+  const int units = kMode == kHalves || kMode == kSingle ? P / kVec + (p.head_dim - 2 * P) / kVec : p.head_dim / kVec;
+  // Up to eight tokens a warp while that leaves sixteen warps for every SM; with few tokens, a token's heads go to several warps.
+  p.warp_tokens = 8;
+  auto warps = [&] { return (long long)p.batch * ((p.tokens + p.warp_tokens - 1) / p.warp_tokens); };
+  while (p.warp_tokens > 1 && (warps() < 16 * 148 || p.warp_tokens >= 2 * p.tokens)) p.warp_tokens /= 2;
+  const long long blocks = (warps() + kWarps - 1) / kWarps;
+  int heads = 0;
+  for (int i = 0; i < p.tensors; ++i) heads = heads > p.tensor[i].heads ? heads : p.tensor[i].heads;
+  const long long most = ((long long)p.warp_tokens * heads * units + 31) / 32;
+  long long parts = 16 * 148 / (blocks * kWarps);
+  p.parts = (int)(parts < 1 ? 1 : parts > most ? most : parts > 64 ? 64 : parts);
+  MF_CHECK_ARG(blocks < (1ll << 31), "mf_rotary: batch * tokens above 2^33");
+  const dim3 grid((unsigned)blocks, (unsigned)p.parts);
+  const size_t smem = (size_t)(kWarps * 2 * p.warp_tokens * P + kVec) * sizeof(float);
+  const cudaError_t e = launch_dependent(rotary_kernel<T, kVec, kMode>, grid, dim3(32 * kWarps), smem, stream, p);
   return e == cudaSuccess ? MF_OK : cuda_error(e, "rotary_kernel");
 }
 
-template <typename T>
-int launch_widest(const RotaryParams& p, int tensors, bool half, int vec, cudaStream_t stream) {
-  if constexpr (sizeof(T) == 2)
-    if (vec == 8) return launch<T, 8>(p, tensors, half, stream);
-  if (vec >= 4) return launch<T, 4>(p, tensors, half, stream);
-  return vec == 2 ? launch<T, 2>(p, tensors, half, stream) : launch<T, 1>(p, tensors, half, stream);
+// `vec` elements at a time: what head_dim, strides and addresses are multiples of
+template <typename T, int kVec>
+int launch_mode(RotaryParams& p, int vec, cudaStream_t stream) {
+  if constexpr (kVec > 1) {
+    if (vec < kVec) return launch_mode<T, kVec / 2>(p, vec, stream);
+    if (!p.half) return launch<T, kVec, kNeighbours>(p, stream);
+    const int P = p.axes * p.pairs;
+    if (P % kVec == 0) return launch<T, kVec, kHalves>(p, stream);
+    p.piece = P % 4 == 0 ? 4 : P % 2 == 0 ? 2 : 1;
+    return launch<T, kVec, kHalvesMixed>(p, stream);
+  } else {
+    return launch<T, 1, kSingle>(p, stream);
+  }
 }
 
 }  // namespace
@@ -187,13 +336,10 @@ extern "C" int mf_rotary(const MfRotaryArgs* a, void* stream) {
   RotaryParams p;
   for (int i = 0; i < P; ++i) p.turns[i] = a->frequencies[i] / 6.283185307179586476925286766559;
   const int size = a->dtype == MF_DTYPE_F32 ? 4 : 2;
-  int vec = 16 / size, most_heads = 0;
-  const bool half = a->layout == MF_ROTARY_HALF;
+  int vec = 16 / size;
   auto fits = [&](long long elements) {
     while (vec > 1 && elements % vec) vec /= 2;
   };
-  fits(half ? P : 2 * P);
-  fits(a->head_dim - 2 * P);
   fits(a->head_dim);
   int used = 0;
   for (int i = 0; i < a->tensors; ++i) {
@@ -206,22 +352,17 @@ extern "C" int mf_rotary(const MfRotaryArgs* a, void* stream) {
                         (long long)(reinterpret_cast<uintptr_t>(t.in) / size), (long long)(reinterpret_cast<uintptr_t>(t.out) / size)})
       fits(s);
     p.tensor[used++] = {t.in, t.out, t.heads, t.rotates, t.in_batch, t.in_token, t.in_head, t.out_batch, t.out_token, t.out_head};
-    if (t.heads > most_heads) most_heads = t.heads;
   }
   if (used == 0) return MF_OK;
   MF_CHECK_ARG(a->positions != nullptr, "%s: null positions", name);
-  p.positions = a->positions, p.position_batch = a->position_batch, p.places = places;
-  p.tokens = a->tokens, p.head_dim = a->head_dim, p.axes = a->axes, p.pairs = a->pairs, p.position_type = a->position_type;
-  p.amplitude = a->amplitude, p.sign = a->inverse ? -1.f : 1.f;
-  // up to 32 tokens a block, so that each head's stretch of a tensor is long, while there are four blocks for every SM
-  p.block_tokens = 32;
-  while (p.block_tokens > 1 && (places + p.block_tokens - 1) / p.block_tokens * used < 4 * 148) p.block_tokens /= 2;
-  const long long blocks = (places + p.block_tokens - 1) / p.block_tokens;
-  MF_CHECK_ARG(blocks < (1ll << 31), "%s: batch * tokens above 2^36", name);
+  p.positions = a->positions, p.position_batch = a->position_batch;
+  p.batch = a->batch, p.tokens = a->tokens, p.head_dim = a->head_dim, p.axes = a->axes, p.pairs = a->pairs, p.position_type = a->position_type;
+  p.half = a->layout == MF_ROTARY_HALF, p.piece = 1;
+  p.tensors = used, p.amplitude = a->amplitude, p.sign = a->inverse ? -1.f : 1.f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
-    case MF_DTYPE_F32: return launch_widest<float>(p, used, half, vec, s);
-    case MF_DTYPE_BF16: return launch_widest<__nv_bfloat16>(p, used, half, vec, s);
-    default: return launch_widest<__half>(p, used, half, vec, s);
+    case MF_DTYPE_F32: return launch_mode<float, 4>(p, vec, s);
+    case MF_DTYPE_BF16: return launch_mode<__nv_bfloat16, 8>(p, vec, s);
+    default: return launch_mode<__half, 8>(p, vec, s);
   }
 }
