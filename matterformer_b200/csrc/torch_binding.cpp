@@ -8,9 +8,11 @@
 // then takes the Python path with its conversions and error messages.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <array>
+#include <cmath>
 #include <mutex>
 
 #include "../../include/matterformer_b200.h"
@@ -326,6 +328,169 @@ std::optional<std::array<Tensor, 2>> knn_topk(const Tensor& pos, const Tensor& l
   return std::array<Tensor, 2>{idx, d2};
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Gated feed-forward block
+// ---------------------------------------------------------------------------------------------------------------------
+bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+
+struct GatedMlp : torch::autograd::Function<GatedMlp> {
+  static void fill(MfGatedMlpArgs& a, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& b_in, const Tensor& b_out, int64_t activation) {
+    a.dim = x.size(-1), a.hidden = w_out.size(1), a.dim_out = w_out.size(0), a.rows = x.numel() / a.dim;
+    a.dtype = a.grad_dtype = dtype_code(x), a.activation = activation;
+    a.x = x.const_data_ptr(), a.w_in = w_in.const_data_ptr(), a.w_out = w_out.const_data_ptr();
+    a.b_in = b_in.defined() ? b_in.const_data_ptr() : nullptr, a.b_out = b_out.defined() ? b_out.const_data_ptr() : nullptr;
+  }
+
+  static Variable forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const OptTensor& b_in, const OptTensor& b_out,
+                          int64_t activation, bool keep) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor bi = b_in ? *b_in : Tensor(), bo = b_out ? *b_out : Tensor();
+    MfGatedMlpArgs a{};
+    fill(a, x, w_in, w_out, bi, bo, activation);
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = a.dim_out;
+    const Tensor y = at::empty(shape, x.options()), act = at::empty({a.rows, a.hidden}, x.options());
+    const Tensor pre = keep ? at::empty({a.rows, 2 * (int64_t)a.hidden}, x.options()) : Tensor();
+    a.y = y.data_ptr(), a.act = act.data_ptr(), a.pre = keep ? pre.data_ptr() : nullptr;
+    check(mf_gated_mlp_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
+    if (keep) {
+      ctx->saved_data["activation"] = activation;
+      ctx->save_for_backward({x, w_in, w_out, bi, bo, pre, act});
+    }
+    return y;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grad_y) {
+    const tensor_list s = ctx->get_saved_variables();
+    const Tensor& x = s[0];
+    const c10::cuda::CUDAGuard guard(x.device());
+    MfGatedMlpArgs a{};
+    tensor_list g(7);  // (one for each argument of forward)
+    {
+      const at::NoGradGuard no_grad;
+      fill(a, x, s[1], s[2], s[3], s[4], ctx->saved_data["activation"].toInt());
+      Tensor gy = grad_y[0].to(x.scalar_type()).contiguous();
+      if (!aligned(gy)) gy = gy.clone();
+      a.pre = s[5].data_ptr(), a.act = s[6].data_ptr(), a.grad_y = gy.const_data_ptr();
+      size_t edge = 0;  // edges of the node are counted over the tensors that were given
+      for (int i = 0; i < 5; ++i)
+        if (s[i].defined() && ctx->needs_input_grad(edge++)) g[i] = at::empty_like(s[i]);
+      auto ptr = [&](int i) { return g[i].defined() ? g[i].data_ptr() : nullptr; };
+      a.grad_x = ptr(0), a.grad_w_in = ptr(1), a.grad_w_out = ptr(2), a.grad_b_in = ptr(3), a.grad_b_out = ptr(4);
+      const Tensor ws = bytes(mf_gated_mlp_bwd_workspace_bytes(&a), x);
+      if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+      check(mf_gated_mlp_bwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
+    }
+    if (at::GradMode::is_enabled()) {  // create_graph: an error for who differentiates again, as torch's once_differentiable has it
+      tensor_list given;
+      for (int i = 0; i < 5; ++i)
+        if (g[i].defined()) given.push_back(g[i].set_requires_grad(true));
+      const auto node = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable",
+                                                                        (int64_t)given.size());
+      const tensor_list out = (*node)(std::move(given));
+      for (int i = 0, j = 0; i < 5; ++i)
+        if (g[i].defined()) g[i] = out[j++];
+    }
+    return g;
+  }
+};
+
+// Parameters in the type of x, everything contiguous and aligned.  (Forward-mode tangents and functorch's wrappers have their own way.)
+std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tensor& w_out, const OptTensor& b_in, const OptTensor& b_out, int64_t activation) {
+  if (!x.is_cuda() || x.dim() < 1 || (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kHalf) || !x.is_contiguous() || x.numel() == 0) return std::nullopt;
+  if (w_out.dim() != 2) return std::nullopt;
+  const int64_t C = x.size(-1), O = w_out.size(0), F = w_out.size(1);
+  if (C % 8 || O % 8 || F % 8 || C < 8 || O < 8 || F < 8) return std::nullopt;
+  const at::ScalarType type = x.scalar_type();
+  if (!ready(w_in, x, type, {2 * F, C}) || !ready(w_out, x, type, {O, F}) || (b_in && !ready(*b_in, x, type, {2 * F})) ||
+      (b_out && !ready(*b_out, x, type, {O})))
+    return std::nullopt;
+  bool keep = false;
+  for (const Tensor* t : {&x, &w_in, &w_out, b_in ? &*b_in : &x, b_out ? &*b_out : &x}) {
+    if (!aligned(*t) || t->_fw_grad(0).defined()) return std::nullopt;
+    keep = keep || t->requires_grad();
+  }
+  return GatedMlp::apply(x, w_in, w_out, b_in, b_out, activation, keep && at::GradMode::is_enabled());
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Rotary positions
+// ---------------------------------------------------------------------------------------------------------------------
+struct Rotary : torch::autograd::Function<Rotary> {
+  // heads 0: one or two head-major tensors; otherwise a packed projection with that many heads
+  static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads,
+                             int64_t layout, double amplitude, bool inverse) {
+    const c10::cuda::CUDAGuard guard(first.device());
+    auto adjacent = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
+    const Tensor x[2] = {adjacent(first), second ? adjacent(*second) : Tensor()};
+    tensor_list out;
+    MfRotaryArgs a{};
+    auto add = [&](const Tensor& t, const Tensor& o, int64_t at, int64_t n, bool rotates, int token, int64_t head_in, int64_t head_out) {
+      const int64_t bytes = at * (int64_t)t.element_size();
+      a.tensor[a.tensors++] = {static_cast<const char*>(t.const_data_ptr()) + bytes, static_cast<char*>(o.data_ptr()) + bytes, (int32_t)n, rotates,
+                               t.stride(0), t.stride(token), head_in, o.stride(0), o.stride(token), head_out};
+    };
+    for (const Tensor& t : x) {
+      if (!t.defined()) continue;
+      out.push_back(at::empty_like(t));
+      const Tensor& o = out.back();
+      a.batch = t.size(0), a.tokens = t.size(heads ? 1 : 2), a.head_dim = heads ? t.size(2) / (3 * heads) : t.size(3);
+      if (heads)
+        for (int i = 0; i < 3; ++i) add(t, o, i * heads * a.head_dim, heads, i < 2, 1, a.head_dim, a.head_dim);
+      else add(t, o, 0, t.size(1), true, 2, t.stride(1), o.stride(1));
+    }
+    a.axes = table.dim() == 1 ? 1 : table.size(0), a.pairs = table.size(-1);
+    a.dtype = dtype_code(first), a.layout = layout, a.inverse = inverse, a.amplitude = amplitude;
+    a.position_type = positions.scalar_type() == at::kInt    ? MF_POSITION_I32
+                      : positions.scalar_type() == at::kLong ? MF_POSITION_I64
+                      : positions.scalar_type() == at::kFloat ? MF_POSITION_F32
+                                                             : MF_POSITION_F64;
+    a.positions = positions.const_data_ptr(), a.position_batch = positions.dim() == table.dim() + 1 ? positions.stride(0) : 0;
+    a.frequencies = table.const_data_ptr<double>();
+    check(mf_rotary(&a, c10::cuda::getCurrentCUDAStream().stream()));
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["positions"] = positions;
+    ctx->saved_data["table"] = table;
+    ctx->saved_data["heads"] = heads, ctx->saved_data["layout"] = layout, ctx->saved_data["amplitude"] = amplitude, ctx->saved_data["inverse"] = inverse;
+    return out;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    tensor_list given, g(8);
+    for (const Tensor& t : grads)
+      if (t.defined()) given.push_back(t);
+    if (given.empty()) return g;
+    auto& s = ctx->saved_data;
+    const tensor_list turned = Rotary::apply(given[0], given.size() > 1 ? OptTensor(given[1]) : std::nullopt, s["positions"].toTensor(), s["table"].toTensor(),
+                                             s["heads"].toInt(), s["layout"].toInt(), s["amplitude"].toDouble(), !s["inverse"].toBool());
+    for (size_t i = 0, j = 0; i < grads.size(); ++i)
+      if (grads[i].defined()) g[i] = turned[j++];
+    return g;
+  }
+};
+
+std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads, int64_t layout,
+                                  double amplitude) {
+  if (!first.is_cuda() || dtype_code(first) < 0 || first.dim() != (heads ? 3 : 4) || first.numel() == 0 || !std::isfinite(amplitude)) return std::nullopt;
+  if (heads < 0 || (heads && first.size(2) % (3 * heads))) return std::nullopt;
+  const int64_t B = first.size(0), N = first.size(heads ? 1 : 2), D = heads ? first.size(2) / (3 * heads) : first.size(3);
+  if (second && (second->dim() != 4 || second->scalar_type() != first.scalar_type() || second->device() != first.device() || second->numel() == 0 ||
+                 second->size(0) != B || second->size(2) != N || second->size(3) != D))
+    return std::nullopt;
+  if (!table.device().is_cpu() || table.scalar_type() != at::kDouble || !table.is_contiguous() || table.dim() < 1 || table.dim() > 2 || table.requires_grad() ||
+      table.numel() < 1 || table.numel() > 128 || 2 * table.numel() > D)
+    return std::nullopt;
+  const at::ScalarType type = positions.scalar_type();
+  std::vector<int64_t> shape = {B, N};
+  if (table.dim() == 2) shape.push_back(table.size(0));
+  if (positions.device() != first.device() || !positions.is_contiguous() || positions.requires_grad() ||
+      (type != at::kInt && type != at::kLong && type != at::kFloat && type != at::kDouble) ||
+      (positions.sizes() != at::IntArrayRef(shape) && positions.sizes() != at::IntArrayRef(shape).slice(1)))
+    return std::nullopt;
+  if (first._fw_grad(0).defined() || (second && second->_fw_grad(0).defined())) return std::nullopt;
+  return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -333,6 +498,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sparse_attention", &sparse_attention);
   m.def("radius_blocks", &radius_blocks);
   m.def("knn_topk", &knn_topk);
+  m.def("gated_mlp", &gated_mlp);
+  m.def("rotary", &rotary);
   m.def("remember_status", &remember_status);
   m.def("last_status", &last_status);
 }

@@ -118,6 +118,11 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
 
     Sums are in fp32 in a fixed order.  The hidden values, and for the backward pass the pre-activations and their gradients, are
     rounded to ``x``'s type.  C, F and O are multiples of 8.  The gradient is once differentiable."""
+    native = _lib.native()
+    if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++
+        out = native.gated_mlp(x, w_in, w_out, b_in, b_out, ACTIVATIONS[activation])
+        if out is not None:
+            return out
     _check(x, w_in, w_out, b_in, b_out, activation)
     return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, activation)
 

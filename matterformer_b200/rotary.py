@@ -127,6 +127,14 @@ def _check(name, tensors, tokens, batch, head_dim, positions, frequencies, layou
                          f"{tuple(positions.shape)} on {positions.device}")  # fmt: skip
 
 
+def _ready(a, b, positions, frequencies, heads, layout, amplitude):
+    """The whole call in C++ where that is built and the operands are ready as they are, else None."""
+    native = _lib.native()
+    if native is None or layout not in _lib.MF_ROTARY or not all(isinstance(t, torch.Tensor) for t in (a, positions, frequencies)):
+        return None
+    return native.rotary(a, b, positions, frequencies, heads, _lib.MF_ROTARY[layout], float(amplitude))
+
+
 def _apply(a, b, positions, frequencies, heads, layout, amplitude):
     positions, table = positions.contiguous(), frequencies.double().contiguous()
     return _Rotary.apply(a, b, positions, table, heads, layout, float(amplitude), False)
@@ -141,6 +149,9 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     (pairs,); (N, A) or (B, N, A) for frequencies (A, pairs), whose pairs follow each other axis by axis; integer or floating.  ``frequencies``: on the
     host (:func:`rotary_frequencies`).  Any strides with adjacent channels; results have the strides of dense inputs.  Differentiable
     in ``q`` and ``k``."""
+    out = _ready(q, k, positions, frequencies, 0, layout, amplitude)
+    if out is not None:
+        return (out[0], None) if k is None else tuple(out)
     tensors = [t for t in (q, k) if t is not None]
     if any(t.ndim != 4 for t in tensors) or (k is not None and (k.shape[0], k.shape[2:]) != (q.shape[0], q.shape[2:])):
         raise ValueError(f"rotary_embedding: q (B, H, N, D) and k (B, K, N, D) expected, got {[tuple(t.shape) for t in tensors]}")
@@ -152,6 +163,9 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
 def rotary_packed(qkv: torch.Tensor, heads: int, positions: torch.Tensor, frequencies: torch.Tensor, *, layout: str = "half",
                   amplitude: float = 1.0) -> torch.Tensor:  # fmt: skip
     """:func:`rotary_embedding` on the packed projection of an attention layer, ``qkv`` (B, N, 3*H*D): queries and keys turned, values copied."""
+    out = _ready(qkv, None, positions, frequencies, int(heads), layout, amplitude) if heads >= 1 else None
+    if out is not None:
+        return out[0]
     if qkv.ndim != 3 or heads < 1 or qkv.shape[2] % (3 * heads) or qkv.shape[2] == 0:
         raise ValueError(f"rotary_packed: qkv (B, N, 3*H*D) with H = {heads} expected, got {tuple(qkv.shape)}")
     _check("rotary_packed", [qkv], qkv.shape[1], qkv.shape[0], qkv.shape[2] // (3 * heads), positions, frequencies, layout, amplitude)
