@@ -12,7 +12,7 @@ from .simplicial import (
 from .batching import AttentionCostBatchSampler, simplicial_tile_steps
 from .gated import gated_mlp, gated_mlp_status
 from .hostio import HostPipelinedSimplicial
-from .rotary import rotary_embedding, rotary_frequencies, rotary_packed
+from .rotary import RotaryPositions, rotary_embedding, rotary_frequencies, rotary_packed
 from .sampler import GraphedDenoiser, edm_sample
 from .sparse import (
     RadiusBlocks,
@@ -29,6 +29,7 @@ from .sparse import (
 __all__ = [
     "gated_mlp",
     "gated_mlp_status",
+    "RotaryPositions",
     "rotary_embedding",
     "rotary_frequencies",
     "rotary_packed",

@@ -510,6 +510,20 @@ def native():
     return _NATIVE[0]
 
 
+def foreign_leaves(*tensors) -> bool:
+    """Whether a pass that is being captured starts from a leaf whose gradients another stream takes (see torch_binding.cpp)."""
+    if not torch.cuda.is_current_stream_capturing():
+        return False
+    module = native()
+    return module is not None and any(t is not None and module.foreign_leaf(t) for t in tensors)
+
+
+def refuse_foreign(foreign: bool, name: str) -> None:
+    if foreign and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name}: a backward pass cannot be captured while a graph of the same leaf from another stream is alive; "
+                           "release that graph (the outputs that hold it) before the capture")  # fmt: skip
+
+
 def last_error() -> str:
     buf = ctypes.create_string_buffer(512)
     lib().mf_last_error(buf, 512)

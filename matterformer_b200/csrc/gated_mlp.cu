@@ -61,17 +61,17 @@ int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
 // ---- gradients of the weights --------------------------------------------------------------------------------------
 // Both are sums over the tokens, of [dg du] x and of dy h: one launch for the tiles of both.  Whole rounds of tiles walk all tokens;
 // the tiles behind them are cut into pieces of the tokens, each with a plane of partial sums of its own, which add_planes_kernel adds in order.
+// The plan goes by the sizes of both gradients, so that one's bits do not depend on whether the other is wanted.
 struct WeightPlan {
-  int k_blocks, tiles1, tiles2, whole, rest, pieces, per;
+  int k_blocks, tiles1, tiles, pieces, per;
+  int first, whole, first_rest, rest;  // of the wanted tiles: the first, how many are whole, and those that are cut
 };
 WeightPlan weight_plan(const MfGatedMlpArgs* a) {
   WeightPlan w;
   w.k_blocks = (int)((a->rows + kBlockK - 1) / kBlockK);
-  w.tiles1 = a->grad_w_in ? tiles_of(2ll * a->hidden, a->dim, kTile) : 0;
-  w.tiles2 = a->grad_w_out ? tiles_of(a->dim_out, a->hidden, kTile) : 0;
-  const int tiles = w.tiles1 + w.tiles2;
-  w.rest = tiles % kPairs;
-  w.whole = tiles - w.rest;
+  w.tiles1 = tiles_of(2ll * a->hidden, a->dim, kTile);
+  w.tiles = w.tiles1 + tiles_of(a->dim_out, a->hidden, kTile);
+  w.rest = w.tiles % kPairs;
   w.pieces = 1, w.per = w.k_blocks;
   // The number of pieces with the least estimated time: rounds of the longest piece, 0.3 us for a block of 64 tokens, and 0.1 us for
   // each plane's way to memory and back.
@@ -82,7 +82,13 @@ WeightPlan weight_plan(const MfGatedMlpArgs* a) {
     const double us = 0.3 * ((w.rest * s + kPairs - 1) / kPairs) * per + (s > 1 ? 0.1 * w.rest * s : 0.);
     if (us < least) least = us, w.pieces = s, w.per = per;
   }
-  if (w.pieces == 1) w.whole = tiles, w.rest = 0;
+  const int cut_from = w.pieces == 1 ? w.tiles : w.tiles - w.rest;
+  const int end = a->grad_w_out ? w.tiles : w.tiles1;
+  w.first = a->grad_w_in ? 0 : w.tiles1;
+  w.first_rest = cut_from < w.first ? w.first : cut_from;
+  w.whole = (cut_from < end ? cut_from : end) - w.first;
+  if (w.whole < 0) w.whole = 0;
+  w.rest = end > w.first_rest ? end - w.first_rest : 0;
   return w;
 }
 size_t plane_bytes(const WeightPlan& w) { return (size_t)w.rest * w.pieces * kTile * kTile * 4; }
@@ -91,7 +97,7 @@ template <typename T, typename TOut>
 __global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict__ planes, WeightPlan w, TOut* __restrict__ out1, int m1, int n1,
                                                          TOut* __restrict__ out2, int m2, int n2) {
   wait_for_previous();
-  const int tile = w.whole + blockIdx.x;
+  const int tile = w.first_rest + blockIdx.x;
   const bool second = tile >= w.tiles1;
   const int m = second ? m2 : m1, n = second ? n2 : n1;
   TOut* out = second ? out2 : out1;
@@ -196,10 +202,11 @@ int weight_gradients(const MfGatedMlpArgs* a, const void* grad_pre, float* plane
   const WeightPlan w = weight_plan(a);
   Params p{};
   p.k = (int)a->rows, p.waits = waits, p.wide_out = a->grad_dtype == MF_DTYPE_F32;
-  p.whole = w.whole, p.rest = w.rest, p.per = w.per, p.first2 = w.tiles1, p.tiles = w.whole + w.rest * w.pieces;
+  p.first = w.first, p.whole = w.whole, p.first_rest = w.first_rest, p.rest = w.rest, p.per = w.per, p.first2 = w.tiles1;
+  p.tiles = w.whole + w.rest * w.pieces;
   p.one.m = 2 * F, p.one.n = C;
-  if (w.tiles1) MF_MAP(weight_problem<T>(p.one, a, grad_pre, 2 * F, a->x, C, a->grad_w_in));
-  if (w.tiles2) MF_MAP(weight_problem<T>(p.two, a, a->grad_y, O, a->act, F, a->grad_w_out));
+  if (a->grad_w_in) MF_MAP(weight_problem<T>(p.one, a, grad_pre, 2 * F, a->x, C, a->grad_w_in));
+  if (a->grad_w_out) MF_MAP(weight_problem<T>(p.two, a, a->grad_y, O, a->act, F, a->grad_w_out));
   if (w.rest) {
     const long long dims[2] = {kTile, (long long)w.rest * w.pieces * kTile}, strides[1] = {4 * kTile};
     MF_MAP(make_tensor_map(&p.pre, planes, MF_DTYPE_F32, 2, dims, strides, 32, 32));

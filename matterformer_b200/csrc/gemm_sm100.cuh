@@ -68,7 +68,8 @@ struct Params {
   int k;
   int whole, cut, tiles;    // tiles of full width, columns of a later one = full width / cut, pieces of work in all
   int first2;               // kWeight: the second product's first tile
-  int rest, per;            // kWeight: tiles that are cut along the contracted dimension, and how many blocks a piece has
+  int first, first_rest;    // kWeight: the first tile, and the first that is cut along the contracted dimension
+  int rest, per;            // kWeight: how many are cut, and how many blocks a piece has
   int keep_pre;
   int wide_out;             // kWeight: fp32 results
   BoundedWaits waits;       // kinds: 0 operands, 1 stages, 2 accumulators, 3 drained accumulators
@@ -250,10 +251,10 @@ struct Walk {
       // The same piece of all cut tiles comes before the next piece of any: pairs that work at the same time read the same stretch of
       // the operands.  (Equal shares of all blocks in a row, where each pair is somewhere else, took 210 us instead of 100 on
       // 29 696 tokens: all operands came from memory again and again.)
-      int tile = t;
+      int tile = p.first + t;
       if (!whole) {
         const int u = t - p.whole;
-        tile = p.whole + u % p.rest;
+        tile = p.first_rest + u % p.rest;
         w.k0 = u / p.rest * p.per, w.k1 = min(k_blocks, w.k0 + p.per), w.plane = u;
       }
       w.second = tile >= p.first2;

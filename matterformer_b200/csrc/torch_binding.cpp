@@ -6,6 +6,7 @@
 // that way and takes 20.  These functions serve calls whose operands are
 // ready as they are (contiguous, on one device, of the types the kernels take) and return None for every other call, which
 // then takes the Python path with its conversions and error messages.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -329,6 +330,32 @@ std::optional<std::array<Tensor, 2>> knn_topk(const Tensor& pos, const Tensor& l
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// A backward pass under capture
+// ---------------------------------------------------------------------------------------------------------------------
+// A leaf has one node that takes its gradients, on the stream on which the first graph that is still alive made it.  The engine joins
+// that stream with the one of a backward pass; if the latter is being captured, that ends the capture with an error of the runtime
+// which names nothing.  The operators below say so instead: noted when their forward pass is captured, raised by its backward pass.
+bool foreign_leaf(const Tensor& t) {
+  if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return false;
+  const auto stream = node->stream();
+  return stream && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap();
+}
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+bool foreign_leaves(std::initializer_list<const Tensor*> inputs) {
+  if (!at::GradMode::is_enabled() || !capturing()) return false;
+  for (const Tensor* t : inputs)
+    if (foreign_leaf(*t)) return true;
+  return false;
+}
+void refuse_foreign(bool foreign, const char* name) {
+  if (foreign && capturing())
+    throw std::runtime_error(std::string(name) + ": a backward pass cannot be captured while a graph of the same leaf from another stream is alive; "
+                             "release that graph (the outputs that hold it) before the capture");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // Gated feed-forward block
 // ---------------------------------------------------------------------------------------------------------------------
 bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
@@ -342,7 +369,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
   }
 
   static Variable forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const OptTensor& b_in, const OptTensor& b_out,
-                          int64_t activation, bool keep) {
+                          int64_t activation, bool keep, bool foreign) {
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor bi = b_in ? *b_in : Tensor(), bo = b_out ? *b_out : Tensor();
     MfGatedMlpArgs a{};
@@ -355,6 +382,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     check(mf_gated_mlp_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
     if (keep) {
       ctx->saved_data["activation"] = activation;
+      ctx->saved_data["foreign"] = foreign;
       ctx->save_for_backward({x, w_in, w_out, bi, bo, pre, act});
     }
     return y;
@@ -365,7 +393,8 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     const Tensor& x = s[0];
     const c10::cuda::CUDAGuard guard(x.device());
     MfGatedMlpArgs a{};
-    tensor_list g(7);  // (one for each argument of forward)
+    tensor_list g(8);  // (one for each argument of forward)
+    refuse_foreign(ctx->saved_data["foreign"].toBool(), "gated_mlp");
     {
       const at::NoGradGuard no_grad;
       fill(a, x, s[1], s[2], s[3], s[4], ctx->saved_data["activation"].toInt());
@@ -410,7 +439,10 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
     if (!aligned(*t) || t->_fw_grad(0).defined()) return std::nullopt;
     keep = keep || t->requires_grad();
   }
-  return GatedMlp::apply(x, w_in, w_out, b_in, b_out, activation, keep && at::GradMode::is_enabled());
+  const Tensor none;
+  const c10::cuda::CUDAGuard guard(x.device());
+  const bool foreign = foreign_leaves({&x, &w_in, &w_out, b_in ? &*b_in : &none, b_out ? &*b_out : &none});
+  return GatedMlp::apply(x, w_in, w_out, b_in, b_out, activation, keep && at::GradMode::is_enabled(), foreign);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -419,7 +451,7 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
 struct Rotary : torch::autograd::Function<Rotary> {
   // heads 0: one or two head-major tensors; otherwise a packed projection with that many heads
   static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads,
-                             int64_t layout, double amplitude, bool inverse) {
+                             int64_t layout, double amplitude, bool inverse, bool foreign) {
     const c10::cuda::CUDAGuard guard(first.device());
     auto adjacent = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
     const Tensor x[2] = {adjacent(first), second ? adjacent(*second) : Tensor()};
@@ -452,17 +484,19 @@ struct Rotary : torch::autograd::Function<Rotary> {
     ctx->saved_data["positions"] = positions;
     ctx->saved_data["table"] = table;
     ctx->saved_data["heads"] = heads, ctx->saved_data["layout"] = layout, ctx->saved_data["amplitude"] = amplitude, ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["foreign"] = foreign;
     return out;
   }
 
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    tensor_list given, g(8);
+    tensor_list given, g(9);
+    refuse_foreign(ctx->saved_data["foreign"].toBool(), "rotary_embedding");
     for (const Tensor& t : grads)
       if (t.defined()) given.push_back(t);
     if (given.empty()) return g;
     auto& s = ctx->saved_data;
     const tensor_list turned = Rotary::apply(given[0], given.size() > 1 ? OptTensor(given[1]) : std::nullopt, s["positions"].toTensor(), s["table"].toTensor(),
-                                             s["heads"].toInt(), s["layout"].toInt(), s["amplitude"].toDouble(), !s["inverse"].toBool());
+                                             s["heads"].toInt(), s["layout"].toInt(), s["amplitude"].toDouble(), !s["inverse"].toBool(), false);
     for (size_t i = 0, j = 0; i < grads.size(); ++i)
       if (grads[i].defined()) g[i] = turned[j++];
     return g;
@@ -488,7 +522,9 @@ std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, 
       (positions.sizes() != at::IntArrayRef(shape) && positions.sizes() != at::IntArrayRef(shape).slice(1)))
     return std::nullopt;
   if (first._fw_grad(0).defined() || (second && second->_fw_grad(0).defined())) return std::nullopt;
-  return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false);
+  const Tensor none;
+  const c10::cuda::CUDAGuard guard(first.device());
+  return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false, foreign_leaves({&first, second ? &*second : &none}));
 }
 
 }  // namespace
@@ -498,6 +534,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sparse_attention", &sparse_attention);
   m.def("radius_blocks", &radius_blocks);
   m.def("knn_topk", &knn_topk);
+  m.def("foreign_leaf", &foreign_leaf);
   m.def("gated_mlp", &gated_mlp);
   m.def("rotary", &rotary);
   m.def("remember_status", &remember_status);

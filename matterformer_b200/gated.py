@@ -11,10 +11,11 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .linear import bf16_copy
+
+_ONCE = b"trying to differentiate twice a function that was marked with @once_differentiable"
 
 _CODE = {torch.bfloat16: _lib.MF_DTYPE_BF16, torch.float16: _lib.MF_DTYPE_F16}
 ACTIVATIONS = {"silu": _lib.MF_ACT_SILU, "gelu_tanh": _lib.MF_ACT_GELU_TANH}
@@ -56,12 +57,24 @@ class _GatedMlp(torch.autograd.Function):
         a.pre, a.act, a.y = _ptr(pre), _ptr(act), _ptr(y)
         _lib.launch(_lib.lib().mf_gated_mlp_fwd, x.device, ctypes.byref(a))
         if keep:
+            ctx.foreign = _lib.foreign_leaves(x, w_in, w_out, b_in, b_out)
             ctx.save_for_backward(x2, *params, pre, act)
         return y.view(*x.shape[:-1], w_out.shape[0])
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_y):
+        _lib.refuse_foreign(ctx.foreign, "gated_mlp")
+        with torch.no_grad():
+            grads = _GatedMlp._gradients(ctx, grad_y)
+        if torch.is_grad_enabled():  # create_graph: an error for who differentiates again, whichever operand the second gradient is of
+            given = [g.requires_grad_() for g in grads if g is not None]
+            made = torch._C._functions.DelayedError(_ONCE, len(given))(*given)
+            made = iter((made,) if len(given) == 1 else made)
+            grads = [None if g is None else next(made) for g in grads]
+        return (*grads, None)
+
+    @staticmethod
+    def _gradients(ctx, grad_y):
         x, w_in, w_out, b_in, b_out, pre, act = ctx.saved_tensors
         grad_y = _ready(grad_y.reshape(-1, w_out.shape[0]).to(x.dtype))
         a = _args(x, w_in, w_out, b_in, b_out, ctx.activation, ctx.grad_dtype)
@@ -77,7 +90,7 @@ class _GatedMlp(torch.autograd.Function):
         _lib.launch(L.mf_gated_mlp_bwd, x.device, ctypes.byref(a))
         if grads[0] is not None:
             grads[0] = grads[0].view(ctx.shape)
-        return (*grads, None)
+        return grads
 
 
 def gated_mlp_applies(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> bool:

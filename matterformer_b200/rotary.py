@@ -9,7 +9,9 @@ Angles are formed in 64 bits, so that positions of millions keep theirs.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -49,6 +51,41 @@ def rotary_frequencies(rotary_dim: int, *, axes: int = 1, base: float = 10000.0,
     return theta if axes == 1 else theta.repeat(axes, 1)
 
 
+@dataclass(frozen=True)
+class RotaryPositions:
+    """How an attention layer turns its queries and keys: the arguments of :func:`rotary_frequencies` and of :func:`rotary_embedding`."""
+
+    rotary_dim: int
+    axes: int = 1
+    base: float = 10000.0
+    layout: str = "half"
+    amplitude: float = 1.0
+    scaling: str = "none"
+    factor: float = 1.0
+    original_length: Optional[float] = None
+
+    @functools.cached_property
+    def frequencies(self) -> torch.Tensor:
+        return rotary_frequencies(self.rotary_dim, axes=self.axes, base=self.base, scaling=self.scaling, factor=self.factor,
+                                  original_length=self.original_length)  # fmt: skip
+
+
+def rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:
+    """:func:`rotary_embedding` of one (B, H, N, D) tensor in plain torch operations, on any device; angles in 64 bits."""
+    table = frequencies.to(positions.device)
+    angle = positions.double()[..., None] * table if table.ndim == 1 else (positions.double()[..., None] * table).flatten(-2)
+    if angle.ndim == 2:
+        angle = angle[None]
+    wide = torch.promote_types(x.dtype, torch.float32)
+    cos, sin = (amplitude * f(angle[:, None]).to(wide) for f in (torch.cos, torch.sin))
+    P = cos.shape[-1]
+    a, b = (x[..., :P], x[..., P : 2 * P]) if layout == "half" else (x[..., 0 : 2 * P : 2], x[..., 1 : 2 * P : 2])
+    a, b = a.to(wide), b.to(wide)
+    turned = (a * cos - b * sin, a * sin + b * cos)
+    turned = torch.cat(turned, dim=-1) if layout == "half" else torch.stack(turned, dim=-1).flatten(-2)
+    return torch.cat([turned.to(x.dtype), x[..., 2 * P :]], dim=-1)
+
+
 def _fill(tensor, x, out, heads, rotates, strides_in, strides_out):
     tensor.input, tensor.out, tensor.heads, tensor.rotates = x, out, heads, rotates
     tensor.in_batch, tensor.in_token, tensor.in_head = strides_in
@@ -62,6 +99,7 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, a, b, positions, table, heads, layout, amplitude, inverse):
         ctx.set_materialize_grads(False)
         ctx.call = (positions, table, heads, layout, amplitude, inverse)
+        ctx.foreign = _lib.foreign_leaves(a, b)
         args = _lib.MfRotaryArgs()
         tensors = [t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (a, b)]
         x = next(t for t in tensors if t is not None)
@@ -90,6 +128,7 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
+        _lib.refuse_foreign(ctx.foreign, "rotary_embedding")
         positions, table, heads, layout, amplitude, inverse = ctx.call
         given = [g for g in grads if g is not None]  # (one of two outputs may be unused)
         out = [None] * 8

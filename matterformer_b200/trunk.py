@@ -13,8 +13,9 @@ so a reference ``state_dict`` of the same configuration loads with ``strict=True
 * :class:`EDMModel`             <- ``QM9EDMModel`` with geometry bias off, src/matterformer/models/qm9.py:249-565
 * :class:`EDMPreconditioner`, :class:`EDMLoss` <- src/matterformer/tasks/edm.py:34-150
 
-Only what that configuration touches is mirrored: no geometry-bias builders, no RoPE, no coordinate
-embedding.  ``impl="cuda"`` (and ``"auto"`` on CUDA tensors) runs the sm_100a kernels through the C ABI;
+Only what that configuration touches is mirrored: no geometry-bias builders, no coordinate embedding.  Two options go beyond it:
+``rotary`` (rotary positions in the MHA layers, as ``RotaryMultiheadAttention`` has them, regular_attention.py:208-271) and
+``mlp_type="gated"`` (:class:`GatedMlp` in the place of :class:`Mlp`).  ``impl="cuda"`` (and ``"auto"`` on CUDA tensors) runs the sm_100a kernels through the C ABI;
 ``impl="torch"`` is the dense formulation in plain torch ops, as in the reference.
 """
 from __future__ import annotations
@@ -30,8 +31,10 @@ from torch import nn
 from . import fused
 from .fused import (fused_applies, gated_layer_norm, gated_ln_modulate, gated_residual, heads_layout_applies, ln_modulate, merge_heads, split_heads,
                     split_modulation)
+from .gated import gated_mlp, gated_mlp_applies
 from .linear import bf16_copies, linear_bf16, linear_bf16_applies, linear_gelu_bf16, pair_linear_bf16, stacked_modulation
-from .simplicial import (normalize_simplicial_precision, packed_projection_applies, simplicial_attention_cuda,
+from .rotary import RotaryPositions, rotary_embedding, rotary_packed, rotate_torch
+from .simplicial import (_DTYPE_CODE, normalize_simplicial_precision, packed_projection_applies, simplicial_attention_cuda,
                          simplicial_attention_packed)  # fmt: skip
 
 
@@ -211,12 +214,19 @@ class RegularAttention(nn.Module):
     ``nn.MultiheadAttention`` like everything else this kernel does not cover.  Rows of padded tokens
     return zeros on the kernel path instead of the reference's average over the real keys; the trunk
     discards those rows.  ``impl="torch"`` always uses ``nn.MultiheadAttention``.
+
+    With ``rotary`` the layer takes ``positions`` and turns its queries and keys before the core, whichever that is; the dense one is
+    then ``F.scaled_dot_product_attention``, since ``nn.MultiheadAttention`` has no place for it.
     """
 
-    def __init__(self, embed_dim: int, num_heads: int, *, dropout: float = 0.0, impl: str = "auto") -> None:
+    def __init__(self, embed_dim: int, num_heads: int, *, dropout: float = 0.0, impl: str = "auto",
+                 rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
         super().__init__()
         if impl not in {"auto", "torch"}:
             raise ValueError(f"Unsupported attention impl: {impl}")
+        if rotary is not None and rotary.rotary_dim > embed_dim // num_heads:
+            raise ValueError(f"rotary_dim {rotary.rotary_dim} above the head size {embed_dim // num_heads}")
+        self.rotary = rotary
         self.attn = nn.MultiheadAttention(embed_dim, num_heads, dropout=dropout, batch_first=True)
         self.impl = impl
         self._last_core_used: Optional[str] = None
@@ -232,7 +242,24 @@ class RegularAttention(nn.Module):
         )
         return bf16 and (self.attn.embed_dim // self.attn.num_heads) in (32, 64, 128)
 
-    def _sparse_forward(self, x: torch.Tensor, plan: SparseAttentionPlan) -> torch.Tensor:
+    def _turned(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
+        """Queries and keys, (B, H, N, D) each."""
+        r = self.rotary
+        if q.is_cuda and self.impl != "torch" and q.dtype in _DTYPE_CODE:
+            return rotary_embedding(q, k, positions, r.frequencies, layout=r.layout, amplitude=r.amplitude)
+        return tuple(rotate_torch(t, positions, r.frequencies, r.layout, r.amplitude) for t in (q, k))
+
+    def _dense_rotary(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor], positions: torch.Tensor) -> torch.Tensor:
+        B, N, C = x.shape
+        H = self.attn.num_heads
+        qkv = linear_bf16(x, self.attn.in_proj_weight, self.attn.in_proj_bias)
+        q, k, v = qkv.view(B, N, 3, H, C // H).permute(2, 0, 3, 1, 4)
+        q, k = self._turned(q, k, positions)
+        visible = None if key_padding_mask is None else ~key_padding_mask.bool()[:, None, None, :]
+        core = F.scaled_dot_product_attention(q, k, v, attn_mask=visible, dropout_p=self.attn.dropout if self.training else 0.0)
+        return linear_bf16(core.transpose(1, 2).reshape(B, N, C), self.attn.out_proj.weight, self.attn.out_proj.bias)
+
+    def _sparse_forward(self, x: torch.Tensor, plan: SparseAttentionPlan, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The layer with its core on the radius block-sparse or the local-window kernel.  Same parameters and
         projections as the dense layer; only the set of visible keys differs."""
         from .sparse import local_window_attention, radius_block_sparse_attention
@@ -242,6 +269,8 @@ class RegularAttention(nn.Module):
         qkv = F.linear(x, self.attn.in_proj_weight, self.attn.in_proj_bias)
         qkv = qkv.to(torch.bfloat16) if low else qkv.float()
         q, k, v = split_heads(qkv, 3, H)  # each (B, H, N, D), one pass
+        if positions is not None:
+            q, k = self._turned(q, k, positions)
         if plan.kind == "radius":
             core = radius_block_sparse_attention(q, k, v, plan.blocks, sorted_inputs=False)
         else:  # band over the cell-sorted order: gather, attend, scatter back
@@ -253,17 +282,22 @@ class RegularAttention(nn.Module):
 
     def forward(self, x: torch.Tensor, *, key_padding_mask: Optional[torch.Tensor] = None,
                 sparse_plan: Optional[SparseAttentionPlan] = None, num_atoms: Optional[torch.Tensor] = None,
-                padding_is_suffix: Optional[bool] = None) -> torch.Tensor:  # fmt: skip
+                padding_is_suffix: Optional[bool] = None, positions: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
         """``num_atoms``: the (B,) int32 counts of real tokens, ``padding_is_suffix``: the form of the mask, when the caller
-        has already found them."""
+        has already found them.  ``positions``: of the tokens, for a layer with ``rotary`` (see :func:`rotary_embedding`); others take none."""
+        if (self.rotary is None) != (positions is None):
+            raise ValueError("a layer with rotary positions needs `positions`" if positions is None else
+                             "`positions` are for a layer with rotary positions")  # fmt: skip
         if sparse_plan is not None:
             if not x.is_cuda:
                 raise RuntimeError("sparse attention plans need CUDA tensors (there is no CPU fallback)")
-            return self._sparse_forward(x, sparse_plan)
+            return self._sparse_forward(x, sparse_plan, positions)
         if not self._core_fits(x, key_padding_mask) or not (
             _padding_is_suffix(self, key_padding_mask) if padding_is_suffix is None else padding_is_suffix
         ):
             self._last_core_used = "torch"
+            if positions is not None:
+                return self._dense_rotary(x, key_padding_mask, positions)
             out, _ = self.attn(x, x, x, key_padding_mask=key_padding_mask, need_weights=False)
             return out
         from .sparse import local_window_attention_packed
@@ -274,6 +308,9 @@ class RegularAttention(nn.Module):
         qkv = linear_bf16(x, self.attn.in_proj_weight, self.attn.in_proj_bias).to(torch.bfloat16)
         if num_atoms is None:
             num_atoms = (~key_padding_mask).sum(dim=1).to(torch.int32)
+        if positions is not None:
+            r = self.rotary
+            qkv = rotary_packed(qkv, H, positions, r.frequencies, layout=r.layout, amplitude=r.amplitude)
         # with at most 32 tokens the window-64 band covers every real token: dense attention, straight on the projection
         core = local_window_attention_packed(qkv, H, num_atoms, window=64)
         return linear_bf16(core, self.attn.out_proj.weight, self.attn.out_proj.bias)
@@ -289,6 +326,30 @@ class Mlp(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear_bf16(linear_gelu_bf16(x, self.fc1.weight, self.fc1.bias), self.fc2.weight, self.fc2.bias)
+
+
+class GatedMlp(nn.Module):
+    """``fc2(act(gate) * up)`` with ``gate, up = fc1(x).chunk(2, -1)``, through :func:`matterformer_b200.gated.gated_mlp` where that takes
+    the operands: CUDA and 16-bit arithmetic (a 16-bit input, or bf16 autocast), widths that are multiples of 8.  ``hidden``: by default two
+    thirds of :class:`Mlp`'s, up to a multiple of 8, which keeps the number of parameters."""
+
+    def __init__(self, d_model: int, mlp_ratio: float = 4.0, *, hidden: Optional[int] = None, activation: str = "silu") -> None:
+        super().__init__()
+        if activation not in {"silu", "gelu_tanh"}:
+            raise ValueError(f"Unsupported activation: {activation}")
+        self.hidden = -(-int(d_model * mlp_ratio * 2) // 24) * 8 if hidden is None else int(hidden)
+        self.activation = activation
+        self.fc1 = nn.Linear(d_model, 2 * self.hidden)
+        self.fc2 = nn.Linear(self.hidden, d_model)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w_in, b_in, w_out, b_out = self.fc1.weight, self.fc1.bias, self.fc2.weight, self.fc2.bias
+        low = x.to(torch.bfloat16) if _bf16_autocast(x) and w_in.dtype in (torch.float32, torch.bfloat16) else x
+        if gated_mlp_applies(low, w_in, w_out):
+            return gated_mlp(low, w_in, w_out, b_in, b_out, activation=self.activation)
+        gate, up = linear_bf16(x, w_in, b_in).chunk(2, dim=-1)
+        act = F.silu(gate) if self.activation == "silu" else F.gelu(gate, approximate="tanh")
+        return linear_bf16(act * up, w_out, b_out)
 
 
 def layer_norm(x: torch.Tensor, norm: nn.LayerNorm, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -322,11 +383,14 @@ class AdaLNBlock(nn.Module):
     """Pre-norm block with adaptive LayerNorm conditioning and gated residuals (transformer.py:154-316)."""
 
     def __init__(self, d_model: int, n_heads: int, *, mlp_ratio: float = 4.0, eps: float = 1e-6,
-                 attn_type: str = "mha", simplicial_impl: str = "auto", simplicial_precision: str = "bf16_tc") -> None:  # fmt: skip
+                 attn_type: str = "mha", simplicial_impl: str = "auto", simplicial_precision: str = "bf16_tc",
+                 mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
         super().__init__()
         attn_type = attn_type.lower()
         if attn_type not in {"mha", "simplicial"}:
             raise ValueError(f"Unsupported attn_type: {attn_type}")
+        if mlp_type not in {"plain", "gated"}:
+            raise ValueError(f"Unsupported mlp_type: {mlp_type}")
         self.attn_type = attn_type
         self.norm1 = nn.LayerNorm(d_model, eps=eps, elementwise_affine=False)
         self.norm2 = nn.LayerNorm(d_model, eps=eps, elementwise_affine=False)
@@ -334,15 +398,15 @@ class AdaLNBlock(nn.Module):
         nn.init.zeros_(self.ada_ln[-1].weight)
         nn.init.zeros_(self.ada_ln[-1].bias)
         if attn_type == "mha":
-            self.attn = RegularAttention(d_model, n_heads)
+            self.attn = RegularAttention(d_model, n_heads, rotary=rotary)
         else:
             self.attn = SimplicialAttention(d_model, n_heads, impl=simplicial_impl, precision=simplicial_precision)
-        self.mlp = Mlp(d_model, mlp_ratio)
+        self.mlp = Mlp(d_model, mlp_ratio) if mlp_type == "plain" else GatedMlp(d_model, mlp_ratio)
         self.fused_elementwise = True  # CUDA fp32 residual stream: fused norm+modulate and gated-residual kernels
 
     def forward(self, x, cond_emb, *, pad_mask=None, simplicial_attention_mask=None, sparse_plan=None,
                 zero_padding: bool = False, cond_act=None, modulation=None, num_atoms=None, h=None, following=None,
-                padding_is_suffix=None):
+                padding_is_suffix=None, positions=None):
         """``zero_padding``: return the block's output with its padded rows cleared (the ``masked_fill`` the trunk
         applies before the next block), folded into the last fused pass when the fused kernels run.  ``cond_act``:
         ``SiLU(cond_emb)`` when the caller has already formed it (it is the same for every block of a trunk).
@@ -350,7 +414,7 @@ class AdaLNBlock(nn.Module):
         real tokens for the attention layer, ``padding_is_suffix``: whether they come first in every row.  ``following``:
         (shift, scale, eps) of the norm that opens the next block; the block then returns its output and that norm's, formed in
         one pass, and the next block takes the latter as ``h``.  (None, None, eps): the norm is the stack's output norm, which has no
-        modulation and is kept in fp32; only its output is returned."""
+        modulation and is kept in fp32; only its output is returned.  ``positions``: of the tokens, for an attention layer with ``rotary``."""
         fused = self.fused_elementwise and fused_applies(x)
         mod = None if modulation is not None else linear_bf16(cond_act if cond_act is not None else self.ada_ln[0](cond_emb), self.ada_ln[-1].weight,
                           self.ada_ln[-1].bias)  # fmt: skip
@@ -367,8 +431,9 @@ class AdaLNBlock(nn.Module):
         else:
             h = _modulate(self.norm1(x), shift_a, scale_a)
         if self.attn_type == "mha":
+            turning = {"positions": positions} if getattr(self.attn, "rotary", None) is not None else {}
             attn_out = self.attn(h, key_padding_mask=pad_mask, sparse_plan=sparse_plan, num_atoms=num_atoms,
-                                 padding_is_suffix=padding_is_suffix)  # fmt: skip
+                                 padding_is_suffix=padding_is_suffix, **turning)  # fmt: skip
         else:
             attn_out = self.attn(h, key_padding_mask=pad_mask, attention_mask=simplicial_attention_mask)
         if fused:
@@ -391,11 +456,12 @@ class TransformerTrunk(nn.Module):
 
     def __init__(self, d_model: int, n_heads: int, attn_types: Sequence[str], *, mlp_ratio: float = 4.0,
                  eps: float = 1e-6, simplicial_impl: str = "auto", simplicial_precision: str = "bf16_tc",
-                 emit_pair_valid: bool = True) -> None:  # fmt: skip
+                 emit_pair_valid: bool = True, mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
         super().__init__()
+        self.rotary = rotary
         self.blocks = nn.ModuleList(
             AdaLNBlock(d_model, n_heads, mlp_ratio=mlp_ratio, eps=eps, attn_type=t, simplicial_impl=simplicial_impl,
-                       simplicial_precision=simplicial_precision)  # fmt: skip
+                       simplicial_precision=simplicial_precision, mlp_type=mlp_type, rotary=rotary)  # fmt: skip
             for t in attn_types
         )
         self.norm_out = nn.LayerNorm(d_model, eps=eps, elementwise_affine=False)
@@ -415,23 +481,28 @@ class TransformerTrunk(nn.Module):
         return out
 
     def forward(self, x: torch.Tensor, cond_emb: torch.Tensor, *, pad_mask: Optional[torch.Tensor] = None,
-                sparse_plan: Optional[SparseAttentionPlan] = None, padding_cleared: bool = False) -> torch.Tensor:  # fmt: skip
+                sparse_plan: Optional[SparseAttentionPlan] = None, padding_cleared: bool = False,
+                positions: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
         """``sparse_plan`` (see :func:`plan_sparse_attention`) makes every MHA layer attend over the plan's
         neighbourhoods instead of all tokens: the periodic-crystal mode of the trunk.  ``padding_cleared``: the rows of ``x`` that
-        ``pad_mask`` marks are zeros already."""
+        ``pad_mask`` marks are zeros already.  ``positions``: of the tokens, needed by a trunk with ``rotary``."""
+        if (self.rotary is None) != (positions is None):
+            raise ValueError("a trunk with rotary positions needs `positions`" if positions is None else
+                             "`positions` are for a trunk with rotary positions")  # fmt: skip
+        turning = {} if positions is None else {"positions": positions}
         bf16 = x.is_cuda and torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16
         layers = [block.ada_ln[-1] for block in self.blocks]
         stacked = bf16 and fused_applies(x) and cond_emb.ndim == 2 and all(
             block.fused_elementwise and m.weight.dtype == torch.float32 and m.bias is not None for block, m in zip(self.blocks, layers)
         )
         if not (bf16 or (x.is_cuda and x.dtype == torch.bfloat16)):
-            return self._forward(x, cond_emb, pad_mask, sparse_plan, None, padding_cleared)
+            return self._forward(x, cond_emb, pad_mask, sparse_plan, None, padding_cleared, turning)
         # the bf16 copies the blocks' Linear layers compute with: all of them in one multi-tensor copy
         stacks = ([m.weight for m in layers], [m.bias for m in layers]) if stacked else ()
         with bf16_copies(self._linear_parameters(), stacks) as made:
-            return self._forward(x, cond_emb, pad_mask, sparse_plan, made if stacked else None, padding_cleared)
+            return self._forward(x, cond_emb, pad_mask, sparse_plan, made if stacked else None, padding_cleared, turning)
 
-    def _forward(self, x, cond_emb, pad_mask, sparse_plan, modulation_copies, padding_cleared):
+    def _forward(self, x, cond_emb, pad_mask, sparse_plan, modulation_copies, padding_cleared, turning):
         """``modulation_copies``: stacked bf16 weights and biases of the modulation layers, where one GEMM serves them all."""
         b, n, _ = x.shape
         if pad_mask is not None:
@@ -474,7 +545,7 @@ class TransformerTrunk(nn.Module):
             following = (*modulation[i + 1][:2], self.blocks[i + 1].norm1.eps) if chain else (None, None, norm.eps) if closing else None
             x = block(x, cond_emb, pad_mask=pad_mask, simplicial_attention_mask=sim_mask, sparse_plan=sparse_plan,
                       zero_padding=pad_mask is not None, cond_act=cond_act, modulation=six, num_atoms=num_atoms, h=h,
-                      following=following, padding_is_suffix=suffix)  # fmt: skip
+                      following=following, padding_is_suffix=suffix, **turning)  # fmt: skip
             x, h = x if chain else (x, None)
         if closing:
             return x
@@ -525,21 +596,25 @@ class EDMModel(nn.Module):
     """Atom/coordinate denoiser: token projection -> trunk -> atom head + equivariant pair head.
 
     Mirrors ``QM9EDMModel(use_geometry_bias=False, coord_embed_mode="none", coord_head_mode="equivariant")``
-    with the default noise conditioning (sigma channel concatenated to the atom features and adaLN).
+    with the default noise conditioning (sigma channel concatenated to the atom features and adaLN).  ``mlp_type`` and ``rotary`` go
+    to the trunk's blocks; rotary positions are the noisy coordinates, on three axes.
     """
 
     def __init__(self, *, atom_channels: int = 6, d_model: int = 512, n_heads: int = 8, n_layers: int = 12,
                  attn_types: Optional[Sequence[str]] = None, mlp_ratio: float = 4.0, simplicial_impl: str = "auto",
                  simplicial_precision: str = "bf16_tc", pair_hidden_dim: int = 128, pair_n_rbf: int = 16,
-                 pair_rbf_max: float = 4.0) -> None:  # fmt: skip
+                 pair_rbf_max: float = 4.0, mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
         super().__init__()
+        if rotary is not None and rotary.axes != 3:
+            raise ValueError(f"the coordinates are positions on 3 axes, rotary has {rotary.axes}")
         if attn_types is None:  # layers alternate MHA and 2-simplicial attention
             attn_types = ["mha" if i % 2 == 0 else "simplicial" for i in range(n_layers)]
         self.atom_channels = int(atom_channels)
         self.atom_proj = nn.Linear(self.atom_channels + 1, d_model)
         self.conditioning = TimeEmbedder(d_model)
         self.trunk = TransformerTrunk(d_model, n_heads, attn_types, mlp_ratio=mlp_ratio,
-                                      simplicial_impl=simplicial_impl, simplicial_precision=simplicial_precision)  # fmt: skip
+                                      simplicial_impl=simplicial_impl, simplicial_precision=simplicial_precision,
+                                      mlp_type=mlp_type, rotary=rotary)  # fmt: skip
         self.atom_head = nn.Sequential(nn.LayerNorm(d_model), nn.Linear(d_model, d_model), nn.SiLU(),
                                        nn.Linear(d_model, atom_channels))  # fmt: skip
         self.pair_head = nn.Sequential(nn.Linear(2 * d_model + pair_n_rbf, pair_hidden_dim), nn.SiLU(),
@@ -612,7 +687,10 @@ class EDMModel(nn.Module):
             feat = sigma_cond[:, None, None].expand(-1, atom_noisy.shape[1], 1).masked_fill(pad_mask[..., None], 0.0)
             tokens = linear_bf16(torch.cat([atom_noisy, feat], dim=-1), proj.weight, proj.bias)
         cond = self.conditioning(sigma_cond, sigma_cond)
-        trunk_out = self.trunk(tokens, cond, pad_mask=pad_mask, **({"padding_cleared": True} if whole and type(self.trunk) is TransformerTrunk else {}))
+        more = {"padding_cleared": True} if whole and type(self.trunk) is TransformerTrunk else {}
+        if getattr(self.trunk, "rotary", None) is not None:
+            more["positions"] = coords_noisy
+        trunk_out = self.trunk(tokens, cond, pad_mask=pad_mask, **more)
         normed = layer_norm(trunk_out, self.atom_head[0], torch.bfloat16 if low else torch.float32)
         atom_delta = _two_layers(self.atom_head[1:], normed).masked_fill(pad_mask[..., None], 0.0)
         return atom_delta, self._coord_delta(trunk_out, coords_noisy, pad_mask)

@@ -1,8 +1,12 @@
 """Gated feed-forward block against its definition in 64 bits."""
+import ctypes
+import threading
+
 import pytest
 import torch
 
 import matterformer_b200 as mfb
+from matterformer_b200 import _lib, gated
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +68,231 @@ def test_forward_and_gradients(rows, C, F, O, dtype):
         assert _off(a, b) < _bound(dtype), f"output {i}: {_off(a, b):.2e}"
     with torch.no_grad():  # nothing kept for a backward pass
         assert torch.equal(mfb.gated_mlp(*ops, activation=act), got[0])
+
+
+def test_gradient_against_differences():
+    """<gradient, direction> for every operand against a central difference of the loss in 64 bits."""
+    ops, dy = _operands(40, 64, 96, 72, BF16, True, seed=3)
+    grads = _run(ops, dy, "silu")[1:]
+    g = torch.Generator().manual_seed(4)
+
+    def loss(i, v, h):
+        x, w_in, w_out, b_in, b_out = (t.double() + (h * v if j == i else 0) for j, t in enumerate(ops))
+        gate, up = torch.nn.functional.linear(x, w_in, b_in).chunk(2, dim=-1)
+        return (torch.nn.functional.linear(torch.nn.functional.silu(gate) * up, w_out, b_out) * dy.double()).sum().item()
+
+    for i, t in enumerate(ops):
+        v = torch.randn(t.shape, generator=g).double().cuda()
+        difference = (loss(i, v, 1e-5) - loss(i, v, -1e-5)) / 2e-5
+        # each entry of the gradient is off by at most _bound of the root mean square; the sum's errors add in squares, times the direction
+        allowed = 6 * _bound(BF16) * grads[i].double().norm().item()
+        assert abs((grads[i].double() * v).sum().item() - difference) < allowed + 1e-4 * abs(difference)
+
+
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (3,), (4,), (0, 2), (1, 4), (1, 2, 3)])
+def test_only_the_wanted_gradients(wanted):
+    ops, dy = _operands(300, 64, 72, 80, BF16, True, seed=5)
+    everything = _run(ops, dy, "silu")[1:]
+    leaves = [t.detach().requires_grad_(i in wanted) for i, t in enumerate(ops)]
+    y = mfb.gated_mlp(*leaves)
+    got = torch.autograd.grad(y, [leaves[i] for i in wanted], dy)
+    for i, g in zip(wanted, got):
+        assert torch.equal(g, everything[i])
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_fp32_parameters(rows):
+    """Their bf16 copies compute, their gradients are not rounded."""
+    ops, dy = _operands(rows, 64, 136, 72, BF16, True, seed=6)
+    wide = [ops[0], *(t.float() for t in ops[1:])]
+    got, want = _run(wide, dy, "gelu_tanh"), _exact(ops, dy, "gelu_tanh")
+    assert [t.dtype for t in got] == [BF16, BF16, F32, F32, F32, F32]
+    low = _run(ops, dy, "gelu_tanh")
+    for a, b, c in zip(got, want, low):
+        assert _off(a, b) < _bound(BF16)
+        assert torch.equal(a.to(BF16), c)  # the same sums, rounded
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 31, 32, 33, 255, 256, 257])
+def test_token_counts(rows):
+    """Around the sizes at which kernels and tiles change; a row's result does not depend on the rows after it."""
+    ops, dy = _operands(rows, 128, 264, 136, BF16, True, seed=7)
+    got, want = _run(ops, dy, "silu"), _exact(ops, dy, "silu")
+    for a, b in zip(got, want):
+        assert _off(a, b) < _bound(BF16)
+
+
+def test_shapes_strides_and_alignment():
+    ops, dy = _operands(12, 64, 72, 80, BF16, True, seed=8, lead=(2, 3))
+    base = _run(ops, dy, "silu")
+    assert base[0].shape == (2, 3, 12, 80) and base[1].shape == ops[0].shape
+    x = ops[0]
+    wide = torch.full((2, 3, 12, 130), float("nan"), dtype=BF16, device="cuda")
+    wide[..., 3:67] = x
+    shifted = [wide[..., 3:67], *(torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape) for t in ops[1:])]
+    order = x.transpose(0, 2).contiguous().transpose(0, 2)
+    for other in (shifted, [order, *ops[1:]], [x, ops[1].t().contiguous().t(), *ops[2:]]):
+        for a, b in zip(_run(other, dy, "silu"), base):
+            assert torch.equal(a, b)
+    for strided in (dy.transpose(0, 1).contiguous().transpose(0, 1), dy[..., :1].expand(dy.shape), torch.cat([dy.flatten()[:1], dy.flatten()])[1:].view(dy.shape)):
+        for a, b in zip(_run(ops, strided, "silu"), _run(ops, strided.clone(memory_format=torch.contiguous_format), "silu")):
+            assert torch.equal(a, b)
+
+
+def test_no_tokens():
+    ops, dy = _operands(0, 64, 72, 80, F16, True)
+    got = _run(ops, dy, "silu")
+    assert got[0].shape == (0, 80) and got[1].shape == (0, 64)
+    assert all(not g.any() for g in got[2:])
+
+
+def test_extreme_values():
+    """Gates of +-30000 and of zero, an infinite and a NaN row: what is finite stays exact, and nothing reaches another row."""
+    for rows in (16, 300):
+        ops, dy = _operands(rows, 64, 72, 80, BF16, False, seed=9)
+        x = ops[0].clone()
+        x[3], x[4], x[5], x[7] = 1e4, -1e4, 0.0, 1e-30
+        clean = _run([x, *ops[1:]], dy, "silu")
+        want = _exact([x, *ops[1:]], dy, "silu")
+        for a, b in zip(clean[:2], want[:2]):  # row by row: their sizes differ by orders of magnitude
+            for r in (0, 3, 4, 5, 7):
+                assert _off(a[r], b[r]) < 2 * _bound(BF16) or b[r].norm() < 1e-25
+        x[3], x[4] = float("nan"), float("inf")
+        bad = _run([x, *ops[1:]], dy, "silu")
+        keep = torch.ones(rows, dtype=torch.bool)
+        keep[[3, 4]] = False
+        assert torch.equal(bad[0][keep], clean[0][keep]) and torch.equal(bad[1][keep], clean[1][keep])
+        assert bad[0][3].isnan().all()
+
+
+def test_same_bits_every_time():
+    ops, dy = _operands(2000, 256, 520, 264, BF16, True, seed=10)
+    first = _run(ops, dy, "silu")
+    for _ in range(3):
+        for a, b in zip(_run(ops, dy, "silu"), first):
+            assert torch.equal(a, b)
+
+
+def test_rows_behind_the_last_are_left_alone():
+    for rows in (5, 130):
+        ops, _ = _operands(rows, 64, 72, 80, BF16, True)
+        out = [torch.full((rows + 200, n), 7.0, dtype=BF16, device="cuda") for n in (80, 72, 144)]
+        a = gated._args(*ops, "silu", BF16)
+        a.y, a.act, a.pre = (t.data_ptr() for t in out)
+        _lib.launch(_lib.lib().mf_gated_mlp_fwd, ops[0].device, ctypes.byref(a))
+        assert torch.equal(out[0][:rows], mfb.gated_mlp(*ops))
+        assert all((t[rows:] == 7.0).all() for t in out)
+
+
+def test_other_stream():
+    ops, dy = _operands(500, 128, 264, 136, BF16, True, seed=11)
+    want = _run(ops, dy, "silu")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(2_000_000)
+        later = [t + 0 for t in ops]  # made on this stream, late
+        got = _run(later, dy, "silu")
+    torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [20, 300])
+def test_captured_passes(rows):
+    """Two graphs of forward and backward, replayed in turn on new data.  While an eager graph of the same leaves is alive the capture is refused."""
+    first, dy = _operands(rows, 64, 136, 72, BF16, True, seed=12)
+    second, _ = _operands(rows, 64, 136, 72, BF16, True, seed=13)
+    want = [_run(first, dy, "silu"), _run(second, dy, "silu")]
+    static = [t.clone().requires_grad_() for t in first]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            torch.autograd.grad(mfb.gated_mlp(*static), static, dy)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    alive = mfb.gated_mlp(*static)
+    for params in (static[1:], [t.detach().float() for t in static[1:]]):  # both host paths
+        with pytest.raises(RuntimeError, match="release that graph"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            y = mfb.gated_mlp(static[0], *params)
+            torch.autograd.grad(y, static[0], dy)
+    del alive, y
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = mfb.gated_mlp(*static)
+            outs.append([y.detach(), *torch.autograd.grad(y, static, dy)])
+        graphs.append(graph)
+    for values, expected in ((first, want[0]), (second, want[1]), (first, want[0])):
+        with torch.no_grad():
+            for t, v in zip(static, values):
+                t.copy_(v)
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            for a, b in zip(out, expected):
+                assert torch.equal(a, b)
+
+
+def test_two_host_threads():
+    """Calls of different sizes from two threads, each on a stream of its own."""
+    jobs = [_operands(rows, 64, F, 80, BF16, True, seed=20 + i) for i, (rows, F) in enumerate(((300, 72), (3000, 264)))]
+    want = [_run(*job, "silu") for job in jobs]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not all(torch.equal(a, b) for a, b in zip(_run(*jobs[i], "silu"), want[i])):
+                    failures.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
+
+def test_once_differentiable():
+    ops, dy = _operands(40, 64, 72, 80, BF16, True)
+    for x in (ops[0], ops[0].repeat(1, 2)[:, :64]):  # both host paths
+        x = x.detach().requires_grad_()
+        (g,) = torch.autograd.grad(mfb.gated_mlp(x, *ops[1:]), x, dy, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.float().sum().backward()
+
+
+def test_inputs_changed_in_place_are_noticed():
+    ops, dy = _operands(40, 64, 72, 80, BF16, True)
+    leaves = [t.detach().requires_grad_() for t in ops]
+    y = mfb.gated_mlp(*leaves)
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaves[0], dy)
+
+
+@pytest.mark.parametrize("backward,kind", [(b, k) for b in (0, 1) for k in range(4)])
+def test_expired_waits(backward, kind):
+    """Hand-offs of one kind withheld: every wait ends at its limit, the call reports it, and the next call is whole.  Sizes with more
+    blocks than stages and more tiles than accumulators for every pair of CTAs, so that each kind is waited for."""
+    ops, dy = _operands(20000, 512, 520, 520, BF16, False, seed=14)
+    want = _run(ops, dy, "silu")
+    rows, F = ops[0].shape[0], 520
+    a = gated._args(*ops, "silu", BF16)
+    made = [torch.empty(rows, n, dtype=BF16, device="cuda") for n in (2 * F, F, 520, 512)] + [torch.empty_like(t) for t in ops[1:3]]
+    a.pre, a.act, a.y, a.grad_x, a.grad_w_in, a.grad_w_out = (t.data_ptr() for t in made)
+    a.grad_y = dy.data_ptr()
+    _lib.launch(_lib.lib().mf_gated_mlp_fwd, dy.device, ctypes.byref(a))
+    need = _lib.lib().mf_gated_mlp_bwd_workspace_bytes(ctypes.byref(a))
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    status = ctypes.c_int32(0)
+    _lib.launch(_lib.lib().mf_selftest_gated_mlp_give_up, dy.device, ctypes.byref(a), backward, kind, 40000, ctypes.byref(status))
+    assert status.value == _lib.MF_ERR_DEVICE_TIMEOUT
+    assert mfb.gated_mlp_status() == 0
+    for g, b in zip(_run(ops, dy, "silu"), want):
+        assert torch.equal(g, b)
