@@ -682,9 +682,11 @@ int mf_rotary(const MfRotaryArgs* args, void* stream);
  * with w_in (2*hidden, dim), the gate's rows first, w_out (dim_out, hidden) and optional biases (NULL).  dtype is bf16 or fp16, of
  * every tensor but the gradients of the parameters, which come in grad_dtype (dtype or fp32).  Widths are multiples of 8; any
  * number of rows.
- * Forward: writes act (rows, hidden), y (rows, dim_out) and, where `pre` is given, the pre-activations (rows, 2*hidden).
+ * Forward: writes act (rows, hidden), y (rows, dim_out) and, where `pre` is given, the pre-activations: mf_gated_mlp_pre_bytes of a
+ * form that the backward call reads (16-bit values with an exponent for every 16 of them).
  * Backward: reads x, w_in, w_out, pre, act and grad_y; writes those of grad_x, grad_w_in, grad_w_out, grad_b_in, grad_b_out that are
- * not NULL.  Sums are in fp32 and in a fixed order; pre, act and the gradients of the pre-activations are rounded to dtype.
+ * not NULL.  Sums are in fp32 and in a fixed order; act and the gradients of the pre-activations are rounded to dtype, the
+ * pre-activations to three bits more.
  * Workspace (backward): mf_gated_mlp_bwd_workspace_bytes, for the same gradients.  An expired device-side wait is reported by
  * mf_gated_mlp_status (which synchronises `stream`); the outputs of such a call are undefined.
  */
@@ -712,6 +714,7 @@ typedef struct MfGatedMlpArgs {
   size_t workspace_bytes;
 } MfGatedMlpArgs;
 
+size_t mf_gated_mlp_pre_bytes(int64_t rows, int32_t hidden);
 size_t mf_gated_mlp_bwd_workspace_bytes(const MfGatedMlpArgs* args);
 int mf_gated_mlp_fwd(const MfGatedMlpArgs* args, void* stream);
 int mf_gated_mlp_bwd(const MfGatedMlpArgs* args, void* stream);

@@ -99,6 +99,7 @@ EXPORTED_SYMBOLS = (
     "mf_pair_head_fwd",
     "mf_pair_head_bwd",
     "mf_rotary",
+    "mf_gated_mlp_pre_bytes",
     "mf_gated_mlp_bwd_workspace_bytes",
     "mf_gated_mlp_fwd",
     "mf_gated_mlp_bwd",
@@ -462,6 +463,8 @@ def lib() -> ctypes.CDLL:
         fn.restype = c_int32
     L.mf_rotary.argtypes = [POINTER(MfRotaryArgs), c_void_p]
     L.mf_rotary.restype = c_int32
+    L.mf_gated_mlp_pre_bytes.argtypes = [c_int64, c_int32]
+    L.mf_gated_mlp_pre_bytes.restype = c_size_t
     L.mf_gated_mlp_bwd_workspace_bytes.argtypes = [POINTER(MfGatedMlpArgs)]
     L.mf_gated_mlp_bwd_workspace_bytes.restype = c_size_t
     for fn in (L.mf_gated_mlp_fwd, L.mf_gated_mlp_bwd):

@@ -3,8 +3,8 @@
 // Forward, two products: one forms g and u of 128 hidden channels side by side in tensor memory and stores h (in training g and u as
 // well), one multiplies h with Wo.  Backward, four: dh = dy Wo, whose epilogue turns dh into dg = dh u act'(g) and du = dh act(g)
 // where they stand (dh is never stored); dx = [dg du] [Wg; Wu]; and the weights' gradients [dg du]^T x and dy^T h.
-// h, g, u, dg, du are rounded to 16 bits on their way through memory: the tensor cores take no wider operands, and g and u in 32 bits
-// would double what the first product stores.  Every sum is in 32 bits.
+// h, dg and du are rounded to the block's type on their way through memory: the tensor cores take no wider operands.  g and u are kept
+// in 16 bits of a form of their own (gated_mlp.cuh), since 32 would double what the first product stores.  Every sum is in 32 bits.
 #include "common.cuh"
 #include "gemm_sm100.cuh"
 
@@ -163,6 +163,8 @@ Params common(long long m, long long n, long long k, const BoundedWaits& waits) 
     }                                                                                                          \
   } while (0)
 
+uint2* exponents_of(const MfGatedMlpArgs* a) { return reinterpret_cast<uint2*>(static_cast<char*>(a->pre) + gated_mlp_pre_values(a->rows, a->hidden)); }
+
 template <typename T>
 int forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t stream) {
   const long long M = a->rows, C = a->dim, F = a->hidden, O = a->dim_out;
@@ -174,6 +176,7 @@ int forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t str
   MF_MAP(map16<T>(&p.b2, w_in + F * C, F, C, C, 64));
   MF_MAP(map16<T>(&p.one.out, a->act, M, F, F, 32));
   if (a->pre) {
+    p.exponents = exponents_of(a);
     MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32));
     MF_MAP(map16<T>(&p.pre2, static_cast<T*>(a->pre) + F, M, F, 2 * F, 32));
   }
@@ -236,6 +239,7 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
   if (a->grad_x || a->grad_w_in || a->grad_b_in) {
     Params p = common(M, F, O, waits);
     p.column_sums = a->grad_b_in ? sums : nullptr;
+    p.exponents = exponents_of(a);
     MF_MAP(map16<T>(&p.one.a, a->grad_y, M, O, O, 64));
     MF_MAP(map16<T>(&p.one.b, a->w_out, O, F, F, 64));
     MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32));
@@ -303,6 +307,9 @@ int read_status(int32_t* host_status, cudaStream_t stream, bool clear) {
 
 using namespace mf;
 
+extern "C" size_t mf_gated_mlp_pre_bytes(int64_t rows, int32_t hidden) {
+  return rows < 0 || hidden < 1 ? 0 : gated_mlp_pre_values(rows, hidden) + (size_t)rows * ((hidden + 63) / 64) * 8;
+}
 extern "C" size_t mf_gated_mlp_bwd_workspace_bytes(const MfGatedMlpArgs* a) {
   if (!a || a->rows < 0 || a->hidden < 1 || a->dim < 1 || a->dim_out < 1) return 0;
   size_t at[4];

@@ -20,7 +20,8 @@ struct SmallParams {
   const void* w;     // (n, k); kGate: (2 n, k)
   const void* bias;  // (n) or (2 n), or null
   void* out;         // (rows, n)
-  void* pre;         // kGate: (rows, 2 n) or null
+  void* pre;         // kGate: pre-activations (rows, 2 n) or null
+  uint8_t* exponents;
   int rows, n, k;
   int activation;
 };
@@ -140,23 +141,37 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p)
   };
   const T* bias = static_cast<const T*>(p.bias);
   const bool biased = bias != nullptr;
-  // the CTAs of a cluster store every ranks-th token
+  // the CTAs of a cluster store every ranks-th token; sixteen lanes hold a token's channels
   for (int i = threadIdx.x; i < 16 * kTokens; i += kWarps * 32) {
     const int r = i & 15, c = i >> 4, n = n0 + r;
-    if (c >= p.rows || n >= p.n || c % ranks != rank) continue;
+    if (c >= p.rows || c % ranks != rank) continue;
     float a = total(r, c);
-    if (biased) a += to_f32(bias[n]);
+    if (biased && n < p.n) a += to_f32(bias[n]);
     if constexpr (kGate) {
       float u = total(16 + r, c);
-      if (biased) u += to_f32(bias[p.n + n]);
+      if (biased && n < p.n) u += to_f32(bias[p.n + n]);
       if (p.pre) {
-        T* pre = static_cast<T*>(p.pre) + (size_t)c * 2 * p.n + n;
-        pre[0] = from_f32<T>(a), pre[p.n] = from_f32<T>(u);
+        const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
+        float most_g = fabsf(a), most_u = fabsf(u);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+          most_g = fmaxf(most_g, __shfl_xor_sync(lanes, most_g, o));
+          most_u = fmaxf(most_u, __shfl_xor_sync(lanes, most_u, o));
+        }
+        const uint32_t eg = group_exponent<T>(most_g), eu = group_exponent<T>(most_u);
+        if (n < p.n) {
+          uint16_t* pre = static_cast<uint16_t*>(p.pre) + (size_t)c * 2 * p.n + n;
+          pre[0] = (uint16_t)pack_pre<T>(make_float2(a, 0.f), group_scale<T>(eg)), pre[p.n] = (uint16_t)pack_pre<T>(make_float2(u, 0.f), group_scale<T>(eu));
+        }
+        if (r == 0) {
+          uint8_t* to = p.exponents + ((size_t)(n0 >> 6) * p.rows + c) * 8 + ((n0 >> 4) & 3);
+          to[0] = (uint8_t)eg, to[4] = (uint8_t)eu;
+        }
       }
       const float2 f = p.activation == MF_ACT_SILU ? activation2<MF_ACT_SILU>(make_float2(a, a)) : activation2<MF_ACT_GELU_TANH>(make_float2(a, a));
       a = f.x * u;
     }
-    static_cast<T*>(p.out)[(size_t)c * p.n + n] = from_f32<T>(a);
+    if (n < p.n) static_cast<T*>(p.out)[(size_t)c * p.n + n] = from_f32<T>(a);
   }
   if (ranks > 1) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // the sums stay until all have read
 }
@@ -187,9 +202,10 @@ int launch_tokens(const SmallParams& p, cudaStream_t stream, const char* what) {
 template <typename T>
 int forward(const MfGatedMlpArgs* a, cudaStream_t stream) {
   const int rows = (int)a->rows;
-  const int rc = launch_tokens<T, true>({a->x, a->w_in, a->b_in, a->act, a->pre, rows, a->hidden, a->dim, a->activation}, stream, "gated_mlp gate product");
+  uint8_t* exponents = a->pre ? static_cast<uint8_t*>(a->pre) + gated_mlp_pre_values(rows, a->hidden) : nullptr;
+  const int rc = launch_tokens<T, true>({a->x, a->w_in, a->b_in, a->act, a->pre, exponents, rows, a->hidden, a->dim, a->activation}, stream, "gated_mlp gate product");
   if (rc != MF_OK) return rc;
-  return launch_tokens<T, false>({a->act, a->w_out, a->b_out, a->y, nullptr, rows, a->dim_out, a->hidden, 0}, stream, "gated_mlp output product");
+  return launch_tokens<T, false>({a->act, a->w_out, a->b_out, a->y, nullptr, nullptr, rows, a->dim_out, a->hidden, 0}, stream, "gated_mlp output product");
 }
 
 }  // namespace

@@ -64,6 +64,7 @@ struct Params {
   CUtensorMap out2;         // kGateGrad: gradients of up
   CUtensorMap pre, pre2;    // pre-activations of gate | up (kGate: written if keep_pre; kGateGrad: read); kWeight: pre = planes of partial sums
   const void* bias;         // kGate: (2 n), kStore: (n); may be null
+  uint2* exponents;         // of the pre-activations: (ceil(n / 64), m)
   float* column_sums;       // kGateGrad: (ceil(m / 32), 2 n) sums of the stored rows, or null
   int k;
   int whole, cut, tiles;    // tiles of full width, columns of a later one = full width / cut, pieces of work in all
@@ -453,6 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         if (chunks) {  // 64 columns of gate and of up
           // the hidden values go to a buffer as they are formed; the words of gate and up wait in registers for theirs
           uint32_t words[2][32], g[2][16], u[2][16];
+          uint2 exponents = make_uint2(0u, 0u);
           const uint32_t hidden = next_buffer();
           tmem_ld16(acc + first, g[0]);
           tmem_ld16(acc + w.cols + first, u[0]);
@@ -471,6 +473,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             } else {
               drained();
             }
+            uint32_t(&gv)[16] = g[c & 1], (&uv)[16] = u[c & 1];
+            float most_g = 0.f, most_u = 0.f;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
               const uint32_t bgw[4] = {bg[v].x, bg[v].y, bg[v].z, bg[v].w}, buw[4] = {bu[v].x, bu[v].y, bu[v].z, bu[v].w};
@@ -478,14 +482,24 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int i = 8 * v + 2 * e;
-                const float2 gate = add2(make_float2(__uint_as_float(g[c & 1][i]), __uint_as_float(g[c & 1][i + 1])), unpack2<T>(bgw[e]));
-                const float2 up = add2(make_float2(__uint_as_float(u[c & 1][i]), __uint_as_float(u[c & 1][i + 1])), unpack2<T>(buw[e]));
+                const float2 gate = add2(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])), unpack2<T>(bgw[e]));
+                const float2 up = add2(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])), unpack2<T>(buw[e]));
                 const float2 h = mul2(activation2<kAct>(gate), up);
-                const int at = 8 * c + 4 * v + e;
                 hw[e] = pack2<T>(h.x, h.y);
-                words[0][at] = pack2<T>(gate.x, gate.y), words[1][at] = pack2<T>(up.x, up.y);
+                gv[i] = __float_as_uint(gate.x), gv[i + 1] = __float_as_uint(gate.y), uv[i] = __float_as_uint(up.x), uv[i + 1] = __float_as_uint(up.y);
+                most_g = fmaxf(most_g, fmaxf(fabsf(gate.x), fabsf(gate.y))), most_u = fmaxf(most_u, fmaxf(fabsf(up.x), fabsf(up.y)));
               }
               sts128(hidden + box_chunk(lane, 2 * c + v), make_uint4(hw[0], hw[1], hw[2], hw[3]));
+            }
+            if (p.keep_pre) {
+              const uint32_t eg = group_exponent<T>(most_g), eu = group_exponent<T>(most_u);
+              const float2 sg = group_scale<T>(eg), su = group_scale<T>(eu);
+              exponents.x |= eg << (8 * c), exponents.y |= eu << (8 * c);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                words[0][8 * c + i / 2] = pack_pre<T>(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])), sg);
+                words[1][8 * c + i / 2] = pack_pre<T>(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])), su);
+              }
             }
           }
           fence_smem_to_async_proxy();
@@ -494,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           if (stores) store_box(&p.one.out, hidden, col0, row0);
           if (lane == 0) store_commit();
           if (p.keep_pre) {
+            if (row0 + lane < p.one.m && col0 < p.one.n) p.exponents[(size_t)(col0 >> 6) * p.one.m + row0 + lane] = exponents;
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
               const uint32_t dst = next_buffer();
@@ -516,6 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
           uint32_t d[2][16];
           tmem_ld16(acc + first + 64 * c, d[0]);
+          uint2 exponents = make_uint2(0x0f0f0f0fu, 0x0f0f0f0fu);
+          if (row0 + lane < p.one.m && col0 + 64 * c < p.one.n) exponents = p.exponents[(size_t)((col0 + 64 * c) >> 6) * p.one.m + row0 + lane];
           if (!mbar_wait_for(&bar_in[2 * ew + (chunk & 1)], (chunk >> 1) & 1, p.waits.limit)) bad = true;
           bad = __any_sync(0xffffffffu, bad);
           if (bad) break;
@@ -528,6 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             tmem_ld_wait();
             if (q < 3) tmem_ld16(acc + first + 64 * c + 16 * (q + 1), d[(q + 1) & 1]);
             else if (last) drained();
+            const float2 fg = group_unscale<T>(exponents.x >> (8 * q) & 255u), fu = group_unscale<T>(exponents.y >> (8 * q) & 255u);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
               const uint32_t gs[4] = {gw[v].x, gw[v].y, gw[v].z, gw[v].w}, us[4] = {uw[v].x, uw[v].y, uw[v].z, uw[v].w};
@@ -536,8 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               for (int e = 0; e < 4; ++e) {
                 const float2 grad = make_float2(__uint_as_float(d[q & 1][8 * v + 2 * e]), __uint_as_float(d[q & 1][8 * v + 2 * e + 1]));
                 float2 value, slope;
-                activation2<kAct>(unpack2<T>(gs[e]), value, slope);
-                const float2 a = mul2(mul2(grad, unpack2<T>(us[e])), slope), b = mul2(grad, value);
+                activation2<kAct>(unpack_pre<T>(gs[e], fg), value, slope);
+                const float2 a = mul2(mul2(grad, unpack_pre<T>(us[e], fu)), slope), b = mul2(grad, value);
                 dg[e] = pack2<T>(a.x, a.y), du[e] = pack2<T>(b.x, b.y);
               }
               sts128(gate + box_chunk(lane, 2 * q + v), make_uint4(dg[0], dg[1], dg[2], dg[3]));

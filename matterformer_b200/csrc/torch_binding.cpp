@@ -377,7 +377,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = a.dim_out;
     const Tensor y = at::empty(shape, x.options()), act = at::empty({a.rows, a.hidden}, x.options());
-    const Tensor pre = keep ? at::empty({a.rows, 2 * (int64_t)a.hidden}, x.options()) : Tensor();
+    const Tensor pre = keep ? at::empty({(int64_t)mf_gated_mlp_pre_bytes(a.rows, a.hidden)}, x.options().dtype(at::kByte)) : Tensor();
     a.y = y.data_ptr(), a.act = act.data_ptr(), a.pre = keep ? pre.data_ptr() : nullptr;
     check(mf_gated_mlp_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
     if (keep) {

@@ -52,7 +52,7 @@ class _GatedMlp(torch.autograd.Function):
         y = torch.empty((rows, w_out.shape[0]), device=x.device, dtype=x.dtype)
         act = torch.empty((rows, F), device=x.device, dtype=x.dtype)
         keep = any(ctx.needs_input_grad)
-        pre = torch.empty((rows, 2 * F), device=x.device, dtype=x.dtype) if keep else None
+        pre = torch.empty(_lib.lib().mf_gated_mlp_pre_bytes(rows, F), device=x.device, dtype=torch.uint8) if keep else None
         a = _args(x2, *params, activation, ctx.grad_dtype)
         a.pre, a.act, a.y = _ptr(pre), _ptr(act), _ptr(y)
         _lib.launch(_lib.lib().mf_gated_mlp_fwd, x.device, ctypes.byref(a))
@@ -129,8 +129,9 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     ``x``'s type, or fp32 beside a bf16 ``x`` (their bf16 copies compute, their gradients are fp32; see
     :func:`matterformer_b200.linear.bf16_copies`).  ``activation``: "silu" or "gelu_tanh".  Returns (..., O) in ``x``'s type.
 
-    Sums are in fp32 in a fixed order.  The hidden values, and for the backward pass the pre-activations and their gradients, are
-    rounded to ``x``'s type.  C, F and O are multiples of 8.  The gradient is once differentiable."""
+    Sums are in fp32 in a fixed order.  The hidden values and the gradients of the pre-activations are rounded to ``x``'s type, what the
+    backward pass gets of the pre-activations to some bits more; hidden values that
+    fp16 cannot hold (above 65504) are infinities there.  C, F and O are multiples of 8.  The gradient is once differentiable."""
     native = _lib.native()
     if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++
         out = native.gated_mlp(x, w_in, w_out, b_in, b_out, ACTIVATIONS[activation])

@@ -176,12 +176,14 @@ def test_same_bits_every_time():
 def test_rows_behind_the_last_are_left_alone():
     for rows in (5, 130):
         ops, _ = _operands(rows, 64, 72, 80, BF16, True)
-        out = [torch.full((rows + 200, n), 7.0, dtype=BF16, device="cuda") for n in (80, 72, 144)]
+        out = [torch.full((rows + 200, n), 7.0, dtype=BF16, device="cuda") for n in (80, 72)]
+        size = _lib.lib().mf_gated_mlp_pre_bytes(rows, 72)
+        pre = torch.full((size + 5000,), 77, dtype=torch.uint8, device="cuda")
         a = gated._args(*ops, "silu", BF16)
-        a.y, a.act, a.pre = (t.data_ptr() for t in out)
+        a.y, a.act, a.pre = (t.data_ptr() for t in (*out, pre))
         _lib.launch(_lib.lib().mf_gated_mlp_fwd, ops[0].device, ctypes.byref(a))
         assert torch.equal(out[0][:rows], mfb.gated_mlp(*ops))
-        assert all((t[rows:] == 7.0).all() for t in out)
+        assert all((t[rows:] == 7.0).all() for t in out) and (pre[size:] == 77).all()
 
 
 def test_other_stream():
@@ -283,7 +285,8 @@ def test_expired_waits(backward, kind):
     want = _run(ops, dy, "silu")
     rows, F = ops[0].shape[0], 520
     a = gated._args(*ops, "silu", BF16)
-    made = [torch.empty(rows, n, dtype=BF16, device="cuda") for n in (2 * F, F, 520, 512)] + [torch.empty_like(t) for t in ops[1:3]]
+    made = [torch.empty(_lib.lib().mf_gated_mlp_pre_bytes(rows, F), dtype=torch.uint8, device="cuda")]
+    made += [torch.empty(rows, n, dtype=BF16, device="cuda") for n in (F, 520, 512)] + [torch.empty_like(t) for t in ops[1:3]]
     a.pre, a.act, a.y, a.grad_x, a.grad_w_in, a.grad_w_out = (t.data_ptr() for t in made)
     a.grad_y = dy.data_ptr()
     _lib.launch(_lib.lib().mf_gated_mlp_fwd, dy.device, ctypes.byref(a))
@@ -296,3 +299,23 @@ def test_expired_waits(backward, kind):
     assert mfb.gated_mlp_status() == 0
     for g, b in zip(_run(ops, dy, "silu"), want):
         assert torch.equal(g, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows", [20, 300])
+def test_pre_activations_of_different_sizes(rows, dtype):
+    """Tokens and channels whose pre-activations span many orders: each token's gradients against its own size.  The kept form goes by
+    the largest of 16 channels, so a channel a thousand times smaller than its neighbour still has what the block's type gives it.
+
+    Hidden values are products of two pre-activations and have to lie in the block's type: fp16 ends at 65504, so its factors stop at 2 and 8
+    (pre-activations to 16 * 5 standard deviations, products to 6400), where bf16 takes 16 and 32."""
+    g = torch.Generator().manual_seed(30)
+    ops, dy = _operands(rows, 64, 80, 72, dtype, False, seed=31)
+    ops[0] *= (2.0 ** torch.randint(-12, 5 if dtype == BF16 else 2, (rows, 1), generator=g)).to(dtype).cuda()
+    ops[1] *= (2.0 ** torch.randint(-5, 6 if dtype == BF16 else 4, (160, 1), generator=g)).to(dtype).cuda()
+    got, want = _run(ops, dy, "silu"), _exact(ops, dy, "silu")
+    tiny = torch.finfo(dtype).tiny * 64  # fp16 has no more bits there
+    for a, b in zip(got, want):
+        size = b.norm(dim=1, keepdim=True) / b.shape[1] ** 0.5
+        off = (a.double() - b).norm(dim=1) / (size.squeeze(1) * b.shape[1] ** 0.5).clamp_min(1e-300)
+        assert (off[size.squeeze(1) > tiny] < 2 * _bound(dtype)).all()
