@@ -16,11 +16,11 @@ using namespace gemm;
 constexpr int kPairs = 74;  // clusters of two CTAs on 148 SMs
 const char* const kName = "mf_gated_mlp";
 
-// 2-D map of a row-major matrix of 16-bit elements, boxes of 64 columns.
+// 2-D map of a row-major matrix of 16-bit elements.
 template <typename T>
-bool map16(CUtensorMap* map, const void* base, long long rows, long long cols, long long row_stride, int box_rows) {
+bool map16(CUtensorMap* map, const void* base, long long rows, long long cols, long long row_stride, int box_rows, int box_cols = 64) {
   const long long dims[2] = {cols, rows}, strides[1] = {row_stride * 2};
-  return make_tensor_map(map, base, std::is_same<T, __nv_bfloat16>::value ? MF_DTYPE_BF16 : MF_DTYPE_F16, 2, dims, strides, 64, box_rows);
+  return make_tensor_map(map, base, std::is_same<T, __nv_bfloat16>::value ? MF_DTYPE_BF16 : MF_DTYPE_F16, 2, dims, strides, box_cols, box_rows);
 }
 
 template <typename T, bool kAMn, bool kBMn, Epilogue kEpi, int kAct>
@@ -47,8 +47,8 @@ int tiles_of(long long rows, long long cols, int width) { return (int)(((rows + 
 // cut into tiles of half (a quarter of) the width.  29 696 x 512 over 2048: 232 tiles are 3.1 rounds.
 template <typename T, bool kAMn, bool kBMn, Epilogue kEpi>
 int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
-  const int tiles = tiles_of(p.one.m, p.one.n, kEpi == kGate ? kTile / 2 : kTile), rest = tiles % kPairs;
-  p.cut = rest == 0 || 2 * rest > kPairs ? 1 : kEpi == kGate || 4 * rest > kPairs ? 2 : 4;
+  const int tiles = tiles_of(p.one.m, p.one.n, projects(kEpi) ? kTile / 2 : kTile), rest = tiles % kPairs;
+  p.cut = rest == 0 || 2 * rest > kPairs ? 1 : projects(kEpi) || 4 * rest > kPairs ? 2 : 4;
   p.whole = p.cut == 1 ? tiles : tiles - rest;
   p.tiles = p.whole + (tiles - p.whole) * p.cut;
   const int pairs = p.tiles < kPairs ? p.tiles : kPairs;
@@ -170,17 +170,18 @@ int forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t str
   const long long M = a->rows, C = a->dim, F = a->hidden, O = a->dim_out;
   const T* w_in = static_cast<const T*>(a->w_in);
   Params p = common(M, F, C, waits);
-  p.bias = a->b_in, p.keep_pre = a->pre != nullptr;
+  p.bias = a->b_in;
   MF_MAP(map16<T>(&p.one.a, a->x, M, C, C, 64));
   MF_MAP(map16<T>(&p.one.b, w_in, F, C, C, 64));
   MF_MAP(map16<T>(&p.b2, w_in + F * C, F, C, C, 64));
   MF_MAP(map16<T>(&p.one.out, a->act, M, F, F, 32));
   if (a->pre) {
     p.exponents = exponents_of(a);
-    MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32));
-    MF_MAP(map16<T>(&p.pre2, static_cast<T*>(a->pre) + F, M, F, 2 * F, 32));
+    MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32, 32));
+    MF_MAP(map16<T>(&p.pre2, static_cast<T*>(a->pre) + F, M, F, 2 * F, 32, 32));
   }
-  int rc = launch<T, false, false, kGate>(p, a->activation, stream, "gated_mlp gate product");
+  int rc = a->pre ? launch<T, false, false, kGateKeep>(p, a->activation, stream, "gated_mlp gate product")
+                  : launch<T, false, false, kGate>(p, a->activation, stream, "gated_mlp gate product");
   if (rc != MF_OK) return rc;
   p = common(M, O, F, waits);
   p.bias = a->b_out;

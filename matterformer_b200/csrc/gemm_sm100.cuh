@@ -29,9 +29,10 @@ namespace gemm {
 
 __device__ int32_t g_gemm_status = 0;  // MF_ERR_DEVICE_TIMEOUT after an expired wait
 
-// kGate: two projections, activation and product;  kGateGrad: its gradient;  kStore: the product and a bias;  kWeight: one or two
+// kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well;  kGateGrad: its gradient;  kStore: the product and a bias;  kWeight: one or two
 // products over the same long dimension, which is cut into pieces for the tiles behind the last whole round
-enum Epilogue { kGate, kGateGrad, kStore, kWeight };
+enum Epilogue { kGate, kGateKeep, kGateGrad, kStore, kWeight };
+__host__ __device__ constexpr bool projects(Epilogue e) { return e == kGate || e == kGateKeep; }
 
 constexpr int kBlockK = 64;                       // elements of the contracted dimension in a stage
 constexpr int kBoxBytes = 64 * 128;               // 64 lines of 64 16-bit elements
@@ -44,9 +45,11 @@ constexpr int kTmemCols = 512;
 
 template <Epilogue kEpi>
 struct Shape {
-  static constexpr int kBuffers = kEpi == kGateGrad ? 4 : 2;  // of 4 KB for each storing warp
+  // Buffers of 4 KB for each storing warp, stages in what they leave.  Six stages instead of five: 8192 x 2048 x 4096 2 %, the
+  // projections of 8192 x 5504 over 2048 4 %.
+  static constexpr int kBuffers = kEpi == kGateGrad ? 4 : kEpi == kGateKeep ? 2 : 1;
   static constexpr int kBufferBytes = kEpilogueWarps * kBuffers * kStageBuffer;
-  static constexpr int kStages = kEpi == kGateGrad ? 3 : 5;
+  static constexpr int kStages = kEpi == kGateGrad ? 3 : kEpi == kGateKeep ? 5 : 6;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kBufferBytes;
   static_assert(kSmem + 1024 <= 232448, "shared memory");
 };
@@ -62,7 +65,7 @@ struct Params {
   Problem two;              // kWeight: the second product
   CUtensorMap b2;           // kGate: the rows of the up projection, the odd CTA's
   CUtensorMap out2;         // kGateGrad: gradients of up
-  CUtensorMap pre, pre2;    // pre-activations of gate | up (kGate: written if keep_pre; kGateGrad: read); kWeight: pre = planes of partial sums
+  CUtensorMap pre, pre2;    // pre-activations of gate | up (kGateKeep: written, boxes of 32 columns; kGateGrad: read); kWeight: pre = planes of partial sums
   const void* bias;         // kGate: (2 n), kStore: (n); may be null
   uint2* exponents;         // of the pre-activations: (ceil(n / 64), m)
   float* column_sums;       // kGateGrad: (ceil(m / 32), 2 n) sums of the stored rows, or null
@@ -71,7 +74,6 @@ struct Params {
   int first2;               // kWeight: the second product's first tile
   int first, first_rest;    // kWeight: the first tile, and the first that is cut along the contracted dimension
   int rest, per;            // kWeight: how many are cut, and how many blocks a piece has
-  int keep_pre;
   int wide_out;             // kWeight: fp32 results
   BoundedWaits waits;       // kinds: 0 operands, 1 stages, 2 accumulators, 3 drained accumulators
 };
@@ -179,39 +181,43 @@ __device__ __forceinline__ uint4 bias8(const T* bias, int c, int n) {
 // Where 16 bytes `chunk` of line `row` of a box lie.
 __device__ __forceinline__ uint32_t box_chunk(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
-// Column sums of a warp's buffer of 32 lines: 1 x 32 ones times the lines, on mma.sync; lane l returns columns 2 l and 2 l + 1.  As
-// loads and additions they were a fifth of the instructions around the product.
+// The same in a box of 32 columns, lines of 64 bytes (64-byte swizzle).
+__device__ __forceinline__ uint32_t half_box_chunk(int row, int chunk) { return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); }
+
+// Column sums of a warp's buffer of 32 lines on mma.sync: the lines' transpose, 16 columns at a time, times ones.  Lane 4 i + j returns
+// columns 16 j + i and 16 j + i + 8.  (As loads and additions they were a fifth of the instructions around the product.)
 template <typename T>
 __device__ __forceinline__ float2 column_sums32(uint32_t buffer, int lane) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   const uint32_t one = kBf16 ? 0x3f803f80u : 0x3c003c00u;
-  float2 sum = make_float2(0.f, 0.f);
+  uint32_t a[4][2][4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {  // 16 columns
-    float d[2][4] = {};
+  for (int c = 0; c < 4; ++c)  // 16 columns
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {  // 16 lines
-      uint32_t b[4];
-      const uint32_t at = buffer + box_chunk(16 * k + (lane & 15), 2 * c + (lane >> 4));
+    for (int k = 0; k < 2; ++k) {  // 16 lines; the four 8 x 8 parts: columns 0-7 | 8-15 of lines 0-7, then of lines 8-15
+      const uint32_t at = buffer + box_chunk(16 * k + (lane & 7) + 8 * (lane >> 4), 2 * c + (lane >> 3 & 1));
       asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3])
+                   : "=r"(a[c][k][0]), "=r"(a[c][k][1]), "=r"(a[c][k][2]), "=r"(a[c][k][3])
                    : "r"(at)
                    : "memory");
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if constexpr (kBf16)
-          asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %4, %4, %4}, {%5, %6}, {%0, %1, %2, %3};"
-              : "+f"(d[t][0]), "+f"(d[t][1]), "+f"(d[t][2]), "+f"(d[t][3])
-              : "r"(one), "r"(b[2 * t]), "r"(b[2 * t + 1]));
-        else
-          asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %4, %4, %4}, {%5, %6}, {%0, %1, %2, %3};"
-              : "+f"(d[t][0]), "+f"(d[t][1]), "+f"(d[t][2]), "+f"(d[t][3])
-              : "r"(one), "r"(b[2 * t]), "r"(b[2 * t + 1]));
-      }
     }
+  float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)  // every line of the result is the same: lanes 4 i .. 4 i + 3 keep the eight columns i
-      if ((lane >> 2) == 2 * c + t) sum = make_float2(d[t][0], d[t][1]);
+  for (int c = 0; c < 4; ++c) {
+    float d[4] = {};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t(&m)[4] = a[c][k];
+      if constexpr (kBf16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3]), "r"(one));
+      else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %8}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3]), "r"(one));
+    }
+    if ((lane & 3) == c) sum = make_float2(d[0], d[2]);  // (all columns of the result are the same)
   }
   return sum;
 }
@@ -242,7 +248,7 @@ struct Walk {
     tiles_m = (p.one.m + kTile - 1) / kTile;
     tiles_n = (p.one.n + full() - 1) / full();
   }
-  __device__ static constexpr int full() { return kEpi == kGate ? kTile / 2 : kTile; }
+  __device__ static constexpr int full() { return projects(kEpi) ? kTile / 2 : kTile; }
   __device__ bool next(Work& w) {
     if (t >= p.tiles) return false;
     const bool whole = t < p.whole;
@@ -315,10 +321,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       uint32_t it = 0;
       while (!bad && walk.next(w)) {
         const CUtensorMap* amap = kEpi == kWeight && w.second ? &p.two.a : &p.one.a;
-        const CUtensorMap* bmap = kEpi == kWeight && w.second ? &p.two.b : kEpi == kGate && rank ? &p.b2 : &p.one.b;
+        const CUtensorMap* bmap = kEpi == kWeight && w.second ? &p.two.b : projects(kEpi) && rank ? &p.b2 : &p.one.b;
         const int row = w.row + 128 * (int)rank;
-        const int col = kEpi == kGate ? w.col : w.col + w.cols / 2 * (int)rank;
-        const bool two = (kEpi == kGate ? w.cols : w.cols / 2) > 64;  // boxes of B (a tile of 64 columns uses half of its box)
+        const int col = projects(kEpi) ? w.col : w.col + w.cols / 2 * (int)rank;
+        const bool two = (projects(kEpi) ? w.cols : w.cols / 2) > 64;  // boxes of B (a tile of 64 columns uses half of its box)
         for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int s = it % kStages;
           if (it >= kStages && !mbar_wait_for(&bar_empty[s], ((it / kStages) & 1) ^ 1, p.waits.limit)) {
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           break;
         }
         tc_fence_after_sync();
-        const uint32_t idesc = instruction<T, kAMn, kBMn>() | ((uint32_t)((kEpi == kGate ? 2 * w.cols : w.cols) >> 3) << 17);
+        const uint32_t idesc = instruction<T, kAMn, kBMn>() | ((uint32_t)((projects(kEpi) ? 2 * w.cols : w.cols) >> 3) << 17);
         for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int s = it % kStages;
           if (!mbar_wait_for(&bar_full[s], (it / kStages) & 1, p.waits.limit)) {
@@ -397,10 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       fence_smem_to_async_proxy();
       __syncwarp();
     };
-    auto next_buffer = [&]() {  // of two in turn, once its previous contents have left
-      if (lane == 0) store_wait_read<1>();
+    auto emptied = [&]() {  // what this warp has handed over has left its buffers
+      if (lane == 0) store_wait_read<0>();
       __syncwarp();
-      return buffers + (chunk++ & 1) * kStageBuffer;
     };
     // Columns of a tile that this warp stores: half of them, all of them or none where they are a single chunk.
     auto mine = [&](const Work& x, int& first) {
@@ -424,6 +429,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       int first;
       if (lane == 0 && more && mine(later, first)) fetch(later.col + first, later.row + lane_row);
     }
+    uint2 exponents_next = make_uint2(0u, 0u);  // kGateGrad: of the chunk after this one
+    auto exponents_at = [&](int col, int row) {
+      uint2 v = make_uint2(0x0f0f0f0fu, 0x0f0f0f0fu);
+      if (row < p.one.m && col < p.one.n) v = p.exponents[(size_t)(col >> 6) * p.one.m + row];
+      return v;
+    };
+    if constexpr (kEpi == kGateGrad) {
+      int first;
+      if (more && mine(later, first)) exponents_next = exponents_at(later.col + first, later.row + lane_row + lane);
+    }
 
     for (int n = 0; more; ++n) {
       w = later;
@@ -435,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       const T* bias = static_cast<const T*>(p.bias);
       const int bias_n = bias ? p.one.n : 0;
       uint4 bias_gate[2], bias_up[2];
-      if constexpr (kEpi == kGate) {
+      if constexpr (projects(kEpi)) {
 #pragma unroll
         for (int v = 0; v < 2; ++v) bias_gate[v] = bias8(bias, col0 + 8 * v, bias_n), bias_up[v] = bias8(bias + bias_n, col0 + 8 * v, bias_n);
       }
@@ -450,12 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       };
       if (chunks == 0) drained();
 
-      if constexpr (kEpi == kGate) {
-        if (chunks) {  // 64 columns of gate and of up
-          // the hidden values go to a buffer as they are formed; the words of gate and up wait in registers for theirs
-          uint32_t words[2][32], g[2][16], u[2][16];
+      if constexpr (projects(kEpi)) {
+        if (chunks) {  // 64 columns of gate and of up: hidden values in one buffer, the pre-activations of 32 columns at a time in the halves of the other
+          uint32_t g[2][16], u[2][16];
           uint2 exponents = make_uint2(0u, 0u);
-          const uint32_t hidden = next_buffer();
+          const uint32_t keep = buffers + kStageBuffer;
+          const bool stores = lane == 0 && row0 < p.one.m && col0 < p.one.n;
           tmem_ld16(acc + first, g[0]);
           tmem_ld16(acc + w.cols + first, u[0]);
 #pragma unroll
@@ -473,66 +488,77 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             } else {
               drained();
             }
-            uint32_t(&gv)[16] = g[c & 1], (&uv)[16] = u[c & 1];
+            uint32_t(&gv)[16] = g[c & 1], (&uv)[16] = u[c & 1], hw[8];
             float most_g = 0.f, most_u = 0.f;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
               const uint32_t bgw[4] = {bg[v].x, bg[v].y, bg[v].z, bg[v].w}, buw[4] = {bu[v].x, bu[v].y, bu[v].z, bu[v].w};
-              uint32_t hw[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int i = 8 * v + 2 * e;
                 const float2 gate = add2(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])), unpack2<T>(bgw[e]));
                 const float2 up = add2(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])), unpack2<T>(buw[e]));
                 const float2 h = mul2(activation2<kAct>(gate), up);
-                hw[e] = pack2<T>(h.x, h.y);
-                gv[i] = __float_as_uint(gate.x), gv[i + 1] = __float_as_uint(gate.y), uv[i] = __float_as_uint(up.x), uv[i + 1] = __float_as_uint(up.y);
-                most_g = fmaxf(most_g, fmaxf(fabsf(gate.x), fabsf(gate.y))), most_u = fmaxf(most_u, fmaxf(fabsf(up.x), fabsf(up.y)));
+                hw[4 * v + e] = pack2<T>(h.x, h.y);
+                if constexpr (kEpi == kGateKeep) {
+                  gv[i] = __float_as_uint(gate.x), gv[i + 1] = __float_as_uint(gate.y), uv[i] = __float_as_uint(up.x), uv[i + 1] = __float_as_uint(up.y);
+                  most_g = fmaxf(most_g, fmaxf(fabsf(gate.x), fabsf(gate.y))), most_u = fmaxf(most_u, fmaxf(fabsf(up.x), fabsf(up.y)));
+                }
               }
-              sts128(hidden + box_chunk(lane, 2 * c + v), make_uint4(hw[0], hw[1], hw[2], hw[3]));
             }
-            if (p.keep_pre) {
+            if (c == 0 || (kEpi == kGateKeep && c == 2)) emptied();  // (asked for after the arithmetic: it has had that long)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) sts128(buffers + box_chunk(lane, 2 * c + v), make_uint4(hw[4 * v], hw[4 * v + 1], hw[4 * v + 2], hw[4 * v + 3]));
+            if constexpr (kEpi == kGateKeep) {
               const uint32_t eg = group_exponent<T>(most_g), eu = group_exponent<T>(most_u);
               const float2 sg = group_scale<T>(eg), su = group_scale<T>(eu);
               exponents.x |= eg << (8 * c), exponents.y |= eu << (8 * c);
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                words[0][8 * c + i / 2] = pack_pre<T>(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])), sg);
-                words[1][8 * c + i / 2] = pack_pre<T>(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])), su);
+              for (int v = 0; v < 2; ++v) {
+                uint32_t gw[4], uw[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int i = 8 * v + 2 * e;
+                  gw[e] = pack_pre<T>(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])), sg);
+                  uw[e] = pack_pre<T>(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])), su);
+                }
+                const uint32_t at = keep + half_box_chunk(lane, 2 * (c & 1) + v);
+                sts128(at, make_uint4(gw[0], gw[1], gw[2], gw[3]));
+                sts128(at + kStageBuffer / 2, make_uint4(uw[0], uw[1], uw[2], uw[3]));
+              }
+            }
+            if (c == 3 || (kEpi == kGateKeep && c == 1)) {
+              fence_smem_to_async_proxy();
+              __syncwarp();
+              if (stores) {
+                if (c == 3) store_box(&p.one.out, buffers, col0, row0);
+                if (kEpi == kGateKeep && col0 + 16 * (c - 1) < p.one.n) {
+                  store_box(&p.pre, keep, col0 + 16 * (c - 1), row0);
+                  store_box(&p.pre2, keep + kStageBuffer / 2, col0 + 16 * (c - 1), row0);
+                }
+                store_commit();
               }
             }
           }
-          fence_smem_to_async_proxy();
-          __syncwarp();
-          const bool stores = lane == 0 && row0 < p.one.m && col0 < p.one.n;
-          if (stores) store_box(&p.one.out, hidden, col0, row0);
-          if (lane == 0) store_commit();
-          if (p.keep_pre) {
-            if (row0 + lane < p.one.m && col0 < p.one.n) p.exponents[(size_t)(col0 >> 6) * p.one.m + row0 + lane] = exponents;
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-              const uint32_t dst = next_buffer();
-              put(dst, words[side]);
-              if (stores) store_box(side ? &p.pre2 : &p.pre, dst, col0, row0);
-              if (lane == 0) store_commit();
-            }
-          }
+          if (kEpi == kGateKeep && row0 + lane < p.one.m && col0 < p.one.n) p.exponents[(size_t)(col0 >> 6) * p.one.m + row0 + lane] = exponents;
         }
       } else if constexpr (kEpi == kGateGrad) {
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c, ++chunk) {
           // the next chunk's pre-activations, once the buffers' previous results have left
           const bool last = c == chunks - 1;
-          int f;
-          if (lane == 0 && (!last || (more && mine(later, f)))) {
-            store_wait_read<0>();
-            if (!last) fetch(col0 + 64 * (c + 1), row0);
-            else fetch(later.col + f, later.row + lane_row);
+          int f = 0;
+          const uint2 exponents = exponents_next;
+          if (!last || (more && mine(later, f))) {
+            const int next_col = last ? later.col + f : col0 + 64 * (c + 1), next_row = last ? later.row + lane_row : row0;
+            exponents_next = exponents_at(next_col, next_row + lane);
+            if (lane == 0) {
+              store_wait_read<0>();
+              fetch(next_col, next_row);
+            }
           }
           uint32_t d[2][16];
           tmem_ld16(acc + first + 64 * c, d[0]);
-          uint2 exponents = make_uint2(0x0f0f0f0fu, 0x0f0f0f0fu);
-          if (row0 + lane < p.one.m && col0 + 64 * c < p.one.n) exponents = p.exponents[(size_t)((col0 + 64 * c) >> 6) * p.one.m + row0 + lane];
           if (!mbar_wait_for(&bar_in[2 * ew + (chunk & 1)], (chunk >> 1) & 1, p.waits.limit)) bad = true;
           bad = __any_sync(0xffffffffu, bad);
           if (bad) break;
@@ -572,11 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
           if (p.column_sums && row0 < p.one.m) {  // of the values as stored (rows beyond the last are zeros)
             const float2 dg = column_sums32<T>(gate, lane), du = column_sums32<T>(up, lane);
-            if (col + 2 * lane < p.one.n) {
-              float* to = p.column_sums + (size_t)(row0 >> 5) * (2 * (size_t)p.one.n) + col + 2 * lane;
-              *reinterpret_cast<float2*>(to) = dg;
-              *reinterpret_cast<float2*>(to + p.one.n) = du;
-            }
+            const int at = col + 16 * (lane & 3) + (lane >> 2);
+            float* to = p.column_sums + (size_t)(row0 >> 5) * (2 * (size_t)p.one.n) + at;
+            if (at < p.one.n) to[0] = dg.x, to[p.one.n] = du.x;
+            if (at + 8 < p.one.n) to[8] = dg.y, to[p.one.n + 8] = du.y;
             __syncwarp();
           }
         }
@@ -590,13 +615,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             tmem_ld32(acc + first + 32 * c, d);
             tmem_ld_wait();
             if (c == 2 * chunks - 1) drained();
-            const uint32_t dst = next_buffer();
-            put(dst, d);
+            emptied();
+            put(buffers, d);
             if (lane == 0 && row0 < prob.m && col0 + 32 * c < prob.n) {
-              if (w.plane >= 0) store_box(&p.pre, dst, first + 32 * c, w.plane * kTile + lane_row);
-              else store_box(&prob.out, dst, col0 + 32 * c, row0);
+              if (w.plane >= 0) store_box(&p.pre, buffers, first + 32 * c, w.plane * kTile + lane_row);
+              else store_box(&prob.out, buffers, col0 + 32 * c, row0);
+              store_commit();
             }
-            if (lane == 0) store_commit();  // (a group for every buffer, stored or not: next_buffer counts them)
           }
         } else {
 #pragma unroll 1
@@ -621,10 +646,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               }
             }
             if (c == chunks - 1) drained();
-            const uint32_t dst = next_buffer();
-            put(dst, words);
-            if (lane == 0 && row0 < prob.m && col0 + 64 * c < prob.n) store_box(&prob.out, dst, col0 + 64 * c, row0);
-            if (lane == 0) store_commit();
+            emptied();
+            put(buffers, words);
+            if (lane == 0 && row0 < prob.m && col0 + 64 * c < prob.n) {
+              store_box(&prob.out, buffers, col0 + 64 * c, row0);
+              store_commit();
+            }
           }
         }
       }

@@ -36,8 +36,8 @@ static thread_local int g_last_encode_result = 0;
 int last_tensor_map_result() { return g_last_encode_result; }
 
 namespace {
-// `rank` dimensions from the innermost, boxes of box_rows lines of 128 bytes; strides in bytes of dimensions 1, 2, ...
-bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, int box_cols, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+// `rank` dimensions from the innermost, boxes of box_rows lines; strides in bytes of dimensions 1, 2, ...
+bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, int box_cols, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
             int box_rows) {
   EncodeTiledFn fn = encoder();
   g_last_encode_result = -1;  // refused before the driver was asked
@@ -50,7 +50,7 @@ bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, int bo
   CUtensorMap tmp;
   auto call = [&]() {
     return fn(&tmp, type, rank, const_cast<void*>(base), dims, strides, box, elem_strides,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = call();
@@ -67,7 +67,7 @@ bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, int bo
   return true;
 }
 bool encode_rows(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, int box_rows) {
-  return encode(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 64, rank, dims, strides, box_rows);
+  return encode(map, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, 64, rank, dims, strides, box_rows);
 }
 }  // namespace
 
@@ -75,7 +75,7 @@ bool make_tensor_map(CUtensorMap* map, const void* base, int dtype, int rank, co
                      int box_rows) {
   const int size = dtype == MF_DTYPE_F32 ? 4 : 2;
   g_last_encode_result = -1;
-  if (rank < 2 || rank > 4 || box_cols * size != 128) return false;
+  if (rank < 2 || rank > 4 || (box_cols * size != 128 && box_cols * size != 64)) return false;
   cuuint64_t d[4], s[3];
   for (int i = 0; i < rank; ++i) {
     if (dims[i] <= 0) return false;
@@ -85,7 +85,7 @@ bool make_tensor_map(CUtensorMap* map, const void* base, int dtype, int rank, co
   const CUtensorMapDataType type = dtype == MF_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == MF_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return encode(map, base, type, box_cols, rank, d, s, box_rows);
+  return encode(map, base, type, box_cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, box_cols, rank, d, s, box_rows);
 }
 
 bool make_rows_tensor_map(CUtensorMap* map, const void* base, int rows_per_matrix, int matrices, int box_rows) {

@@ -25,7 +25,7 @@ bool make_rows_tensor_map(CUtensorMap* map, const void* base, int rows_per_matri
 bool make_strided_rows_tensor_map(CUtensorMap* map, const void* base, int rows, const int (&matrices)[2], long long row_stride,
                                   const long long (&matrix_strides)[2], int box_rows);
 // A tensor of `rank` dimensions from the innermost in an MF_DTYPE_* type, strides in bytes of dimensions 1, 2, ...; boxes of `box_rows`
-// lines of 128 bytes (64 or 32 elements), swizzled as above.
+// lines of 128 bytes, swizzled as above, or of 64 bytes, in the swizzle of that size.
 bool make_tensor_map(CUtensorMap* map, const void* base, int dtype, int rank, const long long* dims, const long long* strides, int box_cols,
                      int box_rows);
 // Result of the calling thread's last make_rows_tensor_map: the driver's code (0 = success), or -1 when the
