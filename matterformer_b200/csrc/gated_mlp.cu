@@ -58,46 +58,62 @@ int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
                                      : launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_GELU_TANH>(p, pairs, stream, what);
 }
 
-// ---- gradients of the weights --------------------------------------------------------------------------------------
-// Both are sums over the tokens, of [dg du] x and of dy h: one launch for the tiles of both.  Whole rounds of tiles walk all tokens;
-// the tiles behind them are cut into pieces of the tokens, each with a plane of partial sums of its own, which add_planes_kernel adds in order.
-// The plan goes by the sizes of both gradients, so that one's bits do not depend on whether the other is wanted.
-struct WeightPlan {
-  int k_blocks, tiles1, tiles, pieces, per;
-  int first, whole, first_rest, rest;  // of the wanted tiles: the first, how many are whole, and those that are cut
+// ---- gradients of the weights and of the input ---------------------------------------------------------------------
+// The weights' are sums over the tokens, of [dg du] x and of dy h, the input's is [dg du] W: one launch for the tiles of all three.  Each
+// pair of CTAs takes tiles of the weights in turn, which are long; those that have none in the last round take tiles of the input's
+// meanwhile, from the first token on as the weights' tiles do, so that [dg du] comes from memory once for both; the rest goes round
+// all pairs.  Where the weights have few tiles and many tokens, they are cut into pieces of the tokens, each with a plane of partial sums of
+// its own, which add_planes_kernel adds in order.  29 696 tokens x 512 x 2048: XX us, in launches of their own 117 + 150 + 11.
+// The plan goes by the sizes alone, so that one gradient's bits do not depend on which others are wanted.
+struct Plan {
+  int k_blocks, tiles1, tiles, pieces, per;  // of the weights
+  int first, wanted;                         // of the wanted ones
 };
-WeightPlan weight_plan(const MfGatedMlpArgs* a) {
-  WeightPlan w;
+// Rounds of the weights' pieces and of `input` tiles of `input_blocks` blocks behind and beside them: how many a pair without a piece in the
+// last round does ahead, and the longest a pair works, in blocks.
+struct Rounds {
+  int pairs, ahead, tiles_ahead;
+  double longest;
+};
+Rounds rounds_of(int pieces, int blocks, int input, int input_blocks) {
+  Rounds r;
+  r.pairs = pieces + 4 * input < kPairs ? pieces + 4 * input : kPairs;
+  const int full = pieces / r.pairs, last = pieces % r.pairs, others = r.pairs - last;
+  r.ahead = last && input_blocks ? blocks / input_blocks : 0;
+  r.tiles_ahead = (long long)r.ahead * others < input ? r.ahead * others : input;
+  const int rest = input - r.tiles_ahead, tail = rest % r.pairs;
+  const double behind = (double)(rest / r.pairs) * input_blocks + (tail == 0 ? 0. : 4 * tail <= r.pairs ? 0.4 : 2 * tail <= r.pairs ? 0.55 : 1.) * input_blocks;
+  const double busy = (double)(full + (last > 0)) * blocks, free = (double)full * blocks + (double)((r.tiles_ahead + others - 1) / others) * input_blocks;
+  r.longest = (busy > free ? busy : free) + behind;
+  return r;
+}
+int input_blocks(const MfGatedMlpArgs* a) { return (2 * a->hidden + kBlockK - 1) / kBlockK; }
+Plan plan_of(const MfGatedMlpArgs* a) {
+  Plan w;
   w.k_blocks = (int)((a->rows + kBlockK - 1) / kBlockK);
   w.tiles1 = tiles_of(2ll * a->hidden, a->dim, kTile);
   w.tiles = w.tiles1 + tiles_of(a->dim_out, a->hidden, kTile);
-  w.rest = w.tiles % kPairs;
+  const int input = tiles_of(a->rows, a->dim, kTile);
   w.pieces = 1, w.per = w.k_blocks;
-  // The number of pieces with the least estimated time: rounds of the longest piece, 0.3 us for a block of 64 tokens, and 0.1 us for
-  // each plane's way to memory and back.
   double least = 1e30;
-  for (int s = 1; w.rest && s <= kPairs && s <= w.k_blocks; ++s) {
+  for (int s = 1; s <= 16 && s <= w.k_blocks; ++s) {
     const int per = (w.k_blocks + s - 1) / s;
     if ((w.k_blocks + per - 1) / per != s) continue;  // a piece would be empty
-    const double us = 0.3 * ((w.rest * s + kPairs - 1) / kPairs) * per + (s > 1 ? 0.1 * w.rest * s : 0.);
-    if (us < least) least = us, w.pieces = s, w.per = per;
+    // a plane's way to memory and back takes a third of the 0.3 us of a block
+    const double blocks = rounds_of(w.tiles * s, per, input, input_blocks(a)).longest + (s > 1 ? 0.33 * w.tiles * s : 0.);
+    if (blocks < least) least = blocks, w.pieces = s, w.per = per;
   }
-  const int cut_from = w.pieces == 1 ? w.tiles : w.tiles - w.rest;
-  const int end = a->grad_w_out ? w.tiles : w.tiles1;
   w.first = a->grad_w_in ? 0 : w.tiles1;
-  w.first_rest = cut_from < w.first ? w.first : cut_from;
-  w.whole = (cut_from < end ? cut_from : end) - w.first;
-  if (w.whole < 0) w.whole = 0;
-  w.rest = end > w.first_rest ? end - w.first_rest : 0;
+  w.wanted = (a->grad_w_out ? w.tiles : w.tiles1) - w.first;
   return w;
 }
-size_t plane_bytes(const WeightPlan& w) { return (size_t)w.rest * w.pieces * kTile * kTile * 4; }
+size_t plane_bytes(const Plan& w) { return w.pieces > 1 ? (size_t)w.wanted * w.pieces * kTile * kTile * 4 : 0; }
 
 template <typename T, typename TOut>
-__global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict__ planes, WeightPlan w, TOut* __restrict__ out1, int m1, int n1,
+__global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict__ planes, Plan w, TOut* __restrict__ out1, int m1, int n1,
                                                          TOut* __restrict__ out2, int m2, int n2) {
   wait_for_previous();
-  const int tile = w.first_rest + blockIdx.x;
+  const int tile = w.first + blockIdx.x;
   const bool second = tile >= w.tiles1;
   const int m = second ? m2 : m1, n = second ? n2 : n1;
   TOut* out = second ? out2 : out1;
@@ -106,7 +122,7 @@ __global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict
   const int row = blockIdx.y * 4 + (threadIdx.x >> 6), col = 4 * (threadIdx.x & 63);
   if (tm * kTile + row >= m || tn * kTile + col >= n) return;
   const float* from = planes + ((size_t)blockIdx.x * kTile + row) * kTile + col;
-  const size_t stride = (size_t)w.rest * kTile * kTile;
+  const size_t stride = (size_t)w.wanted * kTile * kTile;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int q = 0; q < w.pieces; ++q) {
@@ -123,7 +139,7 @@ size_t pieces(const MfGatedMlpArgs* a, bool backward, size_t (&at)[4]) {  // gra
   at[0] = 0;
   if (!backward || rows == 0) return 0;
   at[1] = at[0] + align_up(rows * 2 * F * size, 256);
-  const size_t planes = a->grad_w_in || a->grad_w_out ? plane_bytes(weight_plan(a)) : 0;
+  const size_t planes = a->grad_w_in || a->grad_w_out ? plane_bytes(plan_of(a)) : 0;
   at[2] = at[1] + align_up(planes, 256);
   const long long bands = (a->rows + 31) / 32;
   at[3] = at[2] + (a->grad_b_in ? align_up((size_t)bands * 2 * F * 4, 256) : 0);
@@ -201,25 +217,37 @@ bool weight_problem(Problem& q, const MfGatedMlpArgs* a, const void* left, long 
 }
 
 template <typename T>
-int weight_gradients(const MfGatedMlpArgs* a, const void* grad_pre, float* planes, const BoundedWaits& waits, cudaStream_t stream) {
+int gradients(const MfGatedMlpArgs* a, const void* grad_pre, float* planes, const BoundedWaits& waits, cudaStream_t stream) {
   const int C = a->dim, F = a->hidden, O = a->dim_out;
-  const WeightPlan w = weight_plan(a);
+  const Plan w = plan_of(a);
   Params p{};
-  p.k = (int)a->rows, p.waits = waits, p.wide_out = a->grad_dtype == MF_DTYPE_F32;
-  p.first = w.first, p.whole = w.whole, p.first_rest = w.first_rest, p.rest = w.rest, p.per = w.per, p.first2 = w.tiles1;
-  p.tiles = w.whole + w.rest * w.pieces;
-  p.one.m = 2 * F, p.one.n = C;
+  p.k = (int)a->rows, p.k_input = 2 * F, p.waits = waits, p.wide_out = a->grad_dtype == MF_DTYPE_F32;
+  p.weight_tiles = w.wanted, p.first = w.first, p.first2 = w.tiles1, p.pieces = w.pieces, p.per = w.per;
+  p.one.m = 2 * F, p.one.n = C, p.input.m = (int)a->rows, p.input.n = C;
   if (a->grad_w_in) MF_MAP(weight_problem<T>(p.one, a, grad_pre, 2 * F, a->x, C, a->grad_w_in));
   if (a->grad_w_out) MF_MAP(weight_problem<T>(p.two, a, a->grad_y, O, a->act, F, a->grad_w_out));
-  if (w.rest) {
-    const long long dims[2] = {kTile, (long long)w.rest * w.pieces * kTile}, strides[1] = {4 * kTile};
+  if (a->grad_x) {
+    MF_MAP(map16<T>(&p.input.a, grad_pre, a->rows, 2 * F, 2 * F, 64));
+    MF_MAP(map16<T>(&p.input.b, a->w_in, 2 * F, C, C, 64));
+    MF_MAP(map16<T>(&p.input.out, a->grad_x, a->rows, C, C, 32));
+  }
+  const bool parts = w.pieces > 1;
+  if (parts) {
+    const long long dims[2] = {kTile, (long long)w.wanted * w.pieces * kTile}, strides[1] = {4 * kTile};
     MF_MAP(make_tensor_map(&p.pre, planes, MF_DTYPE_F32, 2, dims, strides, 32, 32));
   }
-  const int rc = launch_kernel<T, true, true, kWeight, 0>(p, p.tiles < kPairs ? p.tiles : kPairs, stream, "gated_mlp weight gradients");
-  if (rc != MF_OK || w.rest == 0) return rc;
+  const int input = a->grad_x ? tiles_of(a->rows, C, kTile) : 0;
+  const Rounds r = rounds_of(w.wanted * w.pieces, w.per, input, input_blocks(a));
+  const int others = input - r.tiles_ahead, rest = others % r.pairs;
+  p.ahead = r.ahead, p.tiles_ahead = r.tiles_ahead;
+  p.cut = rest == 0 || 2 * rest > r.pairs ? 1 : 4 * rest > r.pairs ? 2 : 4;
+  p.whole = p.cut == 1 ? others : others - rest;
+  p.tiles = p.whole + (others - p.whole) * p.cut;
+  const int rc = launch_kernel<T, true, true, kGradients, 0>(p, r.pairs, stream, "gated_mlp gradients");
+  if (rc != MF_OK || !parts) return rc;
   auto add = [&](auto* out1) {
     using TOut = std::remove_pointer_t<decltype(out1)>;
-    launch_dependent(add_planes_kernel<T, TOut>, dim3(w.rest, kTile / 4), dim3(256), 0, stream, planes, w, static_cast<TOut*>(a->grad_w_in), 2 * F, C,
+    launch_dependent(add_planes_kernel<T, TOut>, dim3(w.wanted, kTile / 4), dim3(256), 0, stream, planes, w, static_cast<TOut*>(a->grad_w_in), 2 * F, C,
                      static_cast<TOut*>(a->grad_w_out), O, F);
   };
   if (p.wide_out) add(static_cast<float*>(nullptr));
@@ -249,14 +277,15 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
     MF_MAP(map16<T>(&p.out2, grad_pre + F, M, F, 2 * F, 32));
     if ((rc = launch<T, false, true, kGateGrad>(p, a->activation, stream, "gated_mlp gate gradient")) != MF_OK) return rc;
   }
-  if (a->grad_x) {
+  if (a->grad_w_in || a->grad_w_out) {
+    if ((rc = gradients<T>(a, grad_pre, planes, waits, stream)) != MF_OK) return rc;
+  } else if (a->grad_x) {
     Params p = common(M, C, 2 * F, waits);
     MF_MAP(map16<T>(&p.one.a, grad_pre, M, 2 * F, 2 * F, 64));
     MF_MAP(map16<T>(&p.one.b, a->w_in, 2 * F, C, C, 64));
     MF_MAP(map16<T>(&p.one.out, a->grad_x, M, C, C, 32));
     if ((rc = launch<T, false, true, kStore>(p, 0, stream, "gated_mlp input gradient")) != MF_OK) return rc;
   }
-  if ((a->grad_w_in || a->grad_w_out) && (rc = weight_gradients<T>(a, grad_pre, planes, waits, stream)) != MF_OK) return rc;
   if (a->grad_b_in && (rc = column_sums(sums, MF_DTYPE_F32, (M + 31) / 32, (int)(2 * F), a->grad_b_in, a->grad_dtype, bands, stream)) != MF_OK) return rc;
   if (a->grad_b_out && (rc = column_sums(a->grad_y, a->dtype, M, (int)O, a->grad_b_out, a->grad_dtype, bands, stream)) != MF_OK) return rc;
   return MF_OK;

@@ -29,9 +29,9 @@ namespace gemm {
 
 __device__ int32_t g_gemm_status = 0;  // MF_ERR_DEVICE_TIMEOUT after an expired wait
 
-// kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well;  kGateGrad: its gradient;  kStore: the product and a bias;  kWeight: one or two
-// products over the same long dimension, which is cut into pieces for the tiles behind the last whole round
-enum Epilogue { kGate, kGateKeep, kGateGrad, kStore, kWeight };
+// kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well;  kGateGrad: its gradient;  kStore: the product and a bias;  kGradients: the
+// weights' gradients, two products over the same long dimension (of operands that have it outermost), and the input's, side by side
+enum Epilogue { kGate, kGateKeep, kGateGrad, kStore, kGradients };
 __host__ __device__ constexpr bool projects(Epilogue e) { return e == kGate || e == kGateKeep; }
 
 constexpr int kBlockK = 64;                       // elements of the contracted dimension in a stage
@@ -56,25 +56,27 @@ struct Shape {
 
 struct Problem {
   CUtensorMap a, b;  // boxes of 64 lines
-  CUtensorMap out;   // boxes of 32 lines (kWeight: fp32 or 16-bit elements)
+  CUtensorMap out;   // boxes of 32 lines (kGradients: fp32 or 16-bit elements)
   int m, n;
 };
 
 struct Params {
   Problem one;
-  Problem two;              // kWeight: the second product
-  CUtensorMap b2;           // kGate: the rows of the up projection, the odd CTA's
+  Problem two, input;       // kGradients: one and two are the weights', input the input's
+  CUtensorMap b2;           // projections: the rows of the up projection, the odd CTA's
   CUtensorMap out2;         // kGateGrad: gradients of up
-  CUtensorMap pre, pre2;    // pre-activations of gate | up (kGateKeep: written, boxes of 32 columns; kGateGrad: read); kWeight: pre = planes of partial sums
-  const void* bias;         // kGate: (2 n), kStore: (n); may be null
+  CUtensorMap pre, pre2;    // pre-activations of gate | up (kGateKeep: written, boxes of 32 columns; kGateGrad: read); kGradients: pre = planes of partial sums
+  const void* bias;         // projections: (2 n), kStore: (n); may be null
   uint2* exponents;         // of the pre-activations: (ceil(n / 64), m)
   float* column_sums;       // kGateGrad: (ceil(m / 32), 2 n) sums of the stored rows, or null
   int k;
   int whole, cut, tiles;    // tiles of full width, columns of a later one = full width / cut, pieces of work in all
-  int first2;               // kWeight: the second product's first tile
-  int first, first_rest;    // kWeight: the first tile, and the first that is cut along the contracted dimension
-  int rest, per;            // kWeight: how many are cut, and how many blocks a piece has
-  int wide_out;             // kWeight: fp32 results
+  // kGradients.  The weights' tiles: how many, the first, the first of the second product; in how many pieces their contracted dimension
+  // is cut, and how many blocks a piece has.  The input's: its contracted dimension, and how many tiles the pairs without a weight tile
+  // in the last round of those do meanwhile, each of them `ahead`; whole, cut and tiles are of the others.
+  int weight_tiles, first, first2, pieces, per;
+  int k_input, ahead, tiles_ahead;
+  int wide_out;             // fp32 gradients of the weights
   BoundedWaits waits;       // kinds: 0 operands, 1 stages, 2 accumulators, 3 drained accumulators
 };
 
@@ -224,9 +226,10 @@ __device__ __forceinline__ float2 column_sums32(uint32_t buffer, int lane) {
 
 // ---- the order of the work -----------------------------------------------------------------------------------------
 // What a pair does at a time: `cols` columns from `col` of the rows from `row` on, over the blocks [k0, k1) of the contracted dimension.
+enum Which { kOne, kTwo, kInput };
 struct Work {
   int row, col, cols, k0, k1;
-  bool second;  // of the second product (kWeight)
+  Which which;  // kGradients
   int plane;    // where a part of a tile goes; -1: the whole
 };
 
@@ -243,40 +246,78 @@ template <Epilogue kEpi>
 struct Walk {
   const Params& p;
   int pairs, k_blocks, tiles_m, tiles_n, t;
+  int phase = 0, step = 0, place = 0, others = 0;  // kGradients
   __device__ Walk(const Params& q, int pair, int pairs_) : p(q), pairs(pairs_), t(pair) {
     k_blocks = (p.k + kBlockK - 1) / kBlockK;
-    tiles_m = (p.one.m + kTile - 1) / kTile;
-    tiles_n = (p.one.n + full() - 1) / full();
+    const Problem& tiled = kEpi == kGradients ? p.input : p.one;
+    tiles_m = (tiled.m + kTile - 1) / kTile;
+    tiles_n = (tiled.n + full() - 1) / full();
+    if constexpr (kEpi == kGradients) {  // the pairs that have no tile in the last round of the weights' come first from then on
+      const int last = p.weight_tiles * p.pieces % pairs;
+      others = pairs - last;
+      place = pair >= last ? pair - last : others + pair;
+      step = place;
+    }
   }
   __device__ static constexpr int full() { return projects(kEpi) ? kTile / 2 : kTile; }
   __device__ bool next(Work& w) {
-    if (t >= p.tiles) return false;
-    const bool whole = t < p.whole;
-    int m, n;
-    w.second = false, w.plane = -1, w.cols = full(), w.k0 = 0, w.k1 = k_blocks;
-    if constexpr (kEpi == kWeight) {
-      // The same piece of all cut tiles comes before the next piece of any: pairs that work at the same time read the same stretch of
-      // the operands.  (Equal shares of all blocks in a row, where each pair is somewhere else, took 210 us instead of 100 on
-      // 29 696 tokens: all operands came from memory again and again.)
-      int tile = p.first + t;
-      if (!whole) {
-        const int u = t - p.whole;
-        tile = p.first_rest + u % p.rest;
-        w.k0 = u / p.rest * p.per, w.k1 = min(k_blocks, w.k0 + p.per), w.plane = u;
+    w.which = kOne, w.plane = -1, w.cols = full(), w.k0 = 0, w.k1 = k_blocks;
+    if constexpr (kEpi == kGradients) {
+      int m, n;
+      if (phase == 0) {
+        if (t < p.weight_tiles * p.pieces) {
+          // The same piece of all tiles comes before the next piece of any: pairs that work at the same time read the same stretch of
+          // the operands.  (Equal shares of all blocks in a row, where each pair is somewhere else, took 210 us instead of 100 on
+          // 29 696 tokens: all operands came from memory again and again.)
+          const int piece = t / p.weight_tiles, tile = p.first + t - piece * p.weight_tiles;
+          w.k0 = piece * p.per, w.k1 = min(k_blocks, w.k0 + p.per);
+          if (p.pieces > 1) w.plane = t;
+          if (tile >= p.first2) {
+            w.which = kTwo;
+            tile_at(tile - p.first2, (p.two.m + kTile - 1) / kTile, (p.two.n + kTile - 1) / kTile, m, n);
+          } else {
+            tile_at(tile, (p.one.m + kTile - 1) / kTile, (p.one.n + kTile - 1) / kTile, m, n);
+          }
+          w.row = m * kTile, w.col = n * kTile;
+          t += pairs;
+          return true;
+        }
+        phase = 1;
       }
-      w.second = tile >= p.first2;
-      if (w.second) tile_at(tile - p.first2, (p.two.m + kTile - 1) / kTile, (p.two.n + kTile - 1) / kTile, m, n);
-      else tile_at(tile, tiles_m, tiles_n, m, n);
-      w.col = n * kTile;
+      w.which = kInput;
+      w.k1 = (p.k_input + kBlockK - 1) / kBlockK;
+      int tile, part = 0;
+      if (phase == 1) {  // tiles that the others do ahead, row by row like the weights' tiles: what both read of [dg du] is in L2
+        if (place < others && step < p.tiles_ahead && step < p.ahead * others) {
+          tile = step;
+          step += others;
+          w.row = tile / tiles_n * kTile, w.col = tile % tiles_n * kTile;
+          return true;
+        }
+        phase = 2, step = place;
+      }
+      if (step >= p.tiles) return false;
+      if (step < p.whole) {
+        tile = p.tiles_ahead + step;
+      } else {
+        tile = p.tiles_ahead + p.whole + (step - p.whole) / p.cut, part = (step - p.whole) % p.cut;
+        w.cols = kTile / p.cut;
+      }
+      step += pairs;
+      w.row = tile / tiles_n * kTile, w.col = tile % tiles_n * kTile + part * w.cols;
+      return true;
     } else {
+      if (t >= p.tiles) return false;
+      const bool whole = t < p.whole;
+      int m, n;
       const int part = whole ? 0 : (t - p.whole) % p.cut, tile = whole ? t : p.whole + (t - p.whole) / p.cut;
       if (!whole) w.cols = full() / p.cut;
       tile_at(tile, tiles_m, tiles_n, m, n);
       w.col = n * full() + part * w.cols;
+      w.row = m * kTile;
+      t += pairs;
+      return true;
     }
-    w.row = m * kTile;
-    t += pairs;
-    return true;
   }
 };
 
@@ -314,14 +355,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 
   Walk<kEpi> walk(p, pair, pairs);
   Work w;
+  auto problem = [&](const Work& x) -> const Problem& { return kEpi == kGradients && x.which != kOne ? (x.which == kTwo ? p.two : p.input) : p.one; };
   bool bad = false;
   if (warp == 0) {
     // ---------------------------------------------------------------- copies
     if (elect_one()) {
       uint32_t it = 0;
       while (!bad && walk.next(w)) {
-        const CUtensorMap* amap = kEpi == kWeight && w.second ? &p.two.a : &p.one.a;
-        const CUtensorMap* bmap = kEpi == kWeight && w.second ? &p.two.b : projects(kEpi) && rank ? &p.b2 : &p.one.b;
+        const Problem& prob = problem(w);
+        const CUtensorMap* bmap = projects(kEpi) && rank ? &p.b2 : &prob.b;
+        const bool outermost = kEpi == kGradients ? w.which != kInput : kAMn;  // the contracted dimension of A
         const int row = w.row + 128 * (int)rank;
         const int col = projects(kEpi) ? w.col : w.col + w.cols / 2 * (int)rank;
         const bool two = (projects(kEpi) ? w.cols : w.cols / 2) > 64;  // boxes of B (a tile of 64 columns uses half of its box)
@@ -335,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           const uint32_t bar = map_to_rank(smem_u32(&bar_full[s]), 0), dst = smem + s * kStageBytes;
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            load_box2(dst + i * kBoxBytes, amap, kAMn ? row + 64 * i : kb * kBlockK, kAMn ? kb * kBlockK : row + 64 * i, bar);
+            load_box2(dst + i * kBoxBytes, &prob.a, outermost ? row + 64 * i : kb * kBlockK, outermost ? kb * kBlockK : row + 64 * i, bar);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
             if (i == 0 || two)
@@ -356,8 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     // ---------------------------------------------------------------- products
     if (elect_one()) {
       // K-major: 16 elements of a line further on; MN-major: 16 lines further on, 64-wide chunks a box apart
-      constexpr uint32_t kStepA = kAMn ? 16 * 128 : 32, kStepB = kBMn ? 16 * 128 : 32;
-      const uint64_t a0 = make_smem_desc_sw128(smem, kAMn ? kBoxBytes : 0, 1024);
+      constexpr uint32_t kStepB = kBMn ? 16 * 128 : 32;
       const uint64_t b0 = make_smem_desc_sw128(smem + 2 * kBoxBytes, kBMn ? kBoxBytes : 0, 1024);
       uint32_t it = 0;
       for (int n = 0; !bad && walk.next(w); ++n) {
@@ -367,7 +409,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           break;
         }
         tc_fence_after_sync();
-        const uint32_t idesc = instruction<T, kAMn, kBMn>() | ((uint32_t)((projects(kEpi) ? 2 * w.cols : w.cols) >> 3) << 17);
+        const bool outermost = kEpi == kGradients ? w.which != kInput : kAMn;
+        const uint32_t step_a = outermost ? 16 * 128 : 32;
+        const uint64_t a0 = make_smem_desc_sw128(smem, outermost ? kBoxBytes : 0, 1024);
+        const uint32_t idesc = (outermost ? instruction<T, true, kBMn>() : instruction<T, false, kBMn>()) | ((uint32_t)((projects(kEpi) ? 2 * w.cols : w.cols) >> 3) << 17);
         for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int s = it % kStages;
           if (!mbar_wait_for(&bar_full[s], (it / kStages) & 1, p.waits.limit)) {
@@ -378,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           const uint64_t a = desc_advance(a0, s * kStageBytes), b = desc_advance(b0, s * kStageBytes);
 #pragma unroll
           for (int k = 0; k < kBlockK / 16; ++k)
-            umma2(tmem + buf * kTile, desc_advance(a, k * kStepA), desc_advance(b, k * kStepB), idesc, kb > w.k0 || k > 0);
+            umma2(tmem + buf * kTile, desc_advance(a, k * step_a), desc_advance(b, k * kStepB), idesc, kb > w.k0 || k > 0);
           umma_commit2(&bar_empty[s]);
         }
         if (!bad) umma_commit2(&bar_acc[buf]);
@@ -607,8 +652,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         }
         if (bad) break;
       } else {
-        const Problem& prob = kEpi == kWeight && w.second ? p.two : p.one;
-        if (kEpi == kWeight && (w.plane >= 0 || p.wide_out)) {  // 32 fp32 columns at a time: a part of a tile, or an fp32 result
+        const Problem& prob = problem(w);
+        if (kEpi == kGradients && w.which != kInput && (w.plane >= 0 || p.wide_out)) {  // 32 fp32 columns at a time: a part of a tile, or an fp32 result
 #pragma unroll 1
           for (int c = 0; c < 2 * chunks; ++c) {
             uint32_t d[32];
