@@ -40,17 +40,6 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
   for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
 }
 
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&v)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-    v[2 * e] = f.x, v[2 * e + 1] = f.y;
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]);
 template <>
@@ -176,9 +165,8 @@ __global__ void __launch_bounds__(kWarps * 32) column_sums_band_kernel(const T* 
 
 // Adds the bands: a block of 32 x 8 threads owns 32 columns; thread (x, y) adds the bands y, y + 8, ... (four loads in
 // flight), then the eight slices are added in slice order.
-template <typename TOut>
 __global__ void __launch_bounds__(256) column_sums_final_kernel(const float* __restrict__ part, int bands, int C,
-                                                                TOut* __restrict__ out) {
+                                                                float* __restrict__ out) {
   __shared__ float red[8][32];
   wait_for_previous();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
@@ -199,7 +187,7 @@ __global__ void __launch_bounds__(256) column_sums_final_kernel(const float* __r
     float tot = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) tot += red[w][x];
-    out[c] = from_f32<TOut>(tot);
+    out[c] = tot;
   }
 }
 
@@ -216,24 +204,8 @@ int bands_for(long long rows, int cols) {
 
 }  // namespace
 
-size_t column_sums_workspace(long long rows, int cols) { return (size_t)bands_for(rows, cols) * (size_t)cols * sizeof(float); }
-
-int column_sums(const void* x, int dtype, long long rows, int cols, void* out, int out_dtype, float* part, cudaStream_t stream) {
-  const int bands = bands_for(rows, cols);
-  const long long rows_per_band = (rows + bands - 1) / bands;
-  const dim3 grid((cols + kColsPerBlock - 1) / kColsPerBlock, bands);
-  MF_DISPATCH_DTYPE(dtype, T,
-                    launch_dependent(column_sums_band_kernel<T, false>, grid, dim3(kWarps * 32), 0, stream, static_cast<const T*>(x), nullptr, nullptr,
-                                     rows, cols, rows_per_band, part));
-  MF_CHECK_LAUNCH("column_sums_band_kernel");
-  MF_DISPATCH_DTYPE(out_dtype, T,
-                    launch_dependent(column_sums_final_kernel<T>, dim3((cols + 31) / 32), dim3(256), 0, stream, part, bands, cols, static_cast<T*>(out)));
-  MF_CHECK_LAUNCH("column_sums_final_kernel");
-  return MF_OK;
-}
-
 int add_bands(const float* part, int bands, int cols, float* out, cudaStream_t stream) {
-  launch_dependent(column_sums_final_kernel<float>, dim3((cols + 31) / 32), dim3(256), 0, stream, part, bands, cols, out);
+  launch_dependent(column_sums_final_kernel, dim3((cols + 31) / 32), dim3(256), 0, stream, part, bands, cols, out);
   MF_CHECK_LAUNCH("column_sums_final_kernel");
   return MF_OK;
 }
@@ -243,7 +215,7 @@ using namespace mf;
 
 extern "C" size_t mf_column_sums_workspace_bytes(int64_t rows, int32_t cols) {
   if (rows < 0 || cols < 1) return 0;
-  return column_sums_workspace(rows, cols);
+  return (size_t)bands_for(rows, cols) * (size_t)cols * sizeof(float);
 }
 
 extern "C" int mf_column_sums(const void* x, int32_t dtype, int64_t rows, int32_t cols, float* out, void* workspace,
@@ -257,12 +229,22 @@ extern "C" int mf_column_sums(const void* x, int32_t dtype, int64_t rows, int32_
     cudaError_t e = cudaMemsetAsync(out, 0, (size_t)cols * sizeof(float), s);
     return e == cudaSuccess ? MF_OK : cuda_error(e, "cudaMemsetAsync(mf_column_sums)");
   }
-  const size_t need = column_sums_workspace(rows, cols);
-  if (workspace == nullptr || workspace_bytes < need) {
-    set_error("mf_column_sums: workspace too small (%zu bytes needed)", need);
+  const int bands = bands_for(rows, cols);
+  if (workspace == nullptr || workspace_bytes < (size_t)bands * cols * sizeof(float)) {
+    set_error("mf_column_sums: workspace too small (%zu bytes needed)", (size_t)bands * cols * sizeof(float));
     return MF_ERR_WORKSPACE_TOO_SMALL;
   }
-  return column_sums(x, dtype, rows, cols, out, MF_DTYPE_F32, static_cast<float*>(workspace), s);
+  float* part = static_cast<float*>(workspace);
+  const long long rows_per_band = (rows + bands - 1) / bands;
+  const dim3 grid((cols + kColsPerBlock - 1) / kColsPerBlock, bands);
+  if (dtype == MF_DTYPE_BF16)
+    launch_dependent(column_sums_band_kernel<__nv_bfloat16, false>, grid, dim3(kWarps * 32), 0, s, static_cast<const __nv_bfloat16*>(x),
+                     nullptr, nullptr, rows, cols, rows_per_band, part);
+  else
+    launch_dependent(column_sums_band_kernel<float, false>, grid, dim3(kWarps * 32), 0, s, static_cast<const float*>(x), nullptr, nullptr,
+                     rows, cols, rows_per_band, part);
+  MF_CHECK_LAUNCH("column_sums_band_kernel");
+  return add_bands(part, bands, cols, out, s);
 }
 
 extern "C" int mf_gelu_tanh_fwd(const void* x, int32_t dtype, int64_t n, void* y, void* stream) {

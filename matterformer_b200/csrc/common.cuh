@@ -189,10 +189,6 @@ __device__ __forceinline__ float warp_sum(float v) {
 namespace mf {
 // Kernel timing aid (see mf_profile_enable): record an event on `stream` before/after a main kernel.
 void profile_mark(int which, bool begin, cudaStream_t stream);
-// Column sums of a (rows, cols) matrix, cols a multiple of 8, rows > 0, in any two element types; `part` holds column_sums_workspace
-// bytes (column_sums.cu).
-size_t column_sums_workspace(long long rows, int cols);
-int column_sums(const void* x, int dtype, long long rows, int cols, void* out, int out_dtype, float* part, cudaStream_t stream);
 // out[c] = sum over the bands of part[band][c], in band order (column_sums.cu).
 int add_bands(const float* part, int bands, int cols, float* out, cudaStream_t stream);
 }  // namespace mf

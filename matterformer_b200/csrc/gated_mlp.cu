@@ -141,12 +141,35 @@ size_t pieces(const MfGatedMlpArgs* a, bool backward, size_t (&at)[4]) {  // gra
   at[1] = at[0] + align_up(rows * 2 * F * size, 256);
   const size_t planes = a->grad_w_in || a->grad_w_out ? plane_bytes(plan_of(a)) : 0;
   at[2] = at[1] + align_up(planes, 256);
-  const long long bands = (a->rows + 31) / 32;
-  at[3] = at[2] + (a->grad_b_in ? align_up((size_t)bands * 2 * F * 4, 256) : 0);
-  size_t sums = 0;
-  if (a->grad_b_in) sums = column_sums_workspace(bands, 2 * a->hidden);
-  if (a->grad_b_out && column_sums_workspace(a->rows, a->dim_out) > sums) sums = column_sums_workspace(a->rows, a->dim_out);
-  return at[3] + align_up(sums, 256);
+  at[3] = at[2] + (a->grad_b_in ? align_up((size_t)((a->rows + 31) / 32) * 2 * F * 4, 256) : 0);
+  return at[3] + align_up((size_t)kBands * ((a->grad_b_in ? 2 * F : 0) + (a->grad_b_out ? (size_t)a->dim_out : 0)) * 4, 256);
+}
+
+// ---- gradients of the biases ---------------------------------------------------------------------------------------
+// The bands' sums come from the idle warps of the launch above, where weights are wanted, else from a launch of their own.
+template <typename T>
+__global__ void __launch_bounds__(64) bias_bands_kernel(BiasSums b) {
+  wait_for_previous();
+  bias_band<T>(b, 2 * blockIdx.x + (threadIdx.x >> 5), threadIdx.x & 31);
+}
+// 32 columns a block; thread (x, y) adds the bands y, y + 8, ..., then the eight sums are added in order.
+template <typename TOut>
+__global__ void __launch_bounds__(256) add_bias_bands_kernel(BiasSums b, TOut* __restrict__ out_in, TOut* __restrict__ out_out) {
+  __shared__ float red[8][32];
+  wait_for_previous();
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n = b.n_in + b.n_out, c = blockIdx.x * 32 + x;
+  float s = 0.f;
+  if (c < n) {
+#pragma unroll 8
+    for (int k = y; k < kBands; k += 8) s += b.part[(size_t)k * n + c];
+  }
+  red[y][x] = s;
+  __syncthreads();
+  if (y == 0 && c < n) {
+    for (int k = 1; k < 8; ++k) s += red[k][x];
+    if (c < b.n_in) out_in[c] = from_f32<TOut>(s);
+    else out_out[c - b.n_in] = from_f32<TOut>(s);
+  }
 }
 
 int check(const MfGatedMlpArgs* a) {
@@ -217,11 +240,11 @@ bool weight_problem(Problem& q, const MfGatedMlpArgs* a, const void* left, long 
 }
 
 template <typename T>
-int gradients(const MfGatedMlpArgs* a, const void* grad_pre, float* planes, const BoundedWaits& waits, cudaStream_t stream) {
+int gradients(const MfGatedMlpArgs* a, const void* grad_pre, float* planes, const BiasSums& bias_sums, const BoundedWaits& waits, cudaStream_t stream) {
   const int C = a->dim, F = a->hidden, O = a->dim_out;
   const Plan w = plan_of(a);
   Params p{};
-  p.k = (int)a->rows, p.k_input = 2 * F, p.waits = waits, p.wide_out = a->grad_dtype == MF_DTYPE_F32;
+  p.k = (int)a->rows, p.k_input = 2 * F, p.waits = waits, p.wide_out = a->grad_dtype == MF_DTYPE_F32, p.bias_sums = bias_sums;
   p.weight_tiles = w.wanted, p.first = w.first, p.first2 = w.tiles1, p.pieces = w.pieces, p.per = w.per;
   p.one.m = 2 * F, p.one.n = C, p.input.m = (int)a->rows, p.input.n = C;
   if (a->grad_w_in) MF_MAP(weight_problem<T>(p.one, a, grad_pre, 2 * F, a->x, C, a->grad_w_in));
@@ -263,7 +286,9 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
   pieces(a, true, at);
   char* ws = static_cast<char*>(a->workspace);
   T* grad_pre = reinterpret_cast<T*>(ws + at[0]);
-  float *planes = reinterpret_cast<float*>(ws + at[1]), *sums = reinterpret_cast<float*>(ws + at[2]), *bands = reinterpret_cast<float*>(ws + at[3]);
+  float *planes = reinterpret_cast<float*>(ws + at[1]), *sums = reinterpret_cast<float*>(ws + at[2]);
+  const bool biased = a->grad_b_in || a->grad_b_out;
+  const BiasSums b = {a->grad_y, sums, biased ? reinterpret_cast<float*>(ws + at[3]) : nullptr, M, a->grad_b_out ? (int)O : 0, a->grad_b_in ? (int)(2 * F) : 0};
   int rc;
   if (a->grad_x || a->grad_w_in || a->grad_b_in) {
     Params p = common(M, F, O, waits);
@@ -278,7 +303,7 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
     if ((rc = launch<T, false, true, kGateGrad>(p, a->activation, stream, "gated_mlp gate gradient")) != MF_OK) return rc;
   }
   if (a->grad_w_in || a->grad_w_out) {
-    if ((rc = gradients<T>(a, grad_pre, planes, waits, stream)) != MF_OK) return rc;
+    if ((rc = gradients<T>(a, grad_pre, planes, b, waits, stream)) != MF_OK) return rc;
   } else if (a->grad_x) {
     Params p = common(M, C, 2 * F, waits);
     MF_MAP(map16<T>(&p.one.a, grad_pre, M, 2 * F, 2 * F, 64));
@@ -286,8 +311,16 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
     MF_MAP(map16<T>(&p.one.out, a->grad_x, M, C, C, 32));
     if ((rc = launch<T, false, true, kStore>(p, 0, stream, "gated_mlp input gradient")) != MF_OK) return rc;
   }
-  if (a->grad_b_in && (rc = column_sums(sums, MF_DTYPE_F32, (M + 31) / 32, (int)(2 * F), a->grad_b_in, a->grad_dtype, bands, stream)) != MF_OK) return rc;
-  if (a->grad_b_out && (rc = column_sums(a->grad_y, a->dtype, M, (int)O, a->grad_b_out, a->grad_dtype, bands, stream)) != MF_OK) return rc;
+  if (!biased) return MF_OK;
+  if (!a->grad_w_in && !a->grad_w_out) {
+    launch_dependent(bias_bands_kernel<T>, dim3(kBands / 2), dim3(64), 0, stream, b);
+    MF_CHECK_LAUNCH("bias_bands_kernel");
+  }
+  const dim3 grid((b.n_in + b.n_out + 31) / 32);
+  if (a->grad_dtype == MF_DTYPE_F32)
+    launch_dependent(add_bias_bands_kernel<float>, grid, dim3(256), 0, stream, b, static_cast<float*>(a->grad_b_in), static_cast<float*>(a->grad_b_out));
+  else launch_dependent(add_bias_bands_kernel<T>, grid, dim3(256), 0, stream, b, static_cast<T*>(a->grad_b_in), static_cast<T*>(a->grad_b_out));
+  MF_CHECK_LAUNCH("add_bias_bands_kernel");
   return MF_OK;
 }
 

@@ -60,6 +60,17 @@ struct Problem {
   int m, n;
 };
 
+// Column sums of grad_y (rows, n_out) and of the (rows / 32, n_in) sums of the gradients of the pre-activations, each in kBands bands of
+// rows, each band in the order of its rows: part[band] holds the n_in columns of the second, then those of the first.
+constexpr int kBands = 296;
+struct BiasSums {
+  const void* grad_y;
+  const float* sums;
+  float* part;  // null: none wanted
+  long long rows;
+  int n_out, n_in;  // 0: not wanted
+};
+
 struct Params {
   Problem one;
   Problem two, input;       // kGradients: one and two are the weights', input the input's
@@ -77,6 +88,7 @@ struct Params {
   int weight_tiles, first, first2, pieces, per;
   int k_input, ahead, tiles_ahead;
   int wide_out;             // fp32 gradients of the weights
+  BiasSums bias_sums;       // what the two idle warps of a CTA add meanwhile
   BoundedWaits waits;       // kinds: 0 operands, 1 stages, 2 accumulators, 3 drained accumulators
 };
 
@@ -222,6 +234,41 @@ __device__ __forceinline__ float2 column_sums32(uint32_t buffer, int lane) {
     if ((lane & 3) == c) sum = make_float2(d[0], d[2]);  // (all columns of the result are the same)
   }
   return sum;
+}
+
+template <typename T>
+__device__ __forceinline__ void add8(float (&acc)[8], const T* x) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(x), b = *reinterpret_cast<const float4*>(x + 4);
+    acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w, acc[4] += b.x, acc[5] += b.y, acc[6] += b.z, acc[7] += b.w;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(x);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack2<T>(w[e]);
+      acc[2 * e] += f.x, acc[2 * e + 1] += f.y;
+    }
+  }
+}
+// One warp: a band of the rows of x (rows, n), n a multiple of 8.
+template <typename T>
+__device__ __forceinline__ void column_band(const T* x, long long rows, int n, int band, float* out, int lane) {
+  const long long r0 = rows * band / kBands, r1 = rows * (band + 1) / kBands;
+  for (int c = 8 * lane; c < n; c += 256) {
+    float acc[8] = {};
+    long long r = r0;
+#pragma unroll 4
+    for (; r < r1; ++r) add8(acc, x + r * n + c);
+    reinterpret_cast<float4*>(out + c)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    reinterpret_cast<float4*>(out + c)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void bias_band(const BiasSums& b, int band, int lane) {
+  float* out = b.part + (size_t)band * (b.n_in + b.n_out);
+  if (b.n_in) column_band(b.sums, (b.rows + 31) / 32, b.n_in, band, out, lane);
+  if (b.n_out) column_band(static_cast<const T*>(b.grad_y), b.rows, b.n_out, band, out + b.n_in, lane);
 }
 
 // ---- the order of the work -----------------------------------------------------------------------------------------
@@ -433,6 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         mbar_wait(&bar_end, 0);
       }
     }
+  } else if (kEpi == kGradients && (warp == 2 || warp == 3)) {
+    // ---------------------------------------------------------------- sums beside the products
+    if (p.bias_sums.part)
+      for (int band = 2 * blockIdx.x + warp - 2; band < kBands; band += 2 * gridDim.x) bias_band<T>(p.bias_sums, band, lane);
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- results
     const int ew = warp - 4, quad = warp & 3, half = ew >> 2;
