@@ -3,7 +3,7 @@
 // With at most 32 tokens every weight meets few operands: reading the weights bounds the block, 2 bytes for 2 * 32 operations at most.  The
 // weights are the 16-row operand of mma.sync, the tokens its 8 columns, so that one token costs what eight do and nothing is
 // padded to a 256-row tile.  A CTA owns 16 hidden channels (of gate and of up) or 16 output channels; its eight warps, and those
-// of up to eight CTAs of a cluster where there are few channels, share the contracted dimension, and their sums meet in shared memory,
+// of up to four CTAs of a cluster where there are few channels, share the contracted dimension, and their sums meet in shared memory,
 // added in the order of warps and CTAs.  A lane reads 16 bytes of a weight row and of a token at a time: which k an operand's register
 // stands for is free as long as both sides agree, so no layout of the instruction reaches memory.
 #include "common.cuh"
@@ -55,7 +55,7 @@ __device__ __forceinline__ uint4 stream16(const void* base, size_t bytes, bool v
 
 template <typename T, int kTiles, bool kGate>  // kTiles: of eight tokens
 __global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p) {
-  constexpr int kSides = kGate ? 2 : 1, kRows = 16 * kSides, kTokens = 8 * kTiles, kBatch = kTiles == 4 ? 2 : 4;
+  constexpr int kSides = kGate ? 2 : 1, kRows = 16 * kSides, kTokens = 8 * kTiles, kBatch = 2;
   __shared__ float part[kWarps][kRows][kTokens + 1];
   __shared__ float sums[kRows][kTokens + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -72,14 +72,15 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p)
   for (int side = 0; side < kSides; ++side)
 #pragma unroll
     for (int r = 0; r < 2; ++r) row[side][r] = ((size_t)side * p.n + n0 + g + 8 * r) * p.k * 2;
-  // no value is read before the kernels before this one have ended; the weights may already move to L2
+  // no value is read before the kernels before this one have ended; a short slice of the weights may already move to L2 (29 tokens, 512 x
+  // 2048: 14.0 -> 12.9 us; long slices are slower for it, 57 -> 64 us for one token of 4096 x 10 928)
   launch_dependents();
-  for (int s = s0 + t; s < s1; s += 4)  // (64 bytes of a row a step: one lane in four asks for each)
+  if (s1 - s0 <= 4 && s0 + t < s1)  // (64 bytes of a row a step: one lane in four asks for each)
 #pragma unroll
     for (int side = 0; side < kSides; ++side)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        if (ok[r]) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.w) + row[side][r] + (size_t)s * (2 * kStep)));
+        if (ok[r]) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.w) + row[side][r] + (size_t)(s0 + t) * (2 * kStep)));
   wait_for_previous();
 
   float acc[kSides][kTiles][4] = {};
@@ -179,9 +180,10 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p)
 template <typename T, int kTiles, bool kGate>
 int launch(const SmallParams& p, cudaStream_t stream, const char* what) {
   const int tiles = (p.n + 15) / 16, steps = (p.k + kStep - 1) / kStep;
-  // enough CTAs for three on every SM, while a warp keeps two steps at least
+  // Enough CTAs for two on every SM, while a warp keeps two steps at least.  Sums over a cluster cost more than idle SMs beyond that: 16 tokens,
+  // 1024 x 4096: clusters of 4 15 us, of 8 23 us; one token, 4096 x 10 928: two CTAs an SM 53 us, four 55, eight 82.
   int ranks = 1;
-  while (ranks < 8 && tiles * ranks < 3 * 148 && steps / (2 * ranks * kWarps) >= 2) ranks *= 2;
+  while (ranks < 4 && tiles * ranks < 2 * 148 && steps / (2 * ranks * kWarps) >= 2) ranks *= 2;
   cudaLaunchAttribute attributes[2] = {};
   attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[0].val.programmaticStreamSerializationAllowed = 1;
