@@ -687,7 +687,8 @@ int mf_rotary(const MfRotaryArgs* args, void* stream);
  * Backward: reads x, w_in, w_out, pre, act and grad_y; writes those of grad_x, grad_w_in, grad_w_out, grad_b_in, grad_b_out that are
  * not NULL.  Sums are in fp32 and in a fixed order; act and the gradients of the pre-activations are rounded to dtype, the
  * pre-activations to three bits more.
- * Workspace (backward): mf_gated_mlp_bwd_workspace_bytes, for the same gradients.  An expired device-side wait is reported by
+ * Workspace: forward mf_gated_mlp_fwd_workspace_bytes (without it some sizes take longer), backward mf_gated_mlp_bwd_workspace_bytes
+ * for the same gradients.  An expired device-side wait is reported by
  * mf_gated_mlp_status (which synchronises `stream`); the outputs of such a call are undefined.
  */
 typedef struct MfGatedMlpArgs {
@@ -715,6 +716,7 @@ typedef struct MfGatedMlpArgs {
 } MfGatedMlpArgs;
 
 size_t mf_gated_mlp_pre_bytes(int64_t rows, int32_t hidden);
+size_t mf_gated_mlp_fwd_workspace_bytes(const MfGatedMlpArgs* args);
 size_t mf_gated_mlp_bwd_workspace_bytes(const MfGatedMlpArgs* args);
 int mf_gated_mlp_fwd(const MfGatedMlpArgs* args, void* stream);
 int mf_gated_mlp_bwd(const MfGatedMlpArgs* args, void* stream);

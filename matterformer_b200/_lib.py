@@ -100,6 +100,7 @@ EXPORTED_SYMBOLS = (
     "mf_pair_head_bwd",
     "mf_rotary",
     "mf_gated_mlp_pre_bytes",
+    "mf_gated_mlp_fwd_workspace_bytes",
     "mf_gated_mlp_bwd_workspace_bytes",
     "mf_gated_mlp_fwd",
     "mf_gated_mlp_bwd",
@@ -465,8 +466,9 @@ def lib() -> ctypes.CDLL:
     L.mf_rotary.restype = c_int32
     L.mf_gated_mlp_pre_bytes.argtypes = [c_int64, c_int32]
     L.mf_gated_mlp_pre_bytes.restype = c_size_t
-    L.mf_gated_mlp_bwd_workspace_bytes.argtypes = [POINTER(MfGatedMlpArgs)]
-    L.mf_gated_mlp_bwd_workspace_bytes.restype = c_size_t
+    for fn in (L.mf_gated_mlp_fwd_workspace_bytes, L.mf_gated_mlp_bwd_workspace_bytes):
+        fn.argtypes = [POINTER(MfGatedMlpArgs)]
+        fn.restype = c_size_t
     for fn in (L.mf_gated_mlp_fwd, L.mf_gated_mlp_bwd):
         fn.argtypes = [POINTER(MfGatedMlpArgs), c_void_p]
         fn.restype = c_int32

@@ -41,21 +41,106 @@ int launch_kernel(const Params& p, int pairs, cudaStream_t stream, const char* w
   return l == cudaSuccess ? MF_OK : cuda_error(l, what);
 }
 
+#define MF_MAP(call)                                                                                           \
+  do {                                                                                                         \
+    if (!(call)) {                                                                                             \
+      set_error("%s: tensor map refused (driver code %d)", kName, last_tensor_map_result());                   \
+      return MF_ERR_CUDA;                                                                                      \
+    }                                                                                                          \
+  } while (0)
+
 int tiles_of(long long rows, long long cols, int width) { return (int)(((rows + kTile - 1) / kTile) * ((cols + width - 1) / width)); }
 
 // Tiles of full width in whole rounds of the pairs; a last round that would leave at least half (three quarters) of them without work is
 // cut into tiles of half (a quarter of) the width.  29 696 x 512 over 2048: 232 tiles are 3.1 rounds.
-template <typename T, bool kAMn, bool kBMn, Epilogue kEpi>
-int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
+template <Epilogue kEpi>
+void cut_tiles(Params& p) {
   const int tiles = tiles_of(p.one.m, p.one.n, projects(kEpi) ? kTile / 2 : kTile), rest = tiles % kPairs;
   p.cut = rest == 0 || 2 * rest > kPairs ? 1 : projects(kEpi) || 4 * rest > kPairs ? 2 : 4;
   p.whole = p.cut == 1 ? tiles : tiles - rest;
   p.tiles = p.whole + (tiles - p.whole) * p.cut;
-  const int pairs = p.tiles < kPairs ? p.tiles : kPairs;
+  p.slices = 1;
+}
+
+template <typename T, bool kAMn, bool kBMn, Epilogue kEpi>
+int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
+  const long long items = (long long)p.tiles * p.slices;
+  const int pairs = (int)(items < kPairs ? items : kPairs);
   if constexpr (kEpi == kStore) return launch_kernel<T, kAMn, kBMn, kEpi, 0>(p, pairs, stream, what);
   else
     return activation == MF_ACT_SILU ? launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_SILU>(p, pairs, stream, what)
                                      : launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_GELU_TANH>(p, pairs, stream, what);
+}
+
+// ---- few tiles over a long dimension -------------------------------------------------------------------------------
+// The output product of some hundred tokens: a few tiles for 74 pairs, each over all hidden channels.  Cut into narrower tiles they would
+// still leave pairs idle and give the others less of the weights at a time; cut along the hidden channels, every pair reads a share of the
+// weights at full width, and a second launch adds the planes and the bias.  33 tokens, 1024 x 4096: 27 -> 20 us, 2048 x 8192: 47 -> 32,
+// 4096 x 10 928: 83 -> 68.  Estimated in clocks: a block of 64 channels takes 560,
+// 300, 250 at 256, 128, 64 columns, the second launch 6000 and a clock for every 2500 bytes of planes written and read.
+struct Slices {
+  int cut, slices;
+};
+Slices slices_of(long long m, long long n, long long k) {
+  const int tiles = tiles_of(m, n, kTile), k_blocks = (int)((k + kBlockK - 1) / kBlockK);
+  Slices best = {0, 1};
+  if (tiles > kPairs / 2) return best;
+  const double clocks[5] = {0, 560, 300, 0, 250};
+  const int cut = 4 * tiles <= kPairs ? 4 : 2;
+  double least = (double)k_blocks * clocks[cut];
+  for (int c = 1; c <= 2; c *= 2)
+    for (int s = 2; tiles * c * s <= kPairs && 2 * s <= k_blocks; ++s) {
+      const int per = (k_blocks + s - 1) / s;
+      if ((k_blocks + per - 1) / per != s) continue;
+      const double t = per * clocks[c] + 6000. + 8. * (double)m * n * s / 2500.;
+      if (t < least) least = t, best = {c, s};
+    }
+  return best;
+}
+size_t slice_bytes(long long m, long long n, long long k) {
+  const Slices s = slices_of(m, n, k);
+  return s.slices > 1 ? (size_t)s.slices * m * n * 4 : 0;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) add_slices_kernel(const float* __restrict__ planes, int slices, long long values, int n, const T* __restrict__ bias,
+                                                         T* __restrict__ out) {
+  wait_for_previous();
+  const long long i = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  if (i >= values) return;
+  float4 s = *reinterpret_cast<const float4*>(planes + i);
+#pragma unroll 4
+  for (int k = 1; k < slices; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(planes + k * values + i);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  if (bias) {
+    const uint2 w = *reinterpret_cast<const uint2*>(bias + i % n);
+    const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+    s.x += a.x, s.y += a.y, s.z += b.x, s.w += b.y;
+  }
+  *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
+}
+
+// out (m, n) = A B^T + bias, in slices where that pays and `planes` is given.
+template <typename T, bool kBMn>
+int store_product(Params& p, const T* bias, T* out, float* planes, cudaStream_t stream, const char* what) {
+  const long long m = p.one.m, n = p.one.n;
+  cut_tiles<kStore>(p);
+  const Slices s = planes ? slices_of(m, n, p.k) : Slices{0, 1};
+  if (s.slices > 1) {
+    p.cut = s.cut, p.whole = 0, p.tiles = tiles_of(m, n, kTile) * s.cut, p.slices = s.slices;
+    const long long dims[3] = {n, m, s.slices}, strides[2] = {4 * n, 4 * n * m};
+    MF_MAP(make_tensor_map(&p.pre, planes, MF_DTYPE_F32, 3, dims, strides, 32, 32));
+  } else {
+    p.bias = bias;
+  }
+  MF_MAP(map16<T>(&p.one.out, out, m, n, n, 32));
+  const int rc = launch<T, false, kBMn, kStore>(p, 0, stream, what);
+  if (rc != MF_OK || s.slices == 1) return rc;
+  launch_dependent(add_slices_kernel<T>, dim3((unsigned)((m * n / 4 + 255) / 256)), dim3(256), 0, stream, planes, s.slices, m * n, (int)n, bias, out);
+  MF_CHECK_LAUNCH("add_slices_kernel");
+  return MF_OK;
 }
 
 // ---- gradients of the weights and of the input ---------------------------------------------------------------------
@@ -194,14 +279,6 @@ Params common(long long m, long long n, long long k, const BoundedWaits& waits) 
   return p;
 }
 
-#define MF_MAP(call)                                                                                           \
-  do {                                                                                                         \
-    if (!(call)) {                                                                                             \
-      set_error("%s: tensor map refused (driver code %d)", kName, last_tensor_map_result());                   \
-      return MF_ERR_CUDA;                                                                                      \
-    }                                                                                                          \
-  } while (0)
-
 uint2* exponents_of(const MfGatedMlpArgs* a) { return reinterpret_cast<uint2*>(static_cast<char*>(a->pre) + gated_mlp_pre_values(a->rows, a->hidden)); }
 
 template <typename T>
@@ -219,15 +296,15 @@ int forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t str
     MF_MAP(map16<T>(&p.pre, a->pre, M, F, 2 * F, 32, 32));
     MF_MAP(map16<T>(&p.pre2, static_cast<T*>(a->pre) + F, M, F, 2 * F, 32, 32));
   }
+  cut_tiles<kGate>(p);
   int rc = a->pre ? launch<T, false, false, kGateKeep>(p, a->activation, stream, "gated_mlp gate product")
                   : launch<T, false, false, kGate>(p, a->activation, stream, "gated_mlp gate product");
   if (rc != MF_OK) return rc;
   p = common(M, O, F, waits);
-  p.bias = a->b_out;
   MF_MAP(map16<T>(&p.one.a, a->act, M, F, F, 64));
   MF_MAP(map16<T>(&p.one.b, a->w_out, O, F, F, 64));
-  MF_MAP(map16<T>(&p.one.out, a->y, M, O, O, 32));
-  return launch<T, false, false, kStore>(p, 0, stream, "gated_mlp output product");
+  float* planes = a->workspace && a->workspace_bytes >= slice_bytes(M, O, F) ? static_cast<float*>(a->workspace) : nullptr;
+  return store_product<T, false>(p, static_cast<const T*>(a->b_out), static_cast<T*>(a->y), planes, stream, "gated_mlp output product");
 }
 
 // One of the two weight gradients: the sum over the tokens of left (tokens, m) x right (tokens, n).
@@ -300,6 +377,7 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
     MF_MAP(map16<T>(&p.pre2, static_cast<const T*>(a->pre) + F, M, F, 2 * F, 32));
     MF_MAP(map16<T>(&p.one.out, grad_pre, M, F, 2 * F, 32));
     MF_MAP(map16<T>(&p.out2, grad_pre + F, M, F, 2 * F, 32));
+    cut_tiles<kGateGrad>(p);
     if ((rc = launch<T, false, true, kGateGrad>(p, a->activation, stream, "gated_mlp gate gradient")) != MF_OK) return rc;
   }
   if (a->grad_w_in || a->grad_w_out) {
@@ -308,8 +386,7 @@ int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t st
     Params p = common(M, C, 2 * F, waits);
     MF_MAP(map16<T>(&p.one.a, grad_pre, M, 2 * F, 2 * F, 64));
     MF_MAP(map16<T>(&p.one.b, a->w_in, 2 * F, C, C, 64));
-    MF_MAP(map16<T>(&p.one.out, a->grad_x, M, C, C, 32));
-    if ((rc = launch<T, false, true, kStore>(p, 0, stream, "gated_mlp input gradient")) != MF_OK) return rc;
+    if ((rc = store_product<T, true>(p, nullptr, static_cast<T*>(a->grad_x), nullptr, stream, "gated_mlp input gradient")) != MF_OK) return rc;
   }
   if (!biased) return MF_OK;
   if (!a->grad_w_in && !a->grad_w_out) {
@@ -328,7 +405,7 @@ int run_forward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t
   const int rc = check(a);
   if (rc != MF_OK || a->rows == 0) return rc;
   MF_CHECK_ARG(a->y, "%s: null tensor", kName);
-  if (a->rows <= kSmallRows && waits.withheld < 0) return gated_mlp_small_forward(a, stream);
+  if (gated_mlp_small(a) && waits.withheld < 0) return gated_mlp_small_forward(a, stream);
   return a->dtype == MF_DTYPE_BF16 ? forward<__nv_bfloat16>(a, waits, stream) : forward<__half>(a, waits, stream);
 }
 
@@ -372,6 +449,10 @@ using namespace mf;
 
 extern "C" size_t mf_gated_mlp_pre_bytes(int64_t rows, int32_t hidden) {
   return rows < 0 || hidden < 1 ? 0 : gated_mlp_pre_values(rows, hidden) + (size_t)rows * ((hidden + 63) / 64) * 8;
+}
+extern "C" size_t mf_gated_mlp_fwd_workspace_bytes(const MfGatedMlpArgs* a) {
+  if (!a || a->hidden < 1 || a->dim < 1 || a->dim_out < 1 || gated_mlp_small(a)) return 0;
+  return slice_bytes(a->rows, a->dim_out, a->hidden);
 }
 extern "C" size_t mf_gated_mlp_bwd_workspace_bytes(const MfGatedMlpArgs* a) {
   if (!a || a->rows < 0 || a->hidden < 1 || a->dim < 1 || a->dim_out < 1) return 0;

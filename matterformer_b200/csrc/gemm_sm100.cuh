@@ -82,6 +82,7 @@ struct Params {
   float* column_sums;       // kGateGrad: (ceil(m / 32), 2 n) sums of the stored rows, or null
   int k;
   int whole, cut, tiles;    // tiles of full width, columns of a later one = full width / cut, pieces of work in all
+  int slices;               // kStore: pieces of the contracted dimension, each with a plane (m, n) of partial sums in `pre`; 1: none
   // kGradients.  The weights' tiles: how many, the first, the first of the second product; in how many pieces their contracted dimension
   // is cut, and how many blocks a piece has.  The input's: its contracted dimension, and how many tiles the pairs without a weight tile
   // in the last round of those do meanwhile, each of them `ahead`; whole, cut and tiles are of the others.
@@ -354,10 +355,16 @@ struct Walk {
       w.row = tile / tiles_n * kTile, w.col = tile % tiles_n * kTile + part * w.cols;
       return true;
     } else {
-      if (t >= p.tiles) return false;
-      const bool whole = t < p.whole;
-      int m, n;
-      const int part = whole ? 0 : (t - p.whole) % p.cut, tile = whole ? t : p.whole + (t - p.whole) / p.cut;
+      const int slices = kEpi == kStore ? p.slices : 1;
+      if (t >= p.tiles * slices) return false;
+      int m, n, u = t;
+      if (slices > 1) {
+        const int per = (k_blocks + slices - 1) / slices;
+        w.plane = t / p.tiles, u = t - w.plane * p.tiles;
+        w.k0 = w.plane * per, w.k1 = min(k_blocks, w.k0 + per);
+      }
+      const bool whole = u < p.whole;
+      const int part = whole ? 0 : (u - p.whole) % p.cut, tile = whole ? u : p.whole + (u - p.whole) / p.cut;
       if (!whole) w.cols = full() / p.cut;
       tile_at(tile, tiles_m, tiles_n, m, n);
       w.col = n * full() + part * w.cols;
@@ -704,7 +711,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         if (bad) break;
       } else {
         const Problem& prob = problem(w);
-        if (kEpi == kGradients && w.which != kInput && (w.plane >= 0 || p.wide_out)) {  // 32 fp32 columns at a time: a part of a tile, or an fp32 result
+        const bool sliced = kEpi == kStore && w.plane >= 0;
+        if (sliced || (kEpi == kGradients && w.which != kInput && (w.plane >= 0 || p.wide_out))) {  // 32 fp32 columns at a time: partial sums, or an fp32 result
 #pragma unroll 1
           for (int c = 0; c < 2 * chunks; ++c) {
             uint32_t d[32];
@@ -714,7 +722,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             emptied();
             put(buffers, d);
             if (lane == 0 && row0 < prob.m && col0 + 32 * c < prob.n) {
-              if (w.plane >= 0) store_box(&p.pre, buffers, first + 32 * c, w.plane * kTile + lane_row);
+              if (sliced) store_box3(&p.pre, buffers, col0 + 32 * c, row0, w.plane);
+              else if (w.plane >= 0) store_box(&p.pre, buffers, first + 32 * c, w.plane * kTile + lane_row);
               else store_box(&prob.out, buffers, col0 + 32 * c, row0);
               store_commit();
             }

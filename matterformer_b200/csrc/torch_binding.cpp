@@ -379,6 +379,8 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     const Tensor y = at::empty(shape, x.options()), act = at::empty({a.rows, a.hidden}, x.options());
     const Tensor pre = keep ? at::empty({(int64_t)mf_gated_mlp_pre_bytes(a.rows, a.hidden)}, x.options().dtype(at::kByte)) : Tensor();
     a.y = y.data_ptr(), a.act = act.data_ptr(), a.pre = keep ? pre.data_ptr() : nullptr;
+    const Tensor ws = bytes(mf_gated_mlp_fwd_workspace_bytes(&a), x);
+    if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
     check(mf_gated_mlp_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
     if (keep) {
       ctx->saved_data["activation"] = activation;

@@ -55,7 +55,12 @@ class _GatedMlp(torch.autograd.Function):
         pre = torch.empty(_lib.lib().mf_gated_mlp_pre_bytes(rows, F), device=x.device, dtype=torch.uint8) if keep else None
         a = _args(x2, *params, activation, ctx.grad_dtype)
         a.pre, a.act, a.y = _ptr(pre), _ptr(act), _ptr(y)
-        _lib.launch(_lib.lib().mf_gated_mlp_fwd, x.device, ctypes.byref(a))
+        L = _lib.lib()
+        need = L.mf_gated_mlp_fwd_workspace_bytes(ctypes.byref(a))
+        if need:
+            ws = torch.empty(need, device=x.device, dtype=torch.uint8)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        _lib.launch(L.mf_gated_mlp_fwd, x.device, ctypes.byref(a))
         if keep:
             ctx.foreign = _lib.foreign_leaves(x, w_in, w_out, b_in, b_out)
             ctx.save_for_backward(x2, *params, pre, act)

@@ -53,7 +53,8 @@ def _run(ops, dy, act):
 
 
 SIZES = [(1, 8, 8, 8), (7, 64, 128, 64), (29, 512, 2048, 512), (128, 72, 136, 200), (129, 512, 1368, 512), (257, 200, 72, 328), (300, 1024, 264, 512),
-         (1000, 520, 1032, 264), (4096, 64, 256, 64), (9, 4096, 80, 2048)]  # fmt: skip
+         (1000, 520, 1032, 264), (4096, 64, 256, 64), (9, 4096, 80, 2048),
+         (100, 64, 8200, 520), (30, 512, 8192, 72), (500, 72, 4104, 264)]  # (few tiles over many hidden channels: in slices)  # fmt: skip
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
