@@ -365,6 +365,9 @@ extern "C" int mf_rotary(const MfRotaryArgs* a, void* stream) {
   for (int i = 0; i < a->tensors; ++i) {
     const MfRotaryTensor& t = a->tensor[i];
     MF_CHECK_ARG(t.heads >= 0, "%s: negative size", name);
+    // (a warp counts the pieces of its eight tokens' heads in 32 bits)
+    MF_CHECK_ARG((long long)t.heads * a->head_dim <= 1 << 27, "%s: %d heads of %d channels, more than 2^27 elements a token", name, (int)t.heads,
+                 (int)a->head_dim);
     if (t.heads == 0 || places == 0) continue;
     MF_CHECK_ARG(t.in && t.out, "%s: null tensor", name);
     MF_CHECK_ARG(reinterpret_cast<uintptr_t>(t.in) % size == 0 && reinterpret_cast<uintptr_t>(t.out) % size == 0, "%s: unaligned tensor", name);

@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <mutex>
@@ -453,7 +454,7 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
 struct Rotary : torch::autograd::Function<Rotary> {
   // heads 0: one or two head-major tensors; otherwise a packed projection with that many heads
   static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads,
-                             int64_t layout, double amplitude, bool inverse, bool foreign) {
+                             int64_t layout, double amplitude, bool inverse, bool keep, bool foreign) {
     const c10::cuda::CUDAGuard guard(first.device());
     auto adjacent = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
     const Tensor x[2] = {adjacent(first), second ? adjacent(*second) : Tensor()};
@@ -467,6 +468,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     for (const Tensor& t : x) {
       if (!t.defined()) continue;
       out.push_back(at::empty_like(t));
+      if (out.back().stride(-1) != 1) out.back() = at::empty(t.sizes(), t.options());  // (overlapping inputs may have another order)
       const Tensor& o = out.back();
       a.batch = t.size(0), a.tokens = t.size(heads ? 1 : 2), a.head_dim = heads ? t.size(2) / (3 * heads) : t.size(3);
       if (heads)
@@ -483,22 +485,27 @@ struct Rotary : torch::autograd::Function<Rotary> {
     a.frequencies = table.const_data_ptr<double>();
     check(mf_rotary(&a, c10::cuda::getCurrentCUDAStream().stream()));
     ctx->set_materialize_grads(false);
-    ctx->saved_data["positions"] = positions;
-    ctx->saved_data["table"] = table;
+    if (keep) {
+      ctx->save_for_backward({positions.is_inference() ? positions.clone() : positions});
+      ctx->saved_data["table"] = table.clone();  // (the caller's may have changed by then)
+    }
     ctx->saved_data["heads"] = heads, ctx->saved_data["layout"] = layout, ctx->saved_data["amplitude"] = amplitude, ctx->saved_data["inverse"] = inverse;
     ctx->saved_data["foreign"] = foreign;
     return out;
   }
 
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    tensor_list given, g(9);
+    tensor_list given, g(10);
     refuse_foreign(ctx->saved_data["foreign"].toBool(), "rotary_embedding");
     for (const Tensor& t : grads)
       if (t.defined()) given.push_back(t);
     if (given.empty()) return g;
     auto& s = ctx->saved_data;
-    const tensor_list turned = Rotary::apply(given[0], given.size() > 1 ? OptTensor(given[1]) : std::nullopt, s["positions"].toTensor(), s["table"].toTensor(),
-                                             s["heads"].toInt(), s["layout"].toInt(), s["amplitude"].toDouble(), !s["inverse"].toBool(), false);
+    const Tensor positions = ctx->get_saved_variables()[0];
+    bool keep = false;
+    for (const Tensor& t : given) keep = keep || (at::GradMode::is_enabled() && t.requires_grad());
+    const tensor_list turned = Rotary::apply(given[0], given.size() > 1 ? OptTensor(given[1]) : std::nullopt, positions, s["table"].toTensor(),
+                                             s["heads"].toInt(), s["layout"].toInt(), s["amplitude"].toDouble(), !s["inverse"].toBool(), keep, false);
     for (size_t i = 0, j = 0; i < grads.size(); ++i)
       if (grads[i].defined()) g[i] = turned[j++];
     return g;
@@ -513,6 +520,7 @@ std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, 
   if (second && (second->dim() != 4 || second->scalar_type() != first.scalar_type() || second->device() != first.device() || second->numel() == 0 ||
                  second->size(0) != B || second->size(2) != N || second->size(3) != D))
     return std::nullopt;
+  if (B >= 1ll << 31 || N >= 1ll << 31 || (heads ? heads : std::max(first.size(1), second ? second->size(1) : 0)) * D > 1 << 27) return std::nullopt;
   if (!table.device().is_cpu() || table.scalar_type() != at::kDouble || !table.is_contiguous() || table.dim() < 1 || table.dim() > 2 || table.requires_grad() ||
       table.numel() < 1 || table.numel() > 128 || 2 * table.numel() > D)
     return std::nullopt;
@@ -526,7 +534,8 @@ std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, 
   if (first._fw_grad(0).defined() || (second && second->_fw_grad(0).defined())) return std::nullopt;
   const Tensor none;
   const c10::cuda::CUDAGuard guard(first.device());
-  return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false, foreign_leaves({&first, second ? &*second : &none}));
+  const bool keep = at::GradMode::is_enabled() && (first.requires_grad() || (second && second->requires_grad()));
+  return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false, keep, foreign_leaves({&first, second ? &*second : &none}));
 }
 
 }  // namespace

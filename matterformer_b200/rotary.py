@@ -98,12 +98,15 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b, positions, table, heads, layout, amplitude, inverse):
         ctx.set_materialize_grads(False)
-        ctx.call = (positions, table, heads, layout, amplitude, inverse)
+        ctx.save_for_backward(positions.clone() if positions.is_inference() else positions)
+        ctx.call = (table.clone(), heads, layout, amplitude, inverse)  # (the caller's table may have changed by then)
         ctx.foreign = _lib.foreign_leaves(a, b)
         args = _lib.MfRotaryArgs()
         tensors = [t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (a, b)]
         x = next(t for t in tensors if t is not None)
         outs = [None if t is None else torch.empty_like(t) for t in tensors]
+        # (overlapping inputs may have another order)
+        outs = [o if o is None or o.stride(-1) == 1 else torch.empty(o.shape, dtype=o.dtype, device=o.device) for o in outs]
         if heads:
             args.batch, args.tokens = x.shape[:2]
             args.head_dim, args.tensors = x.shape[2] // (3 * heads), 3
@@ -129,7 +132,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         _lib.refuse_foreign(ctx.foreign, "rotary_embedding")
-        positions, table, heads, layout, amplitude, inverse = ctx.call
+        (positions,), (table, heads, layout, amplitude, inverse) = ctx.saved_tensors, ctx.call
         given = [g for g in grads if g is not None]  # (one of two outputs may be unused)
         out = [None] * 8
         if given:
@@ -140,7 +143,7 @@ class _Rotary(torch.autograd.Function):
         return tuple(out)
 
 
-def _check(name, tensors, tokens, batch, head_dim, positions, frequencies, layout, amplitude):
+def _check(name, tensors, tokens, batch, heads, head_dim, positions, frequencies, layout, amplitude):
     x = tensors[0]
     if any(t.device.type != "cuda" for t in tensors):
         raise RuntimeError(f"{name} requires CUDA tensors")
@@ -148,6 +151,8 @@ def _check(name, tensors, tokens, batch, head_dim, positions, frequencies, layou
         raise RuntimeError(f"{name} only supports float16/bfloat16/float32 inputs, got {x.dtype}")
     if any(t.dtype != x.dtype or t.device != x.device for t in tensors):
         raise ValueError(f"{name}: tensors must share their type and device")
+    if max(batch, tokens) >= 2**31 or heads * head_dim > 2**27:
+        raise ValueError(f"{name}: fewer than 2^31 batch entries and tokens and at most 2^27 elements a token, got {batch}, {tokens} and {heads * head_dim}")
     if layout not in _lib.MF_ROTARY:
         raise ValueError(f"{name}: layout must be one of {sorted(_lib.MF_ROTARY)}, got {layout!r}")
     if not math.isfinite(amplitude):
@@ -194,7 +199,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     tensors = [t for t in (q, k) if t is not None]
     if any(t.ndim != 4 for t in tensors) or (k is not None and (k.shape[0], k.shape[2:]) != (q.shape[0], q.shape[2:])):
         raise ValueError(f"rotary_embedding: q (B, H, N, D) and k (B, K, N, D) expected, got {[tuple(t.shape) for t in tensors]}")
-    _check("rotary_embedding", tensors, q.shape[2], q.shape[0], q.shape[3], positions, frequencies, layout, amplitude)
+    _check("rotary_embedding", tensors, q.shape[2], q.shape[0], max(t.shape[1] for t in tensors), q.shape[3], positions, frequencies, layout, amplitude)
     out = _apply(q, k, positions, frequencies, 0, layout, amplitude)
     return (out, None) if k is None else out
 
@@ -207,5 +212,5 @@ def rotary_packed(qkv: torch.Tensor, heads: int, positions: torch.Tensor, freque
         return out[0]
     if qkv.ndim != 3 or heads < 1 or qkv.shape[2] % (3 * heads) or qkv.shape[2] == 0:
         raise ValueError(f"rotary_packed: qkv (B, N, 3*H*D) with H = {heads} expected, got {tuple(qkv.shape)}")
-    _check("rotary_packed", [qkv], qkv.shape[1], qkv.shape[0], qkv.shape[2] // (3 * heads), positions, frequencies, layout, amplitude)
+    _check("rotary_packed", [qkv], qkv.shape[1], qkv.shape[0], heads, qkv.shape[2] // (3 * heads), positions, frequencies, layout, amplitude)
     return _apply(qkv, None, positions, frequencies, int(heads), layout, amplitude)

@@ -78,6 +78,11 @@ def test_rotary_arguments(over, message):
     assert message in _lib.last_error()
 
 
+def test_rotary_elements_a_token():
+    assert _lib.lib().mf_rotary(ctypes.byref(_rotary(heads=2**23 + 1)), None) == _lib.MF_ERR_INVALID_ARGUMENT
+    assert "more than 2^27 elements a token" in _lib.last_error()
+
+
 def test_rotary_nothing_to_do():
     L = _lib.lib()
     assert L.mf_rotary(None, None) == _lib.MF_ERR_INVALID_ARGUMENT

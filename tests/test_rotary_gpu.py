@@ -244,3 +244,50 @@ def test_many_tokens_and_large_offsets():
     pos = torch.arange(N).cuda()
     y, _ = mfb.rotary_embedding(x, None, pos, table)
     assert torch.equal(y, mfb.rotary_embedding(x.contiguous(), None, pos, table)[0])
+
+
+@pytest.mark.parametrize("inference", [False, True])
+@pytest.mark.parametrize("how", ["native", "python"])
+def test_positions_and_table_changed_before_the_backward_pass(how, inference, monkeypatch):
+    """A changed table does not reach the gradient; changed positions are an error, or kept if nothing notes their changes."""
+    if how == "python":
+        monkeypatch.setattr(mfb._lib, "native", lambda: None)
+    g = torch.Generator().manual_seed(9)
+    with torch.inference_mode(inference):
+        table, pos = mfb.rotary_frequencies(32), torch.arange(5).cuda()
+    x, dy = _randn(g, 2, 3, 5, 32, dtype=F32).requires_grad_(), _randn(g, 2, 3, 5, 32, dtype=F32)
+    want = torch.autograd.grad(mfb.rotary_embedding(x, None, pos, table)[0], x, dy)[0]
+    y = mfb.rotary_embedding(x, None, pos, table)[0]
+    with torch.inference_mode(inference):
+        table.mul_(2)
+    assert torch.equal(torch.autograd.grad(y, x, dy, retain_graph=True)[0], want)
+    with torch.inference_mode(inference):
+        pos.add_(1)
+    if inference:
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+    else:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, x, dy)
+
+
+@pytest.mark.parametrize("how", ["native", "python"])
+def test_overlapping_windows(how, monkeypatch):
+    """Tokens one element apart: their channels are adjacent, and no dense result has the same order of strides."""
+    if how == "python":
+        monkeypatch.setattr(mfb._lib, "native", lambda: None)
+    g = torch.Generator().manual_seed(10)
+    x = _randn(g, 2, 3, 75, dtype=F32).unfold(-1, 16, 1)
+    table, pos = mfb.rotary_frequencies(16), torch.arange(60).cuda()
+    y, z = mfb.rotary_embedding(x, x[:, :1].expand(2, 4, 60, 16), pos, table)
+    _close(y, _exact(x, pos, table, "half"), 1.5 * x.abs().max().item())
+    assert torch.equal(z, y[:, :1].expand(2, 4, 60, 16))
+
+
+def test_sizes_beyond_the_kernel_are_refused():
+    table, pos = mfb.rotary_frequencies(2), torch.zeros(1, device="cuda")
+    x = torch.zeros(1, 1, 1, 2, device="cuda")
+    for shape in ((2**31, 1, 1, 2), (2**32 + 1, 1, 1, 2), (1, 2**32 + 1, 1, 2), (1, 2**26 + 1, 1, 2)):
+        with pytest.raises(ValueError, match="at most 2\\^27 elements a token"):
+            mfb.rotary_embedding(x.expand(shape), None, pos, table)
+        with pytest.raises(ValueError, match="at most 2\\^27 elements a token"):
+            mfb.rotary_embedding(x, x.expand(shape), pos, table) if shape[0] == 1 else mfb.rotary_embedding(x.expand(shape), x.expand(shape), pos, table)
