@@ -29,8 +29,9 @@ namespace gemm {
 
 __device__ int32_t g_gemm_status = 0;  // MF_ERR_DEVICE_TIMEOUT after an expired wait
 
-// kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well;  kGateGrad: its gradient;  kStore: the product and a bias;  kGradients: the
-// weights' gradients, two products over the same long dimension (of operands that have it outermost), and the input's, side by side
+// kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well; kGateGrad: the gradient of both;
+// kStore: the product and a bias; kGradients: the weights' gradients, two products over the same long dimension (of operands that have it
+// outermost), and the input's, side by side
 enum Epilogue { kGate, kGateKeep, kGateGrad, kStore, kGradients };
 __host__ __device__ constexpr bool projects(Epilogue e) { return e == kGate || e == kGateKeep; }
 
@@ -170,11 +171,6 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 
@@ -691,6 +687,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               sts128(up + box_chunk(lane, 2 * q + v), make_uint4(du[0], du[1], du[2], du[3]));
             }
           }
+          if (row0 + lane >= p.one.m) {  // rows beyond the last: zeros times an infinite weight are not zeros
+#pragma unroll
+            for (int v = 0; v < 8; ++v) sts128(gate + box_chunk(lane, v), make_uint4(0u, 0u, 0u, 0u)), sts128(up + box_chunk(lane, v), make_uint4(0u, 0u, 0u, 0u));
+          }
           fence_smem_to_async_proxy();
           __syncwarp();
           const int col = col0 + 64 * c;
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             store_box(&p.out2, up, col, row0);
             store_commit();
           }
-          if (p.column_sums && row0 < p.one.m) {  // of the values as stored (rows beyond the last are zeros)
+          if (p.column_sums && row0 < p.one.m) {  // of the values as stored
             const float2 dg = column_sums32<T>(gate, lane), du = column_sums32<T>(up, lane);
             const int at = col + 16 * (lane & 3) + (lane >> 2);
             float* to = p.column_sums + (size_t)(row0 >> 5) * (2 * (size_t)p.one.n) + at;

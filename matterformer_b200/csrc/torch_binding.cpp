@@ -432,7 +432,7 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
   if (!x.is_cuda() || x.dim() < 1 || (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kHalf) || !x.is_contiguous() || x.numel() == 0) return std::nullopt;
   if (w_out.dim() != 2) return std::nullopt;
   const int64_t C = x.size(-1), O = w_out.size(0), F = w_out.size(1);
-  if (C % 8 || O % 8 || F % 8 || C < 8 || O < 8 || F < 8) return std::nullopt;
+  if (C % 8 || O % 8 || F % 8 || C < 8 || O < 8 || F < 8 || std::max({C, O, F}) > 1 << 28) return std::nullopt;
   const at::ScalarType type = x.scalar_type();
   if (!ready(w_in, x, type, {2 * F, C}) || !ready(w_out, x, type, {O, F}) || (b_in && !ready(*b_in, x, type, {2 * F})) ||
       (b_out && !ready(*b_out, x, type, {O})))

@@ -103,7 +103,7 @@ def gated_mlp_applies(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) 
     multiples of 8."""
     return (x.is_cuda and x.dtype in _CODE and w_in.ndim == w_out.ndim == 2 and w_in.dtype == w_out.dtype
             and (w_in.dtype == x.dtype or (w_in.dtype == torch.float32 and x.dtype == torch.bfloat16))
-            and all(n % 8 == 0 and n > 0 for n in (w_in.shape[1], w_out.shape[1], w_out.shape[0])))  # fmt: skip
+            and all(n % 8 == 0 and 0 < n <= 2**28 for n in (w_in.shape[1], w_out.shape[1], w_out.shape[0])))  # fmt: skip
 
 
 def _check(x, w_in, w_out, b_in, b_out, activation):
@@ -124,8 +124,8 @@ def _check(x, w_in, w_out, b_in, b_out, activation):
                          f"{tuple(w_out.shape)}")  # fmt: skip
     if (b_in is not None and b_in.shape != w_in.shape[:1]) or (b_out is not None and b_out.shape != w_out.shape[:1]):
         raise ValueError("gated_mlp: b_in must have shape (2 F,) and b_out (O,)")
-    if any(n < 8 or n % 8 for n in (x.shape[-1], *w_out.shape)):
-        raise ValueError(f"gated_mlp: widths must be positive multiples of 8, got C={x.shape[-1]}, F={w_out.shape[1]}, O={w_out.shape[0]}")
+    if any(n < 8 or n % 8 or n > 2**28 for n in (x.shape[-1], *w_out.shape)):
+        raise ValueError(f"gated_mlp: widths must be positive multiples of 8 up to 2^28, got C={x.shape[-1]}, F={w_out.shape[1]}, O={w_out.shape[0]}")
 
 
 def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Optional[torch.Tensor] = None,
@@ -134,9 +134,10 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     ``x``'s type, or fp32 beside a bf16 ``x`` (their bf16 copies compute, their gradients are fp32; see
     :func:`matterformer_b200.linear.bf16_copies`).  ``activation``: "silu" or "gelu_tanh".  Returns (..., O) in ``x``'s type.
 
-    Sums are in fp32 in a fixed order.  The hidden values and the gradients of the pre-activations are rounded to ``x``'s type, what the
-    backward pass gets of the pre-activations to some bits more; hidden values that
-    fp16 cannot hold (above 65504) are infinities there.  C, F and O are multiples of 8.  The gradient is once differentiable."""
+    Sums are in fp32 in a fixed order.  The hidden values and the gradients of the pre-activations are rounded to ``x``'s type; hidden values
+    that fp16 cannot hold (above 65504) are infinities there.  What the backward pass gets of the pre-activations has some bits more than
+    ``x``'s type, counted from the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-29 of that (bf16), 13 down to 2^-7 of
+    it and a bit less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable."""
     native = _lib.native()
     if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++
         out = native.gated_mlp(x, w_in, w_out, b_in, b_out, ACTIVATIONS[activation])

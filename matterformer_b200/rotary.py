@@ -40,7 +40,7 @@ def rotary_frequencies(rotary_dim: int, *, axes: int = 1, base: float = 10000.0,
     pairs = rotary_dim // (2 * axes)
     if scaling == "ntk" and pairs > 1:
         base = base * factor ** (pairs / (pairs - 1))
-    theta = base ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+    theta = base ** (-torch.arange(pairs, dtype=torch.float64, device="cpu") / pairs)
     if scaling == "linear" or (scaling == "ntk" and pairs == 1):
         theta = theta / factor
     elif scaling == "parts":

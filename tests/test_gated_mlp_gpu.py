@@ -320,3 +320,27 @@ def test_pre_activations_of_different_sizes(rows, dtype):
         size = b.norm(dim=1, keepdim=True) / b.shape[1] ** 0.5
         off = (a.double() - b).norm(dim=1) / (size.squeeze(1) * b.shape[1] ** 0.5).clamp_min(1e-300)
         assert (off[size.squeeze(1) > tiny] < 2 * _bound(dtype)).all()
+
+
+@pytest.mark.parametrize("rows", [7, 33, 300])
+def test_infinite_weight_and_the_rows_behind_the_last(rows):
+    """An infinite weight makes its channel's gradients infinite; the tile's rows behind the last token, where it meets zeros, add nothing."""
+    ops, dy = _operands(rows, 64, 72, 80, BF16, True, seed=40)
+    ops[1] *= 0.01
+    ops[3].fill_(2.0)  # positive pre-activations and slopes
+    dy = dy.abs() + 0.1
+    leaves = [t.detach().requires_grad_(i == 3) for i, t in enumerate(ops)]
+    clean = torch.autograd.grad(mfb.gated_mlp(*leaves), leaves[3], dy)[0]
+    leaves[2].data[0, 5] = float("inf")
+    got = torch.autograd.grad(mfb.gated_mlp(*leaves), leaves[3], dy)[0]
+    assert got[5] == got[72 + 5] == float("inf")
+    others = torch.ones(144, dtype=torch.bool)
+    others[[5, 77]] = False
+    assert torch.equal(got[others], clean[others])
+
+
+def test_widths_beyond_the_kernel_are_refused():
+    wide, w = torch.zeros(1, 1, dtype=BF16, device="cuda").expand(1, 2**32 + 8), torch.zeros(8, 8, dtype=BF16, device="cuda")
+    assert not gated.gated_mlp_applies(wide, wide.expand(16, -1), w)
+    with pytest.raises(ValueError, match="up to 2\\^28"):
+        mfb.gated_mlp(wide, wide.expand(16, -1), w)

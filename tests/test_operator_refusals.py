@@ -109,6 +109,11 @@ def test_frequencies():
             mfb.rotary_frequencies(**bad)
 
 
+def test_frequencies_stay_on_the_host():
+    with torch.device("meta"):
+        assert mfb.rotary_frequencies(8).device.type == mfb.RotaryPositions(8).frequencies.device.type == "cpu"
+
+
 def test_python_layer():
     x, w, v = torch.zeros(4, 16), torch.zeros(48, 16), torch.zeros(16, 24)
     with pytest.raises(RuntimeError, match="requires CUDA tensors"):
