@@ -369,10 +369,11 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     a.b_in = b_in.defined() ? b_in.const_data_ptr() : nullptr, a.b_out = b_out.defined() ? b_out.const_data_ptr() : nullptr;
   }
 
-  static Variable forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const OptTensor& b_in, const OptTensor& b_out,
-                          int64_t activation, bool keep, bool foreign) {
+  struct Made {
+    Tensor y, pre, act;
+  };
+  static Made block(const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& bi, const Tensor& bo, int64_t activation, bool keep) {
     const c10::cuda::CUDAGuard guard(x.device());
-    const Tensor bi = b_in ? *b_in : Tensor(), bo = b_out ? *b_out : Tensor();
     MfGatedMlpArgs a{};
     fill(a, x, w_in, w_out, bi, bo, activation);
     std::vector<int64_t> shape = x.sizes().vec();
@@ -383,12 +384,17 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     const Tensor ws = bytes(mf_gated_mlp_fwd_workspace_bytes(&a), x);
     if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
     check(mf_gated_mlp_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
-    if (keep) {
-      ctx->saved_data["activation"] = activation;
-      ctx->saved_data["foreign"] = foreign;
-      ctx->save_for_backward({x, w_in, w_out, bi, bo, pre, act});
-    }
-    return y;
+    return {y, pre, act};
+  }
+
+  static Variable forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const OptTensor& b_in, const OptTensor& b_out,
+                          int64_t activation, bool foreign) {
+    const Tensor bi = b_in ? *b_in : Tensor(), bo = b_out ? *b_out : Tensor();
+    const Made made = block(x, w_in, w_out, bi, bo, activation, true);
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["foreign"] = foreign;
+    ctx->save_for_backward({x, w_in, w_out, bi, bo, made.pre, made.act});
+    return made.y;
   }
 
   static tensor_list backward(AutogradContext* ctx, tensor_list grad_y) {
@@ -396,7 +402,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     const Tensor& x = s[0];
     const c10::cuda::CUDAGuard guard(x.device());
     MfGatedMlpArgs a{};
-    tensor_list g(8);  // (one for each argument of forward)
+    tensor_list g(7);  // (one for each argument of forward)
     refuse_foreign(ctx->saved_data["foreign"].toBool(), "gated_mlp");
     {
       const at::NoGradGuard no_grad;
@@ -443,9 +449,10 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
     keep = keep || t->requires_grad();
   }
   const Tensor none;
+  const Tensor &bi = b_in ? *b_in : none, &bo = b_out ? *b_out : none;
+  if (!keep || !at::GradMode::is_enabled()) return GatedMlp::block(x, w_in, w_out, bi, bo, activation, false).y;
   const c10::cuda::CUDAGuard guard(x.device());
-  const bool foreign = foreign_leaves({&x, &w_in, &w_out, b_in ? &*b_in : &none, b_out ? &*b_out : &none});
-  return GatedMlp::apply(x, w_in, w_out, b_in, b_out, activation, keep && at::GradMode::is_enabled(), foreign);
+  return GatedMlp::apply(x, w_in, w_out, b_in, b_out, activation, foreign_leaves({&x, &w_in, &w_out, &bi, &bo}));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -453,8 +460,8 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
 // ---------------------------------------------------------------------------------------------------------------------
 struct Rotary : torch::autograd::Function<Rotary> {
   // heads 0: one or two head-major tensors; otherwise a packed projection with that many heads
-  static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads,
-                             int64_t layout, double amplitude, bool inverse, bool keep, bool foreign) {
+  static tensor_list turn(const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads, int64_t layout,
+                          double amplitude, bool inverse) {
     const c10::cuda::CUDAGuard guard(first.device());
     auto adjacent = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
     const Tensor x[2] = {adjacent(first), second ? adjacent(*second) : Tensor()};
@@ -484,6 +491,12 @@ struct Rotary : torch::autograd::Function<Rotary> {
     a.positions = positions.const_data_ptr(), a.position_batch = positions.dim() == table.dim() + 1 ? positions.stride(0) : 0;
     a.frequencies = table.const_data_ptr<double>();
     check(mf_rotary(&a, c10::cuda::getCurrentCUDAStream().stream()));
+    return out;
+  }
+
+  static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads,
+                             int64_t layout, double amplitude, bool inverse, bool keep, bool foreign) {
+    const tensor_list out = turn(first, second, positions, table, heads, layout, amplitude, inverse);
     ctx->set_materialize_grads(false);
     if (keep) {
       ctx->save_for_backward({positions.is_inference() ? positions.clone() : positions});
@@ -535,6 +548,7 @@ std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, 
   const Tensor none;
   const c10::cuda::CUDAGuard guard(first.device());
   const bool keep = at::GradMode::is_enabled() && (first.requires_grad() || (second && second->requires_grad()));
+  if (!keep) return Rotary::turn(first, second, positions, table, heads, layout, amplitude, false);  // (past autograd: 9.1 -> 6.9 us a call)
   return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false, keep, foreign_leaves({&first, second ? &*second : &none}));
 }
 

@@ -173,10 +173,10 @@ def _check(name, tensors, tokens, batch, heads, head_dim, positions, frequencies
 
 def _ready(a, b, positions, frequencies, heads, layout, amplitude):
     """The whole call in C++ where that is built and the operands are ready as they are, else None."""
-    native = _lib.native()
-    if native is None or layout not in _lib.MF_ROTARY or not all(isinstance(t, torch.Tensor) for t in (a, positions, frequencies)):
+    native, code = _lib.native(), _lib.MF_ROTARY.get(layout)
+    if native is None or code is None or not (isinstance(positions, torch.Tensor) and isinstance(frequencies, torch.Tensor)):
         return None
-    return native.rotary(a, b, positions, frequencies, heads, _lib.MF_ROTARY[layout], float(amplitude))
+    return native.rotary(a, b, positions, frequencies, heads, code, amplitude)
 
 
 def _apply(a, b, positions, frequencies, heads, layout, amplitude):
