@@ -6,7 +6,9 @@
 // The backward pass is the same rotation by the opposite angle.  Every value is read and written once: memory bounds it.  A warp takes a few
 // tokens: its lanes form the tokens' cosines and sines, once for all heads of all tensors, into a table of the warp in shared memory, and
 // then move the tokens' rows, 16 bytes at a time where sizes, strides and addresses allow it, else 8, 4 or a single element.  Warps wait
-// for nobody, so that one's arithmetic hides behind the others' loads.
+// for nobody, so that one's arithmetic hides behind the others' loads.  Copies reach 6.5 TB/s; 20 heads of 128, 32 771 tokens, fp32: 117 us,
+// 5.7 TB/s; 32 x 8 + 8 interleaved heads of 64, 4096 tokens, bf16: 99 us, 5.4; packed projections of 1024 x 29 tokens, three axes, bf16: 44 us,
+// 4.1, where the angles of four tokens come before each warp's 12 KB.  (Its first loads before the angles: 50 us; that takes 117 registers.)
 //
 // Angles are formed in turns in 64 bits, position * (frequency / 2 pi), and lose their whole turns there: a position of a million
 // and a frequency of 1 would leave 4 digits of an angle in 32 bits.  What remains is at most half a turn: its sine and cosine are taken in
