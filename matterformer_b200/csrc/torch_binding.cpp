@@ -6,6 +6,7 @@
 // that way and takes 20.  These functions serve calls whose operands are
 // ready as they are (contiguous, on one device, of the types the kernels take) and return None for every other call, which
 // then takes the Python path with its conversions and error messages.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -359,6 +360,11 @@ void refuse_foreign(bool foreign, const char* name) {
 // ---------------------------------------------------------------------------------------------------------------------
 // Gated feed-forward block
 // ---------------------------------------------------------------------------------------------------------------------
+// A contiguous tensor without the way through the dispatcher, which takes as long again as the allocation.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(sizes, type, like.device(), at::MemoryFormat::Contiguous));
+}
+Tensor fresh_bytes(int64_t n, const Tensor& like) { return n ? fresh({n}, at::kByte, like) : Tensor(); }
 bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
 
 struct GatedMlp : torch::autograd::Function<GatedMlp> {
@@ -378,10 +384,10 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     fill(a, x, w_in, w_out, bi, bo, activation);
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = a.dim_out;
-    const Tensor y = at::empty(shape, x.options()), act = at::empty({a.rows, a.hidden}, x.options());
-    const Tensor pre = keep ? at::empty({(int64_t)mf_gated_mlp_pre_bytes(a.rows, a.hidden)}, x.options().dtype(at::kByte)) : Tensor();
+    const Tensor y = fresh(shape, x.scalar_type(), x), act = fresh({a.rows, a.hidden}, x.scalar_type(), x);
+    const Tensor pre = keep ? fresh_bytes((int64_t)mf_gated_mlp_pre_bytes(a.rows, a.hidden), x) : Tensor();
     a.y = y.data_ptr(), a.act = act.data_ptr(), a.pre = keep ? pre.data_ptr() : nullptr;
-    const Tensor ws = bytes(mf_gated_mlp_fwd_workspace_bytes(&a), x);
+    const Tensor ws = fresh_bytes(mf_gated_mlp_fwd_workspace_bytes(&a), x);
     if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
     check(mf_gated_mlp_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
     return {y, pre, act};
@@ -412,10 +418,10 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
       a.pre = s[5].data_ptr(), a.act = s[6].data_ptr(), a.grad_y = gy.const_data_ptr();
       size_t edge = 0;  // edges of the node are counted over the tensors that were given
       for (int i = 0; i < 5; ++i)
-        if (s[i].defined() && ctx->needs_input_grad(edge++)) g[i] = at::empty_like(s[i]);
+        if (s[i].defined() && ctx->needs_input_grad(edge++)) g[i] = fresh(s[i].sizes(), s[i].scalar_type(), s[i]);
       auto ptr = [&](int i) { return g[i].defined() ? g[i].data_ptr() : nullptr; };
       a.grad_x = ptr(0), a.grad_w_in = ptr(1), a.grad_w_out = ptr(2), a.grad_b_in = ptr(3), a.grad_b_out = ptr(4);
-      const Tensor ws = bytes(mf_gated_mlp_bwd_workspace_bytes(&a), x);
+      const Tensor ws = fresh_bytes(mf_gated_mlp_bwd_workspace_bytes(&a), x);
       if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
       check(mf_gated_mlp_bwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
     }
@@ -474,7 +480,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     };
     for (const Tensor& t : x) {
       if (!t.defined()) continue;
-      out.push_back(at::empty_like(t));
+      out.push_back(t.is_contiguous() ? fresh(t.sizes(), t.scalar_type(), t) : at::empty_like(t));
       if (out.back().stride(-1) != 1) out.back() = at::empty(t.sizes(), t.options());  // (overlapping inputs may have another order)
       const Tensor& o = out.back();
       a.batch = t.size(0), a.tokens = t.size(heads ? 1 : 2), a.head_dim = heads ? t.size(2) / (3 * heads) : t.size(3);

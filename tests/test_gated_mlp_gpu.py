@@ -344,3 +344,12 @@ def test_widths_beyond_the_kernel_are_refused():
     assert not gated.gated_mlp_applies(wide, wide.expand(16, -1), w)
     with pytest.raises(ValueError, match="up to 2\\^28"):
         mfb.gated_mlp(wide, wide.expand(16, -1), w)
+
+
+def test_inference_mode():
+    for rows in (5, 300):
+        ops, _ = _operands(rows, 64, 72, 80, BF16, True, seed=41)
+        want = mfb.gated_mlp(*ops)
+        with torch.inference_mode():
+            got = mfb.gated_mlp(*ops)
+            assert got.is_inference() and torch.equal(got, want)
