@@ -645,7 +645,8 @@ int mf_simplicial_packed_bwd(const MfSimplicialPackedArgs* args, void* stream);
  * opposite angles, which is the backward pass.
  * `frequencies` is a HOST array of P doubles, copied by the call.  positions: (tokens, axes) for each batch entry, position_batch
  * elements apart (0: the same for all).  Tensors: fp32, bf16 or fp16, strides in elements, channels adjacent, out apart from every
- * in.  Any sizes and alignment to an element; 16-byte accesses are used where head_dim, strides and addresses are multiples.  P <= 128.
+ * in.  Any sizes and alignment to an element; 16-byte accesses are used where head_dim, strides and addresses are multiples.  P <= 128,
+ * heads * head_dim <= 2^27.
  */
 typedef struct MfRotaryTensor {
   const void* in;
@@ -680,13 +681,13 @@ int mf_rotary(const MfRotaryArgs* args, void* stream);
  * The gated counterpart of `Mlp` (transformer.py:137-152); no reference operator.  For each of `rows` tokens
  *   [gate up] = x w_in^T + b_in,  act = f(gate) * up,  y = act w_out^T + b_out
  * with w_in (2*hidden, dim), the gate's rows first, w_out (dim_out, hidden) and optional biases (NULL).  dtype is bf16 or fp16, of
- * every tensor but the gradients of the parameters, which come in grad_dtype (dtype or fp32).  Widths are multiples of 8; any
- * number of rows.
+ * every tensor but the gradients of the parameters, which come in grad_dtype (dtype or fp32).  Widths are multiples of 8, at most 2^28; any
+ * number of rows below 2^31 - 512.
  * Forward: writes act (rows, hidden), y (rows, dim_out) and, where `pre` is given, the pre-activations: mf_gated_mlp_pre_bytes of a
  * form that the backward call reads (16-bit values with an exponent for every 16 of them).
  * Backward: reads x, w_in, w_out, pre, act and grad_y; writes those of grad_x, grad_w_in, grad_w_out, grad_b_in, grad_b_out that are
  * not NULL.  Sums are in fp32 and in a fixed order; act and the gradients of the pre-activations are rounded to dtype, the
- * pre-activations to three bits more.
+ * pre-activations to some bits more: of the largest of 16 neighbouring channels 11 (bf16) or 13 (fp16).
  * Workspace: forward mf_gated_mlp_fwd_workspace_bytes (without it some sizes take longer), backward mf_gated_mlp_bwd_workspace_bytes
  * for the same gradients.  An expired device-side wait is reported by
  * mf_gated_mlp_status (which synchronises `stream`); the outputs of such a call are undefined.

@@ -106,8 +106,7 @@ size_t slice_bytes(long long m, long long n, long long k) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) add_slices_kernel(const float* __restrict__ planes, int slices, long long values, int n, const T* __restrict__ bias,
-                                                         T* __restrict__ out) {
+__global__ void __launch_bounds__(256) add_slices_kernel(const float* planes, int slices, long long values, int n, const T* bias, T* out) {
   wait_for_previous();
   const long long i = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
   if (i >= values) return;
@@ -198,8 +197,7 @@ Plan plan_of(const MfGatedMlpArgs* a) {
 size_t plane_bytes(const Plan& w) { return w.pieces > 1 ? (size_t)w.wanted * w.pieces * kTile * kTile * 4 : 0; }
 
 template <typename T, typename TOut>
-__global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict__ planes, Plan w, TOut* __restrict__ out1, int m1, int n1,
-                                                         TOut* __restrict__ out2, int m2, int n2) {
+__global__ void __launch_bounds__(256) add_planes_kernel(const float* planes, Plan w, TOut* out1, int m1, int n1, TOut* out2, int m2, int n2) {
   wait_for_previous();
   const int tile = w.first + blockIdx.x;
   const bool second = tile >= w.tiles1;
@@ -242,7 +240,7 @@ __global__ void __launch_bounds__(64) bias_bands_kernel(BiasSums b) {
 }
 // 32 columns a block; thread (x, y) adds the bands y, y + 8, ..., then the eight sums are added in order.
 template <typename TOut>
-__global__ void __launch_bounds__(256) add_bias_bands_kernel(BiasSums b, TOut* __restrict__ out_in, TOut* __restrict__ out_out) {
+__global__ void __launch_bounds__(256) add_bias_bands_kernel(BiasSums b, TOut* out_in, TOut* out_out) {
   __shared__ float red[8][32];
   wait_for_previous();
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, n = b.n_in + b.n_out, c = blockIdx.x * 32 + x;

@@ -353,3 +353,31 @@ def test_inference_mode():
         with torch.inference_mode():
             got = mfb.gated_mlp(*ops)
             assert got.is_inference() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 32])
+def test_weights_that_the_call_before_makes(rows):
+    """Each call's result is the next call's output weight, without a pause between them: no kernel may read it too soon."""
+    g = torch.Generator().manual_seed(42)
+    x, xs = _randn(g, rows, 64), [_randn(g, 16, 64) for _ in range(100)]
+    w_in, w_weight = _randn(g, 1024, 64) / 8, _randn(g, 512, 512) / 16  # (16, 64) -> a weight (16, 512) of 512 hidden channels
+    weights = [mfb.gated_mlp(t, w_in, w_weight) for t in xs]
+    torch.cuda.synchronize()
+    want = []
+    for w in weights:
+        want.append(mfb.gated_mlp(x, w_in, w))
+        torch.cuda.synchronize()
+    buffer = torch.zeros(16, 512, dtype=BF16, device="cuda")
+    a = gated._args(xs[0], w_in, w_weight, None, None, "silu", BF16)
+    act, made = torch.empty(16, 512, dtype=BF16, device="cuda"), []
+    a.act, a.y = act.data_ptr(), buffer.data_ptr()
+    for t in xs:  # always into the same weight
+        a.x = t.data_ptr()
+        _lib.launch(_lib.lib().mf_gated_mlp_fwd, x.device, ctypes.byref(a))
+        made.append(mfb.gated_mlp(x, w_in, buffer))
+    for got, w in zip(made, want):
+        assert torch.equal(got, w)
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g).to(BF16).cuda()
