@@ -69,7 +69,7 @@ template <typename T, bool kAMn, bool kBMn, Epilogue kEpi>
 int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
   const long long items = (long long)p.tiles * p.slices;
   const int pairs = (int)(items < kPairs ? items : kPairs);
-  if constexpr (kEpi == kStore) return launch_kernel<T, kAMn, kBMn, kEpi, 0>(p, pairs, stream, what);
+  if constexpr (stores(kEpi)) return launch_kernel<T, kAMn, kBMn, kEpi, 0>(p, pairs, stream, what);
   else
     return activation == MF_ACT_SILU ? launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_SILU>(p, pairs, stream, what)
                                      : launch_kernel<T, kAMn, kBMn, kEpi, MF_ACT_GELU_TANH>(p, pairs, stream, what);
@@ -138,7 +138,7 @@ int store_product(Params& p, const T* bias, T* out, float* planes, cudaStream_t 
     p.bias = bias;
   }
   MF_MAP(map16<T>(&p.one.out, out, m, n, n, 32));
-  const int rc = launch<T, false, kBMn, kStore>(p, 0, stream, what);
+  const int rc = p.whole == 0 && p.cut > 1 ? launch<T, false, kBMn, kStoreNarrow>(p, 0, stream, what) : launch<T, false, kBMn, kStore>(p, 0, stream, what);
   if (rc != MF_OK || s.slices == 1) return rc;
   launch_dependent(add_slices_kernel<T>, dim3((unsigned)((m * n / 4 + 255) / 256)), dim3(256), 0, stream, planes, s.slices, m * n, (int)n, bias, out);
   MF_CHECK_LAUNCH("add_slices_kernel");

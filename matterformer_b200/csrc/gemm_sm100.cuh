@@ -32,14 +32,14 @@ __device__ int32_t g_gemm_status = 0;  // MF_ERR_DEVICE_TIMEOUT after an expired
 // kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well; kGateGrad: the gradient of both;
 // kStore: the product and a bias; kGradients: the weights' gradients, two products over the same long dimension (of operands that have it
 // outermost), and the input's, side by side
-enum Epilogue { kGate, kGateKeep, kGateGrad, kStore, kGradients };
+enum Epilogue { kGate, kGateKeep, kGateGrad, kStore, kStoreNarrow, kGradients };  // kStoreNarrow: no tile is wider than 128 columns
 __host__ __device__ constexpr bool projects(Epilogue e) { return e == kGate || e == kGateKeep; }
+__host__ __device__ constexpr bool stores(Epilogue e) { return e == kStore || e == kStoreNarrow; }
 
 constexpr int kBlockK = 64;                       // elements of the contracted dimension in a stage
 constexpr int kBoxBytes = 64 * 128;               // 64 lines of 64 16-bit elements
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (4 + kEpilogueWarps);
-constexpr int kStageBytes = 4 * kBoxBytes;        // 128 rows of A, 128 of B
 constexpr int kStageBuffer = 32 * 128;            // what a warp hands to the copy engine at once: 32 rows of 128 bytes
 constexpr int kTile = 256;
 constexpr int kTmemCols = 512;
@@ -50,7 +50,10 @@ struct Shape {
   // projections of 8192 x 5504 over 2048 4 %.
   static constexpr int kBuffers = kEpi == kGateGrad ? 4 : kEpi == kGateKeep ? 2 : 1;
   static constexpr int kBufferBytes = kEpilogueWarps * kBuffers * kStageBuffer;
-  static constexpr int kStages = kEpi == kGateGrad ? 3 : kEpi == kGateKeep ? 5 : 6;
+  // A stage has 128 rows of A and 128 of B, 64 where tiles are narrow: eight stages then.  One round of narrow tiles is bound by the way from
+  // L2, some 1.2 us for six or eight stages alike: 1856 tokens, 512 x 2048, both products 21.2 -> 20.4 us; 512 tokens, 1024 x 4096 28.5 -> 26.9.
+  static constexpr int kStageBytes = (kEpi == kStoreNarrow ? 3 : 4) * kBoxBytes;
+  static constexpr int kStages = kEpi == kGateGrad ? 3 : kEpi == kGateKeep ? 5 : kEpi == kStoreNarrow ? 8 : 6;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kBufferBytes;
   static_assert(kSmem + 1024 <= 232448, "shared memory");
 };
@@ -351,7 +354,7 @@ struct Walk {
       w.row = tile / tiles_n * kTile, w.col = tile % tiles_n * kTile + part * w.cols;
       return true;
     } else {
-      const int slices = kEpi == kStore ? p.slices : 1;
+      const int slices = stores(kEpi) ? p.slices : 1;
       if (t >= p.tiles * slices) return false;
       int m, n, u = t;
       if (slices > 1) {
@@ -374,7 +377,7 @@ struct Walk {
 template <typename T, bool kAMn, bool kBMn, Epilogue kEpi, int kAct>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Params p) {
   using Sh = Shape<kEpi>;
-  constexpr int kStages = Sh::kStages;
+  constexpr int kStages = Sh::kStages, kStageBytes = Sh::kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   __shared__ uint64_t bar_full[kStages], bar_empty[kStages], bar_acc[2], bar_drained[2], bar_in[2 * kEpilogueWarps], bar_end;
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         const bool outermost = kEpi == kGradients ? w.which != kInput : kAMn;  // the contracted dimension of A
         const int row = w.row + 128 * (int)rank;
         const int col = projects(kEpi) ? w.col : w.col + w.cols / 2 * (int)rank;
-        const bool two = (projects(kEpi) ? w.cols : w.cols / 2) > 64;  // boxes of B (a tile of 64 columns uses half of its box)
+        const bool two = kEpi != kStoreNarrow && (projects(kEpi) ? w.cols : w.cols / 2) > 64;  // boxes of B (a tile of 64 columns uses half of its box)
         for (int kb = w.k0; kb < w.k1; ++kb, ++it) {
           const int s = it % kStages;
           if (it >= kStages && !mbar_wait_for(&bar_empty[s], ((it / kStages) & 1) ^ 1, p.waits.limit)) {
@@ -711,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         if (bad) break;
       } else {
         const Problem& prob = problem(w);
-        const bool sliced = kEpi == kStore && w.plane >= 0;
+        const bool sliced = stores(kEpi) && w.plane >= 0;
         if (sliced || (kEpi == kGradients && w.which != kInput && (w.plane >= 0 || p.wide_out))) {  // 32 fp32 columns at a time: partial sums, or an fp32 result
 #pragma unroll 1
           for (int c = 0; c < 2 * chunks; ++c) {
@@ -738,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               uint4 b[4];
               tmem_ld32(acc + first + 64 * c + 32 * h, d);
 #pragma unroll
-              for (int v = 0; v < 4; ++v) b[v] = kEpi == kStore ? bias8(bias, col0 + 64 * c + 32 * h + 8 * v, bias_n) : make_uint4(0u, 0u, 0u, 0u);
+              for (int v = 0; v < 4; ++v) b[v] = stores(kEpi) ? bias8(bias, col0 + 64 * c + 32 * h + 8 * v, bias_n) : make_uint4(0u, 0u, 0u, 0u);
               tmem_ld_wait();
 #pragma unroll
               for (int v = 0; v < 4; ++v) {
