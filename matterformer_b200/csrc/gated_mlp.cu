@@ -79,8 +79,9 @@ int launch(Params& p, int activation, cudaStream_t stream, const char* what) {
 // The output product of some hundred tokens: a few tiles for 74 pairs, each over all hidden channels.  Cut into narrower tiles they would
 // still leave pairs idle and give the others less of the weights at a time; cut along the hidden channels, every pair reads a share of the
 // weights at full width, and a second launch adds the planes and the bias.  33 tokens, 1024 x 4096: 27 -> 20 us, 2048 x 8192: 47 -> 32,
-// 4096 x 10 928: 83 -> 68.  Estimated in clocks: a block of 64 channels takes 560,
-// 300, 250 at 256, 128, 64 columns, the second launch 6000 and a clock for every 2500 bytes of planes written and read.
+// 4096 x 10 928: 83 -> 68.  Estimated in clocks: a block of 64 channels takes 650, 250, 220 at 256, 128, 64 columns (eight stages for the
+// latter two), the second launch 4500 and a clock for every 2500 bytes of planes written and read; with 560, 300, 250 and 6000 some sizes
+// went whole that gain by slices: 64 tokens, 512 x 2048 15.4 -> 13.2, 128 tokens, 1024 x 2736 18.9 -> 16.0.
 struct Slices {
   int cut, slices;
 };
@@ -88,14 +89,14 @@ Slices slices_of(long long m, long long n, long long k) {
   const int tiles = tiles_of(m, n, kTile), k_blocks = (int)((k + kBlockK - 1) / kBlockK);
   Slices best = {0, 1};
   if (tiles > kPairs / 2) return best;
-  const double clocks[5] = {0, 560, 300, 0, 250};
+  const double clocks[5] = {0, 650, 250, 0, 220};
   const int cut = 4 * tiles <= kPairs ? 4 : 2;
   double least = (double)k_blocks * clocks[cut];
   for (int c = 1; c <= 2; c *= 2)
     for (int s = 2; tiles * c * s <= kPairs && 2 * s <= k_blocks; ++s) {
       const int per = (k_blocks + s - 1) / s;
       if ((k_blocks + per - 1) / per != s) continue;
-      const double t = per * clocks[c] + 6000. + 8. * (double)m * n * s / 2500.;
+      const double t = per * clocks[c] + 4500. + 8. * (double)m * n * s / 2500.;
       if (t < least) least = t, best = {c, s};
     }
   return best;
