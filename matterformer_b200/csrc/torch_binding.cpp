@@ -464,11 +464,31 @@ std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tenso
 // ---------------------------------------------------------------------------------------------------------------------
 // Rotary positions
 // ---------------------------------------------------------------------------------------------------------------------
+// What a call turns by; `table` (axes, pairs), or (pairs) where `flat`, is the caller's.
+struct Turning {
+  const double* table;
+  int64_t axes, pairs;
+  bool flat;
+  int64_t heads, layout;  // heads 0: one or two head-major tensors; otherwise a packed projection with that many heads
+  double amplitude;
+  bool inverse;
+};
+// The same for the backward pass, with a copy of the table, which may have changed by then.
+struct SavedTurning : torch::CustomClassHolder {
+  Turning turning;
+  std::array<double, 128> table;
+  bool foreign;
+  SavedTurning(const Turning& t, bool foreign_) : turning(t), foreign(foreign_) {
+    std::copy_n(t.table, t.axes * t.pairs, table.begin());
+    turning.table = table.data();
+    turning.inverse = !t.inverse;
+  }
+};
+
 struct Rotary : torch::autograd::Function<Rotary> {
-  // heads 0: one or two head-major tensors; otherwise a packed projection with that many heads
-  static tensor_list turn(const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads, int64_t layout,
-                          double amplitude, bool inverse) {
+  static tensor_list turn(const Tensor& first, const OptTensor& second, const Tensor& positions, const Turning& by) {
     const c10::cuda::CUDAGuard guard(first.device());
+    const int64_t heads = by.heads;
     auto adjacent = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
     const Tensor x[2] = {adjacent(first), second ? adjacent(*second) : Tensor()};
     tensor_list out;
@@ -488,43 +508,38 @@ struct Rotary : torch::autograd::Function<Rotary> {
         for (int i = 0; i < 3; ++i) add(t, o, i * heads * a.head_dim, heads, i < 2, 1, a.head_dim, a.head_dim);
       else add(t, o, 0, t.size(1), true, 2, t.stride(1), o.stride(1));
     }
-    a.axes = table.dim() == 1 ? 1 : table.size(0), a.pairs = table.size(-1);
-    a.dtype = dtype_code(first), a.layout = layout, a.inverse = inverse, a.amplitude = amplitude;
+    a.axes = by.axes, a.pairs = by.pairs;
+    a.dtype = dtype_code(first), a.layout = by.layout, a.inverse = by.inverse, a.amplitude = by.amplitude;
     a.position_type = positions.scalar_type() == at::kInt    ? MF_POSITION_I32
                       : positions.scalar_type() == at::kLong ? MF_POSITION_I64
                       : positions.scalar_type() == at::kFloat ? MF_POSITION_F32
                                                              : MF_POSITION_F64;
-    a.positions = positions.const_data_ptr(), a.position_batch = positions.dim() == table.dim() + 1 ? positions.stride(0) : 0;
-    a.frequencies = table.const_data_ptr<double>();
+    a.positions = positions.const_data_ptr(), a.position_batch = positions.dim() == (by.flat ? 2 : 3) ? positions.stride(0) : 0;
+    a.frequencies = by.table;
     check(mf_rotary(&a, c10::cuda::getCurrentCUDAStream().stream()));
     return out;
   }
 
-  static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads,
-                             int64_t layout, double amplitude, bool inverse, bool keep, bool foreign) {
-    const tensor_list out = turn(first, second, positions, table, heads, layout, amplitude, inverse);
+  static tensor_list forward(AutogradContext* ctx, const Tensor& first, const OptTensor& second, const Tensor& positions, const Turning& by, bool foreign) {
+    const tensor_list out = turn(first, second, positions, by);
     ctx->set_materialize_grads(false);
-    if (keep) {
-      ctx->save_for_backward({positions.is_inference() ? positions.clone() : positions});
-      ctx->saved_data["table"] = table.clone();  // (the caller's may have changed by then)
-    }
-    ctx->saved_data["heads"] = heads, ctx->saved_data["layout"] = layout, ctx->saved_data["amplitude"] = amplitude, ctx->saved_data["inverse"] = inverse;
-    ctx->saved_data["foreign"] = foreign;
+    ctx->save_for_backward({positions.is_inference() ? positions.clone() : positions});
+    ctx->saved_data["turning"] = c10::IValue::make_capsule(c10::make_intrusive<SavedTurning>(by, foreign));
     return out;
   }
 
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-    tensor_list given, g(10);
-    refuse_foreign(ctx->saved_data["foreign"].toBool(), "rotary_embedding");
-    for (const Tensor& t : grads)
-      if (t.defined()) given.push_back(t);
-    if (given.empty()) return g;
-    auto& s = ctx->saved_data;
-    const Tensor positions = ctx->get_saved_variables()[0];
+    tensor_list given, g(5);  // (one for each argument of forward)
+    const auto held = ctx->saved_data["turning"].toCapsule();
+    const SavedTurning& saved = static_cast<const SavedTurning&>(*held);
+    refuse_foreign(saved.foreign, "rotary_embedding");
     bool keep = false;
-    for (const Tensor& t : given) keep = keep || (at::GradMode::is_enabled() && t.requires_grad());
-    const tensor_list turned = Rotary::apply(given[0], given.size() > 1 ? OptTensor(given[1]) : std::nullopt, positions, s["table"].toTensor(),
-                                             s["heads"].toInt(), s["layout"].toInt(), s["amplitude"].toDouble(), !s["inverse"].toBool(), keep, false);
+    for (const Tensor& t : grads)
+      if (t.defined()) given.push_back(t), keep = keep || (at::GradMode::is_enabled() && t.requires_grad());
+    if (given.empty()) return g;
+    const Tensor positions = ctx->get_saved_variables()[0];
+    const OptTensor second = given.size() > 1 ? OptTensor(given[1]) : std::nullopt;
+    const tensor_list turned = keep ? Rotary::apply(given[0], second, positions, saved.turning, false) : turn(given[0], second, positions, saved.turning);
     for (size_t i = 0, j = 0; i < grads.size(); ++i)
       if (grads[i].defined()) g[i] = turned[j++];
     return g;
@@ -551,11 +566,12 @@ std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, 
       (positions.sizes() != at::IntArrayRef(shape) && positions.sizes() != at::IntArrayRef(shape).slice(1)))
     return std::nullopt;
   if (first._fw_grad(0).defined() || (second && second->_fw_grad(0).defined())) return std::nullopt;
+  const bool keep = at::GradMode::is_enabled() && (first.requires_grad() || (second && second->requires_grad()));
+  const Turning by = {table.const_data_ptr<double>(), table.dim() == 1 ? 1 : table.size(0), table.size(-1), table.dim() == 1, heads, layout, amplitude, false};
+  if (!keep) return Rotary::turn(first, second, positions, by);  // (past autograd: 9.1 -> 6.9 us a call)
   const Tensor none;
   const c10::cuda::CUDAGuard guard(first.device());
-  const bool keep = at::GradMode::is_enabled() && (first.requires_grad() || (second && second->requires_grad()));
-  if (!keep) return Rotary::turn(first, second, positions, table, heads, layout, amplitude, false);  // (past autograd: 9.1 -> 6.9 us a call)
-  return Rotary::apply(first, second, positions, table, heads, layout, amplitude, false, keep, foreign_leaves({&first, second ? &*second : &none}));
+  return Rotary::apply(first, second, positions, by, foreign_leaves({&first, second ? &*second : &none}));
 }
 
 }  // namespace
