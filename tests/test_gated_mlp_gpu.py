@@ -381,3 +381,18 @@ def test_weights_that_the_call_before_makes(rows):
 
 def _randn(g, *shape):
     return torch.randn(*shape, generator=g).to(BF16).cuda()
+
+
+@pytest.mark.parametrize("kind", range(3))
+def test_expired_waits_in_narrow_tiles(kind):
+    """The same for an output product that is a single round of narrow tiles over more blocks than stages (600 x 520 over 648)."""
+    ops, _ = _operands(600, 64, 648, 520, BF16, True, seed=43)
+    want = mfb.gated_mlp(*ops)
+    a = gated._args(*ops, "silu", BF16)
+    act, y = torch.empty(600, 648, dtype=BF16, device="cuda"), torch.empty(600, 520, dtype=BF16, device="cuda")
+    a.act, a.y = act.data_ptr(), y.data_ptr()
+    status = ctypes.c_int32(0)
+    _lib.launch(_lib.lib().mf_selftest_gated_mlp_give_up, y.device, ctypes.byref(a), 0, kind, 40000, ctypes.byref(status))
+    assert status.value == _lib.MF_ERR_DEVICE_TIMEOUT
+    assert mfb.gated_mlp_status() == 0
+    assert torch.equal(mfb.gated_mlp(*ops), want)
