@@ -29,12 +29,12 @@ template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
 template <>
 __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  const float4 a = load_operand(reinterpret_cast<const float4*>(p)), b = load_operand(reinterpret_cast<const float4*>(p) + 1);
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 template <>
 __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint4 a = load_operand(reinterpret_cast<const uint4*>(p));
   const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
@@ -85,7 +85,7 @@ __device__ __forceinline__ float gelu_tanh_grad(float x) {
 }
 
 template <typename T>
-__global__ void gelu_tanh_fwd_kernel(const T* __restrict__ x, long long n, T* __restrict__ y) {
+__global__ void gelu_tanh_fwd_kernel(const T* x, long long n, T* __restrict__ y) {
   wait_for_previous();
   const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8;
   if (i >= n) return;
@@ -99,7 +99,7 @@ __global__ void gelu_tanh_fwd_kernel(const T* __restrict__ x, long long n, T* __
 // grid (column groups, bands); part[band][C].  kGelu: x is the pre-activation, dy the gradient of the activation;
 // dx = dy * gelu'(x) is stored and summed.
 template <typename T, bool kGelu>
-__global__ void __launch_bounds__(kWarps * 32) column_sums_band_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+__global__ void __launch_bounds__(kWarps * 32) column_sums_band_kernel(const T* x, const T* dy,
                                                                       T* __restrict__ dx, long long rows, int C,
                                                                       long long rows_per_band, float* __restrict__ part) {
   __shared__ float red[kWarps][kColsPerBlock];
@@ -111,15 +111,16 @@ __global__ void __launch_bounds__(kWarps * 32) column_sums_band_kernel(const T* 
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (col < C) {
     long long r = r0 + warp;
-    for (; r + 3 * kWarps < r1; r += 4 * kWarps) {  // four rows in flight per lane
-      float v[4][8], g[kGelu ? 4 : 1][8];
+    constexpr int kRows = kGelu && sizeof(T) == 4 ? 2 : 4;  // in flight per lane
+    for (; r + (kRows - 1) * kWarps < r1; r += kRows * kWarps) {
+      float v[kRows][8], g[kGelu ? kRows : 1][8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         load8<T>(x + (r + u * kWarps) * C + col, v[u]);
         if constexpr (kGelu) load8<T>(dy + (r + u * kWarps) * C + col, g[u]);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         if constexpr (kGelu) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[u][e] = g[u][e] * gelu_tanh_grad<sizeof(T) == 2>(v[u][e]);
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kWarps * 32) column_sums_band_kernel(const T* 
 
 // Adds the bands: a block of 32 x 8 threads owns 32 columns; thread (x, y) adds the bands y, y + 8, ... (four loads in
 // flight), then the eight slices are added in slice order.
-__global__ void __launch_bounds__(256) column_sums_final_kernel(const float* __restrict__ part, int bands, int C,
+__global__ void __launch_bounds__(256) column_sums_final_kernel(const float* part, int bands, int C,
                                                                 float* __restrict__ out) {
   __shared__ float red[8][32];
   wait_for_previous();

@@ -60,6 +60,24 @@ struct BoundedWaits {
 constexpr long long kDependentGrid = 2048;
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// A load that is marked as read-only may be moved above the wait, in front of the results that it is to read.  Such kernels read
+// through pointers that are not `const ... __restrict__` parameters, or with this, which stays behind the wait but, unlike a plain load, not
+// behind stores that come before it.
+template <typename T>
+__device__ __forceinline__ T load_operand(const T* p) {
+  static_assert(sizeof(T) == 16 || sizeof(T) == 1, "");
+  T v;
+  if constexpr (sizeof(T) == 16) {
+    uint4 w;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p));
+    v = *reinterpret_cast<T*>(&w);
+  } else {
+    uint32_t w;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(w) : "l"(p));
+    v = (T)w;
+  }
+  return v;
+}
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchAttribute attribute{};

@@ -13,7 +13,7 @@ namespace mf {
 namespace {
 
 // c_skip, c_out and c_in of the preconditioner, and the network's noise channel log(sigma) / 4: the operations of the element-wise form
-__global__ void edm_scalings_kernel(const float* __restrict__ sigma, int B, float sd, float sd2, float* __restrict__ scalings,
+__global__ void edm_scalings_kernel(const float* sigma, int B, float sd, float sd2, float* __restrict__ scalings,
                                     float* __restrict__ noise) {
   wait_for_previous();
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
@@ -30,7 +30,7 @@ __global__ void edm_scalings_kernel(const float* __restrict__ sigma, int B, floa
 // cos and sin of 2 pi t f for the frequencies f_i = 10000^(-i / half), twice over (the network embeds one noise level for the
 // molecule and one for its atoms, and they are the same)
 template <typename T>
-__global__ void time_embedding_kernel(const float* __restrict__ t, int half, T* __restrict__ out) {
+__global__ void time_embedding_kernel(const float* t, int half, T* __restrict__ out) {
   wait_for_previous();
   const float at = __fmul_rn(6.283185307179586f, t[blockIdx.x]);
   T* row = out + (size_t)blockIdx.x * 4 * half;
@@ -44,7 +44,7 @@ __global__ void time_embedding_kernel(const float* __restrict__ t, int half, T* 
 }
 
 // Real atoms: 1 - pad, and their number per molecule.  A warp per molecule.
-__global__ void pad_counts_kernel(const uint8_t* __restrict__ pad, int B, int N, uint8_t* __restrict__ valid, int32_t* __restrict__ counts) {
+__global__ void pad_counts_kernel(const uint8_t* pad, int B, int N, uint8_t* __restrict__ valid, int32_t* __restrict__ counts) {
   wait_for_previous();
   const int b = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (b >= B) return;
@@ -66,9 +66,9 @@ constexpr int kMaxTokenInputs = 8;
 constexpr int kTokenThreads = 256, kTokenRows = 16;  // rows of a block of a small batch; larger ones make one wave of blocks
 __device__ __forceinline__ float as_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
-__global__ void __launch_bounds__(kTokenThreads) token_projection_kernel(const float* __restrict__ x, const float* __restrict__ noise,
-                                                                         const uint8_t* __restrict__ pad, const float* __restrict__ weight,
-                                                                         const float* __restrict__ bias, long long rows, int rows_per_block,
+__global__ void __launch_bounds__(kTokenThreads) token_projection_kernel(const float* x, const float* noise,
+                                                                         const uint8_t* pad, const float* weight,
+                                                                         const float* bias, long long rows, int rows_per_block,
                                                                          int N, int K, int C, __nv_bfloat16* __restrict__ out) {
   wait_for_previous();
   __shared__ __align__(16) float ws[kMaxTokenInputs * 1024];  // weights by input: a thread's own lie 8 K floats from its neighbour's in memory
@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(kTokenThreads) token_projection_kernel(const f
 // Its weight and bias gradients: part[band] = (C, K) sums of dy x, then C sums of dy, over a band of rows; the bands are added in
 // order.  A thread holds two channels.  1 024 molecules of 29 tokens: a GEMM with seven columns and a reduction took 76 + 10 us.
 constexpr int kTokenChunk = 32;
-__global__ void token_projection_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const float* __restrict__ x, const float* __restrict__ noise,
-                                            const uint8_t* __restrict__ pad, long long rows, long long rows_per_band, int N, int K, int C,
+__global__ void token_projection_bwd_kernel(const __nv_bfloat16* dy, const float* x, const float* noise,
+                                            const uint8_t* pad, long long rows, long long rows_per_band, int N, int K, int C,
                                             float* __restrict__ part) {
   __shared__ float in[kTokenChunk][kMaxTokenInputs + 1];
   wait_for_previous();
@@ -171,7 +171,7 @@ __device__ __forceinline__ void unpack8(uint4 a, float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
 }
-__global__ void split_modulation_kernel(const __nv_bfloat16* __restrict__ mod, int B, int G, int C, float* __restrict__ out) {
+__global__ void split_modulation_kernel(const __nv_bfloat16* mod, int B, int G, int C, float* __restrict__ out) {
   wait_for_previous();
   const int c = 8 * threadIdx.x, g = blockIdx.x, step = gridDim.y * blockDim.y;
 #pragma unroll 4

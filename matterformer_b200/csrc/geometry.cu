@@ -219,8 +219,8 @@ __device__ __forceinline__ float2 nearest_image(float2 d) {
 // per lane, 6.0 us now; 16 of 512-1 024 atoms 66.6 -> 24.8 us.
 constexpr int kListWarps = 16;
 constexpr int kListAtoms = 1024;  // columns in shared memory at a time
-__global__ void __launch_bounds__(32 * kListWarps) block_list_kernel(const float* __restrict__ frac, const StructureInfo* __restrict__ info,
-                                                          const int32_t* __restrict__ num_atoms, const int32_t* __restrict__ perm,
+__global__ void __launch_bounds__(32 * kListWarps) block_list_kernel(const float* frac, const StructureInfo* info,
+                                                          const int32_t* num_atoms, const int32_t* perm,
                                                           int n_max, int tiles, float cutoff, uint32_t* __restrict__ block_mask,
                                                           int32_t* __restrict__ block_count, int32_t* __restrict__ block_cols) {
   extern __shared__ uint32_t active[];  // bit J

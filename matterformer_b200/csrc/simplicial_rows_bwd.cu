@@ -150,7 +150,7 @@ __device__ __forceinline__ int pieces_used(int walked, int pieces) {
   return each > 0 ? (walked + each - 1) / each : 0;
 }
 
-__global__ void delta_rows_kernel(const __nv_bfloat16* __restrict__ grad_out, const float* __restrict__ out,
+__global__ void delta_rows_kernel(const __nv_bfloat16* grad_out, const float* out,
                                   float* __restrict__ delta, int rows) {
   wait_for_previous();
   const int row = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -273,8 +273,8 @@ __global__ void __maxnreg__(168) simplicial_rows_bwd_kernel(const __grid_constan
         const int rr = idx >> 3, c = idx & 7;
         uint4 vk = make_uint4(0, 0, 0, 0), vv = make_uint4(0, 0, 0, 0);
         if (key_live(rr)) {
-          vk = __ldg(reinterpret_cast<const uint4*>(p.k2 + base + (size_t)(k0 + rr) * kD) + c);
-          vv = __ldg(reinterpret_cast<const uint4*>(p.v2 + base + (size_t)(k0 + rr) * kD) + c);
+          vk = load_operand(reinterpret_cast<const uint4*>(p.k2 + base + (size_t)(k0 + rr) * kD) + c);
+          vv = load_operand(reinterpret_cast<const uint4*>(p.v2 + base + (size_t)(k0 + rr) * kD) + c);
         }
         const uint32_t off = rr * 128 + ((c ^ (rr & 7)) << 4);
         *reinterpret_cast<uint4*>(smem + kOffK2 + off) = vk;
@@ -438,7 +438,7 @@ __global__ void __maxnreg__(168) simplicial_rows_bwd_kernel(const __grid_constan
           const int jj = s * G + gg;
           v[q] = make_uint4(0, 0, 0, 0);
           if (gg < G && jj < nj)
-            v[q] = __ldg(reinterpret_cast<const uint4*>((which == 0 ? p.k1 : p.v1) + base + (size_t)jlist[jj] * kD) + part);
+            v[q] = load_operand(reinterpret_cast<const uint4*>((which == 0 ? p.k1 : p.v1) + base + (size_t)jlist[jj] * kD) + part);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -601,7 +601,7 @@ __global__ void __maxnreg__(168) simplicial_rows_bwd_kernel(const __grid_constan
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (row_ok) v = __ldg(xp + c);
+          if (row_ok) v = load_operand(xp + c);
           xreg[4 * c + 0] = v.x;
           xreg[4 * c + 1] = v.y;
           xreg[4 * c + 2] = v.z;

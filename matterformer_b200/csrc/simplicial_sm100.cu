@@ -37,7 +37,7 @@ constexpr int kColW = 192;
 // Per-batch extents and a heaviest-first launch order.
 // ---------------------------------------------------------------------------
 // one warp per batch element: the last valid key / query index + 1
-__global__ void extent_kernel(const uint8_t* __restrict__ query_valid, const uint8_t* __restrict__ key_valid, int B,
+__global__ void extent_kernel(const uint8_t* query_valid, const uint8_t* key_valid, int B,
                               int N, BatchInfo* __restrict__ info, int32_t* __restrict__ status) {
   wait_for_previous();
   if (blockIdx.x == 0 && threadIdx.x < 64) status[threadIdx.x] = 0;  // the 256-byte status block
@@ -68,7 +68,7 @@ __global__ void extent_kernel(const uint8_t* __restrict__ query_valid, const uin
 
 // rank by cost (descending), ties by index: a stable, deterministic order; one warp per batch element, its lanes
 // striding over the elements it is compared with
-__global__ void order_kernel(const BatchInfo* __restrict__ info, int B, int32_t* __restrict__ order) {
+__global__ void order_kernel(const BatchInfo* info, int B, int32_t* __restrict__ order) {
   wait_for_previous();
   const int b = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (b >= B) return;  // uniform per warp

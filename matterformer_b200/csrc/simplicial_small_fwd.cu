@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(32 * kWarps, kBias ? 12 / kWarps : (kWarps == 
 }
 
 // Molecules by their number of keys, the largest first (the order decides when a molecule runs, not what it computes).
-__global__ void __launch_bounds__(1024) simplicial_small_order_kernel(const uint8_t* __restrict__ key_valid, int B, int N, int32_t* keys,
+__global__ void __launch_bounds__(1024) simplicial_small_order_kernel(const uint8_t* key_valid, int B, int N, int32_t* keys,
                                                                      int32_t* order) {
   __shared__ int start[kSmallRows + 1];
   wait_for_previous();
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(1024) simplicial_small_order_kernel(const uint
   for (int b0 = kAtOnce * warp; b0 < B; b0 += 32 * kAtOnce) {
     uint8_t v[kAtOnce];
 #pragma unroll
-    for (int t = 0; t < kAtOnce; ++t) v[t] = __ldg(key_valid + (size_t)min(b0 + t, B - 1) * N + min(lane, N - 1));
+    for (int t = 0; t < kAtOnce; ++t) v[t] = load_operand(key_valid + (size_t)min(b0 + t, B - 1) * N + min(lane, N - 1));
     int mine = 0;
 #pragma unroll
     for (int t = 0; t < kAtOnce; ++t) {

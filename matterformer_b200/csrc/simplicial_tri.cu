@@ -698,7 +698,7 @@ __device__ __forceinline__ void tri_tile(const TriParams& p, TriShared& sh, uint
 #pragma unroll
         for (int c = 0; c < kXw / 4; ++c) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (row_ok) v = __ldg(reinterpret_cast<const uint4*>(src) + c);
+          if (row_ok) v = load_operand(reinterpret_cast<const uint4*>(src) + c);
           xr[4 * c] = v.x, xr[4 * c + 1] = v.y, xr[4 * c + 2] = v.z, xr[4 * c + 3] = v.w;
         }
       }
@@ -869,8 +869,8 @@ __global__ void __maxnreg__(kRegLaunch) simplicial_tri_bwd_kernel(const __grid_c
 // Extents of the molecules and the list of tiles, heavy molecules first (by buckets of their mean extent; the order decides when
 // a tile runs, not what it computes).  One block: the list is short next to the work it describes.
 constexpr int kScheduleThreads = 1024;
-__global__ void __launch_bounds__(kScheduleThreads) simplicial_tri_schedule_kernel(const uint8_t* __restrict__ query_valid,
-                                                                                  const uint8_t* __restrict__ key_valid, int B, int N,
+__global__ void __launch_bounds__(kScheduleThreads) simplicial_tri_schedule_kernel(const uint8_t* query_valid,
+                                                                                  const uint8_t* key_valid, int B, int N,
                                                                                   int backward, BatchInfo* info, int2* items,
                                                                                   int32_t* status) {
   wait_for_previous();
@@ -930,8 +930,8 @@ __global__ void __launch_bounds__(kScheduleThreads) simplicial_tri_schedule_kern
 }
 
 // -lse log2e and -delta = -dO . out of the valid queries
-__global__ void __launch_bounds__(256) simplicial_tri_rows_kernel(const __nv_bfloat16* __restrict__ grad_out, const float* __restrict__ out,
-                                                                 const float* __restrict__ lse, const uint8_t* __restrict__ query_valid,
+__global__ void __launch_bounds__(256) simplicial_tri_rows_kernel(const __nv_bfloat16* grad_out, const float* out,
+                                                                 const float* lse, const uint8_t* query_valid,
                                                                  int H, int N, int rows, float* __restrict__ lse2,
                                                                  float* __restrict__ ndelta) {
   wait_for_previous();
@@ -950,7 +950,7 @@ struct TriClear {
   uint32_t* at[9];
   size_t words[9];
 };
-__global__ void __launch_bounds__(256) simplicial_tri_clear_kernel(const __grid_constant__ TriClear c, const int32_t* __restrict__ status) {
+__global__ void __launch_bounds__(256) simplicial_tri_clear_kernel(const __grid_constant__ TriClear c, const int32_t* status) {
   wait_for_previous();
   if (*status == 0) return;
 #pragma unroll 1

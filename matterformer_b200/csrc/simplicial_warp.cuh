@@ -199,7 +199,7 @@ __device__ __forceinline__ void stage_factors(const RankTile<RK> (&t)[F], const 
 #pragma unroll
       for (int s = 0; s < 4 * RK; ++s) {
         const int idx = lane + 32 * s;
-        x[f][s] = idx < total ? __ldg(reinterpret_cast<const float4*>(src[f]) + idx) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[f][s] = idx < total ? load_operand(reinterpret_cast<const float4*>(src[f]) + idx) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
     for (int s = 0; s < 4 * RK; ++s) {
