@@ -52,6 +52,14 @@ __device__ __forceinline__ void activation2(float2 z, float2& value, float2& slo
 //   fp16: sign, 3 bits of exponent, 12 of fraction: 13 bits down to 2^-7 of the largest, from there steps of 2^-19 of it.  What an fp32
 //   value below 2^-120 has in its bits 11-25 is that form, subnormals included: a multiplication and a shift round to it.
 // A group with an infinity or NaN: bf16 passes it on beside the values that fp16 can hold; fp16 is NaN in all 16.
+// The larger of two magnitudes: in fp16 a NaN wins, so that its group is known; in bf16 the others decide, a NaN needs no exponent.
+template <typename T>
+__device__ __forceinline__ float group_max(float a, float b) {
+  if constexpr (!std::is_same<T, __half>::value) return fmaxf(a, b);
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t group_exponent(float largest) {  // of the largest magnitude
   const uint32_t e = __float_as_uint(largest) >> 23;

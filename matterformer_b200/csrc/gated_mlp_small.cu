@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p)
         float most_g = fabsf(a), most_u = fabsf(u);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) {
-          most_g = fmaxf(most_g, __shfl_xor_sync(lanes, most_g, o));
-          most_u = fmaxf(most_u, __shfl_xor_sync(lanes, most_u, o));
+          most_g = group_max<T>(most_g, __shfl_xor_sync(lanes, most_g, o));
+          most_u = group_max<T>(most_u, __shfl_xor_sync(lanes, most_u, o));
         }
         const uint32_t eg = group_exponent<T>(most_g), eu = group_exponent<T>(most_u);
         if (n < p.n) {

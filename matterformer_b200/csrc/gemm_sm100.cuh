@@ -604,7 +604,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 hw[4 * v + e] = pack2<T>(h.x, h.y);
                 if constexpr (kEpi == kGateKeep) {
                   gv[i] = __float_as_uint(gate.x), gv[i + 1] = __float_as_uint(gate.y), uv[i] = __float_as_uint(up.x), uv[i + 1] = __float_as_uint(up.y);
-                  most_g = fmaxf(most_g, fmaxf(fabsf(gate.x), fabsf(gate.y))), most_u = fmaxf(most_u, fmaxf(fabsf(up.x), fabsf(up.y)));
+                  most_g = group_max<T>(most_g, group_max<T>(fabsf(gate.x), fabsf(gate.y)));
+                  most_u = group_max<T>(most_u, group_max<T>(fabsf(up.x), fabsf(up.y)));
                 }
               }
             }

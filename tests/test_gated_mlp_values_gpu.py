@@ -1,0 +1,62 @@
+"""Gated feed-forward block: values that a kept pre-activation has to survive, and how close its results are."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import matterformer_b200 as mfb
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _operands(rows, C, H, O, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    shapes = ((rows, C), (2 * H, C), (O, H), (2 * H,), (O,), (rows, O))
+    scales = (1.0, C**-0.5, H**-0.5, 0.1, 0.1, 1.0)
+    *ops, dy = [(torch.randn(*s, generator=g) * f).to(dtype).cuda() for s, f in zip(shapes, scales)]
+    return ops, dy
+
+
+def _run(ops, dy, act="silu"):
+    leaves = [t.detach().requires_grad_() for t in ops]
+    y = mfb.gated_mlp(*leaves, activation=act)
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+
+def _exact(ops, dy, act="silu"):
+    ops = [t.detach().double().requires_grad_() for t in ops]
+    gate, up = F.linear(ops[0], ops[1], ops[3]).chunk(2, dim=-1)
+    y = F.linear((F.silu(gate) if act == "silu" else F.gelu(gate, approximate="tanh")) * up, ops[2], ops[4])
+    return [y.detach(), *torch.autograd.grad(y, ops, dy.double())]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows", [16, 300])
+def test_a_nan_token_has_nan_gradients(rows, dtype):
+    """All pre-activations of a token are NaN: so is its gradient, and nobody else's."""
+    ops, dy = _operands(rows, 64, 72, 80, dtype, 1)
+    clean = _run(ops, dy)
+    ops[0][3] = float("nan")
+    y, dx, dw_in, dw_out, db_in, db_out = _run(ops, dy)
+    keep = torch.arange(rows) != 3
+    assert y[3].isnan().all() and dx[3].isnan().all()
+    assert torch.equal(y[keep], clean[0][keep]) and torch.equal(dx[keep], clean[1][keep])
+    assert dw_in.isnan().all() and dw_out.isnan().all() and db_in.isnan().all() and torch.equal(db_out, clean[5])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("rows", [16, 300])
+@pytest.mark.parametrize("side", ["gate", "up"])
+def test_a_nan_bias_reaches_its_gradient(rows, side, dtype):
+    """One channel's pre-activation is NaN in every token.  Of the gate it reaches both gradients of the channel, of the up side the gate's; the
+    other groups of 16 channels of the token's kept values are untouched (in bf16 the other channels of its own as well)."""
+    ops, dy = _operands(rows, 64, 80, 72, dtype, 2)
+    clean = _run(ops, dy)[4]
+    at = 21
+    ops[3][at if side == "gate" else 80 + at] = float("nan")
+    got = _run(ops, dy)[4]
+    assert got[at].isnan()
+    assert got[80 + at].isnan() if side == "gate" else got[80 + at] == clean[80 + at]
+    group = torch.arange(160) % 80 // 16 == at // 16 if dtype == F16 else torch.arange(160) % 80 == at
+    assert torch.equal(got[~group], clean[~group])
