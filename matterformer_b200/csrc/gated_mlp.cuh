@@ -47,10 +47,12 @@ __device__ __forceinline__ void activation2(float2 z, float2& value, float2& slo
 // Kept in 16 bits, 16 neighbouring channels of a token scaled by a power of two that goes by the largest, with its exponent in a byte (the
 // bytes of 64 channels, four for gate, four for up, lie together, token by token).  Rounded to the block's type like everything else
 // that goes through memory, they alone put the gradients 1.75 times as far from 64 bits as the rounding of the gradients does;
-// with two more bits it is 1.4 times.
-//   bf16: fp16 with the largest below 2^15: 11 bits down to 2^-29 of the largest.
-//   fp16: sign, 3 bits of exponent, 12 of fraction: 13 bits down to 2^-7 of the largest, from there steps of 2^-19 of it.  What an fp32
-//   value below 2^-120 has in its bits 11-25 is that form, subnormals included: a multiplication and a shift round to it.
+// with a bit more it is 1.5 times, with three 1.4.  With P the power of two in the largest of a group:
+//   bf16: fp16 with the largest below 2^15: 11 bits down to 2^-28 P.
+//   fp16: sign, 4 bits of exponent, 11 of fraction: 12 bits down to 2^-13 P, from there steps of 2^-24 P.  What an fp32 value below
+//   2^-112 has in its bits 12-26 is that form, subnormals included: a multiplication and a shift round to it.  (3 bits of exponent and 12 of
+//   fraction keep a bit more of most values, but less than fp16 itself from 2^-7 P on and nothing below 2^-18 P: channels beside an
+//   outlier would lose their gradients.)
 // A group with an infinity or NaN: bf16 passes it on beside the values that fp16 can hold; fp16 is NaN in all 16.
 // The larger of two magnitudes: in fp16 a NaN wins, so that its group is known; in bf16 the others decide, a NaN needs no exponent.
 template <typename T>
@@ -72,16 +74,16 @@ __device__ __forceinline__ float2 group_scale(uint32_t exponent) {
 }
 template <typename T>
 __device__ __forceinline__ float2 group_unscale(uint32_t exponent) {
-  if constexpr (std::is_same<T, __half>::value) return twice(__uint_as_float(exponent == 255u ? 0x7fffffffu : (exponent - 6u) << 23));
+  if (std::is_same<T, __half>::value && exponent == 255u) return twice(__uint_as_float(0x7fffffffu));
   return twice(__uint_as_float((exponent - 14u) << 23));
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack_pre(float2 v, float2 scale) {
   v = mul2(v, scale);
   if constexpr (std::is_same<T, __half>::value) {
-    v = mul2(v, twice(__uint_as_float(1u << 14)));  // 2^-135
-    const uint32_t a = __float_as_uint(v.x) + 0x400u, b = __float_as_uint(v.y) + 0x400u;
-    return (a >> 11 & 0x7fffu) | (a >> 16 & 0x8000u) | (b << 5 & 0x7fff0000u) | (b & 0x80000000u);
+    v = mul2(v, twice(__uint_as_float(1u << 22)));  // 2^-127
+    const uint32_t a = __float_as_uint(v.x) + 0x800u, b = __float_as_uint(v.y) + 0x800u;
+    return (a >> 12 & 0x7fffu) | (a >> 16 & 0x8000u) | (b << 4 & 0x7fff0000u) | (b & 0x80000000u);
   } else {
     return pack2<__half>(v.x, v.y);
   }
@@ -90,7 +92,7 @@ template <typename T>
 __device__ __forceinline__ float2 unpack_pre(uint32_t w, float2 unscale) {
   float2 v;
   if constexpr (std::is_same<T, __half>::value) {
-    v = make_float2(__uint_as_float((w << 11 & 0x03fff800u) | (w << 16 & 0x80000000u)), __uint_as_float((w >> 5 & 0x03fff800u) | (w & 0x80000000u)));
+    v = make_float2(__uint_as_float((w << 12 & 0x07fff000u) | (w << 16 & 0x80000000u)), __uint_as_float((w >> 4 & 0x07fff000u) | (w & 0x80000000u)));
     v = mul2(v, twice(__uint_as_float(254u << 23)));  // 2^127
   } else {
     v = unpack2<__half>(w);

@@ -135,9 +135,9 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     :func:`matterformer_b200.linear.bf16_copies`).  ``activation``: "silu" or "gelu_tanh".  Returns (..., O) in ``x``'s type.
 
     Sums are in fp32 in a fixed order.  The hidden values and the gradients of the pre-activations are rounded to ``x``'s type; hidden values
-    that fp16 cannot hold (above 65504) are infinities there.  What the backward pass gets of the pre-activations has some bits more than
-    ``x``'s type, counted from the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-29 of that (bf16), 13 down to 2^-7 of
-    it and a bit less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable."""
+    that fp16 cannot hold (above 65504) are infinities there.  What the backward pass gets of the pre-activations has more bits than
+    ``x``'s type, counted from the power of two in the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-28 of that (bf16),
+    12 down to 2^-13 of it and one less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable."""
     native = _lib.native()
     if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++
         out = native.gated_mlp(x, w_in, w_out, b_in, b_out, ACTIVATIONS[activation])

@@ -60,3 +60,31 @@ def test_a_nan_bias_reaches_its_gradient(rows, side, dtype):
     assert got[80 + at].isnan() if side == "gate" else got[80 + at] == clean[80 + at]
     group = torch.arange(160) % 80 // 16 == at // 16 if dtype == F16 else torch.arange(160) % 80 == at
     assert torch.equal(got[~group], clean[~group])
+
+
+@pytest.mark.parametrize("rows", [16, 300])
+@pytest.mark.parametrize("outlier", [10, 13, 16])
+def test_fp16_channels_beside_an_outlier(rows, outlier):
+    """One channel's up projection is 2^outlier times its neighbours'.  The fp16 form keeps 12 bits, one more than fp16 has, down to 2^-13 of the power
+    of two in the largest of a group, and steps of 2^-24 of that below: a value of the others is off by 2^-12 of itself or half such a step.
+
+    The gradient of the gate's rows is a sum over the tokens of dh act'(g) u x: of the error of u by steps, each token's at most, added in squares
+    (twice for the room of a sum of few); of the roundings of its own, 6 of 2^-11 as for every gradient of the block; of the steps of 2^-24
+    that fp16 itself ends at, in every token's gradient of the pre-activations and in the result."""
+    ops, dy = _operands(rows, 64, 80, 72, F16, 3)
+    ops[1] *= 0.25
+    ops[1][80 + 5] *= 2.0**6  # the projection holds 2^6 of it, the neighbours are made smaller by the rest
+    others = [c for c in range(16) if c != 5]
+    ops[1][[80 + c for c in others]] *= 2.0 ** (6 - outlier)
+    ops[3].zero_()
+    ops[2][:, 5] *= 2.0**-6
+    got, want = _run(ops, dy)[2], _exact(ops, dy)[2]
+    gate, up = F.linear(ops[0].double(), ops[1].double()).chunk(2, dim=-1)
+    s = torch.sigmoid(gate)
+    slope = s * (1 + gate * (1 - s))
+    dh = dy.double() @ ops[2].double()
+    step = up[:, :16].abs().amax(dim=1, keepdim=True) * 2.0**-25
+    of_steps = 2 * ((dh * slope)[:, :16] * step).square().t() @ ops[0].double().square()
+    for c in others:
+        off = (got[c].double() - want[c]).norm()
+        assert off <= 6 * 2.0**-11 * want[c].norm() + of_steps[c].sum().sqrt() + 2.0**-24 * (rows * want.shape[1]) ** 0.5
