@@ -689,8 +689,9 @@ int mf_rotary(const MfRotaryArgs* args, void* stream);
  * not NULL.  Sums are in fp32 and in a fixed order; act and the gradients of the pre-activations are rounded to dtype, the
  * pre-activations to more bits, counted from the largest of 16 neighbouring channels: 11 (bf16) or 12 (fp16).
  * Workspace: forward mf_gated_mlp_fwd_workspace_bytes (without it some sizes take longer), backward mf_gated_mlp_bwd_workspace_bytes
- * for the same gradients.  An expired device-side wait is reported by
- * mf_gated_mlp_status (which synchronises `stream`); the outputs of such a call are undefined.
+ * for the same gradients.  The outputs of a call with an expired
+ * device-side wait are undefined; mf_gated_mlp_status (which synchronises `stream`) returns its code for the calls on the device since it was
+ * last asked, once.
  */
 typedef struct MfGatedMlpArgs {
   int64_t rows;
@@ -723,7 +724,8 @@ int mf_gated_mlp_fwd(const MfGatedMlpArgs* args, void* stream);
 int mf_gated_mlp_bwd(const MfGatedMlpArgs* args, void* stream);
 int mf_gated_mlp_status(int32_t* host_status, void* stream);
 /* Runs the call with the hand-offs of one kind withheld (0 operands, 1 stages, 2 accumulators, 3 drained accumulators) and waits that
- * expire after limit_cycles; returns the status it left and clears it.  The call's outputs are undefined. */
+ * expire after limit_cycles; returns the status it left, which no call and no mf_gated_mlp_status sees.  With host_status NULL it
+ * leaves it to the latter, as an expired call does.  The call's outputs are undefined. */
 int mf_selftest_gated_mlp_give_up(const MfGatedMlpArgs* args, int32_t backward, int32_t kind, int64_t limit_cycles, int32_t* host_status,
                                   void* stream);
 

@@ -50,6 +50,7 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 struct BoundedWaits {
   long long limit = 1ll << 31;  // kWaitLimitCycles
   int withheld = -1;
+  int word = 0;  // of the status words of kernels that have several, the one that an expired wait sets
 };
 
 // ---- launches that begin while the kernel before them ends ------------------------

@@ -8,6 +8,8 @@
 // 29 696 tokens x 512 x 2048, forward and all gradients: 520-590 us, 0.95-1.08 PFLOP/s (cuBLAS sustains 1.39 in one long product, bursts at 1.64):
 // projections 115, output 58, gate gradient 112 (486 MB: memory bounds it, the others the tensor cores at the clock that the power limit
 // leaves), gradients 213.  8192 x 2048 x 5464: 1420 us, 1.16 PFLOP/s.
+#include <mutex>
+
 #include "common.cuh"
 #include "gemm_sm100.cuh"
 
@@ -435,12 +437,16 @@ int run_backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_
   return a->dtype == MF_DTYPE_BF16 ? backward<__nv_bfloat16>(a, waits, stream) : backward<__half>(a, waits, stream);
 }
 
-int read_status(int32_t* host_status, cudaStream_t stream, bool clear) {
-  static const int32_t kNone = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(host_status, g_gemm_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
+// Reads a status word and clears it in one step, so that an expired wait is reported once and none is lost.
+__device__ int32_t g_taken_status;
+__global__ void take_status_kernel(int word) { g_taken_status = atomicExch(&g_gemm_status[word], 0); }
+int take_status(int word, int32_t* host_status, cudaStream_t stream) {
+  static std::mutex one_at_a_time;  // (the word it goes through)
+  const std::lock_guard<std::mutex> lock(one_at_a_time);
+  take_status_kernel<<<1, 1, 0, stream>>>(word);
+  MF_CHECK_LAUNCH("gated_mlp status read-back");
+  cudaError_t e = cudaMemcpyFromSymbolAsync(host_status, g_taken_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
-  if (e == cudaSuccess && clear) e = cudaMemcpyToSymbolAsync(g_gemm_status, &kNone, sizeof(int32_t), 0, cudaMemcpyHostToDevice, stream);
-  if (e == cudaSuccess && clear) e = cudaStreamSynchronize(stream);
   return e == cudaSuccess ? MF_OK : cuda_error(e, "gated_mlp status read-back");
 }
 
@@ -465,15 +471,15 @@ extern "C" int mf_gated_mlp_fwd(const MfGatedMlpArgs* a, void* stream) { return 
 extern "C" int mf_gated_mlp_bwd(const MfGatedMlpArgs* a, void* stream) { return run_backward(a, BoundedWaits{}, static_cast<cudaStream_t>(stream)); }
 extern "C" int mf_gated_mlp_status(int32_t* host_status, void* stream) {
   MF_CHECK_ARG(host_status != nullptr, "mf_gated_mlp_status: null pointer");
-  return read_status(host_status, static_cast<cudaStream_t>(stream), false);
+  return take_status(0, host_status, static_cast<cudaStream_t>(stream));
 }
 extern "C" int mf_selftest_gated_mlp_give_up(const MfGatedMlpArgs* a, int32_t backward, int32_t kind, int64_t limit_cycles, int32_t* host_status,
                                              void* stream) {
-  MF_CHECK_ARG(a && host_status && kind >= 0 && kind <= 3, "mf_selftest_gated_mlp_give_up: bad argument");
+  MF_CHECK_ARG(a && kind >= 0 && kind <= 3, "mf_selftest_gated_mlp_give_up: bad argument");
   MF_CHECK_ARG(limit_cycles > 0 && limit_cycles <= kWaitLimitCycles, "mf_selftest_gated_mlp_give_up: the limit must lie in (0, 2^31] clocks");
   BoundedWaits waits;
-  waits.limit = limit_cycles, waits.withheld = kind;
+  waits.limit = limit_cycles, waits.withheld = kind, waits.word = host_status != nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int rc = backward ? run_backward(a, waits, s) : run_forward(a, waits, s);
-  return rc != MF_OK ? rc : read_status(host_status, s, true);
+  return rc != MF_OK || !host_status ? rc : take_status(1, host_status, s);
 }

@@ -27,7 +27,8 @@
 namespace mf {
 namespace gemm {
 
-__device__ int32_t g_gemm_status = 0;  // MF_ERR_DEVICE_TIMEOUT after an expired wait
+// MF_ERR_DEVICE_TIMEOUT after an expired wait, until it is read: of calls | of the self-test
+__device__ int32_t g_gemm_status[2] = {0, 0};
 
 // kGate: two projections, activation and product; kGateKeep: the pre-activations are stored as well; kGateGrad: the gradient of both;
 // kStore: the product and a bias; kGradients: the weights' gradients, two products over the same long dimension (of operands that have it
@@ -772,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       store_wait_all();
     }
   }
-  if (bad) atomicExch(&g_gemm_status, MF_ERR_DEVICE_TIMEOUT);
+  if (bad) atomicExch(&g_gemm_status[p.waits.word], MF_ERR_DEVICE_TIMEOUT);
   __syncwarp();
   tc_fence_before_sync();
   cluster_sync();  // no arrival, copy or product of either CTA is outstanding

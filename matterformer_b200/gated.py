@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, simplicial
 from .linear import bf16_copy
 
 _ONCE = b"trying to differentiate twice a function that was marked with @once_differentiable"
@@ -42,6 +42,14 @@ def _args(x, w_in, w_out, b_in, b_out, activation, grad_dtype):
     return a
 
 
+def _raise_expired(device: torch.device) -> None:
+    """After a call, where the caller has asked for it (see :func:`matterformer_b200.set_check_status`)."""
+    if simplicial._CHECK_STATUS and not torch.cuda.is_current_stream_capturing():
+        code = gated_mlp_status(device)
+        if code != 0:
+            raise RuntimeError(f"a device-side wait of the gated block's kernels expired (status {code}); the outputs of that call are undefined")
+
+
 class _GatedMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, activation):
@@ -61,6 +69,7 @@ class _GatedMlp(torch.autograd.Function):
             ws = torch.empty(need, device=x.device, dtype=torch.uint8)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _lib.launch(L.mf_gated_mlp_fwd, x.device, ctypes.byref(a))
+        _raise_expired(x.device)
         if keep:
             ctx.foreign = _lib.foreign_leaves(x, w_in, w_out, b_in, b_out)
             ctx.save_for_backward(x2, *params, pre, act)
@@ -93,6 +102,7 @@ class _GatedMlp(torch.autograd.Function):
         ws = torch.empty(max(need, 16), device=x.device, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
         _lib.launch(L.mf_gated_mlp_bwd, x.device, ctypes.byref(a))
+        _raise_expired(x.device)
         if grads[0] is not None:
             grads[0] = grads[0].view(ctx.shape)
         return grads
@@ -138,7 +148,7 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     that fp16 cannot hold (above 65504) are infinities there.  What the backward pass gets of the pre-activations has more bits than
     ``x``'s type, counted from the power of two in the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-28 of that (bf16),
     12 down to 2^-13 of it and one less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable."""
-    native = _lib.native()
+    native = _lib.native() if not simplicial._CHECK_STATUS else None
     if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++
         out = native.gated_mlp(x, w_in, w_out, b_in, b_out, ACTIVATIONS[activation])
         if out is not None:
@@ -148,8 +158,8 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
 
 
 def gated_mlp_status(device=None) -> int:
-    """Status word of the block's kernels: 0, or the code of an expired device-side wait (the outputs of that call are undefined).
-    Synchronises the current stream."""
+    """0, or the code of a device-side wait that expired in one of the block's calls on the device since this was last asked; the outputs
+    of that call are undefined.  Synchronises the current stream.  :func:`set_check_status` asks after every call."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     out = ctypes.c_int32(0)
     _lib.launch(_lib.lib().mf_gated_mlp_status, dev, ctypes.byref(out))

@@ -52,8 +52,8 @@ _CHECK_STATUS = os.environ.get("MF_CHECK_STATUS", "0") not in ("", "0")
 
 
 def set_check_status(on: bool) -> bool:
-    """When on, every tensor-core simplicial call reads its status word back (this synchronises the stream) and
-    raises ``RuntimeError`` if a bounded device-side wait expired.  Skipped while a CUDA graph is being captured.
+    """When on, every tensor-core simplicial call and every call of the gated block reads its status word back (this synchronises
+    the stream) and raises ``RuntimeError`` if a bounded device-side wait expired.  Skipped while a CUDA graph is being captured.
     Also switched on by the environment variable ``MF_CHECK_STATUS=1``.  Returns the previous setting."""
     global _CHECK_STATUS
     prev, _CHECK_STATUS = _CHECK_STATUS, bool(on)
