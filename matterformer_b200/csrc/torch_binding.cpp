@@ -9,8 +9,11 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -344,6 +347,12 @@ bool foreign_leaf(const Tensor& t) {
   const auto stream = node->stream();
   return stream && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap();
 }
+// Whether something follows the operations of this thread and would not see a kernel launched past them: a trace, a dispatch mode, a
+// transform of torch.func.  (What matterformer_b200.fused.watched asks, without its microsecond.)
+bool watched() {
+  return torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::stack_len() > 0 ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
 bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
 bool foreign_leaves(std::initializer_list<const Tensor*> inputs) {
   if (!at::GradMode::is_enabled() || !capturing()) return false;
@@ -439,9 +448,9 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
   }
 };
 
-// Parameters in the type of x, everything contiguous and aligned.  (Forward-mode tangents and functorch's wrappers have their own way.)
+// Parameters in the type of x, everything contiguous and aligned, nothing that watches.
 std::optional<Tensor> gated_mlp(const Tensor& x, const Tensor& w_in, const Tensor& w_out, const OptTensor& b_in, const OptTensor& b_out, int64_t activation) {
-  if (!x.is_cuda() || x.dim() < 1 || (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kHalf) || !x.is_contiguous() || x.numel() == 0) return std::nullopt;
+  if (watched() || !x.is_cuda() || x.dim() < 1 || (x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kHalf) || !x.is_contiguous() || x.numel() == 0) return std::nullopt;
   if (w_out.dim() != 2) return std::nullopt;
   const int64_t C = x.size(-1), O = w_out.size(0), F = w_out.size(1);
   if (C % 8 || O % 8 || F % 8 || C < 8 || O < 8 || F < 8 || std::max({C, O, F}) > 1 << 28) return std::nullopt;
@@ -548,7 +557,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 
 std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, const Tensor& positions, const Tensor& table, int64_t heads, int64_t layout,
                                   double amplitude) {
-  if (!first.is_cuda() || dtype_code(first) < 0 || first.dim() != (heads ? 3 : 4) || first.numel() == 0 || !std::isfinite(amplitude)) return std::nullopt;
+  if (watched() || !first.is_cuda() || dtype_code(first) < 0 || first.dim() != (heads ? 3 : 4) || first.numel() == 0 || !std::isfinite(amplitude)) return std::nullopt;
   if (heads < 0 || (heads && first.size(2) % (3 * heads))) return std::nullopt;
   const int64_t B = first.size(0), N = first.size(heads ? 1 : 2), D = heads ? first.size(2) / (3 * heads) : first.size(3);
   if (second && (second->dim() != 4 || second->scalar_type() != first.scalar_type() || second->device() != first.device() || second->numel() == 0 ||

@@ -11,8 +11,10 @@ import ctypes
 from typing import Optional
 
 import torch
+import torch.nn.functional as F
 
 from . import _lib, simplicial
+from .fused import watched
 from .linear import bf16_copy
 
 _ONCE = b"trying to differentiate twice a function that was marked with @once_differentiable"
@@ -56,11 +58,11 @@ class _GatedMlp(torch.autograd.Function):
         ctx.shape, ctx.activation, ctx.grad_dtype = x.shape, activation, w_in.dtype
         x2 = _ready(x.reshape(-1, x.shape[-1]))
         params = [_ready(bf16_copy(p) if p is not None and p.dtype != x.dtype else p) for p in (w_in, w_out, b_in, b_out)]
-        rows, F = x2.shape[0], w_out.shape[1]
+        rows, hidden = x2.shape[0], w_out.shape[1]
         y = torch.empty((rows, w_out.shape[0]), device=x.device, dtype=x.dtype)
-        act = torch.empty((rows, F), device=x.device, dtype=x.dtype)
+        act = torch.empty((rows, hidden), device=x.device, dtype=x.dtype)
         keep = any(ctx.needs_input_grad)
-        pre = torch.empty(_lib.lib().mf_gated_mlp_pre_bytes(rows, F), device=x.device, dtype=torch.uint8) if keep else None
+        pre = torch.empty(_lib.lib().mf_gated_mlp_pre_bytes(rows, hidden), device=x.device, dtype=torch.uint8) if keep else None
         a = _args(x2, *params, activation, ctx.grad_dtype)
         a.pre, a.act, a.y = _ptr(pre), _ptr(act), _ptr(y)
         L = _lib.lib()
@@ -108,6 +110,13 @@ class _GatedMlp(torch.autograd.Function):
         return grads
 
 
+def _plain(x, w_in, w_out, b_in, b_out, activation):
+    """The block in torch operations, in ``x``'s type."""
+    w_in, w_out, b_in, b_out = (None if p is None else p.to(x.dtype) for p in (w_in, w_out, b_in, b_out))
+    gate, up = F.linear(x, w_in, b_in).chunk(2, dim=-1)
+    return F.linear((F.silu(gate) if activation == "silu" else F.gelu(gate, approximate="tanh")) * up, w_out, b_out)
+
+
 def gated_mlp_applies(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> bool:
     """Whether the kernels take these operands: CUDA, 16-bit ``x``, parameters of its type (or fp32 beside bf16), widths that are
     multiples of 8."""
@@ -147,13 +156,16 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
     Sums are in fp32 in a fixed order.  The hidden values and the gradients of the pre-activations are rounded to ``x``'s type; hidden values
     that fp16 cannot hold (above 65504) are infinities there.  What the backward pass gets of the pre-activations has more bits than
     ``x``'s type, counted from the power of two in the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-28 of that (bf16),
-    12 down to 2^-13 of it and one less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable."""
-    native = _lib.native() if not simplicial._CHECK_STATUS else None
+    12 down to 2^-13 of it and one less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable.  What is traced
+    or under a transform of ``torch.func`` is the same in plain operations, rounded after each."""
+    native = None if simplicial._CHECK_STATUS else _lib.native()
     if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++
         out = native.gated_mlp(x, w_in, w_out, b_in, b_out, ACTIVATIONS[activation])
         if out is not None:
             return out
     _check(x, w_in, w_out, b_in, b_out, activation)
+    if watched(*(t for t in (x, w_in, w_out, b_in, b_out) if t is not None)):
+        return _plain(x, w_in, w_out, b_in, b_out, activation)
     return _GatedMlp.apply(x, w_in, w_out, b_in, b_out, activation)
 
 

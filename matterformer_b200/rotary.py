@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .fused import watched
 from .simplicial import _DTYPE_CODE
 
 MAX_PAIRS = 128
@@ -84,6 +85,14 @@ def rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Te
     turned = (a * cos - b * sin, a * sin + b * cos)
     turned = torch.cat(turned, dim=-1) if layout == "half" else torch.stack(turned, dim=-1).flatten(-2)
     return torch.cat([turned.to(x.dtype), x[..., 2 * P :]], dim=-1)
+
+
+def rotate_packed_torch(qkv: torch.Tensor, heads: int, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half",
+                        amplitude: float = 1.0) -> torch.Tensor:  # fmt: skip
+    """:func:`rotary_packed` in plain torch operations, on any device."""
+    q, k, v = qkv.unflatten(-1, (3, heads, -1)).unbind(-3)  # (B, N, H, D) each
+    q, k = (rotate_torch(t.transpose(1, 2), positions, frequencies, layout, amplitude).transpose(1, 2) for t in (q, k))
+    return torch.stack([q, k, v], dim=-3).flatten(-3)
 
 
 def _fill(tensor, x, out, heads, rotates, strides_in, strides_out):
@@ -180,6 +189,11 @@ def _ready(a, b, positions, frequencies, heads, layout, amplitude):
 
 
 def _apply(a, b, positions, frequencies, heads, layout, amplitude):
+    if watched(*(t for t in (a, b, positions) if t is not None)):  # plain operations, which whatever watches can see
+        if heads:
+            return rotate_packed_torch(a, heads, positions, frequencies, layout, amplitude)
+        turned = [rotate_torch(t, positions, frequencies, layout, amplitude) for t in (a, b) if t is not None]
+        return turned[0] if b is None else tuple(turned)
     positions, table = positions.contiguous(), frequencies.double().contiguous()
     return _Rotary.apply(a, b, positions, table, heads, layout, float(amplitude), False)
 
