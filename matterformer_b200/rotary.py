@@ -173,7 +173,7 @@ def _check(name, tensors, tokens, batch, heads, head_dim, positions, frequencies
     axes = () if frequencies.ndim == 1 else (frequencies.shape[0],)
     if positions.dtype not in _lib.MF_POSITION:
         raise ValueError(f"{name}: positions must be int32, int64, float32 or float64, got {positions.dtype}")
-    if positions.requires_grad:
+    if positions.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: positions get no gradient; pass them detached")
     if positions.device != x.device or positions.shape not in ((tokens, *axes), (batch, tokens, *axes)):
         raise ValueError(f"{name}: positions of shape {(batch, tokens, *axes)} or {(tokens, *axes)} on {x.device} expected, got "
@@ -194,7 +194,7 @@ def _apply(a, b, positions, frequencies, heads, layout, amplitude):
             return rotate_packed_torch(a, heads, positions, frequencies, layout, amplitude)
         turned = [rotate_torch(t, positions, frequencies, layout, amplitude) for t in (a, b) if t is not None]
         return turned[0] if b is None else tuple(turned)
-    positions, table = positions.contiguous(), frequencies.double().contiguous()
+    positions, table = positions.detach().contiguous(), frequencies.double().contiguous()
     return _Rotary.apply(a, b, positions, table, heads, layout, float(amplitude), False)
 
 

@@ -33,7 +33,7 @@ from .fused import (fused_applies, gated_layer_norm, gated_ln_modulate, gated_re
                     split_modulation)
 from .gated import gated_mlp, gated_mlp_applies
 from .linear import bf16_copies, linear_bf16, linear_bf16_applies, linear_gelu_bf16, pair_linear_bf16, stacked_modulation
-from .rotary import RotaryPositions, rotary_embedding, rotary_packed, rotate_torch
+from .rotary import RotaryPositions, rotary_embedding, rotary_packed, rotate_packed_torch, rotate_torch
 from .simplicial import (_DTYPE_CODE, normalize_simplicial_precision, packed_projection_applies, simplicial_attention_cuda,
                          simplicial_attention_packed)  # fmt: skip
 
@@ -245,9 +245,19 @@ class RegularAttention(nn.Module):
     def _turned(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor):
         """Queries and keys, (B, H, N, D) each."""
         r = self.rotary
-        if q.is_cuda and self.impl != "torch" and q.dtype in _DTYPE_CODE:
-            return rotary_embedding(q, k, positions, r.frequencies, layout=r.layout, amplitude=r.amplitude)
+        if q.is_cuda and self.impl != "torch" and q.dtype in _DTYPE_CODE and not self._differentiated(positions):
+            return rotary_embedding(q, k, self._kernel_positions(positions), r.frequencies, layout=r.layout, amplitude=r.amplitude)
         return tuple(rotate_torch(t, positions, r.frequencies, r.layout, r.amplitude) for t in (q, k))
+
+    @staticmethod
+    def _differentiated(positions: torch.Tensor) -> bool:
+        """Whether the positions want a gradient (coordinates under guidance): the plain operations have one, the kernels do not."""
+        return positions.requires_grad and torch.is_grad_enabled()
+
+    @staticmethod
+    def _kernel_positions(positions: torch.Tensor) -> torch.Tensor:
+        """As the kernels take them: 16-bit coordinates in 32 bits."""
+        return positions.float() if positions.dtype in (torch.bfloat16, torch.float16) else positions
 
     def _dense_rotary(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor], positions: torch.Tensor) -> torch.Tensor:
         B, N, C = x.shape
@@ -284,7 +294,8 @@ class RegularAttention(nn.Module):
                 sparse_plan: Optional[SparseAttentionPlan] = None, num_atoms: Optional[torch.Tensor] = None,
                 padding_is_suffix: Optional[bool] = None, positions: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
         """``num_atoms``: the (B,) int32 counts of real tokens, ``padding_is_suffix``: the form of the mask, when the caller
-        has already found them.  ``positions``: of the tokens, for a layer with ``rotary`` (see :func:`rotary_embedding`); others take none."""
+        has already found them.  ``positions``: of the tokens, for a layer with ``rotary`` (see :func:`rotary_embedding`); others take
+        none.  They may be of 16 bits and may want a gradient, which plain operations then form."""
         if (self.rotary is None) != (positions is None):
             raise ValueError("a layer with rotary positions needs `positions`" if positions is None else
                              "`positions` are for a layer with rotary positions")  # fmt: skip
@@ -310,7 +321,10 @@ class RegularAttention(nn.Module):
             num_atoms = (~key_padding_mask).sum(dim=1).to(torch.int32)
         if positions is not None:
             r = self.rotary
-            qkv = rotary_packed(qkv, H, positions, r.frequencies, layout=r.layout, amplitude=r.amplitude)
+            if self._differentiated(positions):
+                qkv = rotate_packed_torch(qkv, H, positions, r.frequencies, r.layout, r.amplitude)
+            else:
+                qkv = rotary_packed(qkv, H, self._kernel_positions(positions), r.frequencies, layout=r.layout, amplitude=r.amplitude)
         # with at most 32 tokens the window-64 band covers every real token: dense attention, straight on the projection
         core = local_window_attention_packed(qkv, H, num_atoms, window=64)
         return linear_bf16(core, self.attn.out_proj.weight, self.attn.out_proj.bias)
