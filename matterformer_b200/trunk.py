@@ -264,8 +264,14 @@ class RegularAttention(nn.Module):
         H = self.attn.num_heads
         qkv = linear_bf16(x, self.attn.in_proj_weight, self.attn.in_proj_bias)
         q, k, v = qkv.view(B, N, 3, H, C // H).permute(2, 0, 3, 1, 4)
+        visible = None
+        if key_padding_mask is not None:
+            visible = ~key_padding_mask.bool()[:, None, None, :]
+            if positions.ndim == self.rotary.frequencies.ndim + 1:  # (each molecule has its own)
+                # the core hides a padded key's score, but one that is not a number would reach every row of the molecule all the same
+                hidden = key_padding_mask.bool()
+                positions = positions.masked_fill((hidden if positions.ndim == 2 else hidden[..., None]) & ~positions.isfinite(), 0)
         q, k = self._turned(q, k, positions)
-        visible = None if key_padding_mask is None else ~key_padding_mask.bool()[:, None, None, :]
         core = F.scaled_dot_product_attention(q, k, v, attn_mask=visible, dropout_p=self.attn.dropout if self.training else 0.0)
         return linear_bf16(core.transpose(1, 2).reshape(B, N, C), self.attn.out_proj.weight, self.attn.out_proj.bias)
 

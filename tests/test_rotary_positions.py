@@ -89,3 +89,20 @@ def test_coordinates_of_16_bits_and_without_grad_mode():
         assert torch.equal(mfb.rotary_embedding(q, None, p, ROTARY.frequencies)[0], mfb.rotary_embedding(q, None, p.detach(), ROTARY.frequencies)[0])
     with pytest.raises(ValueError, match="no gradient"):
         mfb.rotary_embedding(q, None, p, ROTARY.frequencies)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 1e30])
+def test_positions_of_padded_tokens_reach_nobody(device, value):
+    """The dense core masks scores, which a NaN among the keys would survive."""
+    layer, (x, pos, pad, dy) = _layer().to(device), _inputs()
+    x, pos, pad, dy = (t.to(device) for t in (x, pos, pad, dy))
+    for mask, g in ((pad, dy), (pad.flip(1), dy.flip(1))):
+        outs = []
+        for p in (pos, pos.masked_fill(mask[..., None], value)):
+            leaf = x.clone().requires_grad_()
+            y = layer(leaf, key_padding_mask=mask, positions=p)
+            outs.append([y.masked_fill(mask[..., None], 0.0), torch.autograd.grad(y, leaf, g)[0]])
+        assert torch.equal(outs[0][0], outs[1][0])
+        real = ~mask
+        assert torch.equal(outs[0][1][real], outs[1][1][real]) and outs[1][1].isfinite().all()
