@@ -219,6 +219,8 @@ class RegularAttention(nn.Module):
     then ``F.scaled_dot_product_attention``, since ``nn.MultiheadAttention`` has no place for it.
     """
 
+    rotary: Optional[RotaryPositions] = None  # (of the class as well: modules that were stored before it existed have none of their own)
+
     def __init__(self, embed_dim: int, num_heads: int, *, dropout: float = 0.0, impl: str = "auto",
                  rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
         super().__init__()
@@ -473,6 +475,8 @@ class AdaLNBlock(nn.Module):
 
 class TransformerTrunk(nn.Module):
     """Stack of :class:`AdaLNBlock`; ``attn_types`` names the attention of every layer, e.g. alternating."""
+
+    rotary: Optional[RotaryPositions] = None  # (see RegularAttention)
 
     def __init__(self, d_model: int, n_heads: int, attn_types: Sequence[str], *, mlp_ratio: float = 4.0,
                  eps: float = 1e-6, simplicial_impl: str = "auto", simplicial_precision: str = "bf16_tc",

@@ -1,12 +1,13 @@
-"""Positions as models have them: coordinates with a gradient, of 16 bits, not a number on padded tokens."""
+"""Positions as models have them: coordinates with a gradient, of 16 bits, not a number on padded tokens; layers of an earlier version."""
 import copy
+import pickle
 
 import pytest
 import torch
 
 import matterformer_b200 as mfb
 from matterformer_b200.rotary import RotaryPositions
-from matterformer_b200.trunk import EDMModel, RegularAttention
+from matterformer_b200.trunk import EDMModel, RegularAttention, TransformerTrunk
 
 ROTARY = RotaryPositions(rotary_dim=24, axes=3, base=50.0)
 
@@ -106,3 +107,16 @@ def test_positions_of_padded_tokens_reach_nobody(device, value):
         assert torch.equal(outs[0][0], outs[1][0])
         real = ~mask
         assert torch.equal(outs[0][1][real], outs[1][1][real]) and outs[1][1].isfinite().all()
+
+
+def test_layers_of_an_earlier_version():
+    """A module that was stored whole before there were rotary positions has no such attribute."""
+    torch.manual_seed(4)
+    trunk = TransformerTrunk(32, 4, ["mha"])
+    x, cond = torch.randn(2, 5, 32), torch.randn(2, 32)
+    want = trunk(x, cond)
+    state = pickle.dumps(trunk)
+    old = pickle.loads(state)
+    for m in old.modules():
+        m.__dict__.pop("rotary", None)
+    assert torch.equal(old(x, cond), want)
