@@ -67,8 +67,9 @@ class RotaryPositions:
 
     @functools.cached_property
     def frequencies(self) -> torch.Tensor:
-        return rotary_frequencies(self.rotary_dim, axes=self.axes, base=self.base, scaling=self.scaling, factor=self.factor,
-                                  original_length=self.original_length)  # fmt: skip
+        with torch.inference_mode(False):  # (kept: an ordinary tensor, whoever asks first)
+            return rotary_frequencies(self.rotary_dim, axes=self.axes, base=self.base, scaling=self.scaling, factor=self.factor,
+                                      original_length=self.original_length)  # fmt: skip
 
 
 def rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:

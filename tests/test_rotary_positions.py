@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import matterformer_b200 as mfb
-from matterformer_b200.rotary import RotaryPositions
+from matterformer_b200.rotary import RotaryPositions, rotate_torch
 from matterformer_b200.trunk import EDMModel, RegularAttention, TransformerTrunk
 
 ROTARY = RotaryPositions(rotary_dim=24, axes=3, base=50.0)
@@ -120,3 +120,13 @@ def test_layers_of_an_earlier_version():
     for m in old.modules():
         m.__dict__.pop("rotary", None)
     assert torch.equal(old(x, cond), want)
+
+
+def test_frequencies_first_asked_for_in_inference_mode():
+    """They are made once and kept: as ordinary tensors, whoever asks first."""
+    rotary = RotaryPositions(rotary_dim=12, axes=3)
+    with torch.inference_mode():
+        rotary.frequencies
+    pos = torch.randn(1, 4, 3, requires_grad=True)
+    y = rotate_torch(torch.randn(1, 2, 4, 16), pos, rotary.frequencies)
+    assert torch.autograd.grad(y.sum(), pos)[0].isfinite().all()
