@@ -223,11 +223,14 @@ __global__ void __launch_bounds__(256) add_planes_kernel(const float* planes, Pl
   else *reinterpret_cast<uint2*>(to) = make_uint2(pack2<TOut>(s.x, s.y), pack2<TOut>(s.z, s.w));
 }
 
-size_t pieces(const MfGatedMlpArgs* a, bool backward, size_t (&at)[4]) {  // gradient of the pre-activations | planes | bias sums | their bands
+bool forms_pre_gradient(const MfGatedMlpArgs* a) { return a->grad_x || a->grad_w_in || a->grad_b_in; }
+
+// The backward pass's workspace: gradient of the pre-activations | planes | bias sums | their bands
+size_t pieces(const MfGatedMlpArgs* a, size_t (&at)[4]) {
   const size_t size = 2, rows = (size_t)a->rows, F = a->hidden;
-  at[0] = 0;
-  if (!backward || rows == 0) return 0;
-  at[1] = at[0] + align_up(rows * 2 * F * size, 256);
+  at[0] = at[1] = at[2] = at[3] = 0;
+  if (rows == 0) return 0;
+  at[1] = at[0] + (forms_pre_gradient(a) ? align_up(rows * 2 * F * size, 256) : 0);
   const size_t planes = a->grad_w_in || a->grad_w_out ? plane_bytes(plan_of(a)) : 0;
   at[2] = at[1] + align_up(planes, 256);
   at[3] = at[2] + (a->grad_b_in ? align_up((size_t)((a->rows + 31) / 32) * 2 * F * 4, 256) : 0);
@@ -364,14 +367,14 @@ template <typename T>
 int backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_t stream) {
   const long long M = a->rows, C = a->dim, F = a->hidden, O = a->dim_out;
   size_t at[4];
-  pieces(a, true, at);
+  pieces(a, at);
   char* ws = static_cast<char*>(a->workspace);
   T* grad_pre = reinterpret_cast<T*>(ws + at[0]);
   float *planes = reinterpret_cast<float*>(ws + at[1]), *sums = reinterpret_cast<float*>(ws + at[2]);
   const bool biased = a->grad_b_in || a->grad_b_out;
   const BiasSums b = {a->grad_y, sums, biased ? reinterpret_cast<float*>(ws + at[3]) : nullptr, M, a->grad_b_out ? (int)O : 0, a->grad_b_in ? (int)(2 * F) : 0};
   int rc;
-  if (a->grad_x || a->grad_w_in || a->grad_b_in) {
+  if (forms_pre_gradient(a)) {
     Params p = common(M, F, O, waits);
     p.column_sums = a->grad_b_in ? sums : nullptr;
     p.exponents = exponents_of(a);
@@ -429,7 +432,7 @@ int run_backward(const MfGatedMlpArgs* a, const BoundedWaits& waits, cudaStream_
   }
   MF_CHECK_ARG(a->grad_y && a->pre, "%s: null tensor", kName);
   size_t at[4];
-  const size_t need = pieces(a, true, at);
+  const size_t need = pieces(a, at);
   if (need && (!a->workspace || a->workspace_bytes < need)) {
     set_error("%s: workspace too small (%zu bytes needed)", kName, need);
     return MF_ERR_WORKSPACE_TOO_SMALL;
@@ -465,7 +468,7 @@ extern "C" size_t mf_gated_mlp_fwd_workspace_bytes(const MfGatedMlpArgs* a) {
 extern "C" size_t mf_gated_mlp_bwd_workspace_bytes(const MfGatedMlpArgs* a) {
   if (!a || a->rows < 0 || a->hidden < 1 || a->dim < 1 || a->dim_out < 1) return 0;
   size_t at[4];
-  return pieces(a, true, at);
+  return pieces(a, at);
 }
 extern "C" int mf_gated_mlp_fwd(const MfGatedMlpArgs* a, void* stream) { return run_forward(a, BoundedWaits{}, static_cast<cudaStream_t>(stream)); }
 extern "C" int mf_gated_mlp_bwd(const MfGatedMlpArgs* a, void* stream) { return run_backward(a, BoundedWaits{}, static_cast<cudaStream_t>(stream)); }
