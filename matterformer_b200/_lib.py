@@ -516,7 +516,7 @@ def native():
 
 
 def foreign_leaves(*tensors) -> bool:
-    """Whether a pass that is being captured starts from a leaf whose gradients another stream takes (see torch_binding.cpp)."""
+    """Whether a pass that is being captured starts from a leaf whose gradients the default stream takes (see torch_binding.cpp)."""
     if not torch.cuda.is_current_stream_capturing():
         return False
     module = native()
@@ -525,7 +525,7 @@ def foreign_leaves(*tensors) -> bool:
 
 def refuse_foreign(foreign: bool, name: str) -> None:
     if foreign and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{name}: a backward pass cannot be captured while a graph of the same leaf from another stream is alive; "
+        raise RuntimeError(f"{name}: a backward pass cannot be captured while a graph of the same leaf from the default stream is alive; "
                            "release that graph (the outputs that hold it) before the capture")  # fmt: skip
 
 

@@ -338,14 +338,15 @@ std::optional<std::array<Tensor, 2>> knn_topk(const Tensor& pos, const Tensor& l
 // A backward pass under capture
 // ---------------------------------------------------------------------------------------------------------------------
 // A leaf has one node that takes its gradients, on the stream on which the first graph that is still alive made it.  The engine joins
-// that stream with the one of a backward pass; if the latter is being captured, that ends the capture with an error of the runtime
-// which names nothing.  The operators below say so instead: noted when their forward pass is captured, raised by its backward pass.
+// that stream with the one of a backward pass.  While the latter is being captured another stream joins the capture, but the default stream
+// cannot: that ends the capture with an error of the runtime which names nothing.  The operators below say so instead: noted when
+// their forward pass is captured, raised by its backward pass.
 bool foreign_leaf(const Tensor& t) {
   if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) return false;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
   if (!node) return false;
   const auto stream = node->stream();
-  return stream && *stream != c10::cuda::getCurrentCUDAStream(t.device().index()).unwrap();
+  return stream && *stream == c10::cuda::getDefaultCUDAStream(t.device().index()).unwrap();
 }
 // Whether something follows the operations of this thread and would not see a kernel launched past them: a trace, a dispatch mode, a
 // transform of torch.func.  (What matterformer_b200.fused.watched asks, without its microsecond.)
@@ -362,7 +363,7 @@ bool foreign_leaves(std::initializer_list<const Tensor*> inputs) {
 }
 void refuse_foreign(bool foreign, const char* name) {
   if (foreign && capturing())
-    throw std::runtime_error(std::string(name) + ": a backward pass cannot be captured while a graph of the same leaf from another stream is alive; "
+    throw std::runtime_error(std::string(name) + ": a backward pass cannot be captured while a graph of the same leaf from the default stream is alive; "
                              "release that graph (the outputs that hold it) before the capture");
 }
 
