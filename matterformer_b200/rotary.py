@@ -65,6 +65,12 @@ class RotaryPositions:
     factor: float = 1.0
     original_length: Optional[float] = None
 
+    def __post_init__(self) -> None:
+        if self.layout not in _lib.MF_ROTARY:
+            raise ValueError(f"layout must be one of {sorted(_lib.MF_ROTARY)}, got {self.layout!r}")
+        if not math.isfinite(self.amplitude):
+            raise ValueError(f"amplitude must be finite, got {self.amplitude}")
+
     @functools.cached_property
     def frequencies(self) -> torch.Tensor:
         with torch.inference_mode(False):  # (kept: an ordinary tensor, whoever asks first)
@@ -74,6 +80,8 @@ class RotaryPositions:
 
 def rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:
     """:func:`rotary_embedding` of one (B, H, N, D) tensor in plain torch operations, on any device; angles in 64 bits."""
+    if layout not in _lib.MF_ROTARY:
+        raise ValueError(f"layout must be one of {sorted(_lib.MF_ROTARY)}, got {layout!r}")
     table = frequencies.to(positions.device)
     angle = positions.double()[..., None] * table if table.ndim == 1 else (positions.double()[..., None] * table).flatten(-2)
     if angle.ndim == 2:

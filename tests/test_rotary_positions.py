@@ -130,3 +130,13 @@ def test_frequencies_first_asked_for_in_inference_mode():
     pos = torch.randn(1, 4, 3, requires_grad=True)
     y = rotate_torch(torch.randn(1, 2, 4, 16), pos, rotary.frequencies)
     assert torch.autograd.grad(y.sum(), pos)[0].isfinite().all()
+
+
+def test_unknown_layouts_are_refused_on_the_cpu_too():
+    x, pos, table = torch.ones(1, 1, 3, 8), torch.arange(3), mfb.rotary_frequencies(8)
+    with pytest.raises(ValueError, match="layout must be one of"):
+        rotate_torch(x, pos, table, "halves")
+    with pytest.raises(ValueError, match="layout must be one of"):
+        RotaryPositions(8, layout="Half")
+    with pytest.raises(ValueError, match="amplitude must be finite"):
+        RotaryPositions(8, amplitude=float("nan"))
