@@ -64,6 +64,8 @@ class RotaryPositions:
     scaling: str = "none"
     factor: float = 1.0
     original_length: Optional[float] = None
+    slow: float = 1.0
+    fast: float = 32.0
 
     def __post_init__(self) -> None:
         if self.layout not in _lib.MF_ROTARY:
@@ -75,7 +77,7 @@ class RotaryPositions:
     def frequencies(self) -> torch.Tensor:
         with torch.inference_mode(False):  # (kept: an ordinary tensor, whoever asks first)
             return rotary_frequencies(self.rotary_dim, axes=self.axes, base=self.base, scaling=self.scaling, factor=self.factor,
-                                      original_length=self.original_length)  # fmt: skip
+                                      original_length=self.original_length, slow=self.slow, fast=self.fast)  # fmt: skip
 
 
 def rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half", amplitude: float = 1.0) -> torch.Tensor:

@@ -140,3 +140,10 @@ def test_unknown_layouts_are_refused_on_the_cpu_too():
         RotaryPositions(8, layout="Half")
     with pytest.raises(ValueError, match="amplitude must be finite"):
         RotaryPositions(8, amplitude=float("nan"))
+
+
+def test_a_layer_takes_every_argument_of_the_frequencies():
+    more = dict(axes=1, base=500.0, scaling="parts", factor=4.0, original_length=64.0, slow=0.5, fast=3.0)
+    want = mfb.rotary_frequencies(32, **more)
+    assert torch.equal(RotaryPositions(32, **more).frequencies, want)
+    assert not torch.equal(mfb.rotary_frequencies(32, **{**more, "slow": 1.0, "fast": 32.0}), want)
