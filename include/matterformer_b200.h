@@ -687,7 +687,7 @@ int mf_rotary(const MfRotaryArgs* args, void* stream);
  * form that the backward call reads (16-bit values with an exponent for every 16 of them).
  * Backward: reads x, w_in, w_out, pre, act and grad_y; writes those of grad_x, grad_w_in, grad_w_out, grad_b_in, grad_b_out that are
  * not NULL.  Sums are in fp32 and in a fixed order; act and the gradients of the pre-activations are rounded to dtype, the
- * pre-activations to more bits, counted from the largest of 16 neighbouring channels: 11 (bf16) or 12 (fp16).
+ * pre-activations to more bits, counted from the largest of 16 neighbouring channels: 11 (bf16) or 13 to 12 (fp16).
  * Workspace: forward mf_gated_mlp_fwd_workspace_bytes (without it some sizes take longer), backward mf_gated_mlp_bwd_workspace_bytes
  * for the same gradients.  The outputs of a call with an expired
  * device-side wait are undefined; mf_gated_mlp_status (which synchronises `stream`) returns its code for the calls on the device since it was

@@ -200,16 +200,14 @@ __global__ void __launch_bounds__(kWarps * 32) small_kernel(const SmallParams p)
       if (biased && n < p.n) u += to_f32(bias[p.n + n]);
       if (p.pre) {
         const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
-        float most_g = fabsf(a), most_u = fabsf(u);
+        PreGroup<T> of_gate, of_up;
+        of_gate.add(a, a), of_up.add(u, u);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
-          most_g = group_max<T>(most_g, __shfl_xor_sync(lanes, most_g, o));
-          most_u = group_max<T>(most_u, __shfl_xor_sync(lanes, most_u, o));
-        }
-        const uint32_t eg = group_exponent<T>(most_g), eu = group_exponent<T>(most_u);
+        for (int o = 8; o > 0; o >>= 1) of_gate.exchange(lanes, o), of_up.exchange(lanes, o);
+        const uint32_t eg = of_gate.code(), eu = of_up.code();
         if (n < p.n) {
           uint16_t* pre = static_cast<uint16_t*>(p.pre) + (size_t)c * 2 * p.n + n;
-          pre[0] = (uint16_t)pack_pre<T>(make_float2(a, 0.f), group_scale<T>(eg)), pre[p.n] = (uint16_t)pack_pre<T>(make_float2(u, 0.f), group_scale<T>(eu));
+          pre[0] = (uint16_t)PreForm<T>(eg, false).pack(make_float2(a, 0.f)), pre[p.n] = (uint16_t)PreForm<T>(eu, false).pack(make_float2(u, 0.f));
         }
         if (r == 0) {
           uint8_t* to = p.exponents + ((size_t)(n0 >> 6) * p.rows + c) * 8 + ((n0 >> 4) & 3);

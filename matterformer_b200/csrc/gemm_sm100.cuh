@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               drained();
             }
             uint32_t(&gv)[16] = g[c & 1], (&uv)[16] = u[c & 1], hw[8];
-            float most_g = 0.f, most_u = 0.f;
+            PreGroup<T> of_gate, of_up;
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
               const uint32_t bgw[4] = {bg[v].x, bg[v].y, bg[v].z, bg[v].w}, buw[4] = {bu[v].x, bu[v].y, bu[v].z, bu[v].w};
@@ -605,8 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
                 hw[4 * v + e] = pack2<T>(h.x, h.y);
                 if constexpr (kEpi == kGateKeep) {
                   gv[i] = __float_as_uint(gate.x), gv[i + 1] = __float_as_uint(gate.y), uv[i] = __float_as_uint(up.x), uv[i + 1] = __float_as_uint(up.y);
-                  most_g = group_max<T>(most_g, group_max<T>(fabsf(gate.x), fabsf(gate.y)));
-                  most_u = group_max<T>(most_u, group_max<T>(fabsf(up.x), fabsf(up.y)));
+                  of_gate.add(gate.x, gate.y), of_up.add(up.x, up.y);
                 }
               }
             }
@@ -614,8 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
             for (int v = 0; v < 2; ++v) sts128(buffers + box_chunk(lane, 2 * c + v), make_uint4(hw[4 * v], hw[4 * v + 1], hw[4 * v + 2], hw[4 * v + 3]));
             if constexpr (kEpi == kGateKeep) {
-              const uint32_t eg = group_exponent<T>(most_g), eu = group_exponent<T>(most_u);
-              const float2 sg = group_scale<T>(eg), su = group_scale<T>(eu);
+              const uint32_t eg = of_gate.code(), eu = of_up.code();
+              const PreForm<T> form_g(eg, false), form_u(eu, false);
               exponents.x |= eg << (8 * c), exponents.y |= eu << (8 * c);
 #pragma unroll
               for (int v = 0; v < 2; ++v) {
@@ -623,8 +622,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int i = 8 * v + 2 * e;
-                  gw[e] = pack_pre<T>(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])), sg);
-                  uw[e] = pack_pre<T>(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])), su);
+                  gw[e] = form_g.pack(make_float2(__uint_as_float(gv[i]), __uint_as_float(gv[i + 1])));
+                  uw[e] = form_u.pack(make_float2(__uint_as_float(uv[i]), __uint_as_float(uv[i + 1])));
                 }
                 const uint32_t at = keep + half_box_chunk(lane, 2 * (c & 1) + v);
                 sts128(at, make_uint4(gw[0], gw[1], gw[2], gw[3]));
@@ -675,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             tmem_ld_wait();
             if (q < 3) tmem_ld16(acc + first + 64 * c + 16 * (q + 1), d[(q + 1) & 1]);
             else if (last) drained();
-            const float2 fg = group_unscale<T>(exponents.x >> (8 * q) & 255u), fu = group_unscale<T>(exponents.y >> (8 * q) & 255u);
+            const PreForm<T> form_g(exponents.x >> (8 * q) & 255u, true), form_u(exponents.y >> (8 * q) & 255u, true);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
               const uint32_t gs[4] = {gw[v].x, gw[v].y, gw[v].z, gw[v].w}, us[4] = {uw[v].x, uw[v].y, uw[v].z, uw[v].w};
@@ -684,8 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
               for (int e = 0; e < 4; ++e) {
                 const float2 grad = make_float2(__uint_as_float(d[q & 1][8 * v + 2 * e]), __uint_as_float(d[q & 1][8 * v + 2 * e + 1]));
                 float2 value, slope;
-                activation2<kAct>(unpack_pre<T>(gs[e], fg), value, slope);
-                const float2 a = mul2(mul2(grad, unpack_pre<T>(us[e], fu)), slope), b = mul2(grad, value);
+                activation2<kAct>(form_g.unpack(gs[e]), value, slope);
+                const float2 a = mul2(mul2(grad, form_u.unpack(us[e])), slope), b = mul2(grad, value);
                 dg[e] = pack2<T>(a.x, a.y), du[e] = pack2<T>(b.x, b.y);
               }
               sts128(gate + box_chunk(lane, 2 * q + v), make_uint4(dg[0], dg[1], dg[2], dg[3]));

@@ -155,8 +155,8 @@ def gated_mlp(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, b_in: Op
 
     Sums are in fp32 in a fixed order.  The hidden values and the gradients of the pre-activations are rounded to ``x``'s type; hidden values
     that fp16 cannot hold (above 65504) are infinities there.  What the backward pass gets of the pre-activations has more bits than
-    ``x``'s type, counted from the power of two in the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-28 of that (bf16),
-    12 down to 2^-13 of it and one less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable.  What is traced
+    ``x``'s type, counted from the power of two in the largest of 16 neighbouring hidden channels of a token: 11 down to 2^-28 of that (bf16);
+    13 where all are above 2^-7 of it, else 12 down to 2^-13 and one less for each halving beyond (fp16).  C, F and O are multiples of 8, at most 2^28.  The gradient is once differentiable.  What is traced
     or under a transform of ``torch.func`` is the same in plain operations, rounded after each."""
     native = None if simplicial._CHECK_STATUS else _lib.native()
     if native is not None and activation in ACTIVATIONS:  # operands that are ready as they are: one call into C++

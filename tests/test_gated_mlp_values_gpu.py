@@ -65,8 +65,8 @@ def test_a_nan_bias_reaches_its_gradient(rows, side, dtype):
 @pytest.mark.parametrize("rows", [16, 300])
 @pytest.mark.parametrize("outlier", [10, 13, 16])
 def test_fp16_channels_beside_an_outlier(rows, outlier):
-    """One channel's up projection is 2^outlier times its neighbours'.  The fp16 form keeps 12 bits, one more than fp16 has, down to 2^-13 of the power
-    of two in the largest of a group, and steps of 2^-24 of that below: a value of the others is off by 2^-12 of itself or half such a step.
+    """One channel's up projection is 2^outlier times its neighbours'.  In such a group the fp16 form keeps 12 bits, one more than fp16 has, down to 2^-13 of
+    the power of two in the largest, and steps of 2^-24 of that below: a value of the others is off by 2^-12 of itself or half such a step.
 
     The gradient of the gate's rows is a sum over the tokens of dh act'(g) u x: of the error of u by steps, each token's at most, added in squares
     (twice for the room of a sum of few); of the roundings of its own, 6 of 2^-11 as for every gradient of the block; of the steps of 2^-24
@@ -95,15 +95,16 @@ def test_fp16_channels_beside_an_outlier(rows, outlier):
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
 def test_distance_to_the_rounding_of_the_result_alone(rows, C, H, O, act, dtype):
     """Root mean square errors in units of what rounding the exact result gives.  Forward the hidden value and the result are rounded, independently:
-    sqrt(2).  Backward the gradient of the pre-activations and the result are, and the kept pre-activations by 2^-k of a rounding, k = 3 in bf16
-    and 1 in fp16.  For gates of unit variance f(z) takes that up 1.21 times (root mean square of z f'(z) over that of f), f'(z) 0.35 times, a product
-    with the up side once more: at most sqrt(2 + 1.21^2 / 4^k) = 1.42 and 1.54.  5 and 7 % are for sums of a few hundred values.  Pre-activations in the
-    block's own type, k = 0, would be at 1.86."""
+    sqrt(2).  Backward the gradient of the pre-activations and the result are, and the kept pre-activations by 2^-k of a rounding, k = 3 in bf16,
+    in fp16 2 and, in the 15 % of groups that have a value below 2^-7 of the power of two in their largest, 1.  For gates of unit variance f(z)
+    takes that up 1.21 times (root mean square of z f'(z) over that of f), f'(z) 0.35 times, a product with the up side once more: at most
+    sqrt(2 + 1.21^2 / 4^k) = 1.42 and 1.46.  6 % are for sums of a few hundred values.  Pre-activations in the block's own type, k = 0,
+    would be at 1.86."""
     ops, dy = _operands(rows, C, H, O, dtype, 4)
     got, want = _run(ops, dy, act), _exact(ops, dy, act)
     for i, (a, b) in enumerate(zip(got, want)):
         alone = (b.to(dtype).double() - b).norm()
-        assert (a.double() - b).norm() < (1.5 if dtype == BF16 else 1.65) * alone, f"output {i}: {((a.double() - b).norm() / alone).item():.2f}"
+        assert (a.double() - b).norm() < (1.5 if dtype == BF16 else 1.55) * alone, f"output {i}: {((a.double() - b).norm() / alone).item():.2f}"
 
 
 @pytest.mark.parametrize("rows", [2, 8, 16, 17, 32, 33, 257, 600])
