@@ -637,9 +637,10 @@ int mf_simplicial_packed_bwd(const MfSimplicialPackedArgs* args, void* stream);
 #define MF_POSITION_F64 3
 
 /*
- * Rotates the channel pairs of the heads of up to three tensors by angles that depend on their tokens' positions, the operator that
- * `RotaryMultiheadAttention.forward` applies to its queries and keys (regular_attention.py:208-271) in the forms that language models
- * have it: both pair layouts, a part of the head, positions of one or several axes, any table of frequencies.
+ * Rotates the channel pairs of the heads of up to three tensors by angles that depend on their tokens' positions: both pair layouts, a
+ * part of the head, positions of one or several axes, any table of frequencies.  (The reference's `RotaryMultiheadAttention` turns its queries
+ * and keys by 3-D positions, regular_attention.py:208-271.  Here the pairs of all axes follow each other, axis by axis, and half a rotation
+ * is P pairs over all axes; that its checkpoints order them so is not established.)
  * Pair p of P = axes * pairs turns by positions[b, n, p / pairs] * frequencies[p] radians and is scaled by `amplitude`; channels from
  * 2 P on are copied, and so are all channels of a tensor with rotates = 0 (the values of a packed projection).  inverse = 1: by the
  * opposite angles, which is the backward pass.

@@ -5,9 +5,10 @@
 // where they stand (dh is never stored); dx = [dg du] [Wg; Wu]; and the weights' gradients [dg du]^T x and dy^T h.
 // h, dg and du are rounded to the block's type on their way through memory: the tensor cores take no wider operands.  g and u are kept
 // in 16 bits of a form of their own (gated_mlp.cuh), since 32 would double what the first product stores.  Every sum is in 32 bits.
-// 29 696 tokens x 512 x 2048, forward and all gradients: 520-590 us, 0.95-1.08 PFLOP/s (cuBLAS sustains 1.39 in one long product, bursts at 1.64):
-// projections 115, output 58, gate gradient 112 (486 MB: memory bounds it, the others the tensor cores at the clock that the power limit
-// leaves), gradients 213.  8192 x 2048 x 5464: 1420 us, 1.16 PFLOP/s.
+// 29 696 tokens x 512 x 2048, forward and all gradients, a pass among others on several cards: 571-611 us, 0.92-0.98 PFLOP/s (cuBLAS sustains
+// 1.39 in one long product, bursts at 1.64; linear layers and element-wise operations in bf16 take 1360-1410).  Launch by launch, at 1.46-1.68
+// GHz: projections 116, output 52, gate gradient 104 (495 MB, 4.8 TB/s; the tensor pipe at 37 %), gradients 203 (94 %).  8192 x 2048 x
+// 5464: 1404-1474 us, 1.12-1.18 PFLOP/s.
 #include <mutex>
 
 #include "common.cuh"

@@ -123,7 +123,8 @@ inline size_t gated_mlp_pre_values(int64_t rows, int64_t hidden) { return align_
 
 // The kernels for few tokens (gated_mlp_small.cu) take up to 16, up to 32 where there are few weights: they read the tokens again for
 // every 16 channels.  us, 16 | 17 | 32 tokens there, 33 on tcgen05 tiles: 512 x 2048 7.7 | 9.9 | 11.1, 12.8; 1024 x 4096 14 | 23 | 27, 20;
-// 2048 x 8192 28 | 40 | 43, 32; 4096 x 10 928 73 | 93 | 103, 68.
+// 2048 x 8192 28 | 40 | 43, 32; 4096 x 10 928 73 | 93 | 103, 68.  (The line goes by the number of tokens: between 9 and 16 of them the widest
+// weights lose some 5 us to it.)
 inline bool gated_mlp_small(const MfGatedMlpArgs* a) { return a->rows <= 16 || (a->rows <= 32 && (int64_t)a->dim * a->hidden <= 1 << 21); }
 int gated_mlp_small_forward(const MfGatedMlpArgs* a, cudaStream_t stream);
 

@@ -1,8 +1,9 @@
 """Rotary positions on queries and keys, in the layouts that attention layers have them.
 
 The reference turns the heads of ``RotaryMultiheadAttention`` by 3-D positions before its attention core
-(src/matterformer/models/regular_attention.py:208-271).  Here that is one operator for any table of frequencies, pairs of channels
-half a rotation apart or next to each other, a part of the head, positions in a sequence or coordinates: :func:`rotary_embedding` on head-major
+(src/matterformer/models/regular_attention.py:208-271).  Here rotary positions are one operator for any table of frequencies, pairs of channels
+half a rotation apart or next to each other, a part of the head, positions in a sequence or coordinates (pairs axis by axis, halves over all
+axes; not compared with the order of the reference's pairs): :func:`rotary_embedding` on head-major
 ``q, k`` and :func:`rotary_packed` on the packed projection that :func:`matterformer_b200.sparse.local_window_attention_packed` takes.
 Angles are formed in 64 bits, so that positions of millions keep theirs.
 """

@@ -14,7 +14,7 @@ so a reference ``state_dict`` of the same configuration loads with ``strict=True
 * :class:`EDMPreconditioner`, :class:`EDMLoss` <- src/matterformer/tasks/edm.py:34-150
 
 Only what that configuration touches is mirrored: no geometry-bias builders, no coordinate embedding.  Two options go beyond it:
-``rotary`` (rotary positions in the MHA layers, as ``RotaryMultiheadAttention`` has them, regular_attention.py:208-271) and
+``rotary`` (rotary positions in the MHA layers; ``RotaryMultiheadAttention`` has three-dimensional ones, regular_attention.py:208-271) and
 ``mlp_type="gated"`` (:class:`GatedMlp` in the place of :class:`Mlp`).  ``impl="cuda"`` (and ``"auto"`` on CUDA tensors) runs the sm_100a kernels through the C ABI;
 ``impl="torch"`` is the dense formulation in plain torch ops, as in the reference.
 """
