@@ -111,10 +111,11 @@ class _GatedMlp(torch.autograd.Function):
 
 
 def _plain(x, w_in, w_out, b_in, b_out, activation):
-    """The block in torch operations, in ``x``'s type."""
-    w_in, w_out, b_in, b_out = (None if p is None else p.to(x.dtype) for p in (w_in, w_out, b_in, b_out))
-    gate, up = F.linear(x, w_in, b_in).chunk(2, dim=-1)
-    return F.linear((F.silu(gate) if activation == "silu" else F.gelu(gate, approximate="tanh")) * up, w_out, b_out)
+    """The block in torch operations, in ``x``'s type whatever autocast is for."""
+    with torch.autocast(x.device.type, enabled=False):
+        w_in, w_out, b_in, b_out = (None if p is None else p.to(x.dtype) for p in (w_in, w_out, b_in, b_out))
+        gate, up = F.linear(x, w_in, b_in).chunk(2, dim=-1)
+        return F.linear((F.silu(gate) if activation == "silu" else F.gelu(gate, approximate="tanh")) * up, w_out, b_out)
 
 
 def gated_mlp_applies(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor) -> bool:

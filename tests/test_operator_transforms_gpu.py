@@ -50,6 +50,18 @@ def test_a_trace_of_the_block_follows_its_input(how, wide):
             assert _off(f(x), want) < BOUND
 
 
+@pytest.mark.parametrize("how", ["jit", "fx"])
+def test_a_trace_keeps_the_type_under_autocast(how):
+    """An fp16 block under bf16 autocast is one of fp16, traced or not."""
+    w_in, w_out, x = W_IN().half(), W_OUT().half(), _r(40, 64, seed=12, dtype=torch.float16)
+    with torch.no_grad(), torch.autocast("cuda", dtype=BF16):
+        f = _traced(how, lambda t: mfb.gated_mlp(t, w_in, w_out), x)
+        assert mfb.gated_mlp(x, w_in, w_out).dtype == torch.float16
+    got = f(x)  # (a trace that runs under autocast is subject to it like any other operations)
+    assert got.dtype == torch.float16
+    assert _off(got, _block(x.double(), w_in.double(), w_out.double())) < BOUND / 8
+
+
 def test_the_block_under_transforms():
     w_in, w_out = W_IN(), W_OUT()
     x, v = _r(3, 20, 64, seed=6), _r(3, 20, 64, seed=7)
