@@ -731,6 +731,82 @@ int mf_selftest_gated_mlp_give_up(const MfGatedMlpArgs* args, int32_t backward, 
                                   void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* Dense attention with a learned bias by buckets                             */
+/* ------------------------------------------------------------------------- */
+
+#define MF_BUCKETS_NONE 0
+#define MF_BUCKETS_OFFSET 1 /* 2 * reach + 1 entries for the offsets -reach .. reach; the ends stand for all beyond */
+#define MF_BUCKETS_PAIR 2   /* (batch or one, queries, keys) */
+#define MF_DENSE_BACKEND_AUTO 0
+#define MF_DENSE_BACKEND_MMA 1     /* warp-level tiles, whatever the sizes */
+#define MF_DENSE_BACKEND_TCGEN05 2 /* 128-row tiles wherever they take the call */
+
+typedef struct MfRows { /* elements between neighbouring entries; the channels of a row are adjacent */
+  int64_t batch, head, token;
+} MfRows;
+
+/*
+ * out_i = sum_j p_ij v_j, p_i = softmax over the keys j that query i sees of scale * q_i . k_j + bias[bucket(i, j)][head].  The masked core of
+ * RotaryMultiheadAttention.forward (models/regular_attention.py:208-271) with the additive mask replaced by a table.  q and out
+ * (batch, heads, queries, head_dim), k and v (batch, kv_heads, keys, head_dim), bf16 or fp16, heads a multiple of kv_heads, head_dim 32, 64 or 128, rows
+ * at any strides that are multiples of 8 elements.  num_queries and num_keys (batch) int32 or NULL for the padded lengths; what lies
+ * behind them may hold anything, is not read as a number and gets zeros.  key_mask (batch, keys) bytes or NULL: zero hides a key.
+ * causal: key j is seen by the queries i with j - i <= num_keys - num_queries (the last query stands at the last key).  A query that sees no
+ * key returns zeros.
+ *
+ * bias (num_buckets, heads) in bias_dtype or NULL; buckets as bucket_kind says, the offset being j - i - (num_keys - num_queries);
+ * bucket_row and bucket_batch are the strides of the pairs' (bytes).  Up to 128 buckets; a bucket beyond the table has no bias and no
+ * gradient.  An entry of minus infinity or below -1e30 hides its pairs.
+ *
+ * lse (batch, heads, queries) fp32 is written by the forward call where it is not NULL; the backward call takes it and out.  It forms the
+ * probabilities again, and the gradients dq, dk, dv (dtype) and dbias (bias_dtype) where they are not NULL.  Sums are in fp32 and in a
+ * fixed order; p and the gradients of the logits are rounded to dtype before the products that contract them.
+ * Both calls need the workspace of the size that they ask for (its contents mean nothing between calls).
+ */
+typedef struct MfDenseAttnArgs {
+  int32_t batch, heads, kv_heads, queries, keys, head_dim;
+  int32_t dtype;
+  int32_t causal;
+  int32_t backend;
+  float scale;
+  const void* q;
+  const void* k;
+  const void* v;
+  MfRows q_rows, k_rows, v_rows;
+  const int32_t* num_queries;
+  const int32_t* num_keys;
+  const uint8_t* key_mask;
+  int64_t key_mask_batch;
+  const void* bias;
+  int32_t bias_dtype, num_buckets, bucket_kind, reach;
+  const uint8_t* buckets;
+  int64_t bucket_batch, bucket_row;
+  void* out;
+  MfRows out_rows;
+  float* lse;
+  const void* grad_out; /* backward from here on */
+  MfRows grad_out_rows;
+  void* dq;
+  void* dk;
+  void* dv;
+  MfRows dq_rows, dk_rows, dv_rows;
+  void* dbias;
+  void* workspace;
+  size_t workspace_bytes;
+} MfDenseAttnArgs;
+
+size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs* args);
+size_t mf_dense_attn_bwd_workspace_bytes(const MfDenseAttnArgs* args);
+int mf_dense_attn_fwd(const MfDenseAttnArgs* args, void* stream);
+int mf_dense_attn_bwd(const MfDenseAttnArgs* args, void* stream);
+
+/* Buckets of a batch of molecules for the above: buckets[b][i][j] (rows `row` and entries `batch_stride` bytes apart) = how many of the `edges` ascending
+ * host values lie at or below the distance of atoms i and j of coords (batch, tokens, 3) fp32, compared as squares in fp64; 0 where i or j is
+ * at or behind num_atoms (batch) int32.  At most 127 edges, none negative. */
+int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t batch, int32_t tokens, const double* edges, int32_t num_edges,
+                        uint8_t* buckets, int64_t batch_stride, int64_t row, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Equivariant coordinate head                                               */
 /* ------------------------------------------------------------------------- */
 

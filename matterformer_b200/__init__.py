@@ -10,6 +10,7 @@ from .simplicial import (
     simplicial_attention_cuda,
 )
 from .batching import AttentionCostBatchSampler, simplicial_tile_steps
+from .dense import RelativeBias, dense_attention, dense_attention_packed, distance_buckets, offset_buckets, set_dense_backend
 from .gated import gated_mlp, gated_mlp_status
 from .hostio import HostPipelinedSimplicial
 from .rotary import RotaryPositions, rotary_embedding, rotary_frequencies, rotary_packed
@@ -27,6 +28,12 @@ from .sparse import (
 )
 
 __all__ = [
+    "RelativeBias",
+    "dense_attention",
+    "dense_attention_packed",
+    "distance_buckets",
+    "offset_buckets",
+    "set_dense_backend",
     "gated_mlp",
     "gated_mlp_status",
     "RotaryPositions",

@@ -28,6 +28,8 @@ MF_BACKEND = {"auto": 0, "generic": 1, "tcgen05": 2, "tcgen05_tiles": 3}
 MF_SPARSE_BACKEND = {"auto": 0, "mma": 1, "tcgen05": 2}
 MF_ACT_SILU, MF_ACT_GELU_TANH = 0, 1
 MF_ROTARY = {"half": 0, "interleaved": 1}
+MF_BUCKETS_NONE, MF_BUCKETS_OFFSET, MF_BUCKETS_PAIR = 0, 1, 2
+MF_DENSE_BACKEND = {"auto": 0, "mma": 1, "tcgen05": 2}
 MF_POSITION = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
 # Every symbol include/matterformer_b200.h declares.
@@ -106,6 +108,11 @@ EXPORTED_SYMBOLS = (
     "mf_gated_mlp_bwd",
     "mf_gated_mlp_status",
     "mf_selftest_gated_mlp_give_up",
+    "mf_dense_attn_fwd_workspace_bytes",
+    "mf_dense_attn_bwd_workspace_bytes",
+    "mf_dense_attn_fwd",
+    "mf_dense_attn_bwd",
+    "mf_distance_buckets",
     "mf_profile_enable",
     "mf_profile_read",
 )
@@ -325,6 +332,20 @@ class MfGatedMlpArgs(Structure):
                [("workspace_bytes", c_size_t)]  # fmt: skip
 
 
+class MfRows(Structure):
+    _fields_ = [(n, c_int64) for n in ("batch", "head", "token")]
+
+
+class MfDenseAttnArgs(Structure):
+    _fields_ = [(n, c_int32) for n in ("batch", "heads", "kv_heads", "queries", "keys", "head_dim", "dtype", "causal", "backend")] + \
+               [("scale", c_float), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_rows", MfRows), ("k_rows", MfRows), ("v_rows", MfRows),
+                ("num_queries", c_void_p), ("num_keys", c_void_p), ("key_mask", c_void_p), ("key_mask_batch", c_int64), ("bias", c_void_p)] + \
+               [(n, c_int32) for n in ("bias_dtype", "num_buckets", "bucket_kind", "reach")] + \
+               [("buckets", c_void_p), ("bucket_batch", c_int64), ("bucket_row", c_int64), ("out", c_void_p), ("out_rows", MfRows), ("lse", c_void_p),
+                ("grad_out", c_void_p), ("grad_out_rows", MfRows), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dq_rows", MfRows),
+                ("dk_rows", MfRows), ("dv_rows", MfRows), ("dbias", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]  # fmt: skip
+
+
 _LIB = None
 
 
@@ -472,6 +493,12 @@ def lib() -> ctypes.CDLL:
     for fn in (L.mf_gated_mlp_fwd, L.mf_gated_mlp_bwd):
         fn.argtypes = [POINTER(MfGatedMlpArgs), c_void_p]
         fn.restype = c_int32
+    for fn in (L.mf_dense_attn_fwd_workspace_bytes, L.mf_dense_attn_bwd_workspace_bytes):
+        fn.argtypes, fn.restype = [POINTER(MfDenseAttnArgs)], c_size_t
+    for fn in (L.mf_dense_attn_fwd, L.mf_dense_attn_bwd):
+        fn.argtypes, fn.restype = [POINTER(MfDenseAttnArgs), c_void_p], c_int32
+    L.mf_distance_buckets.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int64, c_int64, c_void_p]
+    L.mf_distance_buckets.restype = c_int32
     L.mf_gated_mlp_status.argtypes = [POINTER(c_int32), c_void_p]
     L.mf_gated_mlp_status.restype = c_int32
     L.mf_selftest_gated_mlp_give_up.argtypes = [POINTER(MfGatedMlpArgs), c_int32, c_int32, c_int64, POINTER(c_int32), c_void_p]

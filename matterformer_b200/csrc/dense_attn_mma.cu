@@ -1,0 +1,419 @@
+// Dense attention with a learned bias by buckets on the warp-level tensor cores (mma.sync m16n8k16): any length, head size 32, 64 or 128,
+// any mask.
+//
+// One CTA of four warps owns 64 rows of one (batch, head), a warp 16 of them, and walks over tiles of 64 partner rows that arrive by cp.async
+// while the previous tile is worked on.
+//   FWD : owners = queries, partners = keys     out, lse      (running maximum and sum per row)
+//   DQ  : owners = queries, partners = keys     dq, delta and the table's gradient per bucket
+//   DKV : owners = keys,    partners = queries of all heads that share them     dk, dv  (logits formed transposed)
+// Logits, probabilities and their gradients stay in registers: the C fragment of a product is the A operand of the next.  P and dS are
+// rounded to the operands' type there (half a unit of 2^-8 or 2^-11 each, on terms of a sum), the only type the tensor cores take.
+// Every output has one owner and a fixed order of its sums.
+#include "dense_attn.cuh"
+
+namespace mf {
+namespace {
+
+enum { D_FWD = 0, D_DQ = 1, D_DKV = 2 };
+constexpr int kOwn = 64, kPart = 64, kThreads = 128;
+constexpr int kSpan = kOwn + kPart - 1;  // offsets between the rows of two tiles
+
+template <int D>
+constexpr int kTileBytes = 64 * (D + 8) * 2;
+
+// shared memory: own_a | own_b | part_a[2] | part_b[2] | lse, delta [2][64] each | table[kTableEntries] | bias of offsets [2][128], their buckets [2][128] |
+// DQ with a table: [4 warps][num_buckets + 1][32]
+template <int D>
+constexpr int kFixedBytes = 6 * kTileBytes<D> + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 4 + 2 * 128;
+
+// rows [row0, row0 + 64) of a head, zeros from row_limit on and where `mask` (per row) is zero
+template <typename T, int D>
+__device__ __forceinline__ void load_rows(uint32_t tile, const T* src, long long stride, int row0, int row_limit, const uint8_t* mask) {
+  constexpr int LD = D + 8, PER_ROW = D / 8;
+#pragma unroll
+  for (int it = 0; it < 64 * PER_ROW / kThreads; ++it) {
+    const int idx = it * kThreads + threadIdx.x;
+    const int r = idx / PER_ROW, c = idx % PER_ROW, row = row0 + r;
+    const bool ok = row < row_limit && (!mask || mask[row]);
+    cp_async16(tile + (r * LD + c * 8) * 2, src + (ok ? row * stride : 0) + c * 8, ok);
+  }
+}
+
+template <typename T, int D, int MODE, int KIND>
+__global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_constant__ DenseParams p) {
+  constexpr int LD = D + 8, TILE = kTileBytes<D>, KS = D / 16;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint32_t s_own_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), s_own_b = s_own_a + TILE;
+  const uint32_t s_part_a = s_own_b + TILE, s_part_b = s_part_a + 2 * TILE;
+  float* part_lse = reinterpret_cast<float*>(smem + 6 * TILE);
+  float* part_delta = part_lse + 2 * 64;
+  float* table = part_delta + 2 * 64;
+  float* offset_bias = table + kTableEntries;
+  uint8_t* offset_bucket = reinterpret_cast<uint8_t*>(offset_bias + 2 * 128);
+  float* sums = reinterpret_cast<float*>(offset_bucket + 2 * 128);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const int heads = MODE == D_DKV ? p.K : p.H, group = p.H / p.K;
+  // the longest walks of a causal call first
+  const int entries = p.B * heads, tiles = gridDim.x / entries;
+  const int entry = p.causal ? blockIdx.x % entries : blockIdx.x / tiles;
+  const int tile = !p.causal ? blockIdx.x % tiles : MODE == D_DKV ? blockIdx.x / entries : tiles - 1 - (int)(blockIdx.x / entries);
+  const int b = entry / heads, oh = entry % heads;  // oh: of the owners
+  const int kh = MODE == D_DKV ? oh : oh / group;
+  const DenseLengths len = dense_lengths(p, b);
+  const int row0 = tile * kOwn;
+  const int my = row0 + warp * 16 + g;  // this thread's rows: my, my + 8
+  const uint8_t* mask = p.key_mask ? p.key_mask + b * p.key_mask_batch : nullptr;
+
+  // ---- what the tile walks over: partners [first, last) in tiles, for DKV once for each head of the group
+  const int own_limit = MODE == D_DKV ? len.nk : len.nq;
+  int first = 0, last = 0;
+  if (row0 < own_limit) {
+    if (MODE == D_DKV) first = dense_first(p, len, row0) / kPart * kPart, last = len.nq;
+    else last = dense_limit(p, len, min(row0 + kOwn, len.nq) - 1);
+  }
+  const int per_head = last > first ? (last - first + kPart - 1) / kPart : 0;
+  const int steps = MODE == D_DKV ? per_head * group : per_head;
+
+  const T* K = static_cast<const T*>(p.k) + p.k_rows.at(b, kh, 0);
+  const T* V = static_cast<const T*>(p.v) + p.v_rows.at(b, kh, 0);
+  auto q_of = [&](int h) { return static_cast<const T*>(p.q) + p.q_rows.at(b, h, 0); };
+  auto go_of = [&](int h) { return static_cast<const T*>(p.grad_out) + p.go_rows.at(b, h, 0); };
+  auto stat = [&](int h) { return ((long long)b * p.H + h) * p.M; };
+
+  auto load_step = [&](int t, int stage) {
+    const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
+    const int at = first + (MODE == D_DKV ? t % per_head : t) * kPart;
+    if (MODE == D_DKV) {
+      load_rows<T, D>(s_part_a + stage * TILE, q_of(h), p.q_rows.token, at, len.nq, nullptr);
+      load_rows<T, D>(s_part_b + stage * TILE, go_of(h), p.go_rows.token, at, len.nq, nullptr);
+      if (tid < 64) {
+        const int i = at + tid;
+        part_lse[stage * 64 + tid] = i < len.nq ? p.lse[stat(h) + i] : INFINITY;
+        part_delta[stage * 64 + tid] = i < len.nq ? p.delta[stat(h) + i] : 0.f;
+      }
+    } else {
+      load_rows<T, D>(s_part_a + stage * TILE, K, p.k_rows.token, at, len.nk, mask);
+      load_rows<T, D>(s_part_b + stage * TILE, V, p.v_rows.token, at, len.nk, mask);
+    }
+    if (KIND == MF_BUCKETS_OFFSET && tid < kSpan) {  // offsets of the two tiles: owner - partner or partner - owner runs over 127 values
+      const int offset = (MODE == D_DKV ? row0 - at + tid - (kPart - 1) : at - row0 + tid - (kOwn - 1)) - len.shift;
+      const int bucket = dense_offset_bucket(p, offset);
+      offset_bias[stage * 128 + tid] = dense_bias_entry(p, bucket, h);
+      if (MODE == D_DQ) offset_bucket[stage * 128 + tid] = (uint8_t)bucket;
+    }
+  };
+
+  if (steps > 0) {
+    if (MODE == D_DKV) {
+      load_rows<T, D>(s_own_a, K, p.k_rows.token, row0, len.nk, mask);
+      load_rows<T, D>(s_own_b, V, p.v_rows.token, row0, len.nk, mask);
+    } else {
+      load_rows<T, D>(s_own_a, q_of(oh), p.q_rows.token, row0, len.nq, nullptr);
+      if (MODE == D_DQ) load_rows<T, D>(s_own_b, go_of(oh), p.go_rows.token, row0, len.nq, nullptr);
+    }
+    load_step(0, 0);
+  }
+  cp_async_commit();
+  const int nb = p.num_buckets;
+  if (KIND == MF_BUCKETS_PAIR && MODE != D_DKV)
+    for (int i = tid; i < kTableEntries; i += kThreads) table[i] = dense_bias_entry(p, i, oh);
+  if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part)
+    for (int i = tid; i < 4 * (nb + 1) * 32; i += kThreads) sums[i] = 0.f;
+  float* my_sums = sums + (warp * (nb + 1)) * 32 + lane;
+
+  // ---- visible partners of this thread's two rows: [lo, hi)
+  int lo[2], hi[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int row = my + 8 * e;
+    if (MODE == D_DKV) {
+      lo[e] = dense_first(p, len, row);
+      hi[e] = row < len.nk && (!mask || mask[row]) ? len.nq : 0;
+    } else {
+      lo[e] = 0;
+      hi[e] = dense_limit(p, len, row);
+    }
+  }
+
+  float acc0[D / 8][4], acc1[MODE == D_DKV ? D / 8 : 1][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc0[i][e] = 0.f;
+  if constexpr (MODE == D_DKV) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc1[i][e] = 0.f;
+  }
+  const float sc2 = p.scale * kDenseLog2e;
+  float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f}, lse[2] = {INFINITY, INFINITY}, delta[2] = {0.f, 0.f};
+  if (MODE == D_DQ) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // the four lanes of a row take a quarter of its channels each
+      const int row = my + 8 * e;
+      float d = 0.f;
+      if (row < len.nq) {
+        const T* go = go_of(oh) + row * p.go_rows.token + t4 * (D / 4);
+        const T* o = static_cast<const T*>(p.out) + p.out_rows.at(b, oh, row) + t4 * (D / 4);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(go + 8 * c), y = *reinterpret_cast<const uint4*>(o + 8 * c);
+          const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 u = unpack2<T>(xw[i]), w = unpack2<T>(yw[i]);
+            d = fmaf(u.x, w.x, fmaf(u.y, w.y, d));
+          }
+        }
+        lse[e] = p.lse[stat(oh) + row];
+      }
+      d += __shfl_xor_sync(0xffffffffu, d, 1);
+      d += __shfl_xor_sync(0xffffffffu, d, 2);
+      delta[e] = d;
+      if (t4 == 0 && row < p.M) p.delta[stat(oh) + row] = d;
+    }
+  }
+
+  for (int t = 0; t < steps; ++t) {
+    const int stage = t & 1;
+    const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
+    const int at = first + (MODE == D_DKV ? t % per_head : t) * kPart;
+    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};  // the mask of this tile's keys
+    if (MODE != D_DKV && mask) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int j = at + 32 * w + lane;
+        seen[w] = __ballot_sync(0xffffffffu, j < len.nk && mask[j] != 0);
+      }
+    }
+    if (KIND == MF_BUCKETS_PAIR && MODE == D_DKV && t % per_head == 0) {  // another head: another column of the table
+      __syncthreads();
+      for (int i = tid; i < kTableEntries; i += kThreads) table[i] = dense_bias_entry(p, i, h);
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // tile t has arrived, and everybody is done with the buffers of tile t - 1
+    if (t + 1 < steps) load_step(t + 1, stage ^ 1);
+    cp_async_commit();
+
+    const uint32_t pa = s_part_a + stage * TILE, pb = s_part_b + stage * TILE;
+    float s[8][4], dp[MODE == D_FWD ? 1 : 8][4];
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[nt][e] = 0.f;
+        if constexpr (MODE != D_FWD) dp[nt][e] = 0.f;
+      }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a[4], a2[4];
+      ldmatrix_x4(a, s_own_a + ((warp * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8) * 2);
+      if (MODE != D_FWD) ldmatrix_x4(a2, s_own_b + ((warp * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        const uint32_t off = ((np * 16 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8) * 2;
+        uint32_t w[4];
+        ldmatrix_x4(w, pa + off);
+        mma16816<T>(s[2 * np], a, w[0], w[1]);
+        mma16816<T>(s[2 * np + 1], a, w[2], w[3]);
+        if constexpr (MODE != D_FWD) {
+          ldmatrix_x4(w, pb + off);
+          mma16816<T>(dp[2 * np], a2, w[0], w[1]);
+          mma16816<T>(dp[2 * np + 1], a2, w[2], w[3]);
+        }
+      }
+    }
+
+    // ---- logits in units of log2, minus infinity where nothing is seen
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1), x = at + c;
+        const bool vis = x >= lo[e >> 1] && x < hi[e >> 1] && ((seen[nt >> 2] >> (c & 31)) & 1u);
+        float z = s[nt][e] * sc2;
+        if (KIND == MF_BUCKETS_OFFSET) z += offset_bias[stage * 128 + (MODE == D_DKV ? r - c + kPart - 1 : c - r + kOwn - 1)];
+        if (KIND == MF_BUCKETS_PAIR && vis) {
+          const int i = MODE == D_DKV ? x : row0 + r, j = MODE == D_DKV ? row0 + r : x;
+          z += table[p.buckets[b * p.bucket_batch + i * p.bucket_row + j]];
+        }
+        s[nt][e] = vis ? z : -INFINITY;
+      }
+
+    if (MODE == D_FWD) {
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float m = top[e];
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) m = fmaxf(m, fmaxf(s[nt][2 * e], s[nt][2 * e + 1]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float shift = m == -INFINITY ? 0.f : m;
+        alpha[e] = dense_exp2(top[e] - shift);
+        top[e] = m;
+        float sum = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            s[nt][2 * e + x] = dense_exp2(s[nt][2 * e + x] - shift);
+            sum += s[nt][2 * e + x];
+          }
+        total[e] = total[e] * alpha[e] + sum;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc0[i][e] *= alpha[e >> 1];
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = nt * 8 + 2 * t4 + (e & 1);
+          const float z = s[nt][e];
+          const float l = MODE == D_DQ ? lse[e >> 1] : part_lse[stage * 64 + c];
+          const float d = MODE == D_DQ ? delta[e >> 1] : part_delta[stage * 64 + c];
+          const float pr = z == -INFINITY ? 0.f : dense_exp2(z - l);
+          s[nt][e] = pr;
+          dp[nt][e] = pr == 0.f ? 0.f : pr * (dp[nt][e] - d);
+        }
+      if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
+        // a column of sums for every lane: no two threads meet in one, and the order of a sum is that of the walk
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1), x = at + c;
+            if (x < hi[e >> 1]) {
+              const int bucket = KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1]
+                                                           : p.buckets[b * p.bucket_batch + (row0 + r) * p.bucket_row + x];
+              my_sums[min(bucket, nb) * 32] += dp[nt][e];
+            }
+          }
+      }
+    }
+
+    // ---- products with the partners' rows
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t a[4], a2[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int nt = 2 * kk + (x >> 1), e = 2 * (x & 1);
+        a[x] = pack2<T>(s[nt][e], s[nt][e + 1]);
+        if constexpr (MODE != D_FWD) a2[x] = pack2<T>(dp[nt][e], dp[nt][e + 1]);
+      }
+#pragma unroll
+      for (int np = 0; np < D / 16; ++np) {
+        const uint32_t off = ((kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + np * 16 + (lane >> 4) * 8) * 2;
+        uint32_t w[4];
+        if constexpr (MODE == D_FWD) {
+          ldmatrix_x4_trans(w, pb + off);
+          mma16816<T>(acc0[2 * np], a, w[0], w[1]);
+          mma16816<T>(acc0[2 * np + 1], a, w[2], w[3]);
+        } else {
+          ldmatrix_x4_trans(w, pa + off);
+          mma16816<T>(acc0[2 * np], a2, w[0], w[1]);
+          mma16816<T>(acc0[2 * np + 1], a2, w[2], w[3]);
+        }
+        if constexpr (MODE == D_DKV) {
+          ldmatrix_x4_trans(w, pb + off);
+          mma16816<T>(acc1[2 * np], a, w[0], w[1]);
+          mma16816<T>(acc1[2 * np + 1], a, w[2], w[3]);
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+
+  // ---- rows out: zeros behind the lengths
+  float mul[2] = {1.f, 1.f};
+  if (MODE == D_FWD) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float l = total[e];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      mul[e] = l > 0.f || l != l ? 1.f / l : 0.f;
+      const int row = my + 8 * e;
+      if (p.lse && t4 == 0 && row < p.M) p.lse[stat(oh) + row] = l > 0.f || l != l ? top[e] + log2f(l) : INFINITY;
+    }
+  }
+  const int limit = MODE == D_DKV ? p.N : p.M;
+  auto store = [&](void* base, const DenseRows& rows, const float (&acc)[D / 8][4], float m0, float m1) {
+    T* dst = static_cast<T*>(base) + rows.at(b, oh, 0);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = my + 8 * e;
+      if (row >= limit) continue;
+      const float m = e ? m1 : m0;
+#pragma unroll
+      for (int nt = 0; nt < D / 8; ++nt)
+        *reinterpret_cast<uint32_t*>(dst + row * rows.token + nt * 8 + 2 * t4) = pack2<T>(acc[nt][2 * e] * m, acc[nt][2 * e + 1] * m);
+    }
+  };
+  if (MODE == D_FWD) store(p.out, p.out_rows, acc0, mul[0], mul[1]);
+  if (MODE == D_DQ && p.dq) store(p.dq, p.dq_rows, acc0, p.scale, p.scale);
+  if constexpr (MODE == D_DKV) {
+    if (p.dk) store(p.dk, p.dk_rows, acc0, p.scale, p.scale);
+    if (p.dv) store(p.dv, p.dv_rows, acc1, 1.f, 1.f);
+  }
+  if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
+    __syncthreads();
+    float* part = p.dbias_part + ((long long)entry * tiles + tile) * nb;
+    for (int i = warp; i < nb; i += 4) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v += sums[(w * (nb + 1) + i) * 32 + lane];
+      v = warp_sum(v);
+      if (lane == 0) part[i] = v;
+    }
+  }
+}
+
+template <typename T, int D, int MODE, int KIND>
+int launch(const DenseParams& p, cudaStream_t stream) {
+  const int own = MODE == D_DKV ? p.N : p.M, heads = MODE == D_DKV ? p.K : p.H;
+  if (own == 0) return MF_OK;
+  const int smem = kFixedBytes<D> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
+  auto kernel = dense_attn_mma_kernel<T, D, MODE, KIND>;
+  // one limit for all calls: what the largest table needs
+  constexpr int most = kFixedBytes<D> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
+  static_assert(most <= 227 * 1024, "");
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
+  kernel<<<(own + kOwn - 1) / kOwn * p.B * heads, kThreads, smem, stream>>>(p);
+  MF_CHECK_LAUNCH("dense attention");
+  return MF_OK;
+}
+
+template <typename T, int MODE>
+int pick(const DenseParams& p, int head_dim, int kind, cudaStream_t stream) {
+  auto by_kind = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    return kind == MF_BUCKETS_NONE     ? launch<T, D, MODE, MF_BUCKETS_NONE>(p, stream)
+           : kind == MF_BUCKETS_OFFSET ? launch<T, D, MODE, MF_BUCKETS_OFFSET>(p, stream)
+                                       : launch<T, D, MODE, MF_BUCKETS_PAIR>(p, stream);
+  };
+  return head_dim == 32   ? by_kind(std::integral_constant<int, 32>{})
+         : head_dim == 64 ? by_kind(std::integral_constant<int, 64>{})
+                          : by_kind(std::integral_constant<int, 128>{});
+}
+
+}  // namespace
+
+int dense_attn_mma_tiles(int queries) { return (queries + kOwn - 1) / kOwn; }
+int dense_attn_mma_fwd(const DenseParams& p, int dtype, int head_dim, int kind, cudaStream_t stream) {
+  return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16, D_FWD>(p, head_dim, kind, stream) : pick<__half, D_FWD>(p, head_dim, kind, stream);
+}
+int dense_attn_mma_bwd(const DenseParams& p, int dtype, int head_dim, int kind, cudaStream_t stream) {
+  const int rc = dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16, D_DQ>(p, head_dim, kind, stream) : pick<__half, D_DQ>(p, head_dim, kind, stream);
+  if (rc != MF_OK || (!p.dk && !p.dv)) return rc;
+  return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16, D_DKV>(p, head_dim, kind, stream) : pick<__half, D_DKV>(p, head_dim, kind, stream);
+}
+
+}  // namespace mf
