@@ -7,6 +7,8 @@ namespace {
 // dbias[bucket][head] = sum of the partial sums of all tiles of the head, over batch entries and tiles in order; a block for every (head, bucket),
 // sums in fp64 (they are long and cancel)
 __global__ void __launch_bounds__(128) bias_sum_kernel(const float* part, int B, int H, int tiles, int nb, void* out, int dtype) {
+  launch_dependents();
+  wait_for_previous();
   const int h = blockIdx.x % H, bucket = blockIdx.x / H;
   const long long n = (long long)B * tiles;
   double sum = 0.0;
@@ -27,27 +29,67 @@ __global__ void __launch_bounds__(128) bias_sum_kernel(const float* part, int B,
   }
 }
 
-constexpr int kMaxEdges = kMaxBuckets - 1;
+constexpr int kMaxEdges = kMaxBuckets - 1, kCells = 512;
 struct Edges {
-  double square[kMaxEdges];
+  double square[kMaxEdges + 1];  // of the edges, then infinity
+  float low[kMaxEdges + 1];      // the same in fp32
+  uint8_t first[kCells];         // edges at or below the start of a cell of distances
+  float cells_per_unit;
+  int n;
 };
 
-// One thread per pair.  The squared distance is formed in fp64, where the differences of fp32 coordinates are exact but for far apart exponents,
-// so that a pair next to an edge falls on the side that it belongs to.
-__global__ void __launch_bounds__(256) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int B, int N, const __grid_constant__ Edges edges,
-                                                               int n_edges, uint8_t* out, long long batch_stride, long long row) {
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x, square = (long long)N * N;
-  if (at >= B * square) return;
-  const int b = at / square, i = at % square / N, j = at % N;
-  const int n = num_atoms ? num_atoms[b] : N;
-  int count = 0;
-  if (i < n && j < n) {
-    const float *x = coords + ((long long)b * N + i) * 3, *y = coords + ((long long)b * N + j) * 3;
-    const double dx = (double)x[0] - y[0], dy = (double)x[1] - y[1], dz = (double)x[2] - y[2];
-    const double d2 = __dadd_rn(__dadd_rn(__dmul_rn(dx, dx), __dmul_rn(dy, dy)), __dmul_rn(dz, dz));
-    for (int e = 0; e < n_edges; ++e) count += d2 >= edges.square[e];
+// A warp takes 128 columns, four to a lane, whose coordinates stay in registers, and walks over kBucketRows rows.  The squared distance is formed in
+// fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares) and its bucket found from a table of cells of the distance; a pair within that
+// error of an edge, or whose square leaves fp32's range, is decided in fp64, where the differences of fp32 coordinates are exact but for far apart exponents.  All pairs in fp64
+// against all edges took 463 us for two cells of 4096 atoms and 63 edges.
+constexpr int kBucketRows = 16, kBucketWarps = 8;
+__global__ void __launch_bounds__(kBucketWarps * 32) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int N, const __grid_constant__ Edges edges,
+                                                                             uint8_t* out, long long batch_stride, long long row, int words) {
+  __shared__ float low[kMaxEdges + 2];  // minus infinity first
+  __shared__ uint8_t first[kCells];
+  launch_dependents();
+  wait_for_previous();
+  for (int i = threadIdx.x; i < kCells; i += kBucketWarps * 32) first[i] = edges.first[i];
+  for (int i = threadIdx.x; i <= edges.n + 1; i += kBucketWarps * 32) low[i] = i == 0 ? -INFINITY : edges.low[i - 1];
+  __syncthreads();
+  const int lane = threadIdx.x & 31, column_tiles = (N + 127) / 128, row_tiles = (N + kBucketRows * kBucketWarps - 1) / (kBucketRows * kBucketWarps);
+  const int ct = blockIdx.x % column_tiles, rt = blockIdx.x / column_tiles % row_tiles, b = blockIdx.x / column_tiles / row_tiles;
+  const int n = num_atoms ? min(num_atoms[b], N) : N;
+  const int j0 = ct * 128 + lane * 4, i0 = (rt * kBucketWarps + (threadIdx.x >> 5)) * kBucketRows;
+  const float* x = coords + (long long)b * N * 3;
+  float y[4][3];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int a = 0; a < 3; ++a) y[c][a] = j0 + c < n ? x[(j0 + c) * 3ll + a] : 0.f;
+  for (int i = i0; i < min(i0 + kBucketRows, N); ++i) {
+    uint32_t word = 0;
+    if (i < n) {
+      const float xi[3] = {x[i * 3ll], x[i * 3ll + 1], x[i * 3ll + 2]};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float dx = xi[0] - y[c][0], dy = xi[1] - y[c][1], dz = xi[2] - y[c][2];
+        const float d2 = fmaf(dz, dz, fmaf(dy, dy, dx * dx));
+        float root;
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(d2));
+        int k = first[(int)fminf(root * edges.cells_per_unit, (float)(kCells - 1))];
+        while (d2 >= low[k + 1] && k < edges.n) ++k;
+        const float margin = d2 * 5e-7f;
+        if (!(d2 > 1e-30f && d2 < 1e30f) || d2 - low[k] <= margin || low[k + 1] - d2 <= margin) {
+          const double ex = (double)xi[0] - y[c][0], ey = (double)xi[1] - y[c][1], ez = (double)xi[2] - y[c][2];
+          const double e2 = __dadd_rn(__dadd_rn(__dmul_rn(ex, ex), __dmul_rn(ey, ey)), __dmul_rn(ez, ez));
+          for (k = 0; k < edges.n && e2 >= edges.square[k]; ++k) {}
+        }
+        word |= (j0 + c < n ? (uint32_t)k : 0u) << (8 * c);
+      }
+    }
+    uint8_t* dst = out + b * batch_stride + i * row + j0;
+    if (words) {  // rows that hold whole words, behind the last atom too
+      if (j0 < row) *reinterpret_cast<uint32_t*>(dst) = word;
+    } else {
+      for (int c = 0; c < 4 && j0 + c < N; ++c) dst[c] = (uint8_t)(word >> (8 * c));
+    }
   }
-  out[b * batch_stride + i * row + j] = (uint8_t)count;
 }
 
 DenseRows rows_of(const MfRows& r) { return DenseRows{r.batch, r.head, r.token}; }
@@ -104,16 +146,26 @@ DenseParams params_of(const MfDenseAttnArgs& a) {
   return p;
 }
 
+enum Family { kMma, kSmall, kSplit };
+Family fwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
+  if (a.backend != MF_DENSE_BACKEND_AUTO) return kMma;
+  return dense_attn_small_applies(p, false) ? kSmall : dense_attn_split_applies(p) ? kSplit : kMma;
+}
+Family bwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
+  return a.backend == MF_DENSE_BACKEND_AUTO && dense_attn_small_applies(p, true) ? kSmall : kMma;
+}
+
 struct BwdSpace {
-  size_t delta, part, total;
-  int tiles;
+  size_t part, total;
+  int entries, tiles;  // partial sums of the table's gradient for each head
 };
-BwdSpace bwd_space(const MfDenseAttnArgs& a) {
+BwdSpace bwd_space(const MfDenseAttnArgs& a, const DenseParams& p) {
   BwdSpace s{};
-  s.tiles = dense_attn_mma_tiles(a.queries);
-  s.delta = 0;
-  s.part = align_up((size_t)a.batch * a.heads * a.queries * sizeof(float), 256);
-  s.total = s.part + (a.bias && a.dbias ? align_up((size_t)a.batch * a.heads * s.tiles * a.num_buckets * sizeof(float), 256) : 0);
+  const bool small = bwd_family(a, p) == kSmall;
+  s.entries = small ? dense_attn_small_slots(p, a.head_dim) : a.batch;
+  s.tiles = small ? 1 : dense_attn_mma_tiles(a.queries);
+  s.part = small ? 0 : align_up((size_t)a.batch * a.heads * a.queries * sizeof(float), 256);
+  s.total = s.part + (a.bias && a.dbias ? align_up((size_t)s.entries * a.heads * s.tiles * a.num_buckets * sizeof(float), 256) : 0);
   return s;
 }
 
@@ -122,18 +174,36 @@ BwdSpace bwd_space(const MfDenseAttnArgs& a) {
 
 extern "C" {
 
-size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs*) { return 0; }
+size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs* a) {
+  using namespace mf;
+  if (check_args("mf_dense_attn_fwd_workspace_bytes", a) != MF_OK || a->batch == 0 || a->queries == 0) return 0;
+  const DenseParams p = params_of(*a);
+  return fwd_family(*a, p) == kSplit ? dense_attn_split_workspace_bytes(p, a->head_dim) : 0;
+}
 size_t mf_dense_attn_bwd_workspace_bytes(const MfDenseAttnArgs* a) {
-  if (!a || a->batch < 0 || a->heads < 1 || a->queries < 0 || a->num_buckets < 0) return 0;
-  return mf::bwd_space(*a).total;
+  using namespace mf;
+  if (check_args("mf_dense_attn_bwd_workspace_bytes", a) != MF_OK || a->batch == 0) return 0;
+  return bwd_space(*a, params_of(*a)).total;
 }
 
 int mf_dense_attn_fwd(const MfDenseAttnArgs* a, void* stream_) {
   using namespace mf;
-  const int rc = check_args("mf_dense_attn_fwd", a);
+  const char* name = "mf_dense_attn_fwd";
+  const int rc = check_args(name, a);
   if (rc != MF_OK) return rc;
   if (a->batch == 0 || a->queries == 0) return MF_OK;
-  return dense_attn_mma_fwd(params_of(*a), a->dtype, a->head_dim, a->bucket_kind, static_cast<cudaStream_t>(stream_));
+  const DenseParams p = params_of(*a);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  switch (fwd_family(*a, p)) {
+    case kSmall: return dense_attn_small(p, a->dtype, a->head_dim, a->bucket_kind, false, stream);
+    case kSplit: {
+      const size_t need = dense_attn_split_workspace_bytes(p, a->head_dim);
+      MF_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need && aligned16(a->workspace)), "%s: %zu bytes of workspace needed, got %zu", name, need,
+                   a->workspace_bytes);
+      return dense_attn_split(p, a->dtype, a->head_dim, a->bucket_kind, a->workspace, stream);
+    }
+    default: return dense_attn_mma_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
+  }
 }
 
 int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
@@ -142,45 +212,57 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
   int rc = check_args(name, a);
   if (rc != MF_OK) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (a->batch == 0) return MF_OK;
-  const BwdSpace space = bwd_space(*a);
+  DenseParams p = params_of(*a);
+  const bool table = a->bias && a->dbias;
+  const BwdSpace space = a->batch ? bwd_space(*a, p) : BwdSpace{};
   MF_CHECK_ARG(space.total == 0 || (a->workspace && a->workspace_bytes >= space.total && aligned16(a->workspace)), "%s: %zu bytes of workspace needed, got %zu", name,
                space.total, a->workspace_bytes);
-  MF_CHECK_ARG(a->queries == 0 || (a->grad_out && a->lse), "%s: grad_out and lse must not be NULL", name);
-  if ((a->queries > 0 && MF_OK != (rc = check_rows(name, "grad_out", a->grad_out, a->grad_out_rows))) ||
-      (a->dq && MF_OK != (rc = check_rows(name, "dq", a->dq, a->dq_rows))) || (a->dk && MF_OK != (rc = check_rows(name, "dk", a->dk, a->dk_rows))) ||
-      (a->dv && MF_OK != (rc = check_rows(name, "dv", a->dv, a->dv_rows))))
-    return rc;
-  DenseParams p = params_of(*a);
-  char* ws = static_cast<char*>(a->workspace);
-  p.delta = reinterpret_cast<float*>(ws + space.delta);
-  const bool table = a->bias && a->dbias;
-  if (table) p.dbias_part = reinterpret_cast<float*>(ws + space.part);
-  rc = dense_attn_mma_bwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
-  if (rc != MF_OK || !table) return rc;
-  bias_sum_kernel<<<a->heads * a->num_buckets, 128, 0, stream>>>(p.dbias_part, a->batch, a->heads, space.tiles, a->num_buckets, a->dbias, a->bias_dtype);
-  MF_CHECK_LAUNCH("dense attention table gradient");
-  return MF_OK;
+  if (a->batch > 0) {
+    MF_CHECK_ARG(a->queries == 0 || (a->grad_out && a->lse), "%s: grad_out and lse must not be NULL", name);
+    if ((a->queries > 0 && MF_OK != (rc = check_rows(name, "grad_out", a->grad_out, a->grad_out_rows))) ||
+        (a->dq && MF_OK != (rc = check_rows(name, "dq", a->dq, a->dq_rows))) || (a->dk && MF_OK != (rc = check_rows(name, "dk", a->dk, a->dk_rows))) ||
+        (a->dv && MF_OK != (rc = check_rows(name, "dv", a->dv, a->dv_rows))))
+      return rc;
+    char* ws = static_cast<char*>(a->workspace);
+    p.delta = reinterpret_cast<float*>(ws);
+    if (table) p.dbias_part = reinterpret_cast<float*>(ws + space.part);
+    rc = bwd_family(*a, p) == kSmall ? dense_attn_small(p, a->dtype, a->head_dim, a->bucket_kind, true, stream)
+                                     : dense_attn_mma_bwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
+    if (rc != MF_OK) return rc;
+  }
+  if (!table) return MF_OK;
+  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * a->num_buckets), dim3(128), 0, stream, p.dbias_part, space.entries, a->heads, space.tiles,
+                                           a->num_buckets, a->dbias, a->bias_dtype);
+  return err == cudaSuccess ? MF_OK : cuda_error(err, "dense attention table gradient");
 }
 
 int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t batch, int32_t tokens, const double* edges, int32_t num_edges, uint8_t* buckets,
                         int64_t batch_stride, int64_t row, void* stream) {
   using namespace mf;
   const char* name = "mf_distance_buckets";
-  MF_CHECK_ARG(batch >= 0 && tokens >= 0 && tokens <= 1 << 20 && (long long)batch * tokens * tokens < (1ll << 39), "%s: sizes out of range: %d molecules of %d atoms", name, batch, tokens);
+  const long long tiles = ((tokens + 127ll) / 128) * ((tokens + kBucketRows * kBucketWarps - 1ll) / (kBucketRows * kBucketWarps)) * batch;
+  MF_CHECK_ARG(batch >= 0 && tokens >= 0 && tokens <= 1 << 20 && tiles < (1ll << 31), "%s: sizes out of range: %d molecules of %d atoms", name, batch, tokens);
   MF_CHECK_ARG(num_edges >= 0 && num_edges <= kMaxEdges && (num_edges == 0 || edges), "%s: at most %d edges, got %d", name, kMaxEdges, num_edges);
   Edges e{};
   for (int i = 0; i < num_edges; ++i) {
     MF_CHECK_ARG(edges[i] >= 0.0 && (i == 0 || edges[i] >= edges[i - 1]), "%s: edges must ascend from 0 on", name);
     e.square[i] = edges[i] * edges[i];
+    e.low[i] = (float)e.square[i];
+  }
+  e.n = num_edges, e.square[num_edges] = INFINITY, e.low[num_edges] = INFINITY;
+  const double last = num_edges ? edges[num_edges - 1] : 0.0;
+  e.cells_per_unit = last > 1e-30 && last < 1e30 ? (float)((kCells - 1) / last) : 0.f;
+  for (int c = 0, k = 0; c < kCells; ++c) {  // a cell's start a little lower than it is, for the rounding of the distance
+    const double start = e.cells_per_unit > 0.f ? c / (double)e.cells_per_unit * (1.0 - 1e-5) : 0.0;
+    while (k < num_edges && edges[k] < start) ++k;
+    e.first[c] = (uint8_t)k;
   }
   if (batch == 0 || tokens == 0) return MF_OK;
   MF_CHECK_ARG(coords && buckets && row >= tokens && batch_stride >= (int64_t)(tokens - 1) * row + tokens, "%s: rows of the buckets must hold %d entries", name, tokens);
-  const long long pairs = (long long)batch * tokens * tokens;
-  distance_buckets_kernel<<<(unsigned)((pairs + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(coords, num_atoms, batch, tokens, e, num_edges, buckets, batch_stride,
-                                                                                                       row);
-  MF_CHECK_LAUNCH(name);
-  return MF_OK;
+  const int words = row % 4 == 0 && batch_stride % 4 == 0 && batch_stride >= tokens * row && reinterpret_cast<uintptr_t>(buckets) % 4 == 0;
+  const cudaError_t err = launch_dependent(distance_buckets_kernel, dim3((unsigned)tiles), dim3(kBucketWarps * 32), 0, static_cast<cudaStream_t>(stream), coords, num_atoms,
+                                           tokens, e, buckets, batch_stride, row, words);
+  return err == cudaSuccess ? MF_OK : cuda_error(err, name);
 }
 
 }  // extern "C"

@@ -94,5 +94,13 @@ __device__ __forceinline__ float dense_exp2(float x) {
 int dense_attn_mma_fwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream);
 int dense_attn_mma_bwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream);
 int dense_attn_mma_tiles(int queries);  // query tiles of the backward pass
+// dense_attn_small.cu: at most 32 queries and keys
+bool dense_attn_small_applies(const DenseParams& p, bool backward);
+int dense_attn_small_slots(const DenseParams& p, int head_dim);  // partial sums of the table's gradient for each head
+int dense_attn_small(const DenseParams& p, int dtype, int head_dim, int bucket_kind, bool backward, cudaStream_t stream);
+// dense_attn_split.cu: forward, few queries
+bool dense_attn_split_applies(const DenseParams& p);
+size_t dense_attn_split_workspace_bytes(const DenseParams& p, int head_dim);
+int dense_attn_split(const DenseParams& p, int dtype, int head_dim, int bucket_kind, void* workspace, cudaStream_t stream);
 
 }  // namespace mf

@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     }
   }
   const int limit = MODE == D_DKV ? p.N : p.M;
-  auto store = [&](void* base, const DenseRows& rows, const float (&acc)[D / 8][4], float m0, float m1) {
+  auto store = [&](void* base, const DenseRows& rows, const float (&acc)[D / 8][4], float m0, float m1) {  // a factor of zero: zeros, whatever was summed
     T* dst = static_cast<T*>(base) + rows.at(b, oh, 0);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -353,14 +353,15 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
       const float m = e ? m1 : m0;
 #pragma unroll
       for (int nt = 0; nt < D / 8; ++nt)
-        *reinterpret_cast<uint32_t*>(dst + row * rows.token + nt * 8 + 2 * t4) = pack2<T>(acc[nt][2 * e] * m, acc[nt][2 * e + 1] * m);
+        *reinterpret_cast<uint32_t*>(dst + row * rows.token + nt * 8 + 2 * t4) = m == 0.f ? 0u : pack2<T>(acc[nt][2 * e] * m, acc[nt][2 * e + 1] * m);
     }
   };
   if (MODE == D_FWD) store(p.out, p.out_rows, acc0, mul[0], mul[1]);
-  if (MODE == D_DQ && p.dq) store(p.dq, p.dq_rows, acc0, p.scale, p.scale);
+  const float real0 = hi[0] > 0 ? 1.f : 0.f, real1 = hi[1] > 0 ? 1.f : 0.f;
+  if (MODE == D_DQ && p.dq) store(p.dq, p.dq_rows, acc0, real0 * p.scale, real1 * p.scale);
   if constexpr (MODE == D_DKV) {
-    if (p.dk) store(p.dk, p.dk_rows, acc0, p.scale, p.scale);
-    if (p.dv) store(p.dv, p.dv_rows, acc1, 1.f, 1.f);
+    if (p.dk) store(p.dk, p.dk_rows, acc0, real0 * p.scale, real1 * p.scale);
+    if (p.dv) store(p.dv, p.dv_rows, acc1, real0, real1);
   }
   if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
     __syncthreads();
