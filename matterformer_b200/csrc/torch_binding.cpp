@@ -584,6 +584,213 @@ std::optional<tensor_list> rotary(const Tensor& first, const OptTensor& second, 
   return Rotary::apply(first, second, positions, by, foreign_leaves({&first, second ? &*second : &none}));
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Dense attention with a learned bias by buckets
+// ---------------------------------------------------------------------------------------------------------------------
+struct DenseCall : torch::CustomClassHolder {
+  int64_t heads, backend;  // heads 0: head-major q, k, v; otherwise a packed projection with that many heads
+  bool causal, foreign;
+  double scale;
+  DenseCall(int64_t heads_, int64_t backend_, bool causal_, bool foreign_, double scale_)
+      : heads(heads_), backend(backend_), causal(causal_), foreign(foreign_), scale(scale_) {}
+};
+
+struct DenseAttention : torch::autograd::Function<DenseAttention> {
+  enum { Q, K, V, BIAS, BUCKETS, NUM_Q, NUM_K, MASK, kOperands };
+  using Operands = std::array<Tensor, kOperands>;
+
+  static MfRows rows(const Tensor& t) {
+    auto step = [&](int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+    return {step(0), step(1), step(2)};
+  }
+  // the third `i` of a packed (B, N, 3 H D), or all of a packed (B, N, H D)
+  static MfRows packed_rows(const Tensor& t, int64_t D) { return {t.size(1) * t.size(2), D, t.size(2)}; }
+  static const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+  static void fill(MfDenseAttnArgs& a, const Operands& t, const DenseCall& call) {
+    const Tensor& q = t[Q];
+    a.dtype = dtype_code(q), a.causal = call.causal, a.backend = call.backend, a.scale = call.scale;
+    a.batch = q.size(0);
+    if (call.heads) {
+      const int64_t HD = q.size(2) / 3;
+      a.heads = a.kv_heads = call.heads, a.queries = a.keys = q.size(1), a.head_dim = HD / call.heads;
+      a.q = q.const_data_ptr(), a.k = static_cast<const char*>(a.q) + 2 * HD, a.v = static_cast<const char*>(a.q) + 4 * HD;
+      a.q_rows = a.k_rows = a.v_rows = packed_rows(q, a.head_dim);
+    } else {
+      a.heads = q.size(1), a.queries = q.size(2), a.head_dim = q.size(3), a.kv_heads = t[K].size(1), a.keys = t[K].size(2);
+      a.q = q.const_data_ptr(), a.k = t[K].const_data_ptr(), a.v = t[V].const_data_ptr();
+      a.q_rows = rows(q), a.k_rows = rows(t[K]), a.v_rows = rows(t[V]);
+    }
+    a.num_queries = static_cast<const int32_t*>(ptr(t[NUM_Q])), a.num_keys = static_cast<const int32_t*>(ptr(t[NUM_K]));
+    a.key_mask = static_cast<const uint8_t*>(ptr(t[MASK])), a.key_mask_batch = a.keys;
+    if (t[BIAS].defined()) {
+      const Tensor& buckets = t[BUCKETS];
+      a.bias = t[BIAS].const_data_ptr(), a.bias_dtype = dtype_code(t[BIAS]), a.num_buckets = t[BIAS].size(0);
+      a.buckets = static_cast<const uint8_t*>(buckets.const_data_ptr());
+      if (buckets.dim() == 1) a.bucket_kind = MF_BUCKETS_OFFSET, a.reach = buckets.size(0) / 2;
+      else a.bucket_kind = MF_BUCKETS_PAIR, a.bucket_batch = buckets.size(0) > 1 ? buckets.stride(0) : 0, a.bucket_row = buckets.stride(1);
+    }
+  }
+  // A dense (B, H, N, D) tensor in the order of tokens and heads of t.
+  static Tensor like(const Tensor& t) {
+    const int64_t B = t.size(0), H = t.size(1), N = t.size(2), D = t.size(3);
+    if (H > 1 && N > 1 && t.stride(1) < t.stride(2)) return fresh({B, N, H, D}, t.scalar_type(), t).transpose(1, 2);
+    return fresh({B, H, N, D}, t.scalar_type(), t);
+  }
+
+  struct Made {
+    Tensor out, lse;
+  };
+  static Made attend(const Operands& t, const DenseCall& call, bool keep) {
+    const Tensor& q = t[Q];
+    const c10::cuda::CUDAGuard guard(q.device());
+    MfDenseAttnArgs a{};
+    fill(a, t, call);
+    const Tensor out = call.heads ? fresh({q.size(0), q.size(1), q.size(2) / 3}, q.scalar_type(), q) : like(q);
+    a.out = out.data_ptr(), a.out_rows = call.heads ? packed_rows(out, a.head_dim) : rows(out);
+    const Tensor lse = keep ? fresh({a.batch, a.heads, a.queries}, at::kFloat, q) : Tensor();
+    a.lse = keep ? lse.data_ptr<float>() : nullptr;
+    const Tensor ws = fresh_bytes(mf_dense_attn_fwd_workspace_bytes(&a), q);
+    if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+    check(mf_dense_attn_fwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
+    return {out, lse};
+  }
+
+  static Variable forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& v, const OptTensor& bias, const Operands& t,
+                          const c10::intrusive_ptr<DenseCall>& call) {
+    const Made made = attend(t, *call, true);
+    ctx->saved_data["call"] = c10::IValue::make_capsule(call);
+    tensor_list saved(t.begin(), t.end());
+    saved.push_back(made.out);
+    saved.push_back(made.lse);
+    ctx->save_for_backward(std::move(saved));
+    return made.out;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grad_out) {
+    const auto held = ctx->saved_data["call"].toCapsule();
+    const DenseCall& call = static_cast<const DenseCall&>(*held);
+    refuse_foreign(call.foreign, "dense_attention");
+    const tensor_list s = ctx->get_saved_variables();
+    Operands t;
+    std::copy_n(s.begin(), (int)kOperands, t.begin());
+    const Tensor &q = t[Q], &out = s[kOperands];
+    const c10::cuda::CUDAGuard guard(q.device());
+    tensor_list g(6);  // (one for each argument of forward)
+    {
+      const at::NoGradGuard no_grad;
+      MfDenseAttnArgs a{};
+      fill(a, t, call);
+      Tensor go = grad_out[0].to(q.scalar_type());
+      if (!(call.heads ? go.is_contiguous() && aligned(go) : rows_ready(go))) go = go.is_contiguous() ? go.clone() : go.contiguous();
+      a.out = out.data_ptr(), a.lse = s[kOperands + 1].data_ptr<float>(), a.grad_out = go.const_data_ptr();
+      a.out_rows = call.heads ? packed_rows(out, a.head_dim) : rows(out), a.grad_out_rows = call.heads ? packed_rows(go, a.head_dim) : rows(go);
+      size_t edge = 0;  // edges of the node are counted over the tensors that were given
+      bool wants[4];
+      for (int i = Q; i <= BIAS; ++i) wants[i] = t[i].defined() && ctx->needs_input_grad(edge++);
+      if (call.heads) {
+        if (wants[Q]) {
+          const int64_t HD = q.size(2) / 3;
+          g[Q] = fresh(q.sizes(), q.scalar_type(), q);
+          a.dq = g[Q].data_ptr(), a.dk = static_cast<char*>(a.dq) + 2 * HD, a.dv = static_cast<char*>(a.dq) + 4 * HD;
+          a.dq_rows = a.dk_rows = a.dv_rows = packed_rows(q, a.head_dim);
+        }
+      } else {
+        for (int i = Q; i <= V; ++i)
+          if (wants[i]) g[i] = like(t[i]);
+        if (wants[Q]) a.dq = g[Q].data_ptr(), a.dq_rows = rows(g[Q]);
+        if (wants[K]) a.dk = g[K].data_ptr(), a.dk_rows = rows(g[K]);
+        if (wants[V]) a.dv = g[V].data_ptr(), a.dv_rows = rows(g[V]);
+      }
+      if (wants[BIAS]) g[BIAS] = fresh(t[BIAS].sizes(), t[BIAS].scalar_type(), q), a.dbias = g[BIAS].data_ptr();
+      const Tensor ws = fresh_bytes(mf_dense_attn_bwd_workspace_bytes(&a), q);
+      if (ws.defined()) a.workspace = ws.data_ptr(), a.workspace_bytes = ws.numel();
+      check(mf_dense_attn_bwd(&a, c10::cuda::getCurrentCUDAStream().stream()));
+    }
+    if (at::GradMode::is_enabled()) {  // create_graph: an error for who differentiates again
+      tensor_list given;
+      for (int i = Q; i <= BIAS; ++i)
+        if (g[i].defined()) given.push_back(g[i].set_requires_grad(true));
+      const auto node = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable",
+                                                                        (int64_t)given.size());
+      const tensor_list made = (*node)(std::move(given));
+      for (int i = Q, j = 0; i <= BIAS; ++i)
+        if (g[i].defined()) g[i] = made[j++];
+    }
+    return g;
+  }
+
+  static bool rows_ready(const Tensor& t) {
+    if (t.stride(3) != 1 || !aligned(t)) return false;
+    for (int d = 0; d < 3; ++d)
+      if (t.size(d) > 1 && t.stride(d) % 8) return false;
+    return true;
+  }
+};
+
+// Operands that are ready as they are, nothing that watches; the C ABI checks sizes.
+std::optional<Tensor> dense_attention(const Tensor& q, const OptTensor& k, const OptTensor& v, const OptTensor& bias, const OptTensor& buckets,
+                                      const OptTensor& num_queries, const OptTensor& num_keys, const OptTensor& key_mask, int64_t heads, bool causal,
+                                      std::optional<double> scale, int64_t backend) {
+  using D = DenseAttention;
+  if (watched() || !q.is_cuda() || (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) || q.numel() == 0) return std::nullopt;
+  int64_t B, M, N, H, C;
+  if (heads) {
+    if (heads < 1 || q.dim() != 3 || q.size(2) % (3 * heads) || !q.is_contiguous() || !aligned(q)) return std::nullopt;
+    B = q.size(0), M = N = q.size(1), H = heads, C = q.size(2) / (3 * heads);
+  } else {
+    if (q.dim() != 4 || !k || !v || k->dim() != 4 || k->sizes() != v->sizes() || k->numel() == 0) return std::nullopt;
+    B = q.size(0), M = q.size(2), N = k->size(2), H = q.size(1), C = q.size(3);
+    if (k->size(0) != B || k->size(3) != C || H % k->size(1)) return std::nullopt;
+    for (const Tensor* t : {&q, &*k, &*v})
+      if (t->scalar_type() != q.scalar_type() || t->device() != q.device() || !D::rows_ready(*t)) return std::nullopt;
+  }
+  if (C != 32 && C != 64 && C != 128) return std::nullopt;
+  if (bias.has_value() != buckets.has_value()) return std::nullopt;
+  if (bias) {
+    if (bias->dim() != 2 || bias->size(1) != H || bias->size(0) < 1 || bias->size(0) > 128 || dtype_code(*bias) < 0 || bias->device() != q.device() || !bias->is_contiguous())
+      return std::nullopt;
+    const Tensor& w = *buckets;
+    if (w.scalar_type() != at::kByte || w.device() != q.device() || w.is_inference()) return std::nullopt;
+    if (w.dim() == 1) {
+      if (w.size(0) % 2 == 0 || !w.is_contiguous()) return std::nullopt;
+    } else if (w.dim() != 3 || (w.size(0) != 1 && w.size(0) != B) || w.size(1) != M || w.size(2) != N || (N > 1 && w.stride(2) != 1)) {
+      return std::nullopt;
+    }
+  }
+  for (const OptTensor* n : {&num_queries, &num_keys})
+    if (*n && ((*n)->dim() != 1 || (*n)->is_inference() || !ready(**n, q, at::kInt, {B}))) return std::nullopt;
+  if (key_mask && (key_mask->is_inference() || !ready(*key_mask, q, at::kBool, {B, N}))) return std::nullopt;
+  const double by = scale ? *scale : 1.0 / std::sqrt((double)C);
+  if (!std::isfinite(by)) return std::nullopt;
+  bool keep = false;
+  for (const Tensor* t : {&q, k ? &*k : &q, v ? &*v : &q, bias ? &*bias : &q}) {
+    if (t->_fw_grad(0).defined()) return std::nullopt;
+    keep = keep || t->requires_grad();
+  }
+  const Tensor none;
+  auto given = [&](const OptTensor& t) { return t ? *t : none; };
+  const D::Operands t = {q, given(k), given(v), given(bias), given(buckets), given(num_queries), given(num_keys), given(key_mask)};
+  if (!keep || !at::GradMode::is_enabled()) return D::attend(t, DenseCall(heads, backend, causal, false, by), false).out;
+  const c10::cuda::CUDAGuard guard(q.device());
+  return D::apply(q, k, v, bias, t, c10::make_intrusive<DenseCall>(heads, backend, causal, foreign_leaves({&q, &t[D::K], &t[D::V], &t[D::BIAS]}), by));
+}
+
+std::optional<Tensor> distance_buckets(const Tensor& coords, const Tensor& edges, const OptTensor& num_atoms) {
+  if (watched() || !coords.is_cuda() || coords.dim() != 3 || coords.size(2) != 3 || coords.scalar_type() != at::kFloat || !coords.is_contiguous() || coords.numel() == 0 ||
+      coords._fw_grad(0).defined())
+    return std::nullopt;
+  if (!edges.device().is_cpu() || edges.scalar_type() != at::kDouble || edges.dim() != 1 || !edges.is_contiguous() || edges.numel() > 127) return std::nullopt;
+  const int64_t B = coords.size(0), N = coords.size(1), row = (N + 15) / 16 * 16;
+  if (num_atoms && !ready(*num_atoms, coords, at::kInt, {B})) return std::nullopt;
+  const c10::cuda::CUDAGuard guard(coords.device());
+  const Tensor out = fresh({B, N, row}, at::kByte, coords);
+  check(mf_distance_buckets(coords.const_data_ptr<float>(), num_atoms ? num_atoms->const_data_ptr<int32_t>() : nullptr, B, N, edges.const_data_ptr<double>(),
+                            edges.numel(), static_cast<uint8_t*>(out.data_ptr()), N * row, row, c10::cuda::getCurrentCUDAStream().stream()));
+  const at::AutoDispatchBelowADInplaceOrView guard_view;
+  return out.as_strided({B, N, N}, {N * row, row, 1});
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -594,6 +801,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("foreign_leaf", &foreign_leaf);
   m.def("gated_mlp", &gated_mlp);
   m.def("rotary", &rotary);
+  m.def("dense_attention", &dense_attention);
+  m.def("distance_buckets", &distance_buckets);
   m.def("remember_status", &remember_status);
   m.def("last_status", &last_status);
 }

@@ -85,6 +85,11 @@ def distance_buckets(coords: torch.Tensor, edges: Union[torch.Tensor, Sequence[f
     """(B, N, N) uint8: how many of the ascending ``edges`` (host values in fp64, at most 127, from 0 on) lie at or below the distance of two atoms of
     ``coords`` (B, N, 3) fp32, compared as squares in 64 bits.  0 where one of the two is padding (at or behind ``num_atoms`` (B)).  On CUDA
     the rows start on 16-byte boundaries, as :func:`dense_attention` reads them fastest (the result is a view of a wider tensor).  No gradient."""
+    native = _lib.native()
+    if native is not None and isinstance(edges, torch.Tensor):
+        out = native.distance_buckets(coords, edges, num_atoms)
+        if out is not None:
+            return out
     if coords.ndim != 3 or coords.shape[-1] != 3 or coords.dtype != torch.float32:
         raise ValueError(f"distance_buckets: coords (B, N, 3) float32 expected, got {tuple(coords.shape)} {coords.dtype}")
     B, N, _ = coords.shape
@@ -359,6 +364,11 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_keys:
     Softmax and sums are in fp32 in a fixed order; probabilities and the gradients of the logits are rounded to the operands' type before
     the products that contract them.  Once differentiable in q, k, v and the table.  What is traced or under a transform of
     ``torch.func`` is the same in plain operations."""
+    native = _lib.native()
+    if native is not None:  # operands that are ready as they are: one call into C++
+        out = native.dense_attention(q, k, v, bias, buckets, num_queries, num_keys, key_mask, 0, bool(causal), scale, _lib.MF_DENSE_BACKEND[_BACKEND])
+        if out is not None:
+            return out
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     _check("dense_attention", q, k, v, bias, buckets, key_mask, scale)
     num_keys = _counts("dense_attention", "num_keys", num_keys, q.shape[0], q.device)
@@ -374,6 +384,11 @@ def dense_attention_packed(qkv: torch.Tensor, heads: int, num_tokens: Optional[t
                            scale: Optional[float] = None) -> torch.Tensor:  # fmt: skip
     """:func:`dense_attention` of tokens on themselves on the packed projection of an attention layer: ``qkv`` (B, N, 3*H*D), result (B, N, H*D) as the output
     projection takes it, the gradient in ``qkv``'s shape."""
+    native = _lib.native()
+    if native is not None and heads >= 1:
+        out = native.dense_attention(qkv, None, None, bias, buckets, num_tokens, num_tokens, key_mask, int(heads), bool(causal), scale, _lib.MF_DENSE_BACKEND[_BACKEND])
+        if out is not None:
+            return out
     if qkv.ndim != 3 or heads < 1 or qkv.shape[2] % (3 * heads) or qkv.shape[2] == 0:
         raise ValueError(f"dense_attention_packed: qkv (B, N, 3*H*D) with H = {heads} expected, got {tuple(qkv.shape)}")
     q, k, v = _split(qkv.detach() if qkv.is_contiguous() else qkv.detach().contiguous(), heads)
