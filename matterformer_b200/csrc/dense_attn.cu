@@ -33,55 +33,76 @@ constexpr int kMaxEdges = kMaxBuckets - 1, kCells = 512;
 struct Edges {
   double square[kMaxEdges + 1];  // of the edges, then infinity
   float low[kMaxEdges + 1];      // the same in fp32
-  uint8_t first[kCells];         // edges at or below the start of a cell of distances
+  alignas(4) uint8_t first[kCells];  // edges at or below the start of a cell of distances
   float cells_per_unit;
   int n;
 };
 
-// A warp takes 128 columns, four to a lane, whose coordinates stay in registers, and walks over kBucketRows rows.  The squared distance is formed in
-// fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares) and its bucket found from a table of cells of the distance; a pair within that
-// error of an edge, or whose square leaves fp32's range, is decided in fp64, where the differences of fp32 coordinates are exact but for far apart exponents.  All pairs in fp64
-// against all edges took 463 us for two cells of 4096 atoms and 63 edges.
-constexpr int kBucketRows = 16, kBucketWarps = 8;
-__global__ void __launch_bounds__(kBucketWarps * 32) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int N, const __grid_constant__ Edges edges,
-                                                                             uint8_t* out, long long batch_stride, long long row, int words) {
-  __shared__ float low[kMaxEdges + 2];  // minus infinity first
-  __shared__ uint8_t first[kCells];
+// A thread takes four columns, whose coordinates stay in registers, and walks over rows: `lanes` threads (a power of two up to 32) lie along a row, the rest
+// of the block along the rows.  The squared distance is formed in
+// fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares) and its bucket found from a table of cells of the distance, of which few hold more than
+// one edge; a pair within that error of an edge, or whose square leaves fp32's range, is decided in fp64, where the differences of fp32 coordinates are exact but for
+// far apart exponents.  All pairs in fp64 against all edges took 463 us for two cells of 4096 atoms and 63 edges.
+constexpr int kBucketThreads = 256, kBucketSteps = 16;
+__global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int N, const __grid_constant__ Edges edges,
+                                                                          uint8_t* out, long long batch_stride, long long row, int words, int lanes, int column_tiles,
+                                                                          int row_tiles) {
+  __shared__ float2 around[kMaxEdges + 1];  // the squared edges below and above a bucket
+  __shared__ uint32_t first_words[kCells / 4];
+  const uint8_t* first = reinterpret_cast<const uint8_t*>(first_words);
   launch_dependents();
+  for (int i = threadIdx.x; i < kCells / 4; i += kBucketThreads) first_words[i] = reinterpret_cast<const uint32_t*>(edges.first)[i];
+  for (int i = threadIdx.x; i <= edges.n; i += kBucketThreads) around[i] = make_float2(i ? edges.low[i - 1] : -INFINITY, edges.low[i]);
   wait_for_previous();
-  for (int i = threadIdx.x; i < kCells; i += kBucketWarps * 32) first[i] = edges.first[i];
-  for (int i = threadIdx.x; i <= edges.n + 1; i += kBucketWarps * 32) low[i] = i == 0 ? -INFINITY : edges.low[i - 1];
   __syncthreads();
-  const int lane = threadIdx.x & 31, column_tiles = (N + 127) / 128, row_tiles = (N + kBucketRows * kBucketWarps - 1) / (kBucketRows * kBucketWarps);
   const int ct = blockIdx.x % column_tiles, rt = blockIdx.x / column_tiles % row_tiles, b = blockIdx.x / column_tiles / row_tiles;
   const int n = num_atoms ? min(num_atoms[b], N) : N;
-  const int j0 = ct * 128 + lane * 4, i0 = (rt * kBucketWarps + (threadIdx.x >> 5)) * kBucketRows;
+  const int at_once = kBucketThreads / lanes;
+  const int j0 = (ct * lanes + (threadIdx.x & (lanes - 1))) * 4, i0 = rt * at_once * kBucketSteps + threadIdx.x / lanes;
   const float* x = coords + (long long)b * N * 3;
   float y[4][3];
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int a = 0; a < 3; ++a) y[c][a] = j0 + c < n ? x[(j0 + c) * 3ll + a] : 0.f;
-  for (int i = i0; i < min(i0 + kBucketRows, N); ++i) {
+  const int last = min(i0 + at_once * (kBucketSteps - 1), N - 1);
+  for (int i = i0; i <= last; i += at_once) {
     uint32_t word = 0;
     if (i < n) {
       const float xi[3] = {x[i * 3ll], x[i * 3ll + 1], x[i * 3ll + 2]};
+      int k[4];
+      bool sure = true;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float dx = xi[0] - y[c][0], dy = xi[1] - y[c][1], dz = xi[2] - y[c][2];
         const float d2 = fmaf(dz, dz, fmaf(dy, dy, dx * dx));
         float root;
         asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(d2));
-        int k = first[(int)fminf(root * edges.cells_per_unit, (float)(kCells - 1))];
-        while (d2 >= low[k + 1] && k < edges.n) ++k;
+        k[c] = first[(int)fminf(root * edges.cells_per_unit, (float)(kCells - 1))];
+        k[c] += d2 >= around[k[c]].y && k[c] < edges.n;
+        const float2 e = around[k[c]];
         const float margin = d2 * 5e-7f;
-        if (!(d2 > 1e-30f && d2 < 1e30f) || d2 - low[k] <= margin || low[k + 1] - d2 <= margin) {
+        sure = sure && d2 > 1e-30f && d2 < 1e30f && d2 - e.x > margin && e.y - d2 > margin;
+      }
+      if (!sure) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
           const double ex = (double)xi[0] - y[c][0], ey = (double)xi[1] - y[c][1], ez = (double)xi[2] - y[c][2];
           const double e2 = __dadd_rn(__dadd_rn(__dmul_rn(ex, ex), __dmul_rn(ey, ey)), __dmul_rn(ez, ez));
-          for (k = 0; k < edges.n && e2 >= edges.square[k]; ++k) {}
+          int lo = 0, hi = edges.n;  // edges below lo are at or below the distance, those from hi on above it
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (e2 >= edges.square[mid]) lo = mid + 1;
+            else hi = mid;
+          }
+          if (c == 0) k[0] = lo;
+          else if (c == 1) k[1] = lo;
+          else if (c == 2) k[2] = lo;
+          else k[3] = lo;
         }
-        word |= (j0 + c < n ? (uint32_t)k : 0u) << (8 * c);
       }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) word |= (j0 + c < n ? (uint32_t)k[c] : 0u) << (8 * c);
     }
     uint8_t* dst = out + b * batch_stride + i * row + j0;
     if (words) {  // rows that hold whole words, behind the last atom too
@@ -240,7 +261,10 @@ int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t b
                         int64_t batch_stride, int64_t row, void* stream) {
   using namespace mf;
   const char* name = "mf_distance_buckets";
-  const long long tiles = ((tokens + 127ll) / 128) * ((tokens + kBucketRows * kBucketWarps - 1ll) / (kBucketRows * kBucketWarps)) * batch;
+  int lanes = 32;
+  while (lanes > 1 && lanes / 2 * 4 >= tokens) lanes /= 2;
+  const int at_once = kBucketThreads / lanes * kBucketSteps, column_tiles = (int)((tokens + lanes * 4ll - 1) / (lanes * 4)), row_tiles = (int)((tokens + at_once - 1ll) / at_once);
+  const long long tiles = (long long)column_tiles * row_tiles * batch;
   MF_CHECK_ARG(batch >= 0 && tokens >= 0 && tokens <= 1 << 20 && tiles < (1ll << 31), "%s: sizes out of range: %d molecules of %d atoms", name, batch, tokens);
   MF_CHECK_ARG(num_edges >= 0 && num_edges <= kMaxEdges && (num_edges == 0 || edges), "%s: at most %d edges, got %d", name, kMaxEdges, num_edges);
   Edges e{};
@@ -260,8 +284,8 @@ int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t b
   if (batch == 0 || tokens == 0) return MF_OK;
   MF_CHECK_ARG(coords && buckets && row >= tokens && batch_stride >= (int64_t)(tokens - 1) * row + tokens, "%s: rows of the buckets must hold %d entries", name, tokens);
   const int words = row % 4 == 0 && batch_stride % 4 == 0 && batch_stride >= tokens * row && reinterpret_cast<uintptr_t>(buckets) % 4 == 0;
-  const cudaError_t err = launch_dependent(distance_buckets_kernel, dim3((unsigned)tiles), dim3(kBucketWarps * 32), 0, static_cast<cudaStream_t>(stream), coords, num_atoms,
-                                           tokens, e, buckets, batch_stride, row, words);
+  const cudaError_t err = launch_dependent(distance_buckets_kernel, dim3((unsigned)tiles), dim3(kBucketThreads), 0, static_cast<cudaStream_t>(stream), coords, num_atoms,
+                                           tokens, e, buckets, batch_stride, row, words, lanes, column_tiles, row_tiles);
   return err == cudaSuccess ? MF_OK : cuda_error(err, name);
 }
 
