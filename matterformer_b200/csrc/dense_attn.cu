@@ -1,5 +1,7 @@
 // Entry points of dense attention with a learned bias by buckets, the sum of the table's gradient, and the buckets of a molecule's distances.
-#include "dense_attn.cuh"
+#include "dense_attn_sm100.cuh"
+
+#include <string.h>
 
 namespace mf {
 namespace {
@@ -29,30 +31,33 @@ __global__ void __launch_bounds__(128) bias_sum_kernel(const float* part, int B,
   }
 }
 
-constexpr int kMaxEdges = kMaxBuckets - 1, kCells = 512;
+constexpr int kMaxEdges = kMaxBuckets - 1;
+// Cells of squared distances: 64 to an octave (exponent and six bits of the mantissa), 16 octaves up to the last edge.
+constexpr int kCells = 1024, kCellShift = 17;
 struct Edges {
-  double square[kMaxEdges + 1];  // of the edges, then infinity
-  float low[kMaxEdges + 1];      // the same in fp32
-  alignas(4) uint8_t first[kCells];  // edges at or below the start of a cell of distances
-  float cells_per_unit;
-  int n;
+  double square[kMaxEdges];  // of the edges
+  float low[kMaxEdges];      // the same in fp32
+  alignas(4) uint8_t first[kCells];  // edges below a cell
+  int base, n;
 };
+constexpr float kDistanceError = 5e-7f;  // of a squared distance in fp32, in relation to it; 6 * 2^-24 and an edge's rounding
 
 // A thread takes four columns, whose coordinates stay in registers, and walks over rows: `lanes` threads (a power of two up to 32) lie along a row, the rest
 // of the block along the rows.  The squared distance is formed in
-// fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares) and its bucket found from a table of cells of the distance, of which few hold more than
-// one edge; a pair within that error of an edge, or whose square leaves fp32's range, is decided in fp64, where the differences of fp32 coordinates are exact but for
+// fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares) and its bucket found from a table of cells, of which few hold more than one edge;
+// a pair within that error of an edge, or whose square leaves fp32's range, is decided in fp64, where the differences of fp32 coordinates are exact but for
 // far apart exponents.  All pairs in fp64 against all edges took 463 us for two cells of 4096 atoms and 63 edges.
-constexpr int kBucketThreads = 256, kBucketSteps = 16;
+constexpr int kBucketThreads = 256, kBucketSteps = 8;
 __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int N, const __grid_constant__ Edges edges,
                                                                           uint8_t* out, long long batch_stride, long long row, int words, int lanes, int column_tiles,
                                                                           int row_tiles) {
-  __shared__ float2 around[kMaxEdges + 1];  // the squared edges below and above a bucket
+  __shared__ float2 around[kMaxEdges + 1];  // the squared edges below and above a bucket, a margin within it
   __shared__ uint32_t first_words[kCells / 4];
   const uint8_t* first = reinterpret_cast<const uint8_t*>(first_words);
   launch_dependents();
   for (int i = threadIdx.x; i < kCells / 4; i += kBucketThreads) first_words[i] = reinterpret_cast<const uint32_t*>(edges.first)[i];
-  for (int i = threadIdx.x; i <= edges.n; i += kBucketThreads) around[i] = make_float2(i ? edges.low[i - 1] : -INFINITY, edges.low[i]);
+  for (int i = threadIdx.x; i <= edges.n; i += kBucketThreads)
+    around[i] = make_float2(fmaxf(1e-30f, i ? edges.low[i - 1] * (1.f + kDistanceError) : 0.f), i < edges.n ? fminf(1e30f, edges.low[i] * (1.f - kDistanceError)) : 1e30f);
   wait_for_previous();
   __syncthreads();
   const int ct = blockIdx.x % column_tiles, rt = blockIdx.x / column_tiles % row_tiles, b = blockIdx.x / column_tiles / row_tiles;
@@ -76,13 +81,11 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
       for (int c = 0; c < 4; ++c) {
         const float dx = xi[0] - y[c][0], dy = xi[1] - y[c][1], dz = xi[2] - y[c][2];
         const float d2 = fmaf(dz, dz, fmaf(dy, dy, dx * dx));
-        float root;
-        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(d2));
-        k[c] = first[(int)fminf(root * edges.cells_per_unit, (float)(kCells - 1))];
-        k[c] += d2 >= around[k[c]].y && k[c] < edges.n;
+        const int cell = max(0, min(kCells - 1, (__float_as_int(d2) >> kCellShift) - edges.base));
+        k[c] = first[cell];
+        k[c] = min(k[c] + (d2 >= around[k[c]].y), edges.n);
         const float2 e = around[k[c]];
-        const float margin = d2 * 5e-7f;
-        sure = sure && d2 > 1e-30f && d2 < 1e30f && d2 - e.x > margin && e.y - d2 > margin;
+        sure = sure && d2 > e.x && d2 < e.y;
       }
       if (!sure) {
 #pragma unroll 1
@@ -167,10 +170,12 @@ DenseParams params_of(const MfDenseAttnArgs& a) {
   return p;
 }
 
-enum Family { kMma, kSmall, kSplit };
+enum Family { kMma, kSmall, kSplit, kTensor };
 Family fwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
-  if (a.backend != MF_DENSE_BACKEND_AUTO) return kMma;
-  return dense_attn_small_applies(p, false) ? kSmall : dense_attn_split_applies(p) ? kSplit : kMma;
+  if (a.backend == MF_DENSE_BACKEND_MMA) return kMma;
+  const bool takes = dense_tc_takes(p, a.head_dim, a.bucket_kind);
+  if (a.backend == MF_DENSE_BACKEND_TCGEN05) return takes ? kTensor : kMma;
+  return dense_attn_small_applies(p, false) ? kSmall : dense_attn_split_applies(p) ? kSplit : takes && p.M > 128 && p.N > 256 ? kTensor : kMma;
 }
 Family bwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
   return a.backend == MF_DENSE_BACKEND_AUTO && dense_attn_small_applies(p, true) ? kSmall : kMma;
@@ -223,6 +228,7 @@ int mf_dense_attn_fwd(const MfDenseAttnArgs* a, void* stream_) {
                    a->workspace_bytes);
       return dense_attn_split(p, a->dtype, a->head_dim, a->bucket_kind, a->workspace, stream);
     }
+    case kTensor: return dense_attn_sm100_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
     default: return dense_attn_mma_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
   }
 }
@@ -273,12 +279,15 @@ int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t b
     e.square[i] = edges[i] * edges[i];
     e.low[i] = (float)e.square[i];
   }
-  e.n = num_edges, e.square[num_edges] = INFINITY, e.low[num_edges] = INFINITY;
-  const double last = num_edges ? edges[num_edges - 1] : 0.0;
-  e.cells_per_unit = last > 1e-30 && last < 1e30 ? (float)((kCells - 1) / last) : 0.f;
-  for (int c = 0, k = 0; c < kCells; ++c) {  // a cell's start a little lower than it is, for the rounding of the distance
-    const double start = e.cells_per_unit > 0.f ? c / (double)e.cells_per_unit * (1.0 - 1e-5) : 0.0;
-    while (k < num_edges && edges[k] < start) ++k;
+  e.n = num_edges;
+  auto bits = [](float f) { int i; memcpy(&i, &f, 4); return i; };
+  auto value = [](int i) { float f; memcpy(&f, &i, 4); return f; };
+  const float last = num_edges ? e.low[num_edges - 1] : 0.f;
+  e.base = (bits(last) >> kCellShift) - (kCells - 2);
+  for (int c = 0, k = 0; c < kCells; ++c) {  // what the table says is where the search begins: too low costs time alone
+    const long long start = (long long)(c + e.base) * (1 << kCellShift);
+    const int at = start > 0x7f000000ll ? 0x7f000000 : start > 0 ? (int)start : 0;
+    while (c > 0 && k < num_edges && at > 0 && e.low[k] < value(at) * (1.f - 2 * kDistanceError)) ++k;
     e.first[c] = (uint8_t)k;
   }
   if (batch == 0 || tokens == 0) return MF_OK;

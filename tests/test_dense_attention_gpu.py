@@ -120,6 +120,14 @@ def run_both(q, k, v, grad, num_keys=None, num_queries=None, key_mask=None, caus
     return got
 
 
+@pytest.fixture(autouse=True, params=["auto", "mma", "tcgen05"])
+def backend(request):
+    """Every test on every family of kernels."""
+    prev = mfb.set_dense_backend(request.param)
+    yield
+    mfb.set_dense_backend(prev)
+
+
 def counts(g, B, most):
     n = torch.randint(0, most + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
     n[0] = most
