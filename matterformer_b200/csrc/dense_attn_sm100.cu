@@ -103,8 +103,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
     if (!bad) bad = !mbar_wait_for(bar, phase & 1, tc.waits.limit);
   };
 
-  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegAux));
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegOwner));
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegAux));
   if (warp == 9) {
     // ------------------------------------------------------------------ copies: K of tile j in slot 2 j, V in slot 2 j + 1 (modulo the ring)
     if (lane == 0) {
@@ -194,8 +194,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
         if (lane == 0) mbar_arrive(&bar_clean[slot]);
       }
     }
-  } else if (warp < 8) {
+  }
+  } else {
     // ------------------------------------------------------------------ row owners
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegOwner));
     const int x = warp >> 2, r = tid & 127;
     const int my_head = x ? head[1] : head[0], my_row0 = x ? row0[1] : row0[0], my_tiles = x ? tiles[1] : tiles[0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
