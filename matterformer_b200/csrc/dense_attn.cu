@@ -178,20 +178,22 @@ Family fwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
   return dense_attn_small_applies(p, false) ? kSmall : dense_attn_split_applies(p) ? kSplit : takes && p.M > 128 && p.N > 256 ? kTensor : kMma;
 }
 Family bwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
-  return a.backend == MF_DENSE_BACKEND_AUTO && dense_attn_small_applies(p, true) ? kSmall : kMma;
+  if (a.backend == MF_DENSE_BACKEND_MMA) return kMma;
+  const bool takes = dense_tc_bwd_takes(p, a.head_dim, a.bucket_kind, a.bias && a.dbias);
+  if (a.backend == MF_DENSE_BACKEND_TCGEN05) return takes ? kTensor : kMma;
+  return dense_attn_small_applies(p, true) ? kSmall : takes && p.M > 128 && p.N > 256 ? kTensor : kMma;
 }
 
+// delta, then partial sums of the table's gradient for each head: whichever of the tiled families runs, the smaller tiles' number of them fits.
 struct BwdSpace {
   size_t part, total;
-  int entries, tiles;  // partial sums of the table's gradient for each head
 };
 BwdSpace bwd_space(const MfDenseAttnArgs& a, const DenseParams& p) {
   BwdSpace s{};
   const bool small = bwd_family(a, p) == kSmall;
-  s.entries = small ? dense_attn_small_slots(p, a.head_dim) : a.batch;
-  s.tiles = small ? 1 : dense_attn_mma_tiles(a.queries);
   s.part = small ? 0 : align_up((size_t)a.batch * a.heads * a.queries * sizeof(float), 256);
-  s.total = s.part + (a.bias && a.dbias ? align_up((size_t)s.entries * a.heads * s.tiles * a.num_buckets * sizeof(float), 256) : 0);
+  const size_t sums = small ? dense_attn_small_slots(p, a.head_dim) : (size_t)a.batch * dense_attn_mma_tiles(a.queries);
+  s.total = s.part + (a.bias && a.dbias ? align_up(sums * a.heads * a.num_buckets * sizeof(float), 256) : 0);
   return s;
 }
 
@@ -244,6 +246,7 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
   const BwdSpace space = a->batch ? bwd_space(*a, p) : BwdSpace{};
   MF_CHECK_ARG(space.total == 0 || (a->workspace && a->workspace_bytes >= space.total && aligned16(a->workspace)), "%s: %zu bytes of workspace needed, got %zu", name,
                space.total, a->workspace_bytes);
+  int entries = a->batch, tiles = dense_attn_mma_tiles(a->queries);  // of partial sums for each head
   if (a->batch > 0) {
     MF_CHECK_ARG(a->queries == 0 || (a->grad_out && a->lse), "%s: grad_out and lse must not be NULL", name);
     if ((a->queries > 0 && MF_OK != (rc = check_rows(name, "grad_out", a->grad_out, a->grad_out_rows))) ||
@@ -253,12 +256,24 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
     char* ws = static_cast<char*>(a->workspace);
     p.delta = reinterpret_cast<float*>(ws);
     if (table) p.dbias_part = reinterpret_cast<float*>(ws + space.part);
-    rc = bwd_family(*a, p) == kSmall ? dense_attn_small(p, a->dtype, a->head_dim, a->bucket_kind, true, stream)
-                                     : dense_attn_mma_bwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
+    DenseTcParams tc{p, {}, {}, {}, {}, {}};
+    Family family = bwd_family(*a, p);
+    if (family == kTensor && !dense_tc_maps(tc, a->dtype, a->head_dim, true)) family = kMma;
+    switch (family) {
+      case kSmall:
+        entries = dense_attn_small_slots(p, a->head_dim), tiles = 1;
+        rc = dense_attn_small(p, a->dtype, a->head_dim, a->bucket_kind, true, stream);
+        break;
+      case kTensor:
+        tiles = (a->queries + kTcRows - 1) / kTcRows;
+        rc = dense_attn_sm100_bwd(tc, a->dtype, a->head_dim, a->bucket_kind, stream);
+        break;
+      default: rc = dense_attn_mma_bwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
+    }
     if (rc != MF_OK) return rc;
   }
   if (!table) return MF_OK;
-  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * a->num_buckets), dim3(128), 0, stream, p.dbias_part, space.entries, a->heads, space.tiles,
+  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * a->num_buckets), dim3(128), 0, stream, p.dbias_part, entries, a->heads, tiles,
                                            a->num_buckets, a->dbias, a->bias_dtype);
   return err == cudaSuccess ? MF_OK : cuda_error(err, "dense attention table gradient");
 }

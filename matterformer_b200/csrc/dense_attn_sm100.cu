@@ -373,14 +373,14 @@ int pick(const DenseTcParams& tc, int head_dim, int kind, cudaStream_t stream) {
   return head_dim == 64 ? by_kind(std::integral_constant<int, 64>{}) : by_kind(std::integral_constant<int, 128>{});
 }
 
-bool rows_map(CUtensorMap* map, const void* base, const DenseRows& rows, int dtype, int head_dim, int tokens, int heads, int batch) {
+bool rows_map(CUtensorMap* map, const void* base, const DenseRows& rows, int dtype, int head_dim, int tokens, int heads, int batch, int box_rows) {
   const long long dims[4] = {head_dim, tokens, heads, batch};
   long long strides[3] = {rows.token * 2, rows.head * 2, rows.batch * 2};
   for (int i = 0; i < 3; ++i)
     if (dims[i + 1] == 1) strides[i] = head_dim * 2;  // whatever it is, nothing goes by it
   for (int i = 0; i < 3; ++i)
     if (strides[i] <= 0) return false;  // (an expanded dimension)
-  return make_tensor_map(map, base, dtype, 4, dims, strides, 64, kTcRows);
+  return make_tensor_map(map, base, dtype, 4, dims, strides, 64, box_rows);
 }
 
 }  // namespace
@@ -395,9 +395,10 @@ int dense_attn_take_fwd_status(int word, int32_t* host_status, cudaStream_t stre
 
 bool dense_tc_maps(DenseTcParams& tc, int dtype, int head_dim, bool backward) {
   const DenseParams& p = tc.p;
-  return rows_map(&tc.q, p.q, p.q_rows, dtype, head_dim, p.M, p.H, p.B) && rows_map(&tc.k, p.k, p.k_rows, dtype, head_dim, p.N, p.K, p.B) &&
-         rows_map(&tc.v, p.v, p.v_rows, dtype, head_dim, p.N, p.K, p.B) &&
-         (!backward || rows_map(&tc.grad_out, p.grad_out, p.go_rows, dtype, head_dim, p.M, p.H, p.B));
+  const int box = backward ? 64 : kTcRows;
+  return rows_map(&tc.q, p.q, p.q_rows, dtype, head_dim, p.M, p.H, p.B, box) && rows_map(&tc.k, p.k, p.k_rows, dtype, head_dim, p.N, p.K, p.B, box) &&
+         rows_map(&tc.v, p.v, p.v_rows, dtype, head_dim, p.N, p.K, p.B, box) &&
+         (!backward || rows_map(&tc.grad_out, p.grad_out, p.go_rows, dtype, head_dim, p.M, p.H, p.B, box));
 }
 
 bool dense_tc_takes(const DenseParams& p, int head_dim, int kind) {

@@ -11,7 +11,7 @@ constexpr int kTcRows = 128;  // rows of a tile, queries and keys
 
 struct DenseTcParams {
   DenseParams p;
-  CUtensorMap q, k, v, grad_out;  // {head_dim, tokens, heads, batch}, boxes of 64 channels x 128 rows, 128-byte swizzle
+  CUtensorMap q, k, v, grad_out;  // {head_dim, tokens, heads, batch}, boxes of 64 channels x 128 rows (forward) or 64 (backward), 128-byte swizzle
   BoundedWaits waits;
 };
 
@@ -22,7 +22,7 @@ __host__ __device__ constexpr uint32_t make_idesc_16(int m, int n, bool a_mn_maj
   return std::is_same<T, __nv_bfloat16>::value ? d : d & ~((1u << 7) | (1u << 10));
 }
 
-// A box of 64 channels (from `channel` on, a multiple of 64) x 128 rows.
+// A box of 64 channels, from `channel` on (a multiple of 64).
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int channel, int row, int head, int batch, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
@@ -62,6 +62,7 @@ bool dense_tc_takes(const DenseParams& p, int head_dim, int bucket_kind);
 int dense_attn_take_fwd_status(int word, int32_t* host_status, cudaStream_t stream);
 int dense_attn_take_bwd_status(int word, int32_t* host_status, cudaStream_t stream);
 int dense_attn_sm100_fwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream, BoundedWaits waits = {});
-int dense_attn_sm100_bwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream, BoundedWaits waits = {});
+bool dense_tc_bwd_takes(const DenseParams& p, int head_dim, int bucket_kind, bool table_grad);
+int dense_attn_sm100_bwd(const DenseTcParams& tc, int dtype, int head_dim, int bucket_kind, cudaStream_t stream);
 
 }  // namespace mf

@@ -1,0 +1,519 @@
+// Dense attention with a learned bias by the offset on tcgen05, backward: head size 64 and 128, bf16 and fp16.  The probabilities are formed again.
+//
+// Two passes of one skeleton, a CTA owns tiles of 128 rows and walks over its partners in tiles of 64:
+//   DQ  : owners = queries, partners = keys     S = Q K^T, dP = dO V^T       -> dS        -> dQ += dS K
+//   DKV : owners = keys,    partners = queries  S^T = K Q^T, dP^T = V dO^T   -> P^T, dS^T -> dV += P^T dO, dK += dS^T Q
+// Seven products instead of the five of a single pass, but every sum has one owner and a fixed order, and nothing is added up in memory.
+// A thread owns a row; P and dS are packed to 16 bits over the columns that S and dP had and are the A operands of the second products, whose sums
+// stay in tensor memory over the whole walk.  Two buffers for S and dP, each with a group of four warps: while one group works the tensor cores
+// fill the other's buffer.  At head size 64 a CTA owns two tiles that share the partners they read, a buffer each; at 128, where the sums of two
+// tiles do not fit tensor memory, one tile, and the groups take its steps in turn.
+//
+// The table's gradient (DQ): steps whose offsets all fall into one bucket add up in a register; in the others every thread adds to a column of sums of
+// its own in shared memory.  dS = P (dP - delta) with delta from rounded outputs; the row sums of dS, which are zero but for the error in
+// delta, correct what far buckets got: there thousands of P share one error, which would otherwise be the largest of that sum.
+//
+// Roles as in the forward kernel; warp 10 also brings the queries' log-sum-exp and delta for DKV.
+#include "dense_attn_sm100.cuh"
+
+namespace mf {
+namespace {
+
+__device__ int32_t g_dense_status[2];  // last expired wait: of calls, of the self-test
+__device__ int32_t g_taken_status;
+__global__ void take_status_kernel(int word) { g_taken_status = atomicExch(&g_dense_status[word], 0); }
+
+constexpr int kBwdThreads = 384, kPart = 64, kSpan = kTcRows + kPart - 1;
+constexpr int kRegAux = 56, kRegOwner = 224;
+static_assert(8 * kRegOwner + 4 * kRegAux <= 12 * 168, "register hand-over exceeds the CTA's pool");
+
+template <int D>
+struct BwdShape {
+  static constexpr int kOwn = D == 64 ? 2 : 1;  // owner tiles
+  static constexpr int kChunks = D / 64, kTile = kChunks * kTcRows * 128, kPartTile = kChunks * kPart * 128;
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kOffA = 0, kOffB = kOwn * kTile, kOffRing = 2 * kOwn * kTile, kSmem = kOffRing + kStages * 2 * kPartTile;
+  static constexpr int kMostBuckets = D == 64 ? 64 : 32;  // whose sums fit beside that
+};
+
+template <typename T, int D, bool DKV, bool TABLE>
+__global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const __grid_constant__ DenseTcParams tc) {
+  using Sh = BwdShape<D>;
+  constexpr int OWN = Sh::kOwn, S = Sh::kStages;
+  const DenseParams& p = tc.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem);  // [num_buckets][256 row owners]
+  __shared__ uint64_t bar_own, bar_full[S], bar_free[S], bar_clean[S], bar_s[2], bar_p[2], bar_o, bar_drain;
+  __shared__ uint32_t tmem_base;
+  __shared__ float offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
+  __shared__ uint8_t offset_buckets[TABLE && !DKV ? 2 : 1][2][TABLE && !DKV ? 256 : 1];
+  __shared__ __align__(16) float2 stats[DKV ? S : 1][DKV ? kPart : 1];  // -lse and delta of the partners
+  __shared__ float errors[TABLE && !DKV && OWN == 1 ? 2 : 1][TABLE && !DKV && OWN == 1 ? 128 : 1];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // ---- which rows
+  const int group = p.H / p.K;
+  const bool by_head = OWN == 2 && !DKV && group % 2 == 0;  // two query heads of a group, otherwise neighbouring tiles
+  const int heads = DKV ? p.K : p.H, units = p.B * (by_head ? heads / 2 : heads), row_blocks = gridDim.x / units;
+  const int unit = p.causal ? blockIdx.x % units : blockIdx.x / row_blocks;
+  const int rb = !p.causal ? blockIdx.x % row_blocks : DKV ? blockIdx.x / units : row_blocks - 1 - (int)(blockIdx.x / units);  // the longest walks first
+  const int b = unit / (units / p.B), hu = unit % (units / p.B);
+  const DenseLengths len = dense_lengths(p, b);
+  const int own_rows = DKV ? len.nk : len.nq, own_all = DKV ? p.N : p.M;
+  int head[OWN], row0[OWN], first[OWN], last[OWN];  // partner steps [first, last) of a head
+#pragma unroll
+  for (int x = 0; x < OWN; ++x) {
+    head[x] = by_head ? 2 * hu + x : hu;
+    row0[x] = by_head || OWN == 1 ? rb * kTcRows : (2 * rb + x) * kTcRows;
+    first[x] = 0, last[x] = 0;
+    if (row0[x] < own_rows) {
+      if (DKV) first[x] = dense_first(p, len, row0[x]) / kPart, last[x] = (len.nq + kPart - 1) / kPart;
+      else last[x] = (dense_limit(p, len, min(row0[x] + kTcRows, len.nq) - 1) + kPart - 1) / kPart;
+      if (last[x] <= first[x]) first[x] = last[x] = 0;
+    }
+  }
+  int from = first[0], until = last[0];
+  if (OWN == 2) {
+    if (last[OWN - 1] > first[OWN - 1]) {
+      from = last[0] > first[0] ? min(from, first[OWN - 1]) : first[OWN - 1];
+      until = max(until, last[OWN - 1]);
+    }
+  }
+  const int per_head = until - from, steps = DKV ? per_head * group : per_head;
+  auto seen_by = [&](int x, int t) {  // whether tile x works on step t
+    const int s = from + (DKV ? t % per_head : t);
+    return s >= (x ? first[OWN - 1] : first[0]) && s < (x ? last[OWN - 1] : last[0]);
+  };
+  auto partner_row = [&](int t) { return (from + (DKV ? t % per_head : t)) * kPart; };
+  const int kh = DKV ? hu : head[0] / group;
+  auto partner_head = [&](int t) { return DKV ? kh * group + t / per_head : kh; };
+  const uint8_t* mask = p.key_mask ? p.key_mask + b * p.key_mask_batch : nullptr;
+  const int part_rows = DKV ? len.nq : len.nk, part_all = DKV ? p.M : p.N;
+  const bool cleaning = DKV || mask || part_rows < min(part_all, until * kPart);
+
+  if (steps == 0) {
+    for (int i = tid; i < OWN * kTcRows; i += kBwdThreads) {
+      const int x = i / kTcRows, row = (x ? row0[OWN - 1] : row0[0]) + i % kTcRows, h = x ? head[OWN - 1] : head[0];
+      if (row >= own_all) continue;
+      auto clear = [&](void* base, const DenseRows& rows) {
+        if (!base) return;
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(base) + rows.at(b, h, row));
+        for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+      };
+      if (DKV) {
+        clear(p.dk, p.dk_rows);
+        clear(p.dv, p.dv_rows);
+      } else {
+        clear(p.dq, p.dq_rows);
+        p.delta[((long long)b * p.H + h) * p.M + row] = 0.f;
+      }
+    }
+    if (TABLE && !DKV && p.dbias_part) {
+      const int tiles = (p.M + kTcRows - 1) / kTcRows;
+      for (int x = 0; x < OWN; ++x) {
+        const int r0 = x ? row0[OWN - 1] : row0[0], h = x ? head[OWN - 1] : head[0];
+        if (r0 < p.M)
+          for (int i = tid; i < p.num_buckets; i += kBwdThreads) p.dbias_part[(((long long)b * p.H + h) * tiles + r0 / kTcRows) * p.num_buckets + i] = 0.f;
+      }
+    }
+    return;
+  }
+
+  if (tid == 0) {
+    auto init = [&](uint64_t* bar, int count, int kind) { mbar_init(bar, count + (tc.waits.withheld == kind)); };
+    init(&bar_own, 1, 0);
+    for (int i = 0; i < S; ++i) init(&bar_full[i], 1, 0), init(&bar_free[i], 1, 1), init(&bar_clean[i], 1, 4);
+    for (int x = 0; x < 2; ++x) init(&bar_s[x], 1, 2), init(&bar_p[x], 4, 3);
+    init(&bar_o, 1, 2);
+    mbar_init(&bar_drain, 1);
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (TABLE && !DKV && p.dbias_part)
+    for (int i = tid; i < p.num_buckets * 256; i += kBwdThreads) sums[i] = 0.f;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  bool bad = false;
+  auto wait_on = [&](uint64_t* bar, uint32_t phase) {
+    if (!bad) bad = !mbar_wait_for(bar, phase & 1, tc.waits.limit);
+  };
+  // columns: S and dP of buffer y at 128 y and 128 y + 64; the sums from 256 on
+  auto col_sum = [&](int x, int which) { return 256u + (DKV ? 2 * D * x + D * which : D * x); };
+  const int jobs = OWN * steps;  // job n: tile n & 1 of step n / 2, or step n; buffer and group n & 1
+  auto step_of = [&](int n) { return OWN == 2 ? n >> 1 : n; };
+  auto valid = [&](int n) { return OWN == 1 || seen_by(n & 1, n >> 1); };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegAux));
+    if (warp == 9) {
+      // ---------------------------------------------------------------- copies
+      if (lane == 0) {
+        const CUtensorMap *own_a = DKV ? &tc.k : &tc.q, *own_b = DKV ? &tc.v : &tc.grad_out, *part_a = DKV ? &tc.q : &tc.k, *part_b = DKV ? &tc.grad_out : &tc.v;
+        tma_prefetch_map(own_a);
+        tma_prefetch_map(own_b);
+        tma_prefetch_map(part_a);
+        tma_prefetch_map(part_b);
+        int own = 0;
+        for (int x = 0; x < OWN; ++x) own += last[x] > first[x];
+        mbar_arrive_expect_tx(&bar_own, own * 2 * Sh::kTile);
+        for (int x = 0; x < OWN; ++x)
+          if (last[x] > first[x])
+            for (int c = 0; c < Sh::kChunks; ++c)
+              for (int half = 0; half < 2; ++half) {  // (boxes have 64 rows)
+                const uint32_t at = x * Sh::kTile + (c * kTcRows + half * 64) * 128;
+                tma_box(smem_u32(smem + Sh::kOffA) + at, own_a, c * 64, row0[x] + half * 64, head[x], b, &bar_own);
+                tma_box(smem_u32(smem + Sh::kOffB) + at, own_b, c * 64, row0[x] + half * 64, head[x], b, &bar_own);
+              }
+        int t = 0;
+        for (; t < steps; ++t) {
+          const int stage = t % S;
+          if (t >= S) wait_on(&bar_free[stage], t / S - 1);
+          if (bad) break;
+          mbar_arrive_expect_tx(&bar_full[stage], 2 * Sh::kPartTile);
+          const uint32_t at = smem_u32(smem + Sh::kOffRing) + stage * 2 * Sh::kPartTile;
+          for (int c = 0; c < Sh::kChunks; ++c) {
+            tma_box(at + c * kPart * 128, part_a, c * 64, partner_row(t), partner_head(t), b, &bar_full[stage]);
+            tma_box(at + Sh::kPartTile + c * kPart * 128, part_b, c * 64, partner_row(t), partner_head(t), b, &bar_full[stage]);
+          }
+        }
+        // whoever gave up, no copy may be in flight when the CTA ends
+        if (!mbar_wait(&bar_own, 0)) bad = true;
+        for (int i = max(0, t - S); i < t; ++i)
+          if (!mbar_wait(&bar_full[i % S], (i / S) & 1)) bad = true;
+      }
+    } else if (warp == 8) {
+      // ---------------------------------------------------------------- products
+      if (elect_one()) {
+        const uint32_t l_a = make_desc_lo(smem_u32(smem + Sh::kOffA), 0), l_b = make_desc_lo(smem_u32(smem + Sh::kOffB), 0);
+        const uint32_t l_ring = make_desc_lo(smem_u32(smem + Sh::kOffRing), 0), l_ring_mn = make_desc_lo(smem_u32(smem + Sh::kOffRing), kPart * 128);
+        constexpr uint32_t kTile = Sh::kTile >> 4, kPartTile = Sh::kPartTile >> 4, kChunk = (kTcRows * 128) >> 4, kPartChunk = (kPart * 128) >> 4;
+        constexpr uint32_t idesc_s = make_idesc_16<T>(kTcRows, kPart, false, false), idesc_o = make_idesc_16<T>(kTcRows, D, false, true);
+        auto logits = [&](int n) {
+          const int t = step_of(n), stage = t % S, x = OWN == 2 ? n & 1 : 0;
+          wait_on(cleaning ? &bar_clean[stage] : &bar_full[stage], t / S);
+          tc_fence_after_sync();
+          const uint32_t part = l_ring + stage * 2 * kPartTile, col = tmem + 128 * (n & 1);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            umma_ss_lo(col, l_a + x * kTile + (ks >> 2) * kChunk + (ks & 3) * 2, part + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            umma_ss_lo(col + 64, l_b + x * kTile + (ks >> 2) * kChunk + (ks & 3) * 2, part + kPartTile + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
+          umma_commit(&bar_s[n & 1]);
+        };
+        wait_on(&bar_own, 0);
+        int done[2] = {0, 0}, sum_started[2] = {0, 0};
+        for (int n = 0; n < min(2, jobs); ++n)
+          if (valid(n)) logits(n);
+#pragma unroll 1
+        for (int n0 = 0; n0 < jobs; n0 += 2) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int n = n0 + y, t = step_of(n), stage = t % S, x = OWN == 2 ? y : 0;
+            if (n >= jobs) break;
+            if (valid(n)) {
+              wait_on(&bar_p[y], done[y]++);
+              tc_fence_after_sync();
+              const uint32_t part = l_ring_mn + stage * 2 * kPartTile, col = tmem + 128 * y;
+#pragma unroll
+              for (int kg = 0; kg < kPart / 16; ++kg) {
+                if (DKV) umma_ts_lo(tmem + col_sum(x, 1), col + 8 * kg, part + kPartTile + 128 * kg, idesc_o, sum_started[x] || kg > 0);
+                umma_ts_lo(tmem + col_sum(x, 0), col + 64 + 8 * kg, part + 128 * kg, idesc_o, sum_started[x] || kg > 0);
+              }
+              sum_started[x] = 1;
+            }
+            if (OWN == 1 || y == 1) umma_commit(&bar_free[stage]);
+            if (n + 2 < jobs && valid(n + 2)) logits(n + 2);
+          }
+        }
+        umma_commit(&bar_o);
+        // nor a product when tensor memory is given back
+        umma_commit(&bar_drain);
+        if (!mbar_wait(&bar_drain, 0)) bad = true;
+      }
+    } else if (warp == 10) {
+      // ---------------------------------------------------------------- partners that are none become zeros; log-sum-exp and delta of queries
+      if (cleaning) {
+        for (int t = 0; t < steps; ++t) {
+          const int stage = t % S, at = partner_row(t);
+          wait_on(&bar_full[stage], t / S);
+          if (DKV) {
+            const long long stat = ((long long)b * p.H + partner_head(t)) * p.M;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = lane + 32 * e, i = at + c;
+              stats[stage][c] = i < len.nq ? make_float2(-p.lse[stat + i], p.delta[stat + i]) : make_float2(-INFINITY, 0.f);
+            }
+          }
+          const int rows = min(kPart, part_all - at);  // what lies behind the tensor is zeros already
+          if (!bad && ((!DKV && mask) || at + rows > part_rows)) {
+            for (int r = lane; r < rows; r += 32) {
+              if (at + r < part_rows && (DKV || !mask || mask[at + r])) continue;
+#pragma unroll 1
+              for (int i = 0; i < 2 * Sh::kChunks * 8; ++i)
+                *reinterpret_cast<uint4*>(smem + Sh::kOffRing + (stage * 2 * Sh::kChunks + i / 8) * kPart * 128 + r * 128 + (i % 8) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_smem_to_async_proxy();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_clean[stage]);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ row owners
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegOwner));
+    const int y = warp >> 2, x = OWN == 2 ? y : 0, r = tid & 127;  // group (and buffer), tile
+    const int my_head = x ? head[OWN - 1] : head[0], my_row0 = x ? row0[OWN - 1] : row0[0];
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, col = tmem + lanes + 128 * y;
+    const int row = my_row0 + r;
+    const bool row_ok = row < own_rows;
+    const float sc2 = p.scale * kDenseLog2e;
+    float lse = 0.f, delta = 0.f;
+    // visible partners of this row: [lo, hi) at DKV and DQ; a row that is none may see what it wants
+    int lo = INT32_MIN, hi = INT32_MAX;
+    if (!DKV) {
+      const long long stat = ((long long)b * p.H + my_head) * p.M;
+      if (row_ok) {
+        hi = dense_limit(p, len, row);
+        lse = p.lse[stat + row];
+        const uint4* go = reinterpret_cast<const uint4*>(static_cast<const T*>(p.grad_out) + p.go_rows.at(b, my_head, row));
+        const uint4* o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + p.out_rows.at(b, my_head, row));
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 u = go[c], w = o[c];
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack2<T>(uw[e]), g = unpack2<T>(ww[e]);
+            delta = fmaf(f.x, g.x, fmaf(f.y, g.y, delta));
+          }
+        }
+      }
+      if (row < p.M && (OWN == 2 || y == 0)) p.delta[stat + row] = delta;
+    } else if (row_ok) {
+      lo = dense_first(p, len, row);
+    }
+    const int tile_lo = __reduce_max_sync(0xffffffffu, lo), tile_hi = __reduce_min_sync(0xffffffffu, hi);
+    const bool table_grad = TABLE && !DKV && p.dbias_part;
+    float far[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, all = 0.f;  // sums of dS and of P over steps of one bucket (offsets below, above), of dS over all
+    int fills = 0, done = 0;
+    for (int t = OWN == 2 ? 0 : y; t < steps; t += OWN == 2 ? 1 : 2) {
+      if (OWN == 2 && !seen_by(x, t)) continue;
+      const int at = partner_row(t), stage = t % S;
+      float one = 0.f;
+      const float* near = nullptr;  // bias of column c at near[c] (DQ), near[-c] (DKV)
+      const uint8_t* near_bucket = nullptr;
+      int side = 0;
+      if (TABLE) {
+        const int start = (DKV ? my_row0 - at - (kPart - 1) : at - my_row0 - (kTcRows - 1)) - len.shift;  // the offset of entry 0
+        const int h = DKV ? partner_head(t) : my_head;
+        if (start + kSpan - 1 <= -p.reach || start >= p.reach) {
+          side = start >= p.reach;
+          one = dense_bias_entry(p, p.buckets[side ? 2 * p.reach : 0], h);
+        } else {
+          float* values = offsets[y][fills & 1];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int e = r + 128 * i, bucket = dense_offset_bucket(p, start + e);
+            values[e] = dense_bias_entry(p, bucket, h);
+            if (table_grad) offset_buckets[y][fills & 1][e] = (uint8_t)bucket;
+          }
+          group_barrier(1 + y, 128);
+          near = values + (DKV ? r + kPart - 1 : kTcRows - 1 - r);
+          if (table_grad) near_bucket = offset_buckets[y][fills & 1] + (kTcRows - 1 - r);
+          ++fills;
+        }
+      }
+      uint32_t seen[2] = {~0u, ~0u};
+      if (!DKV && mask) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int key = at + 32 * w + lane;
+          seen[w] = __ballot_sync(0xffffffffu, key < len.nk && mask[key] != 0);
+        }
+      }
+      wait_on(&bar_s[y], done++);
+      tc_fence_after_sync();
+      float z[64], d[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld32(col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * c]));
+#pragma unroll
+      for (int c = 0; c < 2; ++c) tmem_ld32(col + 64 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&d[32 * c]));
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float2 minus = make_float2(-lse, -lse), less = make_float2(delta, delta);
+        if (DKV) {
+          const float4 st = *reinterpret_cast<const float4*>(&stats[stage][c]);
+          minus = make_float2(st.x, st.z), less = make_float2(st.y, st.w);
+        }
+        if (TABLE) {
+          if (near) minus.x += near[DKV ? -c : c], minus.y += near[DKV ? -c - 1 : c + 1];
+          else minus.x += one, minus.y += one;
+        }
+        const float2 e = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), minus);
+        z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
+        d[c] -= less.x, d[c + 1] -= less.y;
+      }
+      if (at < tile_lo || at + kPart > tile_hi || (!DKV && mask)) {
+        const int a = lo == INT32_MIN ? -1 : lo - at, e = hi == INT32_MAX ? kPart : hi - at;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < a || c >= e || !((seen[c >> 5] >> (c & 31)) & 1u)) z[c] = 0.f;
+      }
+      uint32_t w[32];
+      if (DKV) {
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) w[c >> 1] = pack2<T>(z[c], z[c + 1]);
+        tmem_st16(col, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
+        tmem_st16(col + 16, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        const float2 v = mul2(make_float2(z[c], z[c + 1]), make_float2(d[c], d[c + 1]));
+        d[c] = v.x, d[c + 1] = v.y;
+        w[c >> 1] = pack2<T>(v.x, v.y);
+      }
+      tmem_st16(col + 64, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
+      tmem_st16(col + 80, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_p[y]);
+      if (table_grad) {
+        float2 u[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) u[(c >> 1) & 1] = add2(u[(c >> 1) & 1], make_float2(d[c], d[c + 1]));
+        const float sum = (u[0].x + u[0].y) + (u[1].x + u[1].y);
+        all += sum;
+        if (near) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {
+            const int bucket = near_bucket[c];
+            if (bucket < p.num_buckets && row_ok) sums[bucket * 256 + tid] += d[c];
+          }
+        } else {
+          float2 v[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) v[(c >> 1) & 1] = add2(v[(c >> 1) & 1], make_float2(z[c], z[c + 1]));
+          far[0] += side ? 0.f : sum, far[1] += side ? sum : 0.f;
+          const float mass = (v[0].x + v[0].y) + (v[1].x + v[1].y);
+          far_p[0] += side ? 0.f : mass, far_p[1] += side ? mass : 0.f;
+        }
+      }
+    }
+    if (table_grad) {
+      if (OWN == 1) {  // both groups worked on the rows
+        errors[y][r] = all;
+        group_barrier(3, 256);
+        all = errors[0][r] + errors[1][r];
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int bucket = p.buckets[s ? 2 * p.reach : 0];
+        if (bucket < p.num_buckets && row_ok) sums[bucket * 256 + tid] += far[s] - all * far_p[s];
+      }
+      if (OWN == 1) group_barrier(3, 256);
+      else group_barrier(1 + y, 128);
+      const int tiles = (p.M + kTcRows - 1) / kTcRows;
+      if (my_row0 < p.M) {
+        float* part = p.dbias_part + (((long long)b * p.H + my_head) * tiles + my_row0 / kTcRows) * p.num_buckets;
+        const int base = OWN == 2 ? 128 * y : 0, span = OWN == 2 ? 128 : 256;
+        for (int i = OWN == 2 ? warp & 3 : warp; i < p.num_buckets; i += OWN == 2 ? 4 : 8) {
+          float v = 0.f;
+          for (int e = lane; e < span; e += 32) v += sums[i * 256 + base + e];
+          v = warp_sum(v);
+          if (lane == 0) part[i] = v;
+        }
+      }
+    }
+
+    // ---- rows out: zeros for what is no row
+    wait_on(&bar_o, 0);
+    tc_fence_after_sync();
+    const bool any = x ? last[OWN - 1] > first[OWN - 1] : last[0] > first[0];
+    const bool real = row_ok && any && (!DKV || !mask || mask[row]);
+    auto rows_out = [&](void* base, const DenseRows& rows, int which, int c0, int c1, float mul) {
+#pragma unroll 1
+      for (int c = c0; c < c1; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem + lanes + col_sum(x, which) + c, o);
+        tmem_ld_wait();
+        if (base && row < own_all) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(base) + rows.at(b, my_head, row) + c);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = real ? pack2<T>(__uint_as_float(o[e + 2 * i]) * mul, __uint_as_float(o[e + 2 * i + 1]) * mul) : 0u;
+            dst[e >> 3] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+    };
+    if (DKV) {
+      if (OWN == 2 || y == 0) rows_out(p.dk, p.dk_rows, 0, 0, D, p.scale);
+      if (OWN == 2 || y == 1) rows_out(p.dv, p.dv_rows, 1, 0, D, 1.f);
+    } else {
+      rows_out(p.dq, p.dq_rows, 0, OWN == 2 ? 0 : y * (D / 2), OWN == 2 ? D : (y + 1) * (D / 2), p.scale);
+    }
+    tc_fence_before_sync();
+  }
+  if (bad) atomicExch(&g_dense_status[tc.waits.word], MF_ERR_DEVICE_TIMEOUT);
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D, bool DKV, bool TABLE>
+int launch(const DenseTcParams& tc, cudaStream_t stream) {
+  const DenseParams& p = tc.p;
+  using Sh = BwdShape<D>;
+  auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
+  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? Sh::kMostBuckets * 1024 : 0);
+  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? p.num_buckets * 1024 : 0);
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
+  const int heads = DKV ? p.K : p.H;
+  const bool by_head = Sh::kOwn == 2 && !DKV && (p.H / p.K) % 2 == 0;
+  const long long tiles = ((DKV ? p.N : p.M) + kTcRows - 1) / kTcRows;
+  const long long blocks = by_head ? tiles * p.B * (heads / 2) : (tiles + Sh::kOwn - 1) / Sh::kOwn * p.B * heads;
+  kernel<<<(unsigned)blocks, kBwdThreads, smem, stream>>>(tc);
+  MF_CHECK_LAUNCH("dense attention backward on tcgen05");
+  return MF_OK;
+}
+
+template <typename T, int D>
+int pick(const DenseTcParams& tc, bool table, cudaStream_t stream) {
+  const int rc = table ? launch<T, D, false, true>(tc, stream) : launch<T, D, false, false>(tc, stream);
+  if (rc != MF_OK || (!tc.p.dk && !tc.p.dv)) return rc;
+  return table ? launch<T, D, true, true>(tc, stream) : launch<T, D, true, false>(tc, stream);
+}
+
+}  // namespace
+
+int dense_attn_take_bwd_status(int word, int32_t* host_status, cudaStream_t stream) {
+  take_status_kernel<<<1, 1, 0, stream>>>(word);
+  MF_CHECK_LAUNCH("dense attention status read-back");
+  cudaError_t e = cudaMemcpyFromSymbolAsync(host_status, g_taken_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  return e == cudaSuccess ? MF_OK : cuda_error(e, "dense attention status read-back");
+}
+
+bool dense_tc_bwd_takes(const DenseParams& p, int head_dim, int kind, bool table_grad) {
+  return kind != MF_BUCKETS_PAIR && dense_tc_takes(p, head_dim, kind) && (!table_grad || p.num_buckets <= (head_dim == 64 ? 64 : 32));
+}
+
+int dense_attn_sm100_bwd(const DenseTcParams& tc, int dtype, int head_dim, int kind, cudaStream_t stream) {
+  const bool table = kind != MF_BUCKETS_NONE;
+  if (head_dim == 64) return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16, 64>(tc, table, stream) : pick<__half, 64>(tc, table, stream);
+  return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16, 128>(tc, table, stream) : pick<__half, 128>(tc, table, stream);
+}
+
+}  // namespace mf
