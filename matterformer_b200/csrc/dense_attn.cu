@@ -40,6 +40,11 @@ struct Edges {
   alignas(4) uint8_t first[kCells];  // edges below a cell
   int base, n;
 };
+__device__ __forceinline__ uint32_t param_word(const void* at) {
+  uint32_t v;
+  asm volatile("ld.u32 %0, [%1];" : "=r"(v) : "l"(at));
+  return v;
+}
 constexpr float kDistanceError = 5e-7f;  // of a squared distance in fp32, in relation to it; 6 * 2^-24 and an edge's rounding
 
 // A thread takes four columns, whose coordinates stay in registers, and walks over rows: `lanes` threads (a power of two up to 32) lie along a row, the rest
@@ -55,9 +60,11 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
   __shared__ uint32_t first_words[kCells / 4];
   const uint8_t* first = reinterpret_cast<const uint8_t*>(first_words);
   launch_dependents();
-  for (int i = threadIdx.x; i < kCells / 4; i += kBucketThreads) first_words[i] = reinterpret_cast<const uint32_t*>(edges.first)[i];
+  // (through a generic address: loads of parameters go by the constant cache, one address of a warp after the other)
+  for (int i = threadIdx.x; i < kCells / 4; i += kBucketThreads) first_words[i] = param_word(edges.first + 4 * i);
   for (int i = threadIdx.x; i <= edges.n; i += kBucketThreads)
-    around[i] = make_float2(fmaxf(1e-30f, i ? edges.low[i - 1] * (1.f + kDistanceError) : 0.f), i < edges.n ? fminf(1e30f, edges.low[i] * (1.f - kDistanceError)) : 1e30f);
+    around[i] = make_float2(fmaxf(1e-30f, i ? __uint_as_float(param_word(edges.low + i - 1)) * (1.f + kDistanceError) : 0.f),
+                            i < edges.n ? fminf(1e30f, __uint_as_float(param_word(edges.low + i)) * (1.f - kDistanceError)) : 1e30f);
   wait_for_previous();
   __syncthreads();
   const int ct = blockIdx.x % column_tiles, rt = blockIdx.x / column_tiles % row_tiles, b = blockIdx.x / column_tiles / row_tiles;
@@ -192,7 +199,7 @@ BwdSpace bwd_space(const MfDenseAttnArgs& a, const DenseParams& p) {
   BwdSpace s{};
   const bool small = bwd_family(a, p) == kSmall;
   s.part = small ? 0 : align_up((size_t)a.batch * a.heads * a.queries * sizeof(float), 256);
-  const size_t sums = small ? dense_attn_small_slots(p, a.head_dim) : (size_t)a.batch * dense_attn_mma_tiles(a.queries);
+  const size_t sums = small ? dense_attn_small_slots(p, a.head_dim, a.bucket_kind) : (size_t)a.batch * dense_attn_mma_tiles(a.queries);
   s.total = s.part + (a.bias && a.dbias ? align_up(sums * a.heads * a.num_buckets * sizeof(float), 256) : 0);
   return s;
 }
@@ -261,7 +268,7 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
     if (family == kTensor && !dense_tc_maps(tc, a->dtype, a->head_dim, true)) family = kMma;
     switch (family) {
       case kSmall:
-        entries = dense_attn_small_slots(p, a->head_dim), tiles = 1;
+        entries = dense_attn_small_slots(p, a->head_dim, a->bucket_kind), tiles = 1;
         rc = dense_attn_small(p, a->dtype, a->head_dim, a->bucket_kind, true, stream);
         break;
       case kTensor:

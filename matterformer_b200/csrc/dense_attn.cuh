@@ -96,7 +96,7 @@ int dense_attn_mma_bwd(const DenseParams& p, int dtype, int head_dim, int bucket
 int dense_attn_mma_tiles(int queries);  // query tiles of the backward pass
 // dense_attn_small.cu: at most 32 queries and keys
 bool dense_attn_small_applies(const DenseParams& p, bool backward);
-int dense_attn_small_slots(const DenseParams& p, int head_dim);  // partial sums of the table's gradient for each head
+int dense_attn_small_slots(const DenseParams& p, int head_dim, int bucket_kind);  // partial sums of the table's gradient for each head
 int dense_attn_small(const DenseParams& p, int dtype, int head_dim, int bucket_kind, bool backward, cudaStream_t stream);
 // dense_attn_split.cu: forward, few queries
 bool dense_attn_split_applies(const DenseParams& p);
