@@ -6,29 +6,31 @@
 namespace mf {
 namespace {
 
-// dbias[bucket][head] = sum of the partial sums of all tiles of the head, over batch entries and tiles in order; a block for every (head, bucket),
-// sums in fp64 (they are long and cancel)
-__global__ void __launch_bounds__(128) bias_sum_kernel(const float* part, int B, int H, int tiles, int nb, void* out, int dtype) {
+// dbias[bucket][head] = sum of the partial sums of all tiles of the head: a block for a head and 32 buckets, a warp for every 32nd tile, the warps in
+// order.  Sums in fp64: they are long and cancel.
+__global__ void __launch_bounds__(1024) bias_sum_kernel(const float* part, int B, int H, int tiles, int nb, void* out, int dtype) {
   launch_dependents();
   wait_for_previous();
-  const int h = blockIdx.x % H, bucket = blockIdx.x / H;
-  const long long n = (long long)B * tiles;
+  const int h = blockIdx.x % H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bucket = blockIdx.x / H * 32 + lane;
+  const int n = B * tiles;
   double sum = 0.0;
-  for (long long i = threadIdx.x; i < n; i += 128) sum += part[((i / tiles * H + h) * tiles + i % tiles) * nb + bucket];
-  __shared__ double sums[128];
-  sums[threadIdx.x] = sum;
+  if (bucket < nb) {
+#pragma unroll 4
+    for (int i = warp; i < n; i += 32) {
+      const int b = i / tiles, t = i - b * tiles;
+      sum += part[(((long long)b * H + h) * tiles + t) * nb + bucket];
+    }
+  }
+  __shared__ double sums[32][33];
+  sums[warp][lane] = sum;
   __syncthreads();
-  for (int o = 64; o > 0; o >>= 1) {
-    if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    const float v = (float)sums[0];
-    const int at = bucket * H + h;
-    if (dtype == MF_DTYPE_F32) static_cast<float*>(out)[at] = v;
-    else if (dtype == MF_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = from_f32<__nv_bfloat16>(v);
-    else static_cast<__half*>(out)[at] = from_f32<__half>(v);
-  }
+  if (warp > 0 || bucket >= nb) return;
+  for (int w = 1; w < 32; ++w) sum += sums[w][lane];
+  const float v = (float)sum;
+  const int at = bucket * H + h;
+  if (dtype == MF_DTYPE_F32) static_cast<float*>(out)[at] = v;
+  else if (dtype == MF_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = from_f32<__nv_bfloat16>(v);
+  else static_cast<__half*>(out)[at] = from_f32<__half>(v);
 }
 
 constexpr int kMaxEdges = kMaxBuckets - 1;
@@ -280,7 +282,7 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
     if (rc != MF_OK) return rc;
   }
   if (!table) return MF_OK;
-  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * a->num_buckets), dim3(128), 0, stream, p.dbias_part, entries, a->heads, tiles,
+  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * ((a->num_buckets + 31) / 32)), dim3(1024), 0, stream, p.dbias_part, entries, a->heads, tiles,
                                            a->num_buckets, a->dbias, a->bias_dtype);
   return err == cudaSuccess ? MF_OK : cuda_error(err, "dense attention table gradient");
 }

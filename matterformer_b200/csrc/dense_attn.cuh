@@ -69,6 +69,15 @@ __device__ __forceinline__ int dense_offset_bucket(const DenseParams& p, int off
   return p.buckets[max(-p.reach, min(p.reach, offset)) + p.reach];
 }
 
+// Eight bytes from `at` on, of which the first `n` are there: words that hold one of them are read, no others.
+__device__ __forceinline__ uint2 eight_bytes(const uint8_t* at, int n) {
+  const int skip = (int)(reinterpret_cast<uintptr_t>(at) & 3);
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(at - skip);
+  n = n > 8 ? 8 : n;
+  const uint32_t a = n > 0 ? w[0] : 0u, b = skip + n > 4 ? w[1] : 0u, c = skip + n > 8 ? w[2] : 0u;
+  return make_uint2(__funnelshift_r(a, b, 8 * skip), __funnelshift_r(b, c, 8 * skip));
+}
+
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>

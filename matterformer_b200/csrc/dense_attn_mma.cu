@@ -22,9 +22,10 @@ template <int D>
 constexpr int kTileBytes = 64 * (D + 8) * 2;
 
 // shared memory: own_a | own_b | part_a[2] | part_b[2] | lse, delta [2][64] each | table[kTableEntries] | bias of offsets [2][128], their buckets [2][128] |
-// DQ with a table: [4 warps][num_buckets + 1][32]
-template <int D>
-constexpr int kFixedBytes = 6 * kTileBytes<D> + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 4 + 2 * 128;
+// pairs' buckets [2][64][80] | DQ with a table: [4 warps][num_buckets + 1][32]
+constexpr int kPairRow = 80, kPairTile = 64 * kPairRow;  // a row of 64 bytes, in banks of its own among eight neighbours
+template <int D, int KIND>
+constexpr int kFixedBytes = 6 * kTileBytes<D> + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 4 + 2 * 128 + (KIND == MF_BUCKETS_PAIR ? 2 * kPairTile : 0);
 
 // rows [row0, row0 + 64) of a head, zeros from row_limit on and where `mask` (per row) is zero
 template <typename T, int D>
@@ -50,7 +51,8 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
   float* table = part_delta + 2 * 64;
   float* offset_bias = table + kTableEntries;
   uint8_t* offset_bucket = reinterpret_cast<uint8_t*>(offset_bias + 2 * 128);
-  float* sums = reinterpret_cast<float*>(offset_bucket + 2 * 128);
+  uint8_t* pair_tile = offset_bucket + 2 * 128;
+  float* sums = reinterpret_cast<float*>(pair_tile + (KIND == MF_BUCKETS_PAIR ? 2 * kPairTile : 0));
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int heads = MODE == D_DKV ? p.K : p.H, group = p.H / p.K;
@@ -81,6 +83,24 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
   auto go_of = [&](int h) { return static_cast<const T*>(p.grad_out) + p.go_rows.at(b, h, 0); };
   auto stat = [&](int h) { return ((long long)b * p.H + h) * p.M; };
 
+  const bool aligned = KIND == MF_BUCKETS_PAIR && !((reinterpret_cast<uintptr_t>(p.buckets) | p.bucket_row | p.bucket_batch) & 15);
+  // the buckets of 64 queries from i0 on and 64 keys from j0 on, zeros where there are none
+  auto load_pairs = [&](int i0, int j0, int stage) {
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      const int idx = it * kThreads + tid, r = idx >> 2, c = (idx & 3) * 16;
+      const bool ok = i0 + r < len.nq && j0 + c < len.nk;
+      const uint8_t* src = p.buckets + (ok ? b * p.bucket_batch + (i0 + r) * p.bucket_row + j0 + c : 0);
+      uint8_t* dst = pair_tile + stage * kPairTile + r * kPairRow + c;
+      if (aligned) {  // (a row's last 16 bytes may end behind the last key, but not behind the row)
+        cp_async16(static_cast<uint32_t>(__cvta_generic_to_shared(dst)), src, ok);
+      } else {
+        const int n = ok ? p.N - j0 - c : 0;
+        const uint2 x = eight_bytes(src, n), y = eight_bytes(src + 8, n - 8);
+        *reinterpret_cast<uint4*>(dst) = make_uint4(x.x, x.y, y.x, y.y);
+      }
+    }
+  };
   auto load_step = [&](int t, int stage) {
     const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
     const int at = first + (MODE == D_DKV ? t % per_head : t) * kPart;
@@ -96,6 +116,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
       load_rows<T, D>(s_part_a + stage * TILE, K, p.k_rows.token, at, len.nk, mask);
       load_rows<T, D>(s_part_b + stage * TILE, V, p.v_rows.token, at, len.nk, mask);
     }
+    if (KIND == MF_BUCKETS_PAIR) load_pairs(MODE == D_DKV ? at : row0, MODE == D_DKV ? row0 : at, stage);
     if (KIND == MF_BUCKETS_OFFSET && tid < kSpan) {  // offsets of the two tiles: owner - partner or partner - owner runs over 127 values
       const int offset = (MODE == D_DKV ? row0 - at + tid - (kPart - 1) : at - row0 + tid - (kOwn - 1)) - len.shift;
       const int bucket = dense_offset_bucket(p, offset);
@@ -122,19 +143,18 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     for (int i = tid; i < 4 * (nb + 1) * 32; i += kThreads) sums[i] = 0.f;
   float* my_sums = sums + (warp * (nb + 1)) * 32 + lane;
 
-  // ---- visible partners of this thread's two rows: [lo, hi)
+  // ---- visible partners of this thread's two rows: [lo, hi).  Rows that are none see what they want, their results are not used: queries behind the
+  // last have a log-sum-exp of infinity, as have partners, so that their p is zero.
   int lo[2], hi[2];
+  bool real[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int row = my + 8 * e;
-    if (MODE == D_DKV) {
-      lo[e] = dense_first(p, len, row);
-      hi[e] = row < len.nk && (!mask || mask[row]) ? len.nq : 0;
-    } else {
-      lo[e] = 0;
-      hi[e] = dense_limit(p, len, row);
-    }
+    real[e] = row < own_limit && (MODE != D_DKV || !mask || mask[row]);
+    lo[e] = MODE == D_DKV && real[e] ? dense_first(p, len, row) : 0;
+    hi[e] = MODE != D_DKV && real[e] ? dense_limit(p, len, row) : INT32_MAX;
   }
+  const int most_lo = __reduce_max_sync(0xffffffffu, max(lo[0], lo[1])), least_hi = __reduce_min_sync(0xffffffffu, min(hi[0], hi[1]));
 
   float acc0[D / 8][4], acc1[MODE == D_DKV ? D / 8 : 1][4];
 #pragma unroll
@@ -227,20 +247,36 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     }
 
     // ---- logits in units of log2, minus infinity where nothing is seen
+    uint32_t which[KIND == MF_BUCKETS_NONE ? 1 : 8];  // buckets of the 32 elements, a byte each
+    if (KIND == MF_BUCKETS_PAIR) {
+      const uint8_t* tile_at = pair_tile + stage * kPairTile;
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt) {
+        const int c = nt * 8 + 2 * t4, r = warp * 16 + g;
+        if (MODE == D_DKV)
+          which[nt] = tile_at[c * kPairRow + r] | tile_at[(c + 1) * kPairRow + r] << 8 | tile_at[c * kPairRow + r + 8] << 16 | (uint32_t)tile_at[(c + 1) * kPairRow + r + 8] << 24;
+        else
+          which[nt] = *reinterpret_cast<const uint16_t*>(tile_at + r * kPairRow + c) | (uint32_t)*reinterpret_cast<const uint16_t*>(tile_at + (r + 8) * kPairRow + c) << 16;
+      }
+    }
 #pragma unroll
     for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1), x = at + c;
-        const bool vis = x >= lo[e >> 1] && x < hi[e >> 1] && ((seen[nt >> 2] >> (c & 31)) & 1u);
-        float z = s[nt][e] * sc2;
-        if (KIND == MF_BUCKETS_OFFSET) z += offset_bias[stage * 128 + (MODE == D_DKV ? r - c + kPart - 1 : c - r + kOwn - 1)];
-        if (KIND == MF_BUCKETS_PAIR && vis) {
-          const int i = MODE == D_DKV ? x : row0 + r, j = MODE == D_DKV ? row0 + r : x;
-          z += table[p.buckets[b * p.bucket_batch + i * p.bucket_row + j]];
-        }
-        s[nt][e] = vis ? z : -INFINITY;
+        const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
+        if (KIND == MF_BUCKETS_NONE) s[nt][e] *= sc2;
+        if (KIND == MF_BUCKETS_OFFSET) s[nt][e] = fmaf(s[nt][e], sc2, offset_bias[stage * 128 + (MODE == D_DKV ? r - c + kPart - 1 : c - r + kOwn - 1)]);
+        if (KIND == MF_BUCKETS_PAIR) s[nt][e] = fmaf(s[nt][e], sc2, table[(which[nt] >> (8 * e)) & 255u]);
       }
+    if (at < most_lo || at + kPart > least_hi || (MODE != D_DKV && mask)) {
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = nt * 8 + 2 * t4 + (e & 1), x = at + c;
+          if (x < lo[e >> 1] || x >= hi[e >> 1] || !((seen[nt >> 2] >> (c & 31)) & 1u)) s[nt][e] = -INFINITY;
+        }
+    }
 
     if (MODE == D_FWD) {
       float alpha[2];
@@ -277,9 +313,9 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
           const float z = s[nt][e];
           const float l = MODE == D_DQ ? lse[e >> 1] : part_lse[stage * 64 + c];
           const float d = MODE == D_DQ ? delta[e >> 1] : part_delta[stage * 64 + c];
-          const float pr = z == -INFINITY ? 0.f : dense_exp2(z - l);
+          const float pr = dense_exp2(z - l);
           s[nt][e] = pr;
-          dp[nt][e] = pr == 0.f ? 0.f : pr * (dp[nt][e] - d);
+          dp[nt][e] = pr * (dp[nt][e] - d);
         }
       if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
         // a column of sums for every lane: no two threads meet in one, and the order of a sum is that of the walk
@@ -287,12 +323,9 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
         for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1), x = at + c;
-            if (x < hi[e >> 1]) {
-              const int bucket = KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1]
-                                                           : p.buckets[b * p.bucket_batch + (row0 + r) * p.bucket_row + x];
-              my_sums[min(bucket, nb) * 32] += dp[nt][e];
-            }
+            const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
+            const int bucket = KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1] : (which[nt] >> (8 * e)) & 255u;
+            my_sums[min(bucket, nb) * 32] += dp[nt][e];
           }
       }
     }
@@ -338,9 +371,10 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
       float l = total[e];
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
-      mul[e] = l > 0.f || l != l ? 1.f / l : 0.f;
+      const bool some = real[e] && (l > 0.f || l != l);
+      mul[e] = some ? 1.f / l : 0.f;
       const int row = my + 8 * e;
-      if (p.lse && t4 == 0 && row < p.M) p.lse[stat(oh) + row] = l > 0.f || l != l ? top[e] + log2f(l) : INFINITY;
+      if (p.lse && t4 == 0 && row < p.M) p.lse[stat(oh) + row] = some ? top[e] + log2f(l) : INFINITY;
     }
   }
   const int limit = MODE == D_DKV ? p.N : p.M;
@@ -357,7 +391,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     }
   };
   if (MODE == D_FWD) store(p.out, p.out_rows, acc0, mul[0], mul[1]);
-  const float real0 = hi[0] > 0 ? 1.f : 0.f, real1 = hi[1] > 0 ? 1.f : 0.f;
+  const float real0 = real[0] ? 1.f : 0.f, real1 = real[1] ? 1.f : 0.f;
   if (MODE == D_DQ && p.dq) store(p.dq, p.dq_rows, acc0, real0 * p.scale, real1 * p.scale);
   if constexpr (MODE == D_DKV) {
     if (p.dk) store(p.dk, p.dk_rows, acc0, real0 * p.scale, real1 * p.scale);
@@ -380,10 +414,10 @@ template <typename T, int D, int MODE, int KIND>
 int launch(const DenseParams& p, cudaStream_t stream) {
   const int own = MODE == D_DKV ? p.N : p.M, heads = MODE == D_DKV ? p.K : p.H;
   if (own == 0) return MF_OK;
-  const int smem = kFixedBytes<D> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
+  const int smem = kFixedBytes<D, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
   auto kernel = dense_attn_mma_kernel<T, D, MODE, KIND>;
   // one limit for all calls: what the largest table needs
-  constexpr int most = kFixedBytes<D> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
+  constexpr int most = kFixedBytes<D, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
   static_assert(most <= 227 * 1024, "");
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
