@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bar_q, bar_full[Sh::kSlots], bar_free[Sh::kSlots], bar_clean[Sh::kSlots], bar_s[2], bar_p[2], bar_o[2], bar_drain;
   __shared__ uint32_t tmem_base;
-  __shared__ float table[KIND == MF_BUCKETS_PAIR ? 2 : 1][KIND == MF_BUCKETS_PAIR ? kTableEntries : 1];
+  __shared__ float table[KIND == MF_BUCKETS_NONE ? 1 : 2][KIND == MF_BUCKETS_NONE ? 1 : kTableEntries];
   __shared__ float offsets[KIND == MF_BUCKETS_OFFSET ? 2 : 1][2][KIND == MF_BUCKETS_OFFSET ? 256 : 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -209,9 +209,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
     const int least = __reduce_min_sync(0xffffffffu, limit);
     const float sc2 = p.scale * kDenseLog2e;
     float top = -INFINITY, total = 0.f;
-    if (KIND == MF_BUCKETS_PAIR) {
+    float far[2] = {0.f, 0.f};  // bias of the offsets -reach and reach, and beyond
+    if (KIND != MF_BUCKETS_NONE) {
       for (int e = r; e < kTableEntries; e += 128) table[x][e] = dense_bias_entry(p, e, my_head);
       group_barrier(1 + x, 128);
+      if (KIND == MF_BUCKETS_OFFSET) far[0] = table[x][p.buckets[0]], far[1] = table[x][p.buckets[2 * p.reach]];
     }
     const uint8_t* pair_row = KIND == MF_BUCKETS_PAIR ? p.buckets + b * p.bucket_batch + min(i, p.M - 1) * p.bucket_row : nullptr;
     int fills = 0;
@@ -220,9 +222,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
       float one = 0.f;
       const float* near = nullptr;
       if (KIND == MF_BUCKETS_OFFSET) {
-        float* values = offsets[x][fills & 1];
-        int unused;
-        if (dense_offsets(p, key0 - my_row0 - len.shift, my_head, r, values, nullptr, one, unused)) {
+        const int start = key0 - my_row0 - len.shift - 127;  // the offset of entry 0; entry e stands for the columns c of rows r with c - r = e - 127
+        if (start + 254 <= -p.reach) {
+          one = far[0];
+        } else if (start >= p.reach) {
+          one = far[1];
+        } else {
+          float* values = offsets[x][fills & 1];
+          const int b0 = dense_offset_bucket(p, start + r), b1 = dense_offset_bucket(p, start + r + 128);
+          values[r] = table[x][b0], values[r + 128] = table[x][b1];
           group_barrier(1 + x, 128);
           near = values + 127 - r;
           ++fills;
@@ -260,12 +268,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
 #pragma unroll
           for (int e = 0; e < 16; ++e) z[c + e] = fmaf(z[c + e], sc2, table[x][(w[e >> 2] >> (8 * (e & 3))) & 255u]);
         }
-      } else {
+      }
+      // z is the logit where pairs have biases of their own; otherwise z * mul + one is, and its maximum is formed from z's
+      const bool own_bias = KIND == MF_BUCKETS_PAIR || (KIND == MF_BUCKETS_OFFSET && near);
+      float mul = own_bias ? 1.f : sc2;
+      if (mul <= 0.f) {  // (a maximum of products is not the product of the maximum)
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const float2 v = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), make_float2(one, one));
-          z[c] = v.x, z[c + 1] = v.y;
-        }
+        for (int c = 0; c < 128; ++c) z[c] *= mul;
+        mul = 1.f;
       }
       if (key0 + kTcRows > least || mask) {
         const int left = limit - key0;
@@ -281,7 +291,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
         for (int c = 1; c < 31; c += 2) m[q] = max3(m[q], z[32 * q + c], z[32 * q + c + 1]);
         m[q] = fmaxf(m[q], z[32 * q + 31]);
       }
-      const float now = max3(top, fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const float mine = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      const float now = fmaxf(top, mine == -INFINITY ? mine : fmaf(mine, mul, one));
       if (j == 0) {
         top = now;
       } else if (__any_sync(0xffffffffu, now > top + 8.f)) {
@@ -299,14 +310,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
           tmem_st16(col_o + c + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
         }
       }
-      const float shift = top == -INFINITY ? 0.f : -top;
+      const float shift = one == -INFINITY ? one : top == -INFINITY ? 0.f : one - top;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 128; c += 32) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          float2 v = add2(make_float2(z[c + e], z[c + e + 1]), make_float2(shift, shift));
+          float2 v = fma2(make_float2(z[c + e], z[c + e + 1]), make_float2(mul, mul), make_float2(shift, shift));
           v.x = dense_exp2(v.x), v.y = dense_exp2(v.y);
           sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], v);
           w[e >> 1] = pack2<T>(v.x, v.y);

@@ -37,23 +37,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ void group_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// Bias of the offsets between two tiles of 128 rows, by the 128 threads of a group: entry e stands for the offset `base` + e - 127.  False where the tiles
-// lie so far apart that one bucket holds all offsets; `one` is its bias then.
-__device__ __forceinline__ bool dense_offsets(const DenseParams& p, int base, int head, int r, float* values, uint8_t* buckets, float& one, int& one_bucket) {
-  if (base + 127 <= -p.reach || base - 127 >= p.reach) {
-    one_bucket = p.buckets[base > 0 ? 2 * p.reach : 0];
-    one = dense_bias_entry(p, one_bucket, head);
-    return false;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int e = r + 128 * i, bucket = dense_offset_bucket(p, base + e - 127);
-    values[e] = dense_bias_entry(p, bucket, head);
-    if (buckets) buckets[e] = (uint8_t)bucket;
-  }
-  return true;
-}
-
 // Maps of the call's operands; false where the copy engine does not take them.
 bool dense_tc_maps(DenseTcParams& tc, int dtype, int head_dim, bool backward);
 // Whether the call is of a kind that the 128-row kernels take, whatever its size.

@@ -9,8 +9,8 @@
 // fill the other's buffer.  At head size 64 a CTA owns two tiles that share the partners they read, a buffer each; at 128, where the sums of two
 // tiles do not fit tensor memory, one tile, and the groups take its steps in turn.
 //
-// The table's gradient (DQ): steps whose offsets all fall into one bucket add up in a register; in the others every thread adds to a column of sums of
-// its own in shared memory.  dS = P (dP - delta) with delta from rounded outputs; the row sums of dS, which are zero but for the error in
+// The table's gradient (DQ): steps whose offsets all fall into one bucket add up in a register; in the others dS goes through shared memory and threads sum
+// along its diagonals, each into a column of sums of its own.  dS = P (dP - delta) with delta from rounded outputs; the row sums of dS, which are zero but for the error in
 // delta, correct what far buckets got: there thousands of P share one error, which would otherwise be the largest of that sum.
 //
 // Roles as in the forward kernel; warp 10 also brings the queries' log-sum-exp and delta for DKV.
@@ -27,26 +27,29 @@ constexpr int kBwdThreads = 384, kPart = 64, kSpan = kTcRows + kPart - 1;
 constexpr int kRegAux = 56, kRegOwner = 224;
 static_assert(8 * kRegOwner + 4 * kRegAux <= 12 * 168, "register hand-over exceeds the CTA's pool");
 
-template <int D>
+template <int D, bool SUMS>
 struct BwdShape {
   static constexpr int kOwn = D == 64 ? 2 : 1;  // owner tiles
   static constexpr int kChunks = D / 64, kTile = kChunks * kTcRows * 128, kPartTile = kChunks * kPart * 128;
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = D == 64 && !SUMS ? 4 : 3;
   static constexpr int kOffA = 0, kOffB = kOwn * kTile, kOffRing = 2 * kOwn * kTile, kSmem = kOffRing + kStages * 2 * kPartTile;
   static constexpr int kMostBuckets = D == 64 ? 64 : 32;  // whose sums fit beside that
+  static constexpr int kDiagonals = D == 64 ? 32 : 16;    // columns of dS that are summed along their diagonals at a time
+  static constexpr int kDiagonalBytes = kTcRows * (kDiagonals + 1) * 4;
 };
 
 template <typename T, int D, bool DKV, bool TABLE>
 __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const __grid_constant__ DenseTcParams tc) {
-  using Sh = BwdShape<D>;
+  using Sh = BwdShape<D, TABLE && !DKV>;
   constexpr int OWN = Sh::kOwn, S = Sh::kStages;
   const DenseParams& p = tc.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem);  // [num_buckets][256 row owners]
+  float* diagonals = reinterpret_cast<float*>(smem + Sh::kSmem);  // [2 groups][128 rows][kDiagonals + 1]
+  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem + 2 * Sh::kDiagonalBytes);  // [num_buckets][256 row owners]
   __shared__ uint64_t bar_own, bar_full[S], bar_free[S], bar_clean[S], bar_s[2], bar_p[2], bar_o, bar_drain;
   __shared__ uint32_t tmem_base;
-  __shared__ float offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
+  __shared__ float table[TABLE ? 2 : 1][TABLE ? kTableEntries : 1], offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
   __shared__ uint8_t offset_buckets[TABLE && !DKV ? 2 : 1][2][TABLE && !DKV ? 256 : 1];
   __shared__ __align__(16) float2 stats[DKV ? S : 1][DKV ? kPart : 1];  // -lse and delta of the partners
   __shared__ float errors[TABLE && !DKV && OWN == 1 ? 2 : 1][TABLE && !DKV && OWN == 1 ? 128 : 1];
@@ -303,7 +306,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     const int tile_lo = __reduce_max_sync(0xffffffffu, lo), tile_hi = __reduce_min_sync(0xffffffffu, hi);
     const bool table_grad = TABLE && !DKV && p.dbias_part;
     float far[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, all = 0.f;  // sums of dS and of P over steps of one bucket (offsets below, above), of dS over all
-    int fills = 0, done = 0;
+    int fills = 0, done = 0, table_head = -1;
+    float far_bias[2] = {0.f, 0.f};  // of the offsets -reach and reach, and beyond
     for (int t = OWN == 2 ? 0 : y; t < steps; t += OWN == 2 ? 1 : 2) {
       if (OWN == 2 && !seen_by(x, t)) continue;
       const int at = partner_row(t), stage = t % S;
@@ -314,20 +318,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       if (TABLE) {
         const int start = (DKV ? my_row0 - at - (kPart - 1) : at - my_row0 - (kTcRows - 1)) - len.shift;  // the offset of entry 0
         const int h = DKV ? partner_head(t) : my_head;
+        if (h != table_head) {
+          if (table_head >= 0) group_barrier(1 + y, 128);
+          for (int e = r; e < kTableEntries; e += 128) table[y][e] = dense_bias_entry(p, e, h);
+          group_barrier(1 + y, 128);
+          table_head = h;
+          far_bias[0] = table[y][p.buckets[0]], far_bias[1] = table[y][p.buckets[2 * p.reach]];
+        }
         if (start + kSpan - 1 <= -p.reach || start >= p.reach) {
           side = start >= p.reach;
-          one = dense_bias_entry(p, p.buckets[side ? 2 * p.reach : 0], h);
+          one = side ? far_bias[1] : far_bias[0];
         } else {
           float* values = offsets[y][fills & 1];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int e = r + 128 * i, bucket = dense_offset_bucket(p, start + e);
-            values[e] = dense_bias_entry(p, bucket, h);
-            if (table_grad) offset_buckets[y][fills & 1][e] = (uint8_t)bucket;
-          }
+          const int b0 = dense_offset_bucket(p, start + r), b1 = dense_offset_bucket(p, start + r + 128);
+          values[r] = table[y][b0], values[r + 128] = table[y][b1];
+          if (table_grad) offset_buckets[y][fills & 1][r] = (uint8_t)b0, offset_buckets[y][fills & 1][r + 128] = (uint8_t)b1;
           group_barrier(1 + y, 128);
           near = values + (DKV ? r + kPart - 1 : kTcRows - 1 - r);
-          if (table_grad) near_bucket = offset_buckets[y][fills & 1] + (kTcRows - 1 - r);
+          near_bucket = offset_buckets[y][fills & 1];
           ++fills;
         }
       }
@@ -394,10 +402,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         const float sum = (u[0].x + u[0].y) + (u[1].x + u[1].y);
         all += sum;
         if (near) {
+          // Pairs of one offset lie on a diagonal: a thread adds up one or two of them, which have one bucket each.
+          constexpr int W = Sh::kDiagonals;
+          float* tile = diagonals + y * kTcRows * (W + 1);
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            const int bucket = near_bucket[c];
-            if (bucket < p.num_buckets && row_ok) sums[bucket * 256 + tid] += d[c];
+          for (int c0 = 0; c0 < 64; c0 += W) {
+#pragma unroll
+            for (int c = 0; c < W; ++c) tile[r * (W + 1) + c] = row_ok ? d[c0 + c] : 0.f;
+            group_barrier(1 + y, 128);
+            for (int e = r; e < kTcRows + W - 1; e += 128) {  // c - row = e - 127
+              float v = 0.f;
+              const int row_at = kTcRows - 1 - e;
+#pragma unroll
+              for (int c = 0; c < W; ++c)
+                if (row_at + c >= 0 && row_at + c < kTcRows) v += tile[(row_at + c) * (W + 1) + c];
+              const int bucket = near_bucket[c0 + e];
+              if (bucket < p.num_buckets) sums[bucket * 256 + tid] += v;
+            }
+            group_barrier(1 + y, 128);
           }
         } else {
           float2 v[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -474,10 +496,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
 template <typename T, int D, bool DKV, bool TABLE>
 int launch(const DenseTcParams& tc, cudaStream_t stream) {
   const DenseParams& p = tc.p;
-  using Sh = BwdShape<D>;
+  using Sh = BwdShape<D, TABLE && !DKV>;
   auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
-  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? Sh::kMostBuckets * 1024 : 0);
-  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? p.num_buckets * 1024 : 0);
+  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 2 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0);
+  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 2 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0);
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   const int heads = DKV ? p.K : p.H;
