@@ -4,8 +4,8 @@
 //   DQ  : owners = queries, partners = keys     S = Q K^T, dP = dO V^T       -> dS        -> dQ += dS K
 //   DKV : owners = keys,    partners = queries  S^T = K Q^T, dP^T = V dO^T   -> P^T, dS^T -> dV += P^T dO, dK += dS^T Q
 // Seven products instead of the five of a single pass, but every sum has one owner and a fixed order, and nothing is added up in memory.
-// A thread owns a row; P and dS are packed to 16 bits over the columns that S and dP had and are the A operands of the second products, whose sums
-// stay in tensor memory over the whole walk.  Two buffers for S and dP, each with a group of four warps: while one group works the tensor cores
+// Two threads share a row, half of a step's columns each; P and dS are packed to 16 bits over the columns that S and dP had and are the A operands of the second products, whose sums
+// stay in tensor memory over the whole walk.  Two buffers for S and dP, each with a group of eight warps: while one group works the tensor cores
 // fill the other's buffer.  At head size 64 a CTA owns two tiles that share the partners they read, a buffer each; at 128, where the sums of two
 // tiles do not fit tensor memory, one tile, and the groups take its steps in turn.
 //
@@ -13,7 +13,7 @@
 // along its diagonals, each into a column of sums of its own.  dS = P (dP - delta) with delta from rounded outputs; the row sums of dS, which are zero but for the error in
 // delta, correct what far buckets got: there thousands of P share one error, which would otherwise be the largest of that sum.
 //
-// Roles as in the forward kernel; warp 10 also brings the queries' log-sum-exp and delta for DKV.
+// Roles as in the forward kernel; the warp that clears rows also brings the queries' log-sum-exp and delta for DKV.
 #include "dense_attn_sm100.cuh"
 
 namespace mf {
@@ -23,9 +23,9 @@ __device__ int32_t g_dense_status[2];  // last expired wait: of calls, of the se
 __device__ int32_t g_taken_status;
 __global__ void take_status_kernel(int word) { g_taken_status = atomicExch(&g_dense_status[word], 0); }
 
-constexpr int kBwdThreads = 384, kPart = 64, kSpan = kTcRows + kPart - 1;
-constexpr int kRegAux = 56, kRegOwner = 224;
-static_assert(8 * kRegOwner + 4 * kRegAux <= 12 * 168, "register hand-over exceeds the CTA's pool");
+constexpr int kOwnerWarps = 16, kBwdThreads = (kOwnerWarps + 4) * 32, kPart = 64, kCols = 32, kSpan = kTcRows + kPart - 1;
+constexpr int kRegAux = 56, kRegOwner = 104;
+static_assert(kOwnerWarps * kRegOwner + 4 * kRegAux <= (kOwnerWarps + 4) * 96, "register hand-over exceeds the CTA's pool");
 
 template <int D, bool SUMS>
 struct BwdShape {
@@ -34,7 +34,7 @@ struct BwdShape {
   static constexpr int kStages = D == 64 && !SUMS ? 4 : 3;
   static constexpr int kOffA = 0, kOffB = kOwn * kTile, kOffRing = 2 * kOwn * kTile, kSmem = kOffRing + kStages * 2 * kPartTile;
   static constexpr int kMostBuckets = D == 64 ? 64 : 32;  // whose sums fit beside that
-  static constexpr int kDiagonals = D == 64 ? 32 : 16;    // columns of dS that are summed along their diagonals at a time
+  static constexpr int kDiagonals = D == 64 ? 16 : 8;  // columns of dS that 128 threads sum along their diagonals at a time
   static constexpr int kDiagonalBytes = kTcRows * (kDiagonals + 1) * 4;
 };
 
@@ -45,14 +45,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   const DenseParams& p = tc.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* diagonals = reinterpret_cast<float*>(smem + Sh::kSmem);  // [2 groups][128 rows][kDiagonals + 1]
-  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem + 2 * Sh::kDiagonalBytes);  // [num_buckets][256 row owners]
+  float* diagonals = reinterpret_cast<float*>(smem + Sh::kSmem);  // [2 groups][2 halves][128 rows][kDiagonals + 1]
+  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem + 4 * Sh::kDiagonalBytes);  // [num_buckets][4 halves of groups][64]
   __shared__ uint64_t bar_own, bar_full[S], bar_free[S], bar_clean[S], bar_s[2], bar_p[2], bar_o, bar_drain;
   __shared__ uint32_t tmem_base;
   __shared__ float table[TABLE ? 2 : 1][TABLE ? kTableEntries : 1], offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
   __shared__ uint8_t offset_buckets[TABLE && !DKV ? 2 : 1][2][TABLE && !DKV ? 256 : 1];
   __shared__ __align__(16) float2 stats[DKV ? S : 1][DKV ? kPart : 1];  // -lse and delta of the partners
-  __shared__ float errors[TABLE && !DKV && OWN == 1 ? 2 : 1][TABLE && !DKV && OWN == 1 ? 128 : 1];
+  __shared__ float errors[TABLE && !DKV ? 4 : 1][TABLE && !DKV ? 128 : 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // ---- which rows
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     auto init = [&](uint64_t* bar, int count, int kind) { mbar_init(bar, count + (tc.waits.withheld == kind)); };
     init(&bar_own, 1, 0);
     for (int i = 0; i < S; ++i) init(&bar_full[i], 1, 0), init(&bar_free[i], 1, 1), init(&bar_clean[i], 1, 4);
-    for (int x = 0; x < 2; ++x) init(&bar_s[x], 1, 2), init(&bar_p[x], 4, 3);
+    for (int x = 0; x < 2; ++x) init(&bar_s[x], 1, 2), init(&bar_p[x], 8, 3);
     init(&bar_o, 1, 2);
     mbar_init(&bar_drain, 1);
     mbar_fence_init();
@@ -152,9 +152,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   auto step_of = [&](int n) { return OWN == 2 ? n >> 1 : n; };
   auto valid = [&](int n) { return OWN == 1 || seen_by(n & 1, n >> 1); };
 
-  if (warp >= 8) {
+  if (warp >= kOwnerWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegAux));
-    if (warp == 9) {
+    if (warp == kOwnerWarps + 1) {
       // ---------------------------------------------------------------- copies
       if (lane == 0) {
         const CUtensorMap *own_a = DKV ? &tc.k : &tc.q, *own_b = DKV ? &tc.v : &tc.grad_out, *part_a = DKV ? &tc.q : &tc.k, *part_b = DKV ? &tc.grad_out : &tc.v;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         for (int i = max(0, t - S); i < t; ++i)
           if (!mbar_wait(&bar_full[i % S], (i / S) & 1)) bad = true;
       }
-    } else if (warp == 8) {
+    } else if (warp == kOwnerWarps) {
       // ---------------------------------------------------------------- products
       if (elect_one()) {
         const uint32_t l_a = make_desc_lo(smem_u32(smem + Sh::kOffA), 0), l_b = make_desc_lo(smem_u32(smem + Sh::kOffB), 0);
@@ -226,8 +226,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
               const uint32_t part = l_ring_mn + stage * 2 * kPartTile, col = tmem + 128 * y;
 #pragma unroll
               for (int kg = 0; kg < kPart / 16; ++kg) {
-                if (DKV) umma_ts_lo(tmem + col_sum(x, 1), col + 8 * kg, part + kPartTile + 128 * kg, idesc_o, sum_started[x] || kg > 0);
-                umma_ts_lo(tmem + col_sum(x, 0), col + 64 + 8 * kg, part + 128 * kg, idesc_o, sum_started[x] || kg > 0);
+                const uint32_t packed = 32 * (kg >> 1) + 8 * (kg & 1);
+                if (DKV) umma_ts_lo(tmem + col_sum(x, 1), col + packed, part + kPartTile + 128 * kg, idesc_o, sum_started[x] || kg > 0);
+                umma_ts_lo(tmem + col_sum(x, 0), col + 64 + packed, part + 128 * kg, idesc_o, sum_started[x] || kg > 0);
               }
               sum_started[x] = 1;
             }
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         umma_commit(&bar_drain);
         if (!mbar_wait(&bar_drain, 0)) bad = true;
       }
-    } else if (warp == 10) {
+    } else if (warp == kOwnerWarps + 2) {
       // ---------------------------------------------------------------- partners that are none become zeros; log-sum-exp and delta of queries
       if (cleaning) {
         for (int t = 0; t < steps; ++t) {
@@ -272,7 +273,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   } else {
     // ------------------------------------------------------------------ row owners
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegOwner));
-    const int y = warp >> 2, x = OWN == 2 ? y : 0, r = tid & 127;  // group (and buffer), tile
+    const int y = warp >> 3, half = warp >> 2 & 1, x = OWN == 2 ? y : 0, r = tid & 127;  // group (and buffer), half of the columns, tile
+    const int c0 = half * kCols, pair = tid & 255, team = warp >> 2;  // the 256 threads of a group are pairs of 128
     const int my_head = x ? head[OWN - 1] : head[0], my_row0 = x ? row0[OWN - 1] : row0[0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, col = tmem + lanes + 128 * y;
     const int row = my_row0 + r;
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
           }
         }
       }
-      if (row < p.M && (OWN == 2 || y == 0)) p.delta[stat + row] = delta;
+      if (row < p.M && half == 0 && (OWN == 2 || y == 0)) p.delta[stat + row] = delta;
     } else if (row_ok) {
       lo = dense_first(p, len, row);
     }
@@ -312,16 +314,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       if (OWN == 2 && !seen_by(x, t)) continue;
       const int at = partner_row(t), stage = t % S;
       float one = 0.f;
-      const float* near = nullptr;  // bias of column c at near[c] (DQ), near[-c] (DKV)
+      const float* near = nullptr;  // bias of the thread's column c at near[c] (DQ), near[-c] (DKV)
       const uint8_t* near_bucket = nullptr;
       int side = 0;
       if (TABLE) {
         const int start = (DKV ? my_row0 - at - (kPart - 1) : at - my_row0 - (kTcRows - 1)) - len.shift;  // the offset of entry 0
         const int h = DKV ? partner_head(t) : my_head;
         if (h != table_head) {
-          if (table_head >= 0) group_barrier(1 + y, 128);
-          for (int e = r; e < kTableEntries; e += 128) table[y][e] = dense_bias_entry(p, e, h);
-          group_barrier(1 + y, 128);
+          if (table_head >= 0) group_barrier(1 + y, 256);
+          table[y][pair] = dense_bias_entry(p, pair, h);
+          group_barrier(1 + y, 256);
           table_head = h;
           far_bias[0] = table[y][p.buckets[0]], far_bias[1] = table[y][p.buckets[2 * p.reach]];
         }
@@ -330,67 +332,68 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
           one = side ? far_bias[1] : far_bias[0];
         } else {
           float* values = offsets[y][fills & 1];
-          const int b0 = dense_offset_bucket(p, start + r), b1 = dense_offset_bucket(p, start + r + 128);
-          values[r] = table[y][b0], values[r + 128] = table[y][b1];
-          if (table_grad) offset_buckets[y][fills & 1][r] = (uint8_t)b0, offset_buckets[y][fills & 1][r + 128] = (uint8_t)b1;
-          group_barrier(1 + y, 128);
-          near = values + (DKV ? r + kPart - 1 : kTcRows - 1 - r);
+          const int bucket = dense_offset_bucket(p, start + pair);
+          values[pair] = table[y][bucket];
+          if (table_grad) offset_buckets[y][fills & 1][pair] = (uint8_t)bucket;
+          group_barrier(1 + y, 256);
+          near = values + (DKV ? r + kPart - 1 - c0 : kTcRows - 1 - r + c0);
           near_bucket = offset_buckets[y][fills & 1];
           ++fills;
         }
       }
-      uint32_t seen[2] = {~0u, ~0u};
+      uint32_t seen = ~0u;
       if (!DKV && mask) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int key = at + 32 * w + lane;
-          seen[w] = __ballot_sync(0xffffffffu, key < len.nk && mask[key] != 0);
-        }
+        const int key = at + c0 + lane;
+        seen = __ballot_sync(0xffffffffu, key < len.nk && mask[key] != 0);
       }
       wait_on(&bar_s[y], done++);
       tc_fence_after_sync();
-      float z[64], d[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld32(col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * c]));
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld32(col + 64 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&d[32 * c]));
+      float z[kCols], d[kCols];
+      tmem_ld32(col + c0, *reinterpret_cast<uint32_t(*)[32]>(&z[0]));
+      tmem_ld32(col + 64 + c0, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
       tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float2 minus = make_float2(-lse, -lse), less = make_float2(delta, delta);
-        if (DKV) {
-          const float4 st = *reinterpret_cast<const float4*>(&stats[stage][c]);
-          minus = make_float2(st.x, st.z), less = make_float2(st.y, st.w);
-        }
-        if (TABLE) {
-          if (near) minus.x += near[DKV ? -c : c], minus.y += near[DKV ? -c - 1 : c + 1];
-          else minus.x += one, minus.y += one;
-        }
-        const float2 e = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), minus);
-        z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
-        d[c] -= less.x, d[c + 1] -= less.y;
-      }
-      if (at < tile_lo || at + kPart > tile_hi || (!DKV && mask)) {
-        const int a = lo == INT32_MIN ? -1 : lo - at, e = hi == INT32_MAX ? kPart : hi - at;
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < a || c >= e || !((seen[c >> 5] >> (c & 31)) & 1u)) z[c] = 0.f;
-      }
-      uint32_t w[32];
       if (DKV) {
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) w[c >> 1] = pack2<T>(z[c], z[c + 1]);
-        tmem_st16(col, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
-        tmem_st16(col + 16, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+        for (int c = 0; c < kCols; c += 2) {
+          const float4 st = *reinterpret_cast<const float4*>(&stats[stage][c0 + c]);
+          float2 minus = make_float2(st.x, st.z);
+          if (TABLE) minus = add2(minus, near ? make_float2(near[-c], near[-c - 1]) : make_float2(one, one));
+          const float2 e = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), minus);
+          z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
+          const float2 v = add2(make_float2(d[c], d[c + 1]), make_float2(-st.y, -st.w));
+          d[c] = v.x, d[c + 1] = v.y;
+        }
+      } else {
+        const float less = one - lse;
+#pragma unroll
+        for (int c = 0; c < kCols; c += 2) {
+          float2 minus = make_float2(less, less);
+          if (TABLE && near) minus = add2(minus, make_float2(near[c], near[c + 1]));
+          const float2 e = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), minus);
+          z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
+          const float2 v = add2(make_float2(d[c], d[c + 1]), make_float2(-delta, -delta));
+          d[c] = v.x, d[c + 1] = v.y;
+        }
+      }
+      if (at < tile_lo || at + kPart > tile_hi || (!DKV && mask)) {
+        const int a = lo == INT32_MIN ? -1 : lo - at - c0, e = hi == INT32_MAX ? kPart : hi - at - c0;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          if (c < a || c >= e || !((seen >> c) & 1u)) z[c] = 0.f;
+      }
+      uint32_t w[16];
+      if (DKV) {
+#pragma unroll
+        for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack2<T>(z[c], z[c + 1]);
+        tmem_st16(col + c0, w);  // (over the thread's own columns: the other half may not have read its)
       }
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < kCols; c += 2) {
         const float2 v = mul2(make_float2(z[c], z[c + 1]), make_float2(d[c], d[c + 1]));
         d[c] = v.x, d[c + 1] = v.y;
         w[c >> 1] = pack2<T>(v.x, v.y);
       }
-      tmem_st16(col + 64, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
-      tmem_st16(col + 80, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+      tmem_st16(col + 64 + c0, w);
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
@@ -398,33 +401,42 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       if (table_grad) {
         float2 u[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) u[(c >> 1) & 1] = add2(u[(c >> 1) & 1], make_float2(d[c], d[c + 1]));
+        for (int c = 0; c < kCols; c += 2) u[(c >> 1) & 1] = add2(u[(c >> 1) & 1], make_float2(d[c], d[c + 1]));
         const float sum = (u[0].x + u[0].y) + (u[1].x + u[1].y);
         all += sum;
         if (near) {
-          // Pairs of one offset lie on a diagonal: a thread adds up one or two of them, which have one bucket each.
+          // Pairs of one offset lie on a diagonal: a thread adds up one or two of them, which have one bucket each.  Threads 64 apart share a column
+          // of sums and take it in turn.
           constexpr int W = Sh::kDiagonals;
-          float* tile = diagonals + y * kTcRows * (W + 1);
+          float* tile = diagonals + team * kTcRows * (W + 1);
+          float* column = sums + team * 64 + (r & 63);
 #pragma unroll
-          for (int c0 = 0; c0 < 64; c0 += W) {
+          for (int w0 = 0; w0 < kCols; w0 += W) {
 #pragma unroll
-            for (int c = 0; c < W; ++c) tile[r * (W + 1) + c] = row_ok ? d[c0 + c] : 0.f;
-            group_barrier(1 + y, 128);
-            for (int e = r; e < kTcRows + W - 1; e += 128) {  // c - row = e - 127
-              float v = 0.f;
-              const int row_at = kTcRows - 1 - e;
+            for (int c = 0; c < W; ++c) tile[r * (W + 1) + c] = row_ok ? d[w0 + c] : 0.f;
+            group_barrier(3 + team, 128);
+            float v[2] = {0.f, 0.f};  // c - row = r - 127 and r + 1
+            const int row_at = kTcRows - 1 - r;
 #pragma unroll
-              for (int c = 0; c < W; ++c)
-                if (row_at + c >= 0 && row_at + c < kTcRows) v += tile[(row_at + c) * (W + 1) + c];
-              const int bucket = near_bucket[c0 + e];
-              if (bucket < p.num_buckets) sums[bucket * 256 + tid] += v;
+            for (int c = 0; c < W; ++c)
+              if (row_at + c < kTcRows) v[0] += tile[(row_at + c) * (W + 1) + c];
+            if (r < W - 1) {
+#pragma unroll
+              for (int c = 1; c < W; ++c)
+                if (c > r) v[1] += tile[(c - r - 1) * (W + 1) + c];
             }
-            group_barrier(1 + y, 128);
+            const int b0 = near_bucket[c0 + w0 + r], b1 = near_bucket[c0 + w0 + min(r + 128, kSpan - 1 - w0)];
+            if (r < 64) {
+              if (b0 < p.num_buckets) column[b0 * 256] += v[0];
+              if (r < W - 1 && b1 < p.num_buckets) column[b1 * 256] += v[1];
+            }
+            group_barrier(3 + team, 128);
+            if (r >= 64 && b0 < p.num_buckets) column[b0 * 256] += v[0];
           }
         } else {
           float2 v[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int c = 0; c < 64; c += 2) v[(c >> 1) & 1] = add2(v[(c >> 1) & 1], make_float2(z[c], z[c + 1]));
+          for (int c = 0; c < kCols; c += 2) v[(c >> 1) & 1] = add2(v[(c >> 1) & 1], make_float2(z[c], z[c + 1]));
           far[0] += side ? 0.f : sum, far[1] += side ? sum : 0.f;
           const float mass = (v[0].x + v[0].y) + (v[1].x + v[1].y);
           far_p[0] += side ? 0.f : mass, far_p[1] += side ? mass : 0.f;
@@ -432,23 +444,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       }
     }
     if (table_grad) {
-      if (OWN == 1) {  // both groups worked on the rows
-        errors[y][r] = all;
-        group_barrier(3, 256);
-        all = errors[0][r] + errors[1][r];
-      }
+      errors[team][r] = all;  // two or four threads worked on the row
+      if (OWN == 1) group_barrier(7, 512);
+      else group_barrier(1 + y, 256);
+      all = OWN == 1 ? (errors[0][r] + errors[1][r]) + (errors[2][r] + errors[3][r]) : errors[2 * y][r] + errors[2 * y + 1][r];
+      float* column = sums + team * 64 + (r & 63);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int bucket = p.buckets[s ? 2 * p.reach : 0];
-        if (bucket < p.num_buckets && row_ok) sums[bucket * 256 + tid] += far[s] - all * far_p[s];
+      for (int turn = 0; turn < 2; ++turn) {
+        if ((r >= 64) == (turn == 1)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int bucket = p.buckets[e ? 2 * p.reach : 0];
+            if (bucket < p.num_buckets && row_ok) column[bucket * 256] += far[e] - all * far_p[e];
+          }
+        }
+        if (OWN == 1) group_barrier(7, 512);
+        else group_barrier(1 + y, 256);
       }
-      if (OWN == 1) group_barrier(3, 256);
-      else group_barrier(1 + y, 128);
       const int tiles = (p.M + kTcRows - 1) / kTcRows;
       if (my_row0 < p.M) {
         float* part = p.dbias_part + (((long long)b * p.H + my_head) * tiles + my_row0 / kTcRows) * p.num_buckets;
         const int base = OWN == 2 ? 128 * y : 0, span = OWN == 2 ? 128 : 256;
-        for (int i = OWN == 2 ? warp & 3 : warp; i < p.num_buckets; i += OWN == 2 ? 4 : 8) {
+        for (int i = OWN == 2 ? warp & 7 : warp; i < p.num_buckets; i += OWN == 2 ? 8 : 16) {
           float v = 0.f;
           for (int e = lane; e < span; e += 32) v += sums[i * 256 + base + e];
           v = warp_sum(v);
@@ -481,10 +498,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       }
     };
     if (DKV) {
-      if (OWN == 2 || y == 0) rows_out(p.dk, p.dk_rows, 0, 0, D, p.scale);
-      if (OWN == 2 || y == 1) rows_out(p.dv, p.dv_rows, 1, 0, D, 1.f);
+      // two tiles: a half of the group for each gradient; one: a group for each, a half of its channels each
+      if (OWN == 2 ? half == 0 : y == 0) rows_out(p.dk, p.dk_rows, 0, OWN == 2 ? 0 : half * (D / 2), OWN == 2 ? D : (half + 1) * (D / 2), p.scale);
+      else rows_out(p.dv, p.dv_rows, 1, OWN == 2 ? 0 : half * (D / 2), OWN == 2 ? D : (half + 1) * (D / 2), 1.f);
     } else {
-      rows_out(p.dq, p.dq_rows, 0, OWN == 2 ? 0 : y * (D / 2), OWN == 2 ? D : (y + 1) * (D / 2), p.scale);
+      constexpr int share = OWN == 2 ? D / 2 : D / 4;
+      const int first_channel = (OWN == 2 ? half : team) * share;
+      rows_out(p.dq, p.dq_rows, 0, first_channel, first_channel + share, p.scale);
     }
     tc_fence_before_sync();
   }
@@ -498,8 +518,8 @@ int launch(const DenseTcParams& tc, cudaStream_t stream) {
   const DenseParams& p = tc.p;
   using Sh = BwdShape<D, TABLE && !DKV>;
   auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
-  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 2 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0);
-  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 2 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0);
+  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 4 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0);
+  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 4 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0);
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   const int heads = DKV ? p.K : p.H;
