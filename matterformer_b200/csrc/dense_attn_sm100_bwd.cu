@@ -1,13 +1,13 @@
 // Dense attention with a learned bias by the offset on tcgen05, backward: head size 64 and 128, bf16 and fp16.  The probabilities are formed again.
 //
-// Two passes of one skeleton, a CTA owns tiles of 128 rows and walks over its partners in tiles of 64:
+// Two passes of one skeleton, a CTA owns a tile of 128 rows and walks over its partners in tiles of 64:
 //   DQ  : owners = queries, partners = keys     S = Q K^T, dP = dO V^T       -> dS        -> dQ += dS K
 //   DKV : owners = keys,    partners = queries  S^T = K Q^T, dP^T = V dO^T   -> P^T, dS^T -> dV += P^T dO, dK += dS^T Q
 // Seven products instead of the five of a single pass, but every sum has one owner and a fixed order, and nothing is added up in memory.
-// Two threads share a row, half of a step's columns each; P and dS are packed to 16 bits over the columns that S and dP had and are the A operands of the second products, whose sums
-// stay in tensor memory over the whole walk.  Two buffers for S and dP, each with a group of eight warps: while one group works the tensor cores
-// fill the other's buffer.  At head size 64 a CTA owns two tiles that share the partners they read, a buffer each; at 128, where the sums of two
-// tiles do not fit tensor memory, one tile, and the groups take its steps in turn.
+// Two threads share a row, half of a step's columns each; P and dS are packed to 16 bits over the columns that S and dP had and are the A operands of the
+// second products, whose sums stay in tensor memory over the whole walk.  Two groups of eight warps take the steps in turn, and S and dP have three
+// buffers (two where the sums leave no room: DKV at head size 128), so that a group that is done with a step finds the next one ready: with a buffer for each group
+// it waited for the second product of its step and the first ones of its next, and the pipes stood still (two cells of 4096 tokens 219 + 256 us).
 //
 // The table's gradient (DQ): steps whose offsets all fall into one bucket add up in a register; in the others dS goes through shared memory and threads sum
 // along its diagonals, each into a column of sums of its own.  dS = P (dP - delta) with delta from rounded outputs; the row sums of dS, which are zero but for the error in
@@ -27,27 +27,28 @@ constexpr int kOwnerWarps = 16, kBwdThreads = (kOwnerWarps + 4) * 32, kPart = 64
 constexpr int kRegAux = 56, kRegOwner = 104;
 static_assert(kOwnerWarps * kRegOwner + 4 * kRegAux <= (kOwnerWarps + 4) * 96, "register hand-over exceeds the CTA's pool");
 
-template <int D, bool SUMS>
+template <int D, bool DKV, bool SUMS>
 struct BwdShape {
-  static constexpr int kOwn = D == 64 ? 2 : 1;  // owner tiles
   static constexpr int kChunks = D / 64, kTile = kChunks * kTcRows * 128, kPartTile = kChunks * kPart * 128;
-  static constexpr int kStages = D == 64 && !SUMS ? 4 : 3;
-  static constexpr int kOffA = 0, kOffB = kOwn * kTile, kOffRing = 2 * kOwn * kTile, kSmem = kOffRing + kStages * 2 * kPartTile;
+  static constexpr int kBuffers = D == 128 && DKV ? 2 : 3, kColSums = 128 * kBuffers;
+  static_assert(kColSums + (DKV ? 2 : 1) * D <= 512, "");
+  static constexpr int kStages = D == 64 ? (SUMS ? 5 : 6) : SUMS ? 3 : 4;
+  static constexpr int kOffA = 0, kOffB = kTile, kOffRing = 2 * kTile, kSmem = kOffRing + kStages * 2 * kPartTile;
   static constexpr int kMostBuckets = D == 64 ? 64 : 32;  // whose sums fit beside that
-  static constexpr int kDiagonals = D == 64 ? 16 : 8;  // columns of dS that 128 threads sum along their diagonals at a time
+  static constexpr int kDiagonals = D == 64 ? 16 : 8;     // columns of dS that 128 threads sum along their diagonals at a time
   static constexpr int kDiagonalBytes = kTcRows * (kDiagonals + 1) * 4;
 };
 
 template <typename T, int D, bool DKV, bool TABLE>
 __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const __grid_constant__ DenseTcParams tc) {
-  using Sh = BwdShape<D, TABLE && !DKV>;
-  constexpr int OWN = Sh::kOwn, S = Sh::kStages;
+  using Sh = BwdShape<D, DKV, TABLE && !DKV>;
+  constexpr int S = Sh::kStages, BUFFERS = Sh::kBuffers;
   const DenseParams& p = tc.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* diagonals = reinterpret_cast<float*>(smem + Sh::kSmem);  // [2 groups][2 halves][128 rows][kDiagonals + 1]
   float* sums = reinterpret_cast<float*>(smem + Sh::kSmem + 4 * Sh::kDiagonalBytes);  // [num_buckets][4 halves of groups][64]
-  __shared__ uint64_t bar_own, bar_full[S], bar_free[S], bar_clean[S], bar_s[2], bar_p[2], bar_o, bar_drain;
+  __shared__ uint64_t bar_own, bar_full[S], bar_free[S], bar_clean[S], bar_s[BUFFERS], bar_p[BUFFERS], bar_o, bar_drain;
   __shared__ uint32_t tmem_base;
   __shared__ float table[TABLE ? 2 : 1][TABLE ? kTableEntries : 1], offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
   __shared__ uint8_t offset_buckets[TABLE && !DKV ? 2 : 1][2][TABLE && !DKV ? 256 : 1];
@@ -56,52 +57,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // ---- which rows
-  const int group = p.H / p.K;
-  const bool by_head = OWN == 2 && !DKV && group % 2 == 0;  // two query heads of a group, otherwise neighbouring tiles
-  const int heads = DKV ? p.K : p.H, units = p.B * (by_head ? heads / 2 : heads), row_blocks = gridDim.x / units;
-  const int unit = p.causal ? blockIdx.x % units : blockIdx.x / row_blocks;
-  const int rb = !p.causal ? blockIdx.x % row_blocks : DKV ? blockIdx.x / units : row_blocks - 1 - (int)(blockIdx.x / units);  // the longest walks first
-  const int b = unit / (units / p.B), hu = unit % (units / p.B);
+  const int group = p.H / p.K, heads = DKV ? p.K : p.H, units = p.B * heads, tiles = gridDim.x / units;
+  const int unit = p.causal ? blockIdx.x % units : blockIdx.x / tiles;
+  const int tile_at = !p.causal ? blockIdx.x % tiles : DKV ? blockIdx.x / units : tiles - 1 - (int)(blockIdx.x / units);  // the longest walks first
+  const int b = unit / heads, head = unit % heads, row0 = tile_at * kTcRows, kh = DKV ? head : head / group;
   const DenseLengths len = dense_lengths(p, b);
   const int own_rows = DKV ? len.nk : len.nq, own_all = DKV ? p.N : p.M;
-  int head[OWN], row0[OWN], first[OWN], last[OWN];  // partner steps [first, last) of a head
-#pragma unroll
-  for (int x = 0; x < OWN; ++x) {
-    head[x] = by_head ? 2 * hu + x : hu;
-    row0[x] = by_head || OWN == 1 ? rb * kTcRows : (2 * rb + x) * kTcRows;
-    first[x] = 0, last[x] = 0;
-    if (row0[x] < own_rows) {
-      if (DKV) first[x] = dense_first(p, len, row0[x]) / kPart, last[x] = (len.nq + kPart - 1) / kPart;
-      else last[x] = (dense_limit(p, len, min(row0[x] + kTcRows, len.nq) - 1) + kPart - 1) / kPart;
-      if (last[x] <= first[x]) first[x] = last[x] = 0;
-    }
+  int from = 0, until = 0;  // partner steps of a head
+  if (row0 < own_rows) {
+    if (DKV) from = dense_first(p, len, row0) / kPart, until = (len.nq + kPart - 1) / kPart;
+    else until = (dense_limit(p, len, min(row0 + kTcRows, len.nq) - 1) + kPart - 1) / kPart;
   }
-  int from = first[0], until = last[0];
-  if (OWN == 2) {
-    if (last[OWN - 1] > first[OWN - 1]) {
-      from = last[0] > first[0] ? min(from, first[OWN - 1]) : first[OWN - 1];
-      until = max(until, last[OWN - 1]);
-    }
-  }
-  const int per_head = until - from, steps = DKV ? per_head * group : per_head;
-  auto seen_by = [&](int x, int t) {  // whether tile x works on step t
-    const int s = from + (DKV ? t % per_head : t);
-    return s >= (x ? first[OWN - 1] : first[0]) && s < (x ? last[OWN - 1] : last[0]);
-  };
+  const int per_head = max(0, until - from), steps = DKV ? per_head * group : per_head;
   auto partner_row = [&](int t) { return (from + (DKV ? t % per_head : t)) * kPart; };
-  const int kh = DKV ? hu : head[0] / group;
   auto partner_head = [&](int t) { return DKV ? kh * group + t / per_head : kh; };
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.key_mask_batch : nullptr;
   const int part_rows = DKV ? len.nq : len.nk, part_all = DKV ? p.M : p.N;
   const bool cleaning = DKV || mask || part_rows < min(part_all, until * kPart);
 
   if (steps == 0) {
-    for (int i = tid; i < OWN * kTcRows; i += kBwdThreads) {
-      const int x = i / kTcRows, row = (x ? row0[OWN - 1] : row0[0]) + i % kTcRows, h = x ? head[OWN - 1] : head[0];
-      if (row >= own_all) continue;
+    if (tid < kTcRows && row0 + tid < own_all) {
+      const int row = row0 + tid;
       auto clear = [&](void* base, const DenseRows& rows) {
         if (!base) return;
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(base) + rows.at(b, h, row));
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(base) + rows.at(b, head, row));
         for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
       };
       if (DKV) {
@@ -109,17 +88,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         clear(p.dv, p.dv_rows);
       } else {
         clear(p.dq, p.dq_rows);
-        p.delta[((long long)b * p.H + h) * p.M + row] = 0.f;
+        p.delta[((long long)b * p.H + head) * p.M + row] = 0.f;
       }
     }
-    if (TABLE && !DKV && p.dbias_part) {
-      const int tiles = (p.M + kTcRows - 1) / kTcRows;
-      for (int x = 0; x < OWN; ++x) {
-        const int r0 = x ? row0[OWN - 1] : row0[0], h = x ? head[OWN - 1] : head[0];
-        if (r0 < p.M)
-          for (int i = tid; i < p.num_buckets; i += kBwdThreads) p.dbias_part[(((long long)b * p.H + h) * tiles + r0 / kTcRows) * p.num_buckets + i] = 0.f;
-      }
-    }
+    if (TABLE && !DKV && p.dbias_part)
+      for (int i = tid; i < p.num_buckets; i += kBwdThreads) p.dbias_part[((long long)unit * tiles + tile_at) * p.num_buckets + i] = 0.f;
     return;
   }
 
@@ -127,7 +100,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     auto init = [&](uint64_t* bar, int count, int kind) { mbar_init(bar, count + (tc.waits.withheld == kind)); };
     init(&bar_own, 1, 0);
     for (int i = 0; i < S; ++i) init(&bar_full[i], 1, 0), init(&bar_free[i], 1, 1), init(&bar_clean[i], 1, 4);
-    for (int x = 0; x < 2; ++x) init(&bar_s[x], 1, 2), init(&bar_p[x], 8, 3);
+    for (int x = 0; x < BUFFERS; ++x) init(&bar_s[x], 1, 2), init(&bar_p[x], 8, 3);
     init(&bar_o, 1, 2);
     mbar_init(&bar_drain, 1);
     mbar_fence_init();
@@ -146,11 +119,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   auto wait_on = [&](uint64_t* bar, uint32_t phase) {
     if (!bad) bad = !mbar_wait_for(bar, phase & 1, tc.waits.limit);
   };
-  // columns: S and dP of buffer y at 128 y and 128 y + 64; the sums from 256 on
-  auto col_sum = [&](int x, int which) { return 256u + (DKV ? 2 * D * x + D * which : D * x); };
-  const int jobs = OWN * steps;  // job n: tile n & 1 of step n / 2, or step n; buffer and group n & 1
-  auto step_of = [&](int n) { return OWN == 2 ? n >> 1 : n; };
-  auto valid = [&](int n) { return OWN == 1 || seen_by(n & 1, n >> 1); };
+  // columns: S and dP of buffer i at 128 i and 128 i + 64, then the sums
+  auto col_sum = [&](int which) { return (uint32_t)(Sh::kColSums + D * which); };
 
   if (warp >= kOwnerWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegAux));
@@ -162,17 +132,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         tma_prefetch_map(own_b);
         tma_prefetch_map(part_a);
         tma_prefetch_map(part_b);
-        int own = 0;
-        for (int x = 0; x < OWN; ++x) own += last[x] > first[x];
-        mbar_arrive_expect_tx(&bar_own, own * 2 * Sh::kTile);
-        for (int x = 0; x < OWN; ++x)
-          if (last[x] > first[x])
-            for (int c = 0; c < Sh::kChunks; ++c)
-              for (int half = 0; half < 2; ++half) {  // (boxes have 64 rows)
-                const uint32_t at = x * Sh::kTile + (c * kTcRows + half * 64) * 128;
-                tma_box(smem_u32(smem + Sh::kOffA) + at, own_a, c * 64, row0[x] + half * 64, head[x], b, &bar_own);
-                tma_box(smem_u32(smem + Sh::kOffB) + at, own_b, c * 64, row0[x] + half * 64, head[x], b, &bar_own);
-              }
+        mbar_arrive_expect_tx(&bar_own, 2 * Sh::kTile);
+        for (int c = 0; c < Sh::kChunks; ++c)
+          for (int half = 0; half < 2; ++half) {  // (boxes have 64 rows)
+            const uint32_t at = (c * kTcRows + half * 64) * 128;
+            tma_box(smem_u32(smem + Sh::kOffA) + at, own_a, c * 64, row0 + half * 64, head, b, &bar_own);
+            tma_box(smem_u32(smem + Sh::kOffB) + at, own_b, c * 64, row0 + half * 64, head, b, &bar_own);
+          }
         int t = 0;
         for (; t < steps; ++t) {
           const int stage = t % S;
@@ -195,45 +161,40 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       if (elect_one()) {
         const uint32_t l_a = make_desc_lo(smem_u32(smem + Sh::kOffA), 0), l_b = make_desc_lo(smem_u32(smem + Sh::kOffB), 0);
         const uint32_t l_ring = make_desc_lo(smem_u32(smem + Sh::kOffRing), 0), l_ring_mn = make_desc_lo(smem_u32(smem + Sh::kOffRing), kPart * 128);
-        constexpr uint32_t kTile = Sh::kTile >> 4, kPartTile = Sh::kPartTile >> 4, kChunk = (kTcRows * 128) >> 4, kPartChunk = (kPart * 128) >> 4;
+        constexpr uint32_t kPartTile = Sh::kPartTile >> 4, kChunk = (kTcRows * 128) >> 4, kPartChunk = (kPart * 128) >> 4;
         constexpr uint32_t idesc_s = make_idesc_16<T>(kTcRows, kPart, false, false), idesc_o = make_idesc_16<T>(kTcRows, D, false, true);
-        auto logits = [&](int n) {
-          const int t = step_of(n), stage = t % S, x = OWN == 2 ? n & 1 : 0;
+        auto logits = [&](int t, int buffer) {
+          const int stage = t % S;
           wait_on(cleaning ? &bar_clean[stage] : &bar_full[stage], t / S);
           tc_fence_after_sync();
-          const uint32_t part = l_ring + stage * 2 * kPartTile, col = tmem + 128 * (n & 1);
+          const uint32_t part = l_ring + stage * 2 * kPartTile, col = tmem + 128 * buffer;
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
-            umma_ss_lo(col, l_a + x * kTile + (ks >> 2) * kChunk + (ks & 3) * 2, part + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
+            umma_ss_lo(col, l_a + (ks >> 2) * kChunk + (ks & 3) * 2, part + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
-            umma_ss_lo(col + 64, l_b + x * kTile + (ks >> 2) * kChunk + (ks & 3) * 2, part + kPartTile + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
-          umma_commit(&bar_s[n & 1]);
+            umma_ss_lo(col + 64, l_b + (ks >> 2) * kChunk + (ks & 3) * 2, part + kPartTile + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
+          umma_commit(&bar_s[buffer]);
         };
         wait_on(&bar_own, 0);
-        int done[2] = {0, 0}, sum_started[2] = {0, 0};
-        for (int n = 0; n < min(2, jobs); ++n)
-          if (valid(n)) logits(n);
+        for (int t = 0; t < min(BUFFERS, steps); ++t) logits(t, t);
 #pragma unroll 1
-        for (int n0 = 0; n0 < jobs; n0 += 2) {
+        for (int t0 = 0; t0 < steps; t0 += BUFFERS) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int n = n0 + y, t = step_of(n), stage = t % S, x = OWN == 2 ? y : 0;
-            if (n >= jobs) break;
-            if (valid(n)) {
-              wait_on(&bar_p[y], done[y]++);
-              tc_fence_after_sync();
-              const uint32_t part = l_ring_mn + stage * 2 * kPartTile, col = tmem + 128 * y;
+          for (int buffer = 0; buffer < BUFFERS; ++buffer) {
+            const int t = t0 + buffer, stage = t % S;
+            if (t >= steps) break;
+            wait_on(&bar_p[buffer], t / BUFFERS);
+            tc_fence_after_sync();
+            const uint32_t part = l_ring_mn + stage * 2 * kPartTile, col = tmem + 128 * buffer;
 #pragma unroll
-              for (int kg = 0; kg < kPart / 16; ++kg) {
-                const uint32_t packed = 32 * (kg >> 1) + 8 * (kg & 1);
-                if (DKV) umma_ts_lo(tmem + col_sum(x, 1), col + packed, part + kPartTile + 128 * kg, idesc_o, sum_started[x] || kg > 0);
-                umma_ts_lo(tmem + col_sum(x, 0), col + 64 + packed, part + 128 * kg, idesc_o, sum_started[x] || kg > 0);
-              }
-              sum_started[x] = 1;
+            for (int kg = 0; kg < kPart / 16; ++kg) {
+              const uint32_t packed = 32 * (kg >> 1) + 8 * (kg & 1);
+              if (DKV) umma_ts_lo(tmem + col_sum(1), col + packed, part + kPartTile + 128 * kg, idesc_o, t > 0 || kg > 0);
+              umma_ts_lo(tmem + col_sum(0), col + 64 + packed, part + 128 * kg, idesc_o, t > 0 || kg > 0);
             }
-            if (OWN == 1 || y == 1) umma_commit(&bar_free[stage]);
-            if (n + 2 < jobs && valid(n + 2)) logits(n + 2);
+            umma_commit(&bar_free[stage]);
+            if (t + BUFFERS < steps) logits(t + BUFFERS, buffer);
           }
         }
         umma_commit(&bar_o);
@@ -273,23 +234,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   } else {
     // ------------------------------------------------------------------ row owners
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegOwner));
-    const int y = warp >> 3, half = warp >> 2 & 1, x = OWN == 2 ? y : 0, r = tid & 127;  // group (and buffer), half of the columns, tile
+    const int y = warp >> 3, half = warp >> 2 & 1, r = tid & 127;  // group, half of the columns, row
     const int c0 = half * kCols, pair = tid & 255, team = warp >> 2;  // the 256 threads of a group are pairs of 128
-    const int my_head = x ? head[OWN - 1] : head[0], my_row0 = x ? row0[OWN - 1] : row0[0];
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, col = tmem + lanes + 128 * y;
-    const int row = my_row0 + r;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int row = row0 + r;
     const bool row_ok = row < own_rows;
     const float sc2 = p.scale * kDenseLog2e;
     float lse = 0.f, delta = 0.f;
     // visible partners of this row: [lo, hi) at DKV and DQ; a row that is none may see what it wants
     int lo = INT32_MIN, hi = INT32_MAX;
     if (!DKV) {
-      const long long stat = ((long long)b * p.H + my_head) * p.M;
+      const long long stat = ((long long)b * p.H + head) * p.M;
       if (row_ok) {
         hi = dense_limit(p, len, row);
         lse = p.lse[stat + row];
-        const uint4* go = reinterpret_cast<const uint4*>(static_cast<const T*>(p.grad_out) + p.go_rows.at(b, my_head, row));
-        const uint4* o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + p.out_rows.at(b, my_head, row));
+        const uint4* go = reinterpret_cast<const uint4*>(static_cast<const T*>(p.grad_out) + p.go_rows.at(b, head, row));
+        const uint4* o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + p.out_rows.at(b, head, row));
 #pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
           const uint4 u = go[c], w = o[c];
@@ -301,25 +261,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
           }
         }
       }
-      if (row < p.M && half == 0 && (OWN == 2 || y == 0)) p.delta[stat + row] = delta;
+      if (row < p.M && team == 0) p.delta[stat + row] = delta;
     } else if (row_ok) {
       lo = dense_first(p, len, row);
     }
     const int tile_lo = __reduce_max_sync(0xffffffffu, lo), tile_hi = __reduce_min_sync(0xffffffffu, hi);
     const bool table_grad = TABLE && !DKV && p.dbias_part;
     float far[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, all = 0.f;  // sums of dS and of P over steps of one bucket (offsets below, above), of dS over all
-    int fills = 0, done = 0, table_head = -1;
+    int fills = 0, table_head = -1;
     float far_bias[2] = {0.f, 0.f};  // of the offsets -reach and reach, and beyond
-    for (int t = OWN == 2 ? 0 : y; t < steps; t += OWN == 2 ? 1 : 2) {
-      if (OWN == 2 && !seen_by(x, t)) continue;
-      const int at = partner_row(t), stage = t % S;
+    for (int t = y; t < steps; t += 2) {
+      const int at = partner_row(t), stage = t % S, buffer = t % BUFFERS;
+      const uint32_t col = tmem + lanes + 128 * buffer;
       float one = 0.f;
       const float* near = nullptr;  // bias of the thread's column c at near[c] (DQ), near[-c] (DKV)
       const uint8_t* near_bucket = nullptr;
       int side = 0;
       if (TABLE) {
-        const int start = (DKV ? my_row0 - at - (kPart - 1) : at - my_row0 - (kTcRows - 1)) - len.shift;  // the offset of entry 0
-        const int h = DKV ? partner_head(t) : my_head;
+        const int start = (DKV ? row0 - at - (kPart - 1) : at - row0 - (kTcRows - 1)) - len.shift;  // the offset of entry 0
+        const int h = DKV ? partner_head(t) : head;
         if (h != table_head) {
           if (table_head >= 0) group_barrier(1 + y, 256);
           table[y][pair] = dense_bias_entry(p, pair, h);
@@ -346,7 +306,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         const int key = at + c0 + lane;
         seen = __ballot_sync(0xffffffffu, key < len.nk && mask[key] != 0);
       }
-      wait_on(&bar_s[y], done++);
+      wait_on(&bar_s[buffer], t / BUFFERS);
       tc_fence_after_sync();
       float z[kCols], d[kCols];
       tmem_ld32(col + c0, *reinterpret_cast<uint32_t(*)[32]>(&z[0]));
@@ -397,7 +357,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_p[y]);
+      if (lane == 0) mbar_arrive(&bar_p[buffer]);
       if (table_grad) {
         float2 u[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -444,10 +404,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       }
     }
     if (table_grad) {
-      errors[team][r] = all;  // two or four threads worked on the row
-      if (OWN == 1) group_barrier(7, 512);
-      else group_barrier(1 + y, 256);
-      all = OWN == 1 ? (errors[0][r] + errors[1][r]) + (errors[2][r] + errors[3][r]) : errors[2 * y][r] + errors[2 * y + 1][r];
+      errors[team][r] = all;  // four threads worked on the row
+      group_barrier(7, 512);
+      all = (errors[0][r] + errors[1][r]) + (errors[2][r] + errors[3][r]);
       float* column = sums + team * 64 + (r & 63);
 #pragma unroll
       for (int turn = 0; turn < 2; ++turn) {
@@ -458,35 +417,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
             if (bucket < p.num_buckets && row_ok) column[bucket * 256] += far[e] - all * far_p[e];
           }
         }
-        if (OWN == 1) group_barrier(7, 512);
-        else group_barrier(1 + y, 256);
+        group_barrier(7, 512);
       }
-      const int tiles = (p.M + kTcRows - 1) / kTcRows;
-      if (my_row0 < p.M) {
-        float* part = p.dbias_part + (((long long)b * p.H + my_head) * tiles + my_row0 / kTcRows) * p.num_buckets;
-        const int base = OWN == 2 ? 128 * y : 0, span = OWN == 2 ? 128 : 256;
-        for (int i = OWN == 2 ? warp & 7 : warp; i < p.num_buckets; i += OWN == 2 ? 8 : 16) {
-          float v = 0.f;
-          for (int e = lane; e < span; e += 32) v += sums[i * 256 + base + e];
-          v = warp_sum(v);
-          if (lane == 0) part[i] = v;
-        }
+      float* part = p.dbias_part + ((long long)unit * tiles + tile_at) * p.num_buckets;
+      for (int i = warp; i < p.num_buckets; i += kOwnerWarps) {
+        float v = 0.f;
+        for (int e = lane; e < 256; e += 32) v += sums[i * 256 + e];
+        v = warp_sum(v);
+        if (lane == 0) part[i] = v;
       }
     }
 
     // ---- rows out: zeros for what is no row
     wait_on(&bar_o, 0);
     tc_fence_after_sync();
-    const bool any = x ? last[OWN - 1] > first[OWN - 1] : last[0] > first[0];
-    const bool real = row_ok && any && (!DKV || !mask || mask[row]);
+    const bool real = row_ok && (!DKV || !mask || mask[row]);
     auto rows_out = [&](void* base, const DenseRows& rows, int which, int c0, int c1, float mul) {
 #pragma unroll 1
       for (int c = c0; c < c1; c += 32) {
         uint32_t o[32];
-        tmem_ld32(tmem + lanes + col_sum(x, which) + c, o);
+        tmem_ld32(tmem + lanes + col_sum(which) + c, o);
         tmem_ld_wait();
         if (base && row < own_all) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(base) + rows.at(b, my_head, row) + c);
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(base) + rows.at(b, head, row) + c);
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint32_t v[4];
@@ -497,13 +450,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         }
       }
     };
-    if (DKV) {
-      // two tiles: a half of the group for each gradient; one: a group for each, a half of its channels each
-      if (OWN == 2 ? half == 0 : y == 0) rows_out(p.dk, p.dk_rows, 0, OWN == 2 ? 0 : half * (D / 2), OWN == 2 ? D : (half + 1) * (D / 2), p.scale);
-      else rows_out(p.dv, p.dv_rows, 1, OWN == 2 ? 0 : half * (D / 2), OWN == 2 ? D : (half + 1) * (D / 2), 1.f);
-    } else {
-      constexpr int share = OWN == 2 ? D / 2 : D / 4;
-      const int first_channel = (OWN == 2 ? half : team) * share;
+    if (DKV) {  // a group for each gradient
+      if (y == 0) rows_out(p.dk, p.dk_rows, 0, half * (D / 2), (half + 1) * (D / 2), p.scale);
+      else rows_out(p.dv, p.dv_rows, 1, half * (D / 2), (half + 1) * (D / 2), 1.f);
+    } else if (D == 128 || half == 0) {  // a quarter of the channels for 128 threads, or a half
+      constexpr int share = 32;
+      const int first_channel = (D == 128 ? team : y) * share;
       rows_out(p.dq, p.dq_rows, 0, first_channel, first_channel + share, p.scale);
     }
     tc_fence_before_sync();
@@ -516,16 +468,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
 template <typename T, int D, bool DKV, bool TABLE>
 int launch(const DenseTcParams& tc, cudaStream_t stream) {
   const DenseParams& p = tc.p;
-  using Sh = BwdShape<D, TABLE && !DKV>;
+  using Sh = BwdShape<D, DKV, TABLE && !DKV>;
   auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
   constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 4 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0);
   const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 4 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0);
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
-  const int heads = DKV ? p.K : p.H;
-  const bool by_head = Sh::kOwn == 2 && !DKV && (p.H / p.K) % 2 == 0;
-  const long long tiles = ((DKV ? p.N : p.M) + kTcRows - 1) / kTcRows;
-  const long long blocks = by_head ? tiles * p.B * (heads / 2) : (tiles + Sh::kOwn - 1) / Sh::kOwn * p.B * heads;
+  const long long blocks = (long long)(((DKV ? p.N : p.M) + kTcRows - 1) / kTcRows) * p.B * (DKV ? p.K : p.H);
   kernel<<<(unsigned)blocks, kBwdThreads, smem, stream>>>(tc);
   MF_CHECK_LAUNCH("dense attention backward on tcgen05");
   return MF_OK;
