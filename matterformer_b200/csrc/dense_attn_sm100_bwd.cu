@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   __shared__ uint32_t tmem_base;
   __shared__ float table[TABLE ? 2 : 1][TABLE ? kTableEntries : 1], offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
   __shared__ uint8_t offset_buckets[TABLE && !DKV ? 2 : 1][2][TABLE && !DKV ? 256 : 1];
-  __shared__ __align__(16) float2 stats[DKV ? S : 1][DKV ? kPart : 1];  // -lse and delta of the partners
+  __shared__ __align__(16) float stats[DKV ? S : 1][2][DKV ? kPart : 4];  // of the partners: -lse (and the bias where all offsets of the step have one), -delta
   __shared__ float errors[TABLE && !DKV ? 4 : 1][TABLE && !DKV ? 128 : 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   const int per_head = max(0, until - from), steps = DKV ? per_head * group : per_head;
   auto partner_row = [&](int t) { return (from + (DKV ? t % per_head : t)) * kPart; };
   auto partner_head = [&](int t) { return DKV ? kh * group + t / per_head : kh; };
+  auto first_offset = [&](int at) { return (DKV ? row0 - at - (kPart - 1) : at - row0 - (kTcRows - 1)) - len.shift; };  // of the pairs of a step
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.key_mask_batch : nullptr;
   const int part_rows = DKV ? len.nq : len.nk, part_all = DKV ? p.M : p.N;
   const bool cleaning = DKV || mask || part_rows < min(part_all, until * kPart);
@@ -205,15 +206,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     } else if (warp == kOwnerWarps + 2) {
       // ---------------------------------------------------------------- partners that are none become zeros; log-sum-exp and delta of queries
       if (cleaning) {
+        int bias_head = -1;
+        float far_bias[2] = {0.f, 0.f};
         for (int t = 0; t < steps; ++t) {
           const int stage = t % S, at = partner_row(t);
           wait_on(&bar_full[stage], t / S);
           if (DKV) {
-            const long long stat = ((long long)b * p.H + partner_head(t)) * p.M;
+            const int h = partner_head(t);
+            const long long stat = ((long long)b * p.H + h) * p.M;
+            float one = 0.f;
+            if (TABLE) {
+              if (h != bias_head) {
+                bias_head = h;
+                far_bias[0] = dense_bias_entry(p, p.buckets[0], h), far_bias[1] = dense_bias_entry(p, p.buckets[2 * p.reach], h);
+              }
+              const int start = first_offset(at);
+              one = start + kSpan - 1 <= -p.reach ? far_bias[0] : start >= p.reach ? far_bias[1] : 0.f;
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int c = lane + 32 * e, i = at + c;
-              stats[stage][c] = i < len.nq ? make_float2(-p.lse[stat + i], p.delta[stat + i]) : make_float2(-INFINITY, 0.f);
+              stats[stage][0][c] = i < len.nq ? one - p.lse[stat + i] : -INFINITY;
+              stats[stage][1][c] = i < len.nq ? -p.delta[stat + i] : 0.f;
             }
           }
           const int rows = min(kPart, part_all - at);  // what lies behind the tensor is zeros already
@@ -278,14 +292,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       const uint8_t* near_bucket = nullptr;
       int side = 0;
       if (TABLE) {
-        const int start = (DKV ? row0 - at - (kPart - 1) : at - row0 - (kTcRows - 1)) - len.shift;  // the offset of entry 0
+        const int start = first_offset(at);  // entry e: the offset start + e
         const int h = DKV ? partner_head(t) : head;
         if (h != table_head) {
           if (table_head >= 0) group_barrier(1 + y, 256);
           table[y][pair] = dense_bias_entry(p, pair, h);
           group_barrier(1 + y, 256);
           table_head = h;
-          far_bias[0] = table[y][p.buckets[0]], far_bias[1] = table[y][p.buckets[2 * p.reach]];
+          if (!DKV) far_bias[0] = table[y][p.buckets[0]], far_bias[1] = table[y][p.buckets[2 * p.reach]];
         }
         if (start + kSpan - 1 <= -p.reach || start >= p.reach) {
           side = start >= p.reach;
@@ -312,29 +326,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       tmem_ld32(col + c0, *reinterpret_cast<uint32_t(*)[32]>(&z[0]));
       tmem_ld32(col + 64 + c0, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
       tmem_ld_wait();
-      if (DKV) {
+      auto form = [&](auto biased) {  // p into z, dP - delta into d
+        const float2 less = make_float2(one - lse, one - lse), off = make_float2(-delta, -delta), by = make_float2(sc2, sc2);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 2) {
-          const float4 st = *reinterpret_cast<const float4*>(&stats[stage][c0 + c]);
-          float2 minus = make_float2(st.x, st.z);
-          if (TABLE) minus = add2(minus, near ? make_float2(near[-c], near[-c - 1]) : make_float2(one, one));
-          const float2 e = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), minus);
-          z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
-          const float2 v = add2(make_float2(d[c], d[c + 1]), make_float2(-st.y, -st.w));
-          d[c] = v.x, d[c + 1] = v.y;
-        }
-      } else {
-        const float less = one - lse;
+        for (int c = 0; c < kCols; c += 4) {
+          float2 minus[2] = {less, less}, shift[2] = {off, off};
+          if (DKV) {
+            const float4 m = *reinterpret_cast<const float4*>(&stats[stage][0][c0 + c]), n = *reinterpret_cast<const float4*>(&stats[stage][1][c0 + c]);
+            minus[0] = make_float2(m.x, m.y), minus[1] = make_float2(m.z, m.w), shift[0] = make_float2(n.x, n.y), shift[1] = make_float2(n.z, n.w);
+          }
 #pragma unroll
-        for (int c = 0; c < kCols; c += 2) {
-          float2 minus = make_float2(less, less);
-          if (TABLE && near) minus = add2(minus, make_float2(near[c], near[c + 1]));
-          const float2 e = fma2(make_float2(z[c], z[c + 1]), make_float2(sc2, sc2), minus);
-          z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
-          const float2 v = add2(make_float2(d[c], d[c + 1]), make_float2(-delta, -delta));
-          d[c] = v.x, d[c + 1] = v.y;
+          for (int i = 0; i < 2; ++i) {
+            const int at_c = c + 2 * i;
+            if constexpr (decltype(biased)::value)
+              minus[i] = add2(minus[i], make_float2(near[DKV ? -at_c : at_c], near[DKV ? -at_c - 1 : at_c + 1]));
+            const float2 e = fma2(make_float2(z[at_c], z[at_c + 1]), by, minus[i]);
+            z[at_c] = dense_exp2(e.x), z[at_c + 1] = dense_exp2(e.y);
+            const float2 v = add2(make_float2(d[at_c], d[at_c + 1]), shift[i]);
+            d[at_c] = v.x, d[at_c + 1] = v.y;
+          }
         }
-      }
+      };
+      if (TABLE && near) form(std::true_type{});
+      else form(std::false_type{});
       if (at < tile_lo || at + kPart > tile_hi || (!DKV && mask)) {
         const int a = lo == INT32_MIN ? -1 : lo - at - c0, e = hi == INT32_MAX ? kPart : hi - at - c0;
 #pragma unroll
