@@ -9,11 +9,14 @@
 // buffers (two where the sums leave no room: DKV at head size 128), so that a group that is done with a step finds the next one ready: with a buffer for each group
 // it waited for the second product of its step and the first ones of its next, and the pipes stood still (two cells of 4096 tokens 219 + 256 us).
 //
-// The table's gradient (DQ): steps whose offsets all fall into one bucket add up in a register; in the others dS goes through shared memory and threads sum
+// DKV wants the log-sum-exp and delta of the queries, its columns: they enter the products.  Each is three tf32 numbers, together as exact as fp32, in a further
+// piece of the contracted dimension, whose other operand is ones, so that S and dP arrive with them subtracted (from shared memory they took a fifth of the pass).
+//
+// The bias of every offset up to the map's reach lies in shared memory (a few KB), so that a step reads it at its own place.  The table's gradient (DQ): steps whose offsets all fall into one bucket add up in a register; in the others dS goes through shared memory and threads sum
 // along its diagonals, each into a column of sums of its own.  dS = P (dP - delta) with delta from rounded outputs; the row sums of dS, which are zero but for the error in
 // delta, correct what far buckets got: there thousands of P share one error, which would otherwise be the largest of that sum.
 //
-// Roles as in the forward kernel; the warp that clears rows also brings the queries' log-sum-exp and delta for DKV.
+// Roles as in the forward kernel; the two warps that clear rows also bring the queries' log-sum-exp and delta for DKV.
 #include "dense_attn_sm100.cuh"
 
 namespace mf {
@@ -24,6 +27,7 @@ __device__ int32_t g_taken_status;
 __global__ void take_status_kernel(int word) { g_taken_status = atomicExch(&g_dense_status[word], 0); }
 
 constexpr int kOwnerWarps = 16, kBwdThreads = (kOwnerWarps + 4) * 32, kPart = 64, kCols = 32, kSpan = kTcRows + kPart - 1;
+constexpr int kMostReach = 512;  // of the map, whose bias lies in shared memory
 constexpr int kRegAux = 56, kRegOwner = 104;
 static_assert(kOwnerWarps * kRegOwner + 4 * kRegAux <= (kOwnerWarps + 4) * 96, "register hand-over exceeds the CTA's pool");
 
@@ -32,12 +36,35 @@ struct BwdShape {
   static constexpr int kChunks = D / 64, kTile = kChunks * kTcRows * 128, kPartTile = kChunks * kPart * 128;
   static constexpr int kBuffers = D == 128 && DKV ? 2 : 3, kColSums = 128 * kBuffers;
   static_assert(kColSums + (DKV ? 2 : 1) * D <= 512, "");
-  static constexpr int kStages = D == 64 ? (SUMS ? 5 : 6) : SUMS ? 3 : 4;
-  static constexpr int kOffA = 0, kOffB = kTile, kOffRing = 2 * kTile, kSmem = kOffRing + kStages * 2 * kPartTile;
+  static constexpr int kStages = D == 64 ? (SUMS ? 5 : 6) : SUMS || DKV ? 3 : 4;
+  static constexpr int kOnes = DKV ? kTcRows * 128 : 0, kStatTile = DKV ? kPart * 128 : 0;  // lines of 128 bytes, of which 32 and 64 are used
+  static constexpr int kOffA = 0, kOffB = kTile, kOffRing = 2 * kTile, kOffStats = kOffRing + kStages * 2 * kPartTile;
+  static constexpr int kOffOnes = kOffStats + kStages * kStatTile, kSmem = kOffOnes + kOnes;
   static constexpr int kMostBuckets = D == 64 ? 64 : 32;  // whose sums fit beside that
   static constexpr int kDiagonals = D == 64 ? 16 : 8;     // columns of dS that 128 threads sum along their diagonals at a time
   static constexpr int kDiagonalBytes = kTcRows * (kDiagonals + 1) * 4;
 };
+
+// D[tmem] += A[smem] * B[smem] of fp32 words, of which the tensor cores take the leading 11 bits of the mantissa; eight to an instruction
+__device__ __forceinline__ void umma_tf32_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %3, p;\n\t"
+      "}" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHiSw128)
+      : "memory");
+}
+// a number as the sum of three that tf32 holds
+__device__ __forceinline__ float4 three_parts(float v) {
+  const float a = __uint_as_float(__float_as_uint(v) & 0xffffe000u), r = v - a;
+  const float b = __uint_as_float(__float_as_uint(r) & 0xffffe000u);
+  return make_float4(a, b, r - b, 0.f);
+}
 
 template <typename T, int D, bool DKV, bool TABLE>
 __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const __grid_constant__ DenseTcParams tc) {
@@ -46,14 +73,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   const DenseParams& p = tc.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* diagonals = reinterpret_cast<float*>(smem + Sh::kSmem);  // [2 groups][2 halves][128 rows][kDiagonals + 1]
-  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem + 4 * Sh::kDiagonalBytes);  // [num_buckets][4 halves of groups][64]
+  // behind the tiles: [2 groups][2 halves][128 rows][kDiagonals + 1] | [num_buckets][4 halves of groups][64] | bias of the offsets from -reach - kSpan + 1 to
+  // reach + kSpan - 1 (DKV: for each group, they may be at different heads), their buckets
+  const bool table_grad = TABLE && !DKV && p.dbias_part;
+  const int offsets = TABLE ? 2 * p.reach + 2 * kSpan - 1 : 0;
+  float* diagonals = reinterpret_cast<float*>(smem + Sh::kSmem);
+  float* sums = reinterpret_cast<float*>(smem + Sh::kSmem + (table_grad ? 4 * Sh::kDiagonalBytes : 0));
+  float* offset_bias = sums + (table_grad ? p.num_buckets * 256 : 0);
+  uint8_t* offset_bucket = reinterpret_cast<uint8_t*>(offset_bias + (DKV ? 2 : 1) * offsets);
   __shared__ uint64_t bar_own, bar_full[S], bar_free[S], bar_clean[S], bar_s[BUFFERS], bar_p[BUFFERS], bar_o, bar_drain;
   __shared__ uint32_t tmem_base;
-  __shared__ float table[TABLE ? 2 : 1][TABLE ? kTableEntries : 1], offsets[TABLE ? 2 : 1][2][TABLE ? 256 : 1];
-  __shared__ uint8_t offset_buckets[TABLE && !DKV ? 2 : 1][2][TABLE && !DKV ? 256 : 1];
-  __shared__ __align__(16) float stats[DKV ? S : 1][2][DKV ? kPart : 4];  // of the partners: -lse (and the bias where all offsets of the step have one), -delta
-  __shared__ float errors[TABLE && !DKV ? 4 : 1][TABLE && !DKV ? 128 : 1];
+  __shared__ float errors[DKV ? 1 : 4][DKV ? 1 : 128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // ---- which rows
@@ -69,8 +99,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     else until = (dense_limit(p, len, min(row0 + kTcRows, len.nq) - 1) + kPart - 1) / kPart;
   }
   const int per_head = max(0, until - from), steps = DKV ? per_head * group : per_head;
-  auto partner_row = [&](int t) { return (from + (DKV ? t % per_head : t)) * kPart; };
-  auto partner_head = [&](int t) { return DKV ? kh * group + t / per_head : kh; };
+  // A step's partners: row and head, moved on without divisions, which would be most of what some roles execute.
+  struct Walk {
+    int t, row, head;
+  };
+  auto begin = [&](int t) { return Walk{t, (from + (DKV ? t % per_head : t)) * kPart, DKV ? kh * group + t / per_head : kh}; };
+  auto advance = [&](Walk& w, int by) {
+    w.t += by, w.row += by * kPart;
+    if (DKV)
+      while (w.row >= until * kPart) w.row -= per_head * kPart, ++w.head;
+  };
   auto first_offset = [&](int at) { return (DKV ? row0 - at - (kPart - 1) : at - row0 - (kTcRows - 1)) - len.shift; };  // of the pairs of a step
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.key_mask_batch : nullptr;
   const int part_rows = DKV ? len.nq : len.nk, part_all = DKV ? p.M : p.N;
@@ -100,7 +138,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
   if (tid == 0) {
     auto init = [&](uint64_t* bar, int count, int kind) { mbar_init(bar, count + (tc.waits.withheld == kind)); };
     init(&bar_own, 1, 0);
-    for (int i = 0; i < S; ++i) init(&bar_full[i], 1, 0), init(&bar_free[i], 1, 1), init(&bar_clean[i], 1, 4);
+    for (int i = 0; i < S; ++i) init(&bar_full[i], 1, 0), init(&bar_free[i], 1, 1), init(&bar_clean[i], 2, 4);
     for (int x = 0; x < BUFFERS; ++x) init(&bar_s[x], 1, 2), init(&bar_p[x], 8, 3);
     init(&bar_o, 1, 2);
     mbar_init(&bar_drain, 1);
@@ -110,8 +148,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     tmem_alloc(&tmem_base, 512);
     tmem_relinquish();
   }
-  if (TABLE && !DKV && p.dbias_part)
+  if (table_grad)
     for (int i = tid; i < p.num_buckets * 256; i += kBwdThreads) sums[i] = 0.f;
+  if (TABLE && !DKV)
+    for (int i = tid; i < offsets; i += kBwdThreads) {
+      const int bucket = dense_offset_bucket(p, i - p.reach - (kSpan - 1));
+      offset_bias[i] = dense_bias_entry(p, bucket, head);
+      offset_bucket[i] = (uint8_t)bucket;
+    }
+  if (DKV) {
+    for (int i = tid; i < Sh::kOnes / 16; i += kBwdThreads) {  // 1 1 1 0 in the first 16 bytes of a line
+      const int r = i >> 3, chunk = (i & 7) ^ (r & 7);
+      *reinterpret_cast<float4*>(smem + Sh::kOffOnes + i * 16) = chunk == 0 ? make_float4(1.f, 1.f, 1.f, 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int i = tid; i < S * Sh::kStatTile / 16; i += kBwdThreads) *reinterpret_cast<uint4*>(smem + Sh::kOffStats + i * 16) = make_uint4(0, 0, 0, 0);
+    fence_smem_to_async_proxy();
+  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -140,18 +192,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
             tma_box(smem_u32(smem + Sh::kOffA) + at, own_a, c * 64, row0 + half * 64, head, b, &bar_own);
             tma_box(smem_u32(smem + Sh::kOffB) + at, own_b, c * 64, row0 + half * 64, head, b, &bar_own);
           }
-        int t = 0;
-        for (; t < steps; ++t) {
-          const int stage = t % S;
-          if (t >= S) wait_on(&bar_free[stage], t / S - 1);
+        Walk w = begin(0);
+        for (; w.t < steps; advance(w, 1)) {
+          const int stage = w.t % S;
+          if (w.t >= S) wait_on(&bar_free[stage], w.t / S - 1);
           if (bad) break;
           mbar_arrive_expect_tx(&bar_full[stage], 2 * Sh::kPartTile);
           const uint32_t at = smem_u32(smem + Sh::kOffRing) + stage * 2 * Sh::kPartTile;
           for (int c = 0; c < Sh::kChunks; ++c) {
-            tma_box(at + c * kPart * 128, part_a, c * 64, partner_row(t), partner_head(t), b, &bar_full[stage]);
-            tma_box(at + Sh::kPartTile + c * kPart * 128, part_b, c * 64, partner_row(t), partner_head(t), b, &bar_full[stage]);
+            tma_box(at + c * kPart * 128, part_a, c * 64, w.row, w.head, b, &bar_full[stage]);
+            tma_box(at + Sh::kPartTile + c * kPart * 128, part_b, c * 64, w.row, w.head, b, &bar_full[stage]);
           }
         }
+        const int t = w.t;
         // whoever gave up, no copy may be in flight when the CTA ends
         if (!mbar_wait(&bar_own, 0)) bad = true;
         for (int i = max(0, t - S); i < t; ++i)
@@ -163,6 +216,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         const uint32_t l_a = make_desc_lo(smem_u32(smem + Sh::kOffA), 0), l_b = make_desc_lo(smem_u32(smem + Sh::kOffB), 0);
         const uint32_t l_ring = make_desc_lo(smem_u32(smem + Sh::kOffRing), 0), l_ring_mn = make_desc_lo(smem_u32(smem + Sh::kOffRing), kPart * 128);
         constexpr uint32_t kPartTile = Sh::kPartTile >> 4, kChunk = (kTcRows * 128) >> 4, kPartChunk = (kPart * 128) >> 4;
+        const uint32_t l_ones = make_desc_lo(smem_u32(smem + Sh::kOffOnes), 0), l_stats = make_desc_lo(smem_u32(smem + Sh::kOffStats), 0);
+        constexpr uint32_t idesc_stats = (make_idesc_bf16(kTcRows, kPart, false, false) & ~(0x3fu << 7)) | (2u << 7) | (2u << 10);  // tf32 by tf32
         constexpr uint32_t idesc_s = make_idesc_16<T>(kTcRows, kPart, false, false), idesc_o = make_idesc_16<T>(kTcRows, D, false, true);
         auto logits = [&](int t, int buffer) {
           const int stage = t % S;
@@ -175,6 +230,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
             umma_ss_lo(col + 64, l_b + (ks >> 2) * kChunk + (ks & 3) * 2, part + kPartTile + (ks >> 2) * kPartChunk + (ks & 3) * 2, idesc_s, ks > 0);
+          if (DKV) {
+            const uint32_t stat = l_stats + stage * (Sh::kStatTile >> 4);
+            umma_tf32_lo(col, l_ones, stat, idesc_stats);
+            umma_tf32_lo(col + 64, l_ones, stat + 2, idesc_stats);
+          }
           umma_commit(&bar_s[buffer]);
         };
         wait_on(&bar_own, 0);
@@ -203,45 +263,60 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         umma_commit(&bar_drain);
         if (!mbar_wait(&bar_drain, 0)) bad = true;
       }
-    } else if (warp == kOwnerWarps + 2) {
-      // ---------------------------------------------------------------- partners that are none become zeros; log-sum-exp and delta of queries
+    } else {
+      // ---------------------------------------------------------------- two warps, a row of the step for each lane: partners that are none become zeros;
+      // log-sum-exp and delta of queries
+      // (Both wait for every step: a warp that left steps out could meet a barrier two phases on and take it for its own.)
       if (cleaning) {
+        const int c = lane + 32 * (warp - (kOwnerWarps + 2));
         int bias_head = -1;
-        float far_bias[2] = {0.f, 0.f};
-        for (int t = 0; t < steps; ++t) {
-          const int stage = t % S, at = partner_row(t);
-          wait_on(&bar_full[stage], t / S);
-          if (DKV) {
-            const int h = partner_head(t);
-            const long long stat = ((long long)b * p.H + h) * p.M;
-            float one = 0.f;
-            if (TABLE) {
-              if (h != bias_head) {
-                bias_head = h;
-                far_bias[0] = dense_bias_entry(p, p.buckets[0], h), far_bias[1] = dense_bias_entry(p, p.buckets[2 * p.reach], h);
-              }
-              const int start = first_offset(at);
-              one = start + kSpan - 1 <= -p.reach ? far_bias[0] : start >= p.reach ? far_bias[1] : 0.f;
-            }
+        constexpr int AHEAD = DKV ? 3 : 1;
+        float far_bias[2] = {0.f, 0.f}, lse[AHEAD], delta[AHEAD];
+        const float per = 1.f / (p.scale * kDenseLog2e);
+        Walk next = begin(0), w = next;  // of what is fetched, of what is put down
+        auto fetch = [&](float& l, float& d) {  // steps ahead: one takes less time than its loads
+          if (next.t >= steps) return;
+          const int i = next.row + c;
+          const long long stat = ((long long)b * p.H + next.head) * p.M + i;
+          l = i < len.nq ? p.lse[stat] : INFINITY, d = i < len.nq ? p.delta[stat] : 0.f;
+          advance(next, 1);
+        };
+        if (DKV)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int c = lane + 32 * e, i = at + c;
-              stats[stage][0][c] = i < len.nq ? one - p.lse[stat + i] : -INFINITY;
-              stats[stage][1][c] = i < len.nq ? -p.delta[stat + i] : 0.f;
+          for (int u = 0; u < AHEAD; ++u) fetch(lse[u], delta[u]);
+        while (w.t < steps)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          if (w.t >= steps) break;
+          const int stage = w.t % S, at = w.row;
+          float one = 0.f;
+          if (DKV && TABLE) {
+            if (w.head != bias_head) {
+              bias_head = w.head;
+              far_bias[0] = dense_bias_entry(p, p.buckets[0], bias_head), far_bias[1] = dense_bias_entry(p, p.buckets[2 * p.reach], bias_head);
             }
+            const int start = first_offset(at);
+            one = start + kSpan - 1 <= -p.reach ? far_bias[0] : start >= p.reach ? far_bias[1] : 0.f;
           }
-          const int rows = min(kPart, part_all - at);  // what lies behind the tensor is zeros already
-          if (!bad && ((!DKV && mask) || at + rows > part_rows)) {
-            for (int r = lane; r < rows; r += 32) {
-              if (at + r < part_rows && (DKV || !mask || mask[at + r])) continue;
+          wait_on(&bar_full[stage], w.t / S);
+          if (DKV) {
+            float v = (one - lse[u]) * fabsf(per);
+            if (v < -1e30f) v = -1e30f;  // p = 0 (a number: the parts of an infinity are none)
+            uint8_t* line = smem + Sh::kOffStats + stage * Sh::kStatTile + c * 128;
+            *reinterpret_cast<float4*>(line + ((0 ^ (c & 7)) << 4)) = three_parts(per < 0.f ? -v : v);
+            *reinterpret_cast<float4*>(line + ((2 ^ (c & 7)) << 4)) = three_parts(-delta[u]);
+          }
+          const bool there = at + c < part_rows && (DKV || !mask || mask[at + c]);
+          if (!bad && !there && at + c < part_all) {  // (what lies behind the tensor is zeros already)
 #pragma unroll 1
-              for (int i = 0; i < 2 * Sh::kChunks * 8; ++i)
-                *reinterpret_cast<uint4*>(smem + Sh::kOffRing + (stage * 2 * Sh::kChunks + i / 8) * kPart * 128 + r * 128 + (i % 8) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_smem_to_async_proxy();
+            for (int i = 0; i < 2 * Sh::kChunks * 8; ++i)
+              *reinterpret_cast<uint4*>(smem + Sh::kOffRing + (stage * 2 * Sh::kChunks + i / 8) * kPart * 128 + c * 128 + (i % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
+          fence_smem_to_async_proxy();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar_clean[stage]);
+          if (DKV) fetch(lse[u], delta[u]);
+          advance(w, 1);
         }
       }
     }
@@ -262,12 +337,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       if (row_ok) {
         hi = dense_limit(p, len, row);
         lse = p.lse[stat + row];
-        const uint4* go = reinterpret_cast<const uint4*>(static_cast<const T*>(p.grad_out) + p.go_rows.at(b, head, row));
-        const uint4* o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + p.out_rows.at(b, head, row));
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 u = go[c], w = o[c];
-          const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
+        // delta: a quarter of the channels each
+        const uint4* go = reinterpret_cast<const uint4*>(static_cast<const T*>(p.grad_out) + p.go_rows.at(b, head, row) + team * (D / 4));
+        const uint4* o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + p.out_rows.at(b, head, row) + team * (D / 4));
+        uint4 u[D / 32], w[D / 32];
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) u[c] = go[c], w[c] = o[c];
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const uint32_t uw[4] = {u[c].x, u[c].y, u[c].z, u[c].w}, ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = unpack2<T>(uw[e]), g = unpack2<T>(ww[e]);
@@ -275,17 +353,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
           }
         }
       }
+      errors[team][r] = delta;
+      group_barrier(7, 512);
+      delta = (errors[0][r] + errors[1][r]) + (errors[2][r] + errors[3][r]);
       if (row < p.M && team == 0) p.delta[stat + row] = delta;
     } else if (row_ok) {
       lo = dense_first(p, len, row);
     }
     const int tile_lo = __reduce_max_sync(0xffffffffu, lo), tile_hi = __reduce_min_sync(0xffffffffu, hi);
-    const bool table_grad = TABLE && !DKV && p.dbias_part;
     float far[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, all = 0.f;  // sums of dS and of P over steps of one bucket (offsets below, above), of dS over all
-    int fills = 0, table_head = -1;
-    float far_bias[2] = {0.f, 0.f};  // of the offsets -reach and reach, and beyond
-    for (int t = y; t < steps; t += 2) {
-      const int at = partner_row(t), stage = t % S, buffer = t % BUFFERS;
+    int bias_head = -1;
+    const float* const my_bias = offset_bias + (DKV ? y * offsets : 0);
+    Walk w = begin(min(y, steps - 1));
+    int buffer = y, phase = 0;  // step w.t is the phase-th of its buffer
+    for (w.t = y; w.t < steps; advance(w, 2)) {
+      const int at = w.row;
       const uint32_t col = tmem + lanes + 128 * buffer;
       float one = 0.f;
       const float* near = nullptr;  // bias of the thread's column c at near[c] (DQ), near[-c] (DKV)
@@ -293,26 +375,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       int side = 0;
       if (TABLE) {
         const int start = first_offset(at);  // entry e: the offset start + e
-        const int h = DKV ? partner_head(t) : head;
-        if (h != table_head) {
-          if (table_head >= 0) group_barrier(1 + y, 256);
-          table[y][pair] = dense_bias_entry(p, pair, h);
+        if (DKV && w.head != bias_head) {
+          if (bias_head >= 0) group_barrier(1 + y, 256);
+          bias_head = w.head;
+          for (int i = pair; i < offsets; i += 256)
+            offset_bias[y * offsets + i] = dense_bias_entry(p, dense_offset_bucket(p, i - p.reach - (kSpan - 1)), bias_head);
           group_barrier(1 + y, 256);
-          table_head = h;
-          if (!DKV) far_bias[0] = table[y][p.buckets[0]], far_bias[1] = table[y][p.buckets[2 * p.reach]];
         }
         if (start + kSpan - 1 <= -p.reach || start >= p.reach) {
           side = start >= p.reach;
-          one = side ? far_bias[1] : far_bias[0];
+          if (!DKV) one = my_bias[side ? offsets - 1 : 0];  // (DKV: with the log-sum-exp)
         } else {
-          float* values = offsets[y][fills & 1];
-          const int bucket = dense_offset_bucket(p, start + pair);
-          values[pair] = table[y][bucket];
-          if (table_grad) offset_buckets[y][fills & 1][pair] = (uint8_t)bucket;
-          group_barrier(1 + y, 256);
-          near = values + (DKV ? r + kPart - 1 - c0 : kTcRows - 1 - r + c0);
-          near_bucket = offset_buckets[y][fills & 1];
-          ++fills;
+          const int entry = start + p.reach + kSpan - 1;
+          near = my_bias + entry + (DKV ? r + kPart - 1 - c0 : kTcRows - 1 - r + c0);
+          near_bucket = offset_bucket + entry;
         }
       }
       uint32_t seen = ~0u;
@@ -320,30 +396,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         const int key = at + c0 + lane;
         seen = __ballot_sync(0xffffffffu, key < len.nk && mask[key] != 0);
       }
-      wait_on(&bar_s[buffer], t / BUFFERS);
+      wait_on(&bar_s[buffer], phase);
       tc_fence_after_sync();
       float z[kCols], d[kCols];
       tmem_ld32(col + c0, *reinterpret_cast<uint32_t(*)[32]>(&z[0]));
       tmem_ld32(col + 64 + c0, *reinterpret_cast<uint32_t(*)[32]>(&d[0]));
       tmem_ld_wait();
       auto form = [&](auto biased) {  // p into z, dP - delta into d
+        constexpr bool kBiased = decltype(biased)::value;
         const float2 less = make_float2(one - lse, one - lse), off = make_float2(-delta, -delta), by = make_float2(sc2, sc2);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 4) {
-          float2 minus[2] = {less, less}, shift[2] = {off, off};
-          if (DKV) {
-            const float4 m = *reinterpret_cast<const float4*>(&stats[stage][0][c0 + c]), n = *reinterpret_cast<const float4*>(&stats[stage][1][c0 + c]);
-            minus[0] = make_float2(m.x, m.y), minus[1] = make_float2(m.z, m.w), shift[0] = make_float2(n.x, n.y), shift[1] = make_float2(n.z, n.w);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at_c = c + 2 * i;
-            if constexpr (decltype(biased)::value)
-              minus[i] = add2(minus[i], make_float2(near[DKV ? -at_c : at_c], near[DKV ? -at_c - 1 : at_c + 1]));
-            const float2 e = fma2(make_float2(z[at_c], z[at_c + 1]), by, minus[i]);
-            z[at_c] = dense_exp2(e.x), z[at_c + 1] = dense_exp2(e.y);
-            const float2 v = add2(make_float2(d[at_c], d[at_c + 1]), shift[i]);
-            d[at_c] = v.x, d[at_c + 1] = v.y;
+        for (int c = 0; c < kCols; c += 2) {
+          const float2 q = make_float2(z[c], z[c + 1]);
+          float2 e;
+          if constexpr (DKV && !kBiased) e = mul2(q, by);
+          else if constexpr (DKV) e = fma2(q, by, make_float2(near[-c], near[-c - 1]));
+          else if constexpr (kBiased) e = fma2(q, by, add2(less, make_float2(near[c], near[c + 1])));
+          else e = fma2(q, by, less);
+          z[c] = dense_exp2(e.x), z[c + 1] = dense_exp2(e.y);
+          if constexpr (!DKV) {
+            const float2 v = add2(make_float2(d[c], d[c + 1]), off);
+            d[c] = v.x, d[c + 1] = v.y;
           }
         }
       };
@@ -355,23 +428,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         for (int c = 0; c < kCols; ++c)
           if (c < a || c >= e || !((seen >> c) & 1u)) z[c] = 0.f;
       }
-      uint32_t w[16];
+      uint32_t packed[16];
       if (DKV) {
 #pragma unroll
-        for (int c = 0; c < kCols; c += 2) w[c >> 1] = pack2<T>(z[c], z[c + 1]);
-        tmem_st16(col + c0, w);  // (over the thread's own columns: the other half may not have read its)
+        for (int c = 0; c < kCols; c += 2) packed[c >> 1] = pack2<T>(z[c], z[c + 1]);
+        tmem_st16(col + c0, packed);  // (over the thread's own columns: the other half may not have read its)
       }
 #pragma unroll
       for (int c = 0; c < kCols; c += 2) {
         const float2 v = mul2(make_float2(z[c], z[c + 1]), make_float2(d[c], d[c + 1]));
         d[c] = v.x, d[c + 1] = v.y;
-        w[c >> 1] = pack2<T>(v.x, v.y);
+        packed[c >> 1] = pack2<T>(v.x, v.y);
       }
-      tmem_st16(col + 64 + c0, w);
+      tmem_st16(col + 64 + c0, packed);
       tmem_st_wait();
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_p[buffer]);
+      buffer += 2;
+      if (buffer >= BUFFERS) buffer -= BUFFERS, ++phase;
       if (table_grad) {
         float2 u[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -484,8 +559,10 @@ int launch(const DenseTcParams& tc, cudaStream_t stream) {
   const DenseParams& p = tc.p;
   using Sh = BwdShape<D, DKV, TABLE && !DKV>;
   auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
-  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 4 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0);
-  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 4 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0);
+  auto offset_bytes = [](int reach) { return (2 * reach + 2 * kSpan - 1) * (DKV ? 2 * 4 : 4 + 1); };
+  constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 4 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0) + (TABLE ? (2 * kMostReach + 2 * kSpan - 1) * 8 : 0);
+  static_assert(most <= 227 * 1024 - (DKV ? 512 : 2560), "beside the static part");
+  const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 4 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0) + (TABLE ? offset_bytes(p.reach) : 0);
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   const long long blocks = (long long)(((DKV ? p.N : p.M) + kTcRows - 1) / kTcRows) * p.B * (DKV ? p.K : p.H);
@@ -512,7 +589,9 @@ int dense_attn_take_bwd_status(int word, int32_t* host_status, cudaStream_t stre
 }
 
 bool dense_tc_bwd_takes(const DenseParams& p, int head_dim, int kind, bool table_grad) {
-  return kind != MF_BUCKETS_PAIR && dense_tc_takes(p, head_dim, kind) && (!table_grad || p.num_buckets <= (head_dim == 64 ? 64 : 32));
+  if (kind == MF_BUCKETS_PAIR || !dense_tc_takes(p, head_dim, kind)) return false;
+  if (!(fabsf(p.scale) >= 1e-6f && fabsf(p.scale) <= 1e6f)) return false;  // (the log-sum-exp is divided by it)
+  return kind == MF_BUCKETS_NONE || (p.reach <= kMostReach && (!table_grad || p.num_buckets <= (head_dim == 64 ? 64 : 32)));
 }
 
 int dense_attn_sm100_bwd(const DenseTcParams& tc, int dtype, int head_dim, int kind, cudaStream_t stream) {
