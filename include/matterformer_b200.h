@@ -799,6 +799,13 @@ size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs* args);
 size_t mf_dense_attn_bwd_workspace_bytes(const MfDenseAttnArgs* args);
 int mf_dense_attn_fwd(const MfDenseAttnArgs* args, void* stream);
 int mf_dense_attn_bwd(const MfDenseAttnArgs* args, void* stream);
+/* The code of a device-side wait that expired in a call on the device since this was last asked (the outputs of that call are undefined), or 0.  Synchronises
+ * `stream`. */
+int mf_dense_attn_status(int32_t* host_status, void* stream);
+/* Runs the call (backend MF_DENSE_BACKEND_TCGEN05) with the hand-offs of one kind withheld (0 copies, 1 free buffers, 2 products, 3 probabilities, 4 cleared rows)
+ * and waits that expire after limit_cycles (at least 10^4); returns the status it left, which no call and no mf_dense_attn_status sees.  With host_status
+ * NULL it leaves it to the latter.  The call's outputs are undefined. */
+int mf_selftest_dense_attn_give_up(const MfDenseAttnArgs* args, int32_t backward, int32_t kind, int64_t limit_cycles, int32_t* host_status, void* stream);
 
 /* Buckets of a batch of molecules for the above: buckets[b][i][j] (rows `row` and entries `batch_stride` bytes apart) = how many of the `edges` ascending
  * host values lie at or below the distance of atoms i and j of coords (batch, tokens, 3) fp32, compared as squares in fp64; 0 where i or j is

@@ -10,7 +10,7 @@ from .simplicial import (
     simplicial_attention_cuda,
 )
 from .batching import AttentionCostBatchSampler, simplicial_tile_steps
-from .dense import RelativeBias, dense_attention, dense_attention_packed, distance_buckets, offset_buckets, set_dense_backend
+from .dense import RelativeBias, dense_attention, dense_attention_packed, dense_attention_status, distance_buckets, offset_buckets, set_dense_backend
 from .gated import gated_mlp, gated_mlp_status
 from .hostio import HostPipelinedSimplicial
 from .rotary import RotaryPositions, rotary_embedding, rotary_frequencies, rotary_packed
@@ -31,6 +31,7 @@ __all__ = [
     "RelativeBias",
     "dense_attention",
     "dense_attention_packed",
+    "dense_attention_status",
     "distance_buckets",
     "offset_buckets",
     "set_dense_backend",

@@ -112,6 +112,8 @@ EXPORTED_SYMBOLS = (
     "mf_dense_attn_bwd_workspace_bytes",
     "mf_dense_attn_fwd",
     "mf_dense_attn_bwd",
+    "mf_dense_attn_status",
+    "mf_selftest_dense_attn_give_up",
     "mf_distance_buckets",
     "mf_profile_enable",
     "mf_profile_read",
@@ -497,6 +499,9 @@ def lib() -> ctypes.CDLL:
         fn.argtypes, fn.restype = [POINTER(MfDenseAttnArgs)], c_size_t
     for fn in (L.mf_dense_attn_fwd, L.mf_dense_attn_bwd):
         fn.argtypes, fn.restype = [POINTER(MfDenseAttnArgs), c_void_p], c_int32
+    L.mf_dense_attn_status.argtypes, L.mf_dense_attn_status.restype = [POINTER(c_int32), c_void_p], c_int32
+    L.mf_selftest_dense_attn_give_up.argtypes = [POINTER(MfDenseAttnArgs), c_int32, c_int32, c_int64, POINTER(c_int32), c_void_p]
+    L.mf_selftest_dense_attn_give_up.restype = c_int32
     L.mf_distance_buckets.argtypes = [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int64, c_int64, c_void_p]
     L.mf_distance_buckets.restype = c_int32
     L.mf_gated_mlp_status.argtypes = [POINTER(c_int32), c_void_p]

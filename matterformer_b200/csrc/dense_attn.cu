@@ -206,55 +206,40 @@ BwdSpace bwd_space(const MfDenseAttnArgs& a, const DenseParams& p) {
   return s;
 }
 
-}  // namespace
-}  // namespace mf
-
-extern "C" {
-
-size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs* a) {
-  using namespace mf;
-  if (check_args("mf_dense_attn_fwd_workspace_bytes", a) != MF_OK || a->batch == 0 || a->queries == 0) return 0;
-  const DenseParams p = params_of(*a);
-  return fwd_family(*a, p) == kSplit ? dense_attn_split_workspace_bytes(p, a->head_dim) : 0;
-}
-size_t mf_dense_attn_bwd_workspace_bytes(const MfDenseAttnArgs* a) {
-  using namespace mf;
-  if (check_args("mf_dense_attn_bwd_workspace_bytes", a) != MF_OK || a->batch == 0) return 0;
-  return bwd_space(*a, params_of(*a)).total;
+int check_space(const char* name, const MfDenseAttnArgs* a, size_t need) {
+  if (need == 0) return MF_OK;
+  if (!a->workspace || a->workspace_bytes < need) {
+    set_error("%s: %zu bytes of workspace needed, got %zu", name, need, a->workspace ? a->workspace_bytes : (size_t)0);
+    return MF_ERR_WORKSPACE_TOO_SMALL;
+  }
+  MF_CHECK_ALIGNED(name, a->workspace);
+  return MF_OK;
 }
 
-int mf_dense_attn_fwd(const MfDenseAttnArgs* a, void* stream_) {
-  using namespace mf;
-  const char* name = "mf_dense_attn_fwd";
+int forward(const char* name, const MfDenseAttnArgs* a, cudaStream_t stream, BoundedWaits waits) {
   const int rc = check_args(name, a);
   if (rc != MF_OK) return rc;
   if (a->batch == 0 || a->queries == 0) return MF_OK;
   const DenseParams p = params_of(*a);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   switch (fwd_family(*a, p)) {
     case kSmall: return dense_attn_small(p, a->dtype, a->head_dim, a->bucket_kind, false, stream);
     case kSplit: {
       const size_t need = dense_attn_split_workspace_bytes(p, a->head_dim);
-      MF_CHECK_ARG(need == 0 || (a->workspace && a->workspace_bytes >= need && aligned16(a->workspace)), "%s: %zu bytes of workspace needed, got %zu", name, need,
-                   a->workspace_bytes);
+      if (const int rc = check_space(name, a, need)) return rc;
       return dense_attn_split(p, a->dtype, a->head_dim, a->bucket_kind, a->workspace, stream);
     }
-    case kTensor: return dense_attn_sm100_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
+    case kTensor: return dense_attn_sm100_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream, waits);
     default: return dense_attn_mma_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
   }
 }
 
-int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
-  using namespace mf;
-  const char* name = "mf_dense_attn_bwd";
+int backward(const char* name, const MfDenseAttnArgs* a, cudaStream_t stream, BoundedWaits waits) {
   int rc = check_args(name, a);
   if (rc != MF_OK) return rc;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   DenseParams p = params_of(*a);
   const bool table = a->bias && a->dbias;
   const BwdSpace space = a->batch ? bwd_space(*a, p) : BwdSpace{};
-  MF_CHECK_ARG(space.total == 0 || (a->workspace && a->workspace_bytes >= space.total && aligned16(a->workspace)), "%s: %zu bytes of workspace needed, got %zu", name,
-               space.total, a->workspace_bytes);
+  if (MF_OK != (rc = check_space(name, a, space.total))) return rc;
   int entries = a->batch, tiles = dense_attn_mma_tiles(a->queries);  // of partial sums for each head
   if (a->batch > 0) {
     MF_CHECK_ARG(a->queries == 0 || (a->grad_out && a->lse), "%s: grad_out and lse must not be NULL", name);
@@ -265,7 +250,7 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
     char* ws = static_cast<char*>(a->workspace);
     p.delta = reinterpret_cast<float*>(ws);
     if (table) p.dbias_part = reinterpret_cast<float*>(ws + space.part);
-    DenseTcParams tc{p, {}, {}, {}, {}, {}};
+    DenseTcParams tc{p, {}, {}, {}, {}, waits};
     Family family = bwd_family(*a, p);
     if (family == kTensor && !dense_tc_maps(tc, a->dtype, a->head_dim, true)) family = kMma;
     switch (family) {
@@ -285,6 +270,51 @@ int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream_) {
   const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * ((a->num_buckets + 31) / 32)), dim3(1024), 0, stream, p.dbias_part, entries, a->heads, tiles,
                                            a->num_buckets, a->dbias, a->bias_dtype);
   return err == cudaSuccess ? MF_OK : cuda_error(err, "dense attention table gradient");
+}
+
+// The last expired wait of the forward kernels, or of the backward ones.
+int take_status(int word, int32_t* host_status, cudaStream_t stream) {
+  int32_t fwd = 0, bwd = 0;
+  int rc = dense_attn_take_fwd_status(word, &fwd, stream);
+  if (rc == MF_OK) rc = dense_attn_take_bwd_status(word, &bwd, stream);
+  *host_status = fwd ? fwd : bwd;
+  return rc;
+}
+
+}  // namespace
+}  // namespace mf
+
+extern "C" {
+
+size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs* a) {
+  using namespace mf;
+  if (check_args("mf_dense_attn_fwd_workspace_bytes", a) != MF_OK || a->batch == 0 || a->queries == 0) return 0;
+  const DenseParams p = params_of(*a);
+  return fwd_family(*a, p) == kSplit ? dense_attn_split_workspace_bytes(p, a->head_dim) : 0;
+}
+size_t mf_dense_attn_bwd_workspace_bytes(const MfDenseAttnArgs* a) {
+  using namespace mf;
+  if (check_args("mf_dense_attn_bwd_workspace_bytes", a) != MF_OK || a->batch == 0) return 0;
+  return bwd_space(*a, params_of(*a)).total;
+}
+
+int mf_dense_attn_fwd(const MfDenseAttnArgs* a, void* stream) { return mf::forward("mf_dense_attn_fwd", a, static_cast<cudaStream_t>(stream), {}); }
+int mf_dense_attn_bwd(const MfDenseAttnArgs* a, void* stream) { return mf::backward("mf_dense_attn_bwd", a, static_cast<cudaStream_t>(stream), {}); }
+
+int mf_dense_attn_status(int32_t* host_status, void* stream) {
+  MF_CHECK_ARG(host_status != nullptr, "mf_dense_attn_status: null pointer");
+  return mf::take_status(0, host_status, static_cast<cudaStream_t>(stream));
+}
+int mf_selftest_dense_attn_give_up(const MfDenseAttnArgs* a, int32_t backward, int32_t kind, int64_t limit_cycles, int32_t* host_status, void* stream_) {
+  using namespace mf;
+  const char* name = "mf_selftest_dense_attn_give_up";
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  MF_CHECK_ARG(a && kind >= 0 && kind <= 4 && a->backend == MF_DENSE_BACKEND_TCGEN05, "%s: bad argument", name);
+  MF_CHECK_ARG(limit_cycles >= 10000 && limit_cycles <= kWaitLimitCycles, "%s: the limit must lie in [10^4, 2^31] clocks", name);
+  BoundedWaits waits;
+  waits.limit = limit_cycles, waits.withheld = kind, waits.word = host_status != nullptr;
+  const int rc = backward ? mf::backward(name, a, stream, waits) : forward(name, a, stream, waits);
+  return rc != MF_OK || !host_status ? rc : take_status(1, host_status, stream);
 }
 
 int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t batch, int32_t tokens, const double* edges, int32_t num_edges, uint8_t* buckets,

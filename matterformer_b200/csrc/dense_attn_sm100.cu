@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
           tma_box(s_ring + slot * Sh::kTile + c * kTcRows * 128, i & 1 ? &tc.v : &tc.k, c * 64, (i >> 1) * kTcRows, kh, b, &bar_full[slot]);
       }
       // whoever gave up, no copy may be in flight when the CTA ends
-      if (!mbar_wait(&bar_q, 0)) bad = true;
+      if (!mbar_wait_for(&bar_q, 0, tc.waits.limit)) bad = true;
       for (int t = max(0, i - Sh::kSlots); t < i; ++t)
-        if (!mbar_wait(&bar_full[t % Sh::kSlots], (t / Sh::kSlots) & 1)) bad = true;
+        if (!mbar_wait_for(&bar_full[t % Sh::kSlots], (t / Sh::kSlots) & 1, tc.waits.limit)) bad = true;
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------------ products

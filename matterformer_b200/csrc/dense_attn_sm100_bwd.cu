@@ -206,9 +206,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
         }
         const int t = w.t;
         // whoever gave up, no copy may be in flight when the CTA ends
-        if (!mbar_wait(&bar_own, 0)) bad = true;
+        if (!mbar_wait_for(&bar_own, 0, tc.waits.limit)) bad = true;
         for (int i = max(0, t - S); i < t; ++i)
-          if (!mbar_wait(&bar_full[i % S], (i / S) & 1)) bad = true;
+          if (!mbar_wait_for(&bar_full[i % S], (i / S) & 1, tc.waits.limit)) bad = true;
       }
     } else if (warp == kOwnerWarps) {
       // ---------------------------------------------------------------- products

@@ -11,6 +11,7 @@ probabilities again.  :func:`offset_buckets` and :func:`distance_buckets` give t
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 from dataclasses import dataclass
@@ -18,7 +19,7 @@ from typing import Optional, Sequence, Union
 
 import torch
 
-from . import _lib
+from . import _lib, simplicial
 from .fused import watched
 
 MAX_BUCKETS = 128
@@ -122,9 +123,10 @@ class RelativeBias:
         if not (math.isfinite(self.reach) and self.reach > 0) or (self.kind == "offset" and self.reach != int(self.reach)):
             raise ValueError(f"reach must be positive, a whole number for buckets by offset, got {self.reach}")
 
-    @property
+    @functools.cached_property
     def edges(self) -> torch.Tensor:
-        return torch.linspace(0.0, float(self.reach), self.num_buckets, dtype=torch.float64, device="cpu")[1:]
+        with torch.inference_mode(False):  # (kept: an ordinary tensor, whoever asks first)
+            return torch.linspace(0.0, float(self.reach), self.num_buckets, dtype=torch.float64, device="cpu")[1:].contiguous()
 
     def buckets(self, positions: Optional[torch.Tensor], num_tokens: Optional[torch.Tensor], device) -> torch.Tensor:
         """As :func:`dense_attention` takes them; ``positions`` (B, N, 3) for distances."""
@@ -224,6 +226,7 @@ class _DenseAttention(torch.autograd.Function):
         L = _lib.lib()
         ws = _workspace(a, L.mf_dense_attn_fwd_workspace_bytes(ctypes.byref(a)), q.device)  # noqa: F841 (until the launch)
         _lib.launch(L.mf_dense_attn_fwd, q.device, ctypes.byref(a))
+        _raise_expired(q.device)
         out = out.transpose(1, 2).reshape(q.shape[0], q.shape[2], -1) if heads else out
         if keep:
             aux = [t.clone() if t is not None and t.is_inference() else t for t in (buckets, num_queries, num_keys, key_mask)]
@@ -268,7 +271,25 @@ class _DenseAttention(torch.autograd.Function):
         L = _lib.lib()
         ws = _workspace(a, L.mf_dense_attn_bwd_workspace_bytes(ctypes.byref(a)), q.device)  # noqa: F841
         _lib.launch(L.mf_dense_attn_bwd, q.device, ctypes.byref(a))
+        _raise_expired(q.device)
         return [made if ctx.needs_input_grad[0] else None, None, None, dbias] if heads else [dq, dk, dv, dbias]
+
+
+def dense_attention_status(device=None) -> int:
+    """0, or the code of a device-side wait that expired in one of the dense attention calls on the device since this was last asked; the outputs
+    of that call are undefined.  Synchronises the current stream.  :func:`set_check_status` asks after every call."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    out = ctypes.c_int32(0)
+    _lib.launch(_lib.lib().mf_dense_attn_status, dev, ctypes.byref(out))
+    return int(out.value)
+
+
+def _raise_expired(device: torch.device) -> None:
+    """After a call, where the caller has asked for it (see :func:`matterformer_b200.set_check_status`)."""
+    if simplicial._CHECK_STATUS and not torch.cuda.is_current_stream_capturing():
+        code = dense_attention_status(device)
+        if code != 0:
+            raise RuntimeError(f"a device-side wait of the dense attention kernels expired (status {code}); the outputs of that call are undefined")
 
 
 def _lengths(num, most, device):
@@ -364,7 +385,7 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_keys:
     Softmax and sums are in fp32 in a fixed order; probabilities and the gradients of the logits are rounded to the operands' type before
     the products that contract them.  Once differentiable in q, k, v and the table.  What is traced or under a transform of
     ``torch.func`` is the same in plain operations."""
-    native = _lib.native()
+    native = None if simplicial._CHECK_STATUS else _lib.native()
     if native is not None:  # operands that are ready as they are: one call into C++
         out = native.dense_attention(q, k, v, bias, buckets, num_queries, num_keys, key_mask, 0, bool(causal), scale, _lib.MF_DENSE_BACKEND[_BACKEND])
         if out is not None:
@@ -384,7 +405,7 @@ def dense_attention_packed(qkv: torch.Tensor, heads: int, num_tokens: Optional[t
                            scale: Optional[float] = None) -> torch.Tensor:  # fmt: skip
     """:func:`dense_attention` of tokens on themselves on the packed projection of an attention layer: ``qkv`` (B, N, 3*H*D), result (B, N, H*D) as the output
     projection takes it, the gradient in ``qkv``'s shape."""
-    native = _lib.native()
+    native = None if simplicial._CHECK_STATUS else _lib.native()
     if native is not None and heads >= 1:
         out = native.dense_attention(qkv, None, None, bias, buckets, num_tokens, num_tokens, key_mask, int(heads), bool(causal), scale, _lib.MF_DENSE_BACKEND[_BACKEND])
         if out is not None:

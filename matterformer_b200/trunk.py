@@ -13,8 +13,9 @@ so a reference ``state_dict`` of the same configuration loads with ``strict=True
 * :class:`EDMModel`             <- ``QM9EDMModel`` with geometry bias off, src/matterformer/models/qm9.py:249-565
 * :class:`EDMPreconditioner`, :class:`EDMLoss` <- src/matterformer/tasks/edm.py:34-150
 
-Only what that configuration touches is mirrored: no geometry-bias builders, no coordinate embedding.  Two options go beyond it:
-``rotary`` (rotary positions in the MHA layers; ``RotaryMultiheadAttention`` has three-dimensional ones, regular_attention.py:208-271) and
+Only what that configuration touches is mirrored: no geometry-bias builders, no coordinate embedding.  Three options go beyond it:
+``rotary`` (rotary positions in the MHA layers; ``RotaryMultiheadAttention`` has three-dimensional ones, regular_attention.py:208-271),
+``relative_bias`` (a learned bias of the MHA layers by buckets of distances or offsets, on dense attention kernels) and
 ``mlp_type="gated"`` (:class:`GatedMlp` in the place of :class:`Mlp`).  ``impl="cuda"`` (and ``"auto"`` on CUDA tensors) runs the sm_100a kernels through the C ABI;
 ``impl="torch"`` is the dense formulation in plain torch ops, as in the reference.
 """
@@ -29,6 +30,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from . import fused
+from .dense import RelativeBias, dense_attention_packed, dense_attention_torch, offset_buckets
 from .fused import (fused_applies, gated_layer_norm, gated_ln_modulate, gated_residual, heads_layout_applies, ln_modulate, merge_heads, split_heads,
                     split_modulation)
 from .gated import gated_mlp, gated_mlp_applies
@@ -217,15 +219,26 @@ class RegularAttention(nn.Module):
 
     With ``rotary`` the layer takes ``positions`` and turns its queries and keys before the core, whichever that is; the dense one is
     then ``F.scaled_dot_product_attention``, since ``nn.MultiheadAttention`` has no place for it.
+
+    With ``relative_bias`` the layer learns a table, ``bias_table``, and takes the ``buckets`` of its pairs
+    (:meth:`matterformer_b200.dense.RelativeBias.buckets`).  Its core is then :func:`matterformer_b200.dense.dense_attention_packed` for CUDA tensors in 16 bits at head
+    sizes 32, 64 and 128, otherwise (and with ``impl="torch"``) the same in plain operations.  ``impl="cuda"`` takes that kernel without a
+    bias too, at any number of tokens, and raises where it does not apply.
     """
 
     rotary: Optional[RotaryPositions] = None  # (of the class as well: modules that were stored before it existed have none of their own)
+    relative_bias: Optional[RelativeBias] = None
 
     def __init__(self, embed_dim: int, num_heads: int, *, dropout: float = 0.0, impl: str = "auto",
-                 rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
+                 rotary: Optional[RotaryPositions] = None, relative_bias: Optional[RelativeBias] = None) -> None:  # fmt: skip
         super().__init__()
-        if impl not in {"auto", "torch"}:
+        if impl not in {"auto", "torch", "cuda"}:
             raise ValueError(f"Unsupported attention impl: {impl}")
+        if relative_bias is not None and dropout > 0.0:
+            raise ValueError("a layer with a relative bias has no dropout")
+        self.relative_bias = relative_bias
+        if relative_bias is not None:
+            self.bias_table = nn.Parameter(torch.zeros(relative_bias.num_buckets, num_heads))
         if rotary is not None and rotary.rotary_dim > embed_dim // num_heads:
             raise ValueError(f"rotary_dim {rotary.rotary_dim} above the head size {embed_dim // num_heads}")
         self.rotary = rotary
@@ -233,9 +246,47 @@ class RegularAttention(nn.Module):
         self.impl = impl
         self._last_core_used: Optional[str] = None
 
+    def _dense_fits(self, x: torch.Tensor) -> bool:
+        """Whether the core runs on the dense kernels, which ``impl="cuda"`` insists on."""
+        if self.impl == "torch" or (self.impl == "auto" and self.relative_bias is None):
+            return False
+        low = x.dtype in (torch.bfloat16, torch.float16) or (x.is_cuda and torch.is_autocast_enabled("cuda"))
+        fits = x.is_cuda and low and self.attn.embed_dim // self.attn.num_heads in (32, 64, 128) and not (self.training and self.attn.dropout > 0.0)
+        if self.impl == "cuda" and not fits:
+            raise RuntimeError("the dense attention kernels need CUDA tensors in 16 bits, a head size of 32, 64 or 128 and no active dropout")
+        return fits
+
+    def _dense_forward(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor], positions: Optional[torch.Tensor],
+                       buckets: Optional[torch.Tensor], num_atoms: Optional[torch.Tensor], suffix: bool) -> torch.Tensor:  # fmt: skip
+        """The layer on the dense kernels, or with a bias in plain operations.  ``suffix``: the padding is behind the real tokens of every row."""
+        H = self.attn.num_heads
+        qkv = linear_bf16(x, self.attn.in_proj_weight, self.attn.in_proj_bias)
+        kernel = self._dense_fits(x)
+        self._last_core_used = "dense" if kernel else "torch"
+        table = self.bias_table if self.relative_bias is not None else None
+        shown = None if key_padding_mask is None else ~key_padding_mask.bool()
+        if positions is not None:
+            r = self.rotary
+            if key_padding_mask is not None and positions.ndim == r.frequencies.ndim + 1:  # (as in _dense_rotary)
+                hidden = key_padding_mask.bool()
+                positions = positions.masked_fill((hidden if positions.ndim == 2 else hidden[..., None]) & ~positions.isfinite(), 0)
+            if kernel and not self._differentiated(positions):
+                qkv = rotary_packed(qkv, H, self._kernel_positions(positions), r.frequencies, layout=r.layout, amplitude=r.amplitude)
+            else:
+                qkv = rotate_packed_torch(qkv, H, positions, r.frequencies, r.layout, r.amplitude)
+        if kernel:
+            counted = shown is not None and suffix
+            if counted and num_atoms is None:
+                num_atoms = shown.sum(dim=1).to(torch.int32)
+            core = dense_attention_packed(qkv, H, num_atoms if counted else None, key_mask=None if counted else shown, bias=table, buckets=buckets)
+        else:
+            q, k, v = qkv.unflatten(-1, (3, H, -1)).permute(2, 0, 3, 1, 4).unbind(0)
+            core = dense_attention_torch(q, k, v, key_mask=shown, bias=table, buckets=buckets).transpose(1, 2).flatten(2)
+        return linear_bf16(core, self.attn.out_proj.weight, self.attn.out_proj.bias)
+
     def _core_fits(self, x: torch.Tensor, key_padding_mask: Optional[torch.Tensor]) -> bool:
         """Everything but the form of the padding."""
-        if self.impl == "torch" or not x.is_cuda or key_padding_mask is None or x.shape[1] > 32:
+        if self.impl != "auto" or self.relative_bias is not None or not x.is_cuda or key_padding_mask is None or x.shape[1] > 32:
             return False
         if self.training and self.attn.dropout > 0.0:
             return False
@@ -300,17 +351,28 @@ class RegularAttention(nn.Module):
 
     def forward(self, x: torch.Tensor, *, key_padding_mask: Optional[torch.Tensor] = None,
                 sparse_plan: Optional[SparseAttentionPlan] = None, num_atoms: Optional[torch.Tensor] = None,
-                padding_is_suffix: Optional[bool] = None, positions: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
+                padding_is_suffix: Optional[bool] = None, positions: Optional[torch.Tensor] = None,
+                buckets: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
         """``num_atoms``: the (B,) int32 counts of real tokens, ``padding_is_suffix``: the form of the mask, when the caller
         has already found them.  ``positions``: of the tokens, for a layer with ``rotary`` (see :func:`rotary_embedding`); others take
-        none.  They may be of 16 bits and may want a gradient, which plain operations then form."""
+        none.  They may be of 16 bits and may want a gradient, which plain operations then form.  ``buckets``: of the pairs, for a layer with
+        ``relative_bias``; others take none."""
+        if (self.relative_bias is None) != (buckets is None):
+            raise ValueError("a layer with a relative bias needs `buckets`" if buckets is None else "`buckets` are for a layer with a relative bias")
         if (self.rotary is None) != (positions is None):
             raise ValueError("a layer with rotary positions needs `positions`" if positions is None else
                              "`positions` are for a layer with rotary positions")  # fmt: skip
         if sparse_plan is not None:
+            if buckets is not None:
+                raise ValueError("sparse attention plans have no place for a relative bias")
             if not x.is_cuda:
                 raise RuntimeError("sparse attention plans need CUDA tensors (there is no CPU fallback)")
             return self._sparse_forward(x, sparse_plan, positions)
+        if self.relative_bias is not None or self.impl == "cuda":
+            suffix = False
+            if key_padding_mask is not None and self._dense_fits(x):
+                suffix = _padding_is_suffix(self, key_padding_mask) if padding_is_suffix is None else padding_is_suffix
+            return self._dense_forward(x, key_padding_mask, positions, buckets, num_atoms, suffix)
         if not self._core_fits(x, key_padding_mask) or not (
             _padding_is_suffix(self, key_padding_mask) if padding_is_suffix is None else padding_is_suffix
         ):
@@ -406,7 +468,8 @@ class AdaLNBlock(nn.Module):
 
     def __init__(self, d_model: int, n_heads: int, *, mlp_ratio: float = 4.0, eps: float = 1e-6,
                  attn_type: str = "mha", simplicial_impl: str = "auto", simplicial_precision: str = "bf16_tc",
-                 mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
+                 mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None, mha_impl: str = "auto",
+                 relative_bias: Optional[RelativeBias] = None) -> None:  # fmt: skip
         super().__init__()
         attn_type = attn_type.lower()
         if attn_type not in {"mha", "simplicial"}:
@@ -420,7 +483,7 @@ class AdaLNBlock(nn.Module):
         nn.init.zeros_(self.ada_ln[-1].weight)
         nn.init.zeros_(self.ada_ln[-1].bias)
         if attn_type == "mha":
-            self.attn = RegularAttention(d_model, n_heads, rotary=rotary)
+            self.attn = RegularAttention(d_model, n_heads, impl=mha_impl, rotary=rotary, relative_bias=relative_bias)
         else:
             self.attn = SimplicialAttention(d_model, n_heads, impl=simplicial_impl, precision=simplicial_precision)
         self.mlp = Mlp(d_model, mlp_ratio) if mlp_type == "plain" else GatedMlp(d_model, mlp_ratio)
@@ -428,7 +491,7 @@ class AdaLNBlock(nn.Module):
 
     def forward(self, x, cond_emb, *, pad_mask=None, simplicial_attention_mask=None, sparse_plan=None,
                 zero_padding: bool = False, cond_act=None, modulation=None, num_atoms=None, h=None, following=None,
-                padding_is_suffix=None, positions=None):
+                padding_is_suffix=None, positions=None, buckets=None):
         """``zero_padding``: return the block's output with its padded rows cleared (the ``masked_fill`` the trunk
         applies before the next block), folded into the last fused pass when the fused kernels run.  ``cond_act``:
         ``SiLU(cond_emb)`` when the caller has already formed it (it is the same for every block of a trunk).
@@ -436,7 +499,8 @@ class AdaLNBlock(nn.Module):
         real tokens for the attention layer, ``padding_is_suffix``: whether they come first in every row.  ``following``:
         (shift, scale, eps) of the norm that opens the next block; the block then returns its output and that norm's, formed in
         one pass, and the next block takes the latter as ``h``.  (None, None, eps): the norm is the stack's output norm, which has no
-        modulation and is kept in fp32; only its output is returned.  ``positions``: of the tokens, for an attention layer with ``rotary``."""
+        modulation and is kept in fp32; only its output is returned.  ``positions``: of the tokens, for an attention layer with ``rotary``, ``buckets``: of
+        the pairs, for one with ``relative_bias``."""
         fused = self.fused_elementwise and fused_applies(x)
         mod = None if modulation is not None else linear_bf16(cond_act if cond_act is not None else self.ada_ln[0](cond_emb), self.ada_ln[-1].weight,
                           self.ada_ln[-1].bias)  # fmt: skip
@@ -454,6 +518,8 @@ class AdaLNBlock(nn.Module):
             h = _modulate(self.norm1(x), shift_a, scale_a)
         if self.attn_type == "mha":
             turning = {"positions": positions} if getattr(self.attn, "rotary", None) is not None else {}
+            if getattr(self.attn, "relative_bias", None) is not None:
+                turning["buckets"] = buckets
             attn_out = self.attn(h, key_padding_mask=pad_mask, sparse_plan=sparse_plan, num_atoms=num_atoms,
                                  padding_is_suffix=padding_is_suffix, **turning)  # fmt: skip
         else:
@@ -474,18 +540,25 @@ class AdaLNBlock(nn.Module):
 
 
 class TransformerTrunk(nn.Module):
-    """Stack of :class:`AdaLNBlock`; ``attn_types`` names the attention of every layer, e.g. alternating."""
+    """Stack of :class:`AdaLNBlock`; ``attn_types`` names the attention of every layer, e.g. alternating.  ``relative_bias``: every MHA layer has a
+    table of its own; the buckets are formed once for all.  ``mha_impl``: of the MHA layers (see :class:`RegularAttention`)."""
 
     rotary: Optional[RotaryPositions] = None  # (see RegularAttention)
+    relative_bias: Optional[RelativeBias] = None
 
     def __init__(self, d_model: int, n_heads: int, attn_types: Sequence[str], *, mlp_ratio: float = 4.0,
                  eps: float = 1e-6, simplicial_impl: str = "auto", simplicial_precision: str = "bf16_tc",
-                 emit_pair_valid: bool = True, mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
+                 emit_pair_valid: bool = True, mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None, mha_impl: str = "auto",
+                 relative_bias: Optional[RelativeBias] = None) -> None:  # fmt: skip
         super().__init__()
         self.rotary = rotary
+        self.relative_bias = relative_bias
+        if relative_bias is not None and relative_bias.kind == "offset":
+            self.register_buffer("_offset_buckets", offset_buckets(relative_bias.num_buckets, int(relative_bias.reach)), persistent=False)
         self.blocks = nn.ModuleList(
             AdaLNBlock(d_model, n_heads, mlp_ratio=mlp_ratio, eps=eps, attn_type=t, simplicial_impl=simplicial_impl,
-                       simplicial_precision=simplicial_precision, mlp_type=mlp_type, rotary=rotary)  # fmt: skip
+                       simplicial_precision=simplicial_precision, mlp_type=mlp_type, rotary=rotary, mha_impl=mha_impl,
+                       relative_bias=relative_bias)  # fmt: skip
             for t in attn_types
         )
         self.norm_out = nn.LayerNorm(d_model, eps=eps, elementwise_affine=False)
@@ -506,14 +579,22 @@ class TransformerTrunk(nn.Module):
 
     def forward(self, x: torch.Tensor, cond_emb: torch.Tensor, *, pad_mask: Optional[torch.Tensor] = None,
                 sparse_plan: Optional[SparseAttentionPlan] = None, padding_cleared: bool = False,
-                positions: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
+                positions: Optional[torch.Tensor] = None, coords: Optional[torch.Tensor] = None) -> torch.Tensor:  # fmt: skip
         """``sparse_plan`` (see :func:`plan_sparse_attention`) makes every MHA layer attend over the plan's
         neighbourhoods instead of all tokens: the periodic-crystal mode of the trunk.  ``padding_cleared``: the rows of ``x`` that
-        ``pad_mask`` marks are zeros already.  ``positions``: of the tokens, needed by a trunk with ``rotary``."""
+        ``pad_mask`` marks are zeros already.  ``positions``: of the tokens, needed by a trunk with ``rotary``.  ``coords``: (B, N, 3), needed by a trunk
+        whose ``relative_bias`` goes by distances (a molecule's; no gradient)."""
+        by_distance = self.relative_bias is not None and self.relative_bias.kind == "distance"
+        if by_distance != (coords is not None):
+            raise ValueError("a trunk with a bias by distances needs `coords`" if by_distance else "`coords` are for a trunk with a bias by distances")
+        if self.relative_bias is not None and sparse_plan is not None:
+            raise ValueError("sparse attention plans have no place for a relative bias")
         if (self.rotary is None) != (positions is None):
             raise ValueError("a trunk with rotary positions needs `positions`" if positions is None else
                              "`positions` are for a trunk with rotary positions")  # fmt: skip
         turning = {} if positions is None else {"positions": positions}
+        if self.relative_bias is not None:
+            turning["coords"] = coords
         bf16 = x.is_cuda and torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16
         layers = [block.ada_ln[-1] for block in self.blocks]
         stacked = bf16 and fused_applies(x) and cond_emb.ndim == 2 and all(
@@ -556,7 +637,11 @@ class TransformerTrunk(nn.Module):
             modulation = stacked_modulation(cond_act, *modulation_copies, [m.weight for m in layers] + [m.bias for m in layers],
                                             len(layers))  # fmt: skip
         mha = [block.attn for block in self.blocks if isinstance(block.attn, RegularAttention)]
-        reads = sparse_plan is None and any(attn._core_fits(x, pad_mask) for attn in mha)
+        reads = sparse_plan is None and any(attn._core_fits(x, pad_mask) or (pad_mask is not None and attn._dense_fits(x)) for attn in mha)
+        if self.relative_bias is not None:
+            coords = turning.pop("coords")
+            if mha:
+                turning["buckets"] = self._offset_buckets if coords is None else self.relative_bias.buckets(coords, num_atoms, x.device)
         suffix = _padding_is_suffix(self, pad_mask) if reads else None  # one read-back for all layers
         h, norm = None, self.norm_out
         last = len(self.blocks) - 1
@@ -621,13 +706,15 @@ class EDMModel(nn.Module):
 
     Mirrors ``QM9EDMModel(use_geometry_bias=False, coord_embed_mode="none", coord_head_mode="equivariant")``
     with the default noise conditioning (sigma channel concatenated to the atom features and adaLN).  ``mlp_type`` and ``rotary`` go
-    to the trunk's blocks; rotary positions are the noisy coordinates, on three axes.
+    to the trunk's blocks; rotary positions are the noisy coordinates, on three axes.  ``relative_bias`` and ``mha_impl`` go to its MHA layers; distances are those of
+    the noisy coordinates.
     """
 
     def __init__(self, *, atom_channels: int = 6, d_model: int = 512, n_heads: int = 8, n_layers: int = 12,
                  attn_types: Optional[Sequence[str]] = None, mlp_ratio: float = 4.0, simplicial_impl: str = "auto",
                  simplicial_precision: str = "bf16_tc", pair_hidden_dim: int = 128, pair_n_rbf: int = 16,
-                 pair_rbf_max: float = 4.0, mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None) -> None:  # fmt: skip
+                 pair_rbf_max: float = 4.0, mlp_type: str = "plain", rotary: Optional[RotaryPositions] = None, mha_impl: str = "auto",
+                 relative_bias: Optional[RelativeBias] = None) -> None:  # fmt: skip
         super().__init__()
         if rotary is not None and rotary.axes != 3:
             raise ValueError(f"the coordinates are positions on 3 axes, rotary has {rotary.axes}")
@@ -638,7 +725,7 @@ class EDMModel(nn.Module):
         self.conditioning = TimeEmbedder(d_model)
         self.trunk = TransformerTrunk(d_model, n_heads, attn_types, mlp_ratio=mlp_ratio,
                                       simplicial_impl=simplicial_impl, simplicial_precision=simplicial_precision,
-                                      mlp_type=mlp_type, rotary=rotary)  # fmt: skip
+                                      mlp_type=mlp_type, rotary=rotary, mha_impl=mha_impl, relative_bias=relative_bias)  # fmt: skip
         self.atom_head = nn.Sequential(nn.LayerNorm(d_model), nn.Linear(d_model, d_model), nn.SiLU(),
                                        nn.Linear(d_model, atom_channels))  # fmt: skip
         self.pair_head = nn.Sequential(nn.Linear(2 * d_model + pair_n_rbf, pair_hidden_dim), nn.SiLU(),
@@ -714,6 +801,9 @@ class EDMModel(nn.Module):
         more = {"padding_cleared": True} if whole and type(self.trunk) is TransformerTrunk else {}
         if getattr(self.trunk, "rotary", None) is not None:
             more["positions"] = coords_noisy
+        bias = getattr(self.trunk, "relative_bias", None)
+        if bias is not None and bias.kind == "distance":
+            more["coords"] = coords_noisy
         trunk_out = self.trunk(tokens, cond, pad_mask=pad_mask, **more)
         normed = layer_norm(trunk_out, self.atom_head[0], torch.bfloat16 if low else torch.float32)
         atom_delta = _two_layers(self.atom_head[1:], normed).masked_fill(pad_mask[..., None], 0.0)
