@@ -293,7 +293,7 @@ def _raise_expired(device: torch.device) -> None:
 
 
 def _lengths(num, most, device):
-    return torch.full((1, 1, 1), most, device=device) if num is None else num.long().clamp(0, most).reshape(-1, 1, 1)
+    return torch.full((1, 1, 1), most, device=device) if num is None else num.long().clamp(0, int(most)).reshape(-1, 1, 1)
 
 
 def dense_attention_torch(q, k, v, num_keys=None, num_queries=None, *, key_mask=None, causal=False, bias=None, buckets=None, scale=None) -> torch.Tensor:
@@ -313,12 +313,12 @@ def dense_attention_torch(q, k, v, num_keys=None, num_queries=None, *, key_mask=
     # what no query sees, and queries that see nothing, may hold anything: their numbers do not enter
     shown, awake = see.any(1)[:, None, :, None], see.any(2)[:, None, :, None]
     qw = torch.where(awake, q.to(wide), 0.0)
-    kw, vw = (torch.where(shown, t.to(wide), 0.0).repeat_interleave(H // K, dim=1) for t in (k, v))
+    kw, vw = (torch.where(shown, t.to(wide), 0.0).repeat_interleave(int(H) // int(K), dim=1) for t in (k, v))
     logits = (qw @ kw.transpose(-1, -2)) * (D**-0.5 if scale is None else scale)
     see = see[:, None]
     if bias is not None:
         if buckets.ndim == 1:
-            L = buckets.shape[0] // 2
+            L = int(buckets.shape[0]) // 2
             which = buckets[offset.clamp(-L, L) + L].long()
         else:
             which = buckets.long()
