@@ -27,15 +27,21 @@ constexpr int kPairRow = 80, kPairTile = 64 * kPairRow;  // a row of 64 bytes, i
 template <int D, int KIND>
 constexpr int kFixedBytes = 6 * kTileBytes<D> + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 4 + 2 * 128 + (KIND == MF_BUCKETS_PAIR ? 2 * kPairTile : 0);
 
-// rows [row0, row0 + 64) of a head, zeros from row_limit on and where `mask` (per row) is zero
+// bits lo .. hi - 1 of a word
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  const uint32_t below = hi >= 32 ? ~0u : hi > 0 ? (1u << hi) - 1u : 0u, from = lo >= 32 ? 0u : lo > 0 ? ~0u << lo : ~0u;
+  return below & from;
+}
+
+// rows [row0, row0 + 64) of a head, zeros from row_limit on and where `shown` (a bit for each) says so
 template <typename T, int D>
-__device__ __forceinline__ void load_rows(uint32_t tile, const T* src, long long stride, int row0, int row_limit, const uint8_t* mask) {
+__device__ __forceinline__ void load_rows(uint32_t tile, const T* src, long long stride, int row0, int row_limit, uint2 shown) {
   constexpr int LD = D + 8, PER_ROW = D / 8;
 #pragma unroll
   for (int it = 0; it < 64 * PER_ROW / kThreads; ++it) {
     const int idx = it * kThreads + threadIdx.x;
     const int r = idx / PER_ROW, c = idx % PER_ROW, row = row0 + r;
-    const bool ok = row < row_limit && (!mask || mask[row]);
+    const bool ok = row < row_limit && (((r & 32 ? shown.y : shown.x) >> (r & 31)) & 1u);
     cp_async16(tile + (r * LD + c * 8) * 2, src + (ok ? row * stride : 0) + c * 8, ok);
   }
 }
@@ -101,20 +107,27 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
       }
     }
   };
-  auto load_step = [&](int t, int stage) {
+  // The key mask of 64 keys from j0 on: a byte for each lane and half, as bits.  They are asked for a tile before the rows are, which wait for them.
+  auto mask_bytes = [&](int j0) {
+    const int j = j0 + lane;
+    return make_uchar2(j < len.nk ? mask[j] : 0, j + 32 < len.nk ? mask[j + 32] : 0);
+  };
+  auto mask_bits = [&](uchar2 m) { return make_uint2(__ballot_sync(0xffffffffu, m.x != 0), __ballot_sync(0xffffffffu, m.y != 0)); };
+  const uint2 every = make_uint2(~0u, ~0u);
+  auto load_step = [&](int t, int stage, uint2 shown) {
     const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
     const int at = first + (MODE == D_DKV ? t % per_head : t) * kPart;
     if (MODE == D_DKV) {
-      load_rows<T, D>(s_part_a + stage * TILE, q_of(h), p.q_rows.token, at, len.nq, nullptr);
-      load_rows<T, D>(s_part_b + stage * TILE, go_of(h), p.go_rows.token, at, len.nq, nullptr);
+      load_rows<T, D>(s_part_a + stage * TILE, q_of(h), p.q_rows.token, at, len.nq, every);
+      load_rows<T, D>(s_part_b + stage * TILE, go_of(h), p.go_rows.token, at, len.nq, every);
       if (tid < 64) {
         const int i = at + tid;
         part_lse[stage * 64 + tid] = i < len.nq ? p.lse[stat(h) + i] : INFINITY;
         part_delta[stage * 64 + tid] = i < len.nq ? p.delta[stat(h) + i] : 0.f;
       }
     } else {
-      load_rows<T, D>(s_part_a + stage * TILE, K, p.k_rows.token, at, len.nk, mask);
-      load_rows<T, D>(s_part_b + stage * TILE, V, p.v_rows.token, at, len.nk, mask);
+      load_rows<T, D>(s_part_a + stage * TILE, K, p.k_rows.token, at, len.nk, shown);
+      load_rows<T, D>(s_part_b + stage * TILE, V, p.v_rows.token, at, len.nk, shown);
     }
     if (KIND == MF_BUCKETS_PAIR) load_pairs(MODE == D_DKV ? at : row0, MODE == D_DKV ? row0 : at, stage);
     if (KIND == MF_BUCKETS_OFFSET && tid < kSpan) {  // offsets of the two tiles: owner - partner or partner - owner runs over 127 values
@@ -125,15 +138,23 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     }
   };
 
+  uint2 seen = every, seen_next = every;  // the mask of this tile's keys and of the next one's
+  uchar2 bytes = make_uchar2(1, 1);       // of the one after that
+  const bool masked = MODE != D_DKV && mask;
   if (steps > 0) {
-    if (MODE == D_DKV) {
-      load_rows<T, D>(s_own_a, K, p.k_rows.token, row0, len.nk, mask);
-      load_rows<T, D>(s_own_b, V, p.v_rows.token, row0, len.nk, mask);
-    } else {
-      load_rows<T, D>(s_own_a, q_of(oh), p.q_rows.token, row0, len.nq, nullptr);
-      if (MODE == D_DQ) load_rows<T, D>(s_own_b, go_of(oh), p.go_rows.token, row0, len.nq, nullptr);
+    if (masked) {
+      seen_next = mask_bits(mask_bytes(first));
+      bytes = mask_bytes(first + kPart);
     }
-    load_step(0, 0);
+    if (MODE == D_DKV) {
+      const uint2 shown = mask ? mask_bits(mask_bytes(row0)) : every;
+      load_rows<T, D>(s_own_a, K, p.k_rows.token, row0, len.nk, shown);
+      load_rows<T, D>(s_own_b, V, p.v_rows.token, row0, len.nk, shown);
+    } else {
+      load_rows<T, D>(s_own_a, q_of(oh), p.q_rows.token, row0, len.nq, every);
+      if (MODE == D_DQ) load_rows<T, D>(s_own_b, go_of(oh), p.go_rows.token, row0, len.nq, every);
+    }
+    load_step(0, 0, seen_next);
   }
   cp_async_commit();
   const int nb = p.num_buckets;
@@ -192,21 +213,19 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
       d += __shfl_xor_sync(0xffffffffu, d, 1);
       d += __shfl_xor_sync(0xffffffffu, d, 2);
       delta[e] = d;
-      if (t4 == 0 && row < p.M) p.delta[stat(oh) + row] = d;
     }
   }
+  float error[2] = {0.f, 0.f};  // sums of dS, zero but for what delta is off by
+
 
   for (int t = 0; t < steps; ++t) {
     const int stage = t & 1;
     const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
     const int at = first + (MODE == D_DKV ? t % per_head : t) * kPart;
-    uint32_t seen[2] = {0xffffffffu, 0xffffffffu};  // the mask of this tile's keys
-    if (MODE != D_DKV && mask) {
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int j = at + 32 * w + lane;
-        seen[w] = __ballot_sync(0xffffffffu, j < len.nk && mask[j] != 0);
-      }
+    if (masked) {
+      seen = seen_next;
+      seen_next = mask_bits(bytes);
+      bytes = mask_bytes(at + 2 * kPart);
     }
     if (KIND == MF_BUCKETS_PAIR && MODE == D_DKV && t % per_head == 0) {  // another head: another column of the table
       __syncthreads();
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     }
     cp_async_wait<0>();
     __syncthreads();  // tile t has arrived, and everybody is done with the buffers of tile t - 1
-    if (t + 1 < steps) load_step(t + 1, stage ^ 1);
+    if (t + 1 < steps) load_step(t + 1, stage ^ 1, seen_next);
     cp_async_commit();
 
     const uint32_t pa = s_part_a + stage * TILE, pb = s_part_b + stage * TILE;
@@ -268,14 +287,18 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
         if (KIND == MF_BUCKETS_OFFSET) s[nt][e] = fmaf(s[nt][e], sc2, offset_bias[stage * 128 + (MODE == D_DKV ? r - c + kPart - 1 : c - r + kOwn - 1)]);
         if (KIND == MF_BUCKETS_PAIR) s[nt][e] = fmaf(s[nt][e], sc2, table[(which[nt] >> (8 * e)) & 255u]);
       }
-    if (at < most_lo || at + kPart > least_hi || (MODE != D_DKV && mask)) {
+    if (at < most_lo || at + kPart > least_hi || masked) {
+      uint32_t vis[2][2];  // of a row, half of the tile: from the thread's first column on
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        vis[e][0] = (bits_between(lo[e] - at, hi[e] - at) & seen.x) >> (2 * t4);
+        vis[e][1] = (bits_between(lo[e] - at - 32, hi[e] - at - 32) & seen.y) >> (2 * t4);
+      }
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int c = nt * 8 + 2 * t4 + (e & 1), x = at + c;
-          if (x < lo[e >> 1] || x >= hi[e >> 1] || !((seen[nt >> 2] >> (c & 31)) & 1u)) s[nt][e] = -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e)
+          if (!(vis[e >> 1][nt >> 2] & (1u << ((nt & 3) * 8 + (e & 1))))) s[nt][e] = -INFINITY;
     }
 
     if (MODE == D_FWD) {
@@ -316,7 +339,20 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
           const float pr = dense_exp2(z - l);
           s[nt][e] = pr;
           dp[nt][e] = pr * (dp[nt][e] - d);
+          if (MODE == D_DQ) error[e >> 1] += dp[nt][e];
         }
+      if (MODE == D_DQ && steps == 1) {  // the whole row is here: its exact delta
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = error[e];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+#pragma unroll
+          for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) dp[nt][2 * e + i] = fmaf(-x, s[nt][2 * e + i], dp[nt][2 * e + i]);
+        }
+      }
       if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
         // a column of sums for every lane: no two threads meet in one, and the order of a sum is that of the walk
 #pragma unroll
@@ -362,6 +398,15 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     }
   }
   cp_async_wait<0>();
+  if (MODE == D_DQ) {  // what DKV gets of delta has no rounding of the output in it
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = error[e];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      if (t4 == 0 && my + 8 * e < p.M) p.delta[stat(oh) + my + 8 * e] = delta[e] + x;
+    }
+  }
 
   // ---- rows out: zeros behind the lengths
   float mul[2] = {1.f, 1.f};
