@@ -6,26 +6,28 @@
 namespace mf {
 namespace {
 
-// dbias[bucket][head] = sum of the partial sums of all tiles of the head: a block for a head and 32 buckets, a warp for every 32nd tile, the warps in
+// dbias[bucket][head] = sum of the partial sums of all tiles of the head: a block for a head and 32 buckets, a warp for every 16th tile, the warps in
 // order.  Sums in fp64: they are long and cancel.
-__global__ void __launch_bounds__(1024) bias_sum_kernel(const float* part, int B, int H, int tiles, int nb, void* out, int dtype) {
+constexpr int kSumWarps = 16;
+__global__ void __launch_bounds__(kSumWarps * 32) bias_sum_kernel(const float* part, int B, int H, int tiles, int nb, void* out, int dtype) {
   launch_dependents();
   wait_for_previous();
   const int h = blockIdx.x % H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bucket = blockIdx.x / H * 32 + lane;
   const int n = B * tiles;
   double sum = 0.0;
   if (bucket < nb) {
-#pragma unroll 4
-    for (int i = warp; i < n; i += 32) {
-      const int b = i / tiles, t = i - b * tiles;
+#pragma unroll 8
+    for (int i = warp; i < n; i += kSumWarps) {
+      const int b = tiles == 1 ? i : i / tiles, t = i - b * tiles;
       sum += part[(((long long)b * H + h) * tiles + t) * nb + bucket];
     }
   }
-  __shared__ double sums[32][33];
+  __shared__ double sums[kSumWarps][32];
   sums[warp][lane] = sum;
   __syncthreads();
   if (warp > 0 || bucket >= nb) return;
-  for (int w = 1; w < 32; ++w) sum += sums[w][lane];
+  #pragma unroll
+  for (int w = 1; w < kSumWarps; ++w) sum += sums[w][lane];
   const float v = (float)sum;
   const int at = bucket * H + h;
   if (dtype == MF_DTYPE_F32) static_cast<float*>(out)[at] = v;
@@ -193,7 +195,7 @@ Family bwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
   return dense_attn_small_applies(p, true) ? kSmall : takes && p.M > 128 && p.N > 256 ? kTensor : kMma;
 }
 
-// delta, then partial sums of the table's gradient for each head: whichever of the tiled families runs, the smaller tiles' number of them fits.
+// delta, then partial sums of the table's gradient for each head: as many as whichever of the tiled families runs needs.
 struct BwdSpace {
   size_t part, total;
 };
@@ -201,7 +203,8 @@ BwdSpace bwd_space(const MfDenseAttnArgs& a, const DenseParams& p) {
   BwdSpace s{};
   const bool small = bwd_family(a, p) == kSmall;
   s.part = small ? 0 : align_up((size_t)a.batch * a.heads * a.queries * sizeof(float), 256);
-  const size_t sums = small ? dense_attn_small_slots(p, a.head_dim, a.bucket_kind) : (size_t)a.batch * dense_attn_mma_tiles(a.queries);
+  auto most = [](size_t x, size_t y) { return x > y ? x : y; };
+  const size_t sums = small ? dense_attn_small_slots(p, a.head_dim, a.bucket_kind) : most(dense_attn_mma_slots(p, a.head_dim), (size_t)a.batch * ((a.queries + kTcRows - 1) / kTcRows));
   s.total = s.part + (a.bias && a.dbias ? align_up(sums * a.heads * a.num_buckets * sizeof(float), 256) : 0);
   return s;
 }
@@ -240,7 +243,7 @@ int backward(const char* name, const MfDenseAttnArgs* a, cudaStream_t stream, Bo
   const bool table = a->bias && a->dbias;
   const BwdSpace space = a->batch ? bwd_space(*a, p) : BwdSpace{};
   if (MF_OK != (rc = check_space(name, a, space.total))) return rc;
-  int entries = a->batch, tiles = dense_attn_mma_tiles(a->queries);  // of partial sums for each head
+  int entries = a->batch, tiles = 1;  // of partial sums for each head
   if (a->batch > 0) {
     MF_CHECK_ARG(a->queries == 0 || (a->grad_out && a->lse), "%s: grad_out and lse must not be NULL", name);
     if ((a->queries > 0 && MF_OK != (rc = check_rows(name, "grad_out", a->grad_out, a->grad_out_rows))) ||
@@ -262,12 +265,14 @@ int backward(const char* name, const MfDenseAttnArgs* a, cudaStream_t stream, Bo
         tiles = (a->queries + kTcRows - 1) / kTcRows;
         rc = dense_attn_sm100_bwd(tc, a->dtype, a->head_dim, a->bucket_kind, stream);
         break;
-      default: rc = dense_attn_mma_bwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
+      default:
+        entries = dense_attn_mma_slots(p, a->head_dim);
+        rc = dense_attn_mma_bwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
     }
     if (rc != MF_OK) return rc;
   }
   if (!table) return MF_OK;
-  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * ((a->num_buckets + 31) / 32)), dim3(1024), 0, stream, p.dbias_part, entries, a->heads, tiles,
+  const cudaError_t err = launch_dependent(bias_sum_kernel, dim3(a->heads * ((a->num_buckets + 31) / 32)), dim3(kSumWarps * 32), 0, stream, p.dbias_part, entries, a->heads, tiles,
                                            a->num_buckets, a->dbias, a->bias_dtype);
   return err == cudaSuccess ? MF_OK : cuda_error(err, "dense attention table gradient");
 }

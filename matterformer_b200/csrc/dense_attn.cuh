@@ -1,6 +1,8 @@
 // What the kernels of dense attention share: the call's operands, which keys a query sees, and the learned bias by buckets.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 #include "sparse_attn_mma.cuh"
 
@@ -35,6 +37,20 @@ struct DenseParams {
   int causal;
   float scale;
 };
+
+// Adds four values to a lane's column of sums, in order; the sums are read together, so that a value does not wait for the one before it to be
+// written (a chain of 40 clocks each): where two go to one sum, the later store holds both.
+__device__ __forceinline__ void add_four(float* column, const int (&at)[4], const float (&d)[4]) {
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = column[at[i] * 32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < i; ++j) v[i] += at[j] == at[i] ? d[j] : 0.f;
+    column[at[i] * 32] = v[i] += d[i];
+  }
+}
 
 struct DenseLengths {
   int nq, nk, shift;  // shift: where the first query stands among the keys
@@ -99,10 +115,22 @@ __device__ __forceinline__ float dense_exp2(float x) {
   return y;
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory, one value for all its calls: asked for once on a device (it takes a microsecond).
+template <auto kernel>
+cudaError_t allow_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess || (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1))) return err;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess && device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
+  return err;
+}
+
 // dense_attn_mma.cu: any call
 int dense_attn_mma_fwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream);
 int dense_attn_mma_bwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream);
-int dense_attn_mma_tiles(int queries);  // query tiles of the backward pass
+int dense_attn_mma_slots(const DenseParams& p, int head_dim);  // partial sums of the table's gradient for each head
 // dense_attn_small.cu: at most 32 queries and keys
 bool dense_attn_small_applies(const DenseParams& p, bool backward);
 int dense_attn_small_slots(const DenseParams& p, int head_dim, int bucket_kind);  // partial sums of the table's gradient for each head

@@ -62,11 +62,28 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int heads = MODE == D_DKV ? p.K : p.H, group = p.H / p.K;
-  // the longest walks of a causal call first
-  const int entries = p.B * heads, tiles = gridDim.x / entries;
-  const int entry = p.causal ? blockIdx.x % entries : blockIdx.x / tiles;
-  const int tile = !p.causal ? blockIdx.x % tiles : MODE == D_DKV ? blockIdx.x / entries : tiles - 1 - (int)(blockIdx.x / entries);
-  const int b = entry / heads, oh = entry % heads;  // oh: of the owners
+  // DQ with a table: CTAs stay with a head and take every slots-th of its tiles, so that the table's column is laid out and its sums are added up once for
+  // all of them; a tile of a small molecule takes less time than that.  Otherwise a tile each, the longest walks of a causal call first.
+  constexpr bool STAY = MODE == D_DQ && KIND != MF_BUCKETS_NONE;
+  const int entries = p.B * heads, tiles = ((MODE == D_DKV ? p.N : p.M) + kOwn - 1) / kOwn, slots = STAY ? gridDim.x / heads : 1;
+  const int nb = p.num_buckets;
+  float* my_sums = sums + (warp * (nb + 1)) * 32 + lane;
+  if (STAY) {
+    if (KIND == MF_BUCKETS_PAIR)
+      for (int i = tid; i < kTableEntries; i += kThreads) table[i] = dense_bias_entry(p, i, blockIdx.x % heads);
+    if (p.dbias_part)
+      for (int i = tid; i < 4 * (nb + 1) * 32; i += kThreads) sums[i] = 0.f;
+  }
+  for (int item = STAY ? blockIdx.x / heads : 0; item < (STAY ? p.B * tiles : 1); item += slots) {
+  const int place = STAY ? item * heads + (int)(blockIdx.x % heads) : (int)blockIdx.x;
+  int tile, b, oh;  // oh: head of the owners
+  if (STAY) {
+    b = item / tiles, tile = item % tiles, oh = place % heads;
+  } else {
+    const int entry = p.causal ? place % entries : place / tiles;
+    tile = !p.causal ? place % tiles : MODE == D_DKV ? place / entries : tiles - 1 - place / entries;
+    b = entry / heads, oh = entry % heads;
+  }
   const int kh = MODE == D_DKV ? oh : oh / group;
   const DenseLengths len = dense_lengths(p, b);
   const int row0 = tile * kOwn;
@@ -157,12 +174,8 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     load_step(0, 0, seen_next);
   }
   cp_async_commit();
-  const int nb = p.num_buckets;
-  if (KIND == MF_BUCKETS_PAIR && MODE != D_DKV)
+  if (KIND == MF_BUCKETS_PAIR && MODE == D_FWD)
     for (int i = tid; i < kTableEntries; i += kThreads) table[i] = dense_bias_entry(p, i, oh);
-  if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part)
-    for (int i = tid; i < 4 * (nb + 1) * 32; i += kThreads) sums[i] = 0.f;
-  float* my_sums = sums + (warp * (nb + 1)) * 32 + lane;
 
   // ---- visible partners of this thread's two rows: [lo, hi).  Rows that are none see what they want, their results are not used: queries behind the
   // last have a log-sum-exp of infinity, as have partners, so that their p is zero.
@@ -356,13 +369,15 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
       if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
         // a column of sums for every lane: no two threads meet in one, and the order of a sum is that of the walk
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
+        for (int nt = 0; nt < 8; ++nt) {
+          int bucket[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
-            const int bucket = KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1] : (which[nt] >> (8 * e)) & 255u;
-            my_sums[min(bucket, nb) * 32] += dp[nt][e];
+            bucket[e] = min((int)(KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1] : (which[nt] >> (8 * e)) & 255u), nb);
           }
+          add_four(my_sums, bucket, dp[nt]);
+        }
       }
     }
 
@@ -442,9 +457,10 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     if (p.dk) store(p.dk, p.dk_rows, acc0, real0 * p.scale, real1 * p.scale);
     if (p.dv) store(p.dv, p.dv_rows, acc1, real0, real1);
   }
-  if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
-    __syncthreads();
-    float* part = p.dbias_part + ((long long)entry * tiles + tile) * nb;
+  if (STAY) __syncthreads();  // before the next tile's rows arrive
+  }
+  if (STAY && p.dbias_part) {
+    float* part = p.dbias_part + ((long long)(blockIdx.x / heads) * heads + blockIdx.x % heads) * nb;
     for (int i = warp; i < nb; i += 4) {
       float v = 0.f;
 #pragma unroll
@@ -455,18 +471,27 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
   }
 }
 
+// CTAs of a head in the pass that sums the table's gradient: as many as fit the chip, at most one for each tile.
+int slots_of(const DenseParams& p, int head_dim) {
+  const long long tiles = (long long)p.B * ((p.M + kOwn - 1) / kOwn);
+  const int smem = 6 * 64 * (head_dim + 8) * 2 + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 5 + 2 * kPairTile + 4 * (p.num_buckets + 1) * 32 * 4 + 1024;
+  const int fit = 227 * 1024 / smem, most = 148 * (fit < 1 ? 1 : fit > 3 ? 3 : fit) / p.H;
+  return (int)(tiles < most ? tiles : most < 1 ? 1 : most);
+}
+
 template <typename T, int D, int MODE, int KIND>
 int launch(const DenseParams& p, cudaStream_t stream) {
   const int own = MODE == D_DKV ? p.N : p.M, heads = MODE == D_DKV ? p.K : p.H;
   if (own == 0) return MF_OK;
   const int smem = kFixedBytes<D, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
-  auto kernel = dense_attn_mma_kernel<T, D, MODE, KIND>;
+  constexpr auto kernel = dense_attn_mma_kernel<T, D, MODE, KIND>;
   // one limit for all calls: what the largest table needs
   constexpr int most = kFixedBytes<D, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
   static_assert(most <= 227 * 1024, "");
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  const cudaError_t err = allow_shared<dense_attn_mma_kernel<T, D, MODE, KIND>>(most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
-  kernel<<<(own + kOwn - 1) / kOwn * p.B * heads, kThreads, smem, stream>>>(p);
+  const bool stays = MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part;
+  kernel<<<stays ? slots_of(p, D) * heads : (own + kOwn - 1) / kOwn * p.B * heads, kThreads, smem, stream>>>(p);
   MF_CHECK_LAUNCH("dense attention");
   return MF_OK;
 }
@@ -486,7 +511,7 @@ int pick(const DenseParams& p, int head_dim, int kind, cudaStream_t stream) {
 
 }  // namespace
 
-int dense_attn_mma_tiles(int queries) { return (queries + kOwn - 1) / kOwn; }
+int dense_attn_mma_slots(const DenseParams& p, int head_dim) { return p.M ? slots_of(p, head_dim) : 0; }
 int dense_attn_mma_fwd(const DenseParams& p, int dtype, int head_dim, int kind, cudaStream_t stream) {
   return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16, D_FWD>(p, head_dim, kind, stream) : pick<__half, D_FWD>(p, head_dim, kind, stream);
 }

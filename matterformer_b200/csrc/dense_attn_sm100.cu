@@ -363,8 +363,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
 template <typename T, int D, int KIND>
 int launch(const DenseTcParams& tc, cudaStream_t stream) {
   const DenseParams& p = tc.p;
-  auto kernel = dense_attn_tc_kernel<T, D, KIND>;
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdShape<D>::kSmem);
+  constexpr auto kernel = dense_attn_tc_kernel<T, D, KIND>;
+  const cudaError_t err = allow_shared<dense_attn_tc_kernel<T, D, KIND>>(FwdShape<D>::kSmem);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   const bool by_head = (p.H / p.K) % 2 == 0;
   const long long tiles = (p.M + kTcRows - 1) / kTcRows, blocks = by_head ? tiles * p.B * (p.H / 2) : (tiles + 1) / 2 * p.B * p.H;

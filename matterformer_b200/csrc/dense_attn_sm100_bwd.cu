@@ -558,12 +558,12 @@ template <typename T, int D, bool DKV, bool TABLE>
 int launch(const DenseTcParams& tc, cudaStream_t stream) {
   const DenseParams& p = tc.p;
   using Sh = BwdShape<D, DKV, TABLE && !DKV>;
-  auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
+  constexpr auto kernel = dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>;
   auto offset_bytes = [](int reach) { return (2 * reach + 2 * kSpan - 1) * (DKV ? 2 * 4 : 4 + 1); };
   constexpr int most = Sh::kSmem + 1024 + (TABLE && !DKV ? 4 * Sh::kDiagonalBytes + Sh::kMostBuckets * 1024 : 0) + (TABLE ? (2 * kMostReach + 2 * kSpan - 1) * 8 : 0);
   static_assert(most <= 227 * 1024 - (DKV ? 512 : 2560), "beside the static part");
   const int smem = Sh::kSmem + 1024 + (TABLE && !DKV && p.dbias_part ? 4 * Sh::kDiagonalBytes + p.num_buckets * 1024 : 0) + (TABLE ? offset_bytes(p.reach) : 0);
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  const cudaError_t err = allow_shared<dense_attn_tc_bwd_kernel<T, D, DKV, TABLE>>(most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   const long long blocks = (long long)(((DKV ? p.N : p.M) + kTcRows - 1) / kTcRows) * p.B * (DKV ? p.K : p.H);
   kernel<<<(unsigned)blocks, kBwdThreads, smem, stream>>>(tc);

@@ -264,7 +264,11 @@ __global__ void __launch_bounds__(kWarps * 32, BWD || D == 128 ? 5 : 8) dense_at
           }
           if (table_grad) {  // a column of sums for every lane: no two threads meet in one
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sums[bucket_of(row, k) * 32] += dp[k >> 1][2 * x + (k & 1)];
+            for (int k = 0; k < 8; k += 4) {
+              const int at[4] = {bucket_of(row, k), bucket_of(row, k + 1), bucket_of(row, k + 2), bucket_of(row, k + 3)};
+              const float d4[4] = {dp[k >> 1][2 * x], dp[k >> 1][2 * x + 1], dp[(k >> 1) + 1][2 * x], dp[(k >> 1) + 1][2 * x + 1]};
+              add_four(sums, at, d4);
+            }
           }
         }
       }
@@ -367,10 +371,10 @@ int launch(const DenseParams& p, cudaStream_t stream) {
   const bool table_grad = BWD && KIND != MF_BUCKETS_NONE && p.dbias_part;
   const int smem = smem_of(p, D, KIND, BWD, table_grad);
   SmallParams sp{p, slots_of(p, D, KIND, BWD, table_grad)};
-  auto kernel = dense_attn_small_kernel<T, D, KIND, BWD>;
+  constexpr auto kernel = dense_attn_small_kernel<T, D, KIND, BWD>;
   constexpr int most = kWarps * (kTilesBytes<D, BWD> + small_table_bytes(KIND, kMaxBuckets) + (BWD && KIND != MF_BUCKETS_NONE ? (kMaxBuckets + 1) * 32 * 4 : 0));
   static_assert(most <= 227 * 1024, "");
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  cudaError_t err = allow_shared<dense_attn_small_kernel<T, D, KIND, BWD>>(most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   const long long warps = (long long)sp.slots * p.H;
   err = launch_dependent(kernel, dim3((unsigned)((warps + kWarps - 1) / kWarps)), dim3(kWarps * 32), smem, stream, sp);

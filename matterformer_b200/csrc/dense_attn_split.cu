@@ -313,10 +313,10 @@ int launch(const DenseParams& p, void* workspace, cudaStream_t stream) {
   const Plan plan = plan_of(p);
   SplitParams sp{p, plan.pieces, plan.piece, static_cast<float*>(workspace), nullptr};
   sp.stat = sp.acc + plan.blocks * kRows * D;
-  auto kernel = dense_attn_split_kernel<T, D, KIND>;
+  constexpr auto kernel = dense_attn_split_kernel<T, D, KIND>;
   const int group = p.H / p.K, smem = kSplitSmem<D> + (KIND == MF_BUCKETS_NONE ? 0 : (group < kRows ? group : kRows) * (p.num_buckets + 1) * 4);
   constexpr int most = kSplitSmem<D> + (KIND == MF_BUCKETS_NONE ? 0 : kRows * (kMaxBuckets + 1) * 4);
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  cudaError_t err = allow_shared<dense_attn_split_kernel<T, D, KIND>>(most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   err = launch_dependent(kernel, dim3((unsigned)plan.blocks), dim3(kThreads), smem, stream, sp);
   if (err != cudaSuccess) return cuda_error(err, "dense attention of few queries");
