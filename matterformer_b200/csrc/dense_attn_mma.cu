@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
   float error[2] = {0.f, 0.f};  // sums of dS, zero but for what delta is off by
 
 
+  const bool idle = row0 + warp * 16 >= own_limit;  // a warp without a row brings tiles along and no more
   for (int t = 0; t < steps; ++t) {
     const int stage = t & 1;
     const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
@@ -249,6 +250,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_c
     if (t + 1 < steps) load_step(t + 1, stage ^ 1, seen_next);
     cp_async_commit();
 
+    if (idle) continue;
     const uint32_t pa = s_part_a + stage * TILE, pb = s_part_b + stage * TILE;
     float s[8][4], dp[MODE == D_FWD ? 1 : 8][4];
 #pragma unroll
