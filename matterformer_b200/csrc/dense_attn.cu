@@ -52,23 +52,28 @@ __device__ __forceinline__ uint32_t param_word(const void* at) {
 constexpr float kDistanceError = 5e-7f;  // of a squared distance in fp32, in relation to it; 6 * 2^-24 and an edge's rounding
 
 // A thread takes four columns, whose coordinates stay in registers, and walks over rows: `lanes` threads (a power of two up to 32) lie along a row, the rest
-// of the block along the rows.  The squared distance is formed in
-// fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares) and its bucket found from a table of cells, of which few hold more than one edge;
-// a pair within that error of an edge, or whose square leaves fp32's range, is decided in fp64, where the differences of fp32 coordinates are exact but for
-// far apart exponents.  All pairs in fp64 against all edges took 463 us for two cells of 4096 atoms and 63 edges.
-constexpr int kBucketThreads = 256, kBucketSteps = 8;
+// of the block along the rows.  The squared distance is formed in fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares); its leading bits name a cell, which
+// knows the buckets below it and the one edge in it, if any: one load, one comparison.  A pair within that error of the edge, in a cell that several edges share
+// or so near that squares leave fp32's range is decided in fp64, where the differences of fp32 coordinates are exact but for far apart exponents.
+// What bounds it is instructions, some twenty a pair; all pairs in fp64 against all edges took 463 us for two cells of 4096 atoms and 63 edges.
+constexpr int kBucketThreads = 256, kBucketSteps = 16;
 __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int N, const __grid_constant__ Edges edges,
                                                                           uint8_t* out, long long batch_stride, long long row, int words, int lanes, int column_tiles,
                                                                           int row_tiles) {
-  __shared__ float2 around[kMaxEdges + 1];  // the squared edges below and above a bucket, a margin within it
-  __shared__ uint32_t first_words[kCells / 4];
-  const uint8_t* first = reinterpret_cast<const uint8_t*>(first_words);
+  __shared__ float2 cells[kCells];  // the edge (infinity: none; not a number: several), the bucket below it as an integer
   launch_dependents();
-  // (through a generic address: loads of parameters go by the constant cache, one address of a warp after the other)
-  for (int i = threadIdx.x; i < kCells / 4; i += kBucketThreads) first_words[i] = param_word(edges.first + 4 * i);
-  for (int i = threadIdx.x; i <= edges.n; i += kBucketThreads)
-    around[i] = make_float2(fmaxf(1e-30f, i ? __uint_as_float(param_word(edges.low + i - 1)) * (1.f + kDistanceError) : 0.f),
-                            i < edges.n ? fminf(1e30f, __uint_as_float(param_word(edges.low + i)) * (1.f - kDistanceError)) : 1e30f);
+  // (through generic addresses: loads of parameters go by the constant cache, one address of a warp after the other)
+  for (int w = threadIdx.x; w < kCells / 4; w += kBucketThreads) {
+    const uint32_t four = param_word(edges.first + 4 * w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 4 * w + e, k = (four >> (8 * e)) & 255u;
+      const float end = c == kCells - 1 ? INFINITY : __int_as_float(max(0, c + 1 + edges.base) << kCellShift) * (1.f + 2 * kDistanceError);
+      const float one = k < edges.n ? __uint_as_float(param_word(edges.low + k)) : INFINITY;
+      const float two = k + 1 < edges.n ? __uint_as_float(param_word(edges.low + k + 1)) : INFINITY;
+      cells[c] = make_float2(c == 0 || (k + 1 < edges.n && two <= end) ? __int_as_float(0x7fffffff) : one <= end ? one : INFINITY, __int_as_float(k));
+    }
+  }
   wait_for_previous();
   __syncthreads();
   const int ct = blockIdx.x % column_tiles, rt = blockIdx.x / column_tiles % row_tiles, b = blockIdx.x / column_tiles / row_tiles;
@@ -81,27 +86,35 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int a = 0; a < 3; ++a) y[c][a] = j0 + c < n ? x[(j0 + c) * 3ll + a] : 0.f;
+  const uint32_t there = j0 + 4 <= n ? ~0u : j0 < n ? (1u << (8 * (n - j0))) - 1u : 0u;  // bytes of columns that are atoms
   const int last = min(i0 + at_once * (kBucketSteps - 1), N - 1);
-  for (int i = i0; i <= last; i += at_once) {
+  const float* xi = x + i0 * 3ll;
+  uint8_t* dst = out + b * batch_stride + i0 * row + j0;
+  const uint8_t* at_cells = reinterpret_cast<const uint8_t*>(cells) - 8ll * edges.base;
+  const int lowest = edges.base, highest = edges.base + kCells - 1;
+#pragma unroll 2
+  for (int i = i0; i <= last; i += at_once, xi += at_once * 3, dst += at_once * row) {
     uint32_t word = 0;
     if (i < n) {
-      const float xi[3] = {x[i * 3ll], x[i * 3ll + 1], x[i * 3ll + 2]};
-      int k[4];
+      const float p0 = xi[0], p1 = xi[1], p2 = xi[2];
       bool sure = true;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float dx = xi[0] - y[c][0], dy = xi[1] - y[c][1], dz = xi[2] - y[c][2];
+        const float dx = p0 - y[c][0], dy = p1 - y[c][1], dz = p2 - y[c][2];
         const float d2 = fmaf(dz, dz, fmaf(dy, dy, dx * dx));
-        const int cell = max(0, min(kCells - 1, (__float_as_int(d2) >> kCellShift) - edges.base));
-        k[c] = first[cell];
-        k[c] = min(k[c] + (d2 >= around[k[c]].y), edges.n);
-        const float2 e = around[k[c]];
-        sure = sure && d2 > e.x && d2 < e.y;
+        const int cell = max(lowest, min(highest, __float_as_int(d2) >> kCellShift));
+        const float2 e = *reinterpret_cast<const float2*>(at_cells + 8 * cell);
+        const float past = d2 - e.x;
+        sure = sure && fabsf(past) > d2 * kDistanceError;
+        word |= (uint32_t)(__float_as_int(e.y) + (past >= 0.f)) << (8 * c);
       }
       if (!sure) {
+        word = 0;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          const double ex = (double)xi[0] - y[c][0], ey = (double)xi[1] - y[c][1], ez = (double)xi[2] - y[c][2];
+          const float* o = x + (j0 + c) * 3ll;
+          if (j0 + c >= n) break;
+          const double ex = (double)p0 - o[0], ey = (double)p1 - o[1], ez = (double)p2 - o[2];
           const double e2 = __dadd_rn(__dadd_rn(__dmul_rn(ex, ex), __dmul_rn(ey, ey)), __dmul_rn(ez, ez));
           int lo = 0, hi = edges.n;  // edges below lo are at or below the distance, those from hi on above it
           while (lo < hi) {
@@ -109,16 +122,11 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
             if (e2 >= edges.square[mid]) lo = mid + 1;
             else hi = mid;
           }
-          if (c == 0) k[0] = lo;
-          else if (c == 1) k[1] = lo;
-          else if (c == 2) k[2] = lo;
-          else k[3] = lo;
+          word |= (uint32_t)lo << (8 * c);
         }
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) word |= (j0 + c < n ? (uint32_t)k[c] : 0u) << (8 * c);
+      word &= there;
     }
-    uint8_t* dst = out + b * batch_stride + i * row + j0;
     if (words) {  // rows that hold whole words, behind the last atom too
       if (j0 < row) *reinterpret_cast<uint32_t*>(dst) = word;
     } else {
