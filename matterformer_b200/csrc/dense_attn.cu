@@ -42,7 +42,7 @@ struct Edges {
   double square[kMaxEdges];  // of the edges
   float low[kMaxEdges];      // the same in fp32
   alignas(4) uint8_t first[kCells];  // edges below a cell
-  int base, n;
+  int base, n, zeros;  // zeros: edges of a distance of zero
 };
 __device__ __forceinline__ uint32_t param_word(const void* at) {
   uint32_t v;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
     uint32_t word = 0;
     if (i < n) {
       const float p0 = xi[0], p1 = xi[1], p2 = xi[2];
-      bool sure = true;
+      uint32_t unsure = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float dx = p0 - y[c][0], dy = p1 - y[c][1], dz = p2 - y[c][2];
@@ -105,22 +105,28 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
         const int cell = max(lowest, min(highest, __float_as_int(d2) >> kCellShift));
         const float2 e = *reinterpret_cast<const float2*>(at_cells + 8 * cell);
         const float past = d2 - e.x;
-        sure = sure && fabsf(past) > d2 * kDistanceError;
+        if (!(fabsf(past) > d2 * kDistanceError)) unsure |= 255u << (8 * c);
         word |= (uint32_t)(__float_as_int(e.y) + (past >= 0.f)) << (8 * c);
       }
-      if (!sure) {
-        word = 0;
+      unsure &= there;
+      if (unsure) {
+        word &= ~unsure;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
+          if (!((unsure >> (8 * c)) & 1u)) continue;
           const float* o = x + (j0 + c) * 3ll;
-          if (j0 + c >= n) break;
-          const double ex = (double)p0 - o[0], ey = (double)p1 - o[1], ez = (double)p2 - o[2];
-          const double e2 = __dadd_rn(__dadd_rn(__dmul_rn(ex, ex), __dmul_rn(ey, ey)), __dmul_rn(ez, ez));
+          const float q0 = o[0], q1 = o[1], q2 = o[2];
           int lo = 0, hi = edges.n;  // edges below lo are at or below the distance, those from hi on above it
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (e2 >= edges.square[mid]) lo = mid + 1;
-            else hi = mid;
+          if (p0 == q0 && p1 == q1 && p2 == q2) {  // an atom and itself: every row has one
+            lo = hi = edges.zeros;
+          } else {
+            const double ex = (double)p0 - q0, ey = (double)p1 - q1, ez = (double)p2 - q2;
+            const double e2 = __dadd_rn(__dadd_rn(__dmul_rn(ex, ex), __dmul_rn(ey, ey)), __dmul_rn(ez, ez));
+            while (lo < hi) {
+              const int mid = (lo + hi) / 2;
+              if (e2 >= edges.square[mid]) lo = mid + 1;
+              else hi = mid;
+            }
           }
           word |= (uint32_t)lo << (8 * c);
         }
@@ -347,6 +353,7 @@ int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t b
     e.low[i] = (float)e.square[i];
   }
   e.n = num_edges;
+  while (e.zeros < num_edges && e.square[e.zeros] == 0.0) ++e.zeros;
   auto bits = [](float f) { int i; memcpy(&i, &f, 4); return i; };
   auto value = [](int i) { float f; memcpy(&f, &i, 4); return f; };
   const float last = num_edges ? e.low[num_edges - 1] : 0.f;
