@@ -47,7 +47,7 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const T* src, long long
 }
 
 template <typename T, int D, int MODE, int KIND>
-__global__ void __launch_bounds__(kThreads) dense_attn_mma_kernel(const __grid_constant__ DenseParams p) {
+__global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 2) dense_attn_mma_kernel(const __grid_constant__ DenseParams p) {
   constexpr int LD = D + 8, TILE = kTileBytes<D>, KS = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t s_own_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), s_own_b = s_own_a + TILE;
