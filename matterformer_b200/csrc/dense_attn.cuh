@@ -136,7 +136,7 @@ bool dense_attn_small_applies(const DenseParams& p, bool backward);
 int dense_attn_small_slots(const DenseParams& p, int head_dim, int bucket_kind);  // partial sums of the table's gradient for each head
 int dense_attn_small(const DenseParams& p, int dtype, int head_dim, int bucket_kind, bool backward, cudaStream_t stream);
 // dense_attn_split.cu: forward, few queries
-bool dense_attn_split_applies(const DenseParams& p);
+bool dense_attn_split_applies(const DenseParams& p, int head_dim);
 size_t dense_attn_split_workspace_bytes(const DenseParams& p, int head_dim);
 int dense_attn_split(const DenseParams& p, int dtype, int head_dim, int bucket_kind, void* workspace, cudaStream_t stream);
 

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) dense_attn_split_kernel(const __grid
   }
 }
 
-// A block per row: the pieces' weights into shared memory, then 128 / (D / 4) shares of the pieces, four channels to a thread, each share in order
+// More than 32 pieces: a block per row, the pieces' weights into shared memory, then 128 / (D / 4) shares of the pieces, four channels to a thread, each share in order
 // and the shares in order.
 constexpr int kMostPieces = 320;
 template <typename T, int D>
@@ -288,6 +288,53 @@ __global__ void __launch_bounds__(128) dense_attn_join_kernel(const __grid_const
   if (p.lse && tid == 0) p.lse[((long long)b * p.H + h) * p.M + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
 }
 
+// Up to 32 pieces: a warp per row, a lane for the weight of each piece and D / 32 channels, the pieces in order.  (2048 rows of two pieces, with the walk over 512
+// keys each: 13 us; with a block per row 17.)
+template <typename T, int D>
+__global__ void __launch_bounds__(128) dense_attn_join_few_kernel(const __grid_constant__ SplitParams sp, int total_rows) {
+  const DenseParams& p = sp.p;
+  constexpr int E = D / 32;
+  launch_dependents();
+  wait_for_previous();
+  const int lane = threadIdx.x & 31, at = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (at >= total_rows) return;
+  const int group = p.H / p.K, rows = p.M * group, row_tiles = (rows + kRows - 1) / kRows;
+  const int row = at % rows, entry = at / rows, b = entry / p.K, kh = entry % p.K;
+  const long long base = ((long long)entry * row_tiles + row / kRows) * sp.pieces;
+  auto slot = [&](int s) { return (base + s) * kRows + row % kRows; };
+  const float t = lane < sp.pieces ? sp.stat[slot(lane) * 2] : -INFINITY;
+  const float m = warp_max(t), w = t == -INFINITY ? 0.f : dense_exp2(t - m);
+  const float l = warp_sum(w != 0.f ? w * sp.stat[slot(lane) * 2 + 1] : 0.f);
+  float sum[E] = {};
+#pragma unroll 4
+  for (int s = 0; s < sp.pieces; ++s) {
+    const float ws = __shfl_sync(~0u, w, s);
+    if (ws == 0.f) continue;  // (a piece without a key that the row sees wrote nothing)
+    const float* x = sp.acc + slot(s) * D + lane * E;
+    float v[E];
+    if constexpr (E == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(x);
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else if constexpr (E == 2) {
+      const float2 f = *reinterpret_cast<const float2*>(x);
+      v[0] = f.x, v[1] = f.y;
+    } else {
+      v[0] = *x;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = fmaf(ws, v[e], sum[e]);
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int i = row / group, h = kh * group + row % group;
+  T* out = static_cast<T*>(p.out) + p.out_rows.at(b, h, i) + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = inv == 0.f ? 0.f : sum[e] * inv;
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]));
+  else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(out) = pack2<T>(sum[0], sum[1]);
+  else *out = from_f32<T>(sum[0]);
+  if (p.lse && lane == 0) p.lse[((long long)b * p.H + h) * p.M + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
+}
+
 struct Plan {
   int row_tiles, pieces, piece;
   long long blocks;
@@ -322,7 +369,8 @@ int launch(const DenseParams& p, void* workspace, cudaStream_t stream) {
   if (err != cudaSuccess) return cuda_error(err, "dense attention of few queries");
   if (plan.pieces > 1) {
     const long long rows = (long long)p.B * p.H * p.M;
-    err = launch_dependent(dense_attn_join_kernel<T, D>, dim3((unsigned)rows), dim3(128), 0, stream, sp);
+    err = plan.pieces <= 32 ? launch_dependent(dense_attn_join_few_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, sp, (int)rows)
+                            : launch_dependent(dense_attn_join_kernel<T, D>, dim3((unsigned)rows), dim3(128), 0, stream, sp);
     if (err != cudaSuccess) return cuda_error(err, "dense attention join");
   }
   return MF_OK;
@@ -343,11 +391,15 @@ int pick(const DenseParams& p, int head_dim, int kind, void* workspace, cudaStre
 
 }  // namespace
 
-// Few rows to a key head, or so few tiles of 64 queries that most SMs would stand idle through a long walk.
-bool dense_attn_split_applies(const DenseParams& p) {
+// Few rows to a key head, or so few tiles of 64 queries that most SMs would stand idle through a long walk.  Microseconds here | on the better of the other
+// families: one query, 8 heads of 64, 65 keys 3.3 | 5.2, 512 keys 5.8 | 9.8, 64 entries of 1024 keys 31 | 50; 64 queries on 1024 keys, 8 tiles 8 | 15, 32 tiles 13 | 16,
+// 56 tiles 16 | 15; on 2048 keys 64 tiles 24 | 27.  At head size 128 32 tiles on 2048 keys
+// 22 | 31, 64 tiles 45 | 31.
+bool dense_attn_split_applies(const DenseParams& p, int head_dim) {
   if (p.N <= 64 || p.N > (1 << 26)) return false;
+  if ((long long)p.M * (p.H / p.K) <= kRows) return true;
   const long long tiles = (long long)p.B * p.H * ((p.M + 63) / 64);
-  return (long long)p.M * (p.H / p.K) <= kRows || (p.N >= 512 && tiles < 74 && p.M <= 256);
+  return p.M <= 256 && p.N >= 512 && tiles <= (p.N >= 2048 && head_dim < 128 ? 73 : 32);
 }
 size_t dense_attn_split_workspace_bytes(const DenseParams& p, int head_dim) {
   const Plan plan = plan_of(p);
