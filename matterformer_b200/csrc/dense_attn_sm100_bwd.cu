@@ -493,6 +493,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       }
     }
     if (table_grad) {
+      group_barrier(7, 512);  // a group without a step is here while the other may still read its delta
       errors[team][r] = all;  // four threads worked on the row
       group_barrier(7, 512);
       all = (errors[0][r] + errors[1][r]) + (errors[2][r] + errors[3][r]);
