@@ -9,6 +9,10 @@
 // Logits, probabilities and their gradients stay in registers: the C fragment of a product is the A operand of the next.  P and dS are
 // rounded to the operands' type there (half a unit of 2^-8 or 2^-11 each, on terms of a sum), the only type the tensor cores take.
 // Every output has one owner and a fixed order of its sums.
+//
+// Registers bound it: 64 x 64 logits, their gradients and the sums are 128 to 168 of a thread's, three or four CTAs on an SM (without that limit 255 and two, 64
+// molecules of 19 to 192 tokens 124 us instead of 120 for forward and backward), which use a third of the issue slots and a fifth of the tensor pipe. There: forward 27,
+// DQ 49, DKV 45 us; 8 x 577 fp16 queries on 1000 keys, 4 heads of 32, 22 + 26 + 19 us. 64 rows to a tile: fewer waste products for molecules of all lengths.
 #include "dense_attn.cuh"
 
 namespace mf {

