@@ -76,6 +76,7 @@ def _distance_buckets_torch(coords, edges, num_atoms):
     d = x[:, :, None] - x[:, None]
     d2 = d[..., 0].square() + d[..., 1].square() + d[..., 2].square()
     out = torch.searchsorted(edges.square().to(x.device), d2.contiguous(), right=True)
+    out = torch.where(d2.isnan(), 0, out)  # (a search takes what is not a number for the largest)
     if num_atoms is not None:
         real = torch.arange(N, device=x.device) < num_atoms.reshape(-1, 1)
         out = torch.where(real[:, :, None] & real[:, None], out, 0)
@@ -84,7 +85,8 @@ def _distance_buckets_torch(coords, edges, num_atoms):
 
 def distance_buckets(coords: torch.Tensor, edges: Union[torch.Tensor, Sequence[float]], num_atoms: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(B, N, N) uint8: how many of the ascending ``edges`` (host values in fp64, at most 127, from 0 on) lie at or below the distance of two atoms of
-    ``coords`` (B, N, 3) fp32, compared as squares in 64 bits.  0 where one of the two is padding (at or behind ``num_atoms`` (B)).  On CUDA
+    ``coords`` (B, N, 3) fp32, compared as squares in 64 bits.  0 where one of the two is padding (at or behind ``num_atoms`` (B))
+    or where the distance is not a number.  On CUDA
     the rows start on 16-byte boundaries, as :func:`dense_attention` reads them fastest (the result is a view of a wider tensor).  No gradient."""
     native = _lib.native()
     if native is not None and isinstance(edges, torch.Tensor):
@@ -373,7 +375,7 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_keys:
                     key_mask: Optional[torch.Tensor] = None, causal: bool = False, bias: Optional[torch.Tensor] = None,
                     buckets: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:  # fmt: skip
     """``q`` (B, H, M, D), ``k`` and ``v`` (B, K, N, D) bf16 or fp16, H a multiple of K (query head h reads key head h * K // H), D 32, 64 or 128, any
-    strides with adjacent channels.  Returns (B, H, M, D) with the tokens and heads in memory as ``q`` has them.
+    strides with adjacent channels (expanded dimensions keep to the warp-level kernels; shared key heads are fastest as K heads).  Returns (B, H, M, D) with the tokens and heads in memory as ``q`` has them.
 
     ``num_keys``, ``num_queries``: (B,) counts of real keys and queries, which come first; what lies behind them may hold anything and returns
     zeros, as does a query that sees no key.  ``key_mask``: (B, N) bool, False hides a key.  ``causal``: the last real query stands at the last

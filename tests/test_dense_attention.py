@@ -231,3 +231,10 @@ def test_trunks_and_models():
         RegularAttention(64, 2, impl="cuda")(torch.randn(3, 9, 64))
     with pytest.raises(ValueError, match="Unsupported attention impl"):
         AdaLNBlock(64, 2, mha_impl="triton")
+
+
+def test_distances_that_are_no_numbers_have_no_bucket():
+    x = torch.zeros(1, 4, 3)
+    x[0, 1, 0], x[0, 2, 1], x[0, 3, 2] = float("nan"), float("inf"), 1.5
+    want = torch.tensor([[0, 0, 2, 1], [0, 0, 0, 0], [2, 0, 0, 2], [1, 0, 2, 0]], dtype=torch.uint8)
+    assert torch.equal(mfb.distance_buckets(x, [1.0, 2.0])[0], want)

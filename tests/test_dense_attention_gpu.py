@@ -322,6 +322,32 @@ def test_repeated_calls_are_bit_equal(B, H, K, M, N, D, bias):
     assert int(differ) == 0
 
 
+@pytest.mark.parametrize("M,N", [(29, 29), (3, 700), (150, 140), (300, 400)])
+def test_broadcast_operands(request, M, N):
+    """Keys of one head for all, one key for all places, one query for all: strides of zero, and their gradients before they are added up.
+    Such operands run on the warp-level family where dense ones may run on tcgen05: equal bits are asked for where both run on one, the bounds always."""
+    g, q, k, v, grad = operands(M + N, 2, 4, 2, M, N, 64, torch.bfloat16)
+    table, buckets = torch.randn(16, 4, generator=g, device="cuda"), mfb.offset_buckets(16, 40, device="cuda")
+    same = lambda t, d: t.narrow(d, 0, 1).expand_as(t)  # noqa: E731
+    for x, y, z in ((q, same(k, 1), same(v, 1)), (same(q, 2), k, v), (q, same(k, 2), v), (same(q, 0), same(k, 0), same(v, 2))):
+        got = run_both(x, y, z, grad, bias=table, buckets=buckets)
+        if request.node.callspec.params["backend"] == "mma":
+            dense = run_both(*(t.contiguous() for t in (x, y, z)), grad, bias=table, buckets=buckets)
+            assert all(torch.equal(got[n], dense[n]) for n in got)
+    leaf = k[:, :1].detach().clone().requires_grad_()
+    out = mfb.dense_attention(q, leaf.expand_as(k), v, bias=table, buckets=buckets)
+    made = torch.autograd.grad(out, leaf, grad)[0]
+    whole = run_both(q, same(k, 1), v, grad, bias=table, buckets=buckets)["dk"]
+    assert torch.equal(made, whole.sum(1, keepdim=True))
+
+
+def test_distances_that_are_no_numbers():
+    x = torch.randn(2, 70, 3, generator=torch.Generator().manual_seed(0)) * 3
+    x[0, 5, 1], x[1, 0, 0], x[1, 40, 2], x[1, 41, 2] = float("nan"), float("inf"), -float("inf"), 3e38
+    edges = torch.linspace(0.0, 12.0, 32, dtype=torch.float64)[1:]
+    assert torch.equal(mfb.distance_buckets(x.cuda(), edges).cpu(), mfb.distance_buckets(x, edges))
+
+
 def test_no_wait_expired_in_all_of_these():
     """Runs last: the status word gathers since it was last asked for."""
     assert mfb.dense_attention_status() == 0
