@@ -199,25 +199,26 @@ DenseParams params_of(const MfDenseAttnArgs& a) {
 enum Family { kMma, kSmall, kSplit, kTensor };
 // Where tiles of 128 rows on tcgen05 pay against warp-level tiles of 64 (microseconds on tcgen05 | warp-level, forward, then forward with backward, 8 heads, bias by the
 // offset).  Head size 64: 64 x 256 tokens 39 | 57, 203 | 239; 64 x 200 tokens 43 | 54, 202 | 222; 42 x 384 tokens 52 | 75; 64 x 700 queries on 100 keys 85 | 89, 337 | 369;
-// 8 x 64 queries on 1024 keys 17 | 25, 65 | 81 (64 of them 64 | 73, 326 | 289); but 85 x 192 tokens 53 | 46,
-// 128 x 128 tokens 41 | 35, and equal from 257 to 300 tokens, where a third of a tile's rows is padding.  Head size 128, whose products weigh more: 128 x 65 tokens
-// 51 | 54, 209 | 267; 128 x 128 tokens 55 | 65, 257 | 305; but 128 x 64 tokens 51 | 25, and with few entries 2 x 160 tokens 13 | 10, 46 | 38; 8 x 64 queries
-// on 2048 keys 31 | 54.
-bool tensor_pays(const DenseParams& p, int head_dim) {
+// 8 x 64 queries on 1024 keys 17 | 25, 65 | 81 (64 of them 64 | 73, 326 | 289); but 85 x 192 tokens 53 | 46, 128 x 128 tokens 41 | 35, and equal from 257 to 300 tokens,
+// where a third of a tile's rows is padding.  Head size 128: 64 x 256 tokens 55 | 99, 302 | 400; 64 x 700 queries on 100 keys 110 | 157, 511 | 604; 85 x 192 tokens 67 | 80
+// forward, but 279 | 248 backward, and by pairs 76 | 67 forward.  There many short entries pay forward unless by pairs: 128 x 128 tokens 54 | 64, 128 x 65 tokens 51 | 54; few
+// do not: 2 x 160 tokens 13 | 10.
+bool tensor_pays(const DenseParams& p, int head_dim, int kind, bool backward) {
   if (p.M < 64 || p.N <= 64) return false;
-  return ((p.M + 63ll) / 64) * ((p.N + 63ll) / 64) >= 16 || (head_dim == 128 && (long long)p.B * p.H >= 148);
+  if (((p.M + 63ll) / 64) * ((p.N + 63ll) / 64) >= 16) return true;
+  return !backward && head_dim == 128 && kind != MF_BUCKETS_PAIR && (long long)p.B * p.H >= 148;
 }
 Family fwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
   if (a.backend == MF_DENSE_BACKEND_MMA) return kMma;
   const bool takes = dense_tc_takes(p, a.head_dim, a.bucket_kind);
   if (a.backend == MF_DENSE_BACKEND_TCGEN05) return takes ? kTensor : kMma;
-  return dense_attn_small_applies(p, false) ? kSmall : dense_attn_split_applies(p, a.head_dim) ? kSplit : takes && tensor_pays(p, a.head_dim) ? kTensor : kMma;
+  return dense_attn_small_applies(p, false) ? kSmall : dense_attn_split_applies(p, a.head_dim) ? kSplit : takes && tensor_pays(p, a.head_dim, a.bucket_kind, false) ? kTensor : kMma;
 }
 Family bwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
   if (a.backend == MF_DENSE_BACKEND_MMA) return kMma;
   const bool takes = dense_tc_bwd_takes(p, a.head_dim, a.bucket_kind, a.bias && a.dbias);
   if (a.backend == MF_DENSE_BACKEND_TCGEN05) return takes ? kTensor : kMma;
-  return dense_attn_small_applies(p, true) ? kSmall : takes && tensor_pays(p, a.head_dim) ? kTensor : kMma;
+  return dense_attn_small_applies(p, true) ? kSmall : takes && tensor_pays(p, a.head_dim, a.bucket_kind, true) ? kTensor : kMma;
 }
 
 // delta, then partial sums of the table's gradient for each head: as many as whichever of the tiled families runs needs.

@@ -25,11 +25,17 @@ constexpr int kSpan = kOwn + kPart - 1;  // offsets between the rows of two tile
 template <int D>
 constexpr int kTileBytes = 64 * (D + 8) * 2;
 
-// shared memory: own_a | own_b | part_a[2] | part_b[2] | lse, delta [2][64] each | table[kTableEntries] | bias of offsets [2][128], their buckets [2][128] |
-// pairs' buckets [2][64][80] | DQ with a table: [4 warps][num_buckets + 1][32]
+// Buffers of partner tiles.  Backward at head size 128 one: with two, 120 KB, an SM has room for one CTA, while of two CTAs one brings its tile as the other
+// works (forward and backward, by pairs, one | two buffers: 731 x 54 tokens, 4 heads on 1, 238 | 351 us; 64 x 192 tokens, 8 heads, 273 | 366; 2 x 2171 queries on 6439 keys,
+// one head, 702 | 759).
+template <int D, int MODE>
+constexpr int kStages = D == 128 && MODE != D_FWD ? 1 : 2;
+// shared memory: own_a | own_b (backward) | part_a[S] | part_b[S] | lse, delta [S][64] each | table[kTableEntries] | bias of offsets [S][128], their buckets [S][128] |
+// pairs' buckets [S][64][80] | DQ with a table: [4 warps][num_buckets + 1][32]
 constexpr int kPairRow = 80, kPairTile = 64 * kPairRow;  // a row of 64 bytes, in banks of its own among eight neighbours
-template <int D, int KIND>
-constexpr int kFixedBytes = 6 * kTileBytes<D> + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 4 + 2 * 128 + (KIND == MF_BUCKETS_PAIR ? 2 * kPairTile : 0);
+template <int D, int MODE, int KIND>
+constexpr int kFixedBytes = ((MODE == D_FWD ? 1 : 2) + 2 * kStages<D, MODE>)*kTileBytes<D> + kStages<D, MODE> * (2 * 64 * 4 + 128 * 4 + 128) + kTableEntries * 4 +
+                            (KIND == MF_BUCKETS_PAIR ? kStages<D, MODE> * kPairTile : 0);
 
 // bits lo .. hi - 1 of a word
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
@@ -52,17 +58,17 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const T* src, long long
 
 template <typename T, int D, int MODE, int KIND>
 __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 2) dense_attn_mma_kernel(const __grid_constant__ DenseParams p) {
-  constexpr int LD = D + 8, TILE = kTileBytes<D>, KS = D / 16;
+  constexpr int LD = D + 8, TILE = kTileBytes<D>, KS = D / 16, STAGES = kStages<D, MODE>;
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t s_own_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), s_own_b = s_own_a + TILE;
-  const uint32_t s_part_a = s_own_b + TILE, s_part_b = s_part_a + 2 * TILE;
-  float* part_lse = reinterpret_cast<float*>(smem + 6 * TILE);
-  float* part_delta = part_lse + 2 * 64;
-  float* table = part_delta + 2 * 64;
+  const uint32_t s_part_a = MODE == D_FWD ? s_own_b : s_own_b + TILE, s_part_b = s_part_a + STAGES * TILE;
+  float* part_lse = reinterpret_cast<float*>(smem + ((MODE == D_FWD ? 1 : 2) + 2 * STAGES) * TILE);
+  float* part_delta = part_lse + STAGES * 64;
+  float* table = part_delta + STAGES * 64;
   float* offset_bias = table + kTableEntries;
-  uint8_t* offset_bucket = reinterpret_cast<uint8_t*>(offset_bias + 2 * 128);
-  uint8_t* pair_tile = offset_bucket + 2 * 128;
-  float* sums = reinterpret_cast<float*>(pair_tile + (KIND == MF_BUCKETS_PAIR ? 2 * kPairTile : 0));
+  uint8_t* offset_bucket = reinterpret_cast<uint8_t*>(offset_bias + STAGES * 128);
+  uint8_t* pair_tile = offset_bucket + STAGES * 128;
+  float* sums = reinterpret_cast<float*>(pair_tile + (KIND == MF_BUCKETS_PAIR ? STAGES * kPairTile : 0));
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int heads = MODE == D_DKV ? p.K : p.H, group = p.H / p.K;
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
 
   const bool idle = row0 + warp * 16 >= own_limit;  // a warp without a row brings tiles along and no more
   for (int t = 0; t < steps; ++t) {
-    const int stage = t & 1;
+    const int stage = STAGES == 2 ? t & 1 : 0;
     const int h = MODE == D_DKV ? oh * group + t / per_head : oh;
     const int at = first + (MODE == D_DKV ? t % per_head : t) * kPart;
     if (masked) {
@@ -251,171 +257,179 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
     }
     cp_async_wait<0>();
     __syncthreads();  // tile t has arrived, and everybody is done with the buffers of tile t - 1
-    if (t + 1 < steps) load_step(t + 1, stage ^ 1, seen_next);
-    cp_async_commit();
-
-    if (idle) continue;
-    const uint32_t pa = s_part_a + stage * TILE, pb = s_part_b + stage * TILE;
-    float s[8][4], dp[MODE == D_FWD ? 1 : 8][4];
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[nt][e] = 0.f;
-        if constexpr (MODE != D_FWD) dp[nt][e] = 0.f;
-      }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint32_t a[4], a2[4];
-      ldmatrix_x4(a, s_own_a + ((warp * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8) * 2);
-      if (MODE != D_FWD) ldmatrix_x4(a2, s_own_b + ((warp * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8) * 2);
-#pragma unroll
-      for (int np = 0; np < 4; ++np) {
-        const uint32_t off = ((np * 16 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8) * 2;
-        uint32_t w[4];
-        ldmatrix_x4(w, pa + off);
-        mma16816<T>(s[2 * np], a, w[0], w[1]);
-        mma16816<T>(s[2 * np + 1], a, w[2], w[3]);
-        if constexpr (MODE != D_FWD) {
-          ldmatrix_x4(w, pb + off);
-          mma16816<T>(dp[2 * np], a2, w[0], w[1]);
-          mma16816<T>(dp[2 * np + 1], a2, w[2], w[3]);
-        }
-      }
+    if (STAGES == 2) {
+      if (t + 1 < steps) load_step(t + 1, stage ^ 1, seen_next);
+      cp_async_commit();
     }
 
-    // ---- logits in units of log2, minus infinity where nothing is seen
-    uint32_t which[KIND == MF_BUCKETS_NONE ? 1 : 8];  // buckets of the 32 elements, a byte each
-    if (KIND == MF_BUCKETS_PAIR) {
-      const uint8_t* tile_at = pair_tile + stage * kPairTile;
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        const int c = nt * 8 + 2 * t4, r = warp * 16 + g;
-        if (MODE == D_DKV)
-          which[nt] = tile_at[c * kPairRow + r] | tile_at[(c + 1) * kPairRow + r] << 8 | tile_at[c * kPairRow + r + 8] << 16 | (uint32_t)tile_at[(c + 1) * kPairRow + r + 8] << 24;
-        else
-          which[nt] = *reinterpret_cast<const uint16_t*>(tile_at + r * kPairRow + c) | (uint32_t)*reinterpret_cast<const uint16_t*>(tile_at + (r + 8) * kPairRow + c) << 16;
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
-        if (KIND == MF_BUCKETS_NONE) s[nt][e] *= sc2;
-        if (KIND == MF_BUCKETS_OFFSET) s[nt][e] = fmaf(s[nt][e], sc2, offset_bias[stage * 128 + (MODE == D_DKV ? r - c + kPart - 1 : c - r + kOwn - 1)]);
-        if (KIND == MF_BUCKETS_PAIR) s[nt][e] = fmaf(s[nt][e], sc2, table[(which[nt] >> (8 * e)) & 255u]);
-      }
-    if (at < most_lo || at + kPart > least_hi || masked) {
-      uint32_t vis[2][2];  // of a row, half of the tile: from the thread's first column on
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        vis[e][0] = (bits_between(lo[e] - at, hi[e] - at) & seen.x) >> (2 * t4);
-        vis[e][1] = (bits_between(lo[e] - at - 32, hi[e] - at - 32) & seen.y) >> (2 * t4);
-      }
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!(vis[e >> 1][nt >> 2] & (1u << ((nt & 3) * 8 + (e & 1))))) s[nt][e] = -INFINITY;
-    }
-
-    if (MODE == D_FWD) {
-      float alpha[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float m = top[e];
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt) m = fmaxf(m, fmaxf(s[nt][2 * e], s[nt][2 * e + 1]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const float shift = m == -INFINITY ? 0.f : m;
-        alpha[e] = dense_exp2(top[e] - shift);
-        top[e] = m;
-        float sum = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            s[nt][2 * e + x] = dense_exp2(s[nt][2 * e + x] - shift);
-            sum += s[nt][2 * e + x];
-          }
-        total[e] = total[e] * alpha[e] + sum;
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc0[i][e] *= alpha[e >> 1];
-    } else {
+    if (!idle) {
+      const uint32_t pa = s_part_a + stage * TILE, pb = s_part_b + stage * TILE;
+      float s[8][4], dp[MODE == D_FWD ? 1 : 8][4];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int c = nt * 8 + 2 * t4 + (e & 1);
-          const float z = s[nt][e];
-          const float l = MODE == D_DQ ? lse[e >> 1] : part_lse[stage * 64 + c];
-          const float d = MODE == D_DQ ? delta[e >> 1] : part_delta[stage * 64 + c];
-          const float pr = dense_exp2(z - l);
-          s[nt][e] = pr;
-          dp[nt][e] = pr * (dp[nt][e] - d);
-          if (MODE == D_DQ) error[e >> 1] += dp[nt][e];
+          s[nt][e] = 0.f;
+          if constexpr (MODE != D_FWD) dp[nt][e] = 0.f;
         }
-      if (MODE == D_DQ && steps == 1) {  // the whole row is here: its exact delta
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t a[4], a2[4];
+        ldmatrix_x4(a, s_own_a + ((warp * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8) * 2);
+        if (MODE != D_FWD) ldmatrix_x4(a2, s_own_b + ((warp * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+        for (int np = 0; np < 4; ++np) {
+          const uint32_t off = ((np * 16 + (lane & 7) + (lane >> 4) * 8) * LD + ks * 16 + ((lane >> 3) & 1) * 8) * 2;
+          uint32_t w[4];
+          ldmatrix_x4(w, pa + off);
+          mma16816<T>(s[2 * np], a, w[0], w[1]);
+          mma16816<T>(s[2 * np + 1], a, w[2], w[3]);
+          if constexpr (MODE != D_FWD) {
+            ldmatrix_x4(w, pb + off);
+            mma16816<T>(dp[2 * np], a2, w[0], w[1]);
+            mma16816<T>(dp[2 * np + 1], a2, w[2], w[3]);
+          }
+        }
+      }
+
+      // ---- logits in units of log2, minus infinity where nothing is seen
+      uint32_t which[KIND == MF_BUCKETS_NONE ? 1 : 8];  // buckets of the 32 elements, a byte each
+      if (KIND == MF_BUCKETS_PAIR) {
+        const uint8_t* tile_at = pair_tile + stage * kPairTile;
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const int c = nt * 8 + 2 * t4, r = warp * 16 + g;
+          if (MODE == D_DKV)
+            which[nt] = tile_at[c * kPairRow + r] | tile_at[(c + 1) * kPairRow + r] << 8 | tile_at[c * kPairRow + r + 8] << 16 | (uint32_t)tile_at[(c + 1) * kPairRow + r + 8] << 24;
+          else
+            which[nt] = *reinterpret_cast<const uint16_t*>(tile_at + r * kPairRow + c) | (uint32_t)*reinterpret_cast<const uint16_t*>(tile_at + (r + 8) * kPairRow + c) << 16;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
+          if (KIND == MF_BUCKETS_NONE) s[nt][e] *= sc2;
+          if (KIND == MF_BUCKETS_OFFSET) s[nt][e] = fmaf(s[nt][e], sc2, offset_bias[stage * 128 + (MODE == D_DKV ? r - c + kPart - 1 : c - r + kOwn - 1)]);
+          if (KIND == MF_BUCKETS_PAIR) s[nt][e] = fmaf(s[nt][e], sc2, table[(which[nt] >> (8 * e)) & 255u]);
+        }
+      if (at < most_lo || at + kPart > least_hi || masked) {
+        uint32_t vis[2][2];  // of a row, half of the tile: from the thread's first column on
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = error[e];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          vis[e][0] = (bits_between(lo[e] - at, hi[e] - at) & seen.x) >> (2 * t4);
+          vis[e][1] = (bits_between(lo[e] - at - 32, hi[e] - at - 32) & seen.y) >> (2 * t4);
+        }
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(vis[e >> 1][nt >> 2] & (1u << ((nt & 3) * 8 + (e & 1))))) s[nt][e] = -INFINITY;
+      }
+
+      if (MODE == D_FWD) {
+        float alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = top[e];
+#pragma unroll
+          for (int nt = 0; nt < 8; ++nt) m = fmaxf(m, fmaxf(s[nt][2 * e], s[nt][2 * e + 1]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const float shift = m == -INFINITY ? 0.f : m;
+          alpha[e] = dense_exp2(top[e] - shift);
+          top[e] = m;
+          float sum = 0.f;
 #pragma unroll
           for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) dp[nt][2 * e + i] = fmaf(-x, s[nt][2 * e + i], dp[nt][2 * e + i]);
+            for (int x = 0; x < 2; ++x) {
+              s[nt][2 * e + x] = dense_exp2(s[nt][2 * e + x] - shift);
+              sum += s[nt][2 * e + x];
+            }
+          total[e] = total[e] * alpha[e] + sum;
         }
-      }
-      if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
-        // a column of sums for every lane: no two threads meet in one, and the order of a sum is that of the walk
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          int bucket[4];
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc0[i][e] *= alpha[e >> 1];
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
-            bucket[e] = min((int)(KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1] : (which[nt] >> (8 * e)) & 255u), nb);
+            const int c = nt * 8 + 2 * t4 + (e & 1);
+            const float z = s[nt][e];
+            const float l = MODE == D_DQ ? lse[e >> 1] : part_lse[stage * 64 + c];
+            const float d = MODE == D_DQ ? delta[e >> 1] : part_delta[stage * 64 + c];
+            const float pr = dense_exp2(z - l);
+            s[nt][e] = pr;
+            dp[nt][e] = pr * (dp[nt][e] - d);
+            if (MODE == D_DQ) error[e >> 1] += dp[nt][e];
           }
-          add_four(my_sums, bucket, dp[nt]);
+        if (MODE == D_DQ && steps == 1) {  // the whole row is here: its exact delta
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = error[e];
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            x += __shfl_xor_sync(0xffffffffu, x, 2);
+#pragma unroll
+            for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) dp[nt][2 * e + i] = fmaf(-x, s[nt][2 * e + i], dp[nt][2 * e + i]);
+          }
+        }
+        if (KIND != MF_BUCKETS_NONE && MODE == D_DQ && p.dbias_part) {
+          // a column of sums for every lane: no two threads meet in one, and the order of a sum is that of the walk
+#pragma unroll
+          for (int nt = 0; nt < 8; ++nt) {
+            int bucket[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int c = nt * 8 + 2 * t4 + (e & 1), r = warp * 16 + g + 8 * (e >> 1);
+              bucket[e] = min((int)(KIND == MF_BUCKETS_OFFSET ? offset_bucket[stage * 128 + c - r + kOwn - 1] : (which[nt] >> (8 * e)) & 255u), nb);
+            }
+            add_four(my_sums, bucket, dp[nt]);
+          }
+        }
+      }
+
+      // ---- products with the partners' rows
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t a[4], a2[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int nt = 2 * kk + (x >> 1), e = 2 * (x & 1);
+          a[x] = pack2<T>(s[nt][e], s[nt][e + 1]);
+          if constexpr (MODE != D_FWD) a2[x] = pack2<T>(dp[nt][e], dp[nt][e + 1]);
+        }
+#pragma unroll
+        for (int np = 0; np < D / 16; ++np) {
+          const uint32_t off = ((kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + np * 16 + (lane >> 4) * 8) * 2;
+          uint32_t w[4];
+          if constexpr (MODE == D_FWD) {
+            ldmatrix_x4_trans(w, pb + off);
+            mma16816<T>(acc0[2 * np], a, w[0], w[1]);
+            mma16816<T>(acc0[2 * np + 1], a, w[2], w[3]);
+          } else {
+            ldmatrix_x4_trans(w, pa + off);
+            mma16816<T>(acc0[2 * np], a2, w[0], w[1]);
+            mma16816<T>(acc0[2 * np + 1], a2, w[2], w[3]);
+          }
+          if constexpr (MODE == D_DKV) {
+            ldmatrix_x4_trans(w, pb + off);
+            mma16816<T>(acc1[2 * np], a, w[0], w[1]);
+            mma16816<T>(acc1[2 * np + 1], a, w[2], w[3]);
+          }
         }
       }
     }
-
-    // ---- products with the partners' rows
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t a[4], a2[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int nt = 2 * kk + (x >> 1), e = 2 * (x & 1);
-        a[x] = pack2<T>(s[nt][e], s[nt][e + 1]);
-        if constexpr (MODE != D_FWD) a2[x] = pack2<T>(dp[nt][e], dp[nt][e + 1]);
-      }
-#pragma unroll
-      for (int np = 0; np < D / 16; ++np) {
-        const uint32_t off = ((kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + np * 16 + (lane >> 4) * 8) * 2;
-        uint32_t w[4];
-        if constexpr (MODE == D_FWD) {
-          ldmatrix_x4_trans(w, pb + off);
-          mma16816<T>(acc0[2 * np], a, w[0], w[1]);
-          mma16816<T>(acc0[2 * np + 1], a, w[2], w[3]);
-        } else {
-          ldmatrix_x4_trans(w, pa + off);
-          mma16816<T>(acc0[2 * np], a2, w[0], w[1]);
-          mma16816<T>(acc0[2 * np + 1], a2, w[2], w[3]);
-        }
-        if constexpr (MODE == D_DKV) {
-          ldmatrix_x4_trans(w, pb + off);
-          mma16816<T>(acc1[2 * np], a, w[0], w[1]);
-          mma16816<T>(acc1[2 * np + 1], a, w[2], w[3]);
-        }
-      }
+    if (STAGES == 1) {
+      __syncthreads();  // everybody is done with the one buffer
+      if (t + 1 < steps) load_step(t + 1, 0, seen_next);
+      cp_async_commit();
     }
   }
   cp_async_wait<0>();
@@ -480,7 +494,10 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
 // CTAs of a head in the pass that sums the table's gradient: as many as fit the chip, at most one for each tile.
 int slots_of(const DenseParams& p, int head_dim) {
   const long long tiles = (long long)p.B * ((p.M + kOwn - 1) / kOwn);
-  const int smem = 6 * 64 * (head_dim + 8) * 2 + 4 * 64 * 4 + kTableEntries * 4 + 2 * 128 * 5 + 2 * kPairTile + 4 * (p.num_buckets + 1) * 32 * 4 + 1024;
+  const int fixed = head_dim == 32   ? kFixedBytes<32, D_DQ, MF_BUCKETS_PAIR>
+                    : head_dim == 64 ? kFixedBytes<64, D_DQ, MF_BUCKETS_PAIR>
+                                     : kFixedBytes<128, D_DQ, MF_BUCKETS_PAIR>;
+  const int smem = fixed + 4 * (p.num_buckets + 1) * 32 * 4 + 1024;
   const int fit = 227 * 1024 / smem, most = 148 * (fit < 1 ? 1 : fit > 3 ? 3 : fit) / p.H;
   return (int)(tiles < most ? tiles : most < 1 ? 1 : most);
 }
@@ -489,10 +506,10 @@ template <typename T, int D, int MODE, int KIND>
 int launch(const DenseParams& p, cudaStream_t stream) {
   const int own = MODE == D_DKV ? p.N : p.M, heads = MODE == D_DKV ? p.K : p.H;
   if (own == 0) return MF_OK;
-  const int smem = kFixedBytes<D, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
+  const int smem = kFixedBytes<D, MODE, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
   constexpr auto kernel = dense_attn_mma_kernel<T, D, MODE, KIND>;
   // one limit for all calls: what the largest table needs
-  constexpr int most = kFixedBytes<D, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
+  constexpr int most = kFixedBytes<D, MODE, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
   static_assert(most <= 227 * 1024, "");
   const cudaError_t err = allow_shared<dense_attn_mma_kernel<T, D, MODE, KIND>>(most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
