@@ -11,8 +11,8 @@
 // Every output has one owner and a fixed order of its sums.
 //
 // Registers bound it: 64 x 64 logits, their gradients and the sums are 128 to 168 of a thread's, three or four CTAs on an SM (without that limit 255 and two, 64
-// molecules of 19 to 192 tokens 124 us instead of 120 for forward and backward), which use a third of the issue slots and a fifth of the tensor pipe. There: forward 27,
-// DQ 49, DKV 45 us; 8 x 577 fp16 queries on 1000 keys, 4 heads of 32, 22 + 26 + 19 us. 64 rows to a tile: fewer waste products for molecules of all lengths.
+// molecules of 19 to 192 tokens 124 us instead of 120 for forward and backward), which use a third of the issue slots and a fifth of the tensor pipe. There: forward 26,
+// DQ 48, DKV 39 us; 8 x 577 fp16 queries on 1000 keys, 4 heads of 32, 22 + 26 + 19 us. 64 rows to a tile: fewer waste products for molecules of all lengths.
 #include "dense_attn.cuh"
 
 namespace mf {
@@ -27,15 +27,19 @@ constexpr int kTileBytes = 64 * (D + 8) * 2;
 
 // Buffers of partner tiles.  Backward at head size 128 one: with two, 120 KB, an SM has room for one CTA, while of two CTAs one brings its tile as the other
 // works (forward and backward, by pairs, one | two buffers: 731 x 54 tokens, 4 heads on 1, 238 | 351 us; 64 x 192 tokens, 8 heads, 273 | 366; 2 x 2171 queries on 6439 keys,
-// one head, 702 | 759).
-template <int D, int MODE>
-constexpr int kStages = D == 128 && MODE != D_FWD ? 1 : 2;
-// shared memory: own_a | own_b (backward) | part_a[S] | part_b[S] | lse, delta [S][64] each | table[kTableEntries] | bias of offsets [S][128], their buckets [S][128] |
-// pairs' buckets [S][64][80] | DQ with a table: [4 warps][num_buckets + 1][32]
+// one head, 702 | 759).  The queries' gradient by pairs too, for a third CTA beside up to 64 buckets' sums: 64 x 192 tokens, 8 heads of 64, 142 | 155 us.
+template <int D, int MODE, int KIND>
+constexpr int kStages = (D == 128 && MODE != D_FWD) || (MODE == D_DQ && KIND == MF_BUCKETS_PAIR) ? 1 : 2;
+// shared memory: own_a | own_b (backward) | part_a[S] | part_b[S] | lse, delta [S][64] each (DKV) | table[kTableEntries] (pairs) | bias of offsets [S][128], their
+// buckets [S][128] (offsets) | pairs' buckets [S][64][80] | DQ with a table: [4 warps][num_buckets + 1][32]
 constexpr int kPairRow = 80, kPairTile = 64 * kPairRow;  // a row of 64 bytes, in banks of its own among eight neighbours
 template <int D, int MODE, int KIND>
-constexpr int kFixedBytes = ((MODE == D_FWD ? 1 : 2) + 2 * kStages<D, MODE>)*kTileBytes<D> + kStages<D, MODE> * (2 * 64 * 4 + 128 * 4 + 128) + kTableEntries * 4 +
-                            (KIND == MF_BUCKETS_PAIR ? kStages<D, MODE> * kPairTile : 0);
+struct Layout {
+  static constexpr int kS = kStages<D, MODE, KIND>;
+  static constexpr int kStats = ((MODE == D_FWD ? 1 : 2) + 2 * kS) * kTileBytes<D>, kTable = kStats + (MODE == D_DKV ? kS * 2 * 64 * 4 : 0);
+  static constexpr int kOffsets = kTable + (KIND == MF_BUCKETS_PAIR ? kTableEntries * 4 : 0), kPairs = kOffsets + (KIND == MF_BUCKETS_OFFSET ? kS * 128 * 5 : 0);
+  static constexpr int kFixed = kPairs + (KIND == MF_BUCKETS_PAIR ? kS * kPairTile : 0);
+};
 
 // bits lo .. hi - 1 of a word
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
@@ -58,17 +62,18 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const T* src, long long
 
 template <typename T, int D, int MODE, int KIND>
 __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 2) dense_attn_mma_kernel(const __grid_constant__ DenseParams p) {
-  constexpr int LD = D + 8, TILE = kTileBytes<D>, KS = D / 16, STAGES = kStages<D, MODE>;
+  constexpr int LD = D + 8, TILE = kTileBytes<D>, KS = D / 16, STAGES = kStages<D, MODE, KIND>;
   extern __shared__ __align__(16) uint8_t smem[];
   const uint32_t s_own_a = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), s_own_b = s_own_a + TILE;
   const uint32_t s_part_a = MODE == D_FWD ? s_own_b : s_own_b + TILE, s_part_b = s_part_a + STAGES * TILE;
-  float* part_lse = reinterpret_cast<float*>(smem + ((MODE == D_FWD ? 1 : 2) + 2 * STAGES) * TILE);
+  using At = Layout<D, MODE, KIND>;
+  float* part_lse = reinterpret_cast<float*>(smem + At::kStats);
   float* part_delta = part_lse + STAGES * 64;
-  float* table = part_delta + STAGES * 64;
-  float* offset_bias = table + kTableEntries;
+  float* table = reinterpret_cast<float*>(smem + At::kTable);
+  float* offset_bias = reinterpret_cast<float*>(smem + At::kOffsets);
   uint8_t* offset_bucket = reinterpret_cast<uint8_t*>(offset_bias + STAGES * 128);
-  uint8_t* pair_tile = offset_bucket + STAGES * 128;
-  float* sums = reinterpret_cast<float*>(pair_tile + (KIND == MF_BUCKETS_PAIR ? STAGES * kPairTile : 0));
+  uint8_t* pair_tile = smem + At::kPairs;
+  float* sums = reinterpret_cast<float*>(smem + At::kFixed);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int heads = MODE == D_DKV ? p.K : p.H, group = p.H / p.K;
@@ -494,9 +499,9 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
 // CTAs of a head in the pass that sums the table's gradient: as many as fit the chip, at most one for each tile.
 int slots_of(const DenseParams& p, int head_dim) {
   const long long tiles = (long long)p.B * ((p.M + kOwn - 1) / kOwn);
-  const int fixed = head_dim == 32   ? kFixedBytes<32, D_DQ, MF_BUCKETS_PAIR>
-                    : head_dim == 64 ? kFixedBytes<64, D_DQ, MF_BUCKETS_PAIR>
-                                     : kFixedBytes<128, D_DQ, MF_BUCKETS_PAIR>;
+  const int fixed = head_dim == 32   ? Layout<32, D_DQ, MF_BUCKETS_PAIR>::kFixed
+                    : head_dim == 64 ? Layout<64, D_DQ, MF_BUCKETS_PAIR>::kFixed
+                                     : Layout<128, D_DQ, MF_BUCKETS_PAIR>::kFixed;
   const int smem = fixed + 4 * (p.num_buckets + 1) * 32 * 4 + 1024;
   const int fit = 227 * 1024 / smem, most = 148 * (fit < 1 ? 1 : fit > 3 ? 3 : fit) / p.H;
   return (int)(tiles < most ? tiles : most < 1 ? 1 : most);
@@ -506,10 +511,10 @@ template <typename T, int D, int MODE, int KIND>
 int launch(const DenseParams& p, cudaStream_t stream) {
   const int own = MODE == D_DKV ? p.N : p.M, heads = MODE == D_DKV ? p.K : p.H;
   if (own == 0) return MF_OK;
-  const int smem = kFixedBytes<D, MODE, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
+  const int smem = Layout<D, MODE, KIND>::kFixed + (MODE == D_DQ && KIND != MF_BUCKETS_NONE && p.dbias_part ? 4 * (p.num_buckets + 1) * 32 * 4 : 0);
   constexpr auto kernel = dense_attn_mma_kernel<T, D, MODE, KIND>;
   // one limit for all calls: what the largest table needs
-  constexpr int most = kFixedBytes<D, MODE, KIND> + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
+  constexpr int most = Layout<D, MODE, KIND>::kFixed + (MODE == D_DQ && KIND != MF_BUCKETS_NONE ? 4 * (kMaxBuckets + 1) * 32 * 4 : 0);
   static_assert(most <= 227 * 1024, "");
   const cudaError_t err = allow_shared<dense_attn_mma_kernel<T, D, MODE, KIND>>(most);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
