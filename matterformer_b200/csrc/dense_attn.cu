@@ -257,7 +257,10 @@ int forward(const char* name, const MfDenseAttnArgs* a, cudaStream_t stream, Bou
       if (const int rc = check_space(name, a, need)) return rc;
       return dense_attn_split(p, a->dtype, a->head_dim, a->bucket_kind, a->workspace, stream);
     }
-    case kTensor: return dense_attn_sm100_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream, waits);
+    case kTensor: {
+      if (const int rc = check_space(name, a, dense_tc_fwd_workspace_bytes(p, a->head_dim))) return rc;
+      return dense_attn_sm100_fwd(p, a->dtype, a->head_dim, a->bucket_kind, a->workspace, stream, waits);
+    }
     default: return dense_attn_mma_fwd(p, a->dtype, a->head_dim, a->bucket_kind, stream);
   }
 }
@@ -321,7 +324,8 @@ size_t mf_dense_attn_fwd_workspace_bytes(const MfDenseAttnArgs* a) {
   using namespace mf;
   if (check_args("mf_dense_attn_fwd_workspace_bytes", a) != MF_OK || a->batch == 0 || a->queries == 0) return 0;
   const DenseParams p = params_of(*a);
-  return fwd_family(*a, p) == kSplit ? dense_attn_split_workspace_bytes(p, a->head_dim) : 0;
+  const Family family = fwd_family(*a, p);
+  return family == kSplit ? dense_attn_split_workspace_bytes(p, a->head_dim) : family == kTensor ? dense_tc_fwd_workspace_bytes(p, a->head_dim) : 0;
 }
 size_t mf_dense_attn_bwd_workspace_bytes(const MfDenseAttnArgs* a) {
   using namespace mf;

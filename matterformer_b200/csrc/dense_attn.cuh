@@ -138,6 +138,10 @@ int dense_attn_small(const DenseParams& p, int dtype, int head_dim, int bucket_k
 // dense_attn_split.cu: forward, few queries
 bool dense_attn_split_applies(const DenseParams& p, int head_dim);
 size_t dense_attn_split_workspace_bytes(const DenseParams& p, int head_dim);
+// Joins pieces of the keys: acc [entry * key head][tile of 16 rows][piece][16][D] in units of exp2(-top), stat the same without D: top, total.  A row is query * group +
+// head of the group; a top of minus infinity stands for a piece that wrote nothing.
+int dense_attn_join(const DenseParams& p, int dtype, int head_dim, int pieces, float* acc, float* stat, cudaStream_t stream);
+size_t dense_attn_join_bytes(const DenseParams& p, int head_dim, int pieces);
 int dense_attn_split(const DenseParams& p, int dtype, int head_dim, int bucket_kind, void* workspace, cudaStream_t stream);
 
 }  // namespace mf

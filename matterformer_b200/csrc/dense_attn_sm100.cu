@@ -51,9 +51,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
   // ---- which rows: two heads of a group, or two neighbouring tiles of a head
   const int group = p.H / p.K;
   const bool by_head = group % 2 == 0;
-  const int units = p.B * (by_head ? p.H / 2 : p.H), row_blocks = gridDim.x / units;
-  const int unit = p.causal ? blockIdx.x % units : blockIdx.x / row_blocks;
-  const int rb = p.causal ? row_blocks - 1 - (int)(blockIdx.x / units) : blockIdx.x % row_blocks;  // the longest walks first
+  const int piece = blockIdx.x % tc.pieces, block = blockIdx.x / tc.pieces, tile0 = piece * tc.piece_tiles;  // of the keys
+  const int units = p.B * (by_head ? p.H / 2 : p.H), row_blocks = gridDim.x / tc.pieces / units;
+  const int unit = p.causal ? block % units : block / row_blocks;
+  const int rb = p.causal ? row_blocks - 1 - block / units : block % row_blocks;  // the longest walks first
   const int b = unit / (units / p.B), hu = unit % (units / p.B);
   const int head0 = by_head ? 2 * hu : hu, kh = head0 / group;
   const DenseLengths len = dense_lengths(p, b);
@@ -63,18 +64,26 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
     head[x] = by_head ? head0 + x : head0;
     row0[x] = by_head ? rb * kTcRows : (2 * rb + x) * kTcRows;
     const int limit = row0[x] < len.nq ? dense_limit(p, len, min(row0[x] + kTcRows, len.nq) - 1) : 0;
-    tiles[x] = (limit + kTcRows - 1) / kTcRows;
+    tiles[x] = max(0, min((limit + kTcRows - 1) / kTcRows - tile0, tc.piece_tiles));
   }
   const int steps = max(tiles[0], tiles[1]);
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.key_mask_batch : nullptr;
-  const bool cleaning = mask || len.nk < min(p.N, steps * kTcRows);
+  const bool cleaning = mask || len.nk < min(p.N, (tile0 + steps) * kTcRows);
 
   auto row_out = [&](int x, int r) { return static_cast<T*>(p.out) + p.out_rows.at(b, head[x], row0[x] + r); };
   auto row_stat = [&](int x, int r) -> float& { return p.lse[((long long)b * p.H + head[x]) * p.M + row0[x] + r]; };
+  // pieces: where a row leaves its own (see dense_attn_join)
+  auto piece_slot = [&](int h, int i) {
+    const int row = i * group + h - kh * group, row_tiles = (p.M * group + 15) / 16;
+    return (((long long)(b * p.K + kh) * row_tiles + row / 16) * tc.pieces + piece) * 16 + row % 16;
+  };
   if (steps == 0) {  // padding only, or nothing is seen
     if (tid < 256) {
       const int x = tid >> 7, r = tid & 127;
-      if (row0[x] + r < p.M) {
+      if (row0[x] + r < p.M && tc.pieces > 1) {
+        const long long at = piece_slot(head[x], row0[x] + r);
+        tc.stat[2 * at] = -INFINITY, tc.stat[2 * at + 1] = 0.f;
+      } else if (row0[x] + r < p.M) {
         uint4* dst = reinterpret_cast<uint4*>(row_out(x, r));
         for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
         if (p.lse) row_stat(x, r) = INFINITY;
@@ -125,7 +134,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
         if (bad) break;
         mbar_arrive_expect_tx(&bar_full[slot], Sh::kTile);
         for (int c = 0; c < Sh::kChunks; ++c)
-          tma_box(s_ring + slot * Sh::kTile + c * kTcRows * 128, i & 1 ? &tc.v : &tc.k, c * 64, (i >> 1) * kTcRows, kh, b, &bar_full[slot]);
+          tma_box(s_ring + slot * Sh::kTile + c * kTcRows * 128, i & 1 ? &tc.v : &tc.k, c * 64, (tile0 + (i >> 1)) * kTcRows, kh, b, &bar_full[slot]);
       }
       // whoever gave up, no copy may be in flight when the CTA ends
       if (!mbar_wait_for(&bar_q, 0, tc.waits.limit)) bad = true;
@@ -180,10 +189,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
       for (int j = 0; j < steps; ++j) {
         const int iv = 2 * j + 1, slot = iv % Sh::kSlots;
         wait_on(&bar_full[slot], iv / Sh::kSlots);
-        const int last = min(kTcRows, p.N - j * kTcRows);  // rows behind the tensor's are zeros already
-        if (!bad && (mask || j * kTcRows + last > len.nk)) {
+        const int first = (tile0 + j) * kTcRows, last = min(kTcRows, p.N - first);  // rows behind the tensor's are zeros already
+        if (!bad && (mask || first + last > len.nk)) {
           for (int r = lane; r < last; r += 32) {
-            const int key = j * kTcRows + r;
+            const int key = first + r;
             if (key < len.nk && (!mask || mask[key])) continue;
 #pragma unroll
             for (int c = 0; c < Sh::kChunks; ++c)
@@ -220,7 +229,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
     const uint8_t* pair_row = KIND == MF_BUCKETS_PAIR ? p.buckets + b * p.bucket_batch + min(i, p.M - 1) * p.bucket_row : nullptr;
     int fills = 0;
     for (int j = 0; j < my_tiles; ++j) {
-      const int key0 = j * kTcRows;
+      const int key0 = (tile0 + j) * kTcRows;
       float one = 0.f;
       const float* near = nullptr;
       if (KIND == MF_BUCKETS_OFFSET) {
@@ -336,6 +345,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
     tc_fence_after_sync();
     const bool some = row_ok && (total > 0.f || total != total);
     const float inv = some ? 1.f / total : 0.f;
+    const long long slot = tc.pieces > 1 && i < p.M ? piece_slot(my_head, i) : 0;
 #pragma unroll
     for (int c = 0; c < D; c += 32) {
       uint32_t o[32];
@@ -343,7 +353,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
         tmem_ld32(col_o + c, o);
         tmem_ld_wait();
       }
-      if (i < p.M) {
+      if (tc.pieces > 1) {
+        if (i < p.M && some)
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(tc.acc + slot * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      } else if (i < p.M) {
         uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + p.out_rows.at(b, my_head, i) + c);
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
@@ -354,7 +368,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
         }
       }
     }
-    if (p.lse && i < p.M) p.lse[((long long)b * p.H + my_head) * p.M + i] = some ? top + log2f(total) : INFINITY;
+    if (tc.pieces > 1) {
+      if (i < p.M) tc.stat[2 * slot] = some ? top : -INFINITY, tc.stat[2 * slot + 1] = some ? total : 0.f;
+    } else if (p.lse && i < p.M) {
+      p.lse[((long long)b * p.H + my_head) * p.M + i] = some ? top + log2f(total) : INFINITY;
+    }
     tc_fence_before_sync();
   }
   if (bad) atomicExch(&g_dense_status[tc.waits.word], MF_ERR_DEVICE_TIMEOUT);
@@ -362,26 +380,44 @@ __global__ void __launch_bounds__(kFwdThreads, 1) dense_attn_tc_kernel(const __g
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
+// CTAs without pieces of the keys.
+long long blocks_of(const DenseParams& p) {
+  const long long tiles = (p.M + kTcRows - 1) / kTcRows;
+  return (p.H / p.K) % 2 == 0 ? tiles * p.B * (p.H / 2) : (tiles + 1) / 2 * p.B * p.H;
+}
+// Pieces of the keys: where the tiles of the queries would fill less than half of the SMs through long walks, as many as the SMs hold, of four tiles at least.
+int pieces_of(const DenseParams& p) {
+  const long long blocks = blocks_of(p), tiles = (p.N + kTcRows - 1) / kTcRows;
+  if (blocks * 2 > 148 || tiles < 16) return 1;
+  const long long most = 148 / blocks < tiles / 4 ? 148 / blocks : tiles / 4, size = (tiles + most - 1) / most;
+  return (int)((tiles + size - 1) / size);
+}
+
 template <typename T, int D, int KIND>
-int launch(const DenseTcParams& tc, cudaStream_t stream) {
+int launch(DenseTcParams& tc, void* workspace, cudaStream_t stream) {
   const DenseParams& p = tc.p;
+  const int tiles = (p.N + kTcRows - 1) / kTcRows;
+  tc.pieces = pieces_of(p), tc.piece_tiles = (tiles + tc.pieces - 1) / tc.pieces;
+  if (tc.pieces > 1) {
+    tc.acc = static_cast<float*>(workspace);
+    tc.stat = tc.acc + (long long)p.B * p.K * (((long long)p.M * (p.H / p.K) + 15) / 16) * tc.pieces * 16 * D;
+  }
   constexpr auto kernel = dense_attn_tc_kernel<T, D, KIND>;
   const cudaError_t err = allow_shared<dense_attn_tc_kernel<T, D, KIND>>(FwdShape<D>::kSmem);
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
-  const bool by_head = (p.H / p.K) % 2 == 0;
-  const long long tiles = (p.M + kTcRows - 1) / kTcRows, blocks = by_head ? tiles * p.B * (p.H / 2) : (tiles + 1) / 2 * p.B * p.H;
-  kernel<<<(unsigned)blocks, kFwdThreads, FwdShape<D>::kSmem, stream>>>(tc);
+  kernel<<<(unsigned)(blocks_of(p) * tc.pieces), kFwdThreads, FwdShape<D>::kSmem, stream>>>(tc);
   MF_CHECK_LAUNCH("dense attention on tcgen05");
+  if (tc.pieces > 1) return dense_attn_join(p, std::is_same<T, __half>::value ? MF_DTYPE_F16 : MF_DTYPE_BF16, D, tc.pieces, tc.acc, tc.stat, stream);
   return MF_OK;
 }
 
 template <typename T>
-int pick(const DenseTcParams& tc, int head_dim, int kind, cudaStream_t stream) {
+int pick(DenseTcParams& tc, int head_dim, int kind, void* workspace, cudaStream_t stream) {
   auto by_kind = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    return kind == MF_BUCKETS_NONE     ? launch<T, D, MF_BUCKETS_NONE>(tc, stream)
-           : kind == MF_BUCKETS_OFFSET ? launch<T, D, MF_BUCKETS_OFFSET>(tc, stream)
-                                       : launch<T, D, MF_BUCKETS_PAIR>(tc, stream);
+    return kind == MF_BUCKETS_NONE     ? launch<T, D, MF_BUCKETS_NONE>(tc, workspace, stream)
+           : kind == MF_BUCKETS_OFFSET ? launch<T, D, MF_BUCKETS_OFFSET>(tc, workspace, stream)
+                                       : launch<T, D, MF_BUCKETS_PAIR>(tc, workspace, stream);
   };
   return head_dim == 64 ? by_kind(std::integral_constant<int, 64>{}) : by_kind(std::integral_constant<int, 128>{});
 }
@@ -420,10 +456,14 @@ bool dense_tc_takes(const DenseParams& p, int head_dim, int kind) {
   return p.M <= 1 << 24 && p.N <= 1 << 24;
 }
 
-int dense_attn_sm100_fwd(const DenseParams& p, int dtype, int head_dim, int kind, cudaStream_t stream, BoundedWaits waits) {
+size_t dense_tc_fwd_workspace_bytes(const DenseParams& p, int head_dim) {
+  const int pieces = pieces_of(p);
+  return pieces > 1 ? dense_attn_join_bytes(p, head_dim, pieces) : 0;
+}
+int dense_attn_sm100_fwd(const DenseParams& p, int dtype, int head_dim, int kind, void* workspace, cudaStream_t stream, BoundedWaits waits) {
   DenseTcParams tc{p, {}, {}, {}, {}, waits};
   if (!dense_tc_maps(tc, dtype, head_dim, false)) return dense_attn_mma_fwd(p, dtype, head_dim, kind, stream);
-  return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16>(tc, head_dim, kind, stream) : pick<__half>(tc, head_dim, kind, stream);
+  return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16>(tc, head_dim, kind, workspace, stream) : pick<__half>(tc, head_dim, kind, workspace, stream);
 }
 
 }  // namespace mf

@@ -13,6 +13,9 @@ struct DenseTcParams {
   DenseParams p;
   CUtensorMap q, k, v, grad_out;  // {head_dim, tokens, heads, batch}, boxes of 64 channels x 128 rows (forward) or 64 (backward), 128-byte swizzle
   BoundedWaits waits;
+  // forward: pieces of the keys, of piece_tiles tiles each, and where they leave their rows where there are several
+  int pieces = 1, piece_tiles = 0;
+  float *acc = nullptr, *stat = nullptr;
 };
 
 // Instruction descriptor of kind::f16 for 16-bit operands and fp32 sums.
@@ -44,7 +47,8 @@ bool dense_tc_takes(const DenseParams& p, int head_dim, int bucket_kind);
 // The last expired wait of the forward or the backward kernels' calls (word 0) or self-test (word 1), once; synchronises.
 int dense_attn_take_fwd_status(int word, int32_t* host_status, cudaStream_t stream);
 int dense_attn_take_bwd_status(int word, int32_t* host_status, cudaStream_t stream);
-int dense_attn_sm100_fwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, cudaStream_t stream, BoundedWaits waits = {});
+size_t dense_tc_fwd_workspace_bytes(const DenseParams& p, int head_dim);
+int dense_attn_sm100_fwd(const DenseParams& p, int dtype, int head_dim, int bucket_kind, void* workspace, cudaStream_t stream, BoundedWaits waits = {});
 bool dense_tc_bwd_takes(const DenseParams& p, int head_dim, int bucket_kind, bool table_grad);
 int dense_attn_sm100_bwd(const DenseTcParams& tc, int dtype, int head_dim, int bucket_kind, cudaStream_t stream);
 

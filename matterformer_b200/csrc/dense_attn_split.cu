@@ -356,6 +356,14 @@ Plan plan_of(const DenseParams& p) {
   return plan;
 }
 
+template <typename T, int D>
+int join(const SplitParams& sp, cudaStream_t stream) {
+  const long long rows = (long long)sp.p.B * sp.p.H * sp.p.M;
+  const cudaError_t err = sp.pieces <= 32 ? launch_dependent(dense_attn_join_few_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, sp, (int)rows)
+                                          : launch_dependent(dense_attn_join_kernel<T, D>, dim3((unsigned)rows), dim3(128), 0, stream, sp);
+  return err == cudaSuccess ? MF_OK : cuda_error(err, "dense attention join");
+}
+
 template <typename T, int D, int KIND>
 int launch(const DenseParams& p, void* workspace, cudaStream_t stream) {
   const Plan plan = plan_of(p);
@@ -368,13 +376,7 @@ int launch(const DenseParams& p, void* workspace, cudaStream_t stream) {
   if (err != cudaSuccess) return cuda_error(err, "dense attention shared memory");
   err = launch_dependent(kernel, dim3((unsigned)plan.blocks), dim3(kThreads), smem, stream, sp);
   if (err != cudaSuccess) return cuda_error(err, "dense attention of few queries");
-  if (plan.pieces > 1) {
-    const long long rows = (long long)p.B * p.H * p.M;
-    err = plan.pieces <= 32 ? launch_dependent(dense_attn_join_few_kernel<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, sp, (int)rows)
-                            : launch_dependent(dense_attn_join_kernel<T, D>, dim3((unsigned)rows), dim3(128), 0, stream, sp);
-    if (err != cudaSuccess) return cuda_error(err, "dense attention join");
-  }
-  return MF_OK;
+  return plan.pieces > 1 ? join<T, D>(sp, stream) : MF_OK;
 }
 
 template <typename T>
@@ -404,7 +406,16 @@ bool dense_attn_split_applies(const DenseParams& p, int head_dim) {
 }
 size_t dense_attn_split_workspace_bytes(const DenseParams& p, int head_dim) {
   const Plan plan = plan_of(p);
-  return plan.pieces > 1 ? align_up((size_t)plan.blocks * kRows * (head_dim + 2) * sizeof(float), 256) : 0;
+  return plan.pieces > 1 ? dense_attn_join_bytes(p, head_dim, plan.pieces) : 0;
+}
+size_t dense_attn_join_bytes(const DenseParams& p, int head_dim, int pieces) {
+  const long long row_tiles = ((long long)p.M * (p.H / p.K) + kRows - 1) / kRows;
+  return align_up((size_t)p.B * p.K * row_tiles * pieces * kRows * (head_dim + 2) * sizeof(float), 256);
+}
+int dense_attn_join(const DenseParams& p, int dtype, int head_dim, int pieces, float* acc, float* stat, cudaStream_t stream) {
+  const SplitParams sp{p, pieces, 0, acc, stat};
+  if (dtype == MF_DTYPE_BF16) return head_dim == 64 ? join<__nv_bfloat16, 64>(sp, stream) : join<__nv_bfloat16, 128>(sp, stream);
+  return head_dim == 64 ? join<__half, 64>(sp, stream) : join<__half, 128>(sp, stream);
 }
 int dense_attn_split(const DenseParams& p, int dtype, int head_dim, int kind, void* workspace, cudaStream_t stream) {
   return dtype == MF_DTYPE_BF16 ? pick<__nv_bfloat16>(p, head_dim, kind, workspace, stream) : pick<__half>(p, head_dim, kind, workspace, stream);

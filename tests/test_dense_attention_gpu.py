@@ -348,6 +348,40 @@ def test_distances_that_are_no_numbers():
     assert torch.equal(mfb.distance_buckets(x.cuda(), edges).cpu(), mfb.distance_buckets(x, edges))
 
 
+@pytest.mark.parametrize("bias", ["none", "offset", "pair"])
+@pytest.mark.parametrize("mask", ["none", "lengths", "causal", "holes"])
+@pytest.mark.parametrize("B,H,K,M,N,D", [(1, 2, 1, 300, 2500, 128), (2, 3, 1, 270, 2111, 64), (3, 1, 1, 400, 4097, 64), (1, 4, 4, 130, 2048, 128), (1, 1, 1, 2600, 2600, 64)])
+def test_few_tiles_of_queries_on_many_keys(B, H, K, M, N, D, mask, bias):
+    """Keys in pieces on tiles of 128 queries: pieces that some rows see nothing of, or nobody does; rows without a key; garbage in hidden places."""
+    g, q, k, v, grad = operands(M + N, B, H, K, M, N, D, torch.bfloat16)
+    num_k = num_q = key_mask = None
+    if mask == "lengths":
+        num_k, num_q = counts(g, B, N), counts(g, B, M)
+        num_k[-1] = N // 3 if B == 1 else 0
+        num_q[0] = M - 1
+        for b in range(B):
+            k[b, :, num_k[b] :], v[b, :, num_k[b] :], q[b, :, num_q[b] :] = math.nan, math.inf, math.nan
+    if mask == "holes":
+        key_mask = torch.rand(B, N, generator=g, device="cuda") < 0.7
+        key_mask[0, N // 4 : N // 4 + 1000] = False
+        key_mask[-1, :700] = False
+        for b in range(B):
+            k[b, :, ~key_mask[b]], v[b, :, ~key_mask[b]] = math.nan, -math.inf
+    table = buckets = None
+    if bias != "none":
+        table = torch.randn(16, H, generator=g, device="cuda")
+        table[3, 0] = -math.inf
+        buckets = mfb.offset_buckets(16, 40, device="cuda") if bias == "offset" else torch.randint(0, 18, (B, M, N), generator=g, device="cuda", dtype=torch.uint8)
+    kw = dict(num_keys=num_k, num_queries=num_q, key_mask=key_mask, causal=mask == "causal", bias=table, buckets=buckets)
+    with torch.no_grad():
+        out = mfb.dense_attention(q, k, v, num_k, num_q, key_mask=key_mask, causal=mask == "causal", bias=table, buckets=buckets)
+        check({"out": out}, exact(q, k, v, None, num_k, num_q, key_mask, mask == "causal", table, buckets, D**-0.5))
+        again = mfb.dense_attention(q, k, v, num_k, num_q, key_mask=key_mask, causal=mask == "causal", bias=table, buckets=buckets)
+        assert torch.equal(out, again)
+    if N < 2600:  # the log-sum-exp that the backward pass reads
+        run_both(q, k, v, grad, **kw)
+
+
 def test_no_wait_expired_in_all_of_these():
     """Runs last: the status word gathers since it was last asked for."""
     assert mfb.dense_attention_status() == 0
