@@ -386,6 +386,8 @@ long long blocks_of(const DenseParams& p) {
   return (p.H / p.K) % 2 == 0 ? tiles * p.B * (p.H / 2) : (tiles + 1) / 2 * p.B * p.H;
 }
 // Pieces of the keys: where the tiles of the queries would fill less than half of the SMs through long walks, as many as the SMs hold, of four tiles at least.
+// (Microseconds with | without: 2611 queries, 2 heads of 128 on one, 6412 keys 31 | 94; 512 queries, 8 heads of 64, 2048 keys 17 | 33, 4096 keys 20 | 61; 4111 causal, 4 heads of
+// 128 on one 53 | 70.)
 int pieces_of(const DenseParams& p) {
   const long long blocks = blocks_of(p), tiles = (p.N + kTcRows - 1) / kTcRows;
   if (blocks * 2 > 148 || tiles < 16) return 1;
