@@ -203,9 +203,12 @@ enum Family { kMma, kSmall, kSplit, kTensor };
 // where a third of a tile's rows is padding.  Head size 128: 64 x 256 tokens 55 | 99, 302 | 400; 64 x 700 queries on 100 keys 110 | 157, 511 | 604; 85 x 192 tokens 67 | 80
 // forward, but 279 | 248 backward, and by pairs 76 | 67 forward.  There many short entries pay forward unless by pairs: 128 x 128 tokens 54 | 64, 128 x 65 tokens 51 | 54; few
 // do not: 2 x 160 tokens 13 | 10.
+// Fewer than 64 queries: 32 on 4096 keys, 32 heads of 64, 19 | 80, 91 | 185, four such entries 49 | 81, 251 | 266; but 16 entries of 17 on 2048 103 | 62, 512 | 380; heads of 128 122 |
+// 137, 733 | 771.
 bool tensor_pays(const DenseParams& p, int head_dim, int kind, bool backward) {
-  if (p.M < 64 || p.N <= 64) return false;
-  if (((p.M + 63ll) / 64) * ((p.N + 63ll) / 64) >= 16) return true;
+  if (p.N <= 64) return false;
+  if (((p.M + 63ll) / 64) * ((p.N + 63ll) / 64) >= 16) return p.M >= 64 || head_dim == 128 || (long long)p.B * p.H <= 148;
+  if (p.M < 64) return false;
   return !backward && head_dim == 128 && kind != MF_BUCKETS_PAIR && (long long)p.B * p.H >= 148;
 }
 Family fwd_family(const MfDenseAttnArgs& a, const DenseParams& p) {
