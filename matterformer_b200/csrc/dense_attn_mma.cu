@@ -11,7 +11,7 @@
 // Every output has one owner and a fixed order of its sums.
 //
 // Registers bound it: 64 x 64 logits, their gradients and the sums are 128 to 168 of a thread's, three or four CTAs on an SM (without that limit 255 and two, 64
-// molecules of 19 to 192 tokens 124 us instead of 120 for forward and backward), which use a third of the issue slots and a fifth of the tensor pipe. There: forward 26,
+// molecules of 19 to 192 tokens 124 us instead of 120 for forward and backward, 116 now), which use a third of the issue slots and a fifth of the tensor pipe. There: forward 26,
 // DQ 48, DKV 39 us; 8 x 577 fp16 queries on 1000 keys, 4 heads of 32, 22 + 26 + 19 us. 64 rows to a tile: fewer waste products for molecules of all lengths.
 #include "dense_attn.cuh"
 

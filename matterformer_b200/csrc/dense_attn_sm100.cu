@@ -7,8 +7,8 @@
 // products of a tile take 1 024 clocks and its exponentials 1 024 (16 a clock), at head size 64 the exponentials bound it.  The accumulator stays
 // in tensor memory and is scaled only where a row's maximum has grown by more than 2^8 since it last was; until then P may exceed 1, which
 // costs neither type precision.  Sums are of P before it is rounded.
-// Two cells of 4096 tokens, 8 heads of 64, with the bias: 122 us, 563 TFLOP/s, exponential unit 61 %; a causal prompt of 4111 fp16 tokens, 16 heads on 4 of 128: 88 us,
-// 787 TFLOP/s, exponentials and tensor pipe 46 % each.
+// Two cells of 4096 tokens, 8 heads of 64, with the bias: 122 us, 563 TFLOP/s, exponential unit 61 %; a causal prompt of 4111 fp16 tokens, 16 heads on 4 of 128: 85 us,
+// 813 TFLOP/s, exponentials and tensor pipe 46 % each.
 //
 // Roles: warps 0-3 and 4-7 own the rows of the two tiles, one thread of warp 8 issues the products, one of warp 9 the copies, warp 10 clears the rows
 // of V that are no keys (behind the entry's length, or masked), which may hold anything and meet P = 0.  Every wait is bounded; an expired one
