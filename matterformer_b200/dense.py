@@ -131,7 +131,8 @@ class RelativeBias:
             return torch.linspace(0.0, float(self.reach), self.num_buckets, dtype=torch.float64, device="cpu")[1:].contiguous()
 
     def buckets(self, positions: Optional[torch.Tensor], num_tokens: Optional[torch.Tensor], device) -> torch.Tensor:
-        """As :func:`dense_attention` takes them; ``positions`` (B, N, 3) for distances."""
+        """As :func:`dense_attention` takes them; ``positions`` (B, N, 3) for distances.  ``num_tokens``: (B,) counts of real tokens, of entries
+        whose padding is at the end; ``None`` for padding anywhere."""
         if self.kind == "offset":
             return offset_buckets(self.num_buckets, int(self.reach), device=device)
         return distance_buckets(positions.detach().float(), self.edges, num_tokens)

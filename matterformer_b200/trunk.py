@@ -641,7 +641,8 @@ class TransformerTrunk(nn.Module):
         if self.relative_bias is not None:
             coords = turning.pop("coords")
             if mha:
-                turning["buckets"] = self._offset_buckets if coords is None else self.relative_bias.buckets(coords, num_atoms, x.device)
+                # (of all places: the padding may lie anywhere, and the layers hide its keys)
+                turning["buckets"] = self._offset_buckets if coords is None else self.relative_bias.buckets(coords, None, x.device)
         suffix = _padding_is_suffix(self, pad_mask) if reads else None  # one read-back for all layers
         h, norm = None, self.norm_out
         last = len(self.blocks) - 1

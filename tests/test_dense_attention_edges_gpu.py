@@ -1,0 +1,83 @@
+"""Dense attention and distance buckets where inputs are unusual: padding that is not at the end, values that are no numbers, empty calls, strides of
+zero, many query heads on one key head."""
+import copy
+import math
+
+import pytest
+import torch
+from test_dense_attention_gpu import counts, operands, run_both
+
+import matterformer_b200 as mfb
+from matterformer_b200 import _lib
+from matterformer_b200.trunk import EDMModel, RegularAttention, TransformerTrunk
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+NAN = math.nan
+
+
+@pytest.fixture
+def backend(request):
+    prev = mfb.set_dense_backend(request.param)
+    yield request.param
+    mfb.set_dense_backend(prev)
+
+
+def _pad_masks(form, B, N):
+    """Padding in front, in the middle, or at random places; every row keeps at least two atoms."""
+    g = torch.Generator().manual_seed(N)
+    if form == "front":
+        return torch.arange(N) < torch.tensor([0, N // 3, N - 2])[:B, None]
+    if form == "middle":
+        return (torch.arange(N) >= N // 4) & (torch.arange(N) < N // 4 + torch.tensor([1, N // 3, N // 2])[:B, None])
+    mask = torch.rand(B, N, generator=g) < 0.4
+    mask[:, [0, N - 1]] = False
+    return mask
+
+
+@pytest.mark.parametrize("impl", ["auto", "torch"])
+@pytest.mark.parametrize("form", ["front", "middle", "random"])
+@pytest.mark.parametrize("N", [6, 29, 150])
+def test_distances_beside_padding_anywhere(N, form, impl):
+    """A trunk biased by distances: the buckets that its layers get are those of the distances for all pairs of atoms, and its output and the tables' gradients are
+    those of the same trunk in fp32 on the CPU: within 1e-3 of the largest value in fp32 (sums of 1024 terms, each rounded to 2^-24 of what it holds, through two
+    layers and their norms), 2e-2 under bf16 autocast, as the layers' other tests."""
+    torch.manual_seed(N)
+    spec = mfb.RelativeBias(32, "distance", 8.0)
+    trunk = TransformerTrunk(128, 2, ["mha", "mha"], relative_bias=spec, mha_impl=impl)
+    for block in trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].bias, std=0.3)
+        torch.nn.init.normal_(block.attn.bias_table, std=2.0)
+    x, cond, coords, grad = torch.randn(3, N, 128), torch.randn(3, 128), torch.randn(3, N, 3) * 3, torch.randn(3, N, 128)
+    mask = _pad_masks(form, 3, N)
+    there = ~mask
+    pairs = there[:, :, None] & there[:, None]
+    want_buckets = mfb.distance_buckets(coords, spec.edges)
+    results = []
+    for device, low in (("cpu", False), ("cuda", impl == "auto")):
+        net = copy.deepcopy(trunk).to(device)
+        given = []
+        net.blocks[0].attn.register_forward_pre_hook(lambda _, args, kw: given.append(kw["buckets"]), with_kwargs=True)
+        with torch.autocast("cuda", BF16, enabled=low):
+            out = net(x.to(device), cond.to(device), pad_mask=mask.to(device), coords=coords.to(device))
+        (out.float() * grad.to(device)).sum().backward()
+        assert torch.equal(given[0].cpu()[pairs], want_buckets[pairs])
+        results.append([out.detach().float().cpu()] + [b.attn.bias_table.grad.cpu() for b in net.blocks])
+        assert device == "cpu" or {b.attn._last_core_used for b in net.blocks} == {"dense" if low else "torch"}
+    for a, b in zip(*results):
+        assert (a - b).abs().max() <= (2e-2 if impl == "auto" else 1e-3) * a.abs().max()
+
+
+@pytest.mark.parametrize("form", ["front", "random"])
+def test_a_model_with_padding_anywhere(form):
+    """The same through a model, in fp32: two devices, one answer."""
+    torch.manual_seed(1)
+    model = EDMModel(d_model=64, n_heads=2, n_layers=2, attn_types=["mha", "mha"], relative_bias=mfb.RelativeBias(16, "distance", 6.0))
+    for block in model.trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].bias, std=0.3)
+        torch.nn.init.normal_(block.attn.bias_table, std=2.0)
+    atoms, coords, sigma, mask = torch.randn(3, 21, 6), torch.randn(3, 21, 3) * 2, torch.rand(3) + 0.2, _pad_masks(form, 3, 21)
+    want = model(atoms, coords, mask, sigma)
+    got = copy.deepcopy(model).cuda()(atoms.cuda(), coords.cuda(), mask.cuda(), sigma.cuda())
+    for a, b in zip(got, want):
+        assert (a.cpu() - b)[~mask].abs().max() <= 1e-3 * b.abs().max()
