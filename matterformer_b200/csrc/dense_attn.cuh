@@ -139,7 +139,7 @@ int dense_attn_small(const DenseParams& p, int dtype, int head_dim, int bucket_k
 bool dense_attn_split_applies(const DenseParams& p, int head_dim);
 size_t dense_attn_split_workspace_bytes(const DenseParams& p, int head_dim);
 // Joins pieces of the keys: acc [entry * key head][tile of 16 rows][piece][16][D] in units of exp2(-top), stat the same without D: top, total.  A row is query * group +
-// head of the group; a top of minus infinity stands for a piece that wrote nothing.
+// head of the group; a total of zero stands for a piece that wrote no row.  Where all logits are no numbers top is minus infinity and total none.
 int dense_attn_join(const DenseParams& p, int dtype, int head_dim, int pieces, float* acc, float* stat, cudaStream_t stream);
 size_t dense_attn_join_bytes(const DenseParams& p, int head_dim, int pieces);
 int dense_attn_split(const DenseParams& p, int dtype, int head_dim, int bucket_kind, void* workspace, cudaStream_t stream);

@@ -215,7 +215,8 @@ __global__ void __launch_bounds__(kThreads) dense_attn_split_kernel(const __grid
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      l += meet[w][r][0] == -INFINITY ? 0.f : meet[w][r][1] * dense_exp2(meet[w][r][0] - m);
+      // (logits that are no numbers have no maximum, but a total that is none: whether something was seen is for the total to say)
+      l += meet[w][r][0] == -INFINITY ? meet[w][r][1] : meet[w][r][1] * dense_exp2(meet[w][r][0] - m);
       const float4 x = *reinterpret_cast<const float4*>(plane + (w * kRows + r) * D + c);
       v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(128) dense_attn_join_kernel(const __grid_const
   for (int s = tid; s < sp.pieces; s += 128) {
     const float t = sp.stat[slot(s) * 2], w = t == -INFINITY ? 0.f : dense_exp2(t - m);
     weight[s] = w;
-    if (w != 0.f) l = fmaf(w, sp.stat[slot(s) * 2 + 1], l);
+    l = fmaf(w, sp.stat[slot(s) * 2 + 1], l);  // (a weight of zero as well: a total that is no number stays none)
   }
   l = warp_sum(l);
   if (lane == 0) meet[warp][1] = l;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(128) dense_attn_join_few_kernel(const __grid_c
   auto slot = [&](int s) { return (base + s) * kRows + row % kRows; };
   const float t = lane < sp.pieces ? sp.stat[slot(lane) * 2] : -INFINITY;
   const float m = warp_max(t), w = t == -INFINITY ? 0.f : dense_exp2(t - m);
-  const float l = warp_sum(w != 0.f ? w * sp.stat[slot(lane) * 2 + 1] : 0.f);
+  const float l = warp_sum(lane < sp.pieces ? w * sp.stat[slot(lane) * 2 + 1] : 0.f);  // (as above)
   float sum[E] = {};
 #pragma unroll 4
   for (int s = 0; s < sp.pieces; ++s) {

@@ -81,3 +81,48 @@ def test_a_model_with_padding_anywhere(form):
     got = copy.deepcopy(model).cuda()(atoms.cuda(), coords.cuda(), mask.cuda(), sigma.cuda())
     for a, b in zip(got, want):
         assert (a.cpu() - b)[~mask].abs().max() <= 1e-3 * b.abs().max()
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float16])
+@pytest.mark.parametrize("bias", ["none", "offset", "pair"])
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05"], indirect=True)
+@pytest.mark.parametrize("B,H,K,M,N,D", [
+    (2, 2, 2, 9, 29, 64),      # small entries
+    (2, 4, 2, 1, 100, 64),     # few queries, one piece
+    (2, 4, 2, 2, 2000, 128),   # up to 32 pieces
+    (1, 2, 2, 1, 32768, 64),   # more
+    (1, 2, 1, 300, 2500, 128), # tiles of 128 queries, keys in pieces
+    (1, 2, 2, 300, 700, 64),   # the same in one piece
+    (1, 2, 2, 70, 130, 32),
+])  # fmt: skip
+def test_what_is_no_number_stays_none(backend, B, H, K, M, N, D, bias, dtype):
+    """A row that sees a logit that is not a number is none, whatever the sizes: a query of NaN, and a whole stretch of keys (with the others' rows as they
+    are without it); its log-sum-exp is none either, so that the gradients show it."""
+    g, q, k, v, grad = operands(M + N, B, H, K, M, N, D, dtype)
+    table = buckets = None
+    if bias != "none":
+        table = torch.randn(16, H, generator=g, device="cuda")
+        buckets = mfb.offset_buckets(16, 40, device="cuda") if bias == "offset" else torch.randint(0, 18, (B, M, N), generator=g, device="cuda", dtype=torch.uint8)
+
+    def call(q, k):
+        return mfb.dense_attention(q, k, v, bias=table, buckets=buckets)
+
+    want = call(q, k)
+    bad = q.clone()
+    bad[-1, 1, M // 2] = NAN
+    got = call(bad, k)
+    assert got[-1, 1, M // 2].isnan().all()
+    got[-1, 1, M // 2] = want[-1, 1, M // 2]
+    assert torch.equal(got, want)
+    for first, last in ((0, N), (N // 4, N - N // 4), (N - 1, N)):
+        bad = k.clone()
+        bad[-1, 0, first:last] = NAN
+        got = call(q, bad)
+        assert got[-1, : H // K].isnan().all()
+        got[-1, : H // K] = want[-1, : H // K]
+        assert torch.equal(got, want)
+    leaf, keys = q.clone(), k.clone().requires_grad_()
+    leaf[-1, 1, M // 2] = NAN
+    leaf.requires_grad_()
+    dq, dk = torch.autograd.grad(call(leaf, keys), [leaf, keys], grad)
+    assert dq[-1, 1, M // 2].isnan().all() and dk[-1, 1 * K // H].isnan().all()
