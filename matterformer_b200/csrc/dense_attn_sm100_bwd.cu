@@ -48,6 +48,24 @@ struct BwdShape {
   static constexpr int kDiagonalBytes = kTcRows * (kDiagonals + 1) * 4;
 };
 
+// Diagonals of dS of the W columns from c0 + w0 on: offset of the diagonal that starts in row 127 - r (which = 0), or in column r + 1 (1, for r < W - 1 alone), among
+// the kSpan of a step.  What other threads get for the latter is of no use to them, but an entry of the step all the same.
+__host__ __device__ constexpr int diagonal_of(int which, int c0, int w0, int r) {
+  const int e = c0 + w0 + r + (which ? kTcRows : 0);
+  return e < kSpan ? e : kSpan - 1;
+}
+template <int W>
+__host__ __device__ constexpr bool diagonals_fit() {  // entries of the step, and those that are used are the ones meant
+  for (int c0 = 0; c0 < kPart; c0 += kCols)
+    for (int w0 = 0; w0 < kCols; w0 += W)
+      for (int r = 0; r < kTcRows; ++r)
+        for (int which = 0; which < 2; ++which) {
+          const int e = diagonal_of(which, c0, w0, r);
+          if (e < 0 || e >= kSpan || ((which == 0 || r < W - 1) && e != c0 + w0 + r + which * kTcRows)) return false;
+        }
+  return true;
+}
+
 // D[tmem] += A[smem] * B[smem] of fp32 words, of which the tensor cores take the leading 11 bits of the mantissa; eight to an instruction
 __device__ __forceinline__ void umma_tf32_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
@@ -477,7 +495,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
               for (int c = 1; c < W; ++c)
                 if (c > r) v[1] += tile[(c - r - 1) * (W + 1) + c];
             }
-            const int b0 = near_bucket[c0 + w0 + r], b1 = near_bucket[c0 + w0 + min(r + 128, kSpan - 1 - w0)];
+            static_assert(diagonals_fit<W>(), "a step has the buckets of kSpan offsets");
+            const int b0 = near_bucket[diagonal_of(0, c0, w0, r)], b1 = near_bucket[diagonal_of(1, c0, w0, r)];
             if (r < 64) {
               if (b0 < p.num_buckets) column[b0 * 256] += v[0];
               if (r < W - 1 && b1 < p.num_buckets) column[b1 * 256] += v[1];

@@ -126,3 +126,15 @@ def test_what_is_no_number_stays_none(backend, B, H, K, M, N, D, bias, dtype):
     leaf.requires_grad_()
     dq, dk = torch.autograd.grad(call(leaf, keys), [leaf, keys], grad)
     assert dq[-1, 1, M // 2].isnan().all() and dk[-1, 1 * K // H].isnan().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("reach", [1, 5, 63, 64, 100, 190, 512])
+@pytest.mark.parametrize("backend", ["tcgen05"], indirect=True)
+def test_steps_at_either_end_of_the_map(backend, D, reach):
+    """Steps of 64 keys whose offsets end or begin at the map's ends, where the sums along diagonals read its last entries."""
+    for shift in (0, 1, reach % 64):
+        M, N = 200, 200 + reach + shift
+        g, q, k, v, grad = operands(reach + D, 1, 2, 2, M, N, D, BF16)
+        table, buckets = torch.randn(16, 2, generator=g, device="cuda"), mfb.offset_buckets(16, reach, device="cuda")
+        run_both(q, k, v, grad, bias=table, buckets=buckets)
