@@ -94,6 +94,11 @@ __device__ __forceinline__ uint2 eight_bytes(const uint8_t* at, int n) {
   return make_uint2(__funnelshift_r(a, b, 8 * skip), __funnelshift_r(b, c, 8 * skip));
 }
 
+// The first `bytes` of 16, zeros behind them; no others are read.
+__device__ __forceinline__ void cp_async_part16(uint32_t smem_addr, const void* gptr, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr), "l"(gptr), "r"(bytes) : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>

@@ -130,10 +130,10 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
       const bool ok = i0 + r < len.nq && j0 + c < len.nk;
       const uint8_t* src = p.buckets + (ok ? b * p.bucket_batch + (i0 + r) * p.bucket_row + j0 + c : 0);
       uint8_t* dst = pair_tile + stage * kPairTile + r * kPairRow + c;
-      if (aligned) {  // (a row's last 16 bytes may end behind the last key, but not behind the row)
-        cp_async16(static_cast<uint32_t>(__cvta_generic_to_shared(dst)), src, ok);
+      const int n = ok ? p.N - j0 - c : 0;  // (a row's storage may end with its last key, whatever the stride)
+      if (aligned) {
+        cp_async_part16(static_cast<uint32_t>(__cvta_generic_to_shared(dst)), src, min(n, 16));
       } else {
-        const int n = ok ? p.N - j0 - c : 0;
         const uint2 x = eight_bytes(src, n), y = eight_bytes(src + 8, n - 8);
         *reinterpret_cast<uint4*>(dst) = make_uint4(x.x, x.y, y.x, y.y);
       }

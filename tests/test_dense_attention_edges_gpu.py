@@ -138,3 +138,18 @@ def test_steps_at_either_end_of_the_map(backend, D, reach):
         g, q, k, v, grad = operands(reach + D, 1, 2, 2, M, N, D, BF16)
         table, buckets = torch.randn(16, 2, generator=g, device="cuda"), mfb.offset_buckets(16, reach, device="cuda")
         run_both(q, k, v, grad, bias=table, buckets=buckets)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05"], indirect=True)
+@pytest.mark.parametrize("M,N", [(40, 37), (70, 90), (200, 161), (300, 555)])
+def test_pairs_of_one_row_for_all_queries(backend, M, N, D):
+    """Buckets with a stride of zero over the queries, and rows that overlap, each ending with its storage: as a copy with rows of their own."""
+    g, q, k, v, grad = operands(M + N, 2, 2, 2, M, N, D, BF16)
+    table = torch.randn(16, 2, generator=g, device="cuda")
+    store = torch.randint(0, 18, (N + 16 * (M - 1),), generator=g, device="cuda", dtype=torch.uint8)
+    for buckets in (store[:N].expand(2, M, N), store[-N - 16 :][16:].expand(1, M, N), store.as_strided((1, M, N), (0, 16, 1)), store.as_strided((1, M, N), (0, 1, 1))):
+        got = run_both(q, k, v, grad, bias=table, buckets=buckets)
+        want = run_both(q, k, v, grad, bias=table, buckets=buckets.contiguous())
+        if backend == "mma":
+            assert all(torch.equal(got[n], want[n]) for n in want)
