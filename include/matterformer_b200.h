@@ -755,7 +755,7 @@ typedef struct MfRows { /* elements between neighbouring entries; the channels o
  * key returns zeros.
  *
  * bias (num_buckets, heads) in bias_dtype or NULL; buckets as bucket_kind says, the offset being j - i - (num_keys - num_queries);
- * bucket_row and bucket_batch are the strides of the pairs' (bytes).  Up to 128 buckets; a bucket beyond the table has no bias and no
+ * bucket_row and bucket_batch are the strides of the pairs' (bytes), buckets is NULL where there are no pairs.  Up to 128 buckets; a bucket beyond the table has no bias and no
  * gradient.  An entry of minus infinity or below -1e30 hides its pairs.
  *
  * lse (batch, heads, queries) fp32 is written by the forward call where it is not NULL; the backward call takes it and out.  It forms the

@@ -164,7 +164,9 @@ int check_args(const char* name, const MfDenseAttnArgs* a) {
   MF_CHECK_ARG(a->scale == a->scale && a->scale - a->scale == 0.f, "%s: scale must be finite", name);
   MF_CHECK_ARG(a->backend >= MF_DENSE_BACKEND_AUTO && a->backend <= MF_DENSE_BACKEND_TCGEN05, "%s: unknown backend %d", name, a->backend);
   const bool table = a->bias != nullptr;
-  MF_CHECK_ARG(table == (a->bucket_kind != MF_BUCKETS_NONE) && table == (a->buckets != nullptr), "%s: bias, buckets and bucket_kind go together", name);
+  // (the buckets of no pairs have no address)
+  const bool no_pairs = a->bucket_kind == MF_BUCKETS_PAIR && (a->batch == 0 || a->queries == 0 || a->keys == 0);
+  MF_CHECK_ARG(table == (a->bucket_kind != MF_BUCKETS_NONE) && (table == (a->buckets != nullptr) || (table && no_pairs)), "%s: bias, buckets and bucket_kind go together", name);
   if (table) {
     MF_CHECK_ARG(a->bucket_kind == MF_BUCKETS_OFFSET || a->bucket_kind == MF_BUCKETS_PAIR, "%s: unknown bucket_kind %d", name, a->bucket_kind);
     MF_CHECK_ARG(a->num_buckets >= 1 && a->num_buckets <= kMaxBuckets, "%s: between 1 and %d buckets, got %d", name, kMaxBuckets, a->num_buckets);

@@ -153,3 +153,17 @@ def test_pairs_of_one_row_for_all_queries(backend, M, N, D):
         want = run_both(q, k, v, grad, bias=table, buckets=buckets.contiguous())
         if backend == "mma":
             assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05"], indirect=True)
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("B,M,N", [(0, 50, 50), (2, 0, 50), (2, 50, 0), (2, 0, 0), (0, 0, 0)])
+def test_empty_calls_by_pairs(backend, B, M, N, one):
+    """Buckets of no pairs: zeros, forward and backward, as by offsets."""
+    q, k, v = (torch.randn(B, 2, n, 64, device="cuda").to(BF16).requires_grad_() for n in (M, N, N))
+    table = torch.randn(8, 2, device="cuda", requires_grad=True)
+    buckets = torch.zeros(1 if one else B, M, N, device="cuda", dtype=torch.uint8)
+    out = mfb.dense_attention(q, k, v, bias=table, buckets=buckets)
+    assert out.shape == q.shape and not out.any()
+    grads = torch.autograd.grad(out, [q, k, v, table], torch.ones_like(out))
+    assert all(not g.any() and g.shape == t.shape for g, t in zip(grads, (q, k, v, table)))
