@@ -230,7 +230,7 @@ class _DenseAttention(torch.autograd.Function):
         ws = _workspace(a, L.mf_dense_attn_fwd_workspace_bytes(ctypes.byref(a)), q.device)  # noqa: F841 (until the launch)
         _lib.launch(L.mf_dense_attn_fwd, q.device, ctypes.byref(a))
         _raise_expired(q.device)
-        out = out.transpose(1, 2).reshape(q.shape[0], q.shape[2], -1) if heads else out
+        out = out.transpose(1, 2).flatten(2) if heads else out
         if keep:
             aux = [t.clone() if t is not None and t.is_inference() else t for t in (buckets, num_queries, num_keys, key_mask)]
             ctx.save_for_backward(*given, table, out, lse, *aux)
@@ -255,7 +255,7 @@ class _DenseAttention(torch.autograd.Function):
         grad_out = grad_out.to(out.dtype)
         if heads:
             q, k, v = _split(given[0], heads)
-            out, grad_out = (t.reshape(*t.shape[:2], heads, -1).transpose(1, 2) for t in (out, grad_out))
+            out, grad_out = (t.unflatten(-1, (heads, q.shape[-1])).transpose(1, 2) for t in (out, grad_out))
             made = torch.empty_like(given[0])
             dq, dk, dv = _split(made, heads)
         else:

@@ -167,3 +167,16 @@ def test_empty_calls_by_pairs(backend, B, M, N, one):
     assert out.shape == q.shape and not out.any()
     grads = torch.autograd.grad(out, [q, k, v, table], torch.ones_like(out))
     assert all(not g.any() and g.shape == t.shape for g, t in zip(grads, (q, k, v, table)))
+
+
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05"], indirect=True)
+@pytest.mark.parametrize("bias", ["none", "offset", "pair"])
+@pytest.mark.parametrize("B,N", [(0, 50), (2, 0), (0, 0)])
+def test_empty_packed_calls(backend, B, N, bias):
+    qkv = torch.randn(B, N, 3 * 2 * 64, device="cuda").to(BF16).requires_grad_()
+    table = None if bias == "none" else torch.randn(8, 2, device="cuda", requires_grad=True)
+    buckets = {"none": None, "offset": mfb.offset_buckets(8, 10, device="cuda"), "pair": torch.zeros(1, N, N, device="cuda", dtype=torch.uint8)}[bias]
+    out = mfb.dense_attention_packed(qkv, 2, bias=table, buckets=buckets)
+    leaves = [qkv] if table is None else [qkv, table]
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert out.shape == (B, N, 128) and all(not g.any() and g.shape == t.shape for g, t in zip(grads, leaves))
