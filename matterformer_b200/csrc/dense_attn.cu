@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
           const float* o = x + (j0 + c) * 3ll;
           const float q0 = o[0], q1 = o[1], q2 = o[2];
           int lo = 0, hi = edges.n;  // edges below lo are at or below the distance, those from hi on above it
-          if (p0 == q0 && p1 == q1 && p2 == q2) {  // an atom and itself: every row has one
+          if (p0 - q0 == 0.f && p1 - q1 == 0.f && p2 - q2 == 0.f) {  // an atom and itself: every row has one (but at infinity that is no distance)
             lo = hi = edges.zeros;
           } else {
             const double ex = (double)p0 - q0, ey = (double)p1 - q1, ez = (double)p2 - q2;

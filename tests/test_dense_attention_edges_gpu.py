@@ -180,3 +180,14 @@ def test_empty_packed_calls(backend, B, N, bias):
     leaves = [qkv] if table is None else [qkv, table]
     grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
     assert out.shape == (B, N, 128) and all(not g.any() and g.shape == t.shape for g, t in zip(grads, leaves))
+
+
+def test_infinite_places_and_an_edge_at_zero():
+    """An atom at infinity is no distance from itself: bucket 0, as on the CPU, whatever the edges."""
+    x = torch.randn(2, 70, 3, generator=torch.Generator().manual_seed(0)) * 3
+    x[0, 5, 1], x[1, 0, 0], x[1, 40, 2], x[1, 41, 2], x[0, 9] = NAN, math.inf, -math.inf, 3e38, math.inf
+    x[0, 20] = x[0, 30]
+    for edges in (torch.linspace(0.0, 12.0, 32, dtype=torch.float64), torch.zeros(3, dtype=torch.float64), torch.tensor([0.0, 0.0, 1.0, math.inf], dtype=torch.float64)):
+        got = mfb.distance_buckets(x.cuda(), edges).cpu()
+        assert torch.equal(got, mfb.distance_buckets(x, edges))
+        assert got[1, 0, 0] == got[1, 40, 40] == got[0, 5, 5] == 0 and got[0, 0, 0] == got[0, 20, 30] == (edges == 0).sum()
