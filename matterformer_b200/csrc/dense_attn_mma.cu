@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
   }
   const float sc2 = p.scale * kDenseLog2e;
   float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f}, lse[2] = {INFINITY, INFINITY}, delta[2] = {0.f, 0.f};
+  bool blind[2] = {false, false};  // DQ: queries that see nothing: they and their gradients may hold anything
   if (MODE == D_DQ) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // the four lanes of a row take a quarter of its channels each
@@ -237,12 +238,15 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
           }
         }
         lse[e] = p.lse[stat(oh) + row];
+        blind[e] = lse[e] == INFINITY;
       }
       d += __shfl_xor_sync(0xffffffffu, d, 1);
       d += __shfl_xor_sync(0xffffffffu, d, 2);
-      delta[e] = d;
+      delta[e] = blind[e] ? 0.f : d;
+      if (blind[e]) real[e] = false;
     }
   }
+  const bool some_blind = MODE == D_DQ && __any_sync(0xffffffffu, blind[0] || blind[1]);
   float error[2] = {0.f, 0.f};  // sums of dS, zero but for what delta is off by
 
 
@@ -265,6 +269,19 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
     if (STAGES == 2) {
       if (t + 1 < steps) load_step(t + 1, stage ^ 1, seen_next);
       cp_async_commit();
+    }
+    if constexpr (MODE == D_DKV) {  // queries that see nothing, and their gradients, may hold anything; all warps see the same of them
+      auto blind_rows = [&](int i) { return __ballot_sync(0xffffffffu, at + i < len.nq && part_lse[stage * 64 + i] == INFINITY); };
+      const uint2 rows = make_uint2(blind_rows(lane), blind_rows(lane + 32));
+      if (rows.x | rows.y) {
+        uint8_t* tile_at = smem + ((MODE == D_FWD ? 1 : 2) + stage) * TILE;  // part_a; part_b lies STAGES tiles behind it
+        for (int idx = tid; idx < 64 * (D / 8); idx += kThreads) {
+          const int r = idx / (D / 8), c = idx % (D / 8);
+          if (((r & 32 ? rows.y : rows.x) >> (r & 31)) & 1u)
+            *reinterpret_cast<uint4*>(tile_at + (r * LD + c * 8) * 2) = *reinterpret_cast<uint4*>(tile_at + STAGES * TILE + (r * LD + c * 8) * 2) = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+      }
     }
 
     if (!idle) {
@@ -373,6 +390,15 @@ __global__ void __launch_bounds__(kThreads, D <= 64 ? (MODE == D_FWD ? 4 : 3) : 
             dp[nt][e] = pr * (dp[nt][e] - d);
             if (MODE == D_DQ) error[e >> 1] += dp[nt][e];
           }
+        if (MODE == D_DQ && some_blind) {
+#pragma unroll
+          for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (blind[e >> 1]) s[nt][e] = dp[nt][e] = 0.f;
+          if (blind[0]) error[0] = 0.f;
+          if (blind[1]) error[1] = 0.f;
+        }
         if (MODE == D_DQ && steps == 1) {  // the whole row is here: its exact delta
 #pragma unroll
           for (int e = 0; e < 2; ++e) {

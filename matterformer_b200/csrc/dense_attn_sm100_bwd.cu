@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
           if (next.t >= steps) return;
           const int i = next.row + c;
           const long long stat = ((long long)b * p.H + next.head) * p.M + i;
-          l = i < len.nq ? p.lse[stat] : INFINITY, d = i < len.nq ? p.delta[stat] : 0.f;
+          l = i < len.nq ? p.lse[stat] : INFINITY, d = i < len.nq ? p.delta[stat] : 0.f;  // (delta of a query that sees nothing is zero)
           advance(next, 1);
         };
         if (DKV)
@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
             const int start = first_offset(at);
             one = start + kSpan - 1 <= -p.reach ? far_bias[0] : start >= p.reach ? far_bias[1] : 0.f;
           }
+          const bool sees = lse[u] != INFINITY;  // queries that see nothing, and their gradients, may hold anything
           wait_on(&bar_full[stage], w.t / S);
           if (DKV) {
             float v = (one - lse[u]) * fabsf(per);
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
             *reinterpret_cast<float4*>(line + ((0 ^ (c & 7)) << 4)) = three_parts(per < 0.f ? -v : v);
             *reinterpret_cast<float4*>(line + ((2 ^ (c & 7)) << 4)) = three_parts(-delta[u]);
           }
-          const bool there = at + c < part_rows && (DKV || !mask || mask[at + c]);
+          const bool there = at + c < part_rows && (DKV ? sees : !mask || mask[at + c]);
           if (!bad && !there && at + c < part_all) {  // (what lies behind the tensor is zeros already)
 #pragma unroll 1
             for (int i = 0; i < 2 * Sh::kChunks * 8; ++i)
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
     const int c0 = half * kCols, pair = tid & 255, team = warp >> 2;  // the 256 threads of a group are pairs of 128
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const int row = row0 + r;
-    const bool row_ok = row < own_rows;
+    bool row_ok = row < own_rows;
     const float sc2 = p.scale * kDenseLog2e;
     float lse = 0.f, delta = 0.f;
     // visible partners of this row: [lo, hi) at DKV and DQ; a row that is none may see what it wants
@@ -358,6 +359,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       if (row_ok) {
         hi = dense_limit(p, len, row);
         lse = p.lse[stat + row];
+        row_ok = lse != INFINITY;  // a query that sees nothing, and its gradient, may hold anything
         // delta: a quarter of the channels each
         const uint4* go = reinterpret_cast<const uint4*>(static_cast<const T*>(p.grad_out) + p.go_rows.at(b, head, row) + team * (D / 4));
         const uint4* o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + p.out_rows.at(b, head, row) + team * (D / 4));
@@ -377,6 +379,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) dense_attn_tc_bwd_kernel(const
       errors[team][r] = delta;
       group_barrier(7, 512);
       delta = (errors[0][r] + errors[1][r]) + (errors[2][r] + errors[3][r]);
+      if (!row_ok) delta = 0.f;
       if (row < p.M && team == 0) p.delta[stat + row] = delta;
     } else if (row_ok) {
       lo = dense_first(p, len, row);

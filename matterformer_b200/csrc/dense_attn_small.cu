@@ -202,6 +202,16 @@ __global__ void __launch_bounds__(kWarps * 32, BWD || D == 128 ? 5 : 8) dense_at
     const bool q2 = len.nq > 16;
     cp_async_wait<0>();
     __syncwarp();
+    if constexpr (BWD) {  // queries that see nothing, and their gradients, may hold anything
+      auto blind = [&](int x) { return g + 8 * x < len.nq && lse[x] == INFINITY; };
+      if (__any_sync(0xffffffffu, blind(0) || blind(1) || blind(2) || blind(3))) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          for (int c = t4; blind(x) && c < D / 8; c += 4)
+            *reinterpret_cast<uint4*>(t_q + q_place<D>(g + 8 * x, c)) = *reinterpret_cast<uint4*>(t_o + q_place<D>(g + 8 * x, c)) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+      }
+    }
 
     uint32_t P[2][2][4], S[BWD ? 2 : 1][2][4];  // packed, [query half][pair of column tiles]: A operands of products over the keys
 #pragma unroll

@@ -191,3 +191,30 @@ def test_infinite_places_and_an_edge_at_zero():
         got = mfb.distance_buckets(x.cuda(), edges).cpu()
         assert torch.equal(got, mfb.distance_buckets(x, edges))
         assert got[1, 0, 0] == got[1, 40, 40] == got[0, 5, 5] == 0 and got[0, 0, 0] == got[0, 20, 30] == (edges == 0).sum()
+
+
+@pytest.mark.parametrize("bias", ["none", "offset", "pair"])
+@pytest.mark.parametrize("backend", ["auto", "mma", "tcgen05"], indirect=True)
+@pytest.mark.parametrize("B,H,K,M,N,D", [(3, 2, 2, 29, 20, 64), (3, 2, 2, 20, 29, 32), (2, 4, 2, 90, 70, 64), (2, 2, 1, 300, 260, 64), (2, 2, 2, 300, 260, 128), (1, 2, 2, 130, 700, 32)])
+def test_queries_that_see_nothing_may_hold_anything(backend, B, H, K, M, N, D, bias):
+    """Causal entries with more queries than keys, or with keys hidden in front (a batch padded there): rows that see no key return zeros, and what they and
+    their gradients hold reaches nobody else's."""
+    g, q, k, v, grad = operands(M + N + D, B, H, K, M, N, D, BF16)
+    key_mask = torch.rand(B, N, generator=g, device="cuda") < 0.9
+    key_mask[:, : max(N // 3, N - M + M // 3)] = False
+    table = buckets = None
+    if bias != "none":
+        table = torch.randn(16, H, generator=g, device="cuda")
+        buckets = mfb.offset_buckets(16, 40, device="cuda") if bias == "offset" else torch.randint(0, 18, (B, M, N), generator=g, device="cuda", dtype=torch.uint8)
+    i, j = torch.arange(M, device="cuda")[:, None], torch.arange(N, device="cuda")
+    blind = ~((j - i <= N - M) & key_mask[:, None]).any(2)  # (B, M)
+    assert blind.any()
+    at = blind[:, None].expand(B, H, M)
+    q[at], grad[at] = NAN, 0.0
+    got = run_both(q, k, v, grad, key_mask=key_mask, causal=True, bias=table, buckets=buckets)
+    assert not got["out"][at].any() and not got["dq"][at].any()
+    q[at], grad[at] = math.inf, -math.inf
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)] + ([table.detach().requires_grad_()] if table is not None else [])
+    out = mfb.dense_attention(*leaves[:3], key_mask=key_mask, causal=True, bias=leaves[-1] if table is not None else None, buckets=buckets)
+    again = [out.detach(), *torch.autograd.grad(out, leaves, grad)]
+    assert all(torch.equal(a, b) for a, b in zip(again, got.values()))
