@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
           const float* o = x + (j0 + c) * 3ll;
           const float q0 = o[0], q1 = o[1], q2 = o[2];
           int lo = 0, hi = edges.n;  // edges below lo are at or below the distance, those from hi on above it
-          if (p0 - q0 == 0.f && p1 - q1 == 0.f && p2 - q2 == 0.f) {  // an atom and itself: every row has one (but at infinity that is no distance)
-            lo = hi = edges.zeros;
+          if (p0 == q0 && p1 == q1 && p2 == q2) {  // an atom and itself: every row has one
+            lo = hi = (p0 - p0) + (p1 - p1) + (p2 - p2) == 0.f ? edges.zeros : 0;  // (at infinity that is no distance)
           } else {
             const double ex = (double)p0 - q0, ey = (double)p1 - q1, ez = (double)p2 - q2;
             const double e2 = __dadd_rn(__dadd_rn(__dmul_rn(ex, ex), __dmul_rn(ey, ey)), __dmul_rn(ez, ez));
