@@ -809,7 +809,9 @@ int mf_selftest_dense_attn_give_up(const MfDenseAttnArgs* args, int32_t backward
 
 /* Buckets of a batch of molecules for the above: buckets[b][i][j] (rows `row` and entries `batch_stride` bytes apart) = how many of the `edges` ascending
  * host values lie at or below the distance of atoms i and j of coords (batch, tokens, 3) fp32, compared as squares in fp64; 0 where i or j is
- * at or behind num_atoms (batch) int32.  At most 127 edges, none negative. */
+ * at or behind num_atoms (batch) int32.  At most 127 edges, none negative.  Entries that have tokens * row bytes (batch_stride at least
+ * that) are the call's own: it may write zeros behind the pairs of a row, the last one's too.  With a smaller batch_stride (from
+ * (tokens - 1) * row + tokens on) no byte but the pairs' is written: so for buckets that are a part of a wider matrix. */
 int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t batch, int32_t tokens, const double* edges, int32_t num_edges,
                         uint8_t* buckets, int64_t batch_stride, int64_t row, void* stream);
 

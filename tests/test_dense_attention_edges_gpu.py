@@ -218,3 +218,22 @@ def test_queries_that_see_nothing_may_hold_anything(backend, B, H, K, M, N, D, b
     out = mfb.dense_attention(*leaves[:3], key_mask=key_mask, causal=True, bias=leaves[-1] if table is not None else None, buckets=buckets)
     again = [out.detach(), *torch.autograd.grad(out, leaves, grad)]
     assert all(torch.equal(a, b) for a, b in zip(again, got.values()))
+
+
+@pytest.mark.parametrize("N,row", [(1, 4), (5, 8), (29, 32), (30, 64), (129, 160), (131, 140)])
+def test_bytes_behind_a_row(N, row):
+    """Through the C interface, buckets as a part of a wider matrix (entries shorter than their rows): no byte but the pairs' own is written. In entries of whole
+    rows the bytes behind are zeros or as they were, and what lies behind the entries stays."""
+    x = torch.randn(2, N, 3, generator=torch.Generator().manual_seed(N)) * 3
+    edges = torch.linspace(0.0, 8.0, 16, dtype=torch.float64)
+    want, xc = mfb.distance_buckets(x, edges), x.cuda()
+    for batch_stride in (N * row, N * row - 1, (N - 1) * row + N):
+        store = torch.full((2 * N * row + 64,), 77, device="cuda", dtype=torch.uint8)
+        _lib.launch(_lib.lib().mf_distance_buckets, xc.device, xc.data_ptr(), None, 2, N, edges.data_ptr(), edges.numel(), store.data_ptr(), batch_stride, row)
+        out = store.as_strided((2, N, N), (batch_stride, row, 1))
+        assert torch.equal(out.cpu(), want)
+        out.fill_(77)
+        if batch_stride == N * row:
+            assert ((store == 77) | (store == 0))[: 2 * N * row].all() and (store[2 * N * row :] == 77).all()
+        else:
+            assert (store == 77).all()
