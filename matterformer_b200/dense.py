@@ -300,7 +300,12 @@ def _lengths(num, most, device):
 
 
 def dense_attention_torch(q, k, v, num_keys=None, num_queries=None, *, key_mask=None, causal=False, bias=None, buckets=None, scale=None) -> torch.Tensor:
-    """:func:`dense_attention` in plain torch operations, on any device and in any floating type (16-bit operands in fp32)."""
+    """:func:`dense_attention` in plain torch operations, on any device and in any floating type (16-bit operands in fp32), whatever autocast is for."""
+    with torch.autocast(q.device.type, enabled=False):
+        return _plain(q, k, v, num_keys, num_queries, key_mask, causal, bias, buckets, scale)
+
+
+def _plain(q, k, v, num_keys, num_queries, key_mask, causal, bias, buckets, scale):
     B, H, M, D = q.shape
     K, N = k.shape[1:3]
     wide = torch.promote_types(q.dtype, torch.float32)

@@ -19,3 +19,20 @@ def test_buckets_of_no_pairs_have_no_address():
     for over in ({}, {"bucket_kind": _lib.MF_BUCKETS_OFFSET, "queries": 0}, {"bias": None, "queries": 0}):
         assert L.mf_dense_attn_fwd(ctypes.byref(_args(**{**pairs, **over})), None) == _lib.MF_ERR_INVALID_ARGUMENT
         assert "go together" in _lib.last_error()
+
+
+def test_plain_form_under_autocast():
+    """In fp32 whatever autocast is for, forward and backward, in the function and in a layer that has no kernel."""
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (4 * torch.randn(2, 2, 40, 24, generator=g) for _ in range(3))
+    table, buckets = torch.randn(8, 2, generator=g), mfb.offset_buckets(8, 10)
+    for dtype in (torch.float32, torch.bfloat16):
+        made = []
+        for low in (False, True):
+            leaves = [t.to(dtype).requires_grad_() for t in (q, k, v)] + [table.clone().requires_grad_()]
+            with torch.autocast("cpu", torch.bfloat16, enabled=low):
+                out = dense_attention_torch(*leaves[:3], bias=leaves[3], buckets=buckets, causal=True)
+                plain = dense_attention_torch(*leaves[:3])
+            assert out.dtype == dtype
+            made.append([out, plain, *torch.autograd.grad(out.sum(), leaves)])
+        assert all(torch.equal(a, b) for a, b in zip(*made))
