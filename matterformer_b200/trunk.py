@@ -264,12 +264,11 @@ class RegularAttention(nn.Module):
         kernel = self._dense_fits(x)
         self._last_core_used = "dense" if kernel else "torch"
         table = self.bias_table if self.relative_bias is not None else None
-        shown = None if key_padding_mask is None else ~key_padding_mask.bool()
+        shown = None if key_padding_mask is None else ~key_padding_mask
         if positions is not None:
             r = self.rotary
             if key_padding_mask is not None and positions.ndim == r.frequencies.ndim + 1:  # (as in _dense_rotary)
-                hidden = key_padding_mask.bool()
-                positions = positions.masked_fill((hidden if positions.ndim == 2 else hidden[..., None]) & ~positions.isfinite(), 0)
+                positions = positions.masked_fill((key_padding_mask if positions.ndim == 2 else key_padding_mask[..., None]) & ~positions.isfinite(), 0)
             if kernel and not self._differentiated(positions):
                 qkv = rotary_packed(qkv, H, self._kernel_positions(positions), r.frequencies, layout=r.layout, amplitude=r.amplitude)
             else:
@@ -370,6 +369,7 @@ class RegularAttention(nn.Module):
             return self._sparse_forward(x, sparse_plan, positions)
         if self.relative_bias is not None or self.impl == "cuda":
             suffix = False
+            key_padding_mask = None if key_padding_mask is None else key_padding_mask.bool()  # (one of whole numbers, or of zeros and minus infinities, too)
             if key_padding_mask is not None and self._dense_fits(x):
                 suffix = _padding_is_suffix(self, key_padding_mask) if padding_is_suffix is None else padding_is_suffix
             return self._dense_forward(x, key_padding_mask, positions, buckets, num_atoms, suffix)

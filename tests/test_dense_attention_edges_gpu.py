@@ -237,3 +237,14 @@ def test_bytes_behind_a_row(N, row):
             assert ((store == 77) | (store == 0))[: 2 * N * row].all() and (store[2 * N * row :] == 77).all()
         else:
             assert (store == 77).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.float32])
+def test_padding_masks_of_other_types(dtype):
+    """The layer reads a padding mask of whole numbers, or of zeros and minus infinities, as it reads one of truth values: holes stay holes."""
+    torch.manual_seed(0)
+    layer = RegularAttention(128, 2, impl="cuda").cuda()
+    x, mask = torch.randn(3, 40, 128, device="cuda"), _pad_masks("random", 3, 40).cuda()
+    other = mask.to(dtype) if dtype == torch.uint8 else torch.zeros(3, 40, device="cuda").masked_fill(mask, -math.inf)
+    with torch.no_grad(), torch.autocast("cuda", BF16):
+        assert torch.equal(layer(x, key_padding_mask=other), layer(x, key_padding_mask=mask))
