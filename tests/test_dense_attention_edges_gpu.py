@@ -248,3 +248,19 @@ def test_padding_masks_of_other_types(dtype):
     other = mask.to(dtype) if dtype == torch.uint8 else torch.zeros(3, 40, device="cuda").masked_fill(mask, -math.inf)
     with torch.no_grad(), torch.autocast("cuda", BF16):
         assert torch.equal(layer(x, key_padding_mask=other), layer(x, key_padding_mask=mask))
+
+
+@pytest.mark.parametrize("bias", ["none", "offset", "pair"])
+@pytest.mark.parametrize("B,H,K,M,N,D", [(1, 32, 1, 1, 4096, 128), (2, 71, 1, 1, 900, 64), (1, 34, 2, 3, 1500, 64), (2, 17, 1, 1, 1000, 32), (1, 20, 1, 5, 700, 128), (2, 64, 2, 1, 70, 64),
+                                         (1, 24, 1, 40, 600, 64)])  # fmt: skip
+def test_many_query_heads_on_a_key_head(B, H, K, M, N, D, bias):
+    """More query heads to a key head than a tile has rows."""
+    g, q, k, v, grad = operands(H + N, B, H, K, M, N, D, BF16)
+    num_k, key_mask = counts(g, B, N), torch.rand(B, N, generator=g, device="cuda") < 0.8
+    table = buckets = None
+    if bias != "none":
+        table = torch.randn(16, H, generator=g, device="cuda")
+        table[3, H // 2] = -math.inf
+        buckets = mfb.offset_buckets(16, 40, device="cuda") if bias == "offset" else torch.randint(0, 18, (B, M, N), generator=g, device="cuda", dtype=torch.uint8)
+    run_both(q, k, v, grad, bias=table, buckets=buckets)
+    run_both(q, k, v, grad, num_keys=num_k, key_mask=key_mask, causal=True, bias=table, buckets=buckets)
