@@ -53,8 +53,16 @@ def offset_buckets(num_buckets: int, reach: int, *, bidirectional: bool = True, 
     if reach < 0:
         raise ValueError(f"offset_buckets: reach must not be negative, got {reach}")
     near = max(1, side // 2)
-    spread = math.log(max(2.0, reach / near))
-    rank = [n if n < near else min(side - 1, near + int(math.log(n / near) / spread * (side - near))) for n in range(reach + 1)]
+    far, (top, base) = side - near, (reach, near) if reach >= 2 * near else (2, 1)  # of the ratio that `far` buckets span
+    spread = math.log(top / base)
+
+    def beyond(n: int) -> int:
+        """The whole part of far * log(n / near) / log(top / base); next to a whole number, which logarithms may miss, by powers of whole numbers."""
+        x = math.log(n / near) / spread * far
+        k = round(x)
+        return int(x) if abs(x - k) > 1e-9 else k - (n**far * base**k < near**far * top**k)
+
+    rank = [n if n < near else min(side - 1, near + beyond(n)) for n in range(reach + 1)]
     later = [side + r if bidirectional else 0 for r in rank[1:]]
     return torch.tensor(rank[::-1] + later, dtype=torch.uint8, device=device)
 

@@ -36,3 +36,19 @@ def test_plain_form_under_autocast():
             assert out.dtype == dtype
             made.append([out, plain, *torch.autograd.grad(out.sum(), leaves)])
         assert all(torch.equal(a, b) for a, b in zip(*made))
+
+
+def test_offsets_at_the_borders_of_buckets():
+    """Beyond the first half of a side the bucket is the whole part of far * log(n / near) / log(reach / near), also where that is a whole number: compared by
+    powers of whole numbers, without logarithms."""
+    for num_buckets, reach in ((18, 128), (108, 64), (108, 125), (32, 128), (64, 512), (16, 64), (12, 27), (128, 1000)):
+        side = num_buckets // 2
+        near = side // 2
+        far = side - near
+        got = mfb.offset_buckets(num_buckets, reach).tolist()[: reach + 1][::-1]
+        assert got[:near] == list(range(near))
+        for n in range(near, reach + 1):
+            k = got[n] - near
+            assert n**far * near**k >= near**far * reach**k
+            assert k == far - 1 or n**far * near ** (k + 1) < near**far * reach ** (k + 1)
+    assert [mfb.offset_buckets(18, 128).tolist()[128 - n] for n in (7, 8, 15, 16, 31, 32, 63, 64)] == [4, 5, 5, 6, 6, 7, 7, 8]
