@@ -50,6 +50,7 @@ __device__ __forceinline__ uint32_t param_word(const void* at) {
   return v;
 }
 constexpr float kDistanceError = 5e-7f;  // of a squared distance in fp32, in relation to it; 6 * 2^-24 and an edge's rounding
+constexpr int kLeastSquare = 0x0d800000;  // 2^-100 as bits: below, its three squares may leave fp32's normal range, and that error does not hold
 
 // A thread takes four columns, whose coordinates stay in registers, and walks over rows: `lanes` threads (a power of two up to 32) lie along a row, the rest
 // of the block along the rows.  The squared distance is formed in fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares); its leading bits name a cell, which
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const 
       const float end = c == kCells - 1 ? INFINITY : __int_as_float(max(0, c + 1 + edges.base) << kCellShift) * (1.f + 2 * kDistanceError);
       const float one = k < edges.n ? __uint_as_float(param_word(edges.low + k)) : INFINITY;
       const float two = k + 1 < edges.n ? __uint_as_float(param_word(edges.low + k + 1)) : INFINITY;
-      cells[c] = make_float2(c == 0 || (k + 1 < edges.n && two <= end) ? __int_as_float(0x7fffffff) : one <= end ? one : INFINITY, __int_as_float(k));
+      cells[c] = make_float2(c == 0 || c + edges.base <= (kLeastSquare >> kCellShift) || (k + 1 < edges.n && two <= end) ? __int_as_float(0x7fffffff) : one <= end ? one : INFINITY, __int_as_float(k));
     }
   }
   wait_for_previous();
@@ -377,7 +378,7 @@ int mf_distance_buckets(const float* coords, const int32_t* num_atoms, int32_t b
   while (e.zeros < num_edges && e.square[e.zeros] == 0.0) ++e.zeros;
   auto bits = [](float f) { int i; memcpy(&i, &f, 4); return i; };
   auto value = [](int i) { float f; memcpy(&f, &i, 4); return f; };
-  const float last = num_edges ? e.low[num_edges - 1] : 0.f;
+  const float least = value(kLeastSquare), last = num_edges && e.low[num_edges - 1] > least ? e.low[num_edges - 1] : least;
   e.base = (bits(last) >> kCellShift) - (kCells - 2);
   for (int c = 0, k = 0; c < kCells; ++c) {  // what the table says is where the search begins: too low costs time alone
     const long long start = (long long)(c + e.base) * (1 << kCellShift);

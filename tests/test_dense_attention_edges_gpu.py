@@ -264,3 +264,16 @@ def test_many_query_heads_on_a_key_head(B, H, K, M, N, D, bias):
         buckets = mfb.offset_buckets(16, 40, device="cuda") if bias == "offset" else torch.randint(0, 18, (B, M, N), generator=g, device="cuda", dtype=torch.uint8)
     run_both(q, k, v, grad, bias=table, buckets=buckets)
     run_both(q, k, v, grad, num_keys=num_k, key_mask=key_mask, causal=True, bias=table, buckets=buckets)
+
+
+@pytest.mark.parametrize("scale", [1e-24, 3e-23, 1e-22, 2e-21, 1e-20, 1e-19, 1e-15, 1e15, 1e18, 5e18])
+def test_distances_far_from_one(scale):
+    """Squares that fp32 holds as subnormal numbers, as zeros or not at all, beside edges of their size, at distances that occur, and of another: as on the CPU."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(2, 131, 3, generator=g) * scale
+    x[1] = torch.randint(-4, 5, (131, 3), generator=g).float() * scale
+    d = (x.double()[:, :, None] - x.double()[:, None]).norm(dim=-1).flatten()
+    occur = d[torch.randint(0, len(d), (127,), generator=g)].sort().values
+    for edges in (torch.linspace(0.0, 5 * scale, 32, dtype=torch.float64), occur, occur[:1], occur[-1:], occur * (1 + 1e-7), torch.linspace(0.0, 5.0, 32, dtype=torch.float64),
+                  torch.tensor([0.0, scale, math.inf], dtype=torch.float64), torch.zeros(0, dtype=torch.float64)):  # fmt: skip
+        assert torch.equal(mfb.distance_buckets(x.cuda(), edges).cpu(), mfb.distance_buckets(x, edges))
