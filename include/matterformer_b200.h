@@ -752,7 +752,8 @@ typedef struct MfRows { /* elements between neighbouring entries; the channels o
  * at any strides that are multiples of 8 elements.  num_queries and num_keys (batch) int32 or NULL for the padded lengths; what lies
  * behind them may hold anything, is not read as a number and gets zeros.  key_mask (batch, keys) bytes or NULL: zero hides a key.
  * causal: key j is seen by the queries i with j - i <= num_keys - num_queries (the last query stands at the last key).  A query that sees no
- * key returns zeros.
+ * key returns zeros; where lengths, key mask and order say so, it and its grad_out may hold anything (the table's hidden pairs are to be of
+ * numbers).  A query with a logit that is not a number returns none.
  *
  * bias (num_buckets, heads) in bias_dtype or NULL; buckets as bucket_kind says, the offset being j - i - (num_keys - num_queries);
  * bucket_row and bucket_batch are the strides of the pairs' (bytes), buckets is NULL where there are no pairs.  Up to 128 buckets; a bucket beyond the table has no bias and no

@@ -56,7 +56,7 @@ constexpr int kLeastSquare = 0x0d800000;  // 2^-100 as bits: below, its three sq
 // of the block along the rows.  The squared distance is formed in fp32 (off by at most 6 * 2^-24 of itself, a sum of three squares); its leading bits name a cell, which
 // knows the buckets below it and the one edge in it, if any: one load, one comparison.  A pair within that error of the edge, in a cell that several edges share
 // or so near that squares leave fp32's range is decided in fp64, where the differences of fp32 coordinates are exact but for far apart exponents.
-// What bounds it is instructions, some twenty a pair; two cells of 4096 atoms and 63 edges take 43.5 us (78 % of the issue slots; all pairs in fp64
+// What bounds it is instructions, some twenty a pair; two cells of 4096 atoms and 63 edges take 42.6 us (83 % of the issue slots; all pairs in fp64
 // against all edges 463).
 constexpr int kBucketThreads = 256, kBucketSteps = 16;
 __global__ void __launch_bounds__(kBucketThreads) distance_buckets_kernel(const float* coords, const int32_t* num_atoms, int N, const __grid_constant__ Edges edges,

@@ -398,7 +398,8 @@ int pick(const DenseParams& p, int head_dim, int kind, void* workspace, cudaStre
 // Few rows to a key head, or few pairs in all, so that most SMs would stand idle through a long walk.  Microseconds here | on the better of the other families: one
 // query, 8 heads of 64, 65 keys 3.3 | 5.2, 512 keys 5.8 | 9.8, 64 entries of 1024 keys 31 | 50.  8 heads of 64 (of 128 after the comma): 64 queries on 1024 keys 7.4 | 15.4,
 // 10 | 18; 2^21 pairs: 256 on 1024 13 | 20, 15 | 21, 128 on 2048 13.3 | 13.5, 15 | 16, 64 on 4096 11 | 13, 16 | 16; 2^22 pairs: 256 on 2048 20 | 17, 22 | 20; 2^23:
-// 64 on 16384 34 | 20, 34 | 24.  Heads of 32, which tcgen05 does not take: 72 tiles of 64 queries on 4096 keys 33 | 43.
+// 64 on 16384 34 | 20, 34 | 24.  Heads of 32, which tcgen05 does not take: 72 tiles of 64 queries on 4096 keys 33 | 43.  Not measured on this side, since the rule
+// leaves them to the others: batches of more than 16 rows to a key head (64 single tokens of 32 heads of 128 on one, behind 4096 keys, - | 435; the cache alone is 21).
 bool dense_attn_split_applies(const DenseParams& p, int head_dim) {
   if (p.N <= 64 || p.N > (1 << 26)) return false;
   if ((long long)p.M * (p.H / p.K) <= kRows) return true;

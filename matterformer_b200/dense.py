@@ -392,8 +392,9 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_keys:
     strides with adjacent channels (expanded dimensions keep to the warp-level kernels; shared key heads are fastest as K heads).  Returns (B, H, M, D) with the tokens and heads in memory as ``q`` has them.
 
     ``num_keys``, ``num_queries``: (B,) counts of real keys and queries, which come first; what lies behind them may hold anything and returns
-    zeros, as does a query that sees no key.  ``key_mask``: (B, N) bool, False hides a key.  ``causal``: the last real query stands at the last
-    real key, and no query sees later keys than its place.  ``bias``: a table (buckets, H) of up to 128 rows, fp32 or 16 bits, added to the logits
+    zeros, as does a query that sees no key.  By counts, key mask and order: such a query, its gradient and keys that are hidden from all may hold anything; what the
+    order hides from some queries, or the table hides, takes part in products and has to be numbers.  A query with a logit that is not a number returns none.  ``key_mask``: (B, N) bool, False hides a key.
+    ``causal``: the last real query stands at the last real key, and no query sees later keys than its place.  ``bias``: a table (buckets, H) of up to 128 rows, fp32 or 16 bits, added to the logits
     ``scale * q . k`` (scale: D ** -0.5 by default) by the bucket of the pair; ``buckets``: uint8, either (2 L + 1,) for the offsets -L .. L between the place of the key
     and that of the query (:func:`offset_buckets`), which hold their ends for all beyond, or (B or 1, M, N) for every pair (:func:`distance_buckets`).  A
     bucket beyond the table has no bias; a value of minus infinity or below -1e30 hides its pairs.
