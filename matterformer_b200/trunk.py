@@ -391,6 +391,9 @@ class RegularAttention(nn.Module):
             num_atoms = (~key_padding_mask).sum(dim=1).to(torch.int32)
         if positions is not None:
             r = self.rotary
+            if qkv.requires_grad and positions.ndim == r.frequencies.ndim + 1:  # (a padded row's gradient of zeros would turn by an angle that is no number)
+                hidden = key_padding_mask.bool()
+                positions = positions.masked_fill(hidden if positions.ndim == 2 else hidden[..., None], 0)
             if self._differentiated(positions):
                 qkv = rotate_packed_torch(qkv, H, positions, r.frequencies, r.layout, r.amplitude)
             else:

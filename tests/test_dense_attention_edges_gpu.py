@@ -277,3 +277,27 @@ def test_distances_far_from_one(scale):
     for edges in (torch.linspace(0.0, 5 * scale, 32, dtype=torch.float64), occur, occur[:1], occur[-1:], occur * (1 + 1e-7), torch.linspace(0.0, 5.0, 32, dtype=torch.float64),
                   torch.tensor([0.0, scale, math.inf], dtype=torch.float64), torch.zeros(0, dtype=torch.float64)):  # fmt: skip
         assert torch.equal(mfb.distance_buckets(x.cuda(), edges).cpu(), mfb.distance_buckets(x, edges))
+
+
+@pytest.mark.parametrize("axes", [1, 3])
+@pytest.mark.parametrize("impl,biased", [("auto", False), ("cuda", False), ("auto", True)])
+@pytest.mark.parametrize("N", [29, 60])
+def test_padded_positions_that_are_no_numbers(N, impl, biased, axes):
+    """Rotary positions of padding may hold anything: output and gradients as with zeros there."""
+    torch.manual_seed(0)
+    spec = mfb.RelativeBias(16, "offset", 6) if biased else None
+    layer = RegularAttention(128, 2, impl=impl, relative_bias=spec, rotary=mfb.RotaryPositions(24, axes=axes)).cuda()
+    x, mask = torch.randn(3, N, 128, device="cuda"), torch.arange(N, device="cuda") >= torch.tensor([N, N - 4, 3], device="cuda")[:, None]
+    grad = torch.randn_like(x) * ~mask[..., None]
+    more = {"buckets": spec.buckets(None, None, x.device)} if biased else {}
+    places = torch.randn(3, N, *((axes,) if axes > 1 else ()), device="cuda")
+    made = []
+    for value in (0.0, NAN, math.inf):
+        at = places.clone()
+        at[mask] = value
+        leaf = x.clone().requires_grad_()
+        with torch.autocast("cuda", BF16):
+            out = layer(leaf, key_padding_mask=mask, positions=at, **more)
+        made.append([out[~mask], *torch.autograd.grad(out, [leaf, *layer.parameters()], grad.to(out.dtype))])
+    for other in made[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(made[0], other))
